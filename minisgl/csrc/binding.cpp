@@ -20,7 +20,25 @@ using minisgl::DType;
 
 namespace {
 
-#define MSG_CHECK(cond, ...) TORCH_CHECK(cond, "minisgl: ", __VA_ARGS__)
+// Messages are put together here, without streams: where the compiler links
+// its C++ runtime statically, formatting a number through torch's stream
+// helpers uses another copy of the locale and crashes instead of raising.
+inline std::string msg_part(const char* s) { return s; }
+inline std::string msg_part(const std::string& s) { return s; }
+inline std::string msg_part(at::ScalarType t) { return c10::toString(t); }
+inline std::string msg_part(int64_t n) { return std::to_string(n); }
+inline std::string msg_part(at::IntArrayRef a) {
+  std::string s = "[";
+  for (size_t i = 0; i < a.size(); ++i) s += (i ? ", " : "") + std::to_string(a[i]);
+  return s + "]";
+}
+template <typename... Parts>
+std::string msg_text(const Parts&... parts) {
+  std::string s = "minisgl: ";
+  ((s += msg_part(parts)), ...);
+  return s;
+}
+#define MSG_CHECK(cond, ...) TORCH_CHECK(cond, msg_text(__VA_ARGS__))
 
 DType dtype_of(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -458,6 +476,169 @@ void mx8_quantize(at::Tensor q, at::Tensor sf, const at::Tensor& x, const c10::o
   minisgl::launch_mx8_quantize_rows(q.data_ptr(), sf.data_ptr(), x.data_ptr(), ip, static_cast<int>(k),
                                     static_cast<int>(rows), static_cast<int>(K), static_cast<int>(tile), nullptr,
                                     stream_of(x));
+}
+
+// ------------------------------------------------- rows with MXFP8 output ----
+void check_mx8_out(const at::Tensor& x, const at::Tensor& q, const at::Tensor& sf, int64_t rows, int64_t cols,
+                   const char* what) {
+  MSG_CHECK(cols > 0 && cols % 32 == 0, what, ": the width must be a positive multiple of 32, got ", cols);
+  check_same_device(x, q);
+  check_same_device(x, sf);
+  MSG_CHECK(q.scalar_type() == at::kByte && q.dim() == 2 && q.size(0) == rows && q.size(1) == cols &&
+                q.stride(1) == 1 && (rows <= 1 || (q.stride(0) >= cols && q.stride(0) % 16 == 0)) &&
+                reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+            what, ": q must be uint8 [", rows, ", ", cols, "], rows at multiples of 16 bytes");
+  MSG_CHECK(sf.scalar_type() == at::kByte && sf.dim() == 2 && sf.size(0) == rows && sf.size(1) == cols / 32 &&
+                sf.stride(1) == 1 && (rows <= 1 || sf.stride(0) >= cols / 32),
+            what, ": sf must be uint8 [", rows, ", ", cols / 32, "]");
+}
+// rows at multiples of 16 bytes, not overlapping
+void check_vec_rows(const at::Tensor& t, int64_t rows, int64_t cols, at::ScalarType dt, const char* what,
+                    const char* name) {
+  check_cuda(t, name);
+  MSG_CHECK(t.scalar_type() == dt && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.stride(1) == 1,
+            what, ": ", name, " must be ", dt, " [", rows, ", ", cols, "] with unit column stride");
+  MSG_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                (rows <= 1 || (t.stride(0) >= cols && t.stride(0) * t.element_size() % 16 == 0)),
+            what, ": the rows of ", name, " must lie at multiples of 16 bytes");
+}
+
+void rmsnorm_mx8(at::Tensor q, at::Tensor sf, const at::Tensor& x, const c10::optional<at::Tensor>& w, double eps,
+                 const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& residual_out) {
+  check_cuda(x, "x");
+  MSG_CHECK(x.dim() == 2, "rmsnorm_mx8: x must be 2-D");
+  const int64_t rows = x.size(0), cols = x.size(1);
+  minisgl::RmsnormMx8Args a{};
+  a.dtype = dtype_of(x);
+  check_vec_rows(x, rows, cols, x.scalar_type(), "rmsnorm_mx8", "x");
+  check_mx8_out(x, q, sf, rows, cols, "rmsnorm_mx8");
+  MSG_CHECK(cols <= 4096 * (16 / x.element_size()), "rmsnorm_mx8: width ", cols, " is above the supported ",
+            4096 * (16 / x.element_size()));
+  MSG_CHECK(rows < (1ll << 31), "rmsnorm_mx8: too many rows");
+  MSG_CHECK(eps >= 0.0, "rmsnorm_mx8: eps must not be negative");
+  if (w.has_value()) {
+    MSG_CHECK(w->is_cuda() && w->scalar_type() == x.scalar_type() && w->is_contiguous() && w->numel() == cols &&
+                  reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0,
+              "rmsnorm_mx8: w must be a contiguous, 16-byte aligned vector of x's type with ", cols, " elements");
+    check_same_device(x, *w);
+    a.w = w->data_ptr();
+  }
+  MSG_CHECK(residual.has_value() == residual_out.has_value(), "rmsnorm_mx8: residual and residual_out go together");
+  if (residual.has_value()) {
+    check_vec_rows(*residual, rows, cols, x.scalar_type(), "rmsnorm_mx8", "residual");
+    check_vec_rows(*residual_out, rows, cols, x.scalar_type(), "rmsnorm_mx8", "residual_out");
+    check_same_device(x, *residual);
+    check_same_device(x, *residual_out);
+    a.residual = residual->data_ptr();
+    a.residual_out = residual_out->data_ptr();
+    a.ld_res = residual->stride(0);
+    a.ld_res_out = residual_out->stride(0);
+  }
+  a.x = x.data_ptr();
+  a.q = q.data_ptr<uint8_t>();
+  a.sf = sf.data_ptr<uint8_t>();
+  a.rows = rows;
+  a.cols = static_cast<int>(cols);
+  a.ld_x = x.stride(0);
+  a.ld_q = q.stride(0);
+  a.ld_sf = sf.stride(0);
+  a.eps = eps;
+  const c10::cuda::CUDAGuard guard(x.device());
+  minisgl::launch_rmsnorm_mx8(a, stream_of(x));
+}
+
+void act_mx8(at::Tensor q, at::Tensor sf, const at::Tensor& x, int64_t act, bool interleaved) {
+  check_cuda(x, "x");
+  MSG_CHECK(x.dim() == 2 && x.size(1) % 2 == 0, "act_mx8: x must be [rows, 2 d]");
+  const int64_t rows = x.size(0), d = x.size(1) / 2;
+  minisgl::ActMx8Args a{};
+  a.dtype = dtype_of(x);
+  check_vec_rows(x, rows, 2 * d, x.scalar_type(), "act_mx8", "x");
+  check_mx8_out(x, q, sf, rows, d, "act_mx8");
+  MSG_CHECK(!interleaved || d % 64 == 0, "act_mx8: the interleaved width must be a multiple of 64, got ", d);
+  MSG_CHECK(d < (1ll << 30), "act_mx8: too wide");
+  a.x = x.data_ptr();
+  a.q = q.data_ptr<uint8_t>();
+  a.sf = sf.data_ptr<uint8_t>();
+  a.rows = rows;
+  a.d = static_cast<int>(d);
+  a.ld_x = x.stride(0);
+  a.ld_q = q.stride(0);
+  a.ld_sf = sf.stride(0);
+  a.act = static_cast<int>(act);
+  a.interleaved = interleaved;
+  const c10::cuda::CUDAGuard guard(x.device());
+  minisgl::launch_act_mx8(a, stream_of(x));
+}
+
+// ---------------------------------------------------------- 4-bit linear ----
+void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Tensor>& x_scales,
+                 const at::Tensor& packed, const at::Tensor& scales, const c10::optional<at::Tensor>& zeros,
+                 const c10::optional<at::Tensor>& bias, int64_t N, int64_t K, int64_t group) {
+  MSG_CHECK(group == 32 || group == 64 || group == 128, "int4_linear: group of 32, 64 or 128, got ", group);
+  MSG_CHECK(x.dim() == 2 && x.size(1) == K, "int4_linear: x must be [M, ", K, "], got ", x.sizes());
+  check_cuda(x, "x");
+  const int64_t M = x.size(0);
+  MSG_CHECK(N > 0 && K > 0 && K % 8 == 0, "int4_linear: K must be a positive multiple of 8");
+  minisgl::Int4LinearArgs a{};
+  if (x_scales.has_value()) {
+    MSG_CHECK(x.scalar_type() == at::kByte && K % 32 == 0, "int4_linear: MXFP8 rows are uint8 with K % 32 == 0");
+    MSG_CHECK(x_scales->is_cuda() && x_scales->scalar_type() == at::kByte && x_scales->dim() == 2 &&
+                  x_scales->size(0) == M && x_scales->size(1) == K / 32 && x_scales->stride(1) == 1,
+              "int4_linear: x_scales must be uint8 [M, K / 32]");
+    check_same_device(x, *x_scales);
+    a.x_scales = x_scales->data_ptr<uint8_t>();
+    a.ld_xs = x_scales->stride(0);
+    a.x_type = DType::kBF16;
+  } else {
+    MSG_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
+              "int4_linear: x must be bfloat16 or float16 (or MXFP8 rows with x_scales)");
+    a.x_type = dtype_of(x);
+  }
+  check_vec_rows(x, M, K, x.scalar_type(), "int4_linear", "x");
+  const int64_t tiles = (N + 15) / 16, blocks = (K + 63) / 64, groups = (blocks * 64 + group - 1) / group;
+  MSG_CHECK(packed.is_cuda() && packed.scalar_type() == at::kByte && packed.is_contiguous() &&
+                packed.numel() == tiles * blocks * 512 && reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16 == 0,
+            "int4_linear: packed weight of the wrong type or size");
+  MSG_CHECK(scales.is_cuda() && (scales.scalar_type() == at::kBFloat16 || scales.scalar_type() == at::kHalf) &&
+                scales.is_contiguous() && scales.numel() == tiles * groups * 16 &&
+                reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
+            "int4_linear: weight scales of the wrong type or size");
+  check_same_device(x, packed);
+  check_same_device(x, scales);
+  if (zeros.has_value()) {
+    MSG_CHECK(zeros->is_cuda() && zeros->scalar_type() == at::kByte && zeros->is_contiguous() &&
+                  zeros->numel() == tiles * groups * 16 && reinterpret_cast<uintptr_t>(zeros->data_ptr()) % 16 == 0,
+              "int4_linear: weight zero points of the wrong type or size");
+    check_same_device(x, *zeros);
+    a.zeros = zeros->data_ptr<uint8_t>();
+  }
+  if (bias.has_value()) {
+    MSG_CHECK(bias->is_cuda() && bias->is_contiguous() && bias->numel() == N,
+              "int4_linear: bias must be a contiguous vector of ", N, " elements");
+    check_same_device(x, *bias);
+    a.bias = bias->data_ptr();
+    a.bias_type = dtype_of(*bias);
+  }
+  check_cuda(out, "out");
+  check_same_device(x, out);
+  MSG_CHECK(out.dim() == 2 && out.size(0) == M && out.size(1) == N && out.stride(1) == 1 &&
+                (M <= 1 || out.stride(0) >= N),
+            "int4_linear: out must be [", M, ", ", N, "] with unit column stride");
+  a.x = x.data_ptr();
+  a.packed = packed.data_ptr<uint8_t>();
+  a.scales = scales.data_ptr();
+  a.out = out.data_ptr();
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.ldx = x.stride(0);
+  a.ldo = out.stride(0);
+  a.group = static_cast<int>(group);
+  a.scale_type = dtype_of(scales);
+  a.out_type = dtype_of(out);
+  const c10::cuda::CUDAGuard guard(x.device());
+  minisgl::launch_int4_linear(a, stream_of(x));
 }
 
 // Block-scaled MX routed experts: align -> gather + MXFP8 quantise -> gate_up
@@ -1494,6 +1675,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("tile_row"), py::arg("num_tiles"), py::arg("err"), py::arg("combine") = true);
   m.def("mx8_quantize", &mx8_quantize, py::arg("q"), py::arg("sf"), py::arg("x"), py::arg("idx"), py::arg("k"),
         py::arg("rows"), py::arg("tile"));
+  m.def("rmsnorm_mx8", &rmsnorm_mx8);
+  m.def("act_mx8", &act_mx8);
+  m.def("int4_linear", &int4_linear);
   m.def("moe_experts_mx", &moe_experts_mx, py::arg("out"), py::arg("x"), py::arg("w1q"), py::arg("w1sb"),
         py::arg("w2q"), py::arg("w2sb"), py::arg("topk_w"), py::arg("topk_ids"), py::arg("tile"), py::arg("xq"),
         py::arg("xsf"), py::arg("h"), py::arg("hq"), py::arg("hsf"), py::arg("ys"), py::arg("sorted_pair"),

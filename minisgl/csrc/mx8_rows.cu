@@ -1,0 +1,373 @@
+// Row kernels whose output is MXFP8: residual addition + RMSNorm, and the
+// gated activations (SiLU / GELU times the up projection). They stand beside
+// the bf16 / fp16 / fp32 forms of elementwise.cu and feed products that take
+// 8-bit rows (int4.cu).
+//
+// MXFP8 rows (OCP microscaling v1.0), scales row-major:
+//   q  uint8 [rows, cols]       E4M3 elements
+//   sf uint8 [rows, cols / 32]  E8M0: one power of two 2^(byte - 127) per 32 columns
+// For a block of values y: byte - 127 is the smallest e >= -126 with
+// max |y| <= 448 * 2^e (448 is E4M3's largest), the elements are y / 2^e
+// rounded to nearest even; an all-zero block has byte 0 and zero elements; a
+// block that holds an infinity, a NaN or a magnitude beyond float32 has byte
+// 255 and NaN elements.
+//
+// The stored bits are those of the formula in exact arithmetic (64 bits):
+// y is computed in float32 with a bound on its error, and where a value
+// lies closer to a rounding border than that bound (about one element in
+// 10^5) it is computed again in double and rounded to odd on the way to
+// E4M3, so that the second rounding cannot move it. Results then do not
+// depend on how an exponential or a sum of squares is rounded on the way.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <stdexcept>
+
+#include "common.cuh"
+#include "launch.h"
+#include "ops.h"
+
+namespace minisgl {
+namespace {
+
+constexpr int kBlock = 32;  // columns under one scale
+
+template <typename T, int V>
+__device__ __forceinline__ void load_row_vec(const T* p, float (&v)[V]) {
+  static_assert(V * sizeof(T) == 16, "one 16-byte vector");
+  const uint4 raw = *reinterpret_cast<const uint4*>(p);
+  const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = to_f32<T>(e[i]);
+}
+
+// E4M3 bits of a double: truncated to float32 with a sticky last bit
+// (round to odd), then rounded to nearest even once.
+__device__ __forceinline__ uint32_t e4m3_of(double t) {
+  float f = __double2float_rz(t);
+  if (static_cast<double>(f) != t) f = __uint_as_float(__float_as_uint(f) | 1u);
+  return __nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ double pow2(int e) {  // 2^e, |e| <= 1000
+  return __longlong_as_double(static_cast<long long>(1023 + e) << 52);
+}
+
+// The V elements y of this lane, quantised. The 32 / V neighbouring lanes
+// that share a block call it together with the rest of their warp (`active`
+// may differ between blocks, not inside one). `window`: bound on y's error
+// in units of its last place; bit i of `doubt` marks an element whose error
+// may be larger. exact(i): element i in double, `zero` whether all of the
+// lane's inputs are zero (asked only where y is too small for float32).
+template <int V, typename Exact, typename Zero>
+__device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t window, uint32_t doubt, Exact exact,
+                                          Zero zero, uint8_t* q, uint8_t* sf, bool active) {
+  constexpr int G = kBlock / V;  // lanes of a block
+  const int lane = threadIdx.x & 31;
+  uint32_t m = 0;  // max of the magnitudes' bits: NaN above infinity above every number
+#pragma unroll
+  for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(y[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int o = 1; o < G; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (!active) return;
+  // magnitudes far inside float32's range whose scale is in no doubt
+  const uint32_t frac = m & 0x7FFFFFu;
+  const bool plain = m - (30u << 23) < (220u << 23) && frac + window - 0x600000u > 2 * window;
+  uint32_t words[V / 4];
+  uint32_t sbyte;
+  if (plain) {
+    sbyte = ((m + 0x1FFFFFu) >> 23) - 8;  // exponent of m, one up where the fraction is above 448's 1.75
+    const float inv = __uint_as_float((254u - sbyte) << 23);
+    uint32_t near = 0;
+#pragma unroll
+    for (int w = 0; w < V / 4; ++w) {
+      uint32_t half[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float a = y[4 * w + 2 * h] * inv, b = y[4 * w + 2 * h + 1] * inv;
+        half[h] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          // below 2^-6 E4M3's steps are all 2^-9: adding 2^-6 puts the value on the grid of [2^-6, 2^-5)
+          float s = fabsf(k == 0 ? a : b);
+          // an element in doubt matters unless it is far below half of the smallest step
+          if (s > 0.00048828125f) near |= doubt & (1u << (4 * w + 2 * h + k));
+          if (s < 0.015625f) s += 0.015625f;
+          // 20 of the 23 fraction bits are rounded away; borders are at their middle
+          const uint32_t d = (__float_as_uint(s) - 0x80000u + window) & 0xFFFFFu;
+          if (d <= 2 * window) near |= 1u << (4 * w + 2 * h + k);
+        }
+      }
+      words[w] = half[0] | (half[1] << 16);
+    }
+    if (near != 0) {
+      const double s = pow2(127 - static_cast<int>(sbyte));
+#pragma unroll 1
+      for (int i = 0; i < V; ++i) {
+        if ((near >> i & 1u) == 0) continue;
+        const uint32_t b = e4m3_of(exact(i) * s) << (8 * (i & 3)), keep = ~(0xFFu << (8 * (i & 3)));
+#pragma unroll
+        for (int w = 0; w < V / 4; ++w)
+          if (w == (i >> 2)) words[w] = (words[w] & keep) | b;
+      }
+    }
+  } else {
+    // the whole block in double
+    const uint32_t group = (G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (lane & ~(G - 1)));
+    double top = 0.0;
+    bool nan = false;
+    const bool zeros = m == 0 && __all_sync(group, zero());
+    if (!zeros) {
+#pragma unroll 1
+      for (int i = 0; i < V; ++i) {
+        const double a = fabs(exact(i));
+        nan |= !(a <= 3.4028234663852886e38);
+        top = fmax(top, a);
+      }
+#pragma unroll
+      for (int o = 1; o < G; o <<= 1) top = fmax(top, __shfl_xor_sync(group, top, o));
+      nan = __any_sync(group, nan);
+    }
+    if (nan) {
+      sbyte = 255;
+#pragma unroll
+      for (int w = 0; w < V / 4; ++w) words[w] = 0x7F7F7F7Fu;
+    } else if (top == 0.0) {
+      sbyte = 0;
+#pragma unroll
+      for (int w = 0; w < V / 4; ++w) words[w] = 0;
+    } else {
+      const long long bits = __double_as_longlong(top);
+      int e = static_cast<int>(bits >> 52) - 1023 - 8;  // 448 = 1.75 * 2^8
+      if ((bits & 0xFFFFFFFFFFFFFll) > 0xC000000000000ll) ++e;
+      e = max(e, -126);
+      sbyte = static_cast<uint32_t>(e + 127);
+      const double s = pow2(-e);
+#pragma unroll
+      for (int w = 0; w < V / 4; ++w) words[w] = 0;
+#pragma unroll 1
+      for (int i = 0; i < V; ++i) {
+        const uint32_t b = e4m3_of(exact(i) * s) << (8 * (i & 3));
+#pragma unroll
+        for (int w = 0; w < V / 4; ++w)
+          if (w == (i >> 2)) words[w] |= b;
+      }
+    }
+  }
+  if constexpr (V == 8) {
+    *reinterpret_cast<uint2*>(q) = make_uint2(words[0], words[1]);
+  } else {
+    *reinterpret_cast<uint32_t*>(q) = words[0];
+  }
+  if ((lane & (G - 1)) == 0) *sf = static_cast<uint8_t>(sbyte);
+}
+
+// --------------------------------------------------------------- RMSNorm ----
+struct NormArgs {
+  const void* x;
+  const void* res;   // nullptr: no residual
+  void* res_out;
+  const void* w;     // nullptr: no weight
+  uint8_t* q;
+  uint8_t* sf;
+  int cols;
+  int64_t ld_x, ld_res, ld_res_out, ld_q, ld_sf;
+  double eps;
+};
+
+// One CTA per row, the row kept in registers between the two passes.
+// The sum of squares is held in double: the squares of 16-bit inputs are
+// exact there, so the statistic is exact but for the final additions.
+template <typename T, int NV>
+__global__ void __launch_bounds__(1024) rmsnorm_mx8_kernel(const NormArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int V = 16 / sizeof(T);
+  __shared__ double red[32];
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+  const T* res = a.res != nullptr ? static_cast<const T*>(a.res) + row * a.ld_res : nullptr;
+  T* res_out = static_cast<T*>(a.res_out) + row * a.ld_res_out;
+  float v[NV][V];
+  double ss = 0.0;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * blockDim.x + threadIdx.x) * V;
+    if (c < a.cols) {
+      load_row_vec<T, V>(x + c, v[k]);
+      if (res != nullptr) {
+        float r[V];
+        load_row_vec<T, V>(res + c, r);
+        uint4 raw;
+        T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          // the residual stream is kept in the activation's type: the sum is rounded before it is normalised
+          e[i] = from_f32<T>(v[k][i] + r[i]);
+          v[k][i] = to_f32<T>(e[i]);
+        }
+        *reinterpret_cast<uint4*>(res_out + c) = raw;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const double d = v[k][i];
+        ss = fma(d, d, ss);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) red[warp] = ss;
+  __syncthreads();
+  const int nw = blockDim.x >> 5;
+  ss = lane < nw ? red[lane] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const double inv_d = 1.0 / sqrt(ss / a.cols + a.eps);
+  // a row whose factor is at the ends of float32's range is computed in double as a whole (NaN sends it there)
+  const bool tame = inv_d > 1e-30 && inv_d < 1e30;
+  const float inv = tame ? static_cast<float>(inv_d) : __uint_as_float(0x7FC00000u);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * blockDim.x + threadIdx.x) * V;
+    const bool active = c < a.cols;
+    float y[V];
+    if (active) {
+      float w[V];
+      if (a.w != nullptr) load_row_vec<T, V>(static_cast<const T*>(a.w) + c, w);
+      // three roundings (inv and two products): at most 3 units of the last place
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[i] = a.w != nullptr ? v[k][i] * inv * w[i] : v[k][i] * inv;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[i] = 0.f;
+    }
+    const T* src = (res != nullptr ? res_out : x) + c;  // the normalised row's input, as stored
+    const T* wc = static_cast<const T*>(a.w) + c;
+    const bool has_w = a.w != nullptr;
+    mx8_block<V>(
+        y, 4u, 0u,
+        [=](int i) {
+          const double d = static_cast<double>(to_f32<T>(src[i])) * inv_d;
+          return has_w ? d * static_cast<double>(to_f32<T>(wc[i])) : d;
+        },
+        [=]() {
+          bool z = true;
+#pragma unroll 1
+          for (int i = 0; i < V; ++i) z &= to_f32<T>(src[i]) == 0.f;
+          return z;
+        },
+        a.q + row * a.ld_q + c, a.sf + row * a.ld_sf + c / kBlock, active);
+  }
+}
+
+// ------------------------------------------------------ gated activation ----
+struct ActArgs {
+  const void* x;  // [rows, 2 d], row stride ld_x
+  uint8_t* q;
+  uint8_t* sf;
+  int64_t rows, ld_x, ld_q, ld_sf;
+  int d;
+  int interleaved;  // gate|up in alternating blocks of 64 columns
+};
+
+// exact forms, in double
+template <int ACT>
+__device__ __noinline__ double act_exact(double g, double u) {
+  if (ACT == 0) return g / (1.0 + exp(-g)) * u;
+  return 0.5 * g * erfc(-g * 0.70710678118654752440) * u;
+}
+
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int V = 16 / sizeof(T);
+  const int nvec = a.d / V;
+  const int64_t total = a.rows * nvec;
+  const int lane = threadIdx.x & 31;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  // whole warps stay in the loop: total is a multiple of a block's lanes, so `active` is the same in a block
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31); base < total; base += step) {
+    const int64_t i = base + lane;
+    const bool active = i < total;
+    const int64_t r = active ? i / nvec : 0;
+    const int c = active ? static_cast<int>(i - r * nvec) * V : 0;
+    const T* row = static_cast<const T*>(a.x) + r * a.ld_x;
+    const T* gp = row + (a.interleaved ? (c / 64) * 128 + c % 64 : c);
+    const T* up = gp + (a.interleaved ? 64 : a.d);
+    float g[V], u[V], y[V];
+    load_row_vec<T, V>(gp, g);
+    load_row_vec<T, V>(up, u);
+    uint32_t doubt = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float p = g[k] * u[k];  // exact for 16-bit types
+      if (ACT == 0) {
+        // 1 / (1 + e^-g): for g >= -16 the exponential's argument and its own error, the sum, the reciprocal
+        // and the products leave at most 26 * 2^-24; below it is in doubt
+        y[k] = __fdividef(p, 1.f + __expf(-g[k]));
+        if (g[k] < -16.f) doubt |= 1u << k;
+      } else {
+        // g / 2 * erfc(-g / sqrt 2): for g >= -6 the argument's rounding grows by at most 2 * (6 / sqrt 2)^2 = 36
+        y[k] = 0.5f * p * erfcf(-0.70710678f * g[k]);
+        if (g[k] < -6.f) doubt |= 1u << k;
+      }
+    }
+    mx8_block<V>(
+        y, ACT == 0 ? 48u : 160u, doubt,
+        [=](int k) { return act_exact<ACT>(to_f32<T>(gp[k]), to_f32<T>(up[k])); },
+        [=]() {
+          bool z = true;
+#pragma unroll 1
+          for (int k = 0; k < V; ++k) z &= to_f32<T>(gp[k]) == 0.f || to_f32<T>(up[k]) == 0.f;
+          return z;
+        },
+        a.q + r * a.ld_q + c, a.sf + r * a.ld_sf + c / kBlock, active);
+  }
+}
+
+template <typename F>
+void by_dtype(DType dt, F&& f) {
+  switch (dt) {
+    case DType::kBF16: f(__nv_bfloat16{}); break;
+    case DType::kF16: f(__half{}); break;
+    default: f(float{}); break;
+  }
+}
+
+}  // namespace
+
+void launch_rmsnorm_mx8(const RmsnormMx8Args& r, cudaStream_t s) {
+  if (r.rows <= 0) return;
+  by_dtype(r.dtype, [&](auto tag) {
+    using T = decltype(tag);
+    constexpr int V = 16 / sizeof(T);
+    const int vecs = r.cols / V;
+    if (r.cols % kBlock != 0 || vecs > 4 * 1024) throw std::runtime_error("minisgl.rmsnorm_mx8: unsupported width");
+    const NormArgs a{r.x, r.residual, r.residual_out, r.w, r.q, r.sf, r.cols, r.ld_x, r.ld_res, r.ld_res_out,
+                     r.ld_q, r.ld_sf, r.eps};
+    const int threads = std::min(1024, (((vecs + 3) / 4) + 31) / 32 * 32);
+    launch_pdl(rmsnorm_mx8_kernel<T, 4>, dim3(static_cast<unsigned>(r.rows)), dim3(threads), 0, s, a);
+  });
+}
+
+void launch_act_mx8(const ActMx8Args& r, cudaStream_t s) {
+  if (r.rows <= 0) return;
+  by_dtype(r.dtype, [&](auto tag) {
+    using T = decltype(tag);
+    constexpr int V = 16 / sizeof(T);
+    if (r.d % kBlock != 0) throw std::runtime_error("minisgl.act_mx8: width must be a multiple of 32");
+    if (r.interleaved && r.d % 64 != 0)
+      throw std::runtime_error("minisgl.act_mx8: interleaved width must be a multiple of 64");
+    const ActArgs a{r.x, r.q, r.sf, r.rows, r.ld_x, r.ld_q, r.ld_sf, r.d, r.interleaved ? 1 : 0};
+    const int64_t total = r.rows * (r.d / V);
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 148 * 16));
+    if (r.act == 0)
+      launch_pdl(act_mx8_kernel<T, 0>, dim3(blocks), dim3(256), 0, s, a);
+    else
+      launch_pdl(act_mx8_kernel<T, 1>, dim3(blocks), dim3(256), 0, s, a);
+  });
+}
+
+}  // namespace minisgl

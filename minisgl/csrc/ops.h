@@ -412,4 +412,55 @@ void launch_epoch_bump(uint32_t* epoch, cudaStream_t s);
 void launch_gemm_allreduce(const GemmArgs& a, const int64_t* bases, uint32_t* epoch, int64_t own_base, int rank,
                            int world, int64_t half_bytes, void* residual_out, cudaStream_t s);
 
+// ------------------------------------------------- rows with MXFP8 output ----
+// q uint8 [rows, cols] E4M3, sf uint8 [rows, cols / 32] E8M0 (mx8_rows.cu);
+// strides in elements. residual nullptr: plain RMSNorm; else the rounded sum
+// x + residual goes to residual_out (may be residual) and is normalised.
+struct RmsnormMx8Args {
+  const void* x;
+  const void* residual;
+  void* residual_out;
+  const void* w;  // [cols] or nullptr
+  uint8_t* q;
+  uint8_t* sf;
+  int64_t rows;
+  int cols;
+  int64_t ld_x, ld_res, ld_res_out, ld_q, ld_sf;
+  double eps;
+  DType dtype;
+};
+void launch_rmsnorm_mx8(const RmsnormMx8Args& a, cudaStream_t s);
+// act(gate) * up of x [rows, 2 d]; act 0 SiLU, 1 GELU (erf)
+struct ActMx8Args {
+  const void* x;
+  uint8_t* q;
+  uint8_t* sf;
+  int64_t rows;
+  int d;
+  int64_t ld_x, ld_q, ld_sf;
+  int act;
+  bool interleaved;
+  DType dtype;
+};
+void launch_act_mx8(const ActMx8Args& a, cudaStream_t s);
+
+// ------------------------------------------------------- 4-bit linear ----
+// out[m, n] = sum_k x[m, k] (c[n, k] - z[n, k / group]) s[n, k / group] (+ bias[n])
+// with the weight in the tile layout of minisgl.quant.int4 (int4.cu).
+struct Int4LinearArgs {
+  const void* x;            // bf16 / fp16 [M, K] (row stride ldx), or E4M3 bytes
+  const uint8_t* x_scales;  // E8M0 [M, K / 32] (row stride ld_xs) or nullptr
+  const uint8_t* packed;    // [ceil(N / 16), ceil(K / 64), 512]
+  const void* scales;       // bf16 / fp16 [ceil(N / 16), groups, 16]
+  const uint8_t* zeros;     // [ceil(N / 16), groups, 16] or nullptr (8 everywhere)
+  const void* bias;         // [N] or nullptr
+  void* out;                // [M, N], row stride ldo
+  int64_t M, N, K;
+  int64_t ldx, ld_xs, ldo;
+  int group;                // 32, 64 or 128
+  DType x_type;             // kBF16 or kF16 (the products' type; kBF16 for E4M3 rows)
+  DType scale_type, bias_type, out_type;
+};
+void launch_int4_linear(const Int4LinearArgs& a, cudaStream_t s);
+
 }  // namespace minisgl

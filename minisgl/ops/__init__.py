@@ -290,6 +290,110 @@ def _act_and_mul(x: torch.Tensor, act: str, out: Optional[torch.Tensor], interle
     return out
 
 
+# ------------------------------------------------- rows with MXFP8 output
+def _mx8_out(x: torch.Tensor, cols: int, out: Optional[Tuple[torch.Tensor, torch.Tensor]]):
+    if out is not None:
+        return out
+    rows = x.shape[0]
+    return x.new_empty((rows, cols), dtype=torch.uint8), x.new_empty((rows, cols // 32), dtype=torch.uint8)
+
+
+def _mx8_cpu(got: Tuple[torch.Tensor, torch.Tensor], out: Optional[Tuple[torch.Tensor, torch.Tensor]]):
+    if out is None:
+        return got
+    for dst, src in zip(out, got):
+        if dst.shape != src.shape or dst.dtype != src.dtype:
+            raise RuntimeError("minisgl: out must be (q uint8 [rows, cols], sf uint8 [rows, cols / 32])")
+        dst.copy_(src)
+    return out
+
+
+def rmsnorm_mx8(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, residual: Optional[torch.Tensor] = None,
+                residual_out: Optional[torch.Tensor] = None,
+                out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm with an MXFP8 output: (q uint8 [rows, cols] E4M3 bits, sf uint8
+    [rows, cols / 32] E8M0 scales) of y = s / sqrt(mean(s^2) + eps) * w.
+
+    Without ``residual`` s = x. With it s = x + residual, rounded to x's type
+    (the residual stream's), stored to ``residual_out`` (None: in place, to
+    ``residual``) and then normalised, as ``fused_add_rmsnorm`` does; x keeps
+    its values unless it is ``residual_out`` itself. y is not rounded before it
+    is quantised: the stored bits are those of the formula in 64 bits
+    (``minisgl.quant.quantize_mx8_rows_reference`` states the format). x bf16,
+    fp16 or fp32 with any row stride of whole 16-byte vectors; cols a multiple of 32, at most 32768
+    (fp32: 16384)."""
+    if residual is None and residual_out is not None:
+        raise ValueError("rmsnorm_mx8: residual_out needs residual")
+    if residual is not None and residual_out is None:
+        residual_out = residual
+    if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % 32 != 0:
+        raise ValueError(f"rmsnorm_mx8: x must be [rows, a positive multiple of 32], got {tuple(x.shape)}")
+    if not x.is_cuda:
+        return _mx8_cpu(ref.rmsnorm_mx8(x, w, eps, residual, residual_out), out)
+    q, sf = _mx8_out(x, x.shape[1], out)
+    _count()
+    native().rmsnorm_mx8(q, sf, x, w, eps, residual, residual_out)
+    return q, sf
+
+
+def silu_and_mul_mx8(x: torch.Tensor, interleaved: bool = False,
+                     out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """silu(gate) * up of x [rows, 2 d] as MXFP8 rows (q [rows, d], sf
+    [rows, d / 32]); ``interleaved``: gate|up columns alternate in blocks of
+    64. Not rounded before it is quantised (as ``rmsnorm_mx8``)."""
+    return _act_mx8(x, "silu", interleaved, out)
+
+
+def gelu_and_mul_mx8(x: torch.Tensor,
+                     out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """gelu(gate) * up (erf form) of x [rows, 2 d] as MXFP8 rows."""
+    return _act_mx8(x, "gelu", False, out)
+
+
+def _act_mx8(x: torch.Tensor, act: str, interleaved: bool, out):
+    unit = 128 if interleaved else 64
+    if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % unit != 0:
+        raise ValueError(f"{act}_and_mul_mx8: x must be [rows, a positive multiple of {unit}], got {tuple(x.shape)}")
+    if not x.is_cuda:
+        return _mx8_cpu(ref.act_mx8(x, act, interleaved), out)
+    q, sf = _mx8_out(x, x.shape[1] // 2, out)
+    _count()
+    native().act_mx8(q, sf, x, 0 if act == "silu" else 1, interleaved)
+    return q, sf
+
+
+# ---------------------------------------------------------- 4-bit linear
+def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None, x_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out = x @ W^T (+ bias) with a 4-bit weight W = (codes - zeros) * scales
+    (``minisgl.quant.Int4Weight``, made by ``int4_weight`` or
+    ``quantize_int4``). x [M, K] is bf16 or fp16, or MXFP8 rows: uint8 E4M3
+    bits with ``x_scales`` [M, K / 32], as ``rmsnorm_mx8`` and
+    ``silu_and_mul_mx8`` return them. out: bf16, fp16 or fp32 (default: x's
+    type, bf16 for MXFP8 rows). Sums are held in fp32; a group's sum of
+    x * (code - zero) is formed before its scale is applied, so
+    |x| * 15 * group has to stay inside fp32."""
+    if x.dim() != 2 or x.shape[1] != w.k:
+        raise ValueError(f"int4_linear: x must be [M, {w.k}], got {tuple(x.shape)}")
+    if (x.dtype == torch.uint8) != (x_scales is not None):
+        raise ValueError("int4_linear: uint8 x (MXFP8 rows) and x_scales go together")
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else x.dtype if x_scales is None else torch.bfloat16
+    elif out is not None and out.dtype != out_dtype:
+        raise ValueError(f"int4_linear: out is {out.dtype}, out_dtype {out_dtype}")
+    if not x.is_cuda:
+        y = ref.int4_linear(x, w, bias, out_dtype, x_scales)
+        if out is not None:
+            out.copy_(y)
+            return out
+        return y
+    if out is None:
+        out = torch.empty((x.shape[0], w.n), dtype=out_dtype, device=x.device)
+    _count()
+    native().int4_linear(out, x, x_scales, w.packed, w.scales, w.zeros, bias, w.n, w.k, w.group)
+    return out
+
+
 def embedding(ids: torch.Tensor, weight: torch.Tensor, vocab_range: Optional[Tuple[int, int]] = None,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     lo, n = vocab_range if vocab_range is not None else (0, weight.shape[0])

@@ -71,6 +71,47 @@ def fused_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, w: Optional[torch
     x.copy_(rmsnorm(s, w, eps))
 
 
+def rmsnorm_mx8(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, residual: Optional[torch.Tensor],
+                residual_out: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, sf) of rmsnorm(x [+ residual]) in float64; the rounded sum goes to residual_out."""
+    from minisgl.quant.mx8 import quantize_mx8_rows_reference
+
+    v = x.double()
+    if residual is not None:
+        v = (x.float() + residual.float()).to(x.dtype)
+        residual_out.copy_(v)
+        v = v.double()
+    y = v / torch.sqrt(v.square().mean(-1, keepdim=True) + eps)
+    return quantize_mx8_rows_reference(y if w is None else y * w.double())
+
+
+def act_mx8(x: torch.Tensor, act: str, interleaved: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, sf) of act(gate) * up in float64."""
+    from minisgl.quant.mx8 import quantize_mx8_rows_reference
+
+    rows, d = x.shape[0], x.shape[1] // 2
+    xd = x.double()
+    if interleaved:
+        g, u = (t.reshape(rows, d) for t in xd.view(rows, d // 64, 2, 64).unbind(2))
+    else:
+        g, u = xd[:, :d], xd[:, d:]
+    a = g / (1.0 + torch.exp(-g)) if act == "silu" else 0.5 * g * torch.special.erfc(-g * math.sqrt(0.5))
+    return quantize_mx8_rows_reference(a * u)
+
+
+def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor], out_dtype: torch.dtype,
+                x_scales: Optional[torch.Tensor]) -> torch.Tensor:
+    """x @ W^T (+ bias) with W = (codes - zeros) * scales (minisgl.quant.Int4Weight)."""
+    from minisgl.quant.int4 import dequantize_int4
+    from minisgl.quant.mx8 import dequantize_mx8_rows
+
+    xf = x.float() if x_scales is None else dequantize_mx8_rows(x, x_scales)
+    y = xf @ dequantize_int4(w).t()
+    if bias is not None:
+        y = y + bias.float()
+    return y.to(out_dtype)
+
+
 def act_and_mul(x: torch.Tensor, act: str) -> torch.Tensor:
     d = x.shape[-1] // 2
     g, u = x[..., :d].float(), x[..., d:].float()

@@ -1,0 +1,159 @@
+"""4-bit weights with group scales for the dense projections.
+
+A weight W [N, K] is stored as codes c in 0..15 with one scale (and
+optionally one zero point) per row and group of ``group`` columns:
+
+    W[n, k] = (c[n, k] - z[n, k // group]) * s[n, k // group]
+
+z is 8 where a weight has no zero points (symmetric quantisation). Groups are
+32, 64 or 128 columns; the last one may be short (K a multiple of 8). This is
+the form in which group-quantised checkpoints come: ``int4_weight`` takes the
+codes packed two per byte and lays them out once for the kernels
+(``minisgl/csrc/int4.cu``); ``quantize_int4`` makes them from a float weight.
+
+Layout. Rows are cut into tiles of 16, columns into blocks of 64; tile and
+block fill 512 bytes, 16 for each lane of a warp. Lane 4 g + t holds rows g and
+g + 8, columns 8 t .. 8 t + 7 of either half (32 columns) of the block, in four
+words; word j = 2 i + l has columns 32 i + 8 t + 4 l + 2 p + e of row g + 8 h at
+bit 4 (4 e + 2 p + h): masked with 0x000F000F after a shift by 4 r, a word gives
+the r-th of the four registers (two 16-bit values each) that a warp-level
+16 x 8 x 16 product takes of its first operand, in the order in which a lane's
+two runs of 8 values of x fill the second. A word's columns lie in one half, so
+no product mixes two groups. Scales and zero points are [tile, group, row of
+the tile]. Padding rows and columns have scale 0 and code 0.
+
+The reference has no weight quantisation; its projections run bf16 library
+GEMMs (python/minisgl/layers/linear.py:13-127).
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+GROUPS = (32, 64, 128)
+_TILE, _BLOCK = 16, 64
+
+
+class Int4Weight:
+    """A 4-bit weight in the kernels' layout (made by ``int4_weight`` or
+    ``quantize_int4``): ``packed`` uint8 [ceil(N / 16), ceil(K / 64), 512],
+    ``scales`` bf16 / fp16 and ``zeros`` uint8 or None [ceil(N / 16), groups, 16]."""
+
+    __slots__ = ("packed", "scales", "zeros", "n", "k", "group")
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], n: int, k: int,
+                 group: int) -> None:
+        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self.n, self.k, self.group = n, k, group
+
+    @property
+    def device(self) -> torch.device:
+        return self.packed.device
+
+    def to(self, device) -> "Int4Weight":
+        zeros = None if self.zeros is None else self.zeros.to(device)
+        return Int4Weight(self.packed.to(device), self.scales.to(device), zeros, self.n, self.k, self.group)
+
+
+def _groups_padded(k: int, group: int) -> int:
+    """Groups that the blocks of 64 columns reach into."""
+    return -(-(-(-k // _BLOCK) * _BLOCK) // group)
+
+
+def _tile_rows(t: torch.Tensor, groups: int) -> torch.Tensor:
+    """[N, groups of K] -> [ceil(N / 16), groups, 16], padded with zeros."""
+    n, g = t.shape
+    tiles = -(-n // _TILE)
+    full = t.new_zeros(tiles * _TILE, groups)
+    full[:n, :g] = t
+    return full.view(tiles, _TILE, groups).transpose(1, 2).contiguous()
+
+
+def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+                group: int = 128) -> Int4Weight:
+    """``codes`` uint8 [N, K / 2] (column 2i in the low nibble of byte i),
+    ``scales`` bf16 / fp16 [N, ceil(K / group)], ``zeros`` uint8 (0..15) of the
+    same shape or None (8 everywhere) -> the kernels' layout, on the same device."""
+    if codes.dim() != 2 or codes.dtype != torch.uint8:
+        raise ValueError("int4_weight: codes must be uint8 [N, K / 2]")
+    n, k = codes.shape[0], 2 * codes.shape[1]
+    if group not in GROUPS:
+        raise ValueError(f"int4_weight: group of 32, 64 or 128, got {group}")
+    if n == 0 or k == 0 or k % 8 != 0:
+        raise ValueError(f"int4_weight: N >= 1 and K a positive multiple of 8, got N={n}, K={k}")
+    shape = (n, -(-k // group))
+    if tuple(scales.shape) != shape or scales.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"int4_weight: scales must be bf16 or fp16 {shape}, got {scales.dtype} {tuple(scales.shape)}")
+    if zeros is not None and (tuple(zeros.shape) != shape or zeros.dtype != torch.uint8):
+        raise ValueError(f"int4_weight: zeros must be uint8 {shape}, got {zeros.dtype} {tuple(zeros.shape)}")
+    if any(t.device != codes.device for t in (scales, zeros) if t is not None):
+        raise ValueError("int4_weight: codes, scales and zeros must be on one device")
+    if zeros is not None and bool((zeros > 15).any()):
+        raise ValueError("int4_weight: zero points must be 0..15")
+    tiles, blocks = -(-n // _TILE), -(-k // _BLOCK)
+    if tiles * _TILE != n or blocks * _BLOCK != k:
+        full = codes.new_zeros(tiles * _TILE, blocks * _BLOCK // 2)
+        full[:n, : k // 2] = codes
+    else:
+        full = codes
+    # byte b of a row holds columns 2b (e = 0) and 2b + 1 (e = 1): [tile, h, g, block, i, t, l, p]
+    c = full.view(tiles, 2, 8, blocks, 2, 4, 2, 2).permute(1, 0, 3, 2, 5, 4, 6, 7)  # [h, tile, block, g, t, i, l, p]
+    top, low = c[0], c[1]
+    # bytes of a word: (e, p) from the lowest; the nibbles of a byte: h
+    packed = torch.empty(tiles, blocks, 8, 4, 2, 2, 2, 2, dtype=torch.uint8, device=codes.device)
+    packed[..., 0, :] = (top & 15) | (low << 4)
+    packed[..., 1, :] = (top >> 4) | (low & 0xF0)
+    groups = _groups_padded(k, group)
+    return Int4Weight(packed.view(tiles, blocks, 512), _tile_rows(scales, groups),
+                      None if zeros is None else _tile_rows(zeros, groups), n, k, group)
+
+
+def int4_codes(w: Int4Weight) -> torch.Tensor:
+    """The codes of a weight, uint8 [N, K]."""
+    tiles, blocks = w.packed.shape[:2]
+    b = w.packed.view(tiles, blocks, 8, 4, 2, 2, 2, 2)  # [tile, block, g, t, i, l, e, p]
+    c = torch.stack([b & 15, b >> 4], dim=-1)           # ..., h
+    c = c.permute(0, 8, 2, 1, 4, 3, 5, 7, 6)            # [tile, h, g, block, i, t, l, p, e]
+    return c.reshape(tiles * _TILE, blocks * _BLOCK)[: w.n, : w.k]
+
+
+def dequantize_int4(w: Int4Weight, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The weight as [N, K], (c - z) * s computed in float64 and rounded once."""
+    c = int4_codes(w).double()
+    of = torch.arange(w.k, device=w.device) // w.group
+
+    def spread(t: torch.Tensor) -> torch.Tensor:  # [tile, group, 16] -> [N, K]
+        return t.transpose(1, 2).reshape(-1, t.shape[1])[: w.n].double()[:, of]
+
+    return ((c - (8.0 if w.zeros is None else spread(w.zeros))) * spread(w.scales)).to(dtype)
+
+
+def quantize_int4(w: torch.Tensor, group: int = 128, symmetric: bool = True,
+                  scale_dtype: torch.dtype = torch.bfloat16) -> Int4Weight:
+    """Round-to-nearest quantisation of a float weight [N, K]. Symmetric: scale
+    max |w| / 7, codes 1..15 around 8. Otherwise the group's range (widened to
+    hold 0) over 15 steps, with the zero point at the code that stands for 0."""
+    n, k = w.shape
+    if group not in GROUPS:
+        raise ValueError(f"quantize_int4: group of 32, 64 or 128, got {group}")
+    if n == 0 or k == 0 or k % 8 != 0:
+        raise ValueError(f"quantize_int4: N >= 1 and K a positive multiple of 8, got N={n}, K={k}")
+    groups = -(-k // group)
+    x = w.new_zeros(n, groups * group, dtype=torch.float32)
+    x[:, :k] = w
+    x = x.view(n, groups, group)
+    if symmetric:
+        scales = (x.abs().amax(-1) / 7.0).to(scale_dtype)
+        zeros = None
+        z = torch.full_like(scales, 8.0, dtype=torch.float32)
+    else:
+        lo, hi = x.amin(-1).clamp(max=0), x.amax(-1).clamp(min=0)
+        scales = ((hi - lo) / 15.0).to(scale_dtype)
+        live = torch.where(scales > 0, scales.float(), torch.ones_like(lo))
+        z = (-lo / live).round().clamp(0, 15)
+        zeros = z.to(torch.uint8)
+    live = torch.where(scales > 0, scales.float(), torch.ones_like(z))
+    c = (x / live[..., None]).round().add(z[..., None]).clamp(0, 15).to(torch.uint8).view(n, -1)[:, :k]
+    return int4_weight(c[:, 0::2] | (c[:, 1::2] << 4), scales, zeros, group)

@@ -38,6 +38,8 @@ SOURCES = [
     "minisgl/csrc/mxfp4.cu",
     "minisgl/csrc/mx_gemm.cu",
     "minisgl/csrc/ep.cu",
+    "minisgl/csrc/mx8_rows.cu",
+    "minisgl/csrc/int4.cu",
 ]
 
 
