@@ -596,7 +596,7 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
     a.x_type = dtype_of(x);
   }
   check_vec_rows(x, M, K, x.scalar_type(), "int4_linear", "x");
-  const int64_t tiles = (N + 15) / 16, blocks = (K + 63) / 64, groups = (blocks * 64 + group - 1) / group;
+  const int64_t tiles = (N + 15) / 16, blocks = 2 * ((K + 127) / 128), groups = blocks * 64 / group;
   MSG_CHECK(packed.is_cuda() && packed.scalar_type() == at::kByte && packed.is_contiguous() &&
                 packed.numel() == tiles * blocks * 512 && reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16 == 0,
             "int4_linear: packed weight of the wrong type or size");
@@ -608,7 +608,7 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
   check_same_device(x, scales);
   if (zeros.has_value()) {
     MSG_CHECK(zeros->is_cuda() && zeros->scalar_type() == at::kByte && zeros->is_contiguous() &&
-                  zeros->numel() == tiles * groups * 16 && reinterpret_cast<uintptr_t>(zeros->data_ptr()) % 16 == 0,
+                  zeros->numel() == tiles * groups * 8 && reinterpret_cast<uintptr_t>(zeros->data_ptr()) % 16 == 0,
               "int4_linear: weight zero points of the wrong type or size");
     check_same_device(x, *zeros);
     a.zeros = zeros->data_ptr<uint8_t>();

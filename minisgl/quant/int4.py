@@ -11,16 +11,18 @@ the form in which group-quantised checkpoints come: ``int4_weight`` takes the
 codes packed two per byte and lays them out once for the kernels
 (``minisgl/csrc/int4.cu``); ``quantize_int4`` makes them from a float weight.
 
-Layout. Rows are cut into tiles of 16, columns into blocks of 64; tile and
-block fill 512 bytes, 16 for each lane of a warp. Lane 4 g + t holds rows g and
+Layout. Rows are cut into tiles of 16, columns into blocks of 64 (an even
+number: columns are padded to 128); tile and block fill 512 bytes, 16 for each
+lane of a warp. Lane 4 g + t holds rows g and
 g + 8, columns 8 t .. 8 t + 7 of either half (32 columns) of the block, in four
 words; word j = 2 i + l has columns 32 i + 8 t + 4 l + 2 p + e of row g + 8 h at
 bit 4 (4 e + 2 p + h): masked with 0x000F000F after a shift by 4 r, a word gives
 the r-th of the four registers (two 16-bit values each) that a warp-level
 16 x 8 x 16 product takes of its first operand, in the order in which a lane's
 two runs of 8 values of x fill the second. A word's columns lie in one half, so
-no product mixes two groups. Scales and zero points are [tile, group, row of
-the tile]. Padding rows and columns have scale 0 and code 0.
+no product mixes two groups. Scales are [tile, group, g, h], so that a lane's
+two are one word, zero points [tile, group, g] with z[g] | z[g + 8] << 4.
+Padding rows and columns have scale 0 and code 0.
 
 The reference has no weight quantisation; its projections run bf16 library
 GEMMs (python/minisgl/layers/linear.py:13-127).
@@ -33,13 +35,14 @@ from typing import Optional
 import torch
 
 GROUPS = (32, 64, 128)
-_TILE, _BLOCK = 16, 64
+_TILE, _BLOCK, _STEP = 16, 64, 128
 
 
 class Int4Weight:
     """A 4-bit weight in the kernels' layout (made by ``int4_weight`` or
-    ``quantize_int4``): ``packed`` uint8 [ceil(N / 16), ceil(K / 64), 512],
-    ``scales`` bf16 / fp16 and ``zeros`` uint8 or None [ceil(N / 16), groups, 16]."""
+    ``quantize_int4``): ``packed`` uint8 [ceil(N / 16), 2 ceil(K / 128), 512],
+    ``scales`` bf16 / fp16 [ceil(N / 16), groups, 8, 2] and ``zeros`` uint8
+    [ceil(N / 16), groups, 8] or None, groups = 128 ceil(K / 128) / group."""
 
     __slots__ = ("packed", "scales", "zeros", "n", "k", "group")
 
@@ -57,18 +60,13 @@ class Int4Weight:
         return Int4Weight(self.packed.to(device), self.scales.to(device), zeros, self.n, self.k, self.group)
 
 
-def _groups_padded(k: int, group: int) -> int:
-    """Groups that the blocks of 64 columns reach into."""
-    return -(-(-(-k // _BLOCK) * _BLOCK) // group)
-
-
 def _tile_rows(t: torch.Tensor, groups: int) -> torch.Tensor:
-    """[N, groups of K] -> [ceil(N / 16), groups, 16], padded with zeros."""
+    """[N, groups of K] -> [ceil(N / 16), groups, 8, 2] (row g + 8 h at [g, h]), padded with zeros."""
     n, g = t.shape
     tiles = -(-n // _TILE)
     full = t.new_zeros(tiles * _TILE, groups)
     full[:n, :g] = t
-    return full.view(tiles, _TILE, groups).transpose(1, 2).contiguous()
+    return full.view(tiles, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
 
 
 def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
@@ -92,7 +90,7 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
         raise ValueError("int4_weight: codes, scales and zeros must be on one device")
     if zeros is not None and bool((zeros > 15).any()):
         raise ValueError("int4_weight: zero points must be 0..15")
-    tiles, blocks = -(-n // _TILE), -(-k // _BLOCK)
+    tiles, blocks = -(-n // _TILE), 2 * -(-k // _STEP)
     if tiles * _TILE != n or blocks * _BLOCK != k:
         full = codes.new_zeros(tiles * _TILE, blocks * _BLOCK // 2)
         full[:n, : k // 2] = codes
@@ -105,9 +103,12 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
     packed = torch.empty(tiles, blocks, 8, 4, 2, 2, 2, 2, dtype=torch.uint8, device=codes.device)
     packed[..., 0, :] = (top & 15) | (low << 4)
     packed[..., 1, :] = (top >> 4) | (low & 0xF0)
-    groups = _groups_padded(k, group)
-    return Int4Weight(packed.view(tiles, blocks, 512), _tile_rows(scales, groups),
-                      None if zeros is None else _tile_rows(zeros, groups), n, k, group)
+    groups = blocks * _BLOCK // group
+    z = None
+    if zeros is not None:
+        z = _tile_rows(zeros, groups)
+        z = z[..., 0] | (z[..., 1] << 4)
+    return Int4Weight(packed.view(tiles, blocks, 512), _tile_rows(scales, groups), z, n, k, group)
 
 
 def int4_codes(w: Int4Weight) -> torch.Tensor:
@@ -124,10 +125,11 @@ def dequantize_int4(w: Int4Weight, dtype: torch.dtype = torch.float32) -> torch.
     c = int4_codes(w).double()
     of = torch.arange(w.k, device=w.device) // w.group
 
-    def spread(t: torch.Tensor) -> torch.Tensor:  # [tile, group, 16] -> [N, K]
-        return t.transpose(1, 2).reshape(-1, t.shape[1])[: w.n].double()[:, of]
+    def spread(t: torch.Tensor) -> torch.Tensor:  # [tile, group, g, h] -> [N, K]
+        return t.permute(0, 3, 2, 1).reshape(-1, t.shape[1])[: w.n].double()[:, of]
 
-    return ((c - (8.0 if w.zeros is None else spread(w.zeros))) * spread(w.scales)).to(dtype)
+    z = 8.0 if w.zeros is None else spread(torch.stack([w.zeros & 15, w.zeros >> 4], dim=-1))
+    return ((c - z) * spread(w.scales)).to(dtype)
 
 
 def quantize_int4(w: torch.Tensor, group: int = 128, symmetric: bool = True,
