@@ -596,7 +596,7 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
     a.x_type = dtype_of(x);
   }
   check_vec_rows(x, M, K, x.scalar_type(), "int4_linear", "x");
-  const int64_t tiles = (N + 15) / 16, blocks = 2 * ((K + 127) / 128), groups = blocks * 64 / group;
+  const int64_t tiles = 2 * ((N + 31) / 32), blocks = 2 * ((K + 127) / 128), groups = blocks * 64 / group;
   MSG_CHECK(packed.is_cuda() && packed.scalar_type() == at::kByte && packed.is_contiguous() &&
                 packed.numel() == tiles * blocks * 512 && reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16 == 0,
             "int4_linear: packed weight of the wrong type or size");

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kWarps * 32) int4_linear_kernel(const LinArgs 
 #pragma unroll 2
   for (int b = b0; b < b1; ++b) {
     const uint4 w = wp[static_cast<int64_t>(b) * 32];
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t words[4] = {w.x ^ 0x88888888u, w.y ^ 0x88888888u, w.z ^ 0x88888888u, w.w ^ 0x88888888u};
     uint32_t xr[NT][8];
 #pragma unroll
     for (int i = 0; i < NT; ++i) load_x<T, MX8>(xr[i], a, m0 + 8 * i + g, b * 64 + t * 8);
@@ -224,14 +224,21 @@ void launch_type(const LinArgs& a, int group, cudaStream_t s) {
 // ---------------------------------------------------------------------------
 // Few rows (up to 16): the weight stream.
 //
-// One CTA of 16 warps per SM, alone or in a cluster of S = 2, 4 or 8 whose
-// CTAs share the columns of the cluster's tiles. A unit is 16 rows x 128
-// columns (1 KB of codes and its scales); the units of a CTA, tile after tile,
-// are cut into one contiguous range per warp. Each warp copies its own units
-// into its own ring of shared memory (cp.async, kDepth units ahead), waits for
-// them alone and multiplies them; nothing else synchronises the warps while
-// they stream. x lies in shared memory for the CTA's columns, once, as 16-bit
-// values.
+// A unit is R tiles of 16 rows x 128 columns (R KB of codes and their scales).
+// Whole tiles are dealt to clusters of S = 1, 2, 4 or 8 CTAs, whose CTAs share
+// the columns; the units of a CTA, tile after tile, are cut into one contiguous
+// range per warp. Each warp copies its own units into its own ring of shared
+// memory (cp.async, kDepth ahead), waits for them alone and multiplies them;
+// nothing else synchronises the warps while they stream.
+//
+// The products are integer: a value of x under a power of two common to its
+// row's 128 columns is three 8-bit digits, a code minus 8 is a signed byte after
+// one mask, and the tensor cores sum 8-bit products exactly in 32 bits. That
+// takes 3 operations for 8 codes, where unpacking them to 16-bit floats takes 9:
+// at 6.5 TB/s an SM has about 90 cycles for the 2048 codes of a KB, and the
+// unpacking alone was the bound (B200, 1 x 51200 x 5120: 39 us with bf16
+// products). A group's scale (and z - 8 times the sum of x) is applied to its
+// finished sum.
 //
 // A tile whose units lie in one warp's range is finished there. Where a range
 // starts or ends inside a tile, the warp parks its partial sums; after the one
@@ -240,39 +247,48 @@ void launch_type(const LinArgs& a, int group, cudaStream_t s) {
 // are added in rank order after a cluster barrier. Every sum has a fixed order:
 // the same inputs give the same bits.
 // ---------------------------------------------------------------------------
-constexpr int kVecWarps = 16;
-constexpr int kDepth = 4;
+constexpr int kDepth = 3;
 constexpr int kMaxSmem = 227 * 1024;
 
+enum { kXBf16 = 0, kXHalf = 1, kXMx8 = 2 };
 struct VecArgs {
   const void* x;
   const uint8_t* x_scales;
   const uint8_t* packed;
-  const uint32_t* scales;  // [tiles, groups, 8] pairs
-  const uint8_t* zeros;    // [tiles, groups, 8]
+  const uint32_t* scales;  // [16-row tiles, groups, 8] pairs
+  const uint8_t* zeros;    // [16-row tiles, groups, 8]
   const void* bias;
   void* out;
-  int M, N, K, tiles, steps, S;  // steps of 128 columns
+  int M, N, K, tiles, steps, S;  // tiles of 16 R rows, steps of 128 columns
+  int tiles_each, tiles_more, steps_each, steps_more;
+  uint32_t inv_each, inv_more;  // 2^31 / steps_each and / (steps_each + 1), rounded up
   int64_t ldx, ld_xs, ldo;
   int scale_half, bias_type, out_type;
+  int x_kind;
   int x_bytes;     // of the x area
   int recv_slots;  // tiles that a CTA owns at most (S > 1)
 };
 
-template <int G>
+// R: 16-row tiles of a unit, whose products share the reads of x (two for up to 8 rows of x; one for 16, whose
+// sums need the registers)
+template <int W, int NT, int G, bool ZERO>
 struct VecSmem {
+  static constexpr int kR = NT == 1 ? 2 : 1;
   static constexpr int kGroups = 128 / G;
-  static constexpr int kScaleB = kGroups * 32;
-  static constexpr int kZeroB = kGroups * 8 < 16 ? 16 : kGroups * 8;
-  static constexpr int kUnit = 1024 + kScaleB + kZeroB;
-  static constexpr int kRing = kVecWarps * kDepth * kUnit;
-  static int total(int NT, int x_bytes, int recv_slots, int S) {
-    return kRing + kVecWarps * 2 * 512 * NT + x_bytes + recv_slots * S * 512 * NT;
+  static constexpr int kScaleB = kGroups * 32;  // of one tile
+  static constexpr int kZeroB = kGroups * 8;
+  static constexpr int kUnit = (kR * (1024 + kScaleB + kZeroB) + 15) / 16 * 16;  // 16-byte copies into every slot
+  static constexpr int kRing = W * kDepth * kUnit;
+  // per step and 8 rows of x: the power of two and, with zero points, each group's sum in two parts
+  static constexpr int kSide = 32 + (ZERO ? 64 * kGroups : 0);
+  static int total(int x_bytes, int recv_slots, int S) {
+    return kRing + (W * 2 + recv_slots * S) * 512 * kR * NT + x_bytes;
   }
 };
-// bytes between x's rows: an odd multiple of 64, so that the eight 16-byte
-// reads of a quarter warp (two rows x four lanes) fall into distinct banks
-__host__ __device__ inline int vec_x_pitch(int steps) { return steps * 256 + 64; }
+// bytes between x's rows (three digits of 128 columns a step): an odd
+// multiple of 64, so that the eight 16-byte reads of a quarter warp (two rows
+// x four lanes) fall into distinct banks
+__host__ __device__ inline int vec_x_pitch(int steps) { return steps * 384 + 64; }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -288,6 +304,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
 }
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -299,25 +320,80 @@ __device__ __forceinline__ uint32_t lds8(uint32_t a) {
   return v;
 }
 
-// 8 values x[m, k .. k + 7] as 16-bit pairs (zeros past K; K % 8 == 0)
-template <typename T, bool MX8>
-__device__ __forceinline__ uint4 x_run(const VecArgs& a, int m, int k) {
+// 8 values x[m, k .. k + 7] as they lie in memory (zeros past K; K % 8 == 0); MXFP8 rows: two words and the scale
+__device__ __forceinline__ uint4 x_raw(const VecArgs& a, int m, int k) {
   if (k >= a.K) return make_uint4(0, 0, 0, 0);
-  if constexpr (!MX8) {
-    return *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + m * a.ldx + k);
-  } else {  // K % 32 == 0: the 8 values lie under one scale
+  if (a.x_kind == kXMx8) {  // K % 32 == 0: the 8 values lie under one scale
     const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.x) + m * a.ldx + k);
-    const float s = e8m0(a.x_scales[m * a.ld_xs + k / 32]);
-    uint32_t r[4];
+    return make_uint4(q.x, q.y, a.x_scales[m * a.ld_xs + k / 32], 0);
+  }
+  return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + m * a.ldx + k);
+}
+__device__ __forceinline__ void x_values(float (&v)[8], const uint4 raw, int kind) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  if (kind == kXMx8) {
+    const float s = e8m0(raw.z);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t w = i < 2 ? q.x : q.y;
-      const __half2_raw raw = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * (i & 1))), __NV_E4M3);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw));
-      r[i] = pack_bf16x2(f.x * s, f.y * s);  // four significant bits and a power of two: exact in bf16
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      v[2 * i] = f.x * s, v[2 * i + 1] = f.y * s;
     }
-    return make_uint4(r[0], r[1], r[2], r[3]);
+  } else if (kind == kXHalf) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
   }
+}
+
+// D (+)= A B on 8-bit integers, 16 x 8 x 32: codes times a digit of x (the top digit signed, the others not)
+template <bool TOP, bool FIRST>
+__device__ __forceinline__ void mma_i8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+#define MINISGL_MMA(TYPE)                                                                                         \
+  if constexpr (FIRST)                                                                                            \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8." TYPE ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};" \
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                                          \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));                                  \
+  else                                                                                                            \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8." TYPE ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" \
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])                                                          \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1))
+  if constexpr (TOP) {
+    MINISGL_MMA("s8");
+  } else {
+    MINISGL_MMA("u8");
+  }
+#undef MINISGL_MMA
+}
+
+// What the infinities and NaN of x add to an output: sum over columns [k, k_end) with x not finite of x * W
+// (the digits of such values are zero). Never on the path of finite inputs.
+__device__ __noinline__ float not_finite_part(const VecArgs& a, int64_t tile, int r, int m, int group, int k, int k_end) {
+  const int64_t n = tile * 16 + r;
+  if (n >= a.N || m >= a.M) return 0.f;
+  float sum = 0.f;
+  for (; k < k_end; k += 8) {
+    float v[8];
+    x_values(v, x_raw(a, m, k), a.x_kind);
+    for (int j = 0; j < 8; ++j) {
+      if (fabsf(v[j]) <= 3.4028234e38f) continue;
+      const int c = (k + j) % 64, i = c / 32, t = c % 32 / 8, l = c % 8 / 4, q = c % 4 / 2, e = c % 2;
+      const uint32_t word = reinterpret_cast<const uint32_t*>(
+          a.packed)[((tile * a.steps * 2 + (k + j) / 64) * 32 + 4 * (r & 7) + t) * 4 + 2 * i + l];
+      const int code = (word >> (4 * (4 * e + 2 * q + (r >> 3))) & 15) ^ 8;
+      const int64_t gi = tile * (a.steps * 128 / group) + (k + j) / group;
+      const uint32_t zz = a.zeros != nullptr ? a.zeros[gi * 8 + (r & 7)] : 0x88u;
+      const uint32_t sw = a.scales[gi * 8 + (r & 7)];
+      const float s = half_bits_to_f32(r >> 3 ? sw >> 16 : sw & 0xFFFFu, a.scale_half);
+      sum += v[j] * (static_cast<float>(code - static_cast<int>(r >> 3 ? zz >> 4 : zz & 15u)) * s);
+    }
+  }
+  return sum;
 }
 
 __device__ __forceinline__ void store_sum(const VecArgs& a, int64_t tile, int r, int m, float v) {
@@ -327,203 +403,369 @@ __device__ __forceinline__ void store_sum(const VecArgs& a, int64_t tile, int r,
   store_from_f32(a.out, m * a.ldo + n, a.out_type, v);
 }
 
-template <typename T, bool MX8, int NT, int G, bool ZERO>
-__global__ void __launch_bounds__(kVecWarps * 32, 1) int4_vec_kernel(const VecArgs a) {
-  using L = VecSmem<G>;
+template <int W, int NT, int G, bool ZERO>
+__global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs a) {
+  using L = VecSmem<W, NT, G, ZERO>;
+  constexpr int kR = L::kR;
   constexpr int P = L::kGroups;  // groups of a unit
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   pdl_launch_dependents();
-  const int S = a.S, rank = blockIdx.x % S, cluster = blockIdx.x / S, clusters = gridDim.x / S;
-  const int t0 = static_cast<int>(static_cast<int64_t>(a.tiles) * cluster / clusters);
-  const int t1 = static_cast<int>(static_cast<int64_t>(a.tiles) * (cluster + 1) / clusters);
-  const int k0 = a.steps * rank / S, ks = a.steps * (rank + 1) / S - k0;
-  const int64_t units = static_cast<int64_t>(t1 - t0) * ks;
-  const int u0 = static_cast<int>(units * warp / kVecWarps), u1 = static_cast<int>(units * (warp + 1) / kVecWarps);
-  uint8_t* ring = smem + warp * (kDepth * L::kUnit);
-  float4* park = reinterpret_cast<float4*>(smem + L::kRing);  // [warp][2: head, tail][NT][lane]
-  uint8_t* xs = smem + L::kRing + kVecWarps * 2 * 512 * NT;
-  float4* recv = reinterpret_cast<float4*>(xs + a.x_bytes);  // [slot][rank][NT][lane]
+  // whole tiles are dealt to clusters, 128-column steps to the CTAs of a cluster, units to warps; each as even as
+  // can be, the first ones taking one more
+  const int S = a.S;
+  int rank = 0, cluster = blockIdx.x;
+  if (S > 1) rank = blockIdx.x & (S - 1), cluster = blockIdx.x / S;
+  const int t0 = cluster * a.tiles_each + min(cluster, a.tiles_more);
+  const int t1 = t0 + a.tiles_each + (cluster < a.tiles_more ? 1 : 0);
+  const int k0 = rank * a.steps_each + min(rank, a.steps_more);
+  const int ks = a.steps_each + (rank < a.steps_more ? 1 : 0);
+  const int units = (t1 - t0) * ks;
+  auto warp_start = [&](int w) { return units / W * w + (units % W * w) / W; };
+  const int u0 = warp_start(warp), u1 = warp_start(warp + 1);
+  float4* park = reinterpret_cast<float4*>(smem + L::kRing);  // [warp][2: head, tail][R][NT][lane]
+  uint8_t* xs = smem + L::kRing + W * 2 * 512 * kR * NT;
   const int pitch = vec_x_pitch(ks);
+  uint8_t* side = xs + a.M * pitch;                          // [step][power of two | P sums of two parts][8 NT]
+  float4* recv = reinterpret_cast<float4*>(xs + a.x_bytes);  // [slot][rank][R][NT][lane]
+  const uint32_t inv = rank < a.steps_more ? a.inv_more : a.inv_each;
+  auto by_ks = [&](int n) { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * inv >> 31); };  // n / ks
+  const int u0_tile = by_ks(u0);
+  int tile = t0 + u0_tile, k = u0 - u0_tile * ks;
 
-  // the codes of the ring's first fill, on their way to L2 while the kernel before this one ends (a prefetch
+  // the codes of the warp's first units, on their way to L2 while the kernel before this one ends (a prefetch
   // carries no value: the copies below read memory after griddepcontrol.wait)
   {
-    const int u = u0 + (lane >> 3);
-    if (u < u1) {
-      const int64_t tile = t0 + u / ks;
-      const uint8_t* p = a.packed + (tile * a.steps + k0 + u % ks) * 1024 + (lane & 7) * 128;
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+    constexpr int SH = kR == 2 ? 4 : 3;  // lanes of a unit: eight 128-byte lines per KB
+    const int ahead = k + (lane >> SH);  // the units run on through the tile, then in the next
+    if (u0 + (lane >> SH) < u1) {
+      const int on = ahead >= ks ? by_ks(ahead) : 0;
+      const int64_t row16 = static_cast<int64_t>(tile + on) * kR + (lane >> 3 & (kR - 1));
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.packed + (row16 * a.steps + k0 + ahead - on * ks) * 1024 + (lane & 7) * 128));
     }
-    static_assert(kDepth == 4, "eight lanes prefetch one unit");
   }
   pdl_wait();
 
-  int pu = u0, ptile = t0 + (ks > 0 ? u0 / ks : 0), pk = ks > 0 ? u0 % ks : 0;
-  const uint32_t ring_a = smem_u32(ring);
-  auto fetch = [&](int slot) {
-    if (pu < u1) {
-      const int64_t unit = static_cast<int64_t>(ptile) * a.steps + k0 + pk;
-      const uint32_t dst = ring_a + slot * L::kUnit;
-      const uint8_t* src = a.packed + unit * 1024 + lane * 16;
-      cp_async16(dst + lane * 16, src);
-      cp_async16(dst + 512 + lane * 16, src + 512);
-      if (lane < 8 * P) cp_async4(dst + 1024 + lane * 4, a.scales + unit * (8 * P) + lane);
-      if (ZERO && lane < P) cp_async8(dst + 1024 + L::kScaleB + lane * 8, a.zeros + unit * (8 * P) + lane * 8);
-      if (++pk == ks) pk = 0, ++ptile;
+  const uint32_t ring = smem_u32(smem) + warp * (kDepth * L::kUnit);
+  // a unit's second tile lies a.steps units of memory behind its first
+  const int64_t first = static_cast<int64_t>(tile) * kR * a.steps + k0 + k;
+  const uint8_t* src_w = a.packed + first * 1024 + lane * 16;
+  constexpr int SW = 8 * P, ZW = 2 * P;  // scale and zero words of a tile
+  const uint32_t* src_s = a.scales + (first + (P < 4 && lane >= SW ? a.steps : 0)) * SW + (P < 4 ? lane % SW : lane);
+  const uint8_t* src_z = ZERO ? a.zeros + (first + (lane >= ZW ? a.steps : 0)) * SW + lane % ZW * 4 : nullptr;
+  int left = u1 - u0, pk = k;
+  const int skip = kR * a.steps - ks;  // from the end of a unit row to the start of the next
+  const int64_t second = static_cast<int64_t>(a.steps) * 1024;
+  auto fetch = [&](uint32_t dst) {
+    if (left > 0) {
+      --left;
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        cp_async16(dst + r * 1024 + lane * 16, src_w + r * second);
+        cp_async16(dst + r * 1024 + 512 + lane * 16, src_w + r * second + 512);
+      }
+      if constexpr (P < 4) {
+        if (lane < kR * SW) cp_async4(dst + kR * 1024 + lane * 4, src_s);
+      } else {
+#pragma unroll
+        for (int r = 0; r < kR; ++r) cp_async4(dst + kR * 1024 + (r * SW + lane) * 4, src_s + r * a.steps * SW);
+      }
+      if (ZERO && lane < kR * ZW) cp_async4(dst + kR * (1024 + L::kScaleB) + lane * 4, src_z);
+      int on = 1;
+      if (++pk == ks) pk = 0, on += skip;
+      src_w += static_cast<int64_t>(on) * 1024;
+      src_s += static_cast<int64_t>(on) * SW;
+      if (ZERO) src_z += static_cast<int64_t>(on) * SW;
     }
-    ++pu;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // the first of x's loads go ahead of the weights', which they would else queue behind
+  constexpr int kBatch = 4;
+  uint4 raw[kBatch];
+  // run c of row m: a warp's 32 runs are of one row or (ks odd) of two neighbours
+  const int per_row = ks * 16;
+  int xm = 0, xc = threadIdx.x;
+  while (xc >= per_row) xc -= per_row, ++xm;
+  int lm = xm, lc = xc;
+  auto next_run = [&](int& m, int& c) {
+    c += W * 32;
+    while (c >= per_row) c -= per_row, ++m;
+  };
+  auto load_x = [&]() {
 #pragma unroll
-  for (int d = 0; d < kDepth; ++d) fetch(d);
-
-  // x, 16-bit, [row][the CTA's columns]
-  {
-    const int runs = ks * 16;
-    for (int i = threadIdx.x; i < a.M * runs; i += kVecWarps * 32) {
-      const int m = i / runs, c = i - m * runs;
-      *reinterpret_cast<uint4*>(xs + m * pitch + c * 16) = x_run<T, MX8>(a, m, k0 * 128 + c * 8);
+    for (int q = 0; q < kBatch; ++q) {
+      if (lm < a.M) raw[q] = x_raw(a, lm, k0 * 128 + lc * 8);
+      next_run(lm, lc);
     }
-  }
-  if (S > 1)
-    cluster_sync();  // and the peers have started: their shared memory may be written
-  else
-    __syncthreads();
+  };
+  load_x();
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) fetch(ring + d * L::kUnit);
 
-  // a finished tile of this CTA's columns
-  auto emit = [&](int tile, const float (&acc)[NT][4]) {
+  // x as 24-bit integers [row][step][digit][columns]: a row's 128 columns under a power of two that puts their
+  // largest value into [2^21, 2^22), rounded to nearest: exact for what lies above 2^-14 of it (bf16; fp16
+  // 2^-11, E4M3 2^-18), else at most 2^-22 of it off, as much as a rounding of a float32 sum
+  bool odd = false;  // met an infinity or NaN
+  while (xm < a.M) {
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      if (xm >= a.M) break;
+      const int m = xm, c = xc, step = c >> 4;
+      next_run(xm, xc);
+      float v[8];
+      x_values(v, raw[q], a.x_kind);
+      auto largest = [&]() {
+        uint32_t b[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+        return max(__vimax3_u32(b[0], b[1], b[2]), __vimax3_u32(max(b[3], b[4]), b[5], max(b[6], b[7])));
+      };
+      uint32_t top = largest();
+      if (top >= 0x7F800000u) {
+        odd = true;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!(fabsf(v[j]) <= 3.4028234e38f)) v[j] = 0.f;
+        top = largest();
+      }
+      const uint32_t half_warp = 0xFFFFu << (threadIdx.x & 16);  // 16 lanes share a row's 128 columns
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(half_warp, top, o));
+      const uint32_t e = max(top >> 23, 26u);
+      const float up = __uint_as_float((275u - e) << 23);
+      uint32_t xi[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xi[j] = __float_as_uint(fmaf(v[j], up, 12582912.f)) - 0x4B400000u;  // 1.5 * 2^23
+      uint8_t* dst = xs + m * pitch + step * 384 + (c >> 3 & 1) * 64 + (c & 3) * 16 + (c >> 2 & 1) * 8;
+      uint32_t word[3][2];
+#pragma unroll
+      for (int l = 0; l < 2; ++l) {  // columns 0, 2, 1, 3: the order of a code word's bytes
+        const uint32_t t0 = __byte_perm(xi[4 * l], xi[4 * l + 2], 0x5140), t1 = __byte_perm(xi[4 * l + 1], xi[4 * l + 3], 0x5140);
+        const uint32_t t2 = __byte_perm(xi[4 * l], xi[4 * l + 2], 0x0062), t3 = __byte_perm(xi[4 * l + 1], xi[4 * l + 3], 0x0062);
+        word[0][l] = __byte_perm(t0, t1, 0x5410);
+        word[1][l] = __byte_perm(t0, t1, 0x7632);
+        word[2][l] = __byte_perm(t2, t3, 0x5410);
+      }
+#pragma unroll
+      for (int d = 0; d < 3; ++d) *reinterpret_cast<uint2*>(dst + d * 128) = make_uint2(word[d][0], word[d][1]);
+      uint8_t* sd = side + step * (L::kSide * NT);
+      // codes count in sixteenths (they sit in a byte's upper half): 2^-4 goes with the power of two
+      if ((c & 15) == 0) *reinterpret_cast<float*>(sd + m * 4) = __uint_as_float((e - 25u) << 23);
+      if constexpr (ZERO) {
+        int sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += static_cast<int>(xi[j]);
+#pragma unroll
+        for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(half_warp, sum, o);
+        if ((c & (G / 8 - 1)) == 0)
+          *reinterpret_cast<int2*>(sd + NT * 32 + (c & 15) / (G / 8) * (NT * 64) + m * 8) = make_int2(sum & 0xFFFF, sum >> 16);
+      }
+    }
+    load_x();
+  }
+  odd = __syncthreads_or(odd);
+  if (S > 1) cluster_sync();  // the peers have started: their shared memory may be written
+
+  // a finished pair of tiles, this CTA's columns
+  auto emit = [&](int tile, float (&acc)[kR][NT][4]) {
+    if (odd) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[r][i][j] += not_finite_part(a, static_cast<int64_t>(tile) * kR + r, g + (j >> 1) * 8,
+                                            8 * i + 2 * t + (j & 1), G, k0 * 128, min(a.K, (k0 + ks) * 128));
+    }
     if (S == 1) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int r = 0; r < kR; ++r)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) store_sum(a, tile, g + (j >> 1) * 8, 8 * i + 2 * t + (j & 1), acc[i][j]);
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            store_sum(a, static_cast<int64_t>(tile) * kR + r, g + (j >> 1) * 8, 8 * i + 2 * t + (j & 1), acc[r][i][j]);
     } else {
       const int local = tile - t0;
+      const uint32_t base = map_shared_rank(smem_u32(recv + (local / S * S + rank) * (kR * NT * 32) + lane), local & (S - 1));
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const uint32_t dst = map_shared_rank(smem_u32(recv + ((local / S * S + rank) * NT + i) * 32 + lane), local % S);
-        asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "f"(acc[i][0]), "f"(acc[i][1]),
-                     "f"(acc[i][2]), "f"(acc[i][3])
-                     : "memory");
-      }
+      for (int r = 0; r < kR; ++r)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(base + (r * NT + i) * 512),
+                       "f"(acc[r][i][0]), "f"(acc[r][i][1]), "f"(acc[r][i][2]), "f"(acc[r][i][3])
+                       : "memory");
     }
   };
 
-  float acc[NT][4];
+  float acc[kR][NT][4];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-  int tile = t0 + (ks > 0 ? u0 / ks : 0), k = ks > 0 ? u0 % ks : 0;
-  bool head = k != 0;  // the tile was started by the warp before
-  const uint32_t xa = smem_u32(xs) + g * pitch + t * 16;
-  const bool row_in[2] = {g < a.M, 8 + g < a.M};
-  int slot = 0;
-  for (int u = u0; u < u1; ++u) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-    __syncwarp();
-    const uint32_t src = ring_a + slot * L::kUnit;
-    uint4 w[2];
-    w[0] = lds128(src + lane * 16);
-    w[1] = lds128(src + 512 + lane * 16);
-    uint32_t sc[P], zz[P];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      sc[p] = lds32(src + 1024 + (8 * p + g) * 4);
-      zz[p] = ZERO ? lds8(src + 1024 + L::kScaleB + 8 * p + g) : 0x88u;
-    }
-    __syncwarp();  // every lane has read the slot
-    fetch(slot);
-    slot = slot + 1 == kDepth ? 0 : slot + 1;
-    uint4 xv[NT][4];
-    const uint32_t xk = xa + k * 256;
+  for (int r = 0; r < kR; ++r)
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        xv[i][q] = row_in[i] ? lds128(xk + i * 8 * pitch + q * 64) : make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < 4; ++j) acc[r][i][j] = 0.f;
+  bool head = k != 0;  // the pair was started by the warp before
+  const uint32_t x_row = smem_u32(xs) + g * pitch + t * 16;
+  uint32_t side_at = smem_u32(side) + t * 8;
+  uint32_t src = ring;
+  // rows past M stay zero: their lanes never load
+  uint4 xv[NT][3][2];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const uint32_t z0 = Num<T>::offset(zz[p] & 15u), z1 = Num<T>::offset(zz[p] >> 4);
-      float part[NT][4];
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+    for (int d = 0; d < 3; ++d) xv[i][d][0] = xv[i][d][1] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+  for (int u = u0; u < u1;) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    __syncwarp();
+    uint32_t sc[kR][P], zz[kR][P];
+    uint32_t f[kR][4][4];  // the first operand
 #pragma unroll
-        for (int j = 0; j < 4; ++j) part[i][j] = 0.f;
+    for (int r = 0; r < kR; ++r) {
 #pragma unroll
-      for (int j = p * 8 / P; j < (p + 1) * 8 / P; ++j) {
-        const uint4 wv = w[j >> 2];
-        const uint32_t word = (j & 3) == 0 ? wv.x : (j & 3) == 1 ? wv.y : (j & 3) == 2 ? wv.z : wv.w;
-        uint32_t f[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          f[i] = Num<T>::sub(((word >> (4 * i)) & 0x000F000Fu) | Num<T>::kMagic, (i & 1) ? z1 : z0);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const uint4 v = xv[i][j >> 1];
-          Num<T>::mma(part[i], f, (j & 1) ? v.z : v.x, (j & 1) ? v.w : v.y);
-        }
+      for (int p = 0; p < P; ++p) {
+        sc[r][p] = lds32(src + kR * 1024 + (SW * r + 8 * p + g) * 4);
+        zz[r][p] = ZERO ? lds8(src + kR * (1024 + L::kScaleB) + SW * r + 8 * p + g) : 0x88u;
       }
-      const float s0 = half_bits_to_f32(sc[p] & 0xFFFFu, a.scale_half), s1 = half_bits_to_f32(sc[p] >> 16, a.scale_half);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        acc[i][0] += part[i][0] * s0, acc[i][1] += part[i][1] * s0;
-        acc[i][2] += part[i][2] * s1, acc[i][3] += part[i][3] * s1;
+      for (int h = 0; h < 2; ++h) {
+        const uint4 w = lds128(src + r * 1024 + h * 512 + lane * 16);
+        // bytes whose upper halves are the signed codes c - 8: row g's are the low nibbles, row g + 8's the high
+        f[r][2 * h][0] = w.x << 4 & 0xF0F0F0F0u, f[r][2 * h][1] = w.x & 0xF0F0F0F0u;
+        f[r][2 * h][2] = w.y << 4 & 0xF0F0F0F0u, f[r][2 * h][3] = w.y & 0xF0F0F0F0u;
+        f[r][2 * h + 1][0] = w.z << 4 & 0xF0F0F0F0u, f[r][2 * h + 1][1] = w.z & 0xF0F0F0F0u;
+        f[r][2 * h + 1][2] = w.w << 4 & 0xF0F0F0F0u, f[r][2 * h + 1][3] = w.w & 0xF0F0F0F0u;
       }
     }
-    if (++k == ks || u + 1 == u1) {
+    __syncwarp();  // every lane has read the slot
+    fetch(src);
+    src = src + L::kUnit == ring + kDepth * L::kUnit ? ring : src + L::kUnit;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if (8 * i + g < a.M) {
+        const uint32_t at = x_row + 8 * i * pitch + k * 384;
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+          xv[i][d][0] = lds128(at + d * 128);
+          xv[i][d][1] = lds128(at + d * 128 + 64);
+        }
+      }
+      const uint32_t sd = side_at + k * (L::kSide * NT) + i * 32;
+      const uint2 pw = lds64(sd);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        int c[kR][3][4];
+        // products of one digit and tile wait for one another; the 3 R chains run side by side
+#pragma unroll
+        for (int j = p * 4 / P; j < (p + 1) * 4 / P; ++j) {
+#pragma unroll
+          for (int r = 0; r < kR; ++r) {
+#pragma unroll
+            for (int d = 0; d < 3; ++d) {
+              const uint4 v = xv[i][d][j >> 1];
+              const uint32_t b0 = j & 1 ? v.z : v.x, b1 = j & 1 ? v.w : v.y;
+              if (j == p * 4 / P) {
+                if (d == 2)
+                  mma_i8<true, true>(c[r][d], f[r][j], b0, b1);
+                else
+                  mma_i8<false, true>(c[r][d], f[r][j], b0, b1);
+              } else {
+                if (d == 2)
+                  mma_i8<true, false>(c[r][d], f[r][j], b0, b1);
+                else
+                  mma_i8<false, false>(c[r][d], f[r][j], b0, b1);
+              }
+            }
+          }
+        }
+        uint4 sums;
+        if constexpr (ZERO) sums = lds128(sd + NT * 32 + p * (NT * 64) + t * 8 + i * 32);
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+          float s0, s1;
+          if (a.scale_half) {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&sc[r][p]));
+            s0 = h.x, s1 = h.y;
+          } else {
+            s0 = __uint_as_float(sc[r][p] << 16), s1 = __uint_as_float(sc[r][p] & 0xFFFF0000u);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // at most 2^22 (256 + 1) in the lower part, 2^20 in the upper: exact integers, one rounding to float32
+            // each and one where they meet
+            int lo = c[r][1][j] * 256 + c[r][0][j], hi = c[r][2][j];
+            if constexpr (ZERO) {
+              const int z = 16 * static_cast<int>(j < 2 ? zz[r][p] & 15u : zz[r][p] >> 4) - 128;  // 16 (z - 8)
+              lo -= z * static_cast<int>(j & 1 ? sums.z : sums.x);
+              hi -= z * static_cast<int>(j & 1 ? sums.w : sums.y);
+            }
+            const float v = fmaf(static_cast<float>(hi), 65536.f, static_cast<float>(lo));
+            acc[r][i][j] = fmaf(v * (j < 2 ? s0 : s1), __uint_as_float(j & 1 ? pw.y : pw.x), acc[r][i][j]);
+          }
+        }
+      }
+    }
+    ++u;
+    if (++k == ks || u == u1) {
       if (!head && k == ks) {
         emit(tile, acc);
       } else {
-        float4* dst = park + (warp * 2 + (head ? 0 : 1)) * NT * 32 + lane;
+        float4* dst = park + (warp * 2 + (head ? 0 : 1)) * (kR * NT * 32) + lane;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) dst[i * 32] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+        for (int r = 0; r < kR; ++r)
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            dst[(r * NT + i) * 32] = make_float4(acc[r][i][0], acc[r][i][1], acc[r][i][2], acc[r][i][3]);
       }
       head = false;
       ++tile;
       k = 0;
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int r = 0; r < kR; ++r)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[r][i][j] = 0.f;
     }
   }
   __syncthreads();
-  // the tile that this warp started and did not finish: its own part, then the heads of the warps after it
+  // the pair that this warp started and did not finish: its own part, then the heads of the warps after it
   if (u1 > u0) {
-    const int last = (u1 - 1) / ks;                         // tile of the last unit, from t0
-    const int64_t end = static_cast<int64_t>(last + 1) * ks;  // one past the tile's units
-    if (end > u1 && static_cast<int64_t>(last) * ks >= u0) {
-      float4 sum[NT];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) sum[i] = park[((warp * 2 + 1) * NT + i) * 32 + lane];
-      for (int w = warp + 1; w < kVecWarps; ++w) {
-        const int b = static_cast<int>(units * w / kVecWarps), e = static_cast<int>(units * (w + 1) / kVecWarps);
+    const int last = by_ks(u1 - 1);   // pair of the last unit, from t0
+    const int end = (last + 1) * ks;  // one past the pair's units
+    if (end > u1 && last * ks >= u0) {
+      for (int w = warp; w < W; ++w) {
+        const int b = warp_start(w);
         if (b >= end) break;
-        if (e == b) continue;
+        if (warp_start(w + 1) == b) continue;
+        const float4* part = park + (w * 2 + (w == warp ? 1 : 0)) * (kR * NT * 32) + lane;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const float4 v = park[(w * 2 * NT + i) * 32 + lane];
-          sum[i].x += v.x, sum[i].y += v.y, sum[i].z += v.z, sum[i].w += v.w;
-        }
+        for (int r = 0; r < kR; ++r)
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const float4 v = part[(r * NT + i) * 32];
+            acc[r][i][0] += v.x, acc[r][i][1] += v.y, acc[r][i][2] += v.z, acc[r][i][3] += v.w;
+          }
       }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) acc[i][0] = sum[i].x, acc[i][1] = sum[i].y, acc[i][2] = sum[i].z, acc[i][3] = sum[i].w;
       emit(t0 + last, acc);
     }
   }
   if (S > 1) {
     cluster_sync();
-    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(a.recv_slots) * NT * 128; i += kVecWarps * 32) {
-      const int e = static_cast<int>(i % 128), nt = static_cast<int>(i / 128 % NT), sl = static_cast<int>(i / (128 * NT));
-      const int64_t tl = t0 + static_cast<int64_t>(sl) * S + rank;
+    // a row's 16 R outputs of a tile by neighbouring threads
+    for (int i = threadIdx.x; i < a.recv_slots * 16 * kR * a.M; i += W * 32) {
+      const int n = i % (16 * kR), rest = i / (16 * kR), sl = rest / a.M, m = rest - sl * a.M;
+      const int tl = t0 + sl * S + rank;
       if (tl >= t1) break;
+      // where the owning lane put it: lane 4 (n % 8) + m % 8 / 2, value 2 (n / 8) + m % 2
+      const int at = ((n >> 4) * NT + (m >> 3)) * 128 + ((n & 7) * 4 + (m & 7) / 2) * 4 + (n >> 3 & 1) * 2 + (m & 1);
+      const float* part = reinterpret_cast<const float*>(recv) + sl * S * (kR * NT * 128) + at;
       float v = 0.f;
-      for (int r = 0; r < S; ++r) v += reinterpret_cast<const float*>(recv)[((sl * S + r) * NT + nt) * 128 + e];
-      const int ln = e >> 2, j = e & 3;
-      store_sum(a, tl, (ln >> 2) + (j >> 1) * 8, 8 * nt + 2 * (ln & 3) + (j & 1), v);
+      for (int r = 0; r < S; ++r) v += part[r * (kR * NT * 128)];
+      store_sum(a, static_cast<int64_t>(tl) * kR + (n >> 4), n & 15, m, v);
     }
   }
 }
@@ -533,7 +775,7 @@ struct VecPlan {
 };
 
 // Per device and kernel: its shared-memory limit raised, and how many clusters of each size fit at once.
-template <auto kern>
+template <auto kern, int W>
 int resident_clusters(int S) {
   constexpr int kDevices = 64;
   static std::atomic<int> known[kDevices][4];
@@ -546,11 +788,12 @@ int resident_clusters(int S) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("minisgl.int4_linear: ") + cudaGetErrorString(e));
   if (S == 1) {
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    n *= 16 / W;
   } else {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(S);
-    cfg.blockDim = dim3(kVecWarps * 32);
-    cfg.dynamicSmemBytes = kMaxSmem;
+    cfg.blockDim = dim3(W * 32);
+    cfg.dynamicSmemBytes = kMaxSmem / (16 / W);
     cudaLaunchAttribute at2;
     at2.id = cudaLaunchAttributeClusterDimension;
     at2.val.clusterDim.x = S;
@@ -568,40 +811,47 @@ int resident_clusters(int S) {
 // The cluster size whose busiest CTA has the least to stream: whole tiles
 // are dealt to clusters, so many tiles balance alone (S = 1) and few tiles only
 // when their columns are shared. A cluster's two barriers and exchange cost
-// about as much as kClusterCost units. False: x does not fit shared memory.
+// about as much as kClusterCost KB. False: x does not fit shared memory.
 constexpr int kClusterCost = 30;
-template <int G, auto kern>
+template <typename L, auto kern, int W>
 bool vec_plan(int NT, const VecArgs& a, VecPlan& best) {
   int64_t best_cost = -1;
   for (int S = 1; S <= 8; S *= 2) {
     if (S > a.steps) break;
     VecPlan p;
     p.S = S;
-    p.clusters = std::min(resident_clusters<kern>(S), a.tiles);
+    p.clusters = std::min(resident_clusters<kern, W>(S), a.tiles);
     const int per = (a.tiles + p.clusters - 1) / p.clusters, ks = (a.steps + S - 1) / S;
-    if (static_cast<int64_t>(a.M) * vec_x_pitch(ks) > kMaxSmem) continue;
-    p.x_bytes = a.M * vec_x_pitch(ks);
+    const int64_t x_bytes = static_cast<int64_t>(a.M) * vec_x_pitch(ks) + static_cast<int64_t>(ks) * L::kSide * NT;
+    if (x_bytes > kMaxSmem) continue;
+    p.x_bytes = static_cast<int>(x_bytes);
     p.recv_slots = S > 1 ? (per + S - 1) / S : 0;
     if (p.recv_slots > 4096) continue;
-    p.smem = VecSmem<G>::total(NT, p.x_bytes, p.recv_slots, S);
-    if (p.smem > kMaxSmem) continue;
-    const int64_t cost = static_cast<int64_t>(per) * ks + (S > 1 ? kClusterCost : 0);
+    p.smem = L::total(p.x_bytes, p.recv_slots, S);
+    if (p.smem > kMaxSmem / (16 / W) || static_cast<int64_t>(per) * ks > (1 << 30) / a.steps) continue;  // n * ks stays below 2^31: the reciprocals are exact
+    const int64_t cost = static_cast<int64_t>(per) * ks * L::kR + (S > 1 ? kClusterCost : 0);
     if (best_cost < 0 || cost < best_cost) best_cost = cost, best = p;
   }
   return best_cost >= 0;
 }
 
-template <typename T, bool MX8, int NT, int G, bool ZERO>
+template <int W, int NT, int G, bool ZERO>
 bool launch_vec(VecArgs a, cudaStream_t s) {
-  constexpr auto kern = int4_vec_kernel<T, MX8, NT, G, ZERO>;
+  constexpr auto kern = int4_vec_kernel<W, NT, G, ZERO>;
+  using L = VecSmem<W, NT, G, ZERO>;
+  a.tiles = (a.N + 16 * L::kR - 1) / (16 * L::kR);
   VecPlan p;
-  if (!vec_plan<G, kern>(NT, a, p)) return false;
+  if (!vec_plan<L, kern, W>(NT, a, p)) return false;
   a.S = p.S;
+  a.tiles_each = a.tiles / p.clusters, a.tiles_more = a.tiles % p.clusters;
+  a.steps_each = a.steps / p.S, a.steps_more = a.steps % p.S;
+  a.inv_each = static_cast<uint32_t>(((1ull << 31) + a.steps_each - 1) / a.steps_each);
+  a.inv_more = static_cast<uint32_t>(((1ull << 31) + a.steps_each) / (a.steps_each + 1));
   a.x_bytes = p.x_bytes;
   a.recv_slots = p.recv_slots;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.clusters * p.S));
-  cfg.blockDim = dim3(kVecWarps * 32);
+  cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = p.smem;
   cfg.stream = s;
   cudaLaunchAttribute attrs[2];
@@ -623,18 +873,14 @@ bool launch_vec(VecArgs a, cudaStream_t s) {
   return true;
 }
 
-template <typename T, bool MX8, int NT>
+template <int W, int NT>
 bool launch_vec_group(const VecArgs& a, int group, cudaStream_t s) {
   const bool z = a.zeros != nullptr;
   switch (group) {
-    case 32: return z ? launch_vec<T, MX8, NT, 32, true>(a, s) : launch_vec<T, MX8, NT, 32, false>(a, s);
-    case 64: return z ? launch_vec<T, MX8, NT, 64, true>(a, s) : launch_vec<T, MX8, NT, 64, false>(a, s);
-    default: return z ? launch_vec<T, MX8, NT, 128, true>(a, s) : launch_vec<T, MX8, NT, 128, false>(a, s);
+    case 32: return z ? launch_vec<W, NT, 32, true>(a, s) : launch_vec<W, NT, 32, false>(a, s);
+    case 64: return z ? launch_vec<W, NT, 64, true>(a, s) : launch_vec<W, NT, 64, false>(a, s);
+    default: return z ? launch_vec<W, NT, 128, true>(a, s) : launch_vec<W, NT, 128, false>(a, s);
   }
-}
-template <typename T, bool MX8>
-bool launch_vec_type(const VecArgs& a, int group, cudaStream_t s) {
-  return a.M <= 8 ? launch_vec_group<T, MX8, 1>(a, group, s) : launch_vec_group<T, MX8, 2>(a, group, s);
 }
 
 }  // namespace
@@ -648,13 +894,18 @@ void launch_int4_linear(const Int4LinearArgs& r, cudaStream_t s) {
     v.x = r.x, v.x_scales = r.x_scales, v.packed = r.packed;
     v.scales = static_cast<const uint32_t*>(r.scales), v.zeros = r.zeros, v.bias = r.bias, v.out = r.out;
     v.M = static_cast<int>(r.M), v.N = static_cast<int>(r.N), v.K = static_cast<int>(r.K);
-    v.tiles = (v.N + 15) / 16, v.steps = (v.K + 127) / 128;
+    v.steps = (v.K + 127) / 128;
     v.ldx = r.ldx, v.ld_xs = r.ld_xs, v.ldo = r.ldo;
     v.scale_half = r.scale_type == DType::kF16;
     v.bias_type = static_cast<int>(r.bias_type), v.out_type = static_cast<int>(r.out_type);
-    const bool done = r.x_scales != nullptr         ? launch_vec_type<__nv_bfloat16, true>(v, r.group, s)
-                      : r.x_type == DType::kF16 ? launch_vec_type<__half, false>(v, r.group, s)
-                                                : launch_vec_type<__nv_bfloat16, false>(v, r.group, s);
+    v.x_kind = r.x_scales != nullptr ? kXMx8 : r.x_type == DType::kF16 ? kXHalf : kXBf16;
+    // Few codes (up to kSmallSteps KB): CTAs of 8 warps, two of which fit an SM, so that the next kernel's start
+    // overlaps this one's end; more: one CTA of 16 warps, which stages x once per SM. B200, one row: 4096 x 4096
+    // 7.6 us against 8.7, 2048 x 1024 4.1 against 5.1; 12301 x 4168 18.4 against 16.0, 5120 x 25600 30.2 against 19.0.
+    constexpr int64_t kSmallSteps = 12 * 1024;
+    const bool small = (static_cast<int64_t>(v.N) + 15) / 16 * v.steps <= kSmallSteps;
+    const bool done = v.M > 8 ? launch_vec_group<16, 2>(v, r.group, s)
+                              : (small && launch_vec_group<8, 1>(v, r.group, s)) || launch_vec_group<16, 1>(v, r.group, s);
     if (done) return;
   }
   LinArgs a{};

@@ -450,9 +450,9 @@ void launch_act_mx8(const ActMx8Args& a, cudaStream_t s);
 struct Int4LinearArgs {
   const void* x;            // bf16 / fp16 [M, K] (row stride ldx), or E4M3 bytes
   const uint8_t* x_scales;  // E8M0 [M, K / 32] (row stride ld_xs) or nullptr
-  const uint8_t* packed;    // [ceil(N / 16), 2 ceil(K / 128), 512]
-  const void* scales;       // bf16 / fp16 [ceil(N / 16), groups, 8, 2]
-  const uint8_t* zeros;     // [ceil(N / 16), groups, 8] or nullptr (8 everywhere)
+  const uint8_t* packed;    // [tiles = 2 ceil(N / 32), 2 ceil(K / 128), 512]
+  const void* scales;       // bf16 / fp16 [tiles, groups, 8, 2]
+  const uint8_t* zeros;     // [tiles, groups, 8] or nullptr (8 everywhere)
   const void* bias;         // [N] or nullptr
   void* out;                // [M, N], row stride ldo
   int64_t M, N, K;

@@ -372,7 +372,7 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
     ``silu_and_mul_mx8`` return them. out: bf16, fp16 or fp32 (default: x's
     type, bf16 for MXFP8 rows). Sums are held in fp32; a group's sum of
     x * (code - zero) is formed before its scale is applied, so
-    |x| * 15 * group has to stay inside fp32."""
+  """
     if x.dim() != 2 or x.shape[1] != w.k:
         raise ValueError(f"int4_linear: x must be [M, {w.k}], got {tuple(x.shape)}")
     if (x.dtype == torch.uint8) != (x_scales is not None):

@@ -11,18 +11,19 @@ the form in which group-quantised checkpoints come: ``int4_weight`` takes the
 codes packed two per byte and lays them out once for the kernels
 (``minisgl/csrc/int4.cu``); ``quantize_int4`` makes them from a float weight.
 
-Layout. Rows are cut into tiles of 16, columns into blocks of 64 (an even
-number: columns are padded to 128); tile and block fill 512 bytes, 16 for each
-lane of a warp. Lane 4 g + t holds rows g and
-g + 8, columns 8 t .. 8 t + 7 of either half (32 columns) of the block, in four
-words; word j = 2 i + l has columns 32 i + 8 t + 4 l + 2 p + e of row g + 8 h at
-bit 4 (4 e + 2 p + h): masked with 0x000F000F after a shift by 4 r, a word gives
-the r-th of the four registers (two 16-bit values each) that a warp-level
-16 x 8 x 16 product takes of its first operand, in the order in which a lane's
-two runs of 8 values of x fill the second. A word's columns lie in one half, so
-no product mixes two groups. Scales are [tile, group, g, h], so that a lane's
-two are one word, zero points [tile, group, g] with z[g] | z[g + 8] << 4.
-Padding rows and columns have scale 0 and code 0.
+Layout. Rows are cut into tiles of 16, columns into blocks of 64, both an even
+number (rows are padded to 32, columns to 128); tile and block fill 512 bytes,
+16 for each lane of a warp. Lane 4 g + t holds rows g and g + 8, columns 8 t ..
+8 t + 7 of either half (32 columns) of the block, in four words; word
+j = 2 i + l has columns 32 i + 8 t + 4 l + 2 p + e of row g + 8 h at bit
+4 (4 e + 2 p + h), as c - 8 in two's complement. A byte's upper half is thus a
+signed code of row g + 8 (of row g after a shift by 4), and a word gives two of
+the four registers (four 8-bit values each) that a warp-level 16 x 8 x 32
+product takes of its first operand, in the order in which a lane's runs of 8
+values of x fill the second. A word's columns lie in one half, so no product
+mixes two groups. Scales are [tile, group, g, h], so that a lane's two are one
+word, zero points [tile, group, g] with z[g] | z[g + 8] << 4. Padding rows and
+columns have scale 0.
 
 The reference has no weight quantisation; its projections run bf16 library
 GEMMs (python/minisgl/layers/linear.py:13-127).
@@ -35,14 +36,18 @@ from typing import Optional
 import torch
 
 GROUPS = (32, 64, 128)
-_TILE, _BLOCK, _STEP = 16, 64, 128
+_TILE, _BLOCK, _STEP = 16, 64, 128  # rows are padded to two tiles, columns to a step
+
+
+def _tiles(n: int) -> int:
+    return 2 * -(-n // (2 * _TILE))
 
 
 class Int4Weight:
     """A 4-bit weight in the kernels' layout (made by ``int4_weight`` or
-    ``quantize_int4``): ``packed`` uint8 [ceil(N / 16), 2 ceil(K / 128), 512],
-    ``scales`` bf16 / fp16 [ceil(N / 16), groups, 8, 2] and ``zeros`` uint8
-    [ceil(N / 16), groups, 8] or None, groups = 128 ceil(K / 128) / group."""
+    ``quantize_int4``): ``packed`` uint8 [tiles, 2 ceil(K / 128), 512],
+    ``scales`` bf16 / fp16 [tiles, groups, 8, 2] and ``zeros`` uint8
+    [tiles, groups, 8] or None, tiles = 2 ceil(N / 32), groups = 128 ceil(K / 128) / group."""
 
     __slots__ = ("packed", "scales", "zeros", "n", "k", "group")
 
@@ -61,9 +66,9 @@ class Int4Weight:
 
 
 def _tile_rows(t: torch.Tensor, groups: int) -> torch.Tensor:
-    """[N, groups of K] -> [ceil(N / 16), groups, 8, 2] (row g + 8 h at [g, h]), padded with zeros."""
+    """[N, groups of K] -> [tiles, groups, 8, 2] (row g + 8 h at [g, h]), padded with zeros."""
     n, g = t.shape
-    tiles = -(-n // _TILE)
+    tiles = _tiles(n)
     full = t.new_zeros(tiles * _TILE, groups)
     full[:n, :g] = t
     return full.view(tiles, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
@@ -90,7 +95,7 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
         raise ValueError("int4_weight: codes, scales and zeros must be on one device")
     if zeros is not None and bool((zeros > 15).any()):
         raise ValueError("int4_weight: zero points must be 0..15")
-    tiles, blocks = -(-n // _TILE), 2 * -(-k // _STEP)
+    tiles, blocks = _tiles(n), 2 * -(-k // _STEP)
     if tiles * _TILE != n or blocks * _BLOCK != k:
         full = codes.new_zeros(tiles * _TILE, blocks * _BLOCK // 2)
         full[:n, : k // 2] = codes
@@ -103,6 +108,7 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
     packed = torch.empty(tiles, blocks, 8, 4, 2, 2, 2, 2, dtype=torch.uint8, device=codes.device)
     packed[..., 0, :] = (top & 15) | (low << 4)
     packed[..., 1, :] = (top >> 4) | (low & 0xF0)
+    packed ^= 0x88  # c - 8, two's complement
     groups = blocks * _BLOCK // group
     z = None
     if zeros is not None:
@@ -114,7 +120,7 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
 def int4_codes(w: Int4Weight) -> torch.Tensor:
     """The codes of a weight, uint8 [N, K]."""
     tiles, blocks = w.packed.shape[:2]
-    b = w.packed.view(tiles, blocks, 8, 4, 2, 2, 2, 2)  # [tile, block, g, t, i, l, e, p]
+    b = (w.packed ^ 0x88).view(tiles, blocks, 8, 4, 2, 2, 2, 2)  # [tile, block, g, t, i, l, e, p]
     c = torch.stack([b & 15, b >> 4], dim=-1)           # ..., h
     c = c.permute(0, 8, 2, 1, 4, 3, 5, 7, 6)            # [tile, h, g, block, i, t, l, p, e]
     return c.reshape(tiles * _TILE, blocks * _BLOCK)[: w.n, : w.k]
