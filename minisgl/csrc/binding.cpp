@@ -574,7 +574,8 @@ void act_mx8(at::Tensor q, at::Tensor sf, const at::Tensor& x, int64_t act, bool
 // ---------------------------------------------------------- 4-bit linear ----
 void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Tensor>& x_scales,
                  const at::Tensor& packed, const at::Tensor& scales, const c10::optional<at::Tensor>& zeros,
-                 const c10::optional<at::Tensor>& bias, int64_t N, int64_t K, int64_t group) {
+                 const at::Tensor& row_pow, const c10::optional<at::Tensor>& bias, int64_t N, int64_t K, int64_t group,
+                 const c10::optional<at::Tensor>& x_wide, const c10::optional<at::Tensor>& err) {
   MSG_CHECK(group == 32 || group == 64 || group == 128, "int4_linear: group of 32, 64 or 128, got ", group);
   MSG_CHECK(x.dim() == 2 && x.size(1) == K, "int4_linear: x must be [M, ", K, "], got ", x.sizes());
   check_cuda(x, "x");
@@ -606,6 +607,18 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
             "int4_linear: weight scales of the wrong type or size");
   check_same_device(x, packed);
   check_same_device(x, scales);
+  MSG_CHECK(row_pow.is_cuda() && row_pow.scalar_type() == at::kFloat && row_pow.is_contiguous() &&
+                row_pow.numel() == tiles * 16,
+            "int4_linear: row powers of the wrong type or size");
+  check_same_device(x, row_pow);
+  if (x_scales.has_value() && M > 16) {
+    MSG_CHECK(x_wide.has_value() && x_wide->is_cuda() && x_wide->scalar_type() == at::kBFloat16 &&
+                  x_wide->is_contiguous() && x_wide->numel() >= M * K &&
+                  reinterpret_cast<uintptr_t>(x_wide->data_ptr()) % 16 == 0,
+              "int4_linear: bf16 scratch of M * K for more than 16 MXFP8 rows");
+    check_same_device(x, *x_wide);
+    a.x_wide = x_wide->data_ptr();
+  }
   if (zeros.has_value()) {
     MSG_CHECK(zeros->is_cuda() && zeros->scalar_type() == at::kByte && zeros->is_contiguous() &&
                   zeros->numel() == tiles * groups * 8 && reinterpret_cast<uintptr_t>(zeros->data_ptr()) % 16 == 0,
@@ -628,6 +641,7 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
   a.x = x.data_ptr();
   a.packed = packed.data_ptr<uint8_t>();
   a.scales = scales.data_ptr();
+  a.row_pow = row_pow.data_ptr<float>();
   a.out = out.data_ptr();
   a.M = M;
   a.N = N;
@@ -637,6 +651,7 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
   a.group = static_cast<int>(group);
   a.scale_type = dtype_of(scales);
   a.out_type = dtype_of(out);
+  a.err = err_ptr(err);
   const c10::cuda::CUDAGuard guard(x.device());
   minisgl::launch_int4_linear(a, stream_of(x));
 }

@@ -1,0 +1,596 @@
+// Products of many rows with 4-bit weights under group scales (int4.cu has
+// few rows): out[m, n] = sum_k x[m, k] W[n, k] (+ bias[n]) on the 5th-generation
+// tensor cores. Weight layout: minisgl/quant/int4.py.
+//
+// One persistent CTA per SM walks tiles of 128 weight rows x BN rows of x
+// (weights are the 128-row first operand, so that the 4-bit side is unpacked
+// as rarely as possible: once per BN rows of x). Per 64 columns eight
+// converter warps turn 128 x 64 codes into a bf16 (fp16) operand tile in shared
+// memory, four MMAs consume it together with a TMA tile of x, and the sums stay
+// in tensor memory; two accumulators alternate, so that four epilogue warps
+// store one tile while the next is multiplied.
+//
+//   warp 0      x by TMA, a ring of kXs tiles of 64 columns
+//   warp 1      issues the MMAs
+//   warp 2      codes by bulk copies, a ring of kPs steps of 128 columns (8 KB)
+//   warps 4-7   epilogue (tensor-memory lanes 32 (w % 4) ..)
+//   warps 8-15  converters, 16 weight rows each
+//
+// W = (c - z) s is rounded once to bf16 (fp16): the one rounding besides those
+// of the float32 sums. fp16 weights are formed under each row's own power of
+// two, so that neither large nor tiny scales leave fp16's range.
+//
+// Few tiles (N small, M small): S CTAs of a cluster share a tile's columns and
+// add their sums through shared memory in rank order.
+//
+// Every wait is bounded: a timeout records an error, raises an abort flag that
+// the other roles check, and the CTA drains its copies and returns.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <atomic>
+#include <stdexcept>
+#include <string>
+
+#include "common.cuh"
+#include "launch.h"
+#include "ops.h"
+#include "tma_host.h"
+
+namespace minisgl {
+namespace {
+
+constexpr int kRows = 128;       // weight rows of a tile
+constexpr int kThreads = 512;
+constexpr int kConverters = 8;
+constexpr int kAs = 3;           // operand tiles between converters and MMAs
+constexpr int kATile = kRows * 128;
+constexpr int kCodes = 8 * 1024;  // 128 rows x 128 columns
+
+template <int BN>
+struct GSmem {
+  static constexpr int kX = BN * 128;  // one 64-column tile of x
+  static constexpr int kXs = 4;
+  static constexpr int kPs = BN == 256 ? 3 : 6;
+  static constexpr int kAt = 0;
+  static constexpr int kXt = kAs * kATile;
+  static constexpr int kPt = kXt + kXs * kX;
+  static constexpr int kRing = kPt + kPs * kCodes;
+  static constexpr int kBars = 8 * (2 * kXs + 2 * kPs + 2 * kAs + 4) + 16;
+  static constexpr int bytes(int S) { return 1024 + kRing + (kBars + 127) / 128 * 128 + (S > 1 ? kRows * BN * 4 : 0); }
+  static constexpr uint32_t kCols = 2 * BN < 32 ? 32 : 2 * BN;
+};
+
+struct GArgs {
+  const uint8_t* packed;
+  const uint32_t* scales;
+  const uint8_t* zeros;
+  const float* row_pow;  // fp16: power of two taken out of a row's scales
+  const void* bias;
+  void* out;
+  int M, N, steps, tiles16;
+  int m_tiles, n_tiles, S;
+  int64_t ldo;
+  int scale_half, bias_type, out_type;
+  ErrorSink err;
+};
+
+__device__ __forceinline__ float scale_f32(uint32_t bits, int is_half) {
+  return is_half ? __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) : __uint_as_float(bits << 16);
+}
+__device__ __forceinline__ float any_f32(const void* p, int64_t i, int type) {
+  if (type == static_cast<int>(DType::kF32)) return static_cast<const float*>(p)[i];
+  if (type == static_cast<int>(DType::kF16)) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int64_t i, int type, float v) {
+  if (type == static_cast<int>(DType::kF32))
+    static_cast<float*>(p)[i] = v;
+  else if (type == static_cast<int>(DType::kF16))
+    static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else
+    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Pairs of 16-bit floats: a code under an exponent, exactly code - zero, times the scale.
+template <bool HALF>
+struct Pair {
+  static constexpr uint32_t kBase = HALF ? 0x64086408u : 0x43084308u;  // 1024 | 8 or 128 | 8: codes are stored as c ^ 8
+  __device__ static uint32_t zero(uint32_t z) { return ((HALF ? 0x6400u : 0x4300u) + z) * 0x10001u; }
+  __device__ static uint32_t code(uint32_t w) {  // (w & 0x000F000F) ^ base
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(d) : "r"(w), "r"(0x000F000Fu), "r"(kBase));
+    return d;
+  }
+  __device__ static uint32_t sub(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (HALF)
+      asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else
+      asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  __device__ static uint32_t mul(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (HALF)
+      asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else
+      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+};
+
+template <int BN, int G, bool HALF>
+__global__ void __launch_bounds__(kThreads, 1)
+    int4_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const GArgs a) {
+  using L = GSmem<BN>;
+  constexpr int P = 128 / G;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* xfull = reinterpret_cast<uint64_t*>(smem + L::kRing);
+  uint64_t* xempty = xfull + L::kXs;
+  uint64_t* pfull = xempty + L::kXs;
+  uint64_t* pempty = pfull + L::kPs;
+  uint64_t* afull = pempty + L::kPs;
+  uint64_t* aempty = afull + kAs;
+  uint64_t* acc_full = aempty + kAs;   // [2]
+  uint64_t* acc_empty = acc_full + 2;  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
+  float* recv = reinterpret_cast<float*>(smem + L::kRing + (L::kBars + 127) / 128 * 128);  // [rank][BN / S][128]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = a.S, rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int first = static_cast<int>(blockIdx.x) / S, stride = static_cast<int>(gridDim.x) / S;
+  const int num_tiles = a.m_tiles * a.n_tiles;
+  const int k0 = static_cast<int>(static_cast<int64_t>(a.steps) * rank / S);
+  const int k1 = static_cast<int>(static_cast<int64_t>(a.steps) * (rank + 1) / S);
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::kXs; ++s) mbar_init(&xfull[s], 1), mbar_init(&xempty[s], 1);
+    for (int s = 0; s < L::kPs; ++s) mbar_init(&pfull[s], 1), mbar_init(&pempty[s], kConverters);
+    for (int s = 0; s < kAs; ++s) mbar_init(&afull[s], kConverters), mbar_init(&aempty[s], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 4);
+    *s_abort = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tm_x);
+  }
+  // the first codes, on their way to L2 while the kernel before this one ends (a prefetch carries no value)
+  if (warp >= 8 && first < num_tiles) {
+    const int tile16 = first / a.m_tiles * 8 + warp - 8;
+    if (tile16 < a.tiles16 && k0 + (lane >> 3) < k1)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(
+          a.packed + (static_cast<int64_t>(tile16) * a.steps + k0 + (lane >> 3)) * 1024 + (lane & 7) * 128));
+  }
+  pdl_wait();
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, L::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (S > 1) cluster_sync();  // the peers have started: their shared memory may be written
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  volatile int* abort_flag = s_abort;
+  int issued = 0;  // copies this thread has started (warps 0 and 2)
+
+  if (warp == 0) {
+    // -------------------------------------------------------------- x ----
+    if (lane == 0) {
+      int it = 0;
+      for (int tile = first; tile < num_tiles && !*abort_flag; tile += stride) {
+        const int m0 = tile % a.m_tiles * BN;
+        for (int kb = 2 * k0; kb < 2 * k1; ++kb, ++it) {
+          const int s = it % L::kXs;
+          if (it >= L::kXs && !mbar_wait(&xempty[s], ((it / L::kXs) - 1) & 1, a.err, 421)) {
+            *abort_flag = 1;
+            break;
+          }
+          mbar_arrive_expect_tx(&xfull[s], L::kX);
+          tma_load_2d(smem + L::kXt + s * L::kX, &tm_x, &xfull[s], kb * 64, m0);
+          issued = it + 1;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ---------------------------------------------------------- codes ----
+    if (lane == 0) {
+      int it = 0;
+      for (int tile = first; tile < num_tiles && !*abort_flag; tile += stride) {
+        const int t16 = tile / a.m_tiles * 8;
+        const int count = min(8, a.tiles16 - t16);
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % L::kPs;
+          if (it >= L::kPs && !mbar_wait(&pempty[s], ((it / L::kPs) - 1) & 1, a.err, 422)) {
+            *abort_flag = 1;
+            break;
+          }
+          mbar_arrive_expect_tx(&pfull[s], count * 1024);
+          for (int c = 0; c < count; ++c)
+            bulk_load(smem + L::kPt + s * kCodes + c * 1024,
+                      a.packed + (static_cast<int64_t>(t16 + c) * a.steps + k) * 1024, 1024, &pfull[s]);
+          issued = it + 1;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA ----
+    // instruction descriptor: float32 sums, 128 x BN, both operands K-major and of one 16-bit type
+    constexpr uint32_t idesc = HALF ? make_idesc_bf16(kRows, BN) & ~((1u << 7) | (1u << 10)) : make_idesc_bf16(kRows, BN);
+    const uint32_t base = smem_u32(smem);
+    int it = 0, lt = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < num_tiles; tile += stride, ++lt) {
+      const int acc = lt & 1;
+      if (lt >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], ((lt >> 1) - 1) & 1, a.err, 423));
+      if (!ok) break;
+      tc_fence_after();
+      for (int kb = 2 * k0; kb < 2 * k1; ++kb, ++it) {
+        const int xs = it % L::kXs, as = it % kAs;
+        ok = __all_sync(0xffffffffu, mbar_wait(&xfull[xs], (it / L::kXs) & 1, a.err, 424) &&
+                                         mbar_wait(&afull[as], (it / kAs) & 1, a.err, 425));
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t wa = base + L::kAt + as * kATile, xa = base + L::kXt + xs * L::kX;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16(tmem + acc * BN, make_sdesc_k_sw128(wa + k * 32), make_sdesc_k_sw128(xa + k * 32), idesc,
+                       (kb > 2 * k0 || k > 0) ? 1u : 0u);
+          tc_commit(&xempty[xs]);
+          tc_commit(&aempty[as]);
+        }
+        __syncwarp();
+      }
+      if (ok && lane == 0) tc_commit(&acc_full[acc]);
+      __syncwarp();
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+    __syncwarp();
+  } else if (warp >= 8) {
+    // ----------------------------------------------------- converters ----
+    const int c16 = warp - 8, g = lane >> 2, t = lane & 3;
+    // odd rows store their second 32 columns first: the eight lanes of a quarter warp hit distinct banks
+    const bool flip = g & 1;
+    const uint32_t row_at = (16 * c16 + g) * 128;
+    const uint32_t at0 = row_at + (((flip ? 4 + t : t) ^ g) << 4), at1 = row_at + (((flip ? t : 4 + t) ^ g) << 4);
+    int it = 0, pit = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < num_tiles; tile += stride) {
+      const int tile16 = min(tile / a.m_tiles * 8 + c16, a.tiles16 - 1);  // rows past N: any codes, never stored
+      const uint32_t* sp = a.scales + (static_cast<int64_t>(tile16) * a.steps * P) * 8 + g;
+      const uint8_t* zp = a.zeros != nullptr ? a.zeros + (static_cast<int64_t>(tile16) * a.steps * P) * 8 + g : nullptr;
+      float down0 = 1.f, down1 = 1.f;  // 1 / the rows' power of two
+      if constexpr (HALF) down0 = 1.f / a.row_pow[tile16 * 16 + g], down1 = 1.f / a.row_pow[tile16 * 16 + g + 8];
+      uint32_t sc[P], zz[P], sc_next[P], zz_next[P];
+      auto load_scales = [&](int k, uint32_t (&sv)[P], uint32_t (&zv)[P]) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          sv[p] = sp[(k * P + p) * 8];
+          zv[p] = zp != nullptr ? zp[(k * P + p) * 8] : 0x88u;
+        }
+      };
+      load_scales(k0, sc_next, zz_next);
+      for (int k = k0; k < k1 && ok; ++k, ++pit) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) sc[p] = sc_next[p], zz[p] = zz_next[p];
+        if (k + 1 < k1) load_scales(k + 1, sc_next, zz_next);
+        const int ps = pit % L::kPs;
+        ok = __all_sync(0xffffffffu, mbar_wait(&pfull[ps], (pit / L::kPs) & 1, a.err, 426));
+        if (!ok) break;
+        const uint4* codes = reinterpret_cast<const uint4*>(smem + L::kPt + ps * kCodes + c16 * 1024) + lane;
+        const uint4 w[2] = {codes[0], codes[32]};
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pempty[ps]);  // the codes are in registers
+#pragma unroll
+        for (int h = 0; h < 2; ++h, ++it) {
+          const int as = it % kAs;
+          if (it >= kAs) ok = __all_sync(0xffffffffu, mbar_wait(&aempty[as], ((it / kAs) - 1) & 1, a.err, 427));
+          if (!ok) break;
+          uint8_t* dst = smem + L::kAt + as * kATile;
+          // first and second run of 8 columns in this lane's order
+          const uint32_t words[4] = {flip ? w[h].z : w[h].x, flip ? w[h].w : w[h].y, flip ? w[h].x : w[h].z, flip ? w[h].y : w[h].w};
+#pragma unroll
+          for (int run = 0; run < 2; ++run) {
+            constexpr int kHalf = P == 4 ? 2 : 1;  // groups of 64 columns
+            const int p0 = P == 1 ? 0 : kHalf * h;
+            uint32_t sw, zw;
+            if constexpr (P == 4) {
+              sw = (run == 0) != flip ? sc[p0] : sc[p0 + 1];
+              zw = (run == 0) != flip ? zz[p0] : zz[p0 + 1];
+            } else {
+              sw = sc[p0], zw = zz[p0];
+            }
+            const uint32_t z[2] = {Pair<HALF>::zero(zw & 15u), Pair<HALF>::zero(zw >> 4)};
+            uint32_t o[2][4];  // [row g, row g + 8][column pair]
+            const bool exact_scale = HALF || !a.scale_half;
+            uint32_t s[2];
+            if constexpr (HALF) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const __half q = __float2half_rn(scale_f32(r ? sw >> 16 : sw & 0xFFFFu, a.scale_half) * (r ? down1 : down0));
+                s[r] = static_cast<uint32_t>(__half_as_ushort(q)) * 0x10001u;
+              }
+            } else {
+              s[0] = __byte_perm(sw, 0, 0x1010), s[1] = __byte_perm(sw, 0, 0x3232);
+            }
+#pragma unroll
+            for (int l = 0; l < 2; ++l) {
+              const uint32_t word = words[2 * run + l];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {  // r: bit 0 the row half, bit 1 the column pair
+                const uint32_t d = Pair<HALF>::sub(Pair<HALF>::code(word >> (4 * r)), z[r & 1]);
+                o[r & 1][2 * l + (r >> 1)] = d;
+              }
+            }
+            if (exact_scale) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[r][i] = Pair<HALF>::mul(o[r][i], s[r]);
+            } else {
+              // fp16 scales do not fit bf16: the product is formed in float32 and rounded once
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const float f = scale_f32(r ? sw >> 16 : sw & 0xFFFFu, 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  o[r][i] = pack_bf16x2(__uint_as_float(o[r][i] << 16) * f, __uint_as_float(o[r][i] & 0xFFFF0000u) * f);
+              }
+            }
+            const uint32_t at = run == 0 ? at0 : at1;
+            *reinterpret_cast<uint4*>(dst + at) = make_uint4(o[0][0], o[0][1], o[0][2], o[0][3]);
+            *reinterpret_cast<uint4*>(dst + at + 8 * 128) = make_uint4(o[1][0], o[1][1], o[1][2], o[1][3]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&afull[as]);
+        }
+      }
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ------------------------------------------------------- epilogue ----
+    const int quad = warp & 3, row = 32 * quad + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * quad) << 16);
+    int lt = 0;
+    bool ok = true;
+    for (int tile = first; tile < num_tiles; tile += stride, ++lt) {
+      const int acc = lt & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (lt >> 1) & 1, a.err, 428));
+      if (!ok) break;
+      tc_fence_after();
+      const int m0 = tile % a.m_tiles * BN;
+      const int64_t n = static_cast<int64_t>(tile / a.m_tiles) * kRows + row;
+      const bool in = n < a.N;
+      const float bias = in && a.bias != nullptr ? any_f32(a.bias, n, a.bias_type) : 0.f;
+      const float pow = HALF && in ? a.row_pow[n] : 1.f;
+      constexpr int CH = BN < 32 ? 16 : 32;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += CH) {
+        uint32_t r[32];
+        if constexpr (CH == 32)
+          tmem_ld_32x32b_x32(lane_base + acc * BN + c, r);
+        else
+          tmem_ld_32x32b_x16(lane_base + acc * BN + c, *reinterpret_cast<uint32_t(*)[16]>(r));
+        tc_wait_ld();
+        if (c + CH >= BN) {  // the accumulator is read out: the MMAs may reuse it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[acc]);
+        }
+        if (S > 1) {
+          const int per = BN / S;  // rows of x that a CTA of the cluster finishes
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            const uint32_t dst = map_shared_rank(smem_u32(recv + (rank * per + (c + j) % per) * kRows + row), (c + j) / per);
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(__uint_as_float(r[j])) : "memory");
+          }
+        } else if (in) {
+          // neighbouring lanes are neighbouring outputs of one row
+#pragma unroll
+          for (int j = 0; j < CH; ++j)
+            if (m0 + c + j < a.M)
+              store_any(a.out, static_cast<int64_t>(m0 + c + j) * a.ldo + n, a.out_type, __uint_as_float(r[j]) * pow + bias);
+        }
+      }
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && lane == 0) {
+    // after an abort, let the copies still in flight land (bounded)
+    if (warp == 0)
+      for (int it = max(0, issued - L::kXs); it < issued; ++it) mbar_wait(&xfull[it % L::kXs], (it / L::kXs) & 1, a.err, 429);
+    if (warp == 2)
+      for (int it = max(0, issued - L::kPs); it < issued; ++it) mbar_wait(&pfull[it % L::kPs], (it / L::kPs) & 1, a.err, 430);
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kCols);
+  }
+  if (S > 1) {
+    // one tile per cluster: this CTA's BN / S rows of x, the S partial sums in rank order
+    __syncwarp();
+    cluster_sync();
+    const int per = BN / S;
+    const int m0 = first % a.m_tiles * BN + rank * per;
+    const int64_t n0 = static_cast<int64_t>(first / a.m_tiles) * kRows;
+    for (int i = threadIdx.x; i < per * kRows; i += kThreads) {
+      const int m = m0 + i / kRows;
+      const int64_t n = n0 + i % kRows;
+      if (m >= a.M || n >= a.N || *abort_flag) continue;
+      float v = 0.f;
+      for (int r = 0; r < S; ++r) v += recv[r * per * kRows + i];
+      if (HALF) v *= a.row_pow[n];
+      if (a.bias != nullptr) v += any_f32(a.bias, n, a.bias_type);
+      store_any(a.out, static_cast<int64_t>(m) * a.ldo + n, a.out_type, v);
+    }
+  }
+}
+
+// MXFP8 rows as bf16: four significant bits times a power of two are exact
+__global__ void __launch_bounds__(256) mx8_rows_bf16_kernel(uint4* out, const uint8_t* q, const uint8_t* sf, int64_t rows,
+                                                          int K, int64_t ldq, int64_t ldsf) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int runs = K / 8;
+  const int64_t total = rows * runs;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t m = i / runs;
+    const int c = static_cast<int>(i - m * runs) * 8;
+    const uint2 v = *reinterpret_cast<const uint2*>(q + m * ldq + c);
+    const uint32_t byte = sf[m * ldsf + c / 32];
+    const float s = __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
+    uint32_t r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
+          static_cast<__nv_fp8x2_storage_t>((j < 2 ? v.x : v.y) >> (16 * (j & 1))), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      r[j] = pack_bf16x2(f.x * s, f.y * s);
+    }
+    out[i] = make_uint4(r[0], r[1], r[2], r[3]);
+  }
+}
+
+struct GPlan {
+  int S, grid;
+};
+
+template <auto kern>
+int resident(int S, int smem) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices][4];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int at = S == 1 ? 0 : S == 2 ? 1 : S == 4 ? 2 : 3;
+  int n = dev < kDevices ? known[dev][at].load() : 0;
+  if (n > 0) return n;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e == cudaSuccess && S == 1) {
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  } else if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = S;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+  }
+  if (e != cudaSuccess || n < 1)
+    throw std::runtime_error(std::string("minisgl.int4_linear: ") + (e != cudaSuccess ? cudaGetErrorString(e) : "the kernel does not fit this device"));
+  if (dev < kDevices) known[dev][at].store(n);
+  return n;
+}
+
+template <int BN, int G, bool HALF>
+void launch_bn(GArgs a, const CUtensorMap& tm, cudaStream_t s) {
+  constexpr auto kern = int4_gemm_kernel<BN, G, HALF>;
+  using L = GSmem<BN>;
+  a.m_tiles = (a.M + BN - 1) / BN;
+  const int64_t tiles = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
+  a.S = 1;
+  int grid = static_cast<int>(std::min<int64_t>(tiles, resident<kern>(1, L::bytes(1))));
+  if constexpr (BN <= 64) {
+    // columns shared by as many CTAs as leave every cluster resident and each CTA at least two steps
+    for (int S = 2; S <= 8; S *= 2)
+      if (a.steps >= 2 * S && tiles <= resident<kern>(S, L::bytes(S))) a.S = S, grid = static_cast<int>(tiles) * S;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = L::bytes(a.S);
+  cfg.stream = s;
+  cudaLaunchAttribute attrs[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (a.S > 1) {
+    attrs[n].id = cudaLaunchAttributeClusterDimension;
+    attrs[n].val.clusterDim.x = a.S;
+    attrs[n].val.clusterDim.y = attrs[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attrs;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tm, a);
+  if (e != cudaSuccess) throw std::runtime_error(std::string("minisgl: kernel launch failed: ") + cudaGetErrorString(e));
+}
+
+template <int BN, bool HALF>
+void launch_group(const GArgs& a, const CUtensorMap& tm, int group, cudaStream_t s) {
+  switch (group) {
+    case 32: launch_bn<BN, 32, HALF>(a, tm, s); break;
+    case 64: launch_bn<BN, 64, HALF>(a, tm, s); break;
+    default: launch_bn<BN, 128, HALF>(a, tm, s); break;
+  }
+}
+
+template <bool HALF>
+void launch_type(const GArgs& a, const void* x, int64_t ldx, int64_t K, int group, cudaStream_t s) {
+  // rows of x per tile: the size with the least time in the busiest CTA, per 64 columns 2 cycles per row of x in
+  // the tensor cores against about kConvert to unpack 128 weight rows
+  constexpr int kConvert = 250;
+  const int sms = 148;
+  int best = 256;
+  int64_t best_cost = -1;
+  for (int bn : {256, 128, 64, 32}) {
+    const int64_t tiles = (static_cast<int64_t>(a.M) + bn - 1) / bn * a.n_tiles;
+    const int64_t cost = (tiles + sms - 1) / sms * std::max(2 * bn, kConvert);
+    if (best_cost < 0 || cost < best_cost || (cost == best_cost && bn >= a.M)) best = bn, best_cost = cost;
+  }
+  const CUtensorMap tm = make_tmap_bf16_2d_sw128(x, static_cast<uint64_t>(a.M), static_cast<uint64_t>(K),
+                                                 static_cast<uint64_t>(ldx), static_cast<uint32_t>(best));
+  switch (best) {
+    case 32: launch_group<32, HALF>(a, tm, group, s); break;
+    case 64: launch_group<64, HALF>(a, tm, group, s); break;
+    case 128: launch_group<128, HALF>(a, tm, group, s); break;
+    default: launch_group<256, HALF>(a, tm, group, s); break;
+  }
+}
+
+}  // namespace
+
+void launch_int4_gemm(const Int4LinearArgs& r, cudaStream_t s) {
+  GArgs a{};
+  a.packed = r.packed, a.scales = static_cast<const uint32_t*>(r.scales), a.zeros = r.zeros, a.row_pow = r.row_pow;
+  a.bias = r.bias, a.out = r.out;
+  a.M = static_cast<int>(r.M), a.N = static_cast<int>(r.N);
+  a.steps = static_cast<int>((r.K + 127) / 128), a.tiles16 = static_cast<int>(2 * ((r.N + 31) / 32));
+  a.n_tiles = static_cast<int>((r.N + kRows - 1) / kRows);
+  a.ldo = r.ldo;
+  a.scale_half = r.scale_type == DType::kF16;
+  a.bias_type = static_cast<int>(r.bias_type), a.out_type = static_cast<int>(r.out_type);
+  a.err = ErrorSink{r.err};
+  const void* x = r.x;
+  int64_t ldx = r.M > 1 ? r.ldx : r.K;
+  if (r.x_scales != nullptr) {
+    const int64_t runs = r.M * (r.K / 8);
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((runs + 255) / 256, 148 * 8));
+    launch_pdl(mx8_rows_bf16_kernel, dim3(blocks), dim3(256), 0, s, static_cast<uint4*>(r.x_wide),
+               static_cast<const uint8_t*>(r.x), r.x_scales, r.M, static_cast<int>(r.K), r.ldx, r.ld_xs);
+    x = r.x_wide;
+    ldx = r.K;
+  }
+  if (r.x_scales == nullptr && r.x_type == DType::kF16)
+    launch_type<true>(a, x, ldx, r.K, r.group, s);
+  else
+    launch_type<false>(a, x, ldx, r.K, r.group, s);
+}
+
+}  // namespace minisgl

@@ -453,14 +453,18 @@ struct Int4LinearArgs {
   const uint8_t* packed;    // [tiles = 2 ceil(N / 32), 2 ceil(K / 128), 512]
   const void* scales;       // bf16 / fp16 [tiles, groups, 8, 2]
   const uint8_t* zeros;     // [tiles, groups, 8] or nullptr (8 everywhere)
+  const float* row_pow;     // [16 tiles]: a power of two near each row's largest scale
   const void* bias;         // [N] or nullptr
+  void* x_wide;             // E4M3 rows of more than int4_few_rows(): bf16 [M, K] scratch
   void* out;                // [M, N], row stride ldo
   int64_t M, N, K;
   int64_t ldx, ld_xs, ldo;
   int group;                // 32, 64 or 128
   DType x_type;             // kBF16 or kF16 (the products' type; kBF16 for E4M3 rows)
   DType scale_type, bias_type, out_type;
+  int* err;
 };
+void launch_int4_gemm(const Int4LinearArgs& a, cudaStream_t s);  // int4_gemm.cu
 void launch_int4_linear(const Int4LinearArgs& a, cudaStream_t s);
 
 }  // namespace minisgl

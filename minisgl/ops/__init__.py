@@ -389,8 +389,11 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
         return y
     if out is None:
         out = torch.empty((x.shape[0], w.n), dtype=out_dtype, device=x.device)
-    _count()
-    native().int4_linear(out, x, x_scales, w.packed, w.scales, w.zeros, bias, w.n, w.k, w.group)
+    wide = x_scales is not None and x.shape[0] > 16  # MXFP8 rows widened to bf16 for the tensor cores' tiles
+    x_wide = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) if wide else None
+    _count(2 if wide else 1)
+    native().int4_linear(out, x, x_scales, w.packed, w.scales, w.zeros, w.row_pow, bias, w.n, w.k, w.group, x_wide,
+                         error_word(x.device))
     return out
 
 

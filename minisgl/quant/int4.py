@@ -47,13 +47,15 @@ class Int4Weight:
     """A 4-bit weight in the kernels' layout (made by ``int4_weight`` or
     ``quantize_int4``): ``packed`` uint8 [tiles, 2 ceil(K / 128), 512],
     ``scales`` bf16 / fp16 [tiles, groups, 8, 2] and ``zeros`` uint8
-    [tiles, groups, 8] or None, tiles = 2 ceil(N / 32), groups = 128 ceil(K / 128) / group."""
+    [tiles, groups, 8] or None, tiles = 2 ceil(N / 32), groups = 128 ceil(K / 128) / group;
+    ``row_pow`` float32 [16 tiles]: the power of two at or below a row's largest scale
+    (1 where that is 0), which fp16 products take out of the row."""
 
-    __slots__ = ("packed", "scales", "zeros", "n", "k", "group")
+    __slots__ = ("packed", "scales", "zeros", "row_pow", "n", "k", "group")
 
-    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], n: int, k: int,
-                 group: int) -> None:
-        self.packed, self.scales, self.zeros = packed, scales, zeros
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor],
+                 row_pow: torch.Tensor, n: int, k: int, group: int) -> None:
+        self.packed, self.scales, self.zeros, self.row_pow = packed, scales, zeros, row_pow
         self.n, self.k, self.group = n, k, group
 
     @property
@@ -62,7 +64,8 @@ class Int4Weight:
 
     def to(self, device) -> "Int4Weight":
         zeros = None if self.zeros is None else self.zeros.to(device)
-        return Int4Weight(self.packed.to(device), self.scales.to(device), zeros, self.n, self.k, self.group)
+        return Int4Weight(self.packed.to(device), self.scales.to(device), zeros, self.row_pow.to(device), self.n,
+                          self.k, self.group)
 
 
 def _tile_rows(t: torch.Tensor, groups: int) -> torch.Tensor:
@@ -114,7 +117,11 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
     if zeros is not None:
         z = _tile_rows(zeros, groups)
         z = z[..., 0] | (z[..., 1] << 4)
-    return Int4Weight(packed.view(tiles, blocks, 512), _tile_rows(scales, groups), z, n, k, group)
+    tiled = _tile_rows(scales, groups)
+    top = tiled.float().abs().amax(1).transpose(1, 2).reshape(-1)  # [tile, g, h] -> row
+    live = (top > 0) & (top <= torch.finfo(torch.float32).max)
+    row_pow = torch.where(live, torch.exp2(torch.floor(torch.log2(torch.where(live, top, 1.0)))), 1.0)
+    return Int4Weight(packed.view(tiles, blocks, 512), tiled, z, row_pow, n, k, group)
 
 
 def int4_codes(w: Int4Weight) -> torch.Tensor:

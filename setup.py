@@ -40,6 +40,7 @@ SOURCES = [
     "minisgl/csrc/ep.cu",
     "minisgl/csrc/mx8_rows.cu",
     "minisgl/csrc/int4.cu",
+    "minisgl/csrc/int4_gemm.cu",
 ]
 
 

@@ -211,6 +211,6 @@ def test_native_messages_with_numbers():
     x = torch.zeros(2, 64, dtype=torch.bfloat16)
     u8 = torch.zeros(512, dtype=torch.uint8)
     with pytest.raises(RuntimeError, match="group of 32, 64 or 128, got 48"):
-        ops.native().int4_linear(x, x, None, u8, x, None, None, 4, 64, 48)
+        ops.native().int4_linear(x, x, None, u8, x, None, x, None, 4, 64, 48, None, None)
     with pytest.raises(RuntimeError, match=r"x must be \[M, 128\], got \[2, 64\]"):
-        ops.native().int4_linear(x, x, None, u8, x, None, None, 4, 128, 64)
+        ops.native().int4_linear(x, x, None, u8, x, None, x, None, 4, 128, 64, None, None)
