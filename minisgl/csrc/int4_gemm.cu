@@ -4,17 +4,17 @@
 //
 // One persistent CTA per SM walks tiles of 128 weight rows x BN rows of x
 // (weights are the 128-row first operand, so that the 4-bit side is unpacked
-// as rarely as possible: once per BN rows of x). Per 64 columns eight
-// converter warps turn 128 x 64 codes into a bf16 (fp16) operand tile in shared
-// memory, four MMAs consume it together with a TMA tile of x, and the sums stay
+// as rarely as possible: once per BN rows of x). Per step of 128 columns eight
+// converter warps turn 128 x 128 codes into bf16 (fp16) operand tiles in shared
+// memory, eight MMAs consume them together with a TMA tile of x, and the sums stay
 // in tensor memory; two accumulators alternate, so that four epilogue warps
 // store one tile while the next is multiplied.
 //
-//   warp 0      x by TMA, a ring of kXs tiles of 64 columns
+//   warp 0      x by TMA, a ring of kXs steps of 128 columns
 //   warp 1      issues the MMAs
-//   warp 2      codes by bulk copies, a ring of kPs steps of 128 columns (8 KB)
+//   warp 2      codes by TMA, a ring of kPs steps (8 KB)
 //   warps 4-7   epilogue (tensor-memory lanes 32 (w % 4) ..)
-//   warps 8-15  converters, 16 weight rows each
+//   warps 8-23  two sets of converters, 16 weight rows a warp, which take the steps in turn
 //
 // W = (c - z) s is rounded once to bf16 (fp16): the one rounding besides those
 // of the float32 sums. fp16 weights are formed under each row's own power of
@@ -41,23 +41,25 @@ namespace minisgl {
 namespace {
 
 constexpr int kRows = 128;       // weight rows of a tile
-constexpr int kThreads = 512;
+constexpr int kSets = 2;         // converter sets of 8 warps, which take the steps in turn
+constexpr int kThreads = 256 + kSets * 256;
 constexpr int kConverters = 8;
-constexpr int kAs = 3;           // operand tiles between converters and MMAs
-constexpr int kATile = kRows * 128;
+constexpr int kATile = 2 * kRows * 128;  // one step (128 columns) as two 64-column operand tiles
 constexpr int kCodes = 8 * 1024;  // 128 rows x 128 columns
 
 template <int BN>
 struct GSmem {
-  static constexpr int kX = BN * 128;  // one 64-column tile of x
-  static constexpr int kXs = 4;
+  static constexpr int kX = BN * 256;  // one step of x, as two 64-column tiles
+  static constexpr int kXs = BN == 256 ? 2 : BN == 128 ? 3 : 4;
   static constexpr int kPs = BN == 256 ? 3 : 6;
+  static constexpr int kAs = BN >= 64 ? 2 : 3;  // operand steps between converters and MMAs
   static constexpr int kAt = 0;
   static constexpr int kXt = kAs * kATile;
   static constexpr int kPt = kXt + kXs * kX;
   static constexpr int kRing = kPt + kPs * kCodes;
   static constexpr int kBars = 8 * (2 * kXs + 2 * kPs + 2 * kAs + 4) + 16;
   static constexpr int bytes(int S) { return 1024 + kRing + (kBars + 127) / 128 * 128 + (S > 1 ? kRows * BN * 4 : 0); }
+  static_assert(bytes(BN <= 64 ? 2 : 1) <= 227 * 1024, "shared memory");
   static constexpr uint32_t kCols = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
@@ -70,6 +72,7 @@ struct GArgs {
   void* out;
   int M, N, steps, tiles16;
   int m_tiles, n_tiles, S;
+  int x_blocks;  // x by 64-column blocks (K % 64 == 0): one copy a step
   int64_t ldo;
   int scale_half, bias_type, out_type;
   ErrorSink err;
@@ -122,7 +125,7 @@ struct Pair {
 
 template <int BN, int G, bool HALF>
 __global__ void __launch_bounds__(kThreads, 1)
-    int4_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const GArgs a) {
+    int4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const GArgs a) {
   using L = GSmem<BN>;
   constexpr int P = 128 / G;
   extern __shared__ uint8_t smem_raw[];
@@ -132,8 +135,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* pfull = xempty + L::kXs;
   uint64_t* pempty = pfull + L::kPs;
   uint64_t* afull = pempty + L::kPs;
-  uint64_t* aempty = afull + kAs;
-  uint64_t* acc_full = aempty + kAs;   // [2]
+  uint64_t* aempty = afull + L::kAs;
+  uint64_t* acc_full = aempty + L::kAs;  // [2]
   uint64_t* acc_empty = acc_full + 2;  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
@@ -149,14 +152,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kXs; ++s) mbar_init(&xfull[s], 1), mbar_init(&xempty[s], 1);
     for (int s = 0; s < L::kPs; ++s) mbar_init(&pfull[s], 1), mbar_init(&pempty[s], kConverters);
-    for (int s = 0; s < kAs; ++s) mbar_init(&afull[s], kConverters), mbar_init(&aempty[s], 1);
+    for (int s = 0; s < L::kAs; ++s) mbar_init(&afull[s], kConverters), mbar_init(&aempty[s], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 4);
     *s_abort = 0;
     fence_barrier_init();
+    prefetch_tmap(&tm_w);
     prefetch_tmap(&tm_x);
   }
   // the first codes, on their way to L2 while the kernel before this one ends (a prefetch carries no value)
-  if (warp >= 8 && first < num_tiles) {
+  if (warp >= 8 && warp < 16 && first < num_tiles) {
     const int tile16 = first / a.m_tiles * 8 + warp - 8;
     if (tile16 < a.tiles16 && k0 + (lane >> 3) < k1)
       asm volatile("prefetch.global.L2 [%0];" ::"l"(
@@ -181,14 +185,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0;
       for (int tile = first; tile < num_tiles && !*abort_flag; tile += stride) {
         const int m0 = tile % a.m_tiles * BN;
-        for (int kb = 2 * k0; kb < 2 * k1; ++kb, ++it) {
+        for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % L::kXs;
           if (it >= L::kXs && !mbar_wait(&xempty[s], ((it / L::kXs) - 1) & 1, a.err, 421)) {
             *abort_flag = 1;
             break;
           }
           mbar_arrive_expect_tx(&xfull[s], L::kX);
-          tma_load_2d(smem + L::kXt + s * L::kX, &tm_x, &xfull[s], kb * 64, m0);
+          uint8_t* dst = smem + L::kXt + s * L::kX;
+          if (a.x_blocks) {  // both tiles in one copy
+            tma_load_3d(dst, &tm_x, &xfull[s], 0, m0, 2 * k);
+          } else {
+            tma_load_2d(dst, &tm_x, &xfull[s], k * 128, m0);
+            tma_load_2d(dst + L::kX / 2, &tm_x, &xfull[s], k * 128 + 64, m0);
+          }
           issued = it + 1;
         }
       }
@@ -200,17 +210,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0;
       for (int tile = first; tile < num_tiles && !*abort_flag; tile += stride) {
         const int t16 = tile / a.m_tiles * 8;
-        const int count = min(8, a.tiles16 - t16);
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % L::kPs;
           if (it >= L::kPs && !mbar_wait(&pempty[s], ((it / L::kPs) - 1) & 1, a.err, 422)) {
             *abort_flag = 1;
             break;
           }
-          mbar_arrive_expect_tx(&pfull[s], count * 1024);
-          for (int c = 0; c < count; ++c)
-            bulk_load(smem + L::kPt + s * kCodes + c * 1024,
-                      a.packed + (static_cast<int64_t>(t16 + c) * a.steps + k) * 1024, 1024, &pfull[s]);
+          // eight tiles x 1 KB in one copy (eight bulk copies took 130 cycles each to issue)
+          mbar_arrive_expect_tx(&pfull[s], kCodes);
+          tma_load_2d(smem + L::kPt + s * kCodes, &tm_w, &pfull[s], k * 256, t16);
           issued = it + 1;
         }
       }
@@ -228,18 +236,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lt >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], ((lt >> 1) - 1) & 1, a.err, 423));
       if (!ok) break;
       tc_fence_after();
-      for (int kb = 2 * k0; kb < 2 * k1; ++kb, ++it) {
-        const int xs = it % L::kXs, as = it % kAs;
-        ok = __all_sync(0xffffffffu, mbar_wait(&xfull[xs], (it / L::kXs) & 1, a.err, 424) &&
-                                         mbar_wait(&afull[as], (it / kAs) & 1, a.err, 425));
+      for (int k = k0; k < k1 && ok; ++k, ++it) {
+        const int as = it % L::kAs, xs = it % L::kXs;
+        ok = __all_sync(0xffffffffu, mbar_wait(&afull[as], (it / L::kAs) & 1, a.err, 425) &&
+                                         mbar_wait(&xfull[xs], (it / L::kXs) & 1, a.err, 424));
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t wa = base + L::kAt + as * kATile, xa = base + L::kXt + xs * L::kX;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_f16(tmem + acc * BN, make_sdesc_k_sw128(wa + k * 32), make_sdesc_k_sw128(xa + k * 32), idesc,
-                       (kb > 2 * k0 || k > 0) ? 1u : 0u);
+        for (int h = 0; h < 2; ++h) {
+          if (lane == 0) {
+            const uint32_t wa = base + L::kAt + as * kATile + h * (kATile / 2);
+            const uint32_t xa = base + L::kXt + xs * L::kX + h * (L::kX / 2);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              tc_mma_f16(tmem + acc * BN, make_sdesc_k_sw128(wa + q * 32), make_sdesc_k_sw128(xa + q * 32), idesc,
+                         (k > k0 || h > 0 || q > 0) ? 1u : 0u);
+          }
+        }
+        if (lane == 0) {
           tc_commit(&xempty[xs]);
           tc_commit(&aempty[as]);
         }
@@ -252,12 +266,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp >= 8) {
     // ----------------------------------------------------- converters ----
-    const int c16 = warp - 8, g = lane >> 2, t = lane & 3;
+    const int set = (warp - 8) / 8, c16 = (warp - 8) % 8, g = lane >> 2, t = lane & 3;
     // odd rows store their second 32 columns first: the eight lanes of a quarter warp hit distinct banks
     const bool flip = g & 1;
     const uint32_t row_at = (16 * c16 + g) * 128;
     const uint32_t at0 = row_at + (((flip ? 4 + t : t) ^ g) << 4), at1 = row_at + (((flip ? t : 4 + t) ^ g) << 4);
-    int it = 0, pit = 0;
+    int it = 0;
     bool ok = true;
     for (int tile = first; ok && tile < num_tiles; tile += stride) {
       const int tile16 = min(tile / a.m_tiles * 8 + c16, a.tiles16 - 1);  // rows past N: any codes, never stored
@@ -273,24 +287,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           zv[p] = zp != nullptr ? zp[(k * P + p) * 8] : 0x88u;
         }
       };
-      load_scales(k0, sc_next, zz_next);
-      for (int k = k0; k < k1 && ok; ++k, ++pit) {
+      // this set's steps of the tile
+      const int turn = (set + kSets - it % kSets) % kSets;
+      if (k0 + turn < k1) load_scales(k0 + turn, sc_next, zz_next);
+      for (int k = k0; k < k1 && ok; ++k, ++it) {
+        if ((k - k0) % kSets != turn) continue;
 #pragma unroll
         for (int p = 0; p < P; ++p) sc[p] = sc_next[p], zz[p] = zz_next[p];
-        if (k + 1 < k1) load_scales(k + 1, sc_next, zz_next);
-        const int ps = pit % L::kPs;
-        ok = __all_sync(0xffffffffu, mbar_wait(&pfull[ps], (pit / L::kPs) & 1, a.err, 426));
+        if (k + kSets < k1) load_scales(k + kSets, sc_next, zz_next);
+        const int ps = it % L::kPs, as = it % L::kAs;
+        ok = __all_sync(0xffffffffu, mbar_wait(&pfull[ps], (it / L::kPs) & 1, a.err, 426));
         if (!ok) break;
         const uint4* codes = reinterpret_cast<const uint4*>(smem + L::kPt + ps * kCodes + c16 * 1024) + lane;
         const uint4 w[2] = {codes[0], codes[32]};
         __syncwarp();
         if (lane == 0) mbar_arrive(&pempty[ps]);  // the codes are in registers
+        if (it >= L::kAs) ok = __all_sync(0xffffffffu, mbar_wait(&aempty[as], ((it / L::kAs) - 1) & 1, a.err, 427));
+        if (!ok) break;
 #pragma unroll
-        for (int h = 0; h < 2; ++h, ++it) {
-          const int as = it % kAs;
-          if (it >= kAs) ok = __all_sync(0xffffffffu, mbar_wait(&aempty[as], ((it / kAs) - 1) & 1, a.err, 427));
-          if (!ok) break;
-          uint8_t* dst = smem + L::kAt + as * kATile;
+        for (int h = 0; h < 2; ++h) {
+          uint8_t* dst = smem + L::kAt + as * kATile + h * (kATile / 2);
           // first and second run of 8 columns in this lane's order
           const uint32_t words[4] = {flip ? w[h].z : w[h].x, flip ? w[h].w : w[h].y, flip ? w[h].x : w[h].z, flip ? w[h].y : w[h].w};
 #pragma unroll
@@ -345,10 +361,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint4*>(dst + at) = make_uint4(o[0][0], o[0][1], o[0][2], o[0][3]);
             *reinterpret_cast<uint4*>(dst + at + 8 * 128) = make_uint4(o[1][0], o[1][1], o[1][2], o[1][3]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&afull[as]);
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&afull[as]);
       }
     }
     if (!ok && lane == 0) *abort_flag = 1;
@@ -497,7 +513,7 @@ int resident(int S, int smem) {
 }
 
 template <int BN, int G, bool HALF>
-void launch_bn(GArgs a, const CUtensorMap& tm, cudaStream_t s) {
+void launch_bn(GArgs a, const CUtensorMap& tw, const CUtensorMap& tm, cudaStream_t s) {
   constexpr auto kern = int4_gemm_kernel<BN, G, HALF>;
   using L = GSmem<BN>;
   a.m_tiles = (a.M + BN - 1) / BN;
@@ -528,21 +544,21 @@ void launch_bn(GArgs a, const CUtensorMap& tm, cudaStream_t s) {
   }
   cfg.attrs = attrs;
   cfg.numAttrs = n;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tm, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tm, a);
   if (e != cudaSuccess) throw std::runtime_error(std::string("minisgl: kernel launch failed: ") + cudaGetErrorString(e));
 }
 
 template <int BN, bool HALF>
-void launch_group(const GArgs& a, const CUtensorMap& tm, int group, cudaStream_t s) {
+void launch_group(const GArgs& a, const CUtensorMap& tw, const CUtensorMap& tm, int group, cudaStream_t s) {
   switch (group) {
-    case 32: launch_bn<BN, 32, HALF>(a, tm, s); break;
-    case 64: launch_bn<BN, 64, HALF>(a, tm, s); break;
-    default: launch_bn<BN, 128, HALF>(a, tm, s); break;
+    case 32: launch_bn<BN, 32, HALF>(a, tw, tm, s); break;
+    case 64: launch_bn<BN, 64, HALF>(a, tw, tm, s); break;
+    default: launch_bn<BN, 128, HALF>(a, tw, tm, s); break;
   }
 }
 
 template <bool HALF>
-void launch_type(const GArgs& a, const void* x, int64_t ldx, int64_t K, int group, cudaStream_t s) {
+void launch_type(GArgs a, const void* x, int64_t ldx, int64_t K, int group, cudaStream_t s) {
   // rows of x per tile: the size with the least time in the busiest CTA, per 64 columns 2 cycles per row of x in
   // the tensor cores against about kConvert to unpack 128 weight rows
   constexpr int kConvert = 250;
@@ -554,13 +570,18 @@ void launch_type(const GArgs& a, const void* x, int64_t ldx, int64_t K, int grou
     const int64_t cost = (tiles + sms - 1) / sms * std::max(2 * bn, kConvert);
     if (best_cost < 0 || cost < best_cost || (cost == best_cost && bn >= a.M)) best = bn, best_cost = cost;
   }
-  const CUtensorMap tm = make_tmap_bf16_2d_sw128(x, static_cast<uint64_t>(a.M), static_cast<uint64_t>(K),
-                                                 static_cast<uint64_t>(ldx), static_cast<uint32_t>(best));
+  a.x_blocks = K % 64 == 0;
+  const CUtensorMap tm = a.x_blocks ? make_tmap_bf16_kblocks(x, a.M, K, ldx, best, 2) : make_tmap_bf16_2d_sw128(x, a.M, K, ldx, best);
+  // codes: a row of the map is a tile of 16 rows, its columns the tile's 128-column units (256 words)
+  const uint64_t dims[2] = {static_cast<uint64_t>(a.steps) * 256, static_cast<uint64_t>(a.tiles16)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(a.steps) * 1024};
+  const uint32_t box[2] = {256, 8};
+  const CUtensorMap tw = make_tmap(a.packed, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
   switch (best) {
-    case 32: launch_group<32, HALF>(a, tm, group, s); break;
-    case 64: launch_group<64, HALF>(a, tm, group, s); break;
-    case 128: launch_group<128, HALF>(a, tm, group, s); break;
-    default: launch_group<256, HALF>(a, tm, group, s); break;
+    case 32: launch_group<32, HALF>(a, tw, tm, group, s); break;
+    case 64: launch_group<64, HALF>(a, tw, tm, group, s); break;
+    case 128: launch_group<128, HALF>(a, tw, tm, group, s); break;
+    default: launch_group<256, HALF>(a, tw, tm, group, s); break;
   }
 }
 

@@ -370,9 +370,9 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
     ``quantize_int4``). x [M, K] is bf16 or fp16, or MXFP8 rows: uint8 E4M3
     bits with ``x_scales`` [M, K / 32], as ``rmsnorm_mx8`` and
     ``silu_and_mul_mx8`` return them. out: bf16, fp16 or fp32 (default: x's
-    type, bf16 for MXFP8 rows). Sums are held in fp32; a group's sum of
-    x * (code - zero) is formed before its scale is applied, so
-  """
+    type, bf16 for MXFP8 rows). Sums are held in fp32 or
+    exact integers, whatever the number of rows; products of more than 16 rows
+    take the weight rounded once to x's 16-bit type."""
     if x.dim() != 2 or x.shape[1] != w.k:
         raise ValueError(f"int4_linear: x must be [M, {w.k}], got {tuple(x.shape)}")
     if (x.dtype == torch.uint8) != (x_scales is not None):
