@@ -209,9 +209,9 @@ __device__ __noinline__ float not_finite_part(const VecArgs& a, int64_t tile, in
     x_values(v, x_raw(a, m, k), a.x_kind);
     for (int j = 0; j < 8; ++j) {
       if (fabsf(v[j]) <= 3.4028234e38f) continue;
-      const int c = (k + j) % 64, i = c / 32, t = c % 32 / 8, l = c % 8 / 4, q = c % 4 / 2, e = c % 2;
+      const int c = (k + j) % 64, t = c % 16 / 4, q = c % 4 / 2, e = c % 2;
       const uint32_t word = reinterpret_cast<const uint32_t*>(
-          a.packed)[((tile * a.steps * 2 + (k + j) / 64) * 32 + 4 * (r & 7) + t) * 4 + 2 * i + l];
+          a.packed)[((tile * a.steps * 2 + (k + j) / 64) * 32 + 4 * (r & 7) + t) * 4 + c / 16];
       const int code = (word >> (4 * (4 * e + 2 * q + (r >> 3))) & 15) ^ 8;
       const int64_t gi = tile * (a.steps * 128 / group) + (k + j) / group;
       const uint32_t zz = a.zeros != nullptr ? a.zeros[gi * 8 + (r & 7)] : 0x88u;
@@ -364,7 +364,8 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
       uint32_t xi[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) xi[j] = __float_as_uint(fmaf(v[j], up, 12582912.f)) - 0x4B400000u;  // 1.5 * 2^23
-      uint8_t* dst = xs + m * pitch + step * 384 + (c >> 3 & 1) * 64 + (c & 3) * 16 + (c >> 2 & 1) * 8;
+      // lane 4 g + t reads columns 4 t .. 4 t + 3 of each 16: this run is two lanes' words
+      uint8_t* dst = xs + m * pitch + step * 384 + (c >> 3 & 1) * 64 + (c & 1) * 32 + (c >> 1 & 3) * 4;
       uint32_t word[3][2];
 #pragma unroll
       for (int l = 0; l < 2; ++l) {  // columns 0, 2, 1, 3: the order of a code word's bytes
@@ -375,7 +376,10 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
         word[2][l] = __byte_perm(t2, t3, 0x5410);
       }
 #pragma unroll
-      for (int d = 0; d < 3; ++d) *reinterpret_cast<uint2*>(dst + d * 128) = make_uint2(word[d][0], word[d][1]);
+      for (int d = 0; d < 3; ++d) {
+        *reinterpret_cast<uint32_t*>(dst + d * 128) = word[d][0];
+        *reinterpret_cast<uint32_t*>(dst + d * 128 + 16) = word[d][1];
+      }
       uint8_t* sd = side + step * (L::kSide * NT);
       // codes count in sixteenths (they sit in a byte's upper half): 2^-4 goes with the power of two
       if ((c & 15) == 0) *reinterpret_cast<float*>(sd + m * 4) = __uint_as_float((e - 25u) << 23);

@@ -5,16 +5,17 @@
 // One persistent CTA per SM walks tiles of 128 weight rows x BN rows of x
 // (weights are the 128-row first operand, so that the 4-bit side is unpacked
 // as rarely as possible: once per BN rows of x). Per step of 128 columns eight
-// converter warps turn 128 x 128 codes into bf16 (fp16) operand tiles in shared
-// memory, eight MMAs consume them together with a TMA tile of x, and the sums stay
-// in tensor memory; two accumulators alternate, so that four epilogue warps
-// store one tile while the next is multiplied.
+// converter warps turn 128 x 128 codes into bf16 (fp16) values in tensor
+// memory, where the MMAs take their first operand from: shared memory, whose
+// bandwidth bounds the large tiles (x is written and read there once per step),
+// sees nothing of the unpacked weights. The sums stay in tensor memory; four
+// epilogue warps store them.
 //
-//   warp 0      x by TMA, a ring of kXs steps of 128 columns
+//   warp 0      x by TMA, a ring of kXs steps
 //   warp 1      issues the MMAs
 //   warp 2      codes by TMA, a ring of kPs steps (8 KB)
 //   warps 4-7   epilogue (tensor-memory lanes 32 (w % 4) ..)
-//   warps 8-23  two sets of converters, 16 weight rows a warp, which take the steps in turn
+//   warps 8-23  two sets of converters, which take the steps in turn; a warp has 32 rows x 64 columns of a step
 //
 // W = (c - z) s is rounded once to bf16 (fp16): the one rounding besides those
 // of the float32 sums. fp16 weights are formed under each row's own power of
@@ -44,23 +45,23 @@ constexpr int kRows = 128;       // weight rows of a tile
 constexpr int kSets = 2;         // converter sets of 8 warps, which take the steps in turn
 constexpr int kThreads = 256 + kSets * 256;
 constexpr int kConverters = 8;
-constexpr int kATile = 2 * kRows * 128;  // one step (128 columns) as two 64-column operand tiles
+constexpr int kACols = 64;       // tensor-memory columns of one step of weights: 128 values of 16 bits a row
 constexpr int kCodes = 8 * 1024;  // 128 rows x 128 columns
 
 template <int BN>
 struct GSmem {
   static constexpr int kX = BN * 256;  // one step of x, as two 64-column tiles
-  static constexpr int kXs = BN == 256 ? 2 : BN == 128 ? 3 : 4;
-  static constexpr int kPs = BN == 256 ? 3 : 6;
-  static constexpr int kAs = BN >= 64 ? 2 : 3;  // operand steps between converters and MMAs
-  static constexpr int kAt = 0;
-  static constexpr int kXt = kAs * kATile;
-  static constexpr int kPt = kXt + kXs * kX;
+  static constexpr int kXs = BN == 256 ? 3 : BN == 128 ? 5 : 6;
+  static constexpr int kPs = BN == 256 ? 3 : 8;
+  static constexpr int kAs = BN == 32 ? 3 : 4;   // steps of weights in tensor memory
+  static constexpr int kAcc = BN == 256 ? 1 : 2;  // sums in tensor memory
+  static constexpr int kPt = kXs * kX;
   static constexpr int kRing = kPt + kPs * kCodes;
   static constexpr int kBars = 8 * (2 * kXs + 2 * kPs + 2 * kAs + 4) + 16;
   static constexpr int bytes(int S) { return 1024 + kRing + (kBars + 127) / 128 * 128 + (S > 1 ? kRows * BN * 4 : 0); }
   static_assert(bytes(BN <= 64 ? 2 : 1) <= 227 * 1024, "shared memory");
-  static constexpr uint32_t kCols = 2 * BN < 32 ? 32 : 2 * BN;
+  static constexpr uint32_t kCols = BN == 32 ? 256 : 512;
+  static_assert(kAcc * BN + kAs * kACols <= kCols, "tensor memory");
 };
 
 struct GArgs {
@@ -93,6 +94,16 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, int type, float v)
     static_cast<__half*>(p)[i] = __float2half_rn(v);
   else
     static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// 16 rows x 64 values of 16 bits (32 columns) of tensor memory: lane 4 g + t holds of each 8 columns (16 values)
+// columns 2 t, 2 t + 1 of row g, then of row g + 8
+__device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
 // Pairs of 16-bit floats: a code under an exponent, exactly code - zero, times the scale.
@@ -192,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           mbar_arrive_expect_tx(&xfull[s], L::kX);
-          uint8_t* dst = smem + L::kXt + s * L::kX;
+          uint8_t* dst = smem + s * L::kX;
           if (a.x_blocks) {  // both tiles in one copy
             tma_load_3d(dst, &tm_x, &xfull[s], 0, m0, 2 * k);
           } else {
@@ -232,8 +243,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int it = 0, lt = 0;
     bool ok = true;
     for (int tile = first; ok && tile < num_tiles; tile += stride, ++lt) {
-      const int acc = lt & 1;
-      if (lt >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], ((lt >> 1) - 1) & 1, a.err, 423));
+      const int acc = lt % L::kAcc;
+      if (lt >= L::kAcc) ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], (lt / L::kAcc - 1) & 1, a.err, 423));
       if (!ok) break;
       tc_fence_after();
       for (int k = k0; k < k1 && ok; ++k, ++it) {
@@ -245,12 +256,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (lane == 0) {
-            const uint32_t wa = base + L::kAt + as * kATile + h * (kATile / 2);
-            const uint32_t xa = base + L::kXt + xs * L::kX + h * (L::kX / 2);
+            const uint32_t wa = tmem + L::kAcc * BN + as * kACols + h * (kACols / 2);
+            const uint32_t xa = base + xs * L::kX + h * (L::kX / 2);
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              tc_mma_f16(tmem + acc * BN, make_sdesc_k_sw128(wa + q * 32), make_sdesc_k_sw128(xa + q * 32), idesc,
-                         (k > k0 || h > 0 || q > 0) ? 1u : 0u);
+              tc_mma_f16_ta(tmem + acc * BN, wa + q * 8, make_sdesc_k_sw128(xa + q * 32), idesc,
+                            (k > k0 || h > 0 || q > 0) ? 1u : 0u);
           }
         }
         if (lane == 0) {
@@ -266,103 +277,92 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp >= 8) {
     // ----------------------------------------------------- converters ----
-    const int set = (warp - 8) / 8, c16 = (warp - 8) % 8, g = lane >> 2, t = lane & 3;
-    // odd rows store their second 32 columns first: the eight lanes of a quarter warp hit distinct banks
-    const bool flip = g & 1;
-    const uint32_t row_at = (16 * c16 + g) * 128;
-    const uint32_t at0 = row_at + (((flip ? 4 + t : t) ^ g) << 4), at1 = row_at + (((flip ? t : 4 + t) ^ g) << 4);
+    // warp q + 4 h of a set: rows 32 q .. 32 q + 31 (the tensor-memory lanes it reaches), columns 64 h .. of a step
+    const int set = (warp - 8) / 8, quad = warp & 3, half = (warp >> 2) & 1, g = lane >> 2;
+    const uint32_t a_base = tmem + L::kAcc * BN + half * (kACols / 2) + (static_cast<uint32_t>(32 * quad) << 16);
+    constexpr int H = P == 4 ? 2 : 1;  // groups of 64 columns
     int it = 0;
     bool ok = true;
     for (int tile = first; ok && tile < num_tiles; tile += stride) {
-      const int tile16 = min(tile / a.m_tiles * 8 + c16, a.tiles16 - 1);  // rows past N: any codes, never stored
-      const uint32_t* sp = a.scales + (static_cast<int64_t>(tile16) * a.steps * P) * 8 + g;
-      const uint8_t* zp = a.zeros != nullptr ? a.zeros + (static_cast<int64_t>(tile16) * a.steps * P) * 8 + g : nullptr;
-      float down0 = 1.f, down1 = 1.f;  // 1 / the rows' power of two
-      if constexpr (HALF) down0 = 1.f / a.row_pow[tile16 * 16 + g], down1 = 1.f / a.row_pow[tile16 * 16 + g + 8];
-      uint32_t sc[P], zz[P], sc_next[P], zz_next[P];
-      auto load_scales = [&](int k, uint32_t (&sv)[P], uint32_t (&zv)[P]) {
+      const uint32_t* sp[2];
+      const uint8_t* zp[2];
+      float down[2][2];  // 1 / the rows' power of two
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          sv[p] = sp[(k * P + p) * 8];
-          zv[p] = zp != nullptr ? zp[(k * P + p) * 8] : 0x88u;
-        }
+      for (int c = 0; c < 2; ++c) {
+        const int tile16 = min(tile / a.m_tiles * 8 + 2 * quad + c, a.tiles16 - 1);  // rows past N: any codes, never stored
+        const int64_t at = static_cast<int64_t>(tile16) * a.steps * (P * 8) + (P == 1 ? 0 : half * (H * 8)) + g;
+        sp[c] = a.scales + at;
+        zp[c] = a.zeros + at;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) down[c][r] = HALF ? 1.f / a.row_pow[tile16 * 16 + g + 8 * r] : 1.f;
+      }
+      uint32_t sc[2][H], zz[2][H], sc_next[2][H], zz_next[2][H];
+      auto load_scales = [&](int k) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int p = 0; p < H; ++p) {
+            sc_next[c][p] = sp[c][(k * P + p) * 8];
+            zz_next[c][p] = a.zeros != nullptr ? zp[c][(k * P + p) * 8] : 0x88u;
+          }
       };
       // this set's steps of the tile
       const int turn = (set + kSets - it % kSets) % kSets;
-      if (k0 + turn < k1) load_scales(k0 + turn, sc_next, zz_next);
+      if (k0 + turn < k1) load_scales(k0 + turn);
       for (int k = k0; k < k1 && ok; ++k, ++it) {
         if ((k - k0) % kSets != turn) continue;
 #pragma unroll
-        for (int p = 0; p < P; ++p) sc[p] = sc_next[p], zz[p] = zz_next[p];
-        if (k + kSets < k1) load_scales(k + kSets, sc_next, zz_next);
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int p = 0; p < H; ++p) sc[c][p] = sc_next[c][p], zz[c][p] = zz_next[c][p];
+        if (k + kSets < k1) load_scales(k + kSets);
         const int ps = it % L::kPs, as = it % L::kAs;
         ok = __all_sync(0xffffffffu, mbar_wait(&pfull[ps], (it / L::kPs) & 1, a.err, 426));
         if (!ok) break;
-        const uint4* codes = reinterpret_cast<const uint4*>(smem + L::kPt + ps * kCodes + c16 * 1024) + lane;
-        const uint4 w[2] = {codes[0], codes[32]};
+        const uint4* codes = reinterpret_cast<const uint4*>(smem + L::kPt + ps * kCodes + quad * 2048 + half * 512) + lane;
+        const uint4 w[2] = {codes[0], codes[64]};
         __syncwarp();
         if (lane == 0) mbar_arrive(&pempty[ps]);  // the codes are in registers
         if (it >= L::kAs) ok = __all_sync(0xffffffffu, mbar_wait(&aempty[as], ((it / L::kAs) - 1) & 1, a.err, 427));
         if (!ok) break;
+        tc_fence_after();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint8_t* dst = smem + L::kAt + as * kATile + h * (kATile / 2);
-          // first and second run of 8 columns in this lane's order
-          const uint32_t words[4] = {flip ? w[h].z : w[h].x, flip ? w[h].w : w[h].y, flip ? w[h].x : w[h].z, flip ? w[h].y : w[h].w};
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+          uint32_t o[16];  // per word (16 columns): two pairs of row g, two of row g + 8
 #pragma unroll
-          for (int run = 0; run < 2; ++run) {
-            constexpr int kHalf = P == 4 ? 2 : 1;  // groups of 64 columns
-            const int p0 = P == 1 ? 0 : kHalf * h;
-            uint32_t sw, zw;
-            if constexpr (P == 4) {
-              sw = (run == 0) != flip ? sc[p0] : sc[p0 + 1];
-              zw = (run == 0) != flip ? zz[p0] : zz[p0 + 1];
-            } else {
-              sw = sc[p0], zw = zz[p0];
-            }
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t sw = sc[c][j * H / 4], zw = zz[c][j * H / 4];
             const uint32_t z[2] = {Pair<HALF>::zero(zw & 15u), Pair<HALF>::zero(zw >> 4)};
-            uint32_t o[2][4];  // [row g, row g + 8][column pair]
-            const bool exact_scale = HALF || !a.scale_half;
-            uint32_t s[2];
-            if constexpr (HALF) {
+            uint32_t d[4];
 #pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const __half q = __float2half_rn(scale_f32(r ? sw >> 16 : sw & 0xFFFFu, a.scale_half) * (r ? down1 : down0));
-                s[r] = static_cast<uint32_t>(__half_as_ushort(q)) * 0x10001u;
+            for (int r = 0; r < 4; ++r)  // r: bit 0 the row half, bit 1 the column pair
+              d[2 * (r & 1) + (r >> 1)] = Pair<HALF>::sub(Pair<HALF>::code(words[j] >> (4 * r)), z[r & 1]);
+            if (HALF || !a.scale_half) {
+              uint32_t s[2];
+              if constexpr (HALF) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  const __half q = __float2half_rn(scale_f32(r ? sw >> 16 : sw & 0xFFFFu, a.scale_half) * down[c][r]);
+                  s[r] = static_cast<uint32_t>(__half_as_ushort(q)) * 0x10001u;
+                }
+              } else {
+                s[0] = __byte_perm(sw, 0, 0x1010), s[1] = __byte_perm(sw, 0, 0x3232);
               }
-            } else {
-              s[0] = __byte_perm(sw, 0, 0x1010), s[1] = __byte_perm(sw, 0, 0x3232);
-            }
 #pragma unroll
-            for (int l = 0; l < 2; ++l) {
-              const uint32_t word = words[2 * run + l];
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {  // r: bit 0 the row half, bit 1 the column pair
-                const uint32_t d = Pair<HALF>::sub(Pair<HALF>::code(word >> (4 * r)), z[r & 1]);
-                o[r & 1][2 * l + (r >> 1)] = d;
-              }
-            }
-            if (exact_scale) {
-#pragma unroll
-              for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[r][i] = Pair<HALF>::mul(o[r][i], s[r]);
+              for (int i = 0; i < 4; ++i) o[4 * j + i] = Pair<HALF>::mul(d[i], s[i >> 1]);
             } else {
               // fp16 scales do not fit bf16: the product is formed in float32 and rounded once
+              const float f[2] = {scale_f32(sw & 0xFFFFu, 1), scale_f32(sw >> 16, 1)};
 #pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const float f = scale_f32(r ? sw >> 16 : sw & 0xFFFFu, 1);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  o[r][i] = pack_bf16x2(__uint_as_float(o[r][i] << 16) * f, __uint_as_float(o[r][i] & 0xFFFF0000u) * f);
-              }
+              for (int i = 0; i < 4; ++i)
+                o[4 * j + i] = pack_bf16x2(__uint_as_float(d[i] << 16) * f[i >> 1], __uint_as_float(d[i] & 0xFFFF0000u) * f[i >> 1]);
             }
-            const uint32_t at = run == 0 ? at0 : at1;
-            *reinterpret_cast<uint4*>(dst + at) = make_uint4(o[0][0], o[0][1], o[0][2], o[0][3]);
-            *reinterpret_cast<uint4*>(dst + at + 8 * 128) = make_uint4(o[1][0], o[1][1], o[1][2], o[1][3]);
           }
+          tmem_st_16x256b_x4(a_base + as * kACols + (static_cast<uint32_t>(16 * c) << 16), o);
         }
-        fence_proxy_async_smem();
+        tc_wait_st();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&afull[as]);
       }
@@ -376,8 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int lt = 0;
     bool ok = true;
     for (int tile = first; tile < num_tiles; tile += stride, ++lt) {
-      const int acc = lt & 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (lt >> 1) & 1, a.err, 428));
+      const int acc = lt % L::kAcc;
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (lt / L::kAcc) & 1, a.err, 428));
       if (!ok) break;
       tc_fence_after();
       const int m0 = tile % a.m_tiles * BN;

@@ -13,15 +13,14 @@ codes packed two per byte and lays them out once for the kernels
 
 Layout. Rows are cut into tiles of 16, columns into blocks of 64, both an even
 number (rows are padded to 32, columns to 128); tile and block fill 512 bytes,
-16 for each lane of a warp. Lane 4 g + t holds rows g and g + 8, columns 8 t ..
-8 t + 7 of either half (32 columns) of the block, in four words; word
-j = 2 i + l has columns 32 i + 8 t + 4 l + 2 p + e of row g + 8 h at bit
-4 (4 e + 2 p + h), as c - 8 in two's complement. A byte's upper half is thus a
-signed code of row g + 8 (of row g after a shift by 4), and a word gives two of
-the four registers (four 8-bit values each) that a warp-level 16 x 8 x 32
-product takes of its first operand, in the order in which a lane's runs of 8
-values of x fill the second. A word's columns lie in one half, so no product
-mixes two groups. Scales are [tile, group, g, h], so that a lane's two are one
+16 for each lane of a warp. Lane 4 g + t holds columns 4 t .. 4 t + 3 of each 16
+of rows g and g + 8, in four words; word j has columns 16 j + 4 t + 2 p + e of
+row g + 8 h at bit 4 (4 e + 2 p + h), as c - 8 in two's complement. A byte's
+upper half is thus a signed code of row g + 8 (of row g after a shift by 4), and
+a word gives two of the four registers (four 8-bit values each) that a warp-level
+16 x 8 x 32 product takes of its first operand; unpacked to pairs of 16-bit
+values, it is what a lane stores into 16 rows x 8 columns of tensor memory. A
+word's columns lie under one group. Scales are [tile, group, g, h], so that a lane's two are one
 word, zero points [tile, group, g] with z[g] | z[g + 8] << 4. Padding rows and
 columns have scale 0.
 
@@ -104,11 +103,11 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
         full[:n, : k // 2] = codes
     else:
         full = codes
-    # byte b of a row holds columns 2b (e = 0) and 2b + 1 (e = 1): [tile, h, g, block, i, t, l, p]
-    c = full.view(tiles, 2, 8, blocks, 2, 4, 2, 2).permute(1, 0, 3, 2, 5, 4, 6, 7)  # [h, tile, block, g, t, i, l, p]
+    # byte b of a row holds columns 2b (e = 0) and 2b + 1 (e = 1): [tile, h, g, block, j, t, p]
+    c = full.view(tiles, 2, 8, blocks, 4, 4, 2).permute(1, 0, 3, 2, 5, 4, 6)  # [h, tile, block, g, t, j, p]
     top, low = c[0], c[1]
     # bytes of a word: (e, p) from the lowest; the nibbles of a byte: h
-    packed = torch.empty(tiles, blocks, 8, 4, 2, 2, 2, 2, dtype=torch.uint8, device=codes.device)
+    packed = torch.empty(tiles, blocks, 8, 4, 4, 2, 2, dtype=torch.uint8, device=codes.device)
     packed[..., 0, :] = (top & 15) | (low << 4)
     packed[..., 1, :] = (top >> 4) | (low & 0xF0)
     packed ^= 0x88  # c - 8, two's complement
@@ -127,9 +126,9 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
 def int4_codes(w: Int4Weight) -> torch.Tensor:
     """The codes of a weight, uint8 [N, K]."""
     tiles, blocks = w.packed.shape[:2]
-    b = (w.packed ^ 0x88).view(tiles, blocks, 8, 4, 2, 2, 2, 2)  # [tile, block, g, t, i, l, e, p]
-    c = torch.stack([b & 15, b >> 4], dim=-1)           # ..., h
-    c = c.permute(0, 8, 2, 1, 4, 3, 5, 7, 6)            # [tile, h, g, block, i, t, l, p, e]
+    b = (w.packed ^ 0x88).view(tiles, blocks, 8, 4, 4, 2, 2)  # [tile, block, g, t, j, e, p]
+    c = torch.stack([b & 15, b >> 4], dim=-1)        # ..., h
+    c = c.permute(0, 7, 2, 1, 4, 3, 6, 5)            # [tile, h, g, block, j, t, p, e]
     return c.reshape(tiles * _TILE, blocks * _BLOCK)[: w.n, : w.k]
 
 

@@ -39,10 +39,10 @@ def test_int4_layout_words():
         codes[row, col] = 13
         w = int4_weight(codes[:, 0::2] | (codes[:, 1::2] << 4), torch.ones(n, 2, dtype=torch.bfloat16), None, 64)
         tile, r, block, c = row // 16, row % 16, col // 64, col % 64
-        h, g, i, t, l, p, e = r // 8, r % 8, c // 32, c % 32 // 8, c % 8 // 4, c % 4 // 2, c % 2
+        h, g, j, t, p, e = r // 8, r % 8, c // 16, c % 16 // 4, c % 4 // 2, c % 2
         words = (w.packed ^ 0x88).view(torch.int32).view(2, 2, 32, 4)  # [tile, block, lane, word]
         want = torch.zeros_like(words, dtype=torch.int64)
-        want[tile, block, 4 * g + t, 2 * i + l] = 13 << (4 * (4 * e + 2 * p + h))
+        want[tile, block, 4 * g + t, j] = 13 << (4 * (4 * e + 2 * p + h))
         assert torch.equal(words.long() & 0xFFFFFFFF, want)
 
 

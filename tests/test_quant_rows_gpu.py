@@ -397,3 +397,13 @@ def test_refusals_gpu():
         ops.silu_and_mul_mx8(x, out=(torch.zeros(2, 32, device=DEV), torch.zeros(2, 1, device=DEV)))
     with pytest.raises(RuntimeError):
         ops.silu_and_mul_mx8(x, out=(torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(2, 1, dtype=torch.uint8)))
+
+
+@pytest.mark.parametrize("m,n,k,dt", [(600, 20000, 256, "bf16"), (300, 33000, 128, "fp16"), (40, 40000, 384, "bf16"), (1100, 9000, 640, "bf16")])
+def test_int4_linear_many_tiles(m, n, k, dt):
+    """More tiles than SMs: a CTA takes several, one after another."""
+    t = TYPES[dt]
+    w = _weight(n, k, 64, True, n, t)
+    x = torch.randn(m, k, generator=_gen(m), device=DEV).to(t)
+    _check_linear(ops.int4_linear(x, w), x.double(), w, None, rounded=True)
+    ops.check_device_errors(torch.device(DEV))
