@@ -51,17 +51,17 @@ constexpr int kCodes = 8 * 1024;  // 128 rows x 128 columns
 template <int BN>
 struct GSmem {
   static constexpr int kX = BN * 256;  // one step of x, as two 64-column tiles
-  static constexpr int kXs = BN == 256 ? 3 : BN == 128 ? 5 : 6;
-  static constexpr int kPs = BN == 256 ? 3 : 8;
-  static constexpr int kAs = BN == 32 ? 3 : 4;   // steps of weights in tensor memory
-  static constexpr int kAcc = BN == 256 ? 1 : 2;  // sums in tensor memory
+  static constexpr int kXs = BN == 192 ? 4 : BN == 128 ? 5 : 6;
+  static constexpr int kPs = BN == 192 ? 3 : 6;
+  static constexpr int kAs = BN == 192 ? 2 : BN == 32 ? 3 : 4;  // steps of weights in tensor memory
   static constexpr int kPt = kXs * kX;
-  static constexpr int kRing = kPt + kPs * kCodes;
+  static constexpr int kOut = kPt + kPs * kCodes;  // the epilogue's 2 KB a warp
+  static constexpr int kRing = kOut + 4 * 2048;
   static constexpr int kBars = 8 * (2 * kXs + 2 * kPs + 2 * kAs + 4) + 16;
   static constexpr int bytes(int S) { return 1024 + kRing + (kBars + 127) / 128 * 128 + (S > 1 ? kRows * BN * 4 : 0); }
   static_assert(bytes(BN <= 64 ? 2 : 1) <= 227 * 1024, "shared memory");
   static constexpr uint32_t kCols = BN == 32 ? 256 : 512;
-  static_assert(kAcc * BN + kAs * kACols <= kCols, "tensor memory");
+  static_assert(2 * BN + kAs * kACols <= kCols, "tensor memory");
 };
 
 struct GArgs {
@@ -73,6 +73,7 @@ struct GArgs {
   void* out;
   int M, N, steps, tiles16;
   int m_tiles, n_tiles, S;
+  int vec_out;   // 16-bit outputs whose rows lie at multiples of 16 bytes, N % 8 == 0
   int x_blocks;  // x by 64-column blocks (K % 64 == 0): one copy a step
   int64_t ldo;
   int scale_half, bias_type, out_type;
@@ -104,6 +105,15 @@ __device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+// One thread of a converged warp. The asynchronous instructions take their operands from uniform registers: under
+// an elected predicate the compiler keeps them there, under lane == 0 it moves each operand of each instruction
+// over (about 100 cycles an MMA).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 // Pairs of 16-bit floats: a code under an exponent, exactly code - zero, times the scale.
@@ -192,16 +202,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // -------------------------------------------------------------- x ----
-    if (lane == 0) {
-      int it = 0;
-      for (int tile = first; tile < num_tiles && !*abort_flag; tile += stride) {
-        const int m0 = tile % a.m_tiles * BN;
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % L::kXs;
-          if (it >= L::kXs && !mbar_wait(&xempty[s], ((it / L::kXs) - 1) & 1, a.err, 421)) {
-            *abort_flag = 1;
-            break;
-          }
+    int it = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < num_tiles && !*abort_flag; tile += stride) {
+      const int m0 = tile % a.m_tiles * BN;
+      for (int k = k0; k < k1; ++k, ++it) {
+        const int s = it % L::kXs;
+        if (it >= L::kXs) ok = __all_sync(0xffffffffu, mbar_wait(&xempty[s], ((it / L::kXs) - 1) & 1, a.err, 421));
+        if (!ok) break;
+        if (elect_one()) {
           mbar_arrive_expect_tx(&xfull[s], L::kX);
           uint8_t* dst = smem + s * L::kX;
           if (a.x_blocks) {  // both tiles in one copy
@@ -210,41 +219,44 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_2d(dst, &tm_x, &xfull[s], k * 128, m0);
             tma_load_2d(dst + L::kX / 2, &tm_x, &xfull[s], k * 128 + 64, m0);
           }
-          issued = it + 1;
         }
+        __syncwarp();
+        issued = it + 1;
       }
     }
+    if (!ok && lane == 0) *abort_flag = 1;
     __syncwarp();
   } else if (warp == 2) {
     // ---------------------------------------------------------- codes ----
-    if (lane == 0) {
-      int it = 0;
-      for (int tile = first; tile < num_tiles && !*abort_flag; tile += stride) {
-        const int t16 = tile / a.m_tiles * 8;
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % L::kPs;
-          if (it >= L::kPs && !mbar_wait(&pempty[s], ((it / L::kPs) - 1) & 1, a.err, 422)) {
-            *abort_flag = 1;
-            break;
-          }
+    int it = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < num_tiles && !*abort_flag; tile += stride) {
+      const int t16 = tile / a.m_tiles * 8;
+      for (int k = k0; k < k1; ++k, ++it) {
+        const int s = it % L::kPs;
+        if (it >= L::kPs) ok = __all_sync(0xffffffffu, mbar_wait(&pempty[s], ((it / L::kPs) - 1) & 1, a.err, 422));
+        if (!ok) break;
+        if (elect_one()) {
           // eight tiles x 1 KB in one copy (eight bulk copies took 130 cycles each to issue)
           mbar_arrive_expect_tx(&pfull[s], kCodes);
           tma_load_2d(smem + L::kPt + s * kCodes, &tm_w, &pfull[s], k * 256, t16);
-          issued = it + 1;
         }
+        __syncwarp();
+        issued = it + 1;
       }
     }
+    if (!ok && lane == 0) *abort_flag = 1;
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA ----
     // instruction descriptor: float32 sums, 128 x BN, both operands K-major and of one 16-bit type
     constexpr uint32_t idesc = HALF ? make_idesc_bf16(kRows, BN) & ~((1u << 7) | (1u << 10)) : make_idesc_bf16(kRows, BN);
-    const uint32_t base = smem_u32(smem);
+    const uint64_t x_desc = make_sdesc_k_sw128(smem_u32(smem));  // start addresses add up in its low bits
     int it = 0, lt = 0;
     bool ok = true;
     for (int tile = first; ok && tile < num_tiles; tile += stride, ++lt) {
-      const int acc = lt % L::kAcc;
-      if (lt >= L::kAcc) ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], (lt / L::kAcc - 1) & 1, a.err, 423));
+      const int acc = lt & 1;
+      if (lt >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], ((lt >> 1) - 1) & 1, a.err, 423));
       if (!ok) break;
       tc_fence_after();
       for (int k = k0; k < k1 && ok; ++k, ++it) {
@@ -253,24 +265,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                                          mbar_wait(&xfull[xs], (it / L::kXs) & 1, a.err, 424));
         if (!ok) break;
         tc_fence_after();
+        const uint32_t d = tmem + acc * BN, wa = tmem + 2 * BN + as * kACols;
+        const uint64_t xd = x_desc + static_cast<uint32_t>(xs * L::kX >> 4);
+        if (elect_one()) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (lane == 0) {
-            const uint32_t wa = tmem + L::kAcc * BN + as * kACols + h * (kACols / 2);
-            const uint32_t xa = base + xs * L::kX + h * (L::kX / 2);
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              tc_mma_f16_ta(tmem + acc * BN, wa + q * 8, make_sdesc_k_sw128(xa + q * 32), idesc,
-                            (k > k0 || h > 0 || q > 0) ? 1u : 0u);
-          }
-        }
-        if (lane == 0) {
+          for (int q = 0; q < 8; ++q)  // 16 columns: 8 of tensor memory, 32 bytes of a 64-column tile of x
+            tc_mma_f16_ta(d, wa + q * 8, xd + static_cast<uint32_t>((q >> 2) * (L::kX / 2) + (q & 3) * 32 >> 4), idesc,
+                          k > k0 || q > 0 ? 1u : 0u);
           tc_commit(&xempty[xs]);
           tc_commit(&aempty[as]);
         }
         __syncwarp();
       }
-      if (ok && lane == 0) tc_commit(&acc_full[acc]);
+      if (ok && elect_one()) tc_commit(&acc_full[acc]);
       __syncwarp();
     }
     if (!ok && lane == 0) *abort_flag = 1;
@@ -279,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ----------------------------------------------------- converters ----
     // warp q + 4 h of a set: rows 32 q .. 32 q + 31 (the tensor-memory lanes it reaches), columns 64 h .. of a step
     const int set = (warp - 8) / 8, quad = warp & 3, half = (warp >> 2) & 1, g = lane >> 2;
-    const uint32_t a_base = tmem + L::kAcc * BN + half * (kACols / 2) + (static_cast<uint32_t>(32 * quad) << 16);
+    const uint32_t a_base = tmem + 2 * BN + half * (kACols / 2) + (static_cast<uint32_t>(32 * quad) << 16);
     constexpr int H = P == 4 ? 2 : 1;  // groups of 64 columns
     int it = 0;
     bool ok = true;
@@ -376,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int lt = 0;
     bool ok = true;
     for (int tile = first; tile < num_tiles; tile += stride, ++lt) {
-      const int acc = lt % L::kAcc;
-      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (lt / L::kAcc) & 1, a.err, 428));
+      const int acc = lt & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (lt >> 1) & 1, a.err, 428));
       if (!ok) break;
       tc_fence_after();
       const int m0 = tile % a.m_tiles * BN;
@@ -406,6 +413,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t dst = map_shared_rank(smem_u32(recv + (rank * per + (c + j) % per) * kRows + row), (c + j) / per);
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(__uint_as_float(r[j])) : "memory");
           }
+        } else if (a.vec_out) {
+          // 32 rows of x by 32 outputs, turned in shared memory into 16-byte pieces of a row
+          uint16_t* turn = reinterpret_cast<uint16_t*>(smem + L::kOut + quad * 2048);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float v = __uint_as_float(r[j]) * pow + bias;
+            turn[j * 32 + lane] = a.out_type == static_cast<int>(DType::kF16) ? __half_as_ushort(__float2half_rn(v))
+                                                                             : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int i = q * 32 + lane, m = m0 + c + i / 4;
+            const int64_t n8 = n - lane + i % 4 * 8;
+            if (m < a.M && n8 < a.N)  // N is a multiple of 8 here
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + m * a.ldo + n8) =
+                  *reinterpret_cast<const uint4*>(turn + i * 8);
+          }
+          __syncwarp();
         } else if (in) {
           // neighbouring lanes are neighbouring outputs of one row
 #pragma unroll
@@ -561,11 +587,11 @@ template <bool HALF>
 void launch_type(GArgs a, const void* x, int64_t ldx, int64_t K, int group, cudaStream_t s) {
   // rows of x per tile: the size with the least time in the busiest CTA, per 64 columns 2 cycles per row of x in
   // the tensor cores against about kConvert to unpack 128 weight rows
-  constexpr int kConvert = 250;
+  constexpr int kConvert = 350;
   const int sms = 148;
-  int best = 256;
+  int best = 192;
   int64_t best_cost = -1;
-  for (int bn : {256, 128, 64, 32}) {
+  for (int bn : {192, 128, 64, 32}) {
     const int64_t tiles = (static_cast<int64_t>(a.M) + bn - 1) / bn * a.n_tiles;
     const int64_t cost = (tiles + sms - 1) / sms * std::max(2 * bn, kConvert);
     if (best_cost < 0 || cost < best_cost || (cost == best_cost && bn >= a.M)) best = bn, best_cost = cost;
@@ -581,7 +607,7 @@ void launch_type(GArgs a, const void* x, int64_t ldx, int64_t K, int group, cuda
     case 32: launch_group<32, HALF>(a, tw, tm, group, s); break;
     case 64: launch_group<64, HALF>(a, tw, tm, group, s); break;
     case 128: launch_group<128, HALF>(a, tw, tm, group, s); break;
-    default: launch_group<256, HALF>(a, tw, tm, group, s); break;
+    default: launch_group<192, HALF>(a, tw, tm, group, s); break;
   }
 }
 
@@ -598,6 +624,8 @@ void launch_int4_gemm(const Int4LinearArgs& r, cudaStream_t s) {
   a.scale_half = r.scale_type == DType::kF16;
   a.bias_type = static_cast<int>(r.bias_type), a.out_type = static_cast<int>(r.out_type);
   a.err = ErrorSink{r.err};
+  a.vec_out = r.out_type != DType::kF32 && r.N % 8 == 0 && (r.M == 1 || r.ldo % 8 == 0) &&
+              reinterpret_cast<uintptr_t>(r.out) % 16 == 0;
   const void* x = r.x;
   int64_t ldx = r.M > 1 ? r.ldx : r.K;
   if (r.x_scales != nullptr) {
