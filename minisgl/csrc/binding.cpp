@@ -621,7 +621,7 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
   }
   if (zeros.has_value()) {
     MSG_CHECK(zeros->is_cuda() && zeros->scalar_type() == at::kByte && zeros->is_contiguous() &&
-                  zeros->numel() == tiles * groups * 8 && reinterpret_cast<uintptr_t>(zeros->data_ptr()) % 16 == 0,
+                  zeros->numel() == tiles * (groups + groups % 2) * 8 && reinterpret_cast<uintptr_t>(zeros->data_ptr()) % 16 == 0,
               "int4_linear: weight zero points of the wrong type or size");
     check_same_device(x, *zeros);
     a.zeros = zeros->data_ptr<uint8_t>();

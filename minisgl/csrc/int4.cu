@@ -83,13 +83,14 @@ struct VecArgs {
   const uint8_t* x_scales;
   const uint8_t* packed;
   const uint32_t* scales;  // [16-row tiles, groups, 8] pairs
-  const uint8_t* zeros;    // [16-row tiles, groups, 8]
+  const uint8_t* zeros;    // [16-row tiles, groups rounded up to even, 8]
   const void* bias;
   void* out;
   int M, N, K, tiles, steps, S;  // tiles of 16 R rows, steps of 128 columns
   int tiles_each, tiles_more, steps_each, steps_more;
   uint32_t inv_each, inv_more;  // 2^31 / steps_each and / (steps_each + 1), rounded up
   int64_t ldx, ld_xs, ldo;
+  int ld_z;  // bytes of a 16-row tile's zero points
   int scale_half, bias_type, out_type;
   int x_kind;
   int x_bytes;     // of the x area
@@ -214,7 +215,7 @@ __device__ __noinline__ float not_finite_part(const VecArgs& a, int64_t tile, in
           a.packed)[((tile * a.steps * 2 + (k + j) / 64) * 32 + 4 * (r & 7) + t) * 4 + c / 16];
       const int code = (word >> (4 * (4 * e + 2 * q + (r >> 3))) & 15) ^ 8;
       const int64_t gi = tile * (a.steps * 128 / group) + (k + j) / group;
-      const uint32_t zz = a.zeros != nullptr ? a.zeros[gi * 8 + (r & 7)] : 0x88u;
+      const uint32_t zz = a.zeros != nullptr ? a.zeros[tile * a.ld_z + (k + j) / group * 8 + (r & 7)] : 0x88u;
       const uint32_t sw = a.scales[gi * 8 + (r & 7)];
       const float s = half_bits_to_f32(r >> 3 ? sw >> 16 : sw & 0xFFFFu, a.scale_half);
       sum += v[j] * (static_cast<float>(code - static_cast<int>(r >> 3 ? zz >> 4 : zz & 15u)) * s);
@@ -280,7 +281,8 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   const uint8_t* src_w = a.packed + first * 1024 + lane * 16;
   constexpr int SW = 8 * P, ZW = 2 * P;  // scale and zero words of a tile
   const uint32_t* src_s = a.scales + (first + (P < 4 && lane >= SW ? a.steps : 0)) * SW + (P < 4 ? lane % SW : lane);
-  const uint8_t* src_z = ZERO ? a.zeros + (first + (lane >= ZW ? a.steps : 0)) * SW + lane % ZW * 4 : nullptr;
+  const uint8_t* src_z =
+      ZERO ? a.zeros + (static_cast<int64_t>(tile) * kR + (lane >= ZW ? 1 : 0)) * a.ld_z + (k0 + k) * SW + lane % ZW * 4 : nullptr;
   int left = u1 - u0, pk = k;
   const int skip = kR * a.steps - ks;  // from the end of a unit row to the start of the next
   const int64_t second = static_cast<int64_t>(a.steps) * 1024;
@@ -299,11 +301,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
         for (int r = 0; r < kR; ++r) cp_async4(dst + kR * 1024 + (r * SW + lane) * 4, src_s + r * a.steps * SW);
       }
       if (ZERO && lane < kR * ZW) cp_async4(dst + kR * (1024 + L::kScaleB) + lane * 4, src_z);
-      int on = 1;
-      if (++pk == ks) pk = 0, on += skip;
+      int on = 1, on_z = SW;
+      if (++pk == ks) pk = 0, on += skip, on_z = kR * a.ld_z - (ks - 1) * SW;
       src_w += static_cast<int64_t>(on) * 1024;
       src_s += static_cast<int64_t>(on) * SW;
-      if (ZERO) src_z += static_cast<int64_t>(on) * SW;
+      if (ZERO) src_z += on_z;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -727,6 +729,7 @@ void launch_int4_linear(const Int4LinearArgs& r, cudaStream_t s) {
     v.M = static_cast<int>(r.M), v.N = static_cast<int>(r.N), v.K = static_cast<int>(r.K);
     v.steps = (v.K + 127) / 128;
     v.ldx = r.ldx, v.ld_xs = r.ld_xs, v.ldo = r.ldo;
+    v.ld_z = static_cast<int>((v.steps * (128 / r.group) + 1) / 2 * 16);
     v.scale_half = r.scale_type == DType::kF16;
     v.bias_type = static_cast<int>(r.bias_type), v.out_type = static_cast<int>(r.out_type);
     v.x_kind = r.x_scales != nullptr ? kXMx8 : r.x_type == DType::kF16 ? kXHalf : kXBf16;

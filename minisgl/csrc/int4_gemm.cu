@@ -55,8 +55,9 @@ struct GSmem {
   static constexpr int kPs = BN == 192 ? 3 : 6;
   static constexpr int kAs = BN == 192 ? 2 : BN == 32 ? 3 : 4;  // steps of weights in tensor memory
   static constexpr int kPt = kXs * kX;
-  static constexpr int kOut = kPt + kPs * kCodes;  // the epilogue's 2 KB a warp
-  static constexpr int kRing = kOut + 4 * 2048;
+  static constexpr int kSt = kPt + kPs * kCodes;   // the steps' scales, 1 KB apart
+  static constexpr int kZt = kSt + kPs * 1024;     // and zero points, 256 bytes apart
+  static constexpr int kOut = kZt + kPs * 256;    static constexpr int kRing = kOut + 4 * 1024;  // the epilogue's 1 KB a warp
   static constexpr int kBars = 8 * (2 * kXs + 2 * kPs + 2 * kAs + 4) + 16;
   static constexpr int bytes(int S) { return 1024 + kRing + (kBars + 127) / 128 * 128 + (S > 1 ? kRows * BN * 4 : 0); }
   static_assert(bytes(BN <= 64 ? 2 : 1) <= 227 * 1024, "shared memory");
@@ -66,8 +67,7 @@ struct GSmem {
 
 struct GArgs {
   const uint8_t* packed;
-  const uint32_t* scales;
-  const uint8_t* zeros;
+  const uint8_t* zeros;  // nullptr: 8 everywhere
   const float* row_pow;  // fp16: power of two taken out of a row's scales
   const void* bias;
   void* out;
@@ -146,9 +146,11 @@ struct Pair {
 
 template <int BN, int G, bool HALF>
 __global__ void __launch_bounds__(kThreads, 1)
-    int4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const GArgs a) {
+    int4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_s,
+                     const __grid_constant__ CUtensorMap tm_z, const __grid_constant__ CUtensorMap tm_x, const GArgs a) {
   using L = GSmem<BN>;
   constexpr int P = 128 / G;
+  constexpr int kZeroRow = P == 1 ? 16 : 8 * P, kZeroB = 8 * kZeroRow;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* xfull = reinterpret_cast<uint64_t*>(smem + L::kRing);
@@ -178,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     *s_abort = 0;
     fence_barrier_init();
     prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_s);
     prefetch_tmap(&tm_x);
   }
   // the first codes, on their way to L2 while the kernel before this one ends (a prefetch carries no value)
@@ -238,8 +241,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         if (elect_one()) {
           // eight tiles x 1 KB in one copy (eight bulk copies took 130 cycles each to issue)
-          mbar_arrive_expect_tx(&pfull[s], kCodes);
+          mbar_arrive_expect_tx(&pfull[s], kCodes + 256 * P + (a.zeros ? kZeroB : 0));
           tma_load_2d(smem + L::kPt + s * kCodes, &tm_w, &pfull[s], k * 256, t16);
+          tma_load_2d(smem + L::kSt + s * 1024, &tm_s, &pfull[s], k * (8 * P), t16);
+          // zero points by 16 bytes a tile: with one group a step those of an even step and the next
+          if (a.zeros) tma_load_2d(smem + L::kZt + s * 256, &tm_z, &pfull[s], P == 1 ? (k & ~1) * 8 : k * (8 * P), t16);
         }
         __syncwarp();
         issued = it + 1;
@@ -291,43 +297,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     int it = 0;
     bool ok = true;
     for (int tile = first; ok && tile < num_tiles; tile += stride) {
-      const uint32_t* sp[2];
-      const uint8_t* zp[2];
       float down[2][2];  // 1 / the rows' power of two
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int tile16 = min(tile / a.m_tiles * 8 + 2 * quad + c, a.tiles16 - 1);  // rows past N: any codes, never stored
-        const int64_t at = static_cast<int64_t>(tile16) * a.steps * (P * 8) + (P == 1 ? 0 : half * (H * 8)) + g;
-        sp[c] = a.scales + at;
-        zp[c] = a.zeros + at;
+        const int tile16 = min(tile / a.m_tiles * 8 + 2 * quad + c, a.tiles16 - 1);  // rows past N are never stored
 #pragma unroll
         for (int r = 0; r < 2; ++r) down[c][r] = HALF ? 1.f / a.row_pow[tile16 * 16 + g + 8 * r] : 1.f;
       }
-      uint32_t sc[2][H], zz[2][H], sc_next[2][H], zz_next[2][H];
-      auto load_scales = [&](int k) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int p = 0; p < H; ++p) {
-            sc_next[c][p] = sp[c][(k * P + p) * 8];
-            zz_next[c][p] = a.zeros != nullptr ? zp[c][(k * P + p) * 8] : 0x88u;
-          }
-      };
       // this set's steps of the tile
       const int turn = (set + kSets - it % kSets) % kSets;
-      if (k0 + turn < k1) load_scales(k0 + turn);
       for (int k = k0; k < k1 && ok; ++k, ++it) {
         if ((k - k0) % kSets != turn) continue;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int p = 0; p < H; ++p) sc[c][p] = sc_next[c][p], zz[c][p] = zz_next[c][p];
-        if (k + kSets < k1) load_scales(k + kSets);
         const int ps = it % L::kPs, as = it % L::kAs;
         ok = __all_sync(0xffffffffu, mbar_wait(&pfull[ps], (it / L::kPs) & 1, a.err, 426));
         if (!ok) break;
         const uint4* codes = reinterpret_cast<const uint4*>(smem + L::kPt + ps * kCodes + quad * 2048 + half * 512) + lane;
         const uint4 w[2] = {codes[0], codes[64]};
+        uint32_t sc[2][H], zz[2][H];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int p = 0; p < H; ++p) {
+            const int tile16 = 2 * quad + c, group = P == 1 ? 0 : half * H + p;
+            sc[c][p] = *reinterpret_cast<const uint32_t*>(smem + L::kSt + ps * 1024 + (tile16 * P + group) * 32 + g * 4);
+            zz[c][p] = a.zeros == nullptr
+                           ? 0x88u
+                           : smem[L::kZt + ps * 256 + tile16 * kZeroRow + (P == 1 ? (k & 1) * 8 : group * 8) + g];
+          }
         __syncwarp();
         if (lane == 0) mbar_arrive(&pempty[ps]);  // the codes are in registers
         if (it >= L::kAs) ok = __all_sync(0xffffffffu, mbar_wait(&aempty[as], ((it / L::kAs) - 1) & 1, a.err, 427));
@@ -414,24 +410,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(__uint_as_float(r[j])) : "memory");
           }
         } else if (a.vec_out) {
-          // 32 rows of x by 32 outputs, turned in shared memory into 16-byte pieces of a row
-          uint16_t* turn = reinterpret_cast<uint16_t*>(smem + L::kOut + quad * 2048);
+          // 16 rows of x by 32 outputs at a time, turned in shared memory into 16-byte pieces of a row
+          uint16_t* turn = reinterpret_cast<uint16_t*>(smem + L::kOut + quad * 1024);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float v = __uint_as_float(r[j]) * pow + bias;
-            turn[j * 32 + lane] = a.out_type == static_cast<int>(DType::kF16) ? __half_as_ushort(__float2half_rn(v))
-                                                                             : __bfloat16_as_ushort(__float2bfloat16_rn(v));
-          }
-          __syncwarp();
+          for (int b = 0; b < 32; b += 16) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int i = q * 32 + lane, m = m0 + c + i / 4;
-            const int64_t n8 = n - lane + i % 4 * 8;
-            if (m < a.M && n8 < a.N)  // N is a multiple of 8 here
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + m * a.ldo + n8) =
-                  *reinterpret_cast<const uint4*>(turn + i * 8);
+            for (int j = 0; j < 16; ++j) {
+              const float v = __uint_as_float(r[b + j]) * pow + bias;
+              turn[j * 32 + lane] = a.out_type == static_cast<int>(DType::kF16) ? __half_as_ushort(__float2half_rn(v))
+                                                                               : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+            }
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int i = q * 32 + lane, m = m0 + c + b + i / 4;
+              const int64_t n8 = n - lane + i % 4 * 8;
+              if (m < a.M && n8 < a.N)  // N is a multiple of 8 here
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + m * a.ldo + n8) =
+                    *reinterpret_cast<const uint4*>(turn + i * 8);
+            }
+            __syncwarp();
           }
-          __syncwarp();
         } else if (in) {
           // neighbouring lanes are neighbouring outputs of one row
 #pragma unroll
@@ -539,7 +538,7 @@ int resident(int S, int smem) {
 }
 
 template <int BN, int G, bool HALF>
-void launch_bn(GArgs a, const CUtensorMap& tw, const CUtensorMap& tm, cudaStream_t s) {
+void launch_bn(GArgs a, const CUtensorMap* tw, const CUtensorMap& tm, cudaStream_t s) {
   constexpr auto kern = int4_gemm_kernel<BN, G, HALF>;
   using L = GSmem<BN>;
   a.m_tiles = (a.M + BN - 1) / BN;
@@ -570,12 +569,12 @@ void launch_bn(GArgs a, const CUtensorMap& tw, const CUtensorMap& tm, cudaStream
   }
   cfg.attrs = attrs;
   cfg.numAttrs = n;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tm, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw[0], tw[1], tw[2], tm, a);
   if (e != cudaSuccess) throw std::runtime_error(std::string("minisgl: kernel launch failed: ") + cudaGetErrorString(e));
 }
 
 template <int BN, bool HALF>
-void launch_group(const GArgs& a, const CUtensorMap& tw, const CUtensorMap& tm, int group, cudaStream_t s) {
+void launch_group(const GArgs& a, const CUtensorMap* tw, const CUtensorMap& tm, int group, cudaStream_t s) {
   switch (group) {
     case 32: launch_bn<BN, 32, HALF>(a, tw, tm, s); break;
     case 64: launch_bn<BN, 64, HALF>(a, tw, tm, s); break;
@@ -584,10 +583,10 @@ void launch_group(const GArgs& a, const CUtensorMap& tw, const CUtensorMap& tm, 
 }
 
 template <bool HALF>
-void launch_type(GArgs a, const void* x, int64_t ldx, int64_t K, int group, cudaStream_t s) {
+void launch_type(GArgs a, const void* scales, const void* x, int64_t ldx, int64_t K, int group, cudaStream_t s) {
   // rows of x per tile: the size with the least time in the busiest CTA, per 64 columns 2 cycles per row of x in
   // the tensor cores against about kConvert to unpack 128 weight rows
-  constexpr int kConvert = 350;
+  constexpr int kConvert = 400;
   const int sms = 148;
   int best = 192;
   int64_t best_cost = -1;
@@ -598,11 +597,19 @@ void launch_type(GArgs a, const void* x, int64_t ldx, int64_t K, int group, cuda
   }
   a.x_blocks = K % 64 == 0;
   const CUtensorMap tm = a.x_blocks ? make_tmap_bf16_kblocks(x, a.M, K, ldx, best, 2) : make_tmap_bf16_2d_sw128(x, a.M, K, ldx, best);
-  // codes: a row of the map is a tile of 16 rows, its columns the tile's 128-column units (256 words)
-  const uint64_t dims[2] = {static_cast<uint64_t>(a.steps) * 256, static_cast<uint64_t>(a.tiles16)};
-  const uint64_t strides[1] = {static_cast<uint64_t>(a.steps) * 1024};
-  const uint32_t box[2] = {256, 8};
-  const CUtensorMap tw = make_tmap(a.packed, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+  // codes, scales, zero points: a row of a map is a tile of 16 rows, its columns the tile's 128-column units
+  const uint64_t tiles = static_cast<uint64_t>(a.tiles16), steps = static_cast<uint64_t>(a.steps), per = 128 / group;
+  const auto words = [&](const void* p, CUtensorMapDataType type, int size, uint64_t cols, uint32_t box_cols) {
+    const uint64_t dims[2] = {cols, tiles}, strides[1] = {cols * size};
+    const uint32_t box[2] = {box_cols, 8};
+    return make_tmap(p, type, size, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+  };
+  const uint32_t pairs = static_cast<uint32_t>(8 * per);
+  CUtensorMap tw[3];
+  tw[0] = words(a.packed, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, steps * 256, 256);
+  tw[1] = words(scales, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, steps * pairs, pairs);
+  tw[2] = a.zeros == nullptr ? tw[1]
+                             : words(a.zeros, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (steps * per + 1) / 2 * 16, std::max(16u, pairs));
   switch (best) {
     case 32: launch_group<32, HALF>(a, tw, tm, group, s); break;
     case 64: launch_group<64, HALF>(a, tw, tm, group, s); break;
@@ -615,7 +622,7 @@ void launch_type(GArgs a, const void* x, int64_t ldx, int64_t K, int group, cuda
 
 void launch_int4_gemm(const Int4LinearArgs& r, cudaStream_t s) {
   GArgs a{};
-  a.packed = r.packed, a.scales = static_cast<const uint32_t*>(r.scales), a.zeros = r.zeros, a.row_pow = r.row_pow;
+  a.packed = r.packed, a.zeros = r.zeros, a.row_pow = r.row_pow;
   a.bias = r.bias, a.out = r.out;
   a.M = static_cast<int>(r.M), a.N = static_cast<int>(r.N);
   a.steps = static_cast<int>((r.K + 127) / 128), a.tiles16 = static_cast<int>(2 * ((r.N + 31) / 32));
@@ -637,9 +644,9 @@ void launch_int4_gemm(const Int4LinearArgs& r, cudaStream_t s) {
     ldx = r.K;
   }
   if (r.x_scales == nullptr && r.x_type == DType::kF16)
-    launch_type<true>(a, x, ldx, r.K, r.group, s);
+    launch_type<true>(a, r.scales, x, ldx, r.K, r.group, s);
   else
-    launch_type<false>(a, x, ldx, r.K, r.group, s);
+    launch_type<false>(a, r.scales, x, ldx, r.K, r.group, s);
 }
 
 }  // namespace minisgl

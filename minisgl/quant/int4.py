@@ -46,7 +46,8 @@ class Int4Weight:
     """A 4-bit weight in the kernels' layout (made by ``int4_weight`` or
     ``quantize_int4``): ``packed`` uint8 [tiles, 2 ceil(K / 128), 512],
     ``scales`` bf16 / fp16 [tiles, groups, 8, 2] and ``zeros`` uint8
-    [tiles, groups, 8] or None, tiles = 2 ceil(N / 32), groups = 128 ceil(K / 128) / group;
+    [tiles, groups rounded up to even, 8] or None, tiles = 2 ceil(N / 32), groups =
+    128 ceil(K / 128) / group;
     ``row_pow`` float32 [16 tiles]: the power of two at or below a row's largest scale
     (1 where that is 0), which fp16 products take out of the row."""
 
@@ -114,7 +115,7 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
     groups = blocks * _BLOCK // group
     z = None
     if zeros is not None:
-        z = _tile_rows(zeros, groups)
+        z = _tile_rows(zeros, groups + groups % 2)  # whole 16-byte rows
         z = z[..., 0] | (z[..., 1] << 4)
     tiled = _tile_rows(scales, groups)
     top = tiled.float().abs().amax(1).transpose(1, 2).reshape(-1)  # [tile, g, h] -> row
