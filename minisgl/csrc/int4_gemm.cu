@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* acc_empty = acc_full + 2;  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
-  float* recv = reinterpret_cast<float*>(smem + L::kRing + (L::kBars + 127) / 128 * 128);  // [rank][BN / S][128]
+  float* part = reinterpret_cast<float*>(smem + L::kRing + (L::kBars + 127) / 128 * 128);  // S > 1: [BN][128] sums
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int S = a.S, rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -326,13 +326,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         __syncwarp();
         if (lane == 0) mbar_arrive(&pempty[ps]);  // the codes are in registers
-        if (it >= L::kAs) ok = __all_sync(0xffffffffu, mbar_wait(&aempty[as], ((it / L::kAs) - 1) & 1, a.err, 427));
-        if (!ok) break;
-        tc_fence_after();
+        uint32_t o[2][16];  // per tile and word (16 columns): two pairs of row g, two of row g + 8
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
-          uint32_t o[16];  // per word (16 columns): two pairs of row g, two of row g + 8
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const uint32_t sw = sc[c][j * H / 4], zw = zz[c][j * H / 4];
@@ -353,17 +350,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 s[0] = __byte_perm(sw, 0, 0x1010), s[1] = __byte_perm(sw, 0, 0x3232);
               }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) o[4 * j + i] = Pair<HALF>::mul(d[i], s[i >> 1]);
+              for (int i = 0; i < 4; ++i) o[c][4 * j + i] = Pair<HALF>::mul(d[i], s[i >> 1]);
             } else {
               // fp16 scales do not fit bf16: the product is formed in float32 and rounded once
               const float f[2] = {scale_f32(sw & 0xFFFFu, 1), scale_f32(sw >> 16, 1)};
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                o[4 * j + i] = pack_bf16x2(__uint_as_float(d[i] << 16) * f[i >> 1], __uint_as_float(d[i] & 0xFFFF0000u) * f[i >> 1]);
+                o[c][4 * j + i] = pack_bf16x2(__uint_as_float(d[i] << 16) * f[i >> 1], __uint_as_float(d[i] & 0xFFFF0000u) * f[i >> 1]);
             }
           }
-          tmem_st_16x256b_x4(a_base + as * kACols + (static_cast<uint32_t>(16 * c) << 16), o);
         }
+        // only the store waits for the MMAs that read the slot before
+        if (it >= L::kAs) ok = __all_sync(0xffffffffu, mbar_wait(&aempty[as], ((it / L::kAs) - 1) & 1, a.err, 427));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          tmem_st_16x256b_x4(a_base + as * kACols + (static_cast<uint32_t>(16 * c) << 16), o[c]);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -403,12 +406,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&acc_empty[acc]);
         }
         if (S > 1) {
-          const int per = BN / S;  // rows of x that a CTA of the cluster finishes
 #pragma unroll
-          for (int j = 0; j < CH; ++j) {
-            const uint32_t dst = map_shared_rank(smem_u32(recv + (rank * per + (c + j) % per) * kRows + row), (c + j) / per);
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(__uint_as_float(r[j])) : "memory");
-          }
+          for (int j = 0; j < CH; ++j) part[(c + j) * kRows + row] = __uint_as_float(r[j]);
         } else if (a.vec_out) {
           // 16 rows of x by 32 outputs at a time, turned in shared memory into 16-byte pieces of a row
           uint16_t* turn = reinterpret_cast<uint16_t*>(smem + L::kOut + quad * 1024);
@@ -457,22 +456,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_dealloc(tmem, L::kCols);
   }
   if (S > 1) {
-    // one tile per cluster: this CTA's BN / S rows of x, the S partial sums in rank order
+    // one tile per cluster: this CTA adds BN / S of its rows of x, the S partial sums in rank order
     __syncwarp();
     cluster_sync();
     const int per = BN / S;
-    const int m0 = first % a.m_tiles * BN + rank * per;
     const int64_t n0 = static_cast<int64_t>(first / a.m_tiles) * kRows;
-    for (int i = threadIdx.x; i < per * kRows; i += kThreads) {
-      const int m = m0 + i / kRows;
-      const int64_t n = n0 + i % kRows;
-      if (m >= a.M || n >= a.N || *abort_flag) continue;
-      float v = 0.f;
-      for (int r = 0; r < S; ++r) v += recv[r * per * kRows + i];
-      if (HALF) v *= a.row_pow[n];
-      if (a.bias != nullptr) v += any_f32(a.bias, n, a.bias_type);
-      store_any(a.out, static_cast<int64_t>(m) * a.ldo + n, a.out_type, v);
+    for (int i = threadIdx.x; i < per * (kRows / 4); i += kThreads) {
+      const int at = rank * per + i / (kRows / 4), q = i % (kRows / 4) * 4;
+      const int m = first % a.m_tiles * BN + at;
+      if (m >= a.M) continue;
+      const uint32_t local = smem_u32(part + at * kRows + q);
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int r = 0; r < S; ++r) {
+        const float4 p = ld_shared_cluster_v4(map_shared_rank(local, r));
+        v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t n = n0 + q + j;
+        if (n >= a.N || *abort_flag) continue;
+        if (HALF) v[j] *= a.row_pow[n];
+        if (a.bias != nullptr) v[j] += any_f32(a.bias, n, a.bias_type);
+        store_any(a.out, static_cast<int64_t>(m) * a.ldo + n, a.out_type, v[j]);
+      }
     }
+    cluster_sync();  // no CTA leaves while a peer reads its sums
   }
 }
 
