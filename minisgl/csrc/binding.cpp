@@ -611,11 +611,11 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
                 row_pow.numel() == tiles * 16,
             "int4_linear: row powers of the wrong type or size");
   check_same_device(x, row_pow);
-  if (x_scales.has_value() && M > 16) {
+  if (x_scales.has_value() && M > 8) {
     MSG_CHECK(x_wide.has_value() && x_wide->is_cuda() && x_wide->scalar_type() == at::kBFloat16 &&
                   x_wide->is_contiguous() && x_wide->numel() >= M * K &&
                   reinterpret_cast<uintptr_t>(x_wide->data_ptr()) % 16 == 0,
-              "int4_linear: bf16 scratch of M * K for more than 16 MXFP8 rows");
+              "int4_linear: bf16 scratch of M * K for more than 8 MXFP8 rows");
     check_same_device(x, *x_wide);
     a.x_wide = x_wide->data_ptr();
   }

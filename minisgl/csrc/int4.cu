@@ -49,9 +49,9 @@ __device__ __forceinline__ float e8m0(uint32_t byte) {
 
 
 // ---------------------------------------------------------------------------
-// Few rows (up to 16): the weight stream.
+// Few rows (up to 8, one operand of a warp-level product): the weight stream.
 //
-// A unit is R tiles of 16 rows x 128 columns (R KB of codes and their scales).
+// A unit is kR tiles of 16 rows x 128 columns (kR KB of codes and their scales).
 // Whole tiles are dealt to clusters of S = 1, 2, 4 or 8 CTAs, whose CTAs share
 // the columns; the units of a CTA, tile after tile, are cut into one contiguous
 // range per warp. Each warp copies its own units into its own ring of shared
@@ -74,7 +74,9 @@ __device__ __forceinline__ float e8m0(uint32_t byte) {
 // are added in rank order after a cluster barrier. Every sum has a fixed order:
 // the same inputs give the same bits.
 // ---------------------------------------------------------------------------
+constexpr int kFew = 8;  // rows of x
 constexpr int kDepth = 3;
+constexpr int kR = 2;    // 16-row tiles of a unit: their products share the reads of x
 constexpr int kMaxSmem = 227 * 1024;
 
 enum { kXBf16 = 0, kXHalf = 1, kXMx8 = 2 };
@@ -86,7 +88,7 @@ struct VecArgs {
   const uint8_t* zeros;    // [16-row tiles, groups rounded up to even, 8]
   const void* bias;
   void* out;
-  int M, N, K, tiles, steps, S;  // tiles of 16 R rows, steps of 128 columns
+  int M, N, K, tiles, steps, S;  // tiles of 16 kR rows, steps of 128 columns
   int tiles_each, tiles_more, steps_each, steps_more;
   uint32_t inv_each, inv_more;  // 2^31 / steps_each and / (steps_each + 1), rounded up
   int64_t ldx, ld_xs, ldo;
@@ -97,20 +99,17 @@ struct VecArgs {
   int recv_slots;  // tiles that a CTA owns at most (S > 1)
 };
 
-// R: 16-row tiles of a unit, whose products share the reads of x (two for up to 8 rows of x; one for 16, whose
-// sums need the registers)
-template <int W, int NT, int G, bool ZERO>
+template <int W, int G, bool ZERO>
 struct VecSmem {
-  static constexpr int kR = NT == 1 ? 2 : 1;
   static constexpr int kGroups = 128 / G;
   static constexpr int kScaleB = kGroups * 32;  // of one tile
   static constexpr int kZeroB = kGroups * 8;
   static constexpr int kUnit = (kR * (1024 + kScaleB + kZeroB) + 15) / 16 * 16;  // 16-byte copies into every slot
   static constexpr int kRing = W * kDepth * kUnit;
-  // per step and 8 rows of x: the power of two and, with zero points, each group's sum in two parts
+  // per step: each row's power of two and, with zero points, each group's sum in two parts
   static constexpr int kSide = 32 + (ZERO ? 64 * kGroups : 0);
   static int total(int x_bytes, int recv_slots, int S) {
-    return kRing + (W * 2 + recv_slots * S) * 512 * kR * NT + x_bytes;
+    return kRing + (W * 2 + recv_slots * S) * 512 * kR + x_bytes;
   }
 };
 // bytes between x's rows (three digits of 128 columns a step): an odd
@@ -231,10 +230,9 @@ __device__ __forceinline__ void store_sum(const VecArgs& a, int64_t tile, int r,
   store_from_f32(a.out, m * a.ldo + n, a.out_type, v);
 }
 
-template <int W, int NT, int G, bool ZERO>
+template <int W, int G, bool ZERO>
 __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs a) {
-  using L = VecSmem<W, NT, G, ZERO>;
-  constexpr int kR = L::kR;
+  using L = VecSmem<W, G, ZERO>;
   constexpr int P = L::kGroups;  // groups of a unit
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -252,11 +250,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   const int units = (t1 - t0) * ks;
   auto warp_start = [&](int w) { return units / W * w + (units % W * w) / W; };
   const int u0 = warp_start(warp), u1 = warp_start(warp + 1);
-  float4* park = reinterpret_cast<float4*>(smem + L::kRing);  // [warp][2: head, tail][R][NT][lane]
-  uint8_t* xs = smem + L::kRing + W * 2 * 512 * kR * NT;
+  float4* park = reinterpret_cast<float4*>(smem + L::kRing);  // [warp][2: head, tail][R][lane]
+  uint8_t* xs = smem + L::kRing + W * 2 * 512 * kR;
   const int pitch = vec_x_pitch(ks);
-  uint8_t* side = xs + a.M * pitch;                          // [step][power of two | P sums of two parts][8 NT]
-  float4* recv = reinterpret_cast<float4*>(xs + a.x_bytes);  // [slot][rank][R][NT][lane]
+  uint8_t* side = xs + a.M * pitch;                          // [step][power of two | P sums of two parts][8]
+  float4* recv = reinterpret_cast<float4*>(xs + a.x_bytes);  // [slot][rank][R][lane]
   const uint32_t inv = rank < a.steps_more ? a.inv_more : a.inv_each;
   auto by_ks = [&](int n) { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * inv >> 31); };  // n / ks
   const int u0_tile = by_ks(u0);
@@ -265,11 +263,10 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   // the codes of the warp's first units, on their way to L2 while the kernel before this one ends (a prefetch
   // carries no value: the copies below read memory after griddepcontrol.wait)
   {
-    constexpr int SH = kR == 2 ? 4 : 3;  // lanes of a unit: eight 128-byte lines per KB
-    const int ahead = k + (lane >> SH);  // the units run on through the tile, then in the next
-    if (u0 + (lane >> SH) < u1) {
+    const int ahead = k + (lane >> 4);  // the units run on through the tile, then in the next
+    if (u0 + (lane >> 4) < u1) {
       const int on = ahead >= ks ? by_ks(ahead) : 0;
-      const int64_t row16 = static_cast<int64_t>(tile + on) * kR + (lane >> 3 & (kR - 1));
+      const int64_t row16 = static_cast<int64_t>(tile + on) * kR + (lane >> 3 & 1);
       asm volatile("prefetch.global.L2 [%0];" ::"l"(a.packed + (row16 * a.steps + k0 + ahead - on * ks) * 1024 + (lane & 7) * 128));
     }
   }
@@ -382,7 +379,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
         *reinterpret_cast<uint32_t*>(dst + d * 128) = word[d][0];
         *reinterpret_cast<uint32_t*>(dst + d * 128 + 16) = word[d][1];
       }
-      uint8_t* sd = side + step * (L::kSide * NT);
+      uint8_t* sd = side + step * L::kSide;
       // codes count in sixteenths (they sit in a byte's upper half): 2^-4 goes with the power of two
       if ((c & 15) == 0) *reinterpret_cast<float*>(sd + m * 4) = __uint_as_float((e - 25u) << 23);
       if constexpr (ZERO) {
@@ -392,7 +389,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
 #pragma unroll
         for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(half_warp, sum, o);
         if ((c & (G / 8 - 1)) == 0)
-          *reinterpret_cast<int2*>(sd + NT * 32 + (c & 15) / (G / 8) * (NT * 64) + m * 8) = make_int2(sum & 0xFFFF, sum >> 16);
+          *reinterpret_cast<int2*>(sd + 32 + (c & 15) / (G / 8) * 64 + m * 8) = make_int2(sum & 0xFFFF, sum >> 16);
       }
     }
     load_x();
@@ -401,55 +398,45 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   if (S > 1) cluster_sync();  // the peers have started: their shared memory may be written
 
   // a finished pair of tiles, this CTA's columns
-  auto emit = [&](int tile, float (&acc)[kR][NT][4]) {
+  auto emit = [&](int tile, float (&acc)[kR][4]) {
     if (odd) {
 #pragma unroll
       for (int r = 0; r < kR; ++r)
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[r][i][j] += not_finite_part(a, static_cast<int64_t>(tile) * kR + r, g + (j >> 1) * 8,
-                                            8 * i + 2 * t + (j & 1), G, k0 * 128, min(a.K, (k0 + ks) * 128));
+        for (int j = 0; j < 4; ++j)
+          acc[r][j] += not_finite_part(a, static_cast<int64_t>(tile) * kR + r, g + (j >> 1) * 8, 2 * t + (j & 1), G,
+                                       k0 * 128, min(a.K, (k0 + ks) * 128));
     }
     if (S == 1) {
 #pragma unroll
       for (int r = 0; r < kR; ++r)
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            store_sum(a, static_cast<int64_t>(tile) * kR + r, g + (j >> 1) * 8, 8 * i + 2 * t + (j & 1), acc[r][i][j]);
+        for (int j = 0; j < 4; ++j)
+          store_sum(a, static_cast<int64_t>(tile) * kR + r, g + (j >> 1) * 8, 2 * t + (j & 1), acc[r][j]);
     } else {
       const int local = tile - t0;
-      const uint32_t base = map_shared_rank(smem_u32(recv + (local / S * S + rank) * (kR * NT * 32) + lane), local & (S - 1));
+      const uint32_t base = map_shared_rank(smem_u32(recv + (local / S * S + rank) * (kR * 32) + lane), local & (S - 1));
 #pragma unroll
       for (int r = 0; r < kR; ++r)
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-          asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(base + (r * NT + i) * 512),
-                       "f"(acc[r][i][0]), "f"(acc[r][i][1]), "f"(acc[r][i][2]), "f"(acc[r][i][3])
-                       : "memory");
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(base + r * 512), "f"(acc[r][0]),
+                     "f"(acc[r][1]), "f"(acc[r][2]), "f"(acc[r][3])
+                     : "memory");
     }
   };
 
-  float acc[kR][NT][4];
+  float acc[kR][4];
 #pragma unroll
   for (int r = 0; r < kR; ++r)
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[r][i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) acc[r][j] = 0.f;
   bool head = k != 0;  // the pair was started by the warp before
   const uint32_t x_row = smem_u32(xs) + g * pitch + t * 16;
   uint32_t side_at = smem_u32(side) + t * 8;
   uint32_t src = ring;
   // rows past M stay zero: their lanes never load
-  uint4 xv[NT][3][2];
+  uint4 xv[3][2];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int d = 0; d < 3; ++d) xv[i][d][0] = xv[i][d][1] = make_uint4(0, 0, 0, 0);
+  for (int d = 0; d < 3; ++d) xv[d][0] = xv[d][1] = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
   for (int u = u0; u < u1;) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
@@ -476,68 +463,65 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
     __syncwarp();  // every lane has read the slot
     fetch(src);
     src = src + L::kUnit == ring + kDepth * L::kUnit ? ring : src + L::kUnit;
+    if (g < a.M) {
+      const uint32_t at = x_row + k * 384;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      if (8 * i + g < a.M) {
-        const uint32_t at = x_row + 8 * i * pitch + k * 384;
-#pragma unroll
-        for (int d = 0; d < 3; ++d) {
-          xv[i][d][0] = lds128(at + d * 128);
-          xv[i][d][1] = lds128(at + d * 128 + 64);
-        }
+      for (int d = 0; d < 3; ++d) {
+        xv[d][0] = lds128(at + d * 128);
+        xv[d][1] = lds128(at + d * 128 + 64);
       }
-      const uint32_t sd = side_at + k * (L::kSide * NT) + i * 32;
-      const uint2 pw = lds64(sd);
+    }
+    const uint32_t sd = side_at + k * L::kSide;
+    const uint2 pw = lds64(sd);
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        int c[kR][3][4];
-        // products of one digit and tile wait for one another; the 3 R chains run side by side
+    for (int p = 0; p < P; ++p) {
+      int c[kR][3][4];
+      // products of one digit and tile wait for one another; the 3 R chains run side by side
 #pragma unroll
-        for (int j = p * 4 / P; j < (p + 1) * 4 / P; ++j) {
-#pragma unroll
-          for (int r = 0; r < kR; ++r) {
-#pragma unroll
-            for (int d = 0; d < 3; ++d) {
-              const uint4 v = xv[i][d][j >> 1];
-              const uint32_t b0 = j & 1 ? v.z : v.x, b1 = j & 1 ? v.w : v.y;
-              if (j == p * 4 / P) {
-                if (d == 2)
-                  mma_i8<true, true>(c[r][d], f[r][j], b0, b1);
-                else
-                  mma_i8<false, true>(c[r][d], f[r][j], b0, b1);
-              } else {
-                if (d == 2)
-                  mma_i8<true, false>(c[r][d], f[r][j], b0, b1);
-                else
-                  mma_i8<false, false>(c[r][d], f[r][j], b0, b1);
-              }
-            }
-          }
-        }
-        uint4 sums;
-        if constexpr (ZERO) sums = lds128(sd + NT * 32 + p * (NT * 64) + t * 8 + i * 32);
+      for (int j = p * 4 / P; j < (p + 1) * 4 / P; ++j) {
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
-          float s0, s1;
-          if (a.scale_half) {
-            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&sc[r][p]));
-            s0 = h.x, s1 = h.y;
-          } else {
-            s0 = __uint_as_float(sc[r][p] << 16), s1 = __uint_as_float(sc[r][p] & 0xFFFF0000u);
-          }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            // at most 2^22 (256 + 1) in the lower part, 2^20 in the upper: exact integers, one rounding to float32
-            // each and one where they meet
-            int lo = c[r][1][j] * 256 + c[r][0][j], hi = c[r][2][j];
-            if constexpr (ZERO) {
-              const int z = 16 * static_cast<int>(j < 2 ? zz[r][p] & 15u : zz[r][p] >> 4) - 128;  // 16 (z - 8)
-              lo -= z * static_cast<int>(j & 1 ? sums.z : sums.x);
-              hi -= z * static_cast<int>(j & 1 ? sums.w : sums.y);
+          for (int d = 0; d < 3; ++d) {
+            const uint4 v = xv[d][j >> 1];
+            const uint32_t b0 = j & 1 ? v.z : v.x, b1 = j & 1 ? v.w : v.y;
+            if (j == p * 4 / P) {
+              if (d == 2)
+                mma_i8<true, true>(c[r][d], f[r][j], b0, b1);
+              else
+                mma_i8<false, true>(c[r][d], f[r][j], b0, b1);
+            } else {
+              if (d == 2)
+                mma_i8<true, false>(c[r][d], f[r][j], b0, b1);
+              else
+                mma_i8<false, false>(c[r][d], f[r][j], b0, b1);
             }
-            const float v = fmaf(static_cast<float>(hi), 65536.f, static_cast<float>(lo));
-            acc[r][i][j] = fmaf(v * (j < 2 ? s0 : s1), __uint_as_float(j & 1 ? pw.y : pw.x), acc[r][i][j]);
           }
+        }
+      }
+      uint4 sums;
+      if constexpr (ZERO) sums = lds128(sd + 32 + p * 64 + t * 8);
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        float s0, s1;
+        if (a.scale_half) {
+          const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&sc[r][p]));
+          s0 = h.x, s1 = h.y;
+        } else {
+          s0 = __uint_as_float(sc[r][p] << 16), s1 = __uint_as_float(sc[r][p] & 0xFFFF0000u);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // at most 2^22 (256 + 1) in the lower part, 2^20 in the upper: exact integers, one rounding to float32
+          // each and one where they meet
+          int lo = c[r][1][j] * 256 + c[r][0][j], hi = c[r][2][j];
+          if constexpr (ZERO) {
+            const int z = 16 * static_cast<int>(j < 2 ? zz[r][p] & 15u : zz[r][p] >> 4) - 128;  // 16 (z - 8)
+            lo -= z * static_cast<int>(j & 1 ? sums.z : sums.x);
+            hi -= z * static_cast<int>(j & 1 ? sums.w : sums.y);
+          }
+          const float v = fmaf(static_cast<float>(hi), 65536.f, static_cast<float>(lo));
+          acc[r][j] = fmaf(v * (j < 2 ? s0 : s1), __uint_as_float(j & 1 ? pw.y : pw.x), acc[r][j]);
         }
       }
     }
@@ -546,12 +530,9 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
       if (!head && k == ks) {
         emit(tile, acc);
       } else {
-        float4* dst = park + (warp * 2 + (head ? 0 : 1)) * (kR * NT * 32) + lane;
+        float4* dst = park + (warp * 2 + (head ? 0 : 1)) * (kR * 32) + lane;
 #pragma unroll
-        for (int r = 0; r < kR; ++r)
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-            dst[(r * NT + i) * 32] = make_float4(acc[r][i][0], acc[r][i][1], acc[r][i][2], acc[r][i][3]);
+        for (int r = 0; r < kR; ++r) dst[r * 32] = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
       }
       head = false;
       ++tile;
@@ -559,9 +540,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
 #pragma unroll
       for (int r = 0; r < kR; ++r)
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[r][i][j] = 0.f;
+        for (int j = 0; j < 4; ++j) acc[r][j] = 0.f;
     }
   }
   __syncthreads();
@@ -574,14 +553,12 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
         const int b = warp_start(w);
         if (b >= end) break;
         if (warp_start(w + 1) == b) continue;
-        const float4* part = park + (w * 2 + (w == warp ? 1 : 0)) * (kR * NT * 32) + lane;
+        const float4* part = park + (w * 2 + (w == warp ? 1 : 0)) * (kR * 32) + lane;
 #pragma unroll
-        for (int r = 0; r < kR; ++r)
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            const float4 v = part[(r * NT + i) * 32];
-            acc[r][i][0] += v.x, acc[r][i][1] += v.y, acc[r][i][2] += v.z, acc[r][i][3] += v.w;
-          }
+        for (int r = 0; r < kR; ++r) {
+          const float4 v = part[r * 32];
+          acc[r][0] += v.x, acc[r][1] += v.y, acc[r][2] += v.z, acc[r][3] += v.w;
+        }
       }
       emit(t0 + last, acc);
     }
@@ -593,11 +570,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
       const int n = i % (16 * kR), rest = i / (16 * kR), sl = rest / a.M, m = rest - sl * a.M;
       const int tl = t0 + sl * S + rank;
       if (tl >= t1) break;
-      // where the owning lane put it: lane 4 (n % 8) + m % 8 / 2, value 2 (n / 8) + m % 2
-      const int at = ((n >> 4) * NT + (m >> 3)) * 128 + ((n & 7) * 4 + (m & 7) / 2) * 4 + (n >> 3 & 1) * 2 + (m & 1);
-      const float* part = reinterpret_cast<const float*>(recv) + sl * S * (kR * NT * 128) + at;
+      // where the owning lane put it: lane 4 (n % 8) + m / 2, value 2 (n / 8) + m % 2
+      const int at = (n >> 4) * 128 + ((n & 7) * 4 + m / 2) * 4 + (n >> 3 & 1) * 2 + (m & 1);
+      const float* part = reinterpret_cast<const float*>(recv) + sl * S * (kR * 128) + at;
       float v = 0.f;
-      for (int r = 0; r < S; ++r) v += part[r * (kR * NT * 128)];
+      for (int r = 0; r < S; ++r) v += part[r * (kR * 128)];
       store_sum(a, static_cast<int64_t>(tl) * kR + (n >> 4), n & 15, m, v);
     }
   }
@@ -647,7 +624,7 @@ int resident_clusters(int S) {
 // about as much as kClusterCost KB. False: x does not fit shared memory.
 constexpr int kClusterCost = 30;
 template <typename L, auto kern, int W>
-bool vec_plan(int NT, const VecArgs& a, VecPlan& best) {
+bool vec_plan(const VecArgs& a, VecPlan& best) {
   int64_t best_cost = -1;
   for (int S = 1; S <= 8; S *= 2) {
     if (S > a.steps) break;
@@ -655,26 +632,26 @@ bool vec_plan(int NT, const VecArgs& a, VecPlan& best) {
     p.S = S;
     p.clusters = std::min(resident_clusters<kern, W>(S), a.tiles);
     const int per = (a.tiles + p.clusters - 1) / p.clusters, ks = (a.steps + S - 1) / S;
-    const int64_t x_bytes = static_cast<int64_t>(a.M) * vec_x_pitch(ks) + static_cast<int64_t>(ks) * L::kSide * NT;
+    const int64_t x_bytes = static_cast<int64_t>(a.M) * vec_x_pitch(ks) + static_cast<int64_t>(ks) * L::kSide;
     if (x_bytes > kMaxSmem) continue;
     p.x_bytes = static_cast<int>(x_bytes);
     p.recv_slots = S > 1 ? (per + S - 1) / S : 0;
     if (p.recv_slots > 4096) continue;
     p.smem = L::total(p.x_bytes, p.recv_slots, S);
     if (p.smem > kMaxSmem / (16 / W) || static_cast<int64_t>(per) * ks > (1 << 30) / a.steps) continue;  // n * ks stays below 2^31: the reciprocals are exact
-    const int64_t cost = static_cast<int64_t>(per) * ks * L::kR + (S > 1 ? kClusterCost : 0);
+    const int64_t cost = static_cast<int64_t>(per) * ks * kR + (S > 1 ? kClusterCost : 0);
     if (best_cost < 0 || cost < best_cost) best_cost = cost, best = p;
   }
   return best_cost >= 0;
 }
 
-template <int W, int NT, int G, bool ZERO>
+template <int W, int G, bool ZERO>
 bool launch_vec(VecArgs a, cudaStream_t s) {
-  constexpr auto kern = int4_vec_kernel<W, NT, G, ZERO>;
-  using L = VecSmem<W, NT, G, ZERO>;
-  a.tiles = (a.N + 16 * L::kR - 1) / (16 * L::kR);
+  constexpr auto kern = int4_vec_kernel<W, G, ZERO>;
+  using L = VecSmem<W, G, ZERO>;
+  a.tiles = (a.N + 16 * kR - 1) / (16 * kR);
   VecPlan p;
-  if (!vec_plan<L, kern, W>(NT, a, p)) return false;
+  if (!vec_plan<L, kern, W>(a, p)) return false;
   a.S = p.S;
   a.tiles_each = a.tiles / p.clusters, a.tiles_more = a.tiles % p.clusters;
   a.steps_each = a.steps / p.S, a.steps_more = a.steps % p.S;
@@ -706,13 +683,13 @@ bool launch_vec(VecArgs a, cudaStream_t s) {
   return true;
 }
 
-template <int W, int NT>
+template <int W>
 bool launch_vec_group(const VecArgs& a, int group, cudaStream_t s) {
   const bool z = a.zeros != nullptr;
   switch (group) {
-    case 32: return z ? launch_vec<W, NT, 32, true>(a, s) : launch_vec<W, NT, 32, false>(a, s);
-    case 64: return z ? launch_vec<W, NT, 64, true>(a, s) : launch_vec<W, NT, 64, false>(a, s);
-    default: return z ? launch_vec<W, NT, 128, true>(a, s) : launch_vec<W, NT, 128, false>(a, s);
+    case 32: return z ? launch_vec<W, 32, true>(a, s) : launch_vec<W, 32, false>(a, s);
+    case 64: return z ? launch_vec<W, 64, true>(a, s) : launch_vec<W, 64, false>(a, s);
+    default: return z ? launch_vec<W, 128, true>(a, s) : launch_vec<W, 128, false>(a, s);
   }
 }
 
@@ -722,7 +699,7 @@ void launch_int4_linear(const Int4LinearArgs& r, cudaStream_t s) {
   if (r.M <= 0) return;
   if (r.M > 65535 * 32 || r.N > (1ll << 30) || r.K > (1ll << 30))
     throw std::runtime_error("minisgl.int4_linear: size out of range");
-  if (r.M <= 16) {
+  if (r.M <= kFew) {
     VecArgs v{};
     v.x = r.x, v.x_scales = r.x_scales, v.packed = r.packed;
     v.scales = static_cast<const uint32_t*>(r.scales), v.zeros = r.zeros, v.bias = r.bias, v.out = r.out;
@@ -738,9 +715,7 @@ void launch_int4_linear(const Int4LinearArgs& r, cudaStream_t s) {
     // 7.6 us against 8.7, 2048 x 1024 4.1 against 5.1; 12301 x 4168 18.4 against 16.0, 5120 x 25600 30.2 against 19.0.
     constexpr int64_t kSmallSteps = 12 * 1024;
     const bool small = (static_cast<int64_t>(v.N) + 15) / 16 * v.steps <= kSmallSteps;
-    const bool done = v.M > 8 ? launch_vec_group<16, 2>(v, r.group, s)
-                              : (small && launch_vec_group<8, 1>(v, r.group, s)) || launch_vec_group<16, 1>(v, r.group, s);
-    if (done) return;
+    if ((small && launch_vec_group<8>(v, r.group, s)) || launch_vec_group<16>(v, r.group, s)) return;
   }
   launch_int4_gemm(r, s);
 }

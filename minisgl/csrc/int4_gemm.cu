@@ -51,18 +51,19 @@ constexpr int kCodes = 8 * 1024;  // 128 rows x 128 columns
 template <int BN>
 struct GSmem {
   static constexpr int kX = BN * 256;  // one step of x, as two 64-column tiles
-  static constexpr int kXs = BN == 192 ? 4 : BN == 128 ? 5 : 6;
-  static constexpr int kPs = BN == 192 ? 3 : 6;
+  static constexpr int kXs = BN == 256 || BN == 128 ? 3 : BN == 192 ? 4 : 6;
+  static constexpr int kPs = BN >= 192 ? 3 : 6;
   static constexpr int kAs = BN == 192 ? 2 : BN == 32 ? 3 : 4;  // steps of weights in tensor memory
+  static constexpr int kAcc = BN == 256 ? 1 : 2;  // sums in tensor memory; 256 columns leave room for one (one tile a CTA)
   static constexpr int kPt = kXs * kX;
   static constexpr int kSt = kPt + kPs * kCodes;   // the steps' scales, 1 KB apart
   static constexpr int kZt = kSt + kPs * 1024;     // and zero points, 256 bytes apart
   static constexpr int kOut = kZt + kPs * 256;    static constexpr int kRing = kOut + 4 * 1024;  // the epilogue's 1 KB a warp
   static constexpr int kBars = 8 * (2 * kXs + 2 * kPs + 2 * kAs + 4) + 16;
   static constexpr int bytes(int S) { return 1024 + kRing + (kBars + 127) / 128 * 128 + (S > 1 ? kRows * BN * 4 : 0); }
-  static_assert(bytes(BN <= 64 ? 2 : 1) <= 227 * 1024, "shared memory");
+  static_assert(bytes(BN <= 128 ? 2 : 1) <= 227 * 1024, "shared memory");
   static constexpr uint32_t kCols = BN == 32 ? 256 : 512;
-  static_assert(2 * BN + kAs * kACols <= kCols, "tensor memory");
+  static_assert(kAcc * BN + kAs * kACols <= kCols, "tensor memory");
 };
 
 struct GArgs {
@@ -261,8 +262,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int it = 0, lt = 0;
     bool ok = true;
     for (int tile = first; ok && tile < num_tiles; tile += stride, ++lt) {
-      const int acc = lt & 1;
-      if (lt >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], ((lt >> 1) - 1) & 1, a.err, 423));
+      const int acc = lt % L::kAcc;
+      if (lt >= L::kAcc) ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], (lt / L::kAcc - 1) & 1, a.err, 423));
       if (!ok) break;
       tc_fence_after();
       for (int k = k0; k < k1 && ok; ++k, ++it) {
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                          mbar_wait(&xfull[xs], (it / L::kXs) & 1, a.err, 424));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t d = tmem + acc * BN, wa = tmem + 2 * BN + as * kACols;
+        const uint32_t d = tmem + acc * BN, wa = tmem + L::kAcc * BN + as * kACols;
         const uint64_t xd = x_desc + static_cast<uint32_t>(xs * L::kX >> 4);
         if (elect_one()) {
 #pragma unroll
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ----------------------------------------------------- converters ----
     // warp q + 4 h of a set: rows 32 q .. 32 q + 31 (the tensor-memory lanes it reaches), columns 64 h .. of a step
     const int set = (warp - 8) / 8, quad = warp & 3, half = (warp >> 2) & 1, g = lane >> 2;
-    const uint32_t a_base = tmem + 2 * BN + half * (kACols / 2) + (static_cast<uint32_t>(32 * quad) << 16);
+    const uint32_t a_base = tmem + L::kAcc * BN + half * (kACols / 2) + (static_cast<uint32_t>(32 * quad) << 16);
     constexpr int H = P == 4 ? 2 : 1;  // groups of 64 columns
     int it = 0;
     bool ok = true;
@@ -382,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int lt = 0;
     bool ok = true;
     for (int tile = first; tile < num_tiles; tile += stride, ++lt) {
-      const int acc = lt & 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (lt >> 1) & 1, a.err, 428));
+      const int acc = lt % L::kAcc;
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (lt / L::kAcc) & 1, a.err, 428));
       if (!ok) break;
       tc_fence_after();
       const int m0 = tile % a.m_tiles * BN;
@@ -510,10 +511,6 @@ __global__ void __launch_bounds__(256) mx8_rows_bf16_kernel(uint4* out, const ui
   }
 }
 
-struct GPlan {
-  int S, grid;
-};
-
 template <auto kern>
 int resident(int S, int smem) {
   constexpr int kDevices = 64;
@@ -545,19 +542,42 @@ int resident(int S, int smem) {
   return n;
 }
 
+struct GPlan {
+  int bn, S, grid;
+  int64_t cost;
+};
+
+// The rows of x per tile and the CTAs per tile with the least estimated cycles in the busiest CTA. A step costs what
+// its slowest part does: x from L2 (256 BN bytes at about 55 a cycle and SM) or the unpacking of 128 x 128 codes
+// (730 cycles); a tile about kTile more (start, end of its sums), a cluster's exchange kExchange. Measured on a B200
+// (us): 512 x 8192 x 7168 in tiles of 256 56, of 192 75; 2000 x 8192 x 7168 of 192 196, of 256 (with the end of
+// each tile's sums exposed) 287.
+constexpr int64_t kUnpack = 730, kTile = 3000, kExchange = 2500;
 template <int BN, int G, bool HALF>
-void launch_bn(GArgs a, const CUtensorMap* tw, const CUtensorMap& tm, cudaStream_t s) {
+void plan_bn(const GArgs& a, GPlan& best) {
+  constexpr auto kern = int4_gemm_kernel<BN, G, HALF>;
+  using L = GSmem<BN>;
+  const int64_t tiles = static_cast<int64_t>((a.M + BN - 1) / BN) * a.n_tiles;
+  const int64_t step = std::max<int64_t>(BN * 256 / 55, kUnpack);
+  for (int S = 1; S <= 8 && S <= a.steps; S *= 2) {
+    if (S > 1 && BN > 128) break;  // no room for the partial sums
+    const int fit = resident<kern>(S, L::bytes(S));
+    if (S > 1 && tiles > fit) break;  // a cluster has one tile
+    const int64_t waves = (tiles + fit - 1) / fit;
+    if (BN == 256 && waves > 1) break;
+    const int64_t cost = waves * ((a.steps + S - 1) / S * step + kTile) + (S > 1 ? kExchange : 0);
+    if (best.cost < 0 || cost < best.cost)
+      best = GPlan{BN, S, static_cast<int>(S > 1 ? tiles * S : std::min<int64_t>(tiles, fit)), cost};
+  }
+}
+
+template <int BN, int G, bool HALF>
+void launch_bn(GArgs a, const GPlan& p, const CUtensorMap* tw, const CUtensorMap& tm, cudaStream_t s) {
   constexpr auto kern = int4_gemm_kernel<BN, G, HALF>;
   using L = GSmem<BN>;
   a.m_tiles = (a.M + BN - 1) / BN;
-  const int64_t tiles = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
-  a.S = 1;
-  int grid = static_cast<int>(std::min<int64_t>(tiles, resident<kern>(1, L::bytes(1))));
-  if constexpr (BN <= 64) {
-    // columns shared by as many CTAs as leave every cluster resident and each CTA at least two steps
-    for (int S = 2; S <= 8; S *= 2)
-      if (a.steps >= 2 * S && tiles <= resident<kern>(S, L::bytes(S))) a.S = S, grid = static_cast<int>(tiles) * S;
-  }
+  a.S = p.S;
+  const int grid = p.grid;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kThreads);
@@ -581,28 +601,16 @@ void launch_bn(GArgs a, const CUtensorMap* tw, const CUtensorMap& tm, cudaStream
   if (e != cudaSuccess) throw std::runtime_error(std::string("minisgl: kernel launch failed: ") + cudaGetErrorString(e));
 }
 
-template <int BN, bool HALF>
-void launch_group(const GArgs& a, const CUtensorMap* tw, const CUtensorMap& tm, int group, cudaStream_t s) {
-  switch (group) {
-    case 32: launch_bn<BN, 32, HALF>(a, tw, tm, s); break;
-    case 64: launch_bn<BN, 64, HALF>(a, tw, tm, s); break;
-    default: launch_bn<BN, 128, HALF>(a, tw, tm, s); break;
-  }
-}
-
-template <bool HALF>
-void launch_type(GArgs a, const void* scales, const void* x, int64_t ldx, int64_t K, int group, cudaStream_t s) {
-  // rows of x per tile: the size with the least time in the busiest CTA, per 64 columns 2 cycles per row of x in
-  // the tensor cores against about kConvert to unpack 128 weight rows
-  constexpr int kConvert = 400;
-  const int sms = 148;
-  int best = 192;
-  int64_t best_cost = -1;
-  for (int bn : {192, 128, 64, 32}) {
-    const int64_t tiles = (static_cast<int64_t>(a.M) + bn - 1) / bn * a.n_tiles;
-    const int64_t cost = (tiles + sms - 1) / sms * std::max(2 * bn, kConvert);
-    if (best_cost < 0 || cost < best_cost || (cost == best_cost && bn >= a.M)) best = bn, best_cost = cost;
-  }
+template <int G, bool HALF>
+void launch_type(GArgs a, const void* scales, const void* x, int64_t ldx, int64_t K, cudaStream_t s) {
+  constexpr int group = G;
+  GPlan p{0, 1, 0, -1};
+  plan_bn<32, G, HALF>(a, p);
+  plan_bn<64, G, HALF>(a, p);
+  plan_bn<128, G, HALF>(a, p);
+  plan_bn<192, G, HALF>(a, p);
+  plan_bn<256, G, HALF>(a, p);
+  const int best = p.bn;
   a.x_blocks = K % 64 == 0;
   const CUtensorMap tm = a.x_blocks ? make_tmap_bf16_kblocks(x, a.M, K, ldx, best, 2) : make_tmap_bf16_2d_sw128(x, a.M, K, ldx, best);
   // codes, scales, zero points: a row of a map is a tile of 16 rows, its columns the tile's 128-column units
@@ -619,10 +627,20 @@ void launch_type(GArgs a, const void* scales, const void* x, int64_t ldx, int64_
   tw[2] = a.zeros == nullptr ? tw[1]
                              : words(a.zeros, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (steps * per + 1) / 2 * 16, std::max(16u, pairs));
   switch (best) {
-    case 32: launch_group<32, HALF>(a, tw, tm, group, s); break;
-    case 64: launch_group<64, HALF>(a, tw, tm, group, s); break;
-    case 128: launch_group<128, HALF>(a, tw, tm, group, s); break;
-    default: launch_group<192, HALF>(a, tw, tm, group, s); break;
+    case 32: launch_bn<32, G, HALF>(a, p, tw, tm, s); break;
+    case 64: launch_bn<64, G, HALF>(a, p, tw, tm, s); break;
+    case 128: launch_bn<128, G, HALF>(a, p, tw, tm, s); break;
+    case 192: launch_bn<192, G, HALF>(a, p, tw, tm, s); break;
+    default: launch_bn<256, G, HALF>(a, p, tw, tm, s); break;
+  }
+}
+
+template <bool HALF>
+void launch_group(const GArgs& a, const void* scales, const void* x, int64_t ldx, int64_t K, int group, cudaStream_t s) {
+  switch (group) {
+    case 32: launch_type<32, HALF>(a, scales, x, ldx, K, s); break;
+    case 64: launch_type<64, HALF>(a, scales, x, ldx, K, s); break;
+    default: launch_type<128, HALF>(a, scales, x, ldx, K, s); break;
   }
 }
 
@@ -652,9 +670,9 @@ void launch_int4_gemm(const Int4LinearArgs& r, cudaStream_t s) {
     ldx = r.K;
   }
   if (r.x_scales == nullptr && r.x_type == DType::kF16)
-    launch_type<true>(a, r.scales, x, ldx, r.K, r.group, s);
+    launch_group<true>(a, r.scales, x, ldx, r.K, r.group, s);
   else
-    launch_type<false>(a, r.scales, x, ldx, r.K, r.group, s);
+    launch_group<false>(a, r.scales, x, ldx, r.K, r.group, s);
 }
 
 }  // namespace minisgl

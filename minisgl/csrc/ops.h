@@ -455,7 +455,7 @@ struct Int4LinearArgs {
   const uint8_t* zeros;     // [tiles, groups rounded up to even, 8] or nullptr (8 everywhere)
   const float* row_pow;     // [16 tiles]: a power of two near each row's largest scale
   const void* bias;         // [N] or nullptr
-  void* x_wide;             // E4M3 rows of more than int4_few_rows(): bf16 [M, K] scratch
+  void* x_wide;             // more than 8 E4M3 rows: bf16 [M, K] scratch
   void* out;                // [M, N], row stride ldo
   int64_t M, N, K;
   int64_t ldx, ld_xs, ldo;

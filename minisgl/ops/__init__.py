@@ -371,7 +371,7 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
     bits with ``x_scales`` [M, K / 32], as ``rmsnorm_mx8`` and
     ``silu_and_mul_mx8`` return them. out: bf16, fp16 or fp32 (default: x's
     type, bf16 for MXFP8 rows). Sums are held in fp32 or
-    exact integers, whatever the number of rows; products of more than 16 rows
+    exact integers, whatever the number of rows; products of more than 8 rows
     take the weight rounded once to x's 16-bit type."""
     if x.dim() != 2 or x.shape[1] != w.k:
         raise ValueError(f"int4_linear: x must be [M, {w.k}], got {tuple(x.shape)}")
@@ -389,7 +389,7 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
         return y
     if out is None:
         out = torch.empty((x.shape[0], w.n), dtype=out_dtype, device=x.device)
-    wide = x_scales is not None and x.shape[0] > 16  # MXFP8 rows widened to bf16 for the tensor cores' tiles
+    wide = x_scales is not None and x.shape[0] > 8  # MXFP8 rows widened to bf16 for the tensor cores' tiles
     x_wide = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) if wide else None
     _count(2 if wide else 1)
     native().int4_linear(out, x, x_scales, w.packed, w.scales, w.zeros, w.row_pow, bias, w.n, w.k, w.group, x_wide,

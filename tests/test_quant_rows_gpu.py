@@ -183,7 +183,7 @@ def _weight(n, k, group, zeros, seed, dtype):
 def _check_linear(y, xd, w, bias, rounded=False):
     """Against float64. Every product code * x is exact; at most (16 + 1) * 4 roundings inside a block of 64
     columns, one per block and some twenty where partial sums meet (2^-23 each: a tensor core may truncate),
-    then the output's half step. ``rounded``: more than 16 rows, whose product takes weights that are rounded once to
+    then the output's half step. ``rounded``: more than 8 rows, whose product takes weights that are rounded once to
     x's 16-bit type (half a step: 2^-8 of each for bf16, less for fp16)."""
     wd = dequantize_int4(w, torch.float64)
     want = xd @ wd.t()
@@ -214,8 +214,8 @@ def test_int4_linear(m, n, k, group, dt, zeros, bias):
     b = torch.randn(n, generator=g, device=DEV).to(t) if bias else None
     y = ops.int4_linear(x, w, b)
     assert y.dtype == t and y.shape == (m, n)
-    _check_linear(y, x.double(), w, b, rounded=m > 16)
-    _check_linear(ops.int4_linear(x, w, b, out_dtype=torch.float32), x.double(), w, b, rounded=m > 16)
+    _check_linear(y, x.double(), w, b, rounded=m > 8)
+    _check_linear(ops.int4_linear(x, w, b, out_dtype=torch.float32), x.double(), w, b, rounded=m > 8)
     ops.check_device_errors(torch.device(DEV))
 
 
@@ -229,8 +229,8 @@ def test_int4_linear_mx8_rows(m, n, k, group):
         x[1] = 0
     q, sf = ops.rmsnorm_mx8(x, None, 0.0 if m == 1 else 1e-6)
     xd = dequantize_mx8_rows(q, sf, torch.float64)
-    _check_linear(ops.int4_linear(q, w, x_scales=sf), xd, w, None, rounded=m > 16)
-    _check_linear(ops.int4_linear(q, w, x_scales=sf, out_dtype=torch.float32), xd, w, None, rounded=m > 16)
+    _check_linear(ops.int4_linear(q, w, x_scales=sf), xd, w, None, rounded=m > 8)
+    _check_linear(ops.int4_linear(q, w, x_scales=sf, out_dtype=torch.float32), xd, w, None, rounded=m > 8)
     ops.check_device_errors(torch.device(DEV))
 
 
@@ -244,12 +244,12 @@ def test_int4_linear_mixed_types_strides_and_out():
         wide = torch.full((m + 2, 264), 7.0, device=DEV, dtype=torch.float16)
         out = wide[1:m + 1, 8:208]
         assert ops.int4_linear(x, w, bias, out=out) is out
-        _check_linear(out, x.double(), w, bias, rounded=m > 16)
+        _check_linear(out, x.double(), w, bias, rounded=m > 8)
         keep = torch.ones_like(wide, dtype=torch.bool)
         keep[1:m + 1, 8:208] = False
         assert bool((wide[keep] == 7.0).all())
         odd = torch.full((m + 2, 203), 7.0, device=DEV, dtype=torch.bfloat16)[1:m + 1, 1:201]
-        _check_linear(ops.int4_linear(x, w, bias, out=odd), x.double(), w, bias, rounded=m > 16)
+        _check_linear(ops.int4_linear(x, w, bias, out=odd), x.double(), w, bias, rounded=m > 8)
         xs = torch.randn(256, generator=g, device=DEV).to(torch.bfloat16).expand(m, 256)
         with pytest.raises(RuntimeError):
             ops.int4_linear(xs, w)  # rows that lie on one another
@@ -291,9 +291,9 @@ def test_quantised_mlp(T):
     want_res = torch.empty_like(res)
     _same_rows((q, sf), ref.rmsnorm_mx8(x, w, 1e-6, start, want_res))
     assert torch.equal(res, want_res)
-    _check_linear(gu, dequantize_mx8_rows(q, sf, torch.float64), up, None, rounded=T > 16)
+    _check_linear(gu, dequantize_mx8_rows(q, sf, torch.float64), up, None, rounded=T > 8)
     _same_rows((a, asf), ref.act_mx8(gu, "silu", False))
-    _check_linear(y, dequantize_mx8_rows(a, asf, torch.float64), down, None, rounded=T > 16)
+    _check_linear(y, dequantize_mx8_rows(a, asf, torch.float64), down, None, rounded=T > 8)
 
 
 @pytest.mark.parametrize("T", [2, 40])
