@@ -52,7 +52,7 @@ __device__ __forceinline__ float e8m0(uint32_t byte) {
 // Few rows (up to 8, one operand of a warp-level product): the weight stream.
 //
 // A unit is kR tiles of 16 rows x 128 columns (kR KB of codes and their scales).
-// Whole tiles are dealt to clusters of S = 1, 2, 4 or 8 CTAs, whose CTAs share
+// Whole tiles are dealt to clusters of S = 1 to 8 CTAs, whose CTAs share
 // the columns; the units of a CTA, tile after tile, are cut into one contiguous
 // range per warp. Each warp copies its own units into its own ring of shared
 // memory (cp.async, kDepth ahead), waits for them alone and multiplies them;
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   // can be, the first ones taking one more
   const int S = a.S;
   int rank = 0, cluster = blockIdx.x;
-  if (S > 1) rank = blockIdx.x & (S - 1), cluster = blockIdx.x / S;
+  if (S > 1) cluster = blockIdx.x / S, rank = blockIdx.x - cluster * S;
   const int t0 = cluster * a.tiles_each + min(cluster, a.tiles_more);
   const int t1 = t0 + a.tiles_each + (cluster < a.tiles_more ? 1 : 0);
   const int k0 = rank * a.steps_each + min(rank, a.steps_more);
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
           store_sum(a, static_cast<int64_t>(tile) * kR + r, g + (j >> 1) * 8, 2 * t + (j & 1), acc[r][j]);
     } else {
       const int local = tile - t0;
-      const uint32_t base = map_shared_rank(smem_u32(recv + (local / S * S + rank) * (kR * 32) + lane), local & (S - 1));
+      const uint32_t base = map_shared_rank(smem_u32(recv + (local / S * S + rank) * (kR * 32) + lane), local % S);
 #pragma unroll
       for (int r = 0; r < kR; ++r)
         asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(base + r * 512), "f"(acc[r][0]),
@@ -588,10 +588,10 @@ struct VecPlan {
 template <auto kern, int W>
 int resident_clusters(int S) {
   constexpr int kDevices = 64;
-  static std::atomic<int> known[kDevices][4];
+  static std::atomic<int> known[kDevices][8];
   int dev = 0;
   cudaGetDevice(&dev);
-  const int at = S == 1 ? 0 : S == 2 ? 1 : S == 4 ? 2 : 3;
+  const int at = S - 1;
   int n = dev < kDevices ? known[dev][at].load() : 0;
   if (n > 0) return n;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
@@ -626,7 +626,7 @@ constexpr int kClusterCost = 30;
 template <typename L, auto kern, int W>
 bool vec_plan(const VecArgs& a, VecPlan& best) {
   int64_t best_cost = -1;
-  for (int S = 1; S <= 8; S *= 2) {
+  for (int S = 1; S <= 8; ++S) {
     if (S > a.steps) break;
     VecPlan p;
     p.S = S;

@@ -457,13 +457,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_dealloc(tmem, L::kCols);
   }
   if (S > 1) {
-    // one tile per cluster: this CTA adds BN / S of its rows of x, the S partial sums in rank order
+    // one tile per cluster: this CTA adds its share of the rows of x, the S partial sums in rank order
     __syncwarp();
     cluster_sync();
-    const int per = BN / S;
+    const int x0 = BN * rank / S, x1 = BN * (rank + 1) / S;
     const int64_t n0 = static_cast<int64_t>(first / a.m_tiles) * kRows;
-    for (int i = threadIdx.x; i < per * (kRows / 4); i += kThreads) {
-      const int at = rank * per + i / (kRows / 4), q = i % (kRows / 4) * 4;
+    for (int i = threadIdx.x; i < (x1 - x0) * (kRows / 4); i += kThreads) {
+      const int at = x0 + i / (kRows / 4), q = i % (kRows / 4) * 4;
       const int m = first % a.m_tiles * BN + at;
       if (m >= a.M) continue;
       const uint32_t local = smem_u32(part + at * kRows + q);
@@ -514,10 +514,10 @@ __global__ void __launch_bounds__(256) mx8_rows_bf16_kernel(uint4* out, const ui
 template <auto kern>
 int resident(int S, int smem) {
   constexpr int kDevices = 64;
-  static std::atomic<int> known[kDevices][4];
+  static std::atomic<int> known[kDevices][8];
   int dev = 0;
   cudaGetDevice(&dev);
-  const int at = S == 1 ? 0 : S == 2 ? 1 : S == 4 ? 2 : 3;
+  const int at = S - 1;
   int n = dev < kDevices ? known[dev][at].load() : 0;
   if (n > 0) return n;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
@@ -559,7 +559,7 @@ void plan_bn(const GArgs& a, GPlan& best) {
   using L = GSmem<BN>;
   const int64_t tiles = static_cast<int64_t>((a.M + BN - 1) / BN) * a.n_tiles;
   const int64_t step = std::max<int64_t>(BN * 256 / 55, kUnpack);
-  for (int S = 1; S <= 8 && S <= a.steps; S *= 2) {
+  for (int S = 1; S <= 8 && S <= a.steps; ++S) {
     if (S > 1 && BN > 128) break;  // no room for the partial sums
     const int fit = resident<kern>(S, L::bytes(S));
     if (S > 1 && tiles > fit) break;  // a cluster has one tile
