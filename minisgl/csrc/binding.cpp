@@ -481,7 +481,6 @@ void mx8_quantize(at::Tensor q, at::Tensor sf, const at::Tensor& x, const c10::o
 // ------------------------------------------------- rows with MXFP8 output ----
 void check_mx8_out(const at::Tensor& x, const at::Tensor& q, const at::Tensor& sf, int64_t rows, int64_t cols,
                    const char* what) {
-  MSG_CHECK(cols > 0 && cols % 32 == 0, what, ": the width must be a positive multiple of 32, got ", cols);
   check_same_device(x, q);
   check_same_device(x, sf);
   MSG_CHECK(q.scalar_type() == at::kByte && q.dim() == 2 && q.size(0) == rows && q.size(1) == cols &&
@@ -503,19 +502,32 @@ void check_vec_rows(const at::Tensor& t, int64_t rows, int64_t cols, at::ScalarT
             what, ": the rows of ", name, " must lie at multiples of 16 bytes");
 }
 
-void rmsnorm_mx8(at::Tensor q, at::Tensor sf, const at::Tensor& x, const c10::optional<at::Tensor>& w, double eps,
-                 const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& residual_out) {
+// The caller's (q, sf), or new ones: allocated here, which costs a call a third of what two allocations cost in Python.
+std::pair<at::Tensor, at::Tensor> mx8_out(const at::Tensor& x, int64_t rows, int64_t cols,
+                                          const c10::optional<std::pair<at::Tensor, at::Tensor>>& out, const char* what) {
+  MSG_CHECK(cols > 0 && cols % 32 == 0, what, ": the width must be a positive multiple of 32, got ", cols);
+  if (!out.has_value())
+    return {at::empty({rows, cols}, x.options().dtype(at::kByte)), at::empty({rows, cols / 32}, x.options().dtype(at::kByte))};
+  check_mx8_out(x, out->first, out->second, rows, cols, what);
+  return *out;
+}
+
+std::pair<at::Tensor, at::Tensor> rmsnorm_mx8(const at::Tensor& x, const c10::optional<at::Tensor>& w, double eps,
+                                              const c10::optional<at::Tensor>& residual,
+                                              const c10::optional<at::Tensor>& residual_out,
+                                              const c10::optional<std::pair<at::Tensor, at::Tensor>>& out) {
   check_cuda(x, "x");
   MSG_CHECK(x.dim() == 2, "rmsnorm_mx8: x must be 2-D");
   const int64_t rows = x.size(0), cols = x.size(1);
   minisgl::RmsnormMx8Args a{};
   a.dtype = dtype_of(x);
   check_vec_rows(x, rows, cols, x.scalar_type(), "rmsnorm_mx8", "x");
-  check_mx8_out(x, q, sf, rows, cols, "rmsnorm_mx8");
   MSG_CHECK(cols <= 4096 * (16 / x.element_size()), "rmsnorm_mx8: width ", cols, " is above the supported ",
             4096 * (16 / x.element_size()));
   MSG_CHECK(rows < (1ll << 31), "rmsnorm_mx8: too many rows");
   MSG_CHECK(eps >= 0.0, "rmsnorm_mx8: eps must not be negative");
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto [q, sf] = mx8_out(x, rows, cols, out, "rmsnorm_mx8");
   if (w.has_value()) {
     MSG_CHECK(w->is_cuda() && w->scalar_type() == x.scalar_type() && w->is_contiguous() && w->numel() == cols &&
                   reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0,
@@ -523,16 +535,17 @@ void rmsnorm_mx8(at::Tensor q, at::Tensor sf, const at::Tensor& x, const c10::op
     check_same_device(x, *w);
     a.w = w->data_ptr();
   }
-  MSG_CHECK(residual.has_value() == residual_out.has_value(), "rmsnorm_mx8: residual and residual_out go together");
   if (residual.has_value()) {
+    // without residual_out the sum goes back to residual
+    const at::Tensor& sum = residual_out.has_value() ? *residual_out : *residual;
     check_vec_rows(*residual, rows, cols, x.scalar_type(), "rmsnorm_mx8", "residual");
-    check_vec_rows(*residual_out, rows, cols, x.scalar_type(), "rmsnorm_mx8", "residual_out");
+    check_vec_rows(sum, rows, cols, x.scalar_type(), "rmsnorm_mx8", "residual_out");
     check_same_device(x, *residual);
-    check_same_device(x, *residual_out);
+    check_same_device(x, sum);
     a.residual = residual->data_ptr();
-    a.residual_out = residual_out->data_ptr();
+    a.residual_out = sum.data_ptr();
     a.ld_res = residual->stride(0);
-    a.ld_res_out = residual_out->stride(0);
+    a.ld_res_out = sum.stride(0);
   }
   a.x = x.data_ptr();
   a.q = q.data_ptr<uint8_t>();
@@ -543,20 +556,22 @@ void rmsnorm_mx8(at::Tensor q, at::Tensor sf, const at::Tensor& x, const c10::op
   a.ld_q = q.stride(0);
   a.ld_sf = sf.stride(0);
   a.eps = eps;
-  const c10::cuda::CUDAGuard guard(x.device());
   minisgl::launch_rmsnorm_mx8(a, stream_of(x));
+  return {q, sf};
 }
 
-void act_mx8(at::Tensor q, at::Tensor sf, const at::Tensor& x, int64_t act, bool interleaved) {
+std::pair<at::Tensor, at::Tensor> act_mx8(const at::Tensor& x, int64_t act, bool interleaved,
+                                          const c10::optional<std::pair<at::Tensor, at::Tensor>>& out) {
   check_cuda(x, "x");
   MSG_CHECK(x.dim() == 2 && x.size(1) % 2 == 0, "act_mx8: x must be [rows, 2 d]");
   const int64_t rows = x.size(0), d = x.size(1) / 2;
   minisgl::ActMx8Args a{};
   a.dtype = dtype_of(x);
   check_vec_rows(x, rows, 2 * d, x.scalar_type(), "act_mx8", "x");
-  check_mx8_out(x, q, sf, rows, d, "act_mx8");
   MSG_CHECK(!interleaved || d % 64 == 0, "act_mx8: the interleaved width must be a multiple of 64, got ", d);
   MSG_CHECK(d < (1ll << 30), "act_mx8: too wide");
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto [q, sf] = mx8_out(x, rows, d, out, "act_mx8");
   a.x = x.data_ptr();
   a.q = q.data_ptr<uint8_t>();
   a.sf = sf.data_ptr<uint8_t>();
@@ -567,21 +582,53 @@ void act_mx8(at::Tensor q, at::Tensor sf, const at::Tensor& x, int64_t act, bool
   a.ld_sf = sf.stride(0);
   a.act = static_cast<int>(act);
   a.interleaved = interleaved;
-  const c10::cuda::CUDAGuard guard(x.device());
   minisgl::launch_act_mx8(a, stream_of(x));
+  return {q, sf};
 }
 
 // ---------------------------------------------------------- 4-bit linear ----
-void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Tensor>& x_scales,
-                 const at::Tensor& packed, const at::Tensor& scales, const c10::optional<at::Tensor>& zeros,
-                 const at::Tensor& row_pow, const c10::optional<at::Tensor>& bias, int64_t N, int64_t K, int64_t group,
-                 const c10::optional<at::Tensor>& x_wide, const c10::optional<at::Tensor>& err) {
-  MSG_CHECK(group == 32 || group == 64 || group == 128, "int4_linear: group of 32, 64 or 128, got ", group);
+// A weight in the kernels' layout with the error word of its device: checked once, when it is made, and handed over
+// as one argument.
+struct Int4Handle {
+  at::Tensor packed, scales, row_pow, err;
+  c10::optional<at::Tensor> zeros;
+  int64_t N, K, group;
+
+  Int4Handle(at::Tensor packed_, at::Tensor scales_, c10::optional<at::Tensor> zeros_, at::Tensor row_pow_, int64_t n,
+             int64_t k, int64_t group_, at::Tensor err_)
+      : packed(std::move(packed_)), scales(std::move(scales_)), row_pow(std::move(row_pow_)), err(std::move(err_)),
+        zeros(std::move(zeros_)), N(n), K(k), group(group_) {
+    MSG_CHECK(group == 32 || group == 64 || group == 128, "int4 weight: group of 32, 64 or 128, got ", group);
+    MSG_CHECK(N > 0 && K > 0 && K % 8 == 0 && N <= (1ll << 30) && K <= (1ll << 30),
+              "int4 weight: N >= 1 and K a positive multiple of 8, got [", N, ", ", K, "]");
+    const int64_t tiles = 2 * ((N + 31) / 32), blocks = 2 * ((K + 127) / 128), groups = blocks * 64 / group;
+    auto check = [&](const at::Tensor& t, bool type, int64_t numel, const char* name) {
+      MSG_CHECK(t.is_cuda() && type && t.is_contiguous() && t.numel() == numel &&
+                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+                "int4 weight: ", name, " of the wrong type, size or alignment");
+      check_same_device(packed, t);
+    };
+    check(packed, packed.scalar_type() == at::kByte, tiles * blocks * 512, "codes");
+    check(scales, scales.scalar_type() == at::kBFloat16 || scales.scalar_type() == at::kHalf, tiles * groups * 16, "scales");
+    check(row_pow, row_pow.scalar_type() == at::kFloat, tiles * 16, "row powers");
+    if (zeros.has_value())
+      check(*zeros, zeros->scalar_type() == at::kByte, tiles * (groups + groups % 2) * 8, "zero points");
+    err_ptr(err);
+    check_same_device(packed, err);
+  }
+};
+
+at::Tensor int4_linear(const at::Tensor& x, const Int4Handle& w, const c10::optional<at::Tensor>& bias,
+                       const c10::optional<at::Tensor>& out_, const c10::optional<at::ScalarType>& out_dtype,
+                       const c10::optional<at::Tensor>& x_scales) {
+  const int64_t N = w.N, K = w.K;
   MSG_CHECK(x.dim() == 2 && x.size(1) == K, "int4_linear: x must be [M, ", K, "], got ", x.sizes());
   check_cuda(x, "x");
+  check_same_device(x, w.packed);
   const int64_t M = x.size(0);
-  MSG_CHECK(N > 0 && K > 0 && K % 8 == 0, "int4_linear: K must be a positive multiple of 8");
   minisgl::Int4LinearArgs a{};
+  at::Tensor x_wide;
+  const c10::cuda::CUDAGuard guard(x.device());
   if (x_scales.has_value()) {
     MSG_CHECK(x.scalar_type() == at::kByte && K % 32 == 0, "int4_linear: MXFP8 rows are uint8 with K % 32 == 0");
     MSG_CHECK(x_scales->is_cuda() && x_scales->scalar_type() == at::kByte && x_scales->dim() == 2 &&
@@ -591,41 +638,17 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
     a.x_scales = x_scales->data_ptr<uint8_t>();
     a.ld_xs = x_scales->stride(0);
     a.x_type = DType::kBF16;
+    if (M > minisgl::kInt4FewRows) {  // MXFP8 rows widened to bf16 for the tensor cores' tiles
+      x_wide = at::empty({M, K}, x.options().dtype(at::kBFloat16));
+      a.x_wide = x_wide.data_ptr();
+    }
   } else {
     MSG_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
               "int4_linear: x must be bfloat16 or float16 (or MXFP8 rows with x_scales)");
     a.x_type = dtype_of(x);
   }
   check_vec_rows(x, M, K, x.scalar_type(), "int4_linear", "x");
-  const int64_t tiles = 2 * ((N + 31) / 32), blocks = 2 * ((K + 127) / 128), groups = blocks * 64 / group;
-  MSG_CHECK(packed.is_cuda() && packed.scalar_type() == at::kByte && packed.is_contiguous() &&
-                packed.numel() == tiles * blocks * 512 && reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16 == 0,
-            "int4_linear: packed weight of the wrong type or size");
-  MSG_CHECK(scales.is_cuda() && (scales.scalar_type() == at::kBFloat16 || scales.scalar_type() == at::kHalf) &&
-                scales.is_contiguous() && scales.numel() == tiles * groups * 16 &&
-                reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
-            "int4_linear: weight scales of the wrong type or size");
-  check_same_device(x, packed);
-  check_same_device(x, scales);
-  MSG_CHECK(row_pow.is_cuda() && row_pow.scalar_type() == at::kFloat && row_pow.is_contiguous() &&
-                row_pow.numel() == tiles * 16,
-            "int4_linear: row powers of the wrong type or size");
-  check_same_device(x, row_pow);
-  if (x_scales.has_value() && M > 8) {
-    MSG_CHECK(x_wide.has_value() && x_wide->is_cuda() && x_wide->scalar_type() == at::kBFloat16 &&
-                  x_wide->is_contiguous() && x_wide->numel() >= M * K &&
-                  reinterpret_cast<uintptr_t>(x_wide->data_ptr()) % 16 == 0,
-              "int4_linear: bf16 scratch of M * K for more than 8 MXFP8 rows");
-    check_same_device(x, *x_wide);
-    a.x_wide = x_wide->data_ptr();
-  }
-  if (zeros.has_value()) {
-    MSG_CHECK(zeros->is_cuda() && zeros->scalar_type() == at::kByte && zeros->is_contiguous() &&
-                  zeros->numel() == tiles * (groups + groups % 2) * 8 && reinterpret_cast<uintptr_t>(zeros->data_ptr()) % 16 == 0,
-              "int4_linear: weight zero points of the wrong type or size");
-    check_same_device(x, *zeros);
-    a.zeros = zeros->data_ptr<uint8_t>();
-  }
+  if (w.zeros.has_value()) a.zeros = w.zeros->data_ptr<uint8_t>();
   if (bias.has_value()) {
     MSG_CHECK(bias->is_cuda() && bias->is_contiguous() && bias->numel() == N,
               "int4_linear: bias must be a contiguous vector of ", N, " elements");
@@ -633,27 +656,34 @@ void int4_linear(at::Tensor out, const at::Tensor& x, const c10::optional<at::Te
     a.bias = bias->data_ptr();
     a.bias_type = dtype_of(*bias);
   }
-  check_cuda(out, "out");
-  check_same_device(x, out);
-  MSG_CHECK(out.dim() == 2 && out.size(0) == M && out.size(1) == N && out.stride(1) == 1 &&
-                (M <= 1 || out.stride(0) >= N),
-            "int4_linear: out must be [", M, ", ", N, "] with unit column stride");
+  at::Tensor out;
+  if (out_.has_value()) {
+    out = *out_;
+    check_cuda(out, "out");
+    check_same_device(x, out);
+    MSG_CHECK(out.dim() == 2 && out.size(0) == M && out.size(1) == N && out.stride(1) == 1 &&
+                  (M <= 1 || out.stride(0) >= N) && (!out_dtype.has_value() || out.scalar_type() == *out_dtype),
+              "int4_linear: out must be [", M, ", ", N, "] of out_dtype with unit column stride");
+  } else {
+    const at::ScalarType dt = out_dtype.has_value() ? *out_dtype : x_scales.has_value() ? at::kBFloat16 : x.scalar_type();
+    out = at::empty({M, N}, x.options().dtype(dt));
+  }
   a.x = x.data_ptr();
-  a.packed = packed.data_ptr<uint8_t>();
-  a.scales = scales.data_ptr();
-  a.row_pow = row_pow.data_ptr<float>();
+  a.packed = w.packed.data_ptr<uint8_t>();
+  a.scales = w.scales.data_ptr();
+  a.row_pow = w.row_pow.data_ptr<float>();
   a.out = out.data_ptr();
   a.M = M;
   a.N = N;
   a.K = K;
   a.ldx = x.stride(0);
   a.ldo = out.stride(0);
-  a.group = static_cast<int>(group);
-  a.scale_type = dtype_of(scales);
+  a.group = static_cast<int>(w.group);
+  a.scale_type = dtype_of(w.scales);
   a.out_type = dtype_of(out);
-  a.err = err_ptr(err);
-  const c10::cuda::CUDAGuard guard(x.device());
+  a.err = err_ptr(w.err);
   minisgl::launch_int4_linear(a, stream_of(x));
+  return out;
 }
 
 // Block-scaled MX routed experts: align -> gather + MXFP8 quantise -> gate_up
@@ -1692,6 +1722,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("rows"), py::arg("tile"));
   m.def("rmsnorm_mx8", &rmsnorm_mx8);
   m.def("act_mx8", &act_mx8);
+  py::class_<Int4Handle>(m, "Int4Handle")
+      .def(py::init<at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, int64_t, int64_t, int64_t, at::Tensor>());
   m.def("int4_linear", &int4_linear);
   m.def("moe_experts_mx", &moe_experts_mx, py::arg("out"), py::arg("x"), py::arg("w1q"), py::arg("w1sb"),
         py::arg("w2q"), py::arg("w2sb"), py::arg("topk_w"), py::arg("topk_ids"), py::arg("tile"), py::arg("xq"),

@@ -74,7 +74,6 @@ __device__ __forceinline__ float e8m0(uint32_t byte) {
 // are added in rank order after a cluster barrier. Every sum has a fixed order:
 // the same inputs give the same bits.
 // ---------------------------------------------------------------------------
-constexpr int kFew = 8;  // rows of x
 constexpr int kDepth = 3;
 constexpr int kR = 2;    // 16-row tiles of a unit: their products share the reads of x
 constexpr int kMaxSmem = 227 * 1024;
@@ -699,7 +698,7 @@ void launch_int4_linear(const Int4LinearArgs& r, cudaStream_t s) {
   if (r.M <= 0) return;
   if (r.M > 65535 * 32 || r.N > (1ll << 30) || r.K > (1ll << 30))
     throw std::runtime_error("minisgl.int4_linear: size out of range");
-  if (r.M <= kFew) {
+  if (r.M <= kInt4FewRows) {
     VecArgs v{};
     v.x = r.x, v.x_scales = r.x_scales, v.packed = r.packed;
     v.scales = static_cast<const uint32_t*>(r.scales), v.zeros = r.zeros, v.bias = r.bias, v.out = r.out;

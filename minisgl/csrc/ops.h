@@ -447,6 +447,7 @@ void launch_act_mx8(const ActMx8Args& a, cudaStream_t s);
 // ------------------------------------------------------- 4-bit linear ----
 // out[m, n] = sum_k x[m, k] (c[n, k] - z[n, k / group]) s[n, k / group] (+ bias[n])
 // with the weight in the tile layout of minisgl.quant.int4 (int4.cu).
+constexpr int kInt4FewRows = 8;  // up to here the weight is streamed past x (int4.cu), above it is tiled (int4_gemm.cu)
 struct Int4LinearArgs {
   const void* x;            // bf16 / fp16 [M, K] (row stride ldx), or E4M3 bytes
   const uint8_t* x_scales;  // E8M0 [M, K / 32] (row stride ld_xs) or nullptr
@@ -455,7 +456,7 @@ struct Int4LinearArgs {
   const uint8_t* zeros;     // [tiles, groups rounded up to even, 8] or nullptr (8 everywhere)
   const float* row_pow;     // [16 tiles]: a power of two near each row's largest scale
   const void* bias;         // [N] or nullptr
-  void* x_wide;             // more than 8 E4M3 rows: bf16 [M, K] scratch
+  void* x_wide;             // more than kInt4FewRows E4M3 rows: bf16 [M, K] scratch
   void* out;                // [M, N], row stride ldo
   int64_t M, N, K;
   int64_t ldx, ld_xs, ldo;

@@ -291,13 +291,6 @@ def _act_and_mul(x: torch.Tensor, act: str, out: Optional[torch.Tensor], interle
 
 
 # ------------------------------------------------- rows with MXFP8 output
-def _mx8_out(x: torch.Tensor, cols: int, out: Optional[Tuple[torch.Tensor, torch.Tensor]]):
-    if out is not None:
-        return out
-    rows = x.shape[0]
-    return x.new_empty((rows, cols), dtype=torch.uint8), x.new_empty((rows, cols // 32), dtype=torch.uint8)
-
-
 def _mx8_cpu(got: Tuple[torch.Tensor, torch.Tensor], out: Optional[Tuple[torch.Tensor, torch.Tensor]]):
     if out is None:
         return got
@@ -324,16 +317,12 @@ def rmsnorm_mx8(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, residual
     (fp32: 16384)."""
     if residual is None and residual_out is not None:
         raise ValueError("rmsnorm_mx8: residual_out needs residual")
-    if residual is not None and residual_out is None:
-        residual_out = residual
+    if x.is_cuda:
+        _count()
+        return native().rmsnorm_mx8(x, w, eps, residual, residual_out, out)
     if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % 32 != 0:
         raise ValueError(f"rmsnorm_mx8: x must be [rows, a positive multiple of 32], got {tuple(x.shape)}")
-    if not x.is_cuda:
-        return _mx8_cpu(ref.rmsnorm_mx8(x, w, eps, residual, residual_out), out)
-    q, sf = _mx8_out(x, x.shape[1], out)
-    _count()
-    native().rmsnorm_mx8(q, sf, x, w, eps, residual, residual_out)
-    return q, sf
+    return _mx8_cpu(ref.rmsnorm_mx8(x, w, eps, residual, residual if residual_out is None else residual_out), out)
 
 
 def silu_and_mul_mx8(x: torch.Tensor, interleaved: bool = False,
@@ -351,15 +340,13 @@ def gelu_and_mul_mx8(x: torch.Tensor,
 
 
 def _act_mx8(x: torch.Tensor, act: str, interleaved: bool, out):
+    if x.is_cuda:
+        _count()
+        return native().act_mx8(x, 0 if act == "silu" else 1, interleaved, out)
     unit = 128 if interleaved else 64
     if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % unit != 0:
         raise ValueError(f"{act}_and_mul_mx8: x must be [rows, a positive multiple of {unit}], got {tuple(x.shape)}")
-    if not x.is_cuda:
-        return _mx8_cpu(ref.act_mx8(x, act, interleaved), out)
-    q, sf = _mx8_out(x, x.shape[1] // 2, out)
-    _count()
-    native().act_mx8(q, sf, x, 0 if act == "silu" else 1, interleaved)
-    return q, sf
+    return _mx8_cpu(ref.act_mx8(x, act, interleaved), out)
 
 
 # ---------------------------------------------------------- 4-bit linear
@@ -373,6 +360,9 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
     type, bf16 for MXFP8 rows). Sums are held in fp32 or
     exact integers, whatever the number of rows; products of more than 8 rows
     take the weight rounded once to x's 16-bit type."""
+    if x.is_cuda:
+        _count(2 if x_scales is not None and x.shape[0] > 8 else 1)  # MXFP8 rows of a long batch are widened first
+        return native().int4_linear(x, w.native(), bias, out, out_dtype, x_scales)
     if x.dim() != 2 or x.shape[1] != w.k:
         raise ValueError(f"int4_linear: x must be [M, {w.k}], got {tuple(x.shape)}")
     if (x.dtype == torch.uint8) != (x_scales is not None):
@@ -381,20 +371,11 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
         out_dtype = out.dtype if out is not None else x.dtype if x_scales is None else torch.bfloat16
     elif out is not None and out.dtype != out_dtype:
         raise ValueError(f"int4_linear: out is {out.dtype}, out_dtype {out_dtype}")
-    if not x.is_cuda:
-        y = ref.int4_linear(x, w, bias, out_dtype, x_scales)
-        if out is not None:
-            out.copy_(y)
-            return out
-        return y
-    if out is None:
-        out = torch.empty((x.shape[0], w.n), dtype=out_dtype, device=x.device)
-    wide = x_scales is not None and x.shape[0] > 8  # MXFP8 rows widened to bf16 for the tensor cores' tiles
-    x_wide = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) if wide else None
-    _count(2 if wide else 1)
-    native().int4_linear(out, x, x_scales, w.packed, w.scales, w.zeros, w.row_pow, bias, w.n, w.k, w.group, x_wide,
-                         error_word(x.device))
-    return out
+    y = ref.int4_linear(x, w, bias, out_dtype, x_scales)
+    if out is not None:
+        out.copy_(y)
+        return out
+    return y
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, vocab_range: Optional[Tuple[int, int]] = None,

@@ -51,12 +51,31 @@ class Int4Weight:
     ``row_pow`` float32 [16 tiles]: the power of two at or below a row's largest scale
     (1 where that is 0), which fp16 products take out of the row."""
 
-    __slots__ = ("packed", "scales", "zeros", "row_pow", "n", "k", "group")
+    __slots__ = ("_packed", "_scales", "_zeros", "_row_pow", "_n", "_k", "_group", "_handle")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor],
                  row_pow: torch.Tensor, n: int, k: int, group: int) -> None:
-        self.packed, self.scales, self.zeros, self.row_pow = packed, scales, zeros, row_pow
-        self.n, self.k, self.group = n, k, group
+        self._packed, self._scales, self._zeros, self._row_pow = packed, scales, zeros, row_pow
+        self._n, self._k, self._group = n, k, group
+        self._handle = None
+
+    # the parts may be written into, not replaced: the native handle holds them
+    packed = property(lambda self: self._packed)
+    scales = property(lambda self: self._scales)
+    zeros = property(lambda self: self._zeros)
+    row_pow = property(lambda self: self._row_pow)
+    n = property(lambda self: self._n)
+    k = property(lambda self: self._k)
+    group = property(lambda self: self._group)
+
+    def native(self):
+        """The weight as one argument of the native calls (made on the first)."""
+        if self._handle is None:
+            from minisgl import ops
+
+            self._handle = ops.native().Int4Handle(self.packed, self.scales, self.zeros, self.row_pow, self.n, self.k,
+                                                   self.group, ops.error_word(self.device))
+        return self._handle
 
     @property
     def device(self) -> torch.device:

@@ -205,12 +205,19 @@ def test_refusals():
 
 
 def test_native_messages_with_numbers():
-    """A refusal whose message holds numbers and sizes raises (formatting them must not crash the process)."""
+    """A refusal whose message holds numbers raises (formatting them must not crash the process)."""
     if not ops.native_available():
         pytest.skip("native library not built")
-    x = torch.zeros(2, 64, dtype=torch.bfloat16)
-    u8 = torch.zeros(512, dtype=torch.uint8)
+    t = torch.zeros(512, dtype=torch.uint8)
     with pytest.raises(RuntimeError, match="group of 32, 64 or 128, got 48"):
-        ops.native().int4_linear(x, x, None, u8, x, None, x, None, 4, 64, 48, None, None)
-    with pytest.raises(RuntimeError, match=r"x must be \[M, 128\], got \[2, 64\]"):
-        ops.native().int4_linear(x, x, None, u8, x, None, x, None, 4, 128, 64, None, None)
+        ops.native().Int4Handle(t, t, None, t, 4, 64, 48, t)
+    with pytest.raises(RuntimeError, match=r"got \[4, 60\]"):
+        ops.native().Int4Handle(t, t, None, t, 4, 60, 64, t)
+    with pytest.raises(RuntimeError, match="codes of the wrong type, size or alignment"):
+        ops.native().Int4Handle(t, t, None, t, 4, 64, 64, t)  # on the CPU
+
+
+def test_weight_parts_are_not_replaced():
+    w = quantize_int4(torch.randn(32, 64), 64)
+    with pytest.raises(AttributeError):
+        w.packed = w.packed.clone()

@@ -373,6 +373,18 @@ def test_refusals_gpu():
         ops.int4_linear(x.float(), w)
     with pytest.raises(RuntimeError):
         ops.int4_linear(x, w.to("cpu"))
+    with pytest.raises(RuntimeError, match=r"x must be \[M, 64\], got \[2, 32\]"):
+        ops.int4_linear(x[:, :32], w)
+    with pytest.raises(RuntimeError):
+        ops.int4_linear(x, w, out=torch.zeros(2, 32, device=DEV), out_dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError):
+        ops.int4_linear(x.to(torch.uint8), w)
+    with pytest.raises(RuntimeError):
+        ops.int4_linear(x, w, x_scales=torch.zeros(2, 2, device=DEV, dtype=torch.uint8))
+    with pytest.raises(RuntimeError):
+        ops.rmsnorm_mx8(x[:, :48].contiguous(), None, 1e-6)
+    with pytest.raises(RuntimeError):
+        ops.silu_and_mul_mx8(x, interleaved=True)
     with pytest.raises(RuntimeError):
         ops.int4_linear(x, w, torch.zeros(31, device=DEV))
     with pytest.raises(RuntimeError):
