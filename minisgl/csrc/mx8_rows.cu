@@ -33,12 +33,15 @@ namespace {
 constexpr int kBlock = 32;  // columns under one scale
 
 template <typename T, int V>
-__device__ __forceinline__ void load_row_vec(const T* p, float (&v)[V]) {
+__device__ __forceinline__ void unpack_vec(const uint4& raw, float (&v)[V]) {
   static_assert(V * sizeof(T) == 16, "one 16-byte vector");
-  const uint4 raw = *reinterpret_cast<const uint4*>(p);
   const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = to_f32<T>(e[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void load_row_vec(const T* p, float (&v)[V]) {
+  unpack_vec<T, V>(*reinterpret_cast<const uint4*>(p), v);
 }
 
 // E4M3 bits of a double: truncated to float32 with a sticky last bit
@@ -52,54 +55,64 @@ __device__ __forceinline__ double pow2(int e) {  // 2^e, |e| <= 1000
   return __longlong_as_double(static_cast<long long>(1023 + e) << 52);
 }
 
+// max |.| of three with NaN above everything
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t e4m3x4(const float* t, float s) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[0] * s, t[1] * s), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[2] * s, t[3] * s), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
 // The V elements y of this lane, quantised. The 32 / V neighbouring lanes
 // that share a block call it together with the rest of their warp (`active`
-// may differ between blocks, not inside one). `window`: bound on y's error
-// in units of its last place; bit i of `doubt` marks an element whose error
-// may be larger. exact(i): element i in double, `zero` whether all of the
-// lane's inputs are zero (asked only where y is too small for float32).
+// may differ between blocks, not inside one). `slack`: bound on y's relative
+// error in units of 2^-24; bit i of `doubt` marks an element whose error may be
+// larger but not twofold (bit 16 + i: of any size). exact(i): element i in double; zero(): whether all of the lane's
+// inputs make zeros (asked only where y is too small for float32).
+//
+// Rounding is monotonic: where y (1 - slack) and y (1 + slack) round to the
+// same E4M3 value, so does the exact one.
 template <int V, typename Exact, typename Zero>
-__device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t window, uint32_t doubt, Exact exact,
-                                          Zero zero, uint8_t* q, uint8_t* sf, bool active) {
+__device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t slack, uint32_t doubt, Exact exact, Zero zero,
+                                          uint8_t* q, uint8_t* sf, bool active) {
   constexpr int G = kBlock / V;  // lanes of a block
   const int lane = threadIdx.x & 31;
-  uint32_t m = 0;  // max of the magnitudes' bits: NaN above infinity above every number
+  float top_f = max_abs3(y[0], y[1], y[2]);
 #pragma unroll
-  for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(y[i]) & 0x7FFFFFFFu);
+  for (int i = 3; i < V; i += 2) top_f = max_abs3(top_f, y[i], y[i + 1 < V ? i + 1 : i]);
+  uint32_t m = __float_as_uint(top_f);  // as bits: NaN above infinity above every number
 #pragma unroll
   for (int o = 1; o < G; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (!active) return;
-  // magnitudes far inside float32's range whose scale is in no doubt
+  // magnitudes far inside float32's range whose scale is in no doubt (a fraction has units of 2^-23)
   const uint32_t frac = m & 0x7FFFFFu;
-  const bool plain = m - (30u << 23) < (220u << 23) && frac + window - 0x600000u > 2 * window;
+  const bool plain = m - (64u << 23) < (186u << 23) && frac + slack - 0x600000u > 2 * slack;
   uint32_t words[V / 4];
   uint32_t sbyte;
   if (plain) {
     sbyte = ((m + 0x1FFFFFu) >> 23) - 8;  // exponent of m, one up where the fraction is above 448's 1.75
     const float inv = __uint_as_float((254u - sbyte) << 23);
-    uint32_t near = 0;
+    const float eps = static_cast<float>(slack + 1) * 5.9604645e-8f;  // one more: the products below are rounded
+    uint32_t apart[V / 4], any = doubt;
 #pragma unroll
     for (int w = 0; w < V / 4; ++w) {
-      uint32_t half[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float a = y[4 * w + 2 * h] * inv, b = y[4 * w + 2 * h + 1] * inv;
-        half[h] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          // below 2^-6 E4M3's steps are all 2^-9: adding 2^-6 puts the value on the grid of [2^-6, 2^-5)
-          float s = fabsf(k == 0 ? a : b);
-          // an element in doubt matters unless it is far below half of the smallest step
-          if (s > 0.00048828125f) near |= doubt & (1u << (4 * w + 2 * h + k));
-          if (s < 0.015625f) s += 0.015625f;
-          // 20 of the 23 fraction bits are rounded away; borders are at their middle
-          const uint32_t d = (__float_as_uint(s) - 0x80000u + window) & 0xFFFFFu;
-          if (d <= 2 * window) near |= 1u << (4 * w + 2 * h + k);
-        }
-      }
-      words[w] = half[0] | (half[1] << 16);
+      words[w] = e4m3x4(y + 4 * w, inv + inv * eps);
+      apart[w] = words[w] ^ e4m3x4(y + 4 * w, inv - inv * eps);
+      any |= apart[w];
     }
-    if (near != 0) {
+    if (any != 0) {
+      uint32_t near = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if ((apart[i >> 2] >> (8 * (i & 3)) & 0xFFu) != 0) near |= 1u << i;
+        // an element in doubt matters unless it is far below half of the smallest step
+        if (fabsf(y[i] * inv) > 0.00048828125f) near |= doubt & (1u << i);
+      }
+      near |= doubt >> 16;
       const double s = pow2(127 - static_cast<int>(sbyte));
 #pragma unroll 1
       for (int i = 0; i < V; ++i) {
@@ -171,7 +184,7 @@ struct NormArgs {
   uint8_t* sf;
   int cols;
   int64_t ld_x, ld_res, ld_res_out, ld_q, ld_sf;
-  double eps;
+  double eps, inv_cols;
 };
 
 // One CTA per row, the row kept in registers between the two passes.
@@ -223,7 +236,17 @@ __global__ void __launch_bounds__(1024) rmsnorm_mx8_kernel(const NormArgs a) {
   ss = lane < nw ? red[lane] : 0.0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const double inv_d = 1.0 / sqrt(ss / a.cols + a.eps);
+  // 1 / sqrt: two Newton steps in double on the float32 estimate leave some units of 2^-53
+  const double mean = ss * a.inv_cols + a.eps;
+  double inv_d;
+  if (mean > 1e-30 && mean < 1e30) {
+    inv_d = rsqrtf(static_cast<float>(mean));
+    const double half = 0.5 * mean;
+    inv_d = fma(inv_d, fma(-half * inv_d, inv_d, 0.5), inv_d);
+    inv_d = fma(inv_d, fma(-half * inv_d, inv_d, 0.5), inv_d);
+  } else {
+    inv_d = 1.0 / sqrt(mean);
+  }
   // a row whose factor is at the ends of float32's range is computed in double as a whole (NaN sends it there)
   const bool tame = inv_d > 1e-30 && inv_d < 1e30;
   const float inv = tame ? static_cast<float>(inv_d) : __uint_as_float(0x7FC00000u);
@@ -235,7 +258,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_mx8_kernel(const NormArgs a) {
     if (active) {
       float w[V];
       if (a.w != nullptr) load_row_vec<T, V>(static_cast<const T*>(a.w) + c, w);
-      // three roundings (inv and two products): at most 3 units of the last place
+      // three roundings (inv and two products): at most 3 * 2^-24
 #pragma unroll
       for (int i = 0; i < V; ++i) y[i] = a.w != nullptr ? v[k][i] * inv * w[i] : v[k][i] * inv;
     } else {
@@ -278,44 +301,61 @@ __device__ __noinline__ double act_exact(double g, double u) {
   return 0.5 * g * erfc(-g * 0.70710678118654752440) * u;
 }
 
+__device__ __forceinline__ float rcp_approx(float x) {  // 1 unit of the last place
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float ex2_approx(float x) {  // 2 units
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// A block takes 256 V outputs of a row at a time, and the loads of its next row are on their way while it works.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int V = 16 / sizeof(T);
-  const int nvec = a.d / V;
-  const int64_t total = a.rows * nvec;
-  const int lane = threadIdx.x & 31;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  // whole warps stay in the loop: total is a multiple of a block's lanes, so `active` is the same in a block
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31); base < total; base += step) {
-    const int64_t i = base + lane;
-    const bool active = i < total;
-    const int64_t r = active ? i / nvec : 0;
-    const int c = active ? static_cast<int>(i - r * nvec) * V : 0;
-    const T* row = static_cast<const T*>(a.x) + r * a.ld_x;
-    const T* gp = row + (a.interleaved ? (c / 64) * 128 + c % 64 : c);
-    const T* up = gp + (a.interleaved ? 64 : a.d);
+  const int c0 = (blockIdx.x * 256 + threadIdx.x) * V;
+  const bool active = c0 < a.d;  // the same for the lanes of a block: d is a multiple of 32
+  const int c = active ? c0 : 0;
+  const T* gp = static_cast<const T*>(a.x) + blockIdx.y * a.ld_x + (a.interleaved ? (c / 64) * 128 + c % 64 : c);
+  const int to_up = a.interleaved ? 64 : a.d;
+  const int64_t step = gridDim.y * a.ld_x;
+  uint4 next_g = *reinterpret_cast<const uint4*>(gp), next_u = *reinterpret_cast<const uint4*>(gp + to_up);
+  for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y, gp += step) {
     float g[V], u[V], y[V];
-    load_row_vec<T, V>(gp, g);
-    load_row_vec<T, V>(up, u);
-    uint32_t doubt = 0;
+    unpack_vec<T, V>(next_g, g);
+    unpack_vec<T, V>(next_u, u);
+    const T* up = gp + to_up;
+    if (r + gridDim.y < a.rows) {
+      next_g = *reinterpret_cast<const uint4*>(gp + step);
+      next_u = *reinterpret_cast<const uint4*>(up + step);
+    }
+    float low = g[0];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
+      low = fminf(low, g[k]);
       const float p = g[k] * u[k];  // exact for 16-bit types
-      if (ACT == 0) {
-        // 1 / (1 + e^-g): for g >= -16 the exponential's argument and its own error, the sum, the reciprocal
-        // and the products leave at most 26 * 2^-24; below it is in doubt
-        y[k] = __fdividef(p, 1.f + __expf(-g[k]));
-        if (g[k] < -16.f) doubt |= 1u << k;
-      } else {
-        // g / 2 * erfc(-g / sqrt 2): for g >= -6 the argument's rounding grows by at most 2 * (6 / sqrt 2)^2 = 36
+      if (ACT == 0)
+        // p / (1 + e^-g): for g >= -16 the exponential's argument (16 * 2^-24) and value, the sum, the reciprocal
+        // and the products leave at most 26 * 2^-24
+        y[k] = p * rcp_approx(1.f + ex2_approx(-1.44269504f * g[k]));
+      else
+        // p / 2 * erfc(-g / sqrt 2): for g >= -6 the argument's rounding grows by at most 2 (6 / sqrt 2)^2 = 36
         y[k] = 0.5f * p * erfcf(-0.70710678f * g[k]);
-        if (g[k] < -6.f) doubt |= 1u << k;
-      }
+    }
+    uint32_t doubt = 0;
+    if (low < (ACT == 0 ? -16.f : -6.f)) {
+      // the tail; where e^g leaves float32 only a vast product could matter beside a block's ordinary values
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (g[k] < (ACT == 0 ? -16.f : -6.f)) doubt |= (fabsf(g[k] * u[k]) > 1e12f ? 0x10000u : 1u) << k;
     }
     mx8_block<V>(
-        y, ACT == 0 ? 48u : 160u, doubt,
+        y, ACT == 0 ? 32u : 128u, doubt,
         [=](int k) { return act_exact<ACT>(to_f32<T>(gp[k]), to_f32<T>(up[k])); },
         [=]() {
           bool z = true;
@@ -346,12 +386,13 @@ void launch_rmsnorm_mx8(const RmsnormMx8Args& r, cudaStream_t s) {
     const int vecs = r.cols / V;
     if (r.cols % kBlock != 0 || vecs > 4 * 1024) throw std::runtime_error("minisgl.rmsnorm_mx8: unsupported width");
     const NormArgs a{r.x, r.residual, r.residual_out, r.w, r.q, r.sf, r.cols, r.ld_x, r.ld_res, r.ld_res_out,
-                     r.ld_q, r.ld_sf, r.eps};
+                     r.ld_q, r.ld_sf, r.eps, 1.0 / r.cols};
     const int threads = std::min(1024, (((vecs + 3) / 4) + 31) / 32 * 32);
     launch_pdl(rmsnorm_mx8_kernel<T, 4>, dim3(static_cast<unsigned>(r.rows)), dim3(threads), 0, s, a);
   });
 }
 
+constexpr int kActPerSm = 5;
 void launch_act_mx8(const ActMx8Args& r, cudaStream_t s) {
   if (r.rows <= 0) return;
   by_dtype(r.dtype, [&](auto tag) {
@@ -361,12 +402,13 @@ void launch_act_mx8(const ActMx8Args& r, cudaStream_t s) {
     if (r.interleaved && r.d % 64 != 0)
       throw std::runtime_error("minisgl.act_mx8: interleaved width must be a multiple of 64");
     const ActArgs a{r.x, r.q, r.sf, r.rows, r.ld_x, r.ld_q, r.ld_sf, r.d, r.interleaved ? 1 : 0};
-    const int64_t total = r.rows * (r.d / V);
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 148 * 16));
+    const unsigned parts = static_cast<unsigned>((r.d + 256 * V - 1) / (256 * V));
+    // blocks of a column part share its rows; some four per SM
+    const dim3 blocks(parts, static_cast<unsigned>(std::min<int64_t>(r.rows, std::max<int64_t>(1, 148 * kActPerSm / parts))));
     if (r.act == 0)
-      launch_pdl(act_mx8_kernel<T, 0>, dim3(blocks), dim3(256), 0, s, a);
+      launch_pdl(act_mx8_kernel<T, 0>, blocks, dim3(256), 0, s, a);
     else
-      launch_pdl(act_mx8_kernel<T, 1>, dim3(blocks), dim3(256), 0, s, a);
+      launch_pdl(act_mx8_kernel<T, 1>, blocks, dim3(256), 0, s, a);
   });
 }
 
