@@ -569,7 +569,7 @@ std::pair<at::Tensor, at::Tensor> act_mx8(const at::Tensor& x, int64_t act, bool
   a.dtype = dtype_of(x);
   check_vec_rows(x, rows, 2 * d, x.scalar_type(), "act_mx8", "x");
   MSG_CHECK(!interleaved || d % 64 == 0, "act_mx8: the interleaved width must be a multiple of 64, got ", d);
-  MSG_CHECK(d < (1ll << 30), "act_mx8: too wide");
+  MSG_CHECK(d < (1ll << 30) && rows < (1ll << 31), "act_mx8: too wide or too many rows");
   const c10::cuda::CUDAGuard guard(x.device());
   auto [q, sf] = mx8_out(x, rows, d, out, "act_mx8");
   a.x = x.data_ptr();

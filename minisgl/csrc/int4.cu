@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   };
   // the first of x's loads go ahead of the weights', which they would else queue behind
   constexpr int kBatch = 4;
-  uint4 raw[kBatch];
+  uint4 raw[kBatch], ahead[kBatch];
   // run c of row m: a warp's 32 runs are of one row or (ks odd) of two neighbours
   const int per_row = ks * 16;
   int xm = 0, xc = threadIdx.x;
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   auto load_x = [&]() {
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
-      if (lm < a.M) raw[q] = x_raw(a, lm, k0 * 128 + lc * 8);
+      if (lm < a.M) ahead[q] = x_raw(a, lm, k0 * 128 + lc * 8);
       next_run(lm, lc);
     }
   };
@@ -333,6 +333,9 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   // 2^-11, E4M3 2^-18), else at most 2^-22 of it off, as much as a rounding of a float32 sum
   bool odd = false;  // met an infinity or NaN
   while (xm < a.M) {
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) raw[q] = ahead[q];
+    if (lm < a.M) load_x();  // the next batch is on its way while this one is converted
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
       if (xm >= a.M) break;
@@ -391,7 +394,6 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
           *reinterpret_cast<int2*>(sd + 32 + (c & 15) / (G / 8) * 64 + m * 8) = make_int2(sum & 0xFFFF, sum >> 16);
       }
     }
-    load_x();
   }
   odd = __syncthreads_or(odd);
   if (S > 1) cluster_sync();  // the peers have started: their shared memory may be written

@@ -15,7 +15,7 @@
 //   warp 1      issues the MMAs
 //   warp 2      codes by TMA, a ring of kPs steps (8 KB)
 //   warps 4-7   epilogue (tensor-memory lanes 32 (w % 4) ..)
-//   warps 8-23  two sets of converters, which take the steps in turn; a warp has 32 rows x 64 columns of a step
+//   warps 8-..  two or three sets of converters, which take the steps in turn; a warp has 32 rows x 64 columns of a step
 //
 // W = (c - z) s is rounded once to bf16 (fp16): the one rounding besides those
 // of the float32 sums. fp16 weights are formed under each row's own power of
@@ -42,8 +42,6 @@ namespace minisgl {
 namespace {
 
 constexpr int kRows = 128;       // weight rows of a tile
-constexpr int kSets = 2;         // converter sets of 8 warps, which take the steps in turn
-constexpr int kThreads = 256 + kSets * 256;
 constexpr int kConverters = 8;
 constexpr int kACols = 64;       // tensor-memory columns of one step of weights: 128 values of 16 bits a row
 constexpr int kCodes = 8 * 1024;  // 128 rows x 128 columns
@@ -54,6 +52,11 @@ struct GSmem {
   static constexpr int kXs = BN == 256 || BN == 128 ? 3 : BN == 192 ? 4 : 6;
   static constexpr int kPs = BN >= 192 ? 3 : 6;
   static constexpr int kAs = BN == 192 ? 2 : BN == 32 ? 3 : 4;  // steps of weights in tensor memory
+  // converter sets of 8 warps, which take the steps in turn; not more than steps in tensor memory, or a set could meet
+  // a slot's barrier two phases away. Three were no faster than two: the instructions they issue are the bound.
+  static constexpr int kSets = 2;
+  static_assert(kSets <= kAs && kSets <= kPs, "turns");
+  static constexpr int kThreads = 256 + kSets * 256;
   static constexpr int kAcc = BN == 256 ? 1 : 2;  // sums in tensor memory; 256 columns leave room for one (one tile a CTA)
   static constexpr int kPt = kXs * kX;
   static constexpr int kSt = kPt + kPs * kCodes;   // the steps' scales, 1 KB apart
@@ -146,11 +149,11 @@ struct Pair {
 };
 
 template <int BN, int G, bool HALF>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(GSmem<BN>::kThreads, 1)
     int4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_s,
                      const __grid_constant__ CUtensorMap tm_z, const __grid_constant__ CUtensorMap tm_x, const GArgs a) {
   using L = GSmem<BN>;
-  constexpr int P = 128 / G;
+  constexpr int P = 128 / G, kSets = L::kSets;
   constexpr int kZeroRow = P == 1 ? 16 : 8 * P, kZeroB = 8 * kZeroRow;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -295,7 +298,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int set = (warp - 8) / 8, quad = warp & 3, half = (warp >> 2) & 1, g = lane >> 2;
     const uint32_t a_base = tmem + L::kAcc * BN + half * (kACols / 2) + (static_cast<uint32_t>(32 * quad) << 16);
     constexpr int H = P == 4 ? 2 : 1;  // groups of 64 columns
-    int it = 0;
+    // own steps lie kSets apart, over the ends of tiles too: slots and phases are carried along
+    int ps = set, as = set, turn = set;
+    uint32_t ps_phase = 0, as_phase = 1;  // the first use of a slot in tensor memory finds it empty
+    const uint32_t codes_at = L::kPt + quad * 2048 + half * 512 + lane * 16;
+    const uint32_t scales_at = L::kSt + (2 * quad * P + (P == 1 ? 0 : half * H)) * 32 + g * 4;
+    uint32_t zero[2][H][2];  // as the pairs that are subtracted; 8 without zero points
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int p = 0; p < H; ++p) zero[c][p][0] = zero[c][p][1] = Pair<HALF>::zero(8);
     bool ok = true;
     for (int tile = first; ok && tile < num_tiles; tile += stride) {
       float down[2][2];  // 1 / the rows' power of two
@@ -305,40 +317,43 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int r = 0; r < 2; ++r) down[c][r] = HALF ? 1.f / a.row_pow[tile16 * 16 + g + 8 * r] : 1.f;
       }
-      // this set's steps of the tile
-      const int turn = (set + kSets - it % kSets) % kSets;
-      for (int k = k0; k < k1 && ok; ++k, ++it) {
-        if ((k - k0) % kSets != turn) continue;
-        const int ps = it % L::kPs, as = it % L::kAs;
-        ok = __all_sync(0xffffffffu, mbar_wait(&pfull[ps], (it / L::kPs) & 1, a.err, 426));
+      int k = k0 + turn;
+      for (; k < k1; k += kSets) {
+        if (!__all_sync(0xffffffffu, mbar_try_wait(&pfull[ps], ps_phase)))
+          ok = __all_sync(0xffffffffu, mbar_wait(&pfull[ps], ps_phase, a.err, 426));
         if (!ok) break;
-        const uint4* codes = reinterpret_cast<const uint4*>(smem + L::kPt + ps * kCodes + quad * 2048 + half * 512) + lane;
-        const uint4 w[2] = {codes[0], codes[64]};
-        uint32_t sc[2][H], zz[2][H];
+        const uint8_t* codes = smem + codes_at + ps * kCodes;
+        const uint4 w[2] = {*reinterpret_cast<const uint4*>(codes), *reinterpret_cast<const uint4*>(codes + 1024)};
+        uint32_t sc[2][H];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int p = 0; p < H; ++p) {
-            const int tile16 = 2 * quad + c, group = P == 1 ? 0 : half * H + p;
-            sc[c][p] = *reinterpret_cast<const uint32_t*>(smem + L::kSt + ps * 1024 + (tile16 * P + group) * 32 + g * 4);
-            zz[c][p] = a.zeros == nullptr
-                           ? 0x88u
-                           : smem[L::kZt + ps * 256 + tile16 * kZeroRow + (P == 1 ? (k & 1) * 8 : group * 8) + g];
-          }
+          for (int p = 0; p < H; ++p)
+            sc[c][p] = *reinterpret_cast<const uint32_t*>(smem + scales_at + ps * 1024 + (c * P + p) * 32);
+        if (a.zeros != nullptr) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int p = 0; p < H; ++p) {
+              const uint32_t zz = smem[L::kZt + ps * 256 + (2 * quad + c) * kZeroRow + (P == 1 ? (k & 1) * 8 : (half * H + p) * 8) + g];
+              zero[c][p][0] = Pair<HALF>::zero(zz & 15u), zero[c][p][1] = Pair<HALF>::zero(zz >> 4);
+            }
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&pempty[ps]);  // the codes are in registers
+        ps += kSets;
+        if (ps >= L::kPs) ps -= L::kPs, ps_phase ^= 1;
         uint32_t o[2][16];  // per tile and word (16 columns): two pairs of row g, two of row g + 8
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t sw = sc[c][j * H / 4], zw = zz[c][j * H / 4];
-            const uint32_t z[2] = {Pair<HALF>::zero(zw & 15u), Pair<HALF>::zero(zw >> 4)};
+            const uint32_t sw = sc[c][j * H / 4];
             uint32_t d[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r)  // r: bit 0 the row half, bit 1 the column pair
-              d[2 * (r & 1) + (r >> 1)] = Pair<HALF>::sub(Pair<HALF>::code(words[j] >> (4 * r)), z[r & 1]);
+              d[2 * (r & 1) + (r >> 1)] = Pair<HALF>::sub(Pair<HALF>::code(words[j] >> (4 * r)), zero[c][j * H / 4][r & 1]);
             if (HALF || !a.scale_half) {
               uint32_t s[2];
               if constexpr (HALF) {
@@ -362,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // only the store waits for the MMAs that read the slot before
-        if (it >= L::kAs) ok = __all_sync(0xffffffffu, mbar_wait(&aempty[as], ((it / L::kAs) - 1) & 1, a.err, 427));
+        if (!__all_sync(0xffffffffu, mbar_try_wait(&aempty[as], as_phase)))
+          ok = __all_sync(0xffffffffu, mbar_wait(&aempty[as], as_phase, a.err, 427));
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -372,7 +388,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&afull[as]);
+        as += kSets;
+        if (as >= L::kAs) as -= L::kAs, as_phase ^= 1;
       }
+      turn = k - k1;  // of the next tile's steps
     }
     if (!ok && lane == 0) *abort_flag = 1;
     __syncwarp();
@@ -462,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     cluster_sync();
     const int x0 = BN * rank / S, x1 = BN * (rank + 1) / S;
     const int64_t n0 = static_cast<int64_t>(first / a.m_tiles) * kRows;
-    for (int i = threadIdx.x; i < (x1 - x0) * (kRows / 4); i += kThreads) {
+    for (int i = threadIdx.x; i < (x1 - x0) * (kRows / 4); i += L::kThreads) {
       const int at = x0 + i / (kRows / 4), q = i % (kRows / 4) * 4;
       const int m = first % a.m_tiles * BN + at;
       if (m >= a.M) continue;
@@ -512,7 +531,7 @@ __global__ void __launch_bounds__(256) mx8_rows_bf16_kernel(uint4* out, const ui
 }
 
 template <auto kern>
-int resident(int S, int smem) {
+int resident(int S, int smem, int threads) {
   constexpr int kDevices = 64;
   static std::atomic<int> known[kDevices][8];
   int dev = 0;
@@ -526,7 +545,7 @@ int resident(int S, int smem) {
   } else if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(S);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -561,7 +580,7 @@ void plan_bn(const GArgs& a, GPlan& best) {
   const int64_t step = std::max<int64_t>(BN * 256 / 55, kUnpack);
   for (int S = 1; S <= 8 && S <= a.steps; ++S) {
     if (S > 1 && BN > 128) break;  // no room for the partial sums
-    const int fit = resident<kern>(S, L::bytes(S));
+    const int fit = resident<kern>(S, L::bytes(S), L::kThreads);
     if (S > 1 && tiles > fit) break;  // a cluster has one tile
     const int64_t waves = (tiles + fit - 1) / fit;
     if (BN == 256 && waves > 1) break;
@@ -580,7 +599,7 @@ void launch_bn(GArgs a, const GPlan& p, const CUtensorMap* tw, const CUtensorMap
   const int grid = p.grid;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(L::kThreads);
   cfg.dynamicSmemBytes = L::bytes(a.S);
   cfg.stream = s;
   cudaLaunchAttribute attrs[2];

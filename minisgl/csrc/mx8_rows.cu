@@ -21,6 +21,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <atomic>
 #include <stdexcept>
 
 #include "common.cuh"
@@ -31,17 +32,30 @@ namespace minisgl {
 namespace {
 
 constexpr int kBlock = 32;  // columns under one scale
+#ifndef MINCTA
+#define MINCTA 3
+#endif
 
+// A lane's share of a row is two 16-byte vectors: 16 values of a 16-bit type (two lanes share a scale), 8 of float32
+// (four lanes). With one vector a lane the shuffles, the scale and the addresses cost as much as the values.
+struct Pair {
+  uint4 v[2];
+};
+template <typename T>
+__device__ __forceinline__ Pair load_pair(const T* p) {
+  return Pair{{reinterpret_cast<const uint4*>(p)[0], reinterpret_cast<const uint4*>(p)[1]}};
+}
+template <typename T>
+__device__ __forceinline__ void store_pair(T* p, const Pair& r) {
+  reinterpret_cast<uint4*>(p)[0] = r.v[0];
+  reinterpret_cast<uint4*>(p)[1] = r.v[1];
+}
 template <typename T, int V>
-__device__ __forceinline__ void unpack_vec(const uint4& raw, float (&v)[V]) {
-  static_assert(V * sizeof(T) == 16, "one 16-byte vector");
+__device__ __forceinline__ void unpack(const Pair& raw, float (&v)[V]) {
+  static_assert(V * sizeof(T) == 32, "two vectors");
   const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = to_f32<T>(e[i]);
-}
-template <typename T, int V>
-__device__ __forceinline__ void load_row_vec(const T* p, float (&v)[V]) {
-  unpack_vec<T, V>(*reinterpret_cast<const uint4*>(p), v);
 }
 
 // E4M3 bits of a double: truncated to float32 with a sticky last bit
@@ -59,6 +73,11 @@ __device__ __forceinline__ double pow2(int e) {  // 2^e, |e| <= 1000
 __device__ __forceinline__ float max_abs3(float a, float b, float c) {
   float d;
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 __device__ __forceinline__ uint32_t e4m3x4(const float* t, float s) {
@@ -166,10 +185,10 @@ __device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t slack, u
       }
     }
   }
-  if constexpr (V == 8) {
-    *reinterpret_cast<uint2*>(q) = make_uint2(words[0], words[1]);
+  if constexpr (V == 16) {
+    *reinterpret_cast<uint4*>(q) = make_uint4(words[0], words[1], words[2], words[3]);
   } else {
-    *reinterpret_cast<uint32_t*>(q) = words[0];
+    *reinterpret_cast<uint2*>(q) = make_uint2(words[0], words[1]);
   }
   if ((lane & (G - 1)) == 0) *sf = static_cast<uint8_t>(sbyte);
 }
@@ -185,102 +204,128 @@ struct NormArgs {
   int cols;
   int64_t ld_x, ld_res, ld_res_out, ld_q, ld_sf;
   double eps, inv_cols;
+  int64_t rows;
 };
 
-// One CTA per row, the row kept in registers between the two passes.
-// The sum of squares is held in double: the squares of 16-bit inputs are
-// exact there, so the statistic is exact but for the final additions.
-template <typename T, int NV>
-__global__ void __launch_bounds__(1024) rmsnorm_mx8_kernel(const NormArgs a) {
+// A CTA walks rows; a row stays in registers between its two passes. With AHEAD (up to 256 threads, which leaves the
+// registers for it) the loads of the CTA's next row are on their way while this one is reduced and stored; without,
+// the wait for memory at the start of a row and the barrier leave the memory idle (B200, 8192 x 7168 bf16 with
+// residual: 101 us). The sum of squares is held in double: the squares of 16-bit inputs are exact there, so the
+// statistic is exact but for the final additions.
+template <typename T, int NP, int THREADS, bool AHEAD>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? MINCTA : 1) rmsnorm_mx8_kernel(const NormArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int V = 16 / sizeof(T);
-  __shared__ double red[32];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
-  const T* res = a.res != nullptr ? static_cast<const T*>(a.res) + row * a.ld_res : nullptr;
-  T* res_out = static_cast<T*>(a.res_out) + row * a.ld_res_out;
-  float v[NV][V];
-  double ss = 0.0;
+  constexpr int V = 32 / sizeof(T);
+  __shared__ double red[2][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  const bool has_res = a.res != nullptr, has_w = a.w != nullptr;
+  Pair next_x[NP], next_r[NP];
+  auto load = [&](int64_t row) {
+    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+    const T* res = static_cast<const T*>(a.res) + row * a.ld_res;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (k * blockDim.x + threadIdx.x) * V;
-    if (c < a.cols) {
-      load_row_vec<T, V>(x + c, v[k]);
-      if (res != nullptr) {
-        float r[V];
-        load_row_vec<T, V>(res + c, r);
-        uint4 raw;
-        T* e = reinterpret_cast<T*>(&raw);
+    for (int k = 0; k < NP; ++k) {
+      const int c = (k * blockDim.x + threadIdx.x) * V;
+      if (c < a.cols) {
+        next_x[k] = load_pair(x + c);
+        if (has_res) next_r[k] = load_pair(res + c);
+      }
+    }
+  };
+  load(blockIdx.x);
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+    T* res_out = static_cast<T*>(a.res_out) + row * a.ld_res_out;
+    Pair raw[NP];  // what is normalised, in its type
+    double part[4] = {0.0, 0.0, 0.0, 0.0};  // four short chains
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int c = (k * blockDim.x + threadIdx.x) * V;
+      if (c < a.cols) {
+        float v[V];
+        raw[k] = next_x[k];
+        unpack<T, V>(raw[k], v);
+        if (has_res) {
+          float r[V];
+          unpack<T, V>(next_r[k], r);
+          T* e = reinterpret_cast<T*>(&raw[k]);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            // the residual stream is kept in the activation's type: the sum is rounded before it is normalised
+            e[i] = from_f32<T>(v[i] + r[i]);
+            v[i] = to_f32<T>(e[i]);
+          }
+          store_pair(res_out + c, raw[k]);
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          // the residual stream is kept in the activation's type: the sum is rounded before it is normalised
-          e[i] = from_f32<T>(v[k][i] + r[i]);
-          v[k][i] = to_f32<T>(e[i]);
+          const double d = v[i];
+          part[i & 3] = fma(d, d, part[i & 3]);
         }
-        *reinterpret_cast<uint4*>(res_out + c) = raw;
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const double d = v[k][i];
-        ss = fma(d, d, ss);
       }
     }
-  }
+    double ss = (part[0] + part[1]) + (part[2] + part[3]);
+    if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) red[warp] = ss;
-  __syncthreads();
-  const int nw = blockDim.x >> 5;
-  ss = lane < nw ? red[lane] : 0.0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  // 1 / sqrt: two Newton steps in double on the float32 estimate leave some units of 2^-53
-  const double mean = ss * a.inv_cols + a.eps;
-  double inv_d;
-  if (mean > 1e-30 && mean < 1e30) {
-    inv_d = rsqrtf(static_cast<float>(mean));
-    const double half = 0.5 * mean;
-    inv_d = fma(inv_d, fma(-half * inv_d, inv_d, 0.5), inv_d);
-    inv_d = fma(inv_d, fma(-half * inv_d, inv_d, 0.5), inv_d);
-  } else {
-    inv_d = 1.0 / sqrt(mean);
-  }
-  // a row whose factor is at the ends of float32's range is computed in double as a whole (NaN sends it there)
-  const bool tame = inv_d > 1e-30 && inv_d < 1e30;
-  const float inv = tame ? static_cast<float>(inv_d) : __uint_as_float(0x7FC00000u);
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (k * blockDim.x + threadIdx.x) * V;
-    const bool active = c < a.cols;
-    float y[V];
-    if (active) {
-      float w[V];
-      if (a.w != nullptr) load_row_vec<T, V>(static_cast<const T*>(a.w) + c, w);
-      // three roundings (inv and two products): at most 3 * 2^-24
-#pragma unroll
-      for (int i = 0; i < V; ++i) y[i] = a.w != nullptr ? v[k][i] * inv * w[i] : v[k][i] * inv;
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    // the two halves of red alternate: a warp that writes one again has passed the barrier after everybody read it
+    if (lane == 0) red[turn][warp] = ss;
+    __syncthreads();
+    ss = red[turn][0];  // the same order in every thread
+    for (int w = 1; w < nw; ++w) ss += red[turn][w];
+    // 1 / sqrt: two Newton steps in double on the float32 estimate leave some units of 2^-53
+    const double mean = ss * a.inv_cols + a.eps;
+    double inv_d;
+    if (mean > 1e-30 && mean < 1e30) {
+      inv_d = rsqrtf(static_cast<float>(mean));
+      const double half = 0.5 * mean;
+      inv_d = fma(inv_d, fma(-half * inv_d, inv_d, 0.5), inv_d);
+      inv_d = fma(inv_d, fma(-half * inv_d, inv_d, 0.5), inv_d);
     } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) y[i] = 0.f;
+      inv_d = 1.0 / sqrt(mean);
     }
-    const T* src = (res != nullptr ? res_out : x) + c;  // the normalised row's input, as stored
-    const T* wc = static_cast<const T*>(a.w) + c;
-    const bool has_w = a.w != nullptr;
-    mx8_block<V>(
-        y, 4u, 0u,
-        [=](int i) {
-          const double d = static_cast<double>(to_f32<T>(src[i])) * inv_d;
-          return has_w ? d * static_cast<double>(to_f32<T>(wc[i])) : d;
-        },
-        [=]() {
-          bool z = true;
+    // a row whose factor is at the ends of float32's range is computed in double as a whole (NaN sends it there)
+    const bool tame = inv_d > 1e-30 && inv_d < 1e30;
+    const float inv = tame ? static_cast<float>(inv_d) : __uint_as_float(0x7FC00000u);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int c = (k * blockDim.x + threadIdx.x) * V;
+      const bool active = c < a.cols;
+      float y[V];
+      if (active) {
+        unpack<T, V>(raw[k], y);
+        // three roundings (inv and two products): at most 3 * 2^-24
+#pragma unroll
+        for (int i = 0; i < V; ++i) y[i] *= inv;
+        if (has_w) {
+          float w[V];
+          unpack<T, V>(load_pair(static_cast<const T*>(a.w) + c), w);
+#pragma unroll
+          for (int i = 0; i < V; ++i) y[i] *= w[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) y[i] = 0.f;
+      }
+      const T* src = (has_res ? res_out : x) + c;  // the normalised row's input, as stored
+      const T* wc = static_cast<const T*>(a.w) + c;
+      mx8_block<V>(
+          y, 4u, 0u,
+          [=](int i) {
+            const double d = static_cast<double>(to_f32<T>(src[i])) * inv_d;
+            return has_w ? d * static_cast<double>(to_f32<T>(wc[i])) : d;
+          },
+          [=]() {
+            bool z = true;
 #pragma unroll 1
-          for (int i = 0; i < V; ++i) z &= to_f32<T>(src[i]) == 0.f;
-          return z;
-        },
-        a.q + row * a.ld_q + c, a.sf + row * a.ld_sf + c / kBlock, active);
+            for (int i = 0; i < V; ++i) z &= to_f32<T>(src[i]) == 0.f;
+            return z;
+          },
+          a.q + row * a.ld_q + c, a.sf + row * a.ld_sf + c / kBlock, active);
+    }
+    if (!AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
   }
 }
 
@@ -312,32 +357,37 @@ __device__ __forceinline__ float ex2_approx(float x) {  // 2 units
   return r;
 }
 
-// A block takes 256 V outputs of a row at a time, and the loads of its next row are on their way while it works.
+// A block takes a part of a row at a time, and the loads of its next row are on their way while it works.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int V = 16 / sizeof(T);
-  const int c0 = (blockIdx.x * 256 + threadIdx.x) * V;
+  constexpr int V = 32 / sizeof(T);
+  const int c0 = (blockIdx.x * blockDim.x + threadIdx.x) * V;
   const bool active = c0 < a.d;  // the same for the lanes of a block: d is a multiple of 32
   const int c = active ? c0 : 0;
   const T* gp = static_cast<const T*>(a.x) + blockIdx.y * a.ld_x + (a.interleaved ? (c / 64) * 128 + c % 64 : c);
   const int to_up = a.interleaved ? 64 : a.d;
   const int64_t step = gridDim.y * a.ld_x;
-  uint4 next_g = *reinterpret_cast<const uint4*>(gp), next_u = *reinterpret_cast<const uint4*>(gp + to_up);
-  for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y, gp += step) {
+  Pair next_g = load_pair(gp), next_u = load_pair(gp + to_up);
+  uint8_t* q = a.q + blockIdx.y * a.ld_q + c;
+  uint8_t* sf = a.sf + blockIdx.y * a.ld_sf + c / kBlock;
+  const int64_t step_q = gridDim.y * a.ld_q, step_sf = gridDim.y * a.ld_sf;
+  const int rows = static_cast<int>(a.rows), rows_step = static_cast<int>(gridDim.y);
+  for (int r = blockIdx.y; r < rows; r += rows_step, gp += step, q += step_q, sf += step_sf) {
     float g[V], u[V], y[V];
-    unpack_vec<T, V>(next_g, g);
-    unpack_vec<T, V>(next_u, u);
+    unpack<T, V>(next_g, g);
+    unpack<T, V>(next_u, u);
     const T* up = gp + to_up;
-    if (r + gridDim.y < a.rows) {
-      next_g = *reinterpret_cast<const uint4*>(gp + step);
-      next_u = *reinterpret_cast<const uint4*>(up + step);
+    if (r < rows - rows_step) {
+      next_g = load_pair(gp + step);
+      next_u = load_pair(up + step);
     }
     float low = g[0];
 #pragma unroll
+    for (int k = 1; k < V; k += 2) low = min3(low, g[k], g[k + 1 < V ? k + 1 : k]);
+#pragma unroll
     for (int k = 0; k < V; ++k) {
-      low = fminf(low, g[k]);
       const float p = g[k] * u[k];  // exact for 16-bit types
       if (ACT == 0)
         // p / (1 + e^-g): for g >= -16 the exponential's argument (16 * 2^-24) and value, the sum, the reciprocal
@@ -363,7 +413,7 @@ __global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
           for (int k = 0; k < V; ++k) z &= to_f32<T>(gp[k]) == 0.f || to_f32<T>(up[k]) == 0.f;
           return z;
         },
-        a.q + r * a.ld_q + c, a.sf + r * a.ld_sf + c / kBlock, active);
+        q, sf, active);
   }
 }
 
@@ -376,39 +426,62 @@ void by_dtype(DType dt, F&& f) {
   }
 }
 
+// as many CTAs as fit the SMs at once, each walking its rows
+template <auto kern>
+void launch_norm(const NormArgs& a, int threads, cudaStream_t s) {
+  static std::atomic<int> fit[33];  // CTAs of an SM by warps
+  int n = fit[threads / 32].load();
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1) n = 1;
+    fit[threads / 32].store(n);
+  }
+  launch_pdl(kern, dim3(static_cast<unsigned>(std::min<int64_t>(a.rows, 148 * n))), dim3(threads), 0, s, a);
+}
+
 }  // namespace
 
 void launch_rmsnorm_mx8(const RmsnormMx8Args& r, cudaStream_t s) {
   if (r.rows <= 0) return;
   by_dtype(r.dtype, [&](auto tag) {
     using T = decltype(tag);
-    constexpr int V = 16 / sizeof(T);
-    const int vecs = r.cols / V;
-    if (r.cols % kBlock != 0 || vecs > 4 * 1024) throw std::runtime_error("minisgl.rmsnorm_mx8: unsupported width");
+    constexpr int V = 32 / sizeof(T);
+    const int pairs = r.cols / V;
+    if (r.cols % kBlock != 0 || pairs > 2 * 1024) throw std::runtime_error("minisgl.rmsnorm_mx8: unsupported width");
     const NormArgs a{r.x, r.residual, r.residual_out, r.w, r.q, r.sf, r.cols, r.ld_x, r.ld_res, r.ld_res_out,
-                     r.ld_q, r.ld_sf, r.eps, 1.0 / r.cols};
-    const int threads = std::min(1024, (((vecs + 3) / 4) + 31) / 32 * 32);
-    launch_pdl(rmsnorm_mx8_kernel<T, 4>, dim3(static_cast<unsigned>(r.rows)), dim3(threads), 0, s, a);
+                     r.ld_q, r.ld_sf, r.eps, 1.0 / r.cols, r.rows};
+    const auto threads = [&](int np) { return (pairs + np * 32 - 1) / (np * 32) * 32; };
+    if (pairs <= 256)
+      launch_norm<rmsnorm_mx8_kernel<T, 1, 256, true>>(a, threads(1), s);
+    else if (pairs <= 512)
+      launch_norm<rmsnorm_mx8_kernel<T, 2, 256, true>>(a, threads(2), s);
+    else
+      launch_norm<rmsnorm_mx8_kernel<T, 2, 1024, false>>(a, threads(2), s);
   });
 }
 
-constexpr int kActPerSm = 5;
+constexpr int kActPerSm = 3;
 void launch_act_mx8(const ActMx8Args& r, cudaStream_t s) {
   if (r.rows <= 0) return;
   by_dtype(r.dtype, [&](auto tag) {
     using T = decltype(tag);
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 32 / sizeof(T);
     if (r.d % kBlock != 0) throw std::runtime_error("minisgl.act_mx8: width must be a multiple of 32");
     if (r.interleaved && r.d % 64 != 0)
       throw std::runtime_error("minisgl.act_mx8: interleaved width must be a multiple of 64");
     const ActArgs a{r.x, r.q, r.sf, r.rows, r.ld_x, r.ld_q, r.ld_sf, r.d, r.interleaved ? 1 : 0};
-    const unsigned parts = static_cast<unsigned>((r.d + 256 * V - 1) / (256 * V));
-    // blocks of a column part share its rows; some four per SM
-    const dim3 blocks(parts, static_cast<unsigned>(std::min<int64_t>(r.rows, std::max<int64_t>(1, 148 * kActPerSm / parts))));
+    // the largest block that leaves the fewest threads without a share of the row
+    const int lanes = r.d / V;
+    int threads = 256;
+    for (int t = 224; t >= 96; t -= 32)
+      if ((lanes + t - 1) / t * t < (lanes + threads - 1) / threads * threads) threads = t;
+    const unsigned parts = static_cast<unsigned>((lanes + threads - 1) / threads);
+    // blocks of a column part share its rows; some three of 256 threads per SM
+    const int64_t blocks_y = std::min<int64_t>({r.rows, std::max<int64_t>(1, 148 * kActPerSm * 256 / threads / parts), 65535});
+    const dim3 blocks(parts, static_cast<unsigned>(blocks_y));
     if (r.act == 0)
-      launch_pdl(act_mx8_kernel<T, 0>, blocks, dim3(256), 0, s, a);
+      launch_pdl(act_mx8_kernel<T, 0>, blocks, dim3(threads), 0, s, a);
     else
-      launch_pdl(act_mx8_kernel<T, 1>, blocks, dim3(256), 0, s, a);
+      launch_pdl(act_mx8_kernel<T, 1>, blocks, dim3(threads), 0, s, a);
   });
 }
 
