@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   };
   // the first of x's loads go ahead of the weights', which they would else queue behind
   constexpr int kBatch = 4;
-  uint4 raw[kBatch], ahead[kBatch];
+  uint4 ahead[kBatch];
   // run c of row m: a warp's 32 runs are of one row or (ks odd) of two neighbours
   const int per_row = ks * 16;
   int xm = 0, xc = threadIdx.x;
@@ -332,67 +332,81 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   // largest value into [2^21, 2^22), rounded to nearest: exact for what lies above 2^-14 of it (bf16; fp16
   // 2^-11, E4M3 2^-18), else at most 2^-22 of it off, as much as a rounding of a float32 sum
   bool odd = false;  // met an infinity or NaN
-  while (xm < a.M) {
-#pragma unroll
-    for (int q = 0; q < kBatch; ++q) raw[q] = ahead[q];
-    if (lm < a.M) load_x();  // the next batch is on its way while this one is converted
+  const int batches = (a.M * per_row + kBatch * W * 32 - 1) / (kBatch * W * 32);
+#pragma unroll 1
+  for (int batch = 0; batch < batches; ++batch) {
+    // kBatch runs a thread side by side: their shuffles and conversions do not wait for one another
+    float v[kBatch][8];
+    uint32_t top[kBatch];
+    int m[kBatch], c[kBatch];
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
-      if (xm >= a.M) break;
-      const int m = xm, c = xc, step = c >> 4;
+      m[q] = xm, c[q] = xc;
       next_run(xm, xc);
-      float v[8];
-      x_values(v, raw[q], a.x_kind);
+      x_values(v[q], m[q] < a.M ? ahead[q] : make_uint4(0, 0, 0, 0), a.x_kind);
+    }
+    if (batch + 1 < batches) load_x();  // the next batch is on its way while this one is converted
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
       auto largest = [&]() {
         uint32_t b[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+        for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(v[q][j]) & 0x7FFFFFFFu;
         return max(__vimax3_u32(b[0], b[1], b[2]), __vimax3_u32(max(b[3], b[4]), b[5], max(b[6], b[7])));
       };
-      uint32_t top = largest();
-      if (top >= 0x7F800000u) {
+      top[q] = largest();
+      if (top[q] >= 0x7F800000u) {
         odd = true;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (!(fabsf(v[j]) <= 3.4028234e38f)) v[j] = 0.f;
-        top = largest();
+          if (!(fabsf(v[q][j]) <= 3.4028234e38f)) v[q][j] = 0.f;
+        top[q] = largest();
       }
-      const uint32_t half_warp = 0xFFFFu << (threadIdx.x & 16);  // 16 lanes share a row's 128 columns
+    }
+    // 16 lanes share a row's 128 columns
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(half_warp, top, o));
-      const uint32_t e = max(top >> 23, 26u);
+    for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) top[q] = max(top[q], __shfl_xor_sync(0xffffffffu, top[q], o));
+    int sum[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int step = c[q] >> 4;
+      const uint32_t e = max(top[q] >> 23, 26u);
       const float up = __uint_as_float((275u - e) << 23);
       uint32_t xi[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) xi[j] = __float_as_uint(fmaf(v[j], up, 12582912.f)) - 0x4B400000u;  // 1.5 * 2^23
+      for (int j = 0; j < 8; ++j) xi[j] = __float_as_uint(fmaf(v[q][j], up, 12582912.f)) - 0x4B400000u;  // 1.5 * 2^23
+      sum[q] = 0;
+      if constexpr (ZERO) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[q] += static_cast<int>(xi[j]);
+      }
+      if (m[q] >= a.M) continue;
       // lane 4 g + t reads columns 4 t .. 4 t + 3 of each 16: this run is two lanes' words
-      uint8_t* dst = xs + m * pitch + step * 384 + (c >> 3 & 1) * 64 + (c & 1) * 32 + (c >> 1 & 3) * 4;
-      uint32_t word[3][2];
+      uint8_t* dst = xs + m[q] * pitch + step * 384 + (c[q] >> 3 & 1) * 64 + (c[q] & 1) * 32 + (c[q] >> 1 & 3) * 4;
 #pragma unroll
       for (int l = 0; l < 2; ++l) {  // columns 0, 2, 1, 3: the order of a code word's bytes
         const uint32_t t0 = __byte_perm(xi[4 * l], xi[4 * l + 2], 0x5140), t1 = __byte_perm(xi[4 * l + 1], xi[4 * l + 3], 0x5140);
         const uint32_t t2 = __byte_perm(xi[4 * l], xi[4 * l + 2], 0x0062), t3 = __byte_perm(xi[4 * l + 1], xi[4 * l + 3], 0x0062);
-        word[0][l] = __byte_perm(t0, t1, 0x5410);
-        word[1][l] = __byte_perm(t0, t1, 0x7632);
-        word[2][l] = __byte_perm(t2, t3, 0x5410);
+        *reinterpret_cast<uint32_t*>(dst + l * 16) = __byte_perm(t0, t1, 0x5410);
+        *reinterpret_cast<uint32_t*>(dst + l * 16 + 128) = __byte_perm(t0, t1, 0x7632);
+        *reinterpret_cast<uint32_t*>(dst + l * 16 + 256) = __byte_perm(t2, t3, 0x5410);
       }
-#pragma unroll
-      for (int d = 0; d < 3; ++d) {
-        *reinterpret_cast<uint32_t*>(dst + d * 128) = word[d][0];
-        *reinterpret_cast<uint32_t*>(dst + d * 128 + 16) = word[d][1];
-      }
-      uint8_t* sd = side + step * L::kSide;
       // codes count in sixteenths (they sit in a byte's upper half): 2^-4 goes with the power of two
-      if ((c & 15) == 0) *reinterpret_cast<float*>(sd + m * 4) = __uint_as_float((e - 25u) << 23);
-      if constexpr (ZERO) {
-        int sum = 0;
+      if ((c[q] & 15) == 0)
+        *reinterpret_cast<float*>(side + step * L::kSide + m[q] * 4) = __uint_as_float((e - 25u) << 23);
+    }
+    if constexpr (ZERO) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += static_cast<int>(xi[j]);
+      for (int o = 1; o < G / 8; o <<= 1)
 #pragma unroll
-        for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(half_warp, sum, o);
-        if ((c & (G / 8 - 1)) == 0)
-          *reinterpret_cast<int2*>(sd + 32 + (c & 15) / (G / 8) * 64 + m * 8) = make_int2(sum & 0xFFFF, sum >> 16);
-      }
+        for (int q = 0; q < kBatch; ++q) sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], o);
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q)
+        if (m[q] < a.M && (c[q] & (G / 8 - 1)) == 0)
+          *reinterpret_cast<int2*>(side + (c[q] >> 4) * L::kSide + 32 + (c[q] & 15) / (G / 8) * 64 + m[q] * 8) =
+              make_int2(sum[q] & 0xFFFF, sum[q] >> 16);
     }
   }
   odd = __syncthreads_or(odd);
