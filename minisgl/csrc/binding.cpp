@@ -618,6 +618,19 @@ struct Int4Handle {
   }
 };
 
+at::Tensor int4_pack(const at::Tensor& codes) {
+  check_cuda(codes, "codes");
+  check_rowmajor(codes, "codes");
+  const int64_t n = codes.size(0), k = 2 * codes.size(1);
+  MSG_CHECK(codes.scalar_type() == at::kByte && n > 0 && k > 0 && k % 8 == 0 && n <= (1ll << 30) && k <= (1ll << 30) &&
+                (n == 1 || codes.stride(0) >= k / 2),
+            "int4_pack: codes must be uint8 [N, K / 2] with K a positive multiple of 8, got ", codes.sizes());
+  const c10::cuda::CUDAGuard guard(codes.device());
+  at::Tensor packed = at::empty({2 * ((n + 31) / 32), 2 * ((k + 127) / 128), 512}, codes.options());
+  minisgl::launch_int4_pack(packed.data_ptr(), codes.data_ptr<uint8_t>(), n, k, codes.stride(0), stream_of(codes));
+  return packed;
+}
+
 at::Tensor int4_linear(const at::Tensor& x, const Int4Handle& w, const c10::optional<at::Tensor>& bias,
                        const c10::optional<at::Tensor>& out_, const c10::optional<at::ScalarType>& out_dtype,
                        const c10::optional<at::Tensor>& x_scales) {
@@ -1724,6 +1737,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("act_mx8", &act_mx8);
   py::class_<Int4Handle>(m, "Int4Handle")
       .def(py::init<at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, int64_t, int64_t, int64_t, at::Tensor>());
+  m.def("int4_pack", &int4_pack);
   m.def("int4_linear", &int4_linear);
   m.def("moe_experts_mx", &moe_experts_mx, py::arg("out"), py::arg("x"), py::arg("w1q"), py::arg("w1sb"),
         py::arg("w2q"), py::arg("w2sb"), py::arg("topk_w"), py::arg("topk_ids"), py::arg("tile"), py::arg("xq"),

@@ -280,7 +280,9 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   const uint8_t* src_z =
       ZERO ? a.zeros + (static_cast<int64_t>(tile) * kR + (lane >= ZW ? 1 : 0)) * a.ld_z + (k0 + k) * SW + lane % ZW * 4 : nullptr;
   int left = u1 - u0, pk = k;
-  const int skip = kR * a.steps - ks;  // from the end of a unit row to the start of the next
+  // from the end of a pair's columns to the start of the next pair's
+  const int64_t skip = kR * a.steps - ks;
+  const int skip_z = kR * a.ld_z - ks * SW;
   const int64_t second = static_cast<int64_t>(a.steps) * 1024;
   auto fetch = [&](uint32_t dst) {
     if (left > 0) {
@@ -297,11 +299,15 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
         for (int r = 0; r < kR; ++r) cp_async4(dst + kR * 1024 + (r * SW + lane) * 4, src_s + r * a.steps * SW);
       }
       if (ZERO && lane < kR * ZW) cp_async4(dst + kR * (1024 + L::kScaleB) + lane * 4, src_z);
-      int on = 1, on_z = SW;
-      if (++pk == ks) pk = 0, on += skip, on_z = kR * a.ld_z - (ks - 1) * SW;
-      src_w += static_cast<int64_t>(on) * 1024;
-      src_s += static_cast<int64_t>(on) * SW;
-      if (ZERO) src_z += on_z;
+      src_w += 1024;
+      src_s += SW;
+      if (ZERO) src_z += SW;
+      if (++pk == ks) {
+        pk = 0;
+        src_w += skip * 1024;
+        src_s += skip * SW;
+        if (ZERO) src_z += skip_z;
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -454,109 +460,111 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   for (int d = 0; d < 3; ++d) xv[d][0] = xv[d][1] = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
   for (int u = u0; u < u1;) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-    __syncwarp();
-    uint32_t sc[kR][P], zz[kR][P];
-    uint32_t f[kR][4][4];  // the first operand
+    const int run = min(ks - k, u1 - u);  // this warp's units of the pair
+    uint32_t x_at = x_row + k * 384, sd = side_at + k * L::kSide;
+#pragma unroll 1
+    for (int i = 0; i < run; ++i, x_at += 384, sd += L::kSide) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      __syncwarp();
+      uint32_t sc[kR][P], zz[kR][P];
+      uint32_t f[kR][4][4];  // the first operand
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
+      for (int r = 0; r < kR; ++r) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          sc[r][p] = lds32(src + kR * 1024 + (SW * r + 8 * p + g) * 4);
+          zz[r][p] = ZERO ? lds8(src + kR * (1024 + L::kScaleB) + SW * r + 8 * p + g) : 0x88u;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 w = lds128(src + r * 1024 + h * 512 + lane * 16);
+          // bytes whose upper halves are the signed codes c - 8: row g's are the low nibbles, row g + 8's the high
+          f[r][2 * h][0] = w.x << 4 & 0xF0F0F0F0u, f[r][2 * h][1] = w.x & 0xF0F0F0F0u;
+          f[r][2 * h][2] = w.y << 4 & 0xF0F0F0F0u, f[r][2 * h][3] = w.y & 0xF0F0F0F0u;
+          f[r][2 * h + 1][0] = w.z << 4 & 0xF0F0F0F0u, f[r][2 * h + 1][1] = w.z & 0xF0F0F0F0u;
+          f[r][2 * h + 1][2] = w.w << 4 & 0xF0F0F0F0u, f[r][2 * h + 1][3] = w.w & 0xF0F0F0F0u;
+        }
+      }
+      __syncwarp();  // every lane has read the slot
+      fetch(src);
+      src = src + L::kUnit == ring + kDepth * L::kUnit ? ring : src + L::kUnit;
+      if (g < a.M) {
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+          xv[d][0] = lds128(x_at + d * 128);
+          xv[d][1] = lds128(x_at + d * 128 + 64);
+        }
+      }
+      const uint2 pw = lds64(sd);
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        sc[r][p] = lds32(src + kR * 1024 + (SW * r + 8 * p + g) * 4);
-        zz[r][p] = ZERO ? lds8(src + kR * (1024 + L::kScaleB) + SW * r + 8 * p + g) : 0x88u;
-      }
+        int c[kR][3][4];
+        // products of one digit and tile wait for one another; the 3 R chains run side by side
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 w = lds128(src + r * 1024 + h * 512 + lane * 16);
-        // bytes whose upper halves are the signed codes c - 8: row g's are the low nibbles, row g + 8's the high
-        f[r][2 * h][0] = w.x << 4 & 0xF0F0F0F0u, f[r][2 * h][1] = w.x & 0xF0F0F0F0u;
-        f[r][2 * h][2] = w.y << 4 & 0xF0F0F0F0u, f[r][2 * h][3] = w.y & 0xF0F0F0F0u;
-        f[r][2 * h + 1][0] = w.z << 4 & 0xF0F0F0F0u, f[r][2 * h + 1][1] = w.z & 0xF0F0F0F0u;
-        f[r][2 * h + 1][2] = w.w << 4 & 0xF0F0F0F0u, f[r][2 * h + 1][3] = w.w & 0xF0F0F0F0u;
-      }
-    }
-    __syncwarp();  // every lane has read the slot
-    fetch(src);
-    src = src + L::kUnit == ring + kDepth * L::kUnit ? ring : src + L::kUnit;
-    if (g < a.M) {
-      const uint32_t at = x_row + k * 384;
+        for (int j = p * 4 / P; j < (p + 1) * 4 / P; ++j) {
 #pragma unroll
-      for (int d = 0; d < 3; ++d) {
-        xv[d][0] = lds128(at + d * 128);
-        xv[d][1] = lds128(at + d * 128 + 64);
-      }
-    }
-    const uint32_t sd = side_at + k * L::kSide;
-    const uint2 pw = lds64(sd);
+          for (int r = 0; r < kR; ++r) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      int c[kR][3][4];
-      // products of one digit and tile wait for one another; the 3 R chains run side by side
-#pragma unroll
-      for (int j = p * 4 / P; j < (p + 1) * 4 / P; ++j) {
-#pragma unroll
-        for (int r = 0; r < kR; ++r) {
-#pragma unroll
-          for (int d = 0; d < 3; ++d) {
-            const uint4 v = xv[d][j >> 1];
-            const uint32_t b0 = j & 1 ? v.z : v.x, b1 = j & 1 ? v.w : v.y;
-            if (j == p * 4 / P) {
-              if (d == 2)
-                mma_i8<true, true>(c[r][d], f[r][j], b0, b1);
-              else
-                mma_i8<false, true>(c[r][d], f[r][j], b0, b1);
-            } else {
-              if (d == 2)
-                mma_i8<true, false>(c[r][d], f[r][j], b0, b1);
-              else
-                mma_i8<false, false>(c[r][d], f[r][j], b0, b1);
+            for (int d = 0; d < 3; ++d) {
+              const uint4 v = xv[d][j >> 1];
+              const uint32_t b0 = j & 1 ? v.z : v.x, b1 = j & 1 ? v.w : v.y;
+              if (j == p * 4 / P) {
+                if (d == 2)
+                  mma_i8<true, true>(c[r][d], f[r][j], b0, b1);
+                else
+                  mma_i8<false, true>(c[r][d], f[r][j], b0, b1);
+              } else {
+                if (d == 2)
+                  mma_i8<true, false>(c[r][d], f[r][j], b0, b1);
+                else
+                  mma_i8<false, false>(c[r][d], f[r][j], b0, b1);
+              }
             }
           }
         }
-      }
-      uint4 sums;
-      if constexpr (ZERO) sums = lds128(sd + 32 + p * 64 + t * 8);
+        uint4 sums;
+        if constexpr (ZERO) sums = lds128(sd + 32 + p * 64 + t * 8);
 #pragma unroll
-      for (int r = 0; r < kR; ++r) {
-        float s0, s1;
-        if (a.scale_half) {
-          const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&sc[r][p]));
-          s0 = h.x, s1 = h.y;
-        } else {
-          s0 = __uint_as_float(sc[r][p] << 16), s1 = __uint_as_float(sc[r][p] & 0xFFFF0000u);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // at most 2^22 (256 + 1) in the lower part, 2^20 in the upper: exact integers, one rounding to float32
-          // each and one where they meet
-          int lo = c[r][1][j] * 256 + c[r][0][j], hi = c[r][2][j];
-          if constexpr (ZERO) {
-            const int z = 16 * static_cast<int>(j < 2 ? zz[r][p] & 15u : zz[r][p] >> 4) - 128;  // 16 (z - 8)
-            lo -= z * static_cast<int>(j & 1 ? sums.z : sums.x);
-            hi -= z * static_cast<int>(j & 1 ? sums.w : sums.y);
+        for (int r = 0; r < kR; ++r) {
+          float s0, s1;
+          if (a.scale_half) {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&sc[r][p]));
+            s0 = h.x, s1 = h.y;
+          } else {
+            s0 = __uint_as_float(sc[r][p] << 16), s1 = __uint_as_float(sc[r][p] & 0xFFFF0000u);
           }
-          const float v = fmaf(static_cast<float>(hi), 65536.f, static_cast<float>(lo));
-          acc[r][j] = fmaf(v * (j < 2 ? s0 : s1), __uint_as_float(j & 1 ? pw.y : pw.x), acc[r][j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // at most 2^22 (256 + 1) in the lower part, 2^20 in the upper: exact integers, one rounding to float32
+            // each and one where they meet
+            int lo = c[r][1][j] * 256 + c[r][0][j], hi = c[r][2][j];
+            if constexpr (ZERO) {
+              const int z = 16 * static_cast<int>(j < 2 ? zz[r][p] & 15u : zz[r][p] >> 4) - 128;  // 16 (z - 8)
+              lo -= z * static_cast<int>(j & 1 ? sums.z : sums.x);
+              hi -= z * static_cast<int>(j & 1 ? sums.w : sums.y);
+            }
+            const float v = fmaf(static_cast<float>(hi), 65536.f, static_cast<float>(lo));
+            acc[r][j] = fmaf(v * (j < 2 ? s0 : s1), __uint_as_float(j & 1 ? pw.y : pw.x), acc[r][j]);
+          }
         }
       }
     }
-    ++u;
-    if (++k == ks || u == u1) {
-      if (!head && k == ks) {
-        emit(tile, acc);
-      } else {
-        float4* dst = park + (warp * 2 + (head ? 0 : 1)) * (kR * 32) + lane;
+    u += run;
+    k += run;
+    if (!head && k == ks) {
+      emit(tile, acc);
+    } else {
+      float4* dst = park + (warp * 2 + (head ? 0 : 1)) * (kR * 32) + lane;
 #pragma unroll
-        for (int r = 0; r < kR; ++r) dst[r * 32] = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
-      }
-      head = false;
-      ++tile;
-      k = 0;
-#pragma unroll
-      for (int r = 0; r < kR; ++r)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[r][j] = 0.f;
+      for (int r = 0; r < kR; ++r) dst[r * 32] = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
     }
+    head = false;
+    ++tile;
+    k = 0;
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[r][j] = 0.f;
   }
   __syncthreads();
   // the pair that this warp started and did not finish: its own part, then the heads of the warps after it
@@ -593,6 +601,40 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
       store_sum(a, static_cast<int64_t>(tl) * kR + (n >> 4), n & 15, m, v);
     }
   }
+}
+
+// Codes two per byte, row after row, into the tile layout (minisgl/quant/int4.py): one thread makes the 16 bytes of
+// one lane. Words are 4 columns of rows g and g + 8, two bytes of each.
+__global__ void __launch_bounds__(256) int4_pack_kernel(uint4* out, const uint8_t* codes, int64_t n, int64_t row_bytes,
+                                                        int64_t ld, int blocks, int64_t total) {
+  pdl_wait();  // no early launch of the kernels after it: they may read the layout at once
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i >= total) return;
+  const int lane = static_cast<int>(i & 31), g = lane >> 2, t = lane & 3;
+  const int64_t unit = i >> 5, tile = unit / blocks, block = unit - tile * blocks;
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t at = block * 32 + 8 * j + 2 * t;  // columns 2 at .. of the row
+    uint32_t b[2][2] = {};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t row = tile * 16 + g + 8 * h;
+      if (row < n && at < row_bytes) {  // whole runs of 4 columns: K is a multiple of 8
+        b[h][0] = codes[row * ld + at];
+        b[h][1] = codes[row * ld + at + 1];
+      }
+    }
+    // bytes (e, p): the low nibble is row g's column 2 p + e, the high one row g + 8's
+    w[j] = 0;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      w[j] |= ((b[0][p] & 15u) | (b[1][p] & 15u) << 4) << (8 * p);
+      w[j] |= (b[0][p] >> 4 | (b[1][p] >> 4) << 4) << (16 + 8 * p);
+    }
+    w[j] ^= 0x88888888u;  // c - 8, two's complement
+  }
+  out[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 struct VecPlan {
@@ -637,7 +679,7 @@ int resident_clusters(int S) {
 // are dealt to clusters, so many tiles balance alone (S = 1) and few tiles only
 // when their columns are shared. A cluster's two barriers and exchange cost
 // about as much as kClusterCost KB. False: x does not fit shared memory.
-constexpr int kClusterCost = 30;
+constexpr int kClusterCost = 100;
 template <typename L, auto kern, int W>
 bool vec_plan(const VecArgs& a, VecPlan& best) {
   int64_t best_cost = -1;
@@ -709,6 +751,13 @@ bool launch_vec_group(const VecArgs& a, int group, cudaStream_t s) {
 }
 
 }  // namespace
+
+void launch_int4_pack(void* out, const uint8_t* codes, int64_t n, int64_t k, int64_t ld, cudaStream_t s) {
+  const int blocks = static_cast<int>(2 * ((k + 127) / 128));
+  const int64_t total = 2 * ((n + 31) / 32) * blocks * 32;
+  launch_pdl(int4_pack_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0, s, static_cast<uint4*>(out),
+             codes, n, k / 2, ld, blocks, total);
+}
 
 void launch_int4_linear(const Int4LinearArgs& r, cudaStream_t s) {
   if (r.M <= 0) return;

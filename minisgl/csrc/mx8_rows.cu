@@ -32,9 +32,6 @@ namespace minisgl {
 namespace {
 
 constexpr int kBlock = 32;  // columns under one scale
-#ifndef MINCTA
-#define MINCTA 3
-#endif
 
 // A lane's share of a row is two 16-byte vectors: 16 values of a 16-bit type (two lanes share a scale), 8 of float32
 // (four lanes). With one vector a lane the shuffles, the scale and the addresses cost as much as the values.
@@ -213,7 +210,7 @@ struct NormArgs {
 // residual: 101 us). The sum of squares is held in double: the squares of 16-bit inputs are exact there, so the
 // statistic is exact but for the final additions.
 template <typename T, int NP, int THREADS, bool AHEAD>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? MINCTA : 1) rmsnorm_mx8_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rmsnorm_mx8_kernel(const NormArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int V = 32 / sizeof(T);
@@ -469,11 +466,8 @@ void launch_act_mx8(const ActMx8Args& r, cudaStream_t s) {
     if (r.interleaved && r.d % 64 != 0)
       throw std::runtime_error("minisgl.act_mx8: interleaved width must be a multiple of 64");
     const ActArgs a{r.x, r.q, r.sf, r.rows, r.ld_x, r.ld_q, r.ld_sf, r.d, r.interleaved ? 1 : 0};
-    // the largest block that leaves the fewest threads without a share of the row
     const int lanes = r.d / V;
-    int threads = 256;
-    for (int t = 224; t >= 96; t -= 32)
-      if ((lanes + t - 1) / t * t < (lanes + threads - 1) / threads * threads) threads = t;
+    const int threads = std::min(256, (lanes + 31) / 32 * 32);
     const unsigned parts = static_cast<unsigned>((lanes + threads - 1) / threads);
     // blocks of a column part share its rows; some three of 256 threads per SM
     const int64_t blocks_y = std::min<int64_t>({r.rows, std::max<int64_t>(1, 148 * kActPerSm * 256 / threads / parts), 65535});

@@ -465,6 +465,8 @@ struct Int4LinearArgs {
   DType scale_type, bias_type, out_type;
   int* err;
 };
+// codes uint8 [n, k / 2] (row stride ld) -> packed
+void launch_int4_pack(void* packed, const uint8_t* codes, int64_t n, int64_t k, int64_t ld, cudaStream_t s);
 void launch_int4_gemm(const Int4LinearArgs& a, cudaStream_t s);  // int4_gemm.cu
 void launch_int4_linear(const Int4LinearArgs& a, cudaStream_t s);
 

@@ -96,6 +96,26 @@ def _tile_rows(t: torch.Tensor, groups: int) -> torch.Tensor:
     return full.view(tiles, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
 
 
+def _pack_reference(codes: torch.Tensor) -> torch.Tensor:
+    """The layout's statement: codes [N, K / 2] -> packed [tiles, blocks, 512]."""
+    n, k = codes.shape[0], 2 * codes.shape[1]
+    tiles, blocks = _tiles(n), 2 * -(-k // _STEP)
+    if tiles * _TILE != n or blocks * _BLOCK != k:
+        full = codes.new_zeros(tiles * _TILE, blocks * _BLOCK // 2)
+        full[:n, : k // 2] = codes
+    else:
+        full = codes
+    # byte b of a row holds columns 2b (e = 0) and 2b + 1 (e = 1): [tile, h, g, block, j, t, p]
+    c = full.view(tiles, 2, 8, blocks, 4, 4, 2).permute(1, 0, 3, 2, 5, 4, 6)  # [h, tile, block, g, t, j, p]
+    top, low = c[0], c[1]
+    # bytes of a word: (e, p) from the lowest; the nibbles of a byte: h
+    packed = torch.empty(tiles, blocks, 8, 4, 4, 2, 2, dtype=torch.uint8, device=codes.device)
+    packed[..., 0, :] = (top & 15) | (low << 4)
+    packed[..., 1, :] = (top >> 4) | (low & 0xF0)
+    packed ^= 0x88  # c - 8, two's complement
+    return packed.view(tiles, blocks, 512)
+
+
 def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
                 group: int = 128) -> Int4Weight:
     """``codes`` uint8 [N, K / 2] (column 2i in the low nibble of byte i),
@@ -117,20 +137,14 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
         raise ValueError("int4_weight: codes, scales and zeros must be on one device")
     if zeros is not None and bool((zeros > 15).any()):
         raise ValueError("int4_weight: zero points must be 0..15")
-    tiles, blocks = _tiles(n), 2 * -(-k // _STEP)
-    if tiles * _TILE != n or blocks * _BLOCK != k:
-        full = codes.new_zeros(tiles * _TILE, blocks * _BLOCK // 2)
-        full[:n, : k // 2] = codes
+    if codes.is_cuda:
+        from minisgl import ops
+
+        ops._count()
+        packed = ops.native().int4_pack(codes if codes.stride(1) == 1 else codes.contiguous())
     else:
-        full = codes
-    # byte b of a row holds columns 2b (e = 0) and 2b + 1 (e = 1): [tile, h, g, block, j, t, p]
-    c = full.view(tiles, 2, 8, blocks, 4, 4, 2).permute(1, 0, 3, 2, 5, 4, 6)  # [h, tile, block, g, t, j, p]
-    top, low = c[0], c[1]
-    # bytes of a word: (e, p) from the lowest; the nibbles of a byte: h
-    packed = torch.empty(tiles, blocks, 8, 4, 4, 2, 2, dtype=torch.uint8, device=codes.device)
-    packed[..., 0, :] = (top & 15) | (low << 4)
-    packed[..., 1, :] = (top >> 4) | (low & 0xF0)
-    packed ^= 0x88  # c - 8, two's complement
+        packed = _pack_reference(codes)
+    blocks = packed.shape[1]
     groups = blocks * _BLOCK // group
     z = None
     if zeros is not None:
@@ -140,7 +154,7 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
     top = tiled.float().abs().amax(1).transpose(1, 2).reshape(-1)  # [tile, g, h] -> row
     live = (top > 0) & (top <= torch.finfo(torch.float32).max)
     row_pow = torch.where(live, torch.exp2(torch.floor(torch.log2(torch.where(live, top, 1.0)))), 1.0)
-    return Int4Weight(packed.view(tiles, blocks, 512), tiled, z, row_pow, n, k, group)
+    return Int4Weight(packed, tiled, z, row_pow, n, k, group)
 
 
 def int4_codes(w: Int4Weight) -> torch.Tensor:

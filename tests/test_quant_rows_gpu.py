@@ -8,6 +8,7 @@ import torch
 from minisgl import ops
 from minisgl.ops import reference as ref
 from minisgl.quant import dequantize_int4, dequantize_mx8_rows, int4_weight, quantize_int4
+from minisgl.quant.int4 import _pack_reference
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -197,6 +198,17 @@ def _check_linear(y, xd, w, bias, rounded=False):
         room = room + size * 2 ** -8
     err = (y.double() - want).abs()
     assert bool((err <= room).all()), (err / room).max().item()
+
+
+@pytest.mark.parametrize("n,k", [(1, 8), (16, 64), (17, 72), (100, 1096), (33, 256), (2048, 1024)])
+def test_int4_pack(n, k):
+    """The kernel's layout against its statement; rows of a wider tensor too."""
+    codes = torch.randint(0, 256, (n, k // 2), generator=_gen(n), device=DEV, dtype=torch.uint8)
+    want = _pack_reference(codes.cpu())
+    assert torch.equal(ops.native().int4_pack(codes).cpu(), want)
+    wide = torch.full((n, k // 2 + 24), 0x5A, device=DEV, dtype=torch.uint8)
+    wide[:, 3:3 + k // 2] = codes
+    assert torch.equal(ops.native().int4_pack(wide[:, 3:3 + k // 2]).cpu(), want)
 
 
 SHAPES = [(1, 16, 64), (1, 2048, 1024), (3, 17, 8), (8, 33, 72), (9, 128, 4168), (16, 1000, 512), (17, 256, 640),
