@@ -651,10 +651,6 @@ at::Tensor int4_linear(const at::Tensor& x, const Int4Handle& w, const c10::opti
     a.x_scales = x_scales->data_ptr<uint8_t>();
     a.ld_xs = x_scales->stride(0);
     a.x_type = DType::kBF16;
-    if (M > minisgl::kInt4FewRows) {  // MXFP8 rows widened to bf16 for the tensor cores' tiles
-      x_wide = at::empty({M, K}, x.options().dtype(at::kBFloat16));
-      a.x_wide = x_wide.data_ptr();
-    }
   } else {
     MSG_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
               "int4_linear: x must be bfloat16 or float16 (or MXFP8 rows with x_scales)");
@@ -695,7 +691,14 @@ at::Tensor int4_linear(const at::Tensor& x, const Int4Handle& w, const c10::opti
   a.scale_type = dtype_of(w.scales);
   a.out_type = dtype_of(out);
   a.err = err_ptr(w.err);
-  minisgl::launch_int4_linear(a, stream_of(x));
+  if (M == 0) return out;
+  if (!minisgl::launch_int4_stream(a, stream_of(x))) {
+    if (x_scales.has_value()) {  // MXFP8 rows are widened to bf16 for the tensor cores' tiles
+      x_wide = at::empty({M, K}, x.options().dtype(at::kBFloat16));
+      a.x_wide = x_wide.data_ptr();
+    }
+    minisgl::launch_int4_gemm(a, stream_of(x));
+  }
   return out;
 }
 

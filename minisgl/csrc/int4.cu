@@ -336,7 +336,9 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
 
   // x as 24-bit integers [row][step][digit][columns]: a row's 128 columns under a power of two that puts their
   // largest value into [2^21, 2^22), rounded to nearest: exact for what lies above 2^-14 of it (bf16; fp16
-  // 2^-11, E4M3 2^-18), else at most 2^-22 of it off, as much as a rounding of a float32 sum
+  // 2^-11, E4M3 2^-18), else at most 2^-22 of it off: what one rounding of a float32 sum that holds the largest
+  // value costs. The power stops at 2^122: a block below 2^-101 keeps an absolute 2^-123. Two digits would do for
+  // bf16 results beside moderate outliers, three keep float32 results right.
   bool odd = false;  // met an infinity or NaN
   const int batches = (a.M * per_row + kBatch * W * 32 - 1) / (kBatch * W * 32);
 #pragma unroll 1
@@ -759,29 +761,24 @@ void launch_int4_pack(void* out, const uint8_t* codes, int64_t n, int64_t k, int
              codes, n, k / 2, ld, blocks, total);
 }
 
-void launch_int4_linear(const Int4LinearArgs& r, cudaStream_t s) {
-  if (r.M <= 0) return;
-  if (r.M > 65535 * 32 || r.N > (1ll << 30) || r.K > (1ll << 30))
-    throw std::runtime_error("minisgl.int4_linear: size out of range");
-  if (r.M <= kInt4FewRows) {
-    VecArgs v{};
-    v.x = r.x, v.x_scales = r.x_scales, v.packed = r.packed;
-    v.scales = static_cast<const uint32_t*>(r.scales), v.zeros = r.zeros, v.bias = r.bias, v.out = r.out;
-    v.M = static_cast<int>(r.M), v.N = static_cast<int>(r.N), v.K = static_cast<int>(r.K);
-    v.steps = (v.K + 127) / 128;
-    v.ldx = r.ldx, v.ld_xs = r.ld_xs, v.ldo = r.ldo;
-    v.ld_z = static_cast<int>((v.steps * (128 / r.group) + 1) / 2 * 16);
-    v.scale_half = r.scale_type == DType::kF16;
-    v.bias_type = static_cast<int>(r.bias_type), v.out_type = static_cast<int>(r.out_type);
-    v.x_kind = r.x_scales != nullptr ? kXMx8 : r.x_type == DType::kF16 ? kXHalf : kXBf16;
-    // Few codes (up to kSmallSteps KB): CTAs of 8 warps, two of which fit an SM, so that the next kernel's start
-    // overlaps this one's end; more: one CTA of 16 warps, which stages x once per SM. B200, one row: 4096 x 4096
-    // 7.6 us against 8.7, 2048 x 1024 4.1 against 5.1; 12301 x 4168 18.4 against 16.0, 5120 x 25600 30.2 against 19.0.
-    constexpr int64_t kSmallSteps = 12 * 1024;
-    const bool small = (static_cast<int64_t>(v.N) + 15) / 16 * v.steps <= kSmallSteps;
-    if ((small && launch_vec_group<8>(v, r.group, s)) || launch_vec_group<16>(v, r.group, s)) return;
-  }
-  launch_int4_gemm(r, s);
+bool launch_int4_stream(const Int4LinearArgs& r, cudaStream_t s) {
+  if (r.M > kInt4FewRows) return false;
+  VecArgs v{};
+  v.x = r.x, v.x_scales = r.x_scales, v.packed = r.packed;
+  v.scales = static_cast<const uint32_t*>(r.scales), v.zeros = r.zeros, v.bias = r.bias, v.out = r.out;
+  v.M = static_cast<int>(r.M), v.N = static_cast<int>(r.N), v.K = static_cast<int>(r.K);
+  v.steps = (v.K + 127) / 128;
+  v.ldx = r.ldx, v.ld_xs = r.ld_xs, v.ldo = r.ldo;
+  v.ld_z = static_cast<int>((v.steps * (128 / r.group) + 1) / 2 * 16);
+  v.scale_half = r.scale_type == DType::kF16;
+  v.bias_type = static_cast<int>(r.bias_type), v.out_type = static_cast<int>(r.out_type);
+  v.x_kind = r.x_scales != nullptr ? kXMx8 : r.x_type == DType::kF16 ? kXHalf : kXBf16;
+  // Few codes (up to kSmallSteps KB): CTAs of 8 warps, two of which fit an SM, so that the next kernel's start
+  // overlaps this one's end; more: one CTA of 16 warps, which stages x once per SM. B200, one row: 4096 x 4096
+  // 7.6 us against 8.7, 2048 x 1024 4.1 against 5.1; 12301 x 4168 18.4 against 16.0, 5120 x 25600 30.2 against 19.0.
+  constexpr int64_t kSmallSteps = 12 * 1024;
+  const bool small = (static_cast<int64_t>(v.N) + 15) / 16 * v.steps <= kSmallSteps;
+  return (small && launch_vec_group<8>(v, r.group, s)) || launch_vec_group<16>(v, r.group, s);
 }
 
 }  // namespace minisgl

@@ -666,6 +666,12 @@ void launch_group(const GArgs& a, const void* scales, const void* x, int64_t ldx
 }  // namespace
 
 void launch_int4_gemm(const Int4LinearArgs& r, cudaStream_t s) {
+  if (r.M <= 0) return;
+  if ((r.M + 31) / 32 * ((r.N + kRows - 1) / kRows) >= (1ll << 31) || r.M >= (1ll << 31) || r.N > (1ll << 30) ||
+      r.K > (1ll << 30))
+    throw std::runtime_error("minisgl.int4_linear: size out of range");
+  if (r.x_scales != nullptr && r.x_wide == nullptr)
+    throw std::runtime_error("minisgl.int4_linear: scratch for the widened rows is missing");
   GArgs a{};
   a.packed = r.packed, a.zeros = r.zeros, a.row_pow = r.row_pow;
   a.bias = r.bias, a.out = r.out;

@@ -456,7 +456,7 @@ struct Int4LinearArgs {
   const uint8_t* zeros;     // [tiles, groups rounded up to even, 8] or nullptr (8 everywhere)
   const float* row_pow;     // [16 tiles]: a power of two near each row's largest scale
   const void* bias;         // [N] or nullptr
-  void* x_wide;             // more than kInt4FewRows E4M3 rows: bf16 [M, K] scratch
+  void* x_wide;             // launch_int4_gemm with E4M3 rows: bf16 [M, K] scratch
   void* out;                // [M, N], row stride ldo
   int64_t M, N, K;
   int64_t ldx, ld_xs, ldo;
@@ -467,7 +467,9 @@ struct Int4LinearArgs {
 };
 // codes uint8 [n, k / 2] (row stride ld) -> packed
 void launch_int4_pack(void* packed, const uint8_t* codes, int64_t n, int64_t k, int64_t ld, cudaStream_t s);
-void launch_int4_gemm(const Int4LinearArgs& a, cudaStream_t s);  // int4_gemm.cu
-void launch_int4_linear(const Int4LinearArgs& a, cudaStream_t s);
+// false (nothing launched): more than kInt4FewRows rows, or too many columns for x to fit shared memory
+bool launch_int4_stream(const Int4LinearArgs& a, cudaStream_t s);
+// any number of rows; E4M3 rows need x_wide
+void launch_int4_gemm(const Int4LinearArgs& a, cudaStream_t s);
 
 }  // namespace minisgl

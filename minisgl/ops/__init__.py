@@ -357,11 +357,12 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
     ``quantize_int4``). x [M, K] is bf16 or fp16, or MXFP8 rows: uint8 E4M3
     bits with ``x_scales`` [M, K / 32], as ``rmsnorm_mx8`` and
     ``silu_and_mul_mx8`` return them. out: bf16, fp16 or fp32 (default: x's
-    type, bf16 for MXFP8 rows). Sums are held in fp32 or
-    exact integers, whatever the number of rows; products of more than 8 rows
-    take the weight rounded once to x's 16-bit type."""
+    type, bf16 for MXFP8 rows). Products of up to 8
+    rows sum exact integers (x as 22-bit integers under a power of two common
+    to 128 columns) and groups in fp32; longer batches sum fp32 products of
+    the weight rounded once to x's 16-bit type."""
     if x.is_cuda:
-        _count(2 if x_scales is not None and x.shape[0] > 8 else 1)  # MXFP8 rows of a long batch are widened first
+        _count(2 if x_scales is not None and x.shape[0] > 8 else 1)  # the MXFP8 rows of a long batch are widened first
         return native().int4_linear(x, w.native(), bias, out, out_dtype, x_scales)
     if x.dim() != 2 or x.shape[1] != w.k:
         raise ValueError(f"int4_linear: x must be [M, {w.k}], got {tuple(x.shape)}")

@@ -77,6 +77,9 @@ class Int4Weight:
                                                    self.group, ops.error_word(self.device))
         return self._handle
 
+    def __reduce__(self):
+        return Int4Weight, (self.packed, self.scales, self.zeros, self.row_pow, self.n, self.k, self.group)
+
     @property
     def device(self) -> torch.device:
         return self.packed.device
@@ -153,8 +156,12 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
     tiled = _tile_rows(scales, groups)
     top = tiled.float().abs().amax(1).transpose(1, 2).reshape(-1)  # [tile, g, h] -> row
     live = (top > 0) & (top <= torch.finfo(torch.float32).max)
-    row_pow = torch.where(live, torch.exp2(torch.floor(torch.log2(torch.where(live, top, 1.0)))), 1.0)
-    return Int4Weight(packed, tiled, z, row_pow, n, k, group)
+    power = (top.view(torch.int32) & 0x7F800000).view(torch.float32)  # the exponent's bits alone
+    row_pow = torch.where(live & (power > 0), power, 1.0)
+    w = Int4Weight(packed, tiled, z, row_pow, n, k, group)
+    if codes.is_cuda:
+        w.native()  # checked and registered here, not inside somebody's graph capture
+    return w
 
 
 def int4_codes(w: Int4Weight) -> torch.Tensor:

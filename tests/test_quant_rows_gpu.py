@@ -431,3 +431,96 @@ def test_int4_linear_many_tiles(m, n, k, dt):
     x = torch.randn(m, k, generator=_gen(m), device=DEV).to(t)
     _check_linear(ops.int4_linear(x, w), x.double(), w, None, rounded=True)
     ops.check_device_errors(torch.device(DEV))
+
+
+@pytest.mark.parametrize("m,k", [(8, 40000), (3, 100000), (1, 300000)])
+@pytest.mark.parametrize("kind", ["bf16", "mx8"])
+def test_int4_linear_few_rows_too_wide_to_stream(m, k, kind):
+    """Rows that shared memory cannot hold take the tiles of the longer batches."""
+    w = _weight(48, k, 128, True, m, torch.bfloat16)
+    x = torch.randn(m, k, generator=_gen(k), device=DEV)
+    if kind == "mx8":
+        q = torch.randint(0, 0x7E, (m, k), generator=_gen(k), device=DEV, dtype=torch.uint8)
+        sf = torch.randint(118, 124, (m, k // 32), generator=_gen(m), device=DEV, dtype=torch.uint8)
+        _check_linear(ops.int4_linear(q, w, x_scales=sf), dequantize_mx8_rows(q, sf, torch.float64), w, None, rounded=True)
+    else:
+        x = x.to(torch.bfloat16)
+        _check_linear(ops.int4_linear(x, w), x.double(), w, None, rounded=True)
+    ops.check_device_errors(torch.device(DEV))
+
+
+@pytest.mark.parametrize("m", [2, 12])
+def test_int4_linear_wide_range_of_x(m):
+    """Magnitudes from one end of bf16 to the other, in columns of their own and beside one another; every group
+    has weights other than its zero point under its largest x, so the sum is as large as its terms."""
+    w = _weight(64, 1024, 64, False, 2, torch.bfloat16)
+    x = torch.randn(m, 1024, generator=_gen(9), device=DEV)
+    x[:, :128] *= 1e30
+    x[:, 128:256] *= 1e-30
+    x[:, 256:384] *= torch.logspace(-20, 20, 128, device=DEV)
+    x[0] *= 1e-5
+    x = x.to(torch.bfloat16)
+    y = ops.int4_linear(x, w, out_dtype=torch.float32)
+    wd = dequantize_int4(w, torch.float64)
+    want, size = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    # x's integers: at most half a unit off each. The unit is 2^-21 of the largest value's power of two, but never
+    # below 2^-122, because its inverse is a float32 factor (2^122) and the factor that undoes it and the codes'
+    # sixteenths, 2^-126, has to be normal.
+    def half_units(z, weights):
+        top = z.double().abs().view(m, -1, 128).amax(-1)
+        return torch.einsum("mb,nb->mn", (top * 2 ** -22).clamp(min=2.0 ** -123), weights.abs().view(64, -1, 128).sum(-1))
+
+    fixed = half_units(x, wd)
+    room = size * (68 + 1024 / 64 + 20) * 2 ** -23 + want.abs() * 2 ** -24 + (fixed if m <= 8 else size * 2 ** -8)
+    assert bool(((y.double() - want).abs() <= room).all())
+    if m <= 8:  # tiny and huge alone
+        for cols in (slice(0, 128), slice(128, 256)):
+            z = torch.zeros_like(x)
+            z[:, cols] = x[:, cols]
+            got, ref_ = ops.int4_linear(z, w, out_dtype=torch.float32).double(), z.double() @ wd.t()
+            s = z.double().abs() @ wd.abs().t()
+            assert bool(((got - ref_).abs() <= s * 104 * 2 ** -23 + half_units(z[:, cols], wd[:, cols]) + 1e-45).all())
+
+
+def test_int4_linear_nan_block_of_mx8():
+    w = _weight(40, 256, 32, True, 6, torch.bfloat16)
+    for m in (2, 20):
+        q, sf = ops.rmsnorm_mx8(torch.randn(m, 256, generator=_gen(1), device=DEV), None, 1e-6)
+        q[1, 32:64], sf[1, 1] = 0x7F, 255
+        y = ops.int4_linear(q, w, x_scales=sf)
+        assert y[1].isnan().all() and y[0].isfinite().all() and y[2:].isfinite().all()
+
+
+@pytest.mark.parametrize("scale", [1e-7, 6e-5, 3e4])
+def test_int4_linear_fp16_scales_at_the_ends(scale):
+    """Tiny and large fp16 scales: the products of longer batches take each row's power of two out."""
+    g = _gen(3)
+    codes = torch.randint(0, 256, (64, 256), generator=g, device=DEV, dtype=torch.uint8)
+    scales = (scale * (1 + torch.rand(64, 4, generator=g, device=DEV))).to(torch.float16)
+    w = int4_weight(codes, scales, None, 128)
+    for m in (4, 40):
+        x = (torch.randn(m, 512, generator=g, device=DEV) * 1e-3).to(torch.float16)
+        _check_linear(ops.int4_linear(x, w, out_dtype=torch.float32), x.double(), w, None, rounded=m > 8)
+
+
+@pytest.mark.parametrize("m,group", [(1, 64), (7, 32), (200, 64), (30, 32)])
+def test_first_call_inside_a_capture(m, group):
+    """A variant's first call may be captured: nothing of its set-up is a stream operation."""
+    w = _weight(704, 1152, group, True, m, torch.float16)
+    x = torch.randn(m, 1152, generator=_gen(m), device=DEV).to(torch.float16)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.int4_linear(x, w)
+    graph.replay()
+    torch.cuda.synchronize()
+    _check_linear(y, x.double(), w, None, rounded=m > 8)
+
+
+def test_weight_copies():
+    import copy
+
+    w = _weight(32, 128, 32, True, 1, torch.bfloat16)
+    x = torch.randn(3, 128, generator=_gen(1), device=DEV).to(torch.bfloat16)
+    assert torch.equal(ops.int4_linear(x, copy.deepcopy(w)), ops.int4_linear(x, w))
+    assert torch.equal(ops.int4_linear(x, w.to("cpu").to(DEV)), ops.int4_linear(x, w))
