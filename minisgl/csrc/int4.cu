@@ -2,14 +2,9 @@
 //   out[m, n] = sum_k x[m, k] (c[n, k] - z[n, k / G]) s[n, k / G] (+ bias[n])
 // for few rows x (decode batches). Weight layout: minisgl/quant/int4.py.
 //
-// The weights are read once and dominate the bytes, so a tile of them goes
-// straight from memory to the registers of the lane that multiplies it: 16
-// bytes per lane are 16 rows x 64 columns per warp, already in the order of
-// the first operand of the warp-level 16 x 8 x 16 product. x is the second
-// operand (8 rows of x per product). Codes become exact bf16 / fp16 integers
-// (a nibble under the exponent of 128 / 1024, minus 128 / 1024 + z), are
-// multiplied exactly and summed in float32 over at most 64 columns; only then
-// is the group's scale applied, in float32.
+// The weights are read once and dominate the bytes: 16 bytes per lane are 16
+// rows x 64 columns per warp, already in the order of the first operand of the
+// warp-level 16 x 8 x 32 integer product; x (up to 8 rows) is the second.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -51,8 +46,8 @@ __device__ __forceinline__ float e8m0(uint32_t byte) {
 // ---------------------------------------------------------------------------
 // Few rows (up to 8, one operand of a warp-level product): the weight stream.
 //
-// A unit is kR tiles of 16 rows x 128 columns (kR KB of codes and their scales).
-// Whole tiles are dealt to clusters of S = 1 to 8 CTAs, whose CTAs share
+// A unit is kR tiles (1 or 2) of 16 rows x 128 columns: kR KB of codes and their
+// scales. Whole tiles are dealt to clusters of S = 1 to 8 CTAs, whose CTAs share
 // the columns; the units of a CTA, tile after tile, are cut into one contiguous
 // range per warp. Each warp copies its own units into its own ring of shared
 // memory (cp.async, kDepth ahead), waits for them alone and multiplies them;
@@ -73,10 +68,21 @@ __device__ __forceinline__ float e8m0(uint32_t byte) {
 // S > 1 finished tiles go to the shared memory of the CTA that owns them and
 // are added in rank order after a cluster barrier. Every sum has a fixed order:
 // the same inputs give the same bits.
+//
+// Measured (B200, cold weights, bf16): 1 x 51200 x 5120 in groups of 128 29.9 us
+// (4.5 TB/s; a plain read of the bytes 20.6), 1 x 5120 x 25600 19.6, 8 x 5120 x
+// 25600 with zero points 24.9, 1 x 5120 x 5120 7.3. What bounds it is the issue of
+// instructions (some 120 a KB of codes, 1.7 a cycle and SM) and, in small calls,
+// about 4 us of launch, staging of x and the joins; deeper rings, 20 or 24 warps
+// and two batches of x in flight measured no better.
 // ---------------------------------------------------------------------------
 constexpr int kDepth = 3;
-constexpr int kR = 2;    // 16-row tiles of a unit: their products share the reads of x
 constexpr int kMaxSmem = 227 * 1024;
+// of a CTA of W warps, 16 of which share an SM: the SM's 228 KB less 1 KB of the system's a CTA
+template <int W>
+constexpr int kCtaSmem = 228 * 1024 * W / 16 - 1024;
+static_assert(kCtaSmem<16> == kMaxSmem);
+constexpr int kBatch = 4;  // runs of 8 values of x that a thread converts side by side
 
 enum { kXBf16 = 0, kXHalf = 1, kXMx8 = 2 };
 struct VecArgs {
@@ -98,7 +104,7 @@ struct VecArgs {
   int recv_slots;  // tiles that a CTA owns at most (S > 1)
 };
 
-template <int W, int G, bool ZERO>
+template <int W, int kR, int G, bool ZERO>
 struct VecSmem {
   static constexpr int kGroups = 128 / G;
   static constexpr int kScaleB = kGroups * 32;  // of one tile
@@ -107,9 +113,6 @@ struct VecSmem {
   static constexpr int kRing = W * kDepth * kUnit;
   // per step: each row's power of two and, with zero points, each group's sum in two parts
   static constexpr int kSide = 32 + (ZERO ? 64 * kGroups : 0);
-  static int total(int x_bytes, int recv_slots, int S) {
-    return kRing + (W * 2 + recv_slots * S) * 512 * kR + x_bytes;
-  }
 };
 // bytes between x's rows (three digits of 128 columns a step): an odd
 // multiple of 64, so that the eight 16-byte reads of a quarter warp (two rows
@@ -229,9 +232,9 @@ __device__ __forceinline__ void store_sum(const VecArgs& a, int64_t tile, int r,
   store_from_f32(a.out, m * a.ldo + n, a.out_type, v);
 }
 
-template <int W, int G, bool ZERO>
+template <int W, int kR, int G, bool ZERO>
 __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs a) {
-  using L = VecSmem<W, G, ZERO>;
+  using L = VecSmem<W, kR, G, ZERO>;
   constexpr int P = L::kGroups;  // groups of a unit
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -262,10 +265,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
   // the codes of the warp's first units, on their way to L2 while the kernel before this one ends (a prefetch
   // carries no value: the copies below read memory after griddepcontrol.wait)
   {
-    const int ahead = k + (lane >> 4);  // the units run on through the tile, then in the next
-    if (u0 + (lane >> 4) < u1) {
+    constexpr int kLanes = 8 * kR;  // of a unit: a 128-byte line each
+    const int ahead = k + lane / kLanes;  // the units run on through the tile, then in the next
+    if (u0 + lane / kLanes < u1) {
       const int on = ahead >= ks ? by_ks(ahead) : 0;
-      const int64_t row16 = static_cast<int64_t>(tile + on) * kR + (lane >> 3 & 1);
+      const int64_t row16 = static_cast<int64_t>(tile + on) * kR + (lane >> 3 & (kR - 1));
       asm volatile("prefetch.global.L2 [%0];" ::"l"(a.packed + (row16 * a.steps + k0 + ahead - on * ks) * 1024 + (lane & 7) * 128));
     }
   }
@@ -312,7 +316,6 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int4_vec_kernel(const VecArgs 
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // the first of x's loads go ahead of the weights', which they would else queue behind
-  constexpr int kBatch = 4;
   uint4 ahead[kBatch];
   // run c of row m: a warp's 32 runs are of one row or (ks odd) of two neighbours
   const int per_row = ks * 16;
@@ -639,8 +642,10 @@ __global__ void __launch_bounds__(256) int4_pack_kernel(uint4* out, const uint8_
   out[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// How a call is cut up: warps of a CTA, tiles of 16 rows that a unit holds, CTAs that share a tile's columns.
 struct VecPlan {
-  int S, clusters, x_bytes, recv_slots, smem;
+  int W, R, S, clusters, tiles, x_bytes, recv_slots, smem;
+  int64_t cost;
 };
 
 // Per device and kernel: its shared-memory limit raised, and how many clusters of each size fit at once.
@@ -662,7 +667,7 @@ int resident_clusters(int S) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(S);
     cfg.blockDim = dim3(W * 32);
-    cfg.dynamicSmemBytes = kMaxSmem / (16 / W);
+    cfg.dynamicSmemBytes = kCtaSmem<W>;
     cudaLaunchAttribute at2;
     at2.id = cudaLaunchAttributeClusterDimension;
     at2.val.clusterDim.x = S;
@@ -677,40 +682,50 @@ int resident_clusters(int S) {
   return n;
 }
 
-// The cluster size whose busiest CTA has the least to stream: whole tiles
-// are dealt to clusters, so many tiles balance alone (S = 1) and few tiles only
-// when their columns are shared. A cluster's two barriers and exchange cost
-// about as much as kClusterCost KB. False: x does not fit shared memory.
-constexpr int kClusterCost = 100;
-template <typename L, auto kern, int W>
-bool vec_plan(const VecArgs& a, VecPlan& best) {
-  int64_t best_cost = -1;
-  for (int S = 1; S <= 8; ++S) {
-    if (S > a.steps) break;
-    VecPlan p;
-    p.S = S;
-    p.clusters = std::min(resident_clusters<kern, W>(S), a.tiles);
-    const int per = (a.tiles + p.clusters - 1) / p.clusters, ks = (a.steps + S - 1) / S;
-    const int64_t x_bytes = static_cast<int64_t>(a.M) * vec_x_pitch(ks) + static_cast<int64_t>(ks) * L::kSide;
-    if (x_bytes > kMaxSmem) continue;
-    p.x_bytes = static_cast<int>(x_bytes);
-    p.recv_slots = S > 1 ? (per + S - 1) / S : 0;
-    if (p.recv_slots > 4096) continue;
-    p.smem = L::total(p.x_bytes, p.recv_slots, S);
-    if (p.smem > kMaxSmem / (16 / W) || static_cast<int64_t>(per) * ks > (1 << 30) / a.steps) continue;  // n * ks stays below 2^31: the reciprocals are exact
-    const int64_t cost = static_cast<int64_t>(per) * ks * kR + (S > 1 ? kClusterCost : 0);
-    if (best_cost < 0 || cost < best_cost) best_cost = cost, best = p;
+// Estimated time of a call under each plan, in hundredths of what a CTA of 16 warps takes to stream a KB of codes
+// (about 0.035 us); fitted to 68 sizes under every plan (B200, cold weights), where the chosen plan is 2.4% slower
+// than the best one in the geometric mean and at worst 27%. Both sides of each choice, one of its sizes:
+//  - 8 warps, two CTAs to an SM (the next kernel's start overlaps this one's end, few tiles spread further)
+//    against 16 (x is staged once per SM): 1 x 2048 x 1024 3.9 against 5.7 us; 8 x 25600 x 5120 27.9 against 24.3.
+//  - one 16-row tile to a unit (finer shares of the work) against two (x is read once for both): 1 x 10240 x 5120
+//    9.9 against 11.0 us; 2 x 28672 x 4096 with zero points, whose sums are x's too, 19.9 against 17.8.
+//  - columns shared by a cluster (less of x to stage, even shares of few tiles) against whole tiles: 6 x 7168 x 7168
+//    12.5 (4 CTAs) against 14.6 us; 1 x 28672 x 640 8.1 (2 CTAs) against 6.7. Clusters of 3, 5, 6 and 7 CTAs lost
+//    against their neighbours (8 x 14336 x 5120: 5 CTAs 20.7, 4 CTAs 16.2, 8 CTAs 18.1): only powers of two.
+constexpr int64_t kCostKb = 100, kCostOneTile = 5, kCostOneTileZeros = 20, kCostXStep = 40, kCostXBatch = 3000,
+                  kCostCluster = 8000, kCostClusterCta = 400, kCostWide = 1000, kCostTwoTiles = 3200;
+template <int W, int kR, int G, bool ZERO>
+void vec_plan(const VecArgs& a, VecPlan& best) {
+  using L = VecSmem<W, kR, G, ZERO>;
+  constexpr int kPerSm = 16 / W;
+  VecPlan p;
+  p.W = W, p.R = kR;
+  p.tiles = (a.N + 16 * kR - 1) / (16 * kR);
+  for (p.S = 1; p.S <= std::min(8, a.steps); p.S *= 2) {
+    const int slots = resident_clusters<int4_vec_kernel<W, kR, G, ZERO>, W>(p.S);
+    p.clusters = std::min(slots, p.tiles);
+    const int64_t per = (p.tiles + p.clusters - 1) / p.clusters, ks = (a.steps + p.S - 1) / p.S;
+    const int64_t x_bytes = a.M * static_cast<int64_t>(vec_x_pitch(static_cast<int>(ks))) + ks * L::kSide;
+    const int64_t recv_slots = p.S > 1 ? (per + p.S - 1) / p.S : 0;
+    const int64_t smem = L::kRing + (W * 2 + recv_slots * p.S) * 512 * kR + x_bytes;
+    // n * ks stays below 2^31: the reciprocals are exact
+    if (smem > kCtaSmem<W> || per * ks > (1 << 30) / a.steps) continue;
+    p.x_bytes = static_cast<int>(x_bytes), p.recv_slots = static_cast<int>(recv_slots), p.smem = static_cast<int>(smem);
+    const int sms = std::max(1, slots / kPerSm);  // clusters side by side with one CTA to an SM
+    const int64_t on_sm = std::min(kPerSm, (p.clusters + sms - 1) / sms);
+    int64_t kb = (per * ks + W - 1) / W * W * kR;  // of a CTA whose warps all take the longest share
+    if (kPerSm > 1) kb = std::max(kb, (p.tiles + sms - 1) / sms * ks * kR);
+    const int64_t x_batches = (a.M * ks * 16 + kBatch * W * 32 - 1) / (kBatch * W * 32);
+    p.cost = kb * (kCostKb + (kR == 1 ? kCostOneTile + (ZERO ? kCostOneTileZeros : 0) : 0)) +
+             on_sm * (a.M * ks * kCostXStep + x_batches * kCostXBatch / kPerSm) +
+             (p.S > 1 ? kCostCluster + p.S * kCostClusterCta : 0) + (W == 16 ? kCostWide : 0) + (kR == 2 ? kCostTwoTiles : 0);
+    if (best.S == 0 || p.cost < best.cost) best = p;
   }
-  return best_cost >= 0;
 }
 
-template <int W, int G, bool ZERO>
-bool launch_vec(VecArgs a, cudaStream_t s) {
-  constexpr auto kern = int4_vec_kernel<W, G, ZERO>;
-  using L = VecSmem<W, G, ZERO>;
-  a.tiles = (a.N + 16 * kR - 1) / (16 * kR);
-  VecPlan p;
-  if (!vec_plan<L, kern, W>(a, p)) return false;
+template <int W, int kR, int G, bool ZERO>
+void launch_vec(VecArgs a, const VecPlan& p, cudaStream_t s) {
+  a.tiles = p.tiles;
   a.S = p.S;
   a.tiles_each = a.tiles / p.clusters, a.tiles_more = a.tiles % p.clusters;
   a.steps_each = a.steps / p.S, a.steps_more = a.steps % p.S;
@@ -737,19 +752,24 @@ bool launch_vec(VecArgs a, cudaStream_t s) {
   }
   cfg.attrs = attrs;
   cfg.numAttrs = n;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, int4_vec_kernel<W, kR, G, ZERO>, a);
   if (e != cudaSuccess) throw std::runtime_error(std::string("minisgl: kernel launch failed: ") + cudaGetErrorString(e));
-  return true;
 }
 
-template <int W>
-bool launch_vec_group(const VecArgs& a, int group, cudaStream_t s) {
-  const bool z = a.zeros != nullptr;
-  switch (group) {
-    case 32: return z ? launch_vec<W, 32, true>(a, s) : launch_vec<W, 32, false>(a, s);
-    case 64: return z ? launch_vec<W, 64, true>(a, s) : launch_vec<W, 64, false>(a, s);
-    default: return z ? launch_vec<W, 128, true>(a, s) : launch_vec<W, 128, false>(a, s);
-  }
+// false: x does not fit shared memory under any plan
+template <int G, bool ZERO>
+bool launch_vec_group(const VecArgs& a, cudaStream_t s) {
+  VecPlan p{};
+  vec_plan<8, 1, G, ZERO>(a, p);
+  vec_plan<8, 2, G, ZERO>(a, p);
+  vec_plan<16, 1, G, ZERO>(a, p);
+  vec_plan<16, 2, G, ZERO>(a, p);
+  if (p.S == 0) return false;
+  if (p.W == 8)
+    p.R == 1 ? launch_vec<8, 1, G, ZERO>(a, p, s) : launch_vec<8, 2, G, ZERO>(a, p, s);
+  else
+    p.R == 1 ? launch_vec<16, 1, G, ZERO>(a, p, s) : launch_vec<16, 2, G, ZERO>(a, p, s);
+  return true;
 }
 
 }  // namespace
@@ -773,12 +793,12 @@ bool launch_int4_stream(const Int4LinearArgs& r, cudaStream_t s) {
   v.scale_half = r.scale_type == DType::kF16;
   v.bias_type = static_cast<int>(r.bias_type), v.out_type = static_cast<int>(r.out_type);
   v.x_kind = r.x_scales != nullptr ? kXMx8 : r.x_type == DType::kF16 ? kXHalf : kXBf16;
-  // Few codes (up to kSmallSteps KB): CTAs of 8 warps, two of which fit an SM, so that the next kernel's start
-  // overlaps this one's end; more: one CTA of 16 warps, which stages x once per SM. B200, one row: 4096 x 4096
-  // 7.6 us against 8.7, 2048 x 1024 4.1 against 5.1; 12301 x 4168 18.4 against 16.0, 5120 x 25600 30.2 against 19.0.
-  constexpr int64_t kSmallSteps = 12 * 1024;
-  const bool small = (static_cast<int64_t>(v.N) + 15) / 16 * v.steps <= kSmallSteps;
-  return (small && launch_vec_group<8>(v, r.group, s)) || launch_vec_group<16>(v, r.group, s);
+  const bool z = v.zeros != nullptr;
+  switch (r.group) {
+    case 32: return z ? launch_vec_group<32, true>(v, s) : launch_vec_group<32, false>(v, s);
+    case 64: return z ? launch_vec_group<64, true>(v, s) : launch_vec_group<64, false>(v, s);
+    default: return z ? launch_vec_group<128, true>(v, s) : launch_vec_group<128, false>(v, s);
+  }
 }
 
 }  // namespace minisgl
