@@ -87,14 +87,15 @@ __device__ __forceinline__ uint32_t e4m3x4(const float* t, float s) {
 // that share a block call it together with the rest of their warp (`active`
 // may differ between blocks, not inside one). `slack`: bound on y's relative
 // error in units of 2^-24; bit i of `doubt` marks an element whose error may be
-// larger but not twofold (bit 16 + i: of any size). exact(i): element i in double; zero(): whether all of the lane's
-// inputs make zeros (asked only where y is too small for float32).
+// larger but not twofold, and at most `edge` such units where |y| is above 1e-20 (below, no such element decides a
+// scale: those blocks are done in double). An element that float32 cannot tell is NaN: its block is done in double. exact(i): element i in double;
+// zero(): whether all of the lane's inputs make zeros (asked only where y is too small for float32).
 //
 // Rounding is monotonic: where y (1 - slack) and y (1 + slack) round to the
 // same E4M3 value, so does the exact one.
 template <int V, typename Exact, typename Zero>
-__device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t slack, uint32_t doubt, Exact exact, Zero zero,
-                                          uint8_t* q, uint8_t* sf, bool active) {
+__device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t slack, uint32_t edge, uint32_t doubt, Exact exact,
+                                          Zero zero, uint8_t* q, uint8_t* sf, bool active) {
   constexpr int G = kBlock / V;  // lanes of a block
   const int lane = threadIdx.x & 31;
   float top_f = max_abs3(y[0], y[1], y[2]);
@@ -104,13 +105,28 @@ __device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t slack, u
 #pragma unroll
   for (int o = 1; o < G; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (!active) return;
-  // magnitudes far inside float32's range whose scale is in no doubt (a fraction has units of 2^-23)
-  const uint32_t frac = m & 0x7FFFFFu;
-  const bool plain = m - (64u << 23) < (186u << 23) && frac + slack - 0x600000u > 2 * slack;
+  const uint32_t group = ((1u << G) - 1u) << (lane & ~(G - 1));
   uint32_t words[V / 4];
   uint32_t sbyte;
-  if (plain) {
-    sbyte = ((m + 0x1FFFFFu) >> 23) - 8;  // exponent of m, one up where the fraction is above 448's 1.75
+  if (m - (64u << 23) < (186u << 23)) {  // magnitudes far inside float32's range
+    // exponent of the largest, one up where the fraction is above 448's 1.75
+    sbyte = ((m + 0x1FFFFFu) >> 23) - 8;
+    if ((m & 0x7FFFFFu) + edge - 0x600000u <= 2 * edge) {
+      // closer to 1.75 than its error (a fraction has units of 2^-23): what may be the largest, in double
+      const float least = __uint_as_float(m) * (1.f - static_cast<float>(edge) * 2.3841858e-7f);
+      double top = 0.0;
+#pragma unroll 1
+      for (int i = 0; i < V; ++i) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (k == i) v = y[k];
+        if (fabsf(v) >= least) top = fmax(top, fabs(exact(i)));
+      }
+#pragma unroll
+      for (int o = 1; o < G; o <<= 1) top = fmax(top, __shfl_xor_sync(group, top, o));
+      sbyte = (m >> 23) - 8 + (top > 1.75 * pow2(static_cast<int>(m >> 23) - 127) ? 1 : 0);
+    }
     const float inv = __uint_as_float((254u - sbyte) << 23);
     const float eps = static_cast<float>(slack + 1) * 5.9604645e-8f;  // one more: the products below are rounded
     uint32_t apart[V / 4], any = doubt;
@@ -128,7 +144,6 @@ __device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t slack, u
         // an element in doubt matters unless it is far below half of the smallest step
         if (fabsf(y[i] * inv) > 0.00048828125f) near |= doubt & (1u << i);
       }
-      near |= doubt >> 16;
       const double s = pow2(127 - static_cast<int>(sbyte));
 #pragma unroll 1
       for (int i = 0; i < V; ++i) {
@@ -141,7 +156,6 @@ __device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t slack, u
     }
   } else {
     // the whole block in double
-    const uint32_t group = (G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (lane & ~(G - 1)));
     double top = 0.0;
     bool nan = false;
     const bool zeros = m == 0 && __all_sync(group, zero());
@@ -309,7 +323,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rmsnorm_mx8_k
       const T* src = (has_res ? res_out : x) + c;  // the normalised row's input, as stored
       const T* wc = static_cast<const T*>(a.w) + c;
       mx8_block<V>(
-          y, 4u, 0u,
+          y, 4u, 4u, 0u,
           [=](int i) {
             const double d = static_cast<double>(to_f32<T>(src[i])) * inv_d;
             return has_w ? d * static_cast<double>(to_f32<T>(wc[i])) : d;
@@ -354,6 +368,28 @@ __device__ __forceinline__ float ex2_approx(float x) {  // 2 units
   return r;
 }
 
+// P(X < -a) of a standard normal X, a >= 0: e^(-a^2 / 2) times a polynomial in t = 1 / (1 + a / 4), fitted to
+// erfcx(a / sqrt 2) / 2 on [0, 13.4] by iteratively reweighted least squares (relative error 2^-26). a^2 and its
+// product with log2(e) / 2 are carried with their rounding errors, which e^-85 would magnify. Compared with double
+// for every float32 a up to 12.5: at most 9.5 * 2^-24 off.
+__device__ __forceinline__ float normal_tail(float a) {
+  const float t = rcp_approx(fmaf(a, 0.25f, 1.f));
+  float r = 3.4584614e-2f;
+  r = fmaf(r, t, -1.9962448e-1f);
+  r = fmaf(r, t, 4.0307708e-1f);
+  r = fmaf(r, t, -3.4421673e-1f);
+  r = fmaf(r, t, 3.1342766e-1f);
+  r = fmaf(r, t, -2.5198551e-2f);
+  r = fmaf(r, t, 1.2324397e-1f);
+  r = fmaf(r, t, 9.4456886e-2f);
+  r = fmaf(r, t, 1.0027349e-1f);
+  r = fmaf(r, t, -2.3943172e-5f);
+  constexpr float kHi = -0.72134752f, kLo = -0.72134752044448170 - static_cast<double>(kHi);
+  const float a2 = a * a, e = a2 * kHi;
+  const float low = fmaf(a2, kLo, fmaf(fmaf(a, a, -a2), kHi, fmaf(a2, kHi, -e)));  // of the exponent
+  return r * fmaf(ex2_approx(e), low * 0.69314718f, ex2_approx(e));
+}
+
 // A block takes a part of a row at a time, and the loads of its next row are on their way while it works.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
@@ -380,6 +416,7 @@ __global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
       next_g = load_pair(gp + step);
       next_u = load_pair(up + step);
     }
+    constexpr float kTail = ACT == 0 ? -16.f : -12.5f;
     float low = g[0];
 #pragma unroll
     for (int k = 1; k < V; k += 2) low = min3(low, g[k], g[k + 1 < V ? k + 1 : k]);
@@ -390,19 +427,26 @@ __global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
         // p / (1 + e^-g): for g >= -16 the exponential's argument (16 * 2^-24) and value, the sum, the reciprocal
         // and the products leave at most 26 * 2^-24
         y[k] = p * rcp_approx(1.f + ex2_approx(-1.44269504f * g[k]));
-      else
-        // p / 2 * erfc(-g / sqrt 2): for g >= -6 the argument's rounding grows by at most 2 (6 / sqrt 2)^2 = 36
-        y[k] = 0.5f * p * erfcf(-0.70710678f * g[k]);
+      else {
+        // with the tail's error, the difference's and the product's: at most 12 * 2^-24 for g >= -12.5
+        const float h = normal_tail(fabsf(g[k]));
+        y[k] = p * (g[k] < 0.f ? h : 1.f - h);
+      }
     }
     uint32_t doubt = 0;
-    if (low < (ACT == 0 ? -16.f : -6.f)) {
+    if (low < kTail) {
       // the tail; where e^g leaves float32 only a vast product could matter beside a block's ordinary values
 #pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (g[k] < (ACT == 0 ? -16.f : -6.f)) doubt |= (fabsf(g[k] * u[k]) > 1e12f ? 0x10000u : 1u) << k;
+      for (int k = 0; k < V; ++k) {
+        if (g[k] < kTail) {
+          doubt |= 1u << k;
+          if (fabsf(g[k] * u[k]) > 1e12f) y[k] = __uint_as_float(0x7FC00000u);
+        }
+      }
     }
     mx8_block<V>(
-        y, ACT == 0 ? 32u : 128u, doubt,
+        // edge: SiLU's exponent of up to 128 is off by 2^-17 and its value by 180 * 2^-24 in the tail, until y < 1e-20
+        y, ACT == 0 ? 32u : 16u, ACT == 0 ? 256u : 16u, doubt,
         [=](int k) { return act_exact<ACT>(to_f32<T>(gp[k]), to_f32<T>(up[k])); },
         [=]() {
           bool z = true;
@@ -423,16 +467,32 @@ void by_dtype(DType dt, F&& f) {
   }
 }
 
-// as many CTAs as fit the SMs at once, each walking its rows
+// how many CTAs of so many threads fit the SMs at once
 template <auto kern>
-void launch_norm(const NormArgs& a, int threads, cudaStream_t s) {
-  static std::atomic<int> fit[33];  // CTAs of an SM by warps
+int64_t resident_ctas(int threads) {
+  static std::atomic<int> fit[33];  // of an SM, by warps
   int n = fit[threads / 32].load();
   if (n == 0) {
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1) n = 1;
     fit[threads / 32].store(n);
   }
-  launch_pdl(kern, dim3(static_cast<unsigned>(std::min<int64_t>(a.rows, 148 * n))), dim3(threads), 0, s, a);
+  return 148 * n;
+}
+
+// each CTA walks its rows
+template <auto kern>
+void launch_norm(const NormArgs& a, int threads, cudaStream_t s) {
+  launch_pdl(kern, dim3(static_cast<unsigned>(std::min<int64_t>(a.rows, resident_ctas<kern>(threads)))), dim3(threads), 0,
+             s, a);
+}
+
+// CTAs of up to 256 threads for each part of the columns, which share its rows
+template <auto kern, int V>
+void launch_act(const ActArgs& a, cudaStream_t s) {
+  const int lanes = a.d / V, threads = std::min(256, (lanes + 31) / 32 * 32);
+  const int64_t parts = (lanes + threads - 1) / threads;
+  const int64_t walkers = std::min<int64_t>({a.rows, std::max<int64_t>(1, resident_ctas<kern>(threads) / parts), 65535});
+  launch_pdl(kern, dim3(static_cast<unsigned>(parts), static_cast<unsigned>(walkers)), dim3(threads), 0, s, a);
 }
 
 }  // namespace
@@ -456,26 +516,18 @@ void launch_rmsnorm_mx8(const RmsnormMx8Args& r, cudaStream_t s) {
   });
 }
 
-constexpr int kActPerSm = 3;
 void launch_act_mx8(const ActMx8Args& r, cudaStream_t s) {
   if (r.rows <= 0) return;
   by_dtype(r.dtype, [&](auto tag) {
     using T = decltype(tag);
-    constexpr int V = 32 / sizeof(T);
     if (r.d % kBlock != 0) throw std::runtime_error("minisgl.act_mx8: width must be a multiple of 32");
     if (r.interleaved && r.d % 64 != 0)
       throw std::runtime_error("minisgl.act_mx8: interleaved width must be a multiple of 64");
     const ActArgs a{r.x, r.q, r.sf, r.rows, r.ld_x, r.ld_q, r.ld_sf, r.d, r.interleaved ? 1 : 0};
-    const int lanes = r.d / V;
-    const int threads = std::min(256, (lanes + 31) / 32 * 32);
-    const unsigned parts = static_cast<unsigned>((lanes + threads - 1) / threads);
-    // blocks of a column part share its rows; some three of 256 threads per SM
-    const int64_t blocks_y = std::min<int64_t>({r.rows, std::max<int64_t>(1, 148 * kActPerSm * 256 / threads / parts), 65535});
-    const dim3 blocks(parts, static_cast<unsigned>(blocks_y));
     if (r.act == 0)
-      launch_pdl(act_mx8_kernel<T, 0>, blocks, dim3(threads), 0, s, a);
+      launch_act<act_mx8_kernel<T, 0>, 32 / sizeof(T)>(a, s);
     else
-      launch_pdl(act_mx8_kernel<T, 1>, blocks, dim3(threads), 0, s, a);
+      launch_act<act_mx8_kernel<T, 1>, 32 / sizeof(T)>(a, s);
   });
 }
 

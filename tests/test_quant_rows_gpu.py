@@ -152,6 +152,22 @@ def test_act_mx8_hard_values(dt, act):
         _same_rows(fn(x.to(t)), ref.act_mx8(x.to(t), act, False))
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_act_mx8_gate_tails(dt, act):
+    """Gates far below zero beside vast products: what they leave may decide a block's scale."""
+    g = torch.empty(4096, 64, device=DEV).uniform_(-110, -4, generator=_gen(21))
+    g[::2] = g[::2, :1]  # half of the rows: one gate a row
+    u = torch.randn(4096, 64, generator=_gen(22), device=DEV)
+    u *= 10.0 ** torch.empty(4096, 1, device=DEV).uniform_(-3, 37, generator=_gen(23))
+    u[:, ::8] *= 10.0 ** torch.empty(4096, 1, device=DEV).uniform_(-30, 0, generator=_gen(24))
+    g[3::4, 1::2] = torch.randn(1024, 32, generator=_gen(25), device=DEV)  # ordinary values beside them
+    u[3::4, 1::2] = torch.randn(1024, 32, generator=_gen(26), device=DEV)
+    x = torch.cat([g, u], dim=1).to(TYPES[dt])
+    fn = ops.silu_and_mul_mx8 if act == "silu" else ops.gelu_and_mul_mx8
+    _same_rows(fn(x), ref.act_mx8(x, act, False))
+
+
 def test_rows_strided_and_given_out():
     g = _gen(8)
     base = torch.randn(9, 1024, generator=g, device=DEV).to(torch.bfloat16)
