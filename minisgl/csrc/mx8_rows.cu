@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <atomic>
 #include <stdexcept>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.h"
@@ -47,12 +48,45 @@ __device__ __forceinline__ void store_pair(T* p, const Pair& r) {
   reinterpret_cast<uint4*>(p)[0] = r.v[0];
   reinterpret_cast<uint4*>(p)[1] = r.v[1];
 }
+// whole words at a time: a 16-bit value taken out alone costs one more instruction
 template <typename T, int V>
 __device__ __forceinline__ void unpack(const Pair& raw, float (&v)[V]) {
   static_assert(V * sizeof(T) == 32, "two vectors");
-  const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = to_f32<T>(e[i]);
+  for (int i = 0; i < 8; ++i) {
+    const uint4& q = raw.v[i >> 2];
+    const uint32_t w = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(w);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    } else {
+      v[2 * i] = __uint_as_float(w << 16), v[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
+    }
+  }
+}
+// v rounded to T, as stored and as floats again
+template <typename T, int V>
+__device__ __forceinline__ Pair round_to(float (&v)[V]) {
+  Pair r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t w;
+    if constexpr (sizeof(T) == 4) {
+      w = __float_as_uint(v[i]);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    uint4& q = r.v[i >> 2];
+    ((i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w) = w;
+  }
+  unpack<T, V>(r, v);
+  return r;
 }
 
 // E4M3 bits of a double: truncated to float32 with a sticky last bit
@@ -77,13 +111,21 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// a and b times s, in one instruction
+__device__ __forceinline__ float2 times2(float a, float b, float s) {
+  float2 r;
+  asm("{\n.reg .b64 v, f, p;\nmov.b64 v, {%2, %3};\nmov.b64 f, {%4, %4};\nmul.rn.f32x2 p, v, f;\nmov.b64 {%0, %1}, p;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a), "f"(b), "f"(s));
+  return r;
+}
 __device__ __forceinline__ uint32_t e4m3x4(const float* t, float s) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[0] * s, t[1] * s), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[2] * s, t[3] * s), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(times2(t[0], t[1], s), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(times2(t[2], t[3], s), __NV_SATFINITE, __NV_E4M3);
   return lo | hi << 16;
 }
 
-// The V elements y of this lane, quantised. The 32 / V neighbouring lanes
+// The V elements y = v * factor of this lane, quantised. The 32 / V neighbouring lanes
 // that share a block call it together with the rest of their warp (`active`
 // may differ between blocks, not inside one). `slack`: bound on y's relative
 // error in units of 2^-24; bit i of `doubt` marks an element whose error may be
@@ -94,46 +136,48 @@ __device__ __forceinline__ uint32_t e4m3x4(const float* t, float s) {
 // Rounding is monotonic: where y (1 - slack) and y (1 + slack) round to the
 // same E4M3 value, so does the exact one.
 template <int V, typename Exact, typename Zero>
-__device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t slack, uint32_t edge, uint32_t doubt, Exact exact,
-                                          Zero zero, uint8_t* q, uint8_t* sf, bool active) {
+__device__ __forceinline__ void mx8_block(const float (&v)[V], float factor, uint32_t slack, uint32_t edge, uint32_t doubt,
+                                          Exact exact, Zero zero, uint8_t* q, uint8_t* sf, bool active) {
   constexpr int G = kBlock / V;  // lanes of a block
   const int lane = threadIdx.x & 31;
-  float top_f = max_abs3(y[0], y[1], y[2]);
+  float top_v = max_abs3(v[0], v[1], v[2]);
 #pragma unroll
-  for (int i = 3; i < V; i += 2) top_f = max_abs3(top_f, y[i], y[i + 1 < V ? i + 1 : i]);
-  uint32_t m = __float_as_uint(top_f);  // as bits: NaN above infinity above every number
+  for (int i = 3; i < V; i += 2) top_v = max_abs3(top_v, v[i], v[i + 1 < V ? i + 1 : i]);
+  uint32_t mv = __float_as_uint(top_v);  // as bits: NaN above infinity above every number
 #pragma unroll
-  for (int o = 1; o < G; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 1; o < G; o <<= 1) mv = max(mv, __shfl_xor_sync(0xffffffffu, mv, o));
+  const uint32_t m = __float_as_uint(__uint_as_float(mv) * factor);
   if (!active) return;
   const uint32_t group = ((1u << G) - 1u) << (lane & ~(G - 1));
   uint32_t words[V / 4];
   uint32_t sbyte;
-  if (m - (64u << 23) < (186u << 23)) {  // magnitudes far inside float32's range
+  // magnitudes far inside float32's range (v's down to 2^-118, of which more could not be seen)
+  if (m - (64u << 23) < (186u << 23) && mv - (27u << 23) < (220u << 23)) {
     // exponent of the largest, one up where the fraction is above 448's 1.75
     sbyte = ((m + 0x1FFFFFu) >> 23) - 8;
     if ((m & 0x7FFFFFu) + edge - 0x600000u <= 2 * edge) {
       // closer to 1.75 than its error (a fraction has units of 2^-23): what may be the largest, in double
-      const float least = __uint_as_float(m) * (1.f - static_cast<float>(edge) * 2.3841858e-7f);
+      const float least = __uint_as_float(mv) * (1.f - static_cast<float>(edge) * 2.3841858e-7f);
       double top = 0.0;
 #pragma unroll 1
       for (int i = 0; i < V; ++i) {
-        float v = 0.f;
+        float vi = 0.f;
 #pragma unroll
         for (int k = 0; k < V; ++k)
-          if (k == i) v = y[k];
-        if (fabsf(v) >= least) top = fmax(top, fabs(exact(i)));
+          if (k == i) vi = v[k];
+        if (fabsf(vi) >= least) top = fmax(top, fabs(exact(i)));
       }
 #pragma unroll
       for (int o = 1; o < G; o <<= 1) top = fmax(top, __shfl_xor_sync(group, top, o));
       sbyte = (m >> 23) - 8 + (top > 1.75 * pow2(static_cast<int>(m >> 23) - 127) ? 1 : 0);
     }
-    const float inv = __uint_as_float((254u - sbyte) << 23);
-    const float eps = static_cast<float>(slack + 1) * 5.9604645e-8f;  // one more: the products below are rounded
+    const float inv = factor * __uint_as_float((254u - sbyte) << 23);  // about 448 / top_v: no overflow
+    const float eps = static_cast<float>(slack + 2) * 5.9604645e-8f;  // two more: this factor and the products are rounded
     uint32_t apart[V / 4], any = doubt;
 #pragma unroll
     for (int w = 0; w < V / 4; ++w) {
-      words[w] = e4m3x4(y + 4 * w, inv + inv * eps);
-      apart[w] = words[w] ^ e4m3x4(y + 4 * w, inv - inv * eps);
+      words[w] = e4m3x4(v + 4 * w, inv + inv * eps);
+      apart[w] = words[w] ^ e4m3x4(v + 4 * w, inv - inv * eps);
       any |= apart[w];
     }
     if (any != 0) {
@@ -142,7 +186,7 @@ __device__ __forceinline__ void mx8_block(const float (&y)[V], uint32_t slack, u
       for (int i = 0; i < V; ++i) {
         if ((apart[i >> 2] >> (8 * (i & 3)) & 0xFFu) != 0) near |= 1u << i;
         // an element in doubt matters unless it is far below half of the smallest step
-        if (fabsf(y[i] * inv) > 0.00048828125f) near |= doubt & (1u << i);
+        if (fabsf(v[i] * inv) > 0.00048828125f) near |= doubt & (1u << i);
       }
       const double s = pow2(127 - static_cast<int>(sbyte));
 #pragma unroll 1
@@ -261,13 +305,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rmsnorm_mx8_k
         if (has_res) {
           float r[V];
           unpack<T, V>(next_r[k], r);
-          T* e = reinterpret_cast<T*>(&raw[k]);
+          // the residual stream is kept in the activation's type: the sum is rounded before it is normalised
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            // the residual stream is kept in the activation's type: the sum is rounded before it is normalised
-            e[i] = from_f32<T>(v[i] + r[i]);
-            v[i] = to_f32<T>(e[i]);
-          }
+          for (int i = 0; i < V; ++i) v[i] += r[i];
+          raw[k] = round_to<T, V>(v);
           store_pair(res_out + c, raw[k]);
         }
 #pragma unroll
@@ -304,26 +345,23 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rmsnorm_mx8_k
     for (int k = 0; k < NP; ++k) {
       const int c = (k * blockDim.x + threadIdx.x) * V;
       const bool active = c < a.cols;
-      float y[V];
+      float v[V];
       if (active) {
-        unpack<T, V>(raw[k], y);
-        // three roundings (inv and two products): at most 3 * 2^-24
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[i] *= inv;
-        if (has_w) {
+        unpack<T, V>(raw[k], v);
+        if (has_w) {  // exact for 16-bit types
           float w[V];
           unpack<T, V>(load_pair(static_cast<const T*>(a.w) + c), w);
 #pragma unroll
-          for (int i = 0; i < V; ++i) y[i] *= w[i];
+          for (int i = 0; i < V; ++i) v[i] *= w[i];
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = 0.f;
+        for (int i = 0; i < V; ++i) v[i] = 0.f;
       }
       const T* src = (has_res ? res_out : x) + c;  // the normalised row's input, as stored
       const T* wc = static_cast<const T*>(a.w) + c;
       mx8_block<V>(
-          y, 4u, 4u, 0u,
+          v, inv, 2u, 4u, 0u,  // roundings: inv and v w; for the scale their product
           [=](int i) {
             const double d = static_cast<double>(to_f32<T>(src[i])) * inv_d;
             return has_w ? d * static_cast<double>(to_f32<T>(wc[i])) : d;
@@ -446,7 +484,7 @@ __global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
     }
     mx8_block<V>(
         // edge: SiLU's exponent of up to 128 is off by 2^-17 and its value by 180 * 2^-24 in the tail, until y < 1e-20
-        y, ACT == 0 ? 32u : 16u, ACT == 0 ? 256u : 16u, doubt,
+        y, 1.f, ACT == 0 ? 32u : 16u, ACT == 0 ? 256u : 16u, doubt,
         [=](int k) { return act_exact<ACT>(to_f32<T>(gp[k]), to_f32<T>(up[k])); },
         [=]() {
           bool z = true;
