@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <atomic>
 #include <stdexcept>
+#include <string>
 #include <type_traits>
 
 #include "common.cuh"
@@ -262,49 +263,66 @@ struct NormArgs {
   int64_t rows;
 };
 
-// A CTA walks rows; a row stays in registers between its two passes. With AHEAD (up to 256 threads, which leaves the
-// registers for it) the loads of the CTA's next row are on their way while this one is reduced and stored; without,
-// the wait for memory at the start of a row and the barrier leave the memory idle (B200, 8192 x 7168 bf16 with
-// residual: 101 us). The sum of squares is held in double: the squares of 16-bit inputs are exact there, so the
-// statistic is exact but for the final additions.
-template <typename T, int NP, int THREADS, bool AHEAD>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rmsnorm_mx8_kernel(const NormArgs a) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// A CTA walks rows; a row stays in registers between its two passes. The rows after it (DEPTH of them) are on their way
+// to shared memory: each warp copies what it will read itself, so that only its own copies' arrival is waited for. Held in registers instead, one row ahead, they cost the occupancy that hides the barrier and the conversions
+// (B200, 8192 x 7168 bf16 with residual: 98 us). The sum of squares is held in double: the squares of 16-bit inputs are
+// exact there, so the statistic is exact but for the final additions.
+template <typename T, int NP, int THREADS, int DEPTH>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) rmsnorm_mx8_kernel(const NormArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int V = 32 / sizeof(T);
+  extern __shared__ __align__(16) uint4 ring[];  // [row][x, residual][NP][warp][64]
   __shared__ double red[2][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
   const bool has_res = a.res != nullptr, has_w = a.w != nullptr;
-  Pair next_x[NP], next_r[NP];
-  auto load = [&](int64_t row) {
-    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
-    const T* res = static_cast<const T*>(a.res) + row * a.ld_res;
+  const int tensor = NP * 2 * blockDim.x, stage = tensor * (has_res ? 2 : 1);
+  // A warp's 64 vectors of a part are copied in memory's order (an instruction takes whole sectors) and read in pairs:
+  // the lowest bit of a vector's place is flipped in every other 8, so that eight lanes' reads meet 8 banks of 16 bytes.
+  auto load = [&](int64_t row, uint4* slot) {
+    if (row < a.rows) {
+      const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+      const T* res = static_cast<const T*>(a.res) + row * a.ld_res;
+      const uint32_t dst = smem_u32(slot + warp * 64 + (lane ^ (lane >> 3 & 1)));
 #pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      const int c = (k * blockDim.x + threadIdx.x) * V;
-      if (c < a.cols) {
-        next_x[k] = load_pair(x + c);
-        if (has_res) next_r[k] = load_pair(res + c);
+      for (int k = 0; k < NP; ++k) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int at = 2 * k * blockDim.x + h * 32, c = (at + warp * 64 + lane) * (V / 2);
+          if (c < a.cols) {
+            cp_async16(dst + at * 16, x + c);
+            if (has_res) cp_async16(dst + (tensor + at) * 16, res + c);
+          }
+        }
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  load(blockIdx.x);
-  int turn = 0;
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) load(blockIdx.x + static_cast<int64_t>(d) * gridDim.x, ring + d * stage);
+  int turn = 0, slot = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
     T* res_out = static_cast<T*>(a.res_out) + row * a.ld_res_out;
     Pair raw[NP];  // what is normalised, in its type
     double part[4] = {0.0, 0.0, 0.0, 0.0};  // four short chains
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+    __syncwarp();
+    const uint4* mine = ring + slot * stage + warp * 64 + 2 * lane;
+    const int flip = lane >> 2 & 1;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       const int c = (k * blockDim.x + threadIdx.x) * V;
       if (c < a.cols) {
         float v[V];
-        raw[k] = next_x[k];
+        raw[k] = Pair{{mine[2 * k * blockDim.x + flip], mine[2 * k * blockDim.x + 1 - flip]}};
         unpack<T, V>(raw[k], v);
         if (has_res) {
           float r[V];
-          unpack<T, V>(next_r[k], r);
+          unpack<T, V>(Pair{{mine[tensor + 2 * k * blockDim.x + flip], mine[tensor + 2 * k * blockDim.x + 1 - flip]}}, r);
           // the residual stream is kept in the activation's type: the sum is rounded before it is normalised
 #pragma unroll
           for (int i = 0; i < V; ++i) v[i] += r[i];
@@ -319,12 +337,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rmsnorm_mx8_k
       }
     }
     double ss = (part[0] + part[1]) + (part[2] + part[3]);
-    if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     // the two halves of red alternate: a warp that writes one again has passed the barrier after everybody read it
     if (lane == 0) red[turn][warp] = ss;
     __syncthreads();
+    // every read of the slot lies before the barrier
+    load(row + static_cast<int64_t>(DEPTH) * gridDim.x, ring + slot * stage);
+    slot = slot + 1 == DEPTH ? 0 : slot + 1;
     ss = red[turn][0];  // the same order in every thread
     for (int w = 1; w < nw; ++w) ss += red[turn][w];
     // 1 / sqrt: two Newton steps in double on the float32 estimate leave some units of 2^-53
@@ -358,7 +378,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rmsnorm_mx8_k
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = 0.f;
       }
-      const T* src = (has_res ? res_out : x) + c;  // the normalised row's input, as stored
+      const T* src = (has_res ? res_out : static_cast<const T*>(a.x) + row * a.ld_x) + c;  // the normalised row's input, as stored
       const T* wc = static_cast<const T*>(a.w) + c;
       mx8_block<V>(
           v, inv, 2u, 4u, 0u,  // roundings: inv and v w; for the scale their product
@@ -374,7 +394,6 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rmsnorm_mx8_k
           },
           a.q + row * a.ld_q + c, a.sf + row * a.ld_sf + c / kBlock, active);
     }
-    if (!AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
   }
 }
 
@@ -505,23 +524,33 @@ void by_dtype(DType dt, F&& f) {
   }
 }
 
-// how many CTAs of so many threads fit the SMs at once
+// CTAs of so many threads and bytes of shared memory that fit the SMs at once
 template <auto kern>
-int64_t resident_ctas(int threads) {
-  static std::atomic<int> fit[33];  // of an SM, by warps
-  int n = fit[threads / 32].load();
+int64_t resident_ctas(int threads, int smem, bool residual) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> fit[kDevices][33][2];  // of an SM
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int n = dev < kDevices ? fit[dev][threads / 32][residual].load() : 0;
   if (n == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1) n = 1;
-    fit[threads / 32].store(n);
+    if (smem > 0) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+      if (e != cudaSuccess) throw std::runtime_error(std::string("minisgl.rmsnorm_mx8: ") + cudaGetErrorString(e));
+    }
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n < 1) n = 1;
+    if (dev < kDevices) fit[dev][threads / 32][residual].store(n);
   }
   return 148 * n;
 }
 
 // each CTA walks its rows
-template <auto kern>
-void launch_norm(const NormArgs& a, int threads, cudaStream_t s) {
-  launch_pdl(kern, dim3(static_cast<unsigned>(std::min<int64_t>(a.rows, resident_ctas<kern>(threads)))), dim3(threads), 0,
-             s, a);
+template <typename T, int NP, int THREADS, int DEPTH>
+void launch_norm(const NormArgs& a, int pairs, cudaStream_t s) {
+  constexpr auto kern = rmsnorm_mx8_kernel<T, NP, THREADS, DEPTH>;
+  const bool residual = a.res != nullptr;
+  const int threads = (pairs + NP * 32 - 1) / (NP * 32) * 32, smem = threads * NP * 32 * DEPTH * (residual ? 2 : 1);
+  const int64_t ctas = std::min<int64_t>(a.rows, resident_ctas<kern>(threads, smem, residual));
+  launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(threads), smem, s, a);
 }
 
 // CTAs of up to 256 threads for each part of the columns, which share its rows
@@ -529,7 +558,7 @@ template <auto kern, int V>
 void launch_act(const ActArgs& a, cudaStream_t s) {
   const int lanes = a.d / V, threads = std::min(256, (lanes + 31) / 32 * 32);
   const int64_t parts = (lanes + threads - 1) / threads;
-  const int64_t walkers = std::min<int64_t>({a.rows, std::max<int64_t>(1, resident_ctas<kern>(threads) / parts), 65535});
+  const int64_t walkers = std::min<int64_t>({a.rows, std::max<int64_t>(1, resident_ctas<kern>(threads, 0, false) / parts), 65535});
   launch_pdl(kern, dim3(static_cast<unsigned>(parts), static_cast<unsigned>(walkers)), dim3(threads), 0, s, a);
 }
 
@@ -544,13 +573,12 @@ void launch_rmsnorm_mx8(const RmsnormMx8Args& r, cudaStream_t s) {
     if (r.cols % kBlock != 0 || pairs > 2 * 1024) throw std::runtime_error("minisgl.rmsnorm_mx8: unsupported width");
     const NormArgs a{r.x, r.residual, r.residual_out, r.w, r.q, r.sf, r.cols, r.ld_x, r.ld_res, r.ld_res_out,
                      r.ld_q, r.ld_sf, r.eps, 1.0 / r.cols, r.rows};
-    const auto threads = [&](int np) { return (pairs + np * 32 - 1) / (np * 32) * 32; };
     if (pairs <= 256)
-      launch_norm<rmsnorm_mx8_kernel<T, 1, 256, true>>(a, threads(1), s);
+      launch_norm<T, 1, 256, 2>(a, pairs, s);
     else if (pairs <= 512)
-      launch_norm<rmsnorm_mx8_kernel<T, 2, 256, true>>(a, threads(2), s);
+      launch_norm<T, 2, 256, 2>(a, pairs, s);
     else
-      launch_norm<rmsnorm_mx8_kernel<T, 2, 1024, false>>(a, threads(2), s);
+      launch_norm<T, 2, 1024, 1>(a, pairs, s);
   });
 }
 
