@@ -267,27 +267,30 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// A CTA walks rows; a row stays in registers between its two passes. The rows after it (DEPTH of them) are on their way
-// to shared memory: each warp copies what it will read itself, so that only its own copies' arrival is waited for. Held in registers instead, one row ahead, they cost the occupancy that hides the barrier and the conversions
-// (B200, 8192 x 7168 bf16 with residual: 98 us). The sum of squares is held in double: the squares of 16-bit inputs are
-// exact there, so the statistic is exact but for the final additions.
-template <typename T, int NP, int THREADS, int DEPTH>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) rmsnorm_mx8_kernel(const NormArgs a) {
+// A CTA walks rows; a row stays in registers between its two passes, and the next one is on its way to shared memory
+// meanwhile: each warp copies what it will read itself, so that only its own copies' arrival is waited for. Held in
+// registers (two vectors a lane, so that each load takes half sectors) the row ahead cost the occupancy that hides the
+// barrier and the conversions: B200, 8192 x 7168 bf16 with residual 98 us, now 73 (5.7 TB/s, 87% of a copy's rate); two
+// rows ahead cost it again (83). Short rows are bound by the instructions, some 25 an element: 8192 x 2048 without
+// residual 19 us, 2.7 TB/s. The sum of squares is held in double: the squares of 16-bit inputs are exact there, so the
+// statistic is exact but for the final additions.
+template <typename T, int NP, int THREADS>
+__global__ void __launch_bounds__(THREADS) rmsnorm_mx8_kernel(const NormArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int V = 32 / sizeof(T);
-  extern __shared__ __align__(16) uint4 ring[];  // [row][x, residual][NP][warp][64]
+  extern __shared__ __align__(16) uint4 ahead[];  // [x, residual][NP][warp][64]
   __shared__ double red[2][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
   const bool has_res = a.res != nullptr, has_w = a.w != nullptr;
-  const int tensor = NP * 2 * blockDim.x, stage = tensor * (has_res ? 2 : 1);
+  const int tensor = NP * 2 * blockDim.x;
   // A warp's 64 vectors of a part are copied in memory's order (an instruction takes whole sectors) and read in pairs:
   // the lowest bit of a vector's place is flipped in every other 8, so that eight lanes' reads meet 8 banks of 16 bytes.
-  auto load = [&](int64_t row, uint4* slot) {
+  auto load = [&](int64_t row) {
     if (row < a.rows) {
       const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
       const T* res = static_cast<const T*>(a.res) + row * a.ld_res;
-      const uint32_t dst = smem_u32(slot + warp * 64 + (lane ^ (lane >> 3 & 1)));
+      const uint32_t dst = smem_u32(ahead + warp * 64 + (lane ^ (lane >> 3 & 1)));
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
 #pragma unroll
@@ -300,18 +303,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) rmsnorm_mx8_k
         }
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-#pragma unroll
-  for (int d = 0; d < DEPTH; ++d) load(blockIdx.x + static_cast<int64_t>(d) * gridDim.x, ring + d * stage);
-  int turn = 0, slot = 0;
+  load(blockIdx.x);
+  int turn = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
     T* res_out = static_cast<T*>(a.res_out) + row * a.ld_res_out;
     Pair raw[NP];  // what is normalised, in its type
     double part[4] = {0.0, 0.0, 0.0, 0.0};  // four short chains
-    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
-    const uint4* mine = ring + slot * stage + warp * 64 + 2 * lane;
+    const uint4* mine = ahead + warp * 64 + 2 * lane;
     const int flip = lane >> 2 & 1;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
@@ -342,9 +343,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) rmsnorm_mx8_k
     // the two halves of red alternate: a warp that writes one again has passed the barrier after everybody read it
     if (lane == 0) red[turn][warp] = ss;
     __syncthreads();
-    // every read of the slot lies before the barrier
-    load(row + static_cast<int64_t>(DEPTH) * gridDim.x, ring + slot * stage);
-    slot = slot + 1 == DEPTH ? 0 : slot + 1;
+    load(row + gridDim.x);  // every read of this row's copy lies before the barrier
     ss = red[turn][0];  // the same order in every thread
     for (int w = 1; w < nw; ++w) ss += red[turn][w];
     // 1 / sqrt: two Newton steps in double on the float32 estimate leave some units of 2^-53
@@ -544,11 +543,11 @@ int64_t resident_ctas(int threads, int smem, bool residual) {
 }
 
 // each CTA walks its rows
-template <typename T, int NP, int THREADS, int DEPTH>
+template <typename T, int NP, int THREADS>
 void launch_norm(const NormArgs& a, int pairs, cudaStream_t s) {
-  constexpr auto kern = rmsnorm_mx8_kernel<T, NP, THREADS, DEPTH>;
+  constexpr auto kern = rmsnorm_mx8_kernel<T, NP, THREADS>;
   const bool residual = a.res != nullptr;
-  const int threads = (pairs + NP * 32 - 1) / (NP * 32) * 32, smem = threads * NP * 32 * DEPTH * (residual ? 2 : 1);
+  const int threads = (pairs + NP * 32 - 1) / (NP * 32) * 32, smem = threads * NP * 32 * (residual ? 2 : 1);
   const int64_t ctas = std::min<int64_t>(a.rows, resident_ctas<kern>(threads, smem, residual));
   launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(threads), smem, s, a);
 }
@@ -573,12 +572,13 @@ void launch_rmsnorm_mx8(const RmsnormMx8Args& r, cudaStream_t s) {
     if (r.cols % kBlock != 0 || pairs > 2 * 1024) throw std::runtime_error("minisgl.rmsnorm_mx8: unsupported width");
     const NormArgs a{r.x, r.residual, r.residual_out, r.w, r.q, r.sf, r.cols, r.ld_x, r.ld_res, r.ld_res_out,
                      r.ld_q, r.ld_sf, r.eps, 1.0 / r.cols, r.rows};
-    if (pairs <= 256)
-      launch_norm<T, 1, 256, 2>(a, pairs, s);
-    else if (pairs <= 512)
-      launch_norm<T, 2, 256, 2>(a, pairs, s);
+    // One pair a thread: shorter chains (B200, bf16 with residual: 1 x 5120 2.8 us against 3.6 with two pairs,
+    // 2048 x 5120 16.1 against 17.4). Two: many rows whose CTAs of one pair a thread leave an SM's registers unused
+    // (8192 x 7168 73.0 against 77.2), and wide ones (4096 x 16384 82 against 100).
+    if (pairs <= 384 || (pairs <= 512 && r.rows <= 2 * 148))
+      launch_norm<T, 1, 512>(a, pairs, s);
     else
-      launch_norm<T, 2, 1024, 1>(a, pairs, s);
+      launch_norm<T, 2, 1024>(a, pairs, s);
   });
 }
 
