@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_mx8_kernel(const NormArgs a) 
       const T* src = (has_res ? res_out : static_cast<const T*>(a.x) + row * a.ld_x) + c;  // the normalised row's input, as stored
       const T* wc = static_cast<const T*>(a.w) + c;
       mx8_block<V>(
-          v, inv, 2u, 4u, 0u,  // roundings: inv and v w; for the scale their product
+          v, inv, 3u, 4u, 0u,  // two roundings, inv and v w, with room for the bounds' own; for the scale their product
           [=](int i) {
             const double d = static_cast<double>(to_f32<T>(src[i])) * inv_d;
             return has_w ? d * static_cast<double>(to_f32<T>(wc[i])) : d;
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(256) act_mx8_kernel(const ActArgs a) {
         // and the products leave at most 26 * 2^-24
         y[k] = p * rcp_approx(1.f + ex2_approx(-1.44269504f * g[k]));
       else {
-        // with the tail's error, the difference's and the product's: at most 12 * 2^-24 for g >= -12.5
+        // with the tail's error, the difference's and the product's: at most 13 * 2^-24 for g >= -12.5
         const float h = normal_tail(fabsf(g[k]));
         y[k] = p * (g[k] < 0.f ? h : 1.f - h);
       }

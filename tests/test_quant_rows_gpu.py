@@ -561,3 +561,41 @@ def test_weight_copies():
     x = torch.randn(3, 128, generator=_gen(1), device=DEV).to(torch.bfloat16)
     assert torch.equal(ops.int4_linear(x, copy.deepcopy(w)), ops.int4_linear(x, w))
     assert torch.equal(ops.int4_linear(x, w.to("cpu").to(DEV)), ops.int4_linear(x, w))
+
+
+# Sizes at which the estimate takes each of the few-row product's plans on 148 SMs (8 or 16 warps a CTA, one or two
+# 16-row tiles a unit, a tile's columns on 1 to 8 CTAs), with rows and columns that end inside a tile
+@pytest.mark.parametrize("m,n,k,group,zeros", [
+    (1, 8200, 4104, 32, True), (1, 1001, 26120, 128, True),                             # 8 warps, two tiles
+    (3, 4111, 2056, 64, False), (3, 1001, 8200, 32, False), (8, 333, 4104, 32, True), (8, 24, 4104, 128, False),
+    (8, 6151, 520, 32, True), (3, 8200, 8200, 32, False), (8, 1001, 4104, 64, True), (8, 24, 26120, 32, False),
+    (1, 8200, 8200, 32, True), (8, 20501, 4104, 128, True), (8, 10251, 4104, 32, True), (8, 6151, 8200, 128, True)])
+def test_int4_linear_every_plan(m, n, k, group, zeros):
+    w = _weight(n, k, group, zeros, n, torch.bfloat16)
+    x = torch.randn(m, k, generator=_gen(k), device=DEV).to(torch.bfloat16)
+    b = torch.randn(n, generator=_gen(n + 1), device=DEV)
+    y = ops.int4_linear(x, w, b, out_dtype=torch.float32)
+    _check_linear(y, x.double(), w, b)
+    assert torch.equal(y, ops.int4_linear(x, w, b, out_dtype=torch.float32))  # every sum has one order
+    x[0, k // 2] = float("inf")
+    x[m - 1, k - 1] = float("nan")
+    odd = ops.int4_linear(x, w, b, out_dtype=torch.float32)
+    assert bool(odd[m - 1].isnan().all())
+    if m > 2:
+        assert torch.equal(odd[1], y[1]) and not bool(odd[0].isfinite().any())
+
+
+@pytest.mark.parametrize("m,k", [(8, 80000), (3, 220000), (1, 700000)])
+@pytest.mark.parametrize("kind", ["bf16", "mx8"])
+def test_int4_linear_few_rows_beyond_any_plan(m, k, kind):
+    """Rows that shared memory cannot hold under any plan take the tiles of the longer batches and their scratch."""
+    w = _weight(40, k, 64, True, m, torch.bfloat16)
+    if kind == "mx8":
+        q = torch.randint(0, 0x7E, (m, k), generator=_gen(k), device=DEV, dtype=torch.uint8)
+        sf = torch.randint(118, 124, (m, k // 32), generator=_gen(m), device=DEV, dtype=torch.uint8)
+        y, xd = ops.int4_linear(q, w, x_scales=sf), dequantize_mx8_rows(q, sf, torch.float64)
+    else:
+        x = torch.randn(m, k, generator=_gen(k), device=DEV).to(torch.bfloat16)
+        y, xd = ops.int4_linear(x, w), x.double()
+    _check_linear(y, xd, w, None, rounded=True)
+    ops.check_device_errors(torch.device(DEV))
