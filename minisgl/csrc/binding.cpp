@@ -6,6 +6,7 @@
 // plain launchers declared in ops.h on the current CUDA stream.
 #include <cstring>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -502,12 +503,17 @@ void check_vec_rows(const at::Tensor& t, int64_t rows, int64_t cols, at::ScalarT
             what, ": the rows of ", name, " must lie at multiples of 16 bytes");
 }
 
+// A new tensor on x's device that a kernel writes as a whole, past torch's dispatcher (a small call's time is the host's)
+at::Tensor new_beside(const at::Tensor& x, at::IntArrayRef sizes, at::ScalarType dt) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dt, x.device(), std::nullopt));
+}
+
 // The caller's (q, sf), or new ones: allocated here, which costs a call a third of what two allocations cost in Python.
 std::pair<at::Tensor, at::Tensor> mx8_out(const at::Tensor& x, int64_t rows, int64_t cols,
                                           const c10::optional<std::pair<at::Tensor, at::Tensor>>& out, const char* what) {
   MSG_CHECK(cols > 0 && cols % 32 == 0, what, ": the width must be a positive multiple of 32, got ", cols);
   if (!out.has_value())
-    return {at::empty({rows, cols}, x.options().dtype(at::kByte)), at::empty({rows, cols / 32}, x.options().dtype(at::kByte))};
+    return {new_beside(x, {rows, cols}, at::kByte), new_beside(x, {rows, cols / 32}, at::kByte)};
   check_mx8_out(x, out->first, out->second, rows, cols, what);
   return *out;
 }
@@ -675,7 +681,7 @@ at::Tensor int4_linear(const at::Tensor& x, const Int4Handle& w, const c10::opti
               "int4_linear: out must be [", M, ", ", N, "] of out_dtype with unit column stride");
   } else {
     const at::ScalarType dt = out_dtype.has_value() ? *out_dtype : x_scales.has_value() ? at::kBFloat16 : x.scalar_type();
-    out = at::empty({M, N}, x.options().dtype(dt));
+    out = new_beside(x, {M, N}, dt);
   }
   a.x = x.data_ptr();
   a.packed = w.packed.data_ptr<uint8_t>();
@@ -694,7 +700,7 @@ at::Tensor int4_linear(const at::Tensor& x, const Int4Handle& w, const c10::opti
   if (M == 0) return out;
   if (!minisgl::launch_int4_stream(a, stream_of(x))) {
     if (x_scales.has_value()) {  // MXFP8 rows are widened to bf16 for the tensor cores' tiles
-      x_wide = at::empty({M, K}, x.options().dtype(at::kBFloat16));
+      x_wide = new_beside(x, {M, K}, at::kBFloat16);
       a.x_wide = x_wide.data_ptr();
     }
     minisgl::launch_int4_gemm(a, stream_of(x));

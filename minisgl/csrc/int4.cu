@@ -759,11 +759,26 @@ void launch_vec(VecArgs a, const VecPlan& p, cudaStream_t s) {
 // false: x does not fit shared memory under any plan
 template <int G, bool ZERO>
 bool launch_vec_group(const VecArgs& a, cudaStream_t s) {
-  VecPlan p{};
-  vec_plan<8, 1, G, ZERO>(a, p);
-  vec_plan<8, 2, G, ZERO>(a, p);
-  vec_plan<16, 1, G, ZERO>(a, p);
-  vec_plan<16, 2, G, ZERO>(a, p);
+  // the sixteen estimates cost a small call's launch some 15% of its time: a decode loop's next sizes are mostly the
+  // last layer's, so a thread keeps a few
+  struct Known {
+    int M = 0, N, K, dev;
+    VecPlan p;
+  };
+  constexpr int kKnown = 64;
+  static thread_local Known known[kKnown];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  Known& e = known[(static_cast<unsigned>(a.N) * 2654435761u + static_cast<unsigned>(a.K) * 40503u + a.M) >> 16 & (kKnown - 1)];
+  if (e.M != a.M || e.N != a.N || e.K != a.K || e.dev != dev) {
+    VecPlan p{};
+    vec_plan<8, 1, G, ZERO>(a, p);
+    vec_plan<8, 2, G, ZERO>(a, p);
+    vec_plan<16, 1, G, ZERO>(a, p);
+    vec_plan<16, 2, G, ZERO>(a, p);
+    e = Known{a.M, a.N, a.K, dev, p};
+  }
+  const VecPlan& p = e.p;
   if (p.S == 0) return false;
   if (p.W == 8)
     p.R == 1 ? launch_vec<8, 1, G, ZERO>(a, p, s) : launch_vec<8, 2, G, ZERO>(a, p, s);
