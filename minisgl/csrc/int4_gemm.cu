@@ -419,14 +419,11 @@ __global__ void __launch_bounds__(GSmem<BN>::kThreads, 1)
       const bool in = n < a.N;
       const float bias = in && a.bias != nullptr ? any_f32(a.bias, n, a.bias_type) : 0.f;
       const float pow = HALF && in ? a.row_pow[n] : 1.f;
-      constexpr int CH = BN < 32 ? 16 : 32;
+      constexpr int CH = 32;
 #pragma unroll 1
       for (int c = 0; c < BN; c += CH) {
         uint32_t r[32];
-        if constexpr (CH == 32)
-          tmem_ld_32x32b_x32(lane_base + acc * BN + c, r);
-        else
-          tmem_ld_32x32b_x16(lane_base + acc * BN + c, *reinterpret_cast<uint32_t(*)[16]>(r));
+        tmem_ld_32x32b_x32(lane_base + acc * BN + c, r);
         tc_wait_ld();
         if (c + CH >= BN) {  // the accumulator is read out: the MMAs may reuse it
           tc_fence_before();
