@@ -28,8 +28,9 @@
 // 214 where power holds the clock down, as it does a library product: 1.38 of
 // 1.63 PFLOP/s), 512 x 8192 x 7168 49, 128 x 8192 x 7168 22.5, 24 x 7168 x 8192
 // (groups of 64, MXFP8 rows) 19.5. Large tiles are bound by x on its way from L2
-// and by power, small ones (some 730 cycles a step) by the instructions of the
-// converters: about 1500 warp instructions for 16384 codes.
+// and by power, small ones (some 730 cycles a step) by instructions: 2200 a step
+// of 16384 codes, two thirds of them the converters'. More steps in tensor memory
+// or a third set of converters measured no better.
 //
 // Every wait is bounded: a timeout records an error, raises an abort flag that
 // the other roles check, and the CTA drains its copies and returns.
