@@ -112,17 +112,24 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// a and b times s, in one instruction
-__device__ __forceinline__ float2 times2(float a, float b, float s) {
+// two products or sums in one instruction
+__device__ __forceinline__ float2 mul2(float a, float b, float c, float d) {
   float2 r;
-  asm("{\n.reg .b64 v, f, p;\nmov.b64 v, {%2, %3};\nmov.b64 f, {%4, %4};\nmul.rn.f32x2 p, v, f;\nmov.b64 {%0, %1}, p;\n}"
+  asm("{\n.reg .b64 v, w;\nmov.b64 v, {%2, %3};\nmov.b64 w, {%4, %5};\nmul.rn.f32x2 v, v, w;\nmov.b64 {%0, %1}, v;\n}"
       : "=f"(r.x), "=f"(r.y)
-      : "f"(a), "f"(b), "f"(s));
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float a, float b, float c, float d) {
+  float2 r;
+  asm("{\n.reg .b64 v, w;\nmov.b64 v, {%2, %3};\nmov.b64 w, {%4, %5};\nadd.rn.f32x2 v, v, w;\nmov.b64 {%0, %1}, v;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
   return r;
 }
 __device__ __forceinline__ uint32_t e4m3x4(const float* t, float s) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(times2(t[0], t[1], s), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(times2(t[2], t[3], s), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(mul2(t[0], t[1], s, s), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(mul2(t[2], t[3], s, s), __NV_SATFINITE, __NV_E4M3);
   return lo | hi << 16;
 }
 
@@ -326,7 +333,10 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_mx8_kernel(const NormArgs a) 
           unpack<T, V>(Pair{{mine[tensor + 2 * k * blockDim.x + flip], mine[tensor + 2 * k * blockDim.x + 1 - flip]}}, r);
           // the residual stream is kept in the activation's type: the sum is rounded before it is normalised
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i] += r[i];
+          for (int i = 0; i < V; i += 2) {
+            const float2 t = add2(v[i], v[i + 1], r[i], r[i + 1]);
+            v[i] = t.x, v[i + 1] = t.y;
+          }
           raw[k] = round_to<T, V>(v);
           store_pair(res_out + c, raw[k]);
         }
@@ -371,7 +381,10 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_mx8_kernel(const NormArgs a) 
           float w[V];
           unpack<T, V>(load_pair(static_cast<const T*>(a.w) + c), w);
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i] *= w[i];
+          for (int i = 0; i < V; i += 2) {
+            const float2 t = mul2(v[i], v[i + 1], w[i], w[i + 1]);
+            v[i] = t.x, v[i + 1] = t.y;
+          }
         }
       } else {
 #pragma unroll
