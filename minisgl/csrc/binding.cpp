@@ -1748,6 +1748,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def(py::init<at::Tensor, at::Tensor, c10::optional<at::Tensor>, at::Tensor, int64_t, int64_t, int64_t, at::Tensor>());
   m.def("int4_pack", &int4_pack);
   m.def("int4_linear", &int4_linear);
+  m.def("int4_rings", &minisgl::int4_rings);
   m.def("moe_experts_mx", &moe_experts_mx, py::arg("out"), py::arg("x"), py::arg("w1q"), py::arg("w1sb"),
         py::arg("w2q"), py::arg("w2sb"), py::arg("topk_w"), py::arg("topk_ids"), py::arg("tile"), py::arg("xq"),
         py::arg("xsf"), py::arg("h"), py::arg("hq"), py::arg("hsf"), py::arg("ys"), py::arg("sorted_pair"),

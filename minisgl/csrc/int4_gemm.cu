@@ -57,13 +57,19 @@ constexpr int kCodes = 8 * 1024;  // 128 rows x 128 columns
 template <int BN>
 struct GSmem {
   static constexpr int kX = BN * 256;  // one step of x, as two 64-column tiles
-  static constexpr int kXs = BN == 256 || BN == 128 ? 3 : BN == 192 ? 4 : 6;
-  static constexpr int kPs = BN >= 192 ? 3 : 6;
+  // 192 rows: 3 steps of x and 4 of codes 193 us at 2000 x 8192 x 7168 and 384 at 1536 x 5120 x 25600 (B200), 4 and 2 191
+  // and 398
+  static constexpr int kXs = BN >= 128 ? 3 : 6;
+  static constexpr int kPs = BN == 256 ? 2 : BN == 192 ? 4 : 6;
   static constexpr int kAs = BN == 192 ? 2 : BN == 32 ? 3 : 4;  // steps of weights in tensor memory
-  // converter sets of 8 warps, which take the steps in turn; not more than steps in tensor memory, or a set could meet
-  // a slot's barrier two phases away. Three were no faster than two: the instructions they issue are the bound.
+  // Converter sets of 8 warps, which take the steps in turn. A wait by parity is sure only for a waiter that knows the
+  // phase before the awaited one to have ended: while that is open it passes too. So each slot of codes belongs to one
+  // set, which has then waited for every earlier fill of it (copies may land in any order; with three slots a set could
+  // read one whose last but one fill, the other set's, was still on its way). Slots in tensor memory change sets, but
+  // MMAs end in order, and the set's step before waited for step n - kAs - kSets, which is no earlier than n - 2 kAs.
+  // Three sets were no faster than two.
   static constexpr int kSets = 2;
-  static_assert(kSets <= kAs && kSets <= kPs, "turns");
+  static_assert(kPs % kSets == 0 && kSets <= kAs, "turns");
   static constexpr int kThreads = 256 + kSets * 256;
   static constexpr int kAcc = BN == 256 ? 1 : 2;  // sums in tensor memory; 256 columns leave room for one (one tile a CTA)
   static constexpr int kPt = kXs * kX;
@@ -669,7 +675,17 @@ void launch_group(const GArgs& a, const void* scales, const void* x, int64_t ldx
   }
 }
 
+template <int BN>
+std::array<int, 5> ring_of() {
+  using L = GSmem<BN>;
+  return {BN, L::kXs, L::kPs, L::kAs, L::kSets};
+}
+
 }  // namespace
+
+std::vector<std::array<int, 5>> int4_rings() {
+  return {ring_of<32>(), ring_of<64>(), ring_of<128>(), ring_of<192>(), ring_of<256>()};
+}
 
 void launch_int4_gemm(const Int4LinearArgs& r, cudaStream_t s) {
   if (r.M <= 0) return;

@@ -6,6 +6,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <array>
+#include <vector>
+
 namespace minisgl {
 
 enum class DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
@@ -469,6 +472,8 @@ struct Int4LinearArgs {
 void launch_int4_pack(void* packed, const uint8_t* codes, int64_t n, int64_t k, int64_t ld, cudaStream_t s);
 // false (nothing launched): more than kInt4FewRows rows, or too many columns for x to fit shared memory
 bool launch_int4_stream(const Int4LinearArgs& a, cudaStream_t s);
+// the slots of the many-row product's tiles: {rows of x, slots of x, of codes, of unpacked weights, converter sets}
+std::vector<std::array<int, 5>> int4_rings();
 // any number of rows; E4M3 rows need x_wide
 void launch_int4_gemm(const Int4LinearArgs& a, cudaStream_t s);
 
