@@ -1749,6 +1749,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int4_pack", &int4_pack);
   m.def("int4_linear", &int4_linear);
   m.def("int4_rings", &minisgl::int4_rings);
+  m.def("int4_tiles", [](int64_t m, int64_t n, int64_t k, int64_t group, bool half) {
+    MSG_CHECK(m > 0 && m < (1ll << 31) && n > 0 && n <= (1ll << 30) && k > 0 && k <= (1ll << 30),
+              "int4_tiles: size out of range");
+    MSG_CHECK(group == 32 || group == 64 || group == 128, "int4_tiles: group of 32, 64 or 128, got ", group);
+    return minisgl::int4_tiles(m, n, k, static_cast<int>(group), half);
+  });
   m.def("moe_experts_mx", &moe_experts_mx, py::arg("out"), py::arg("x"), py::arg("w1q"), py::arg("w1sb"),
         py::arg("w2q"), py::arg("w2sb"), py::arg("topk_w"), py::arg("topk_ids"), py::arg("tile"), py::arg("xq"),
         py::arg("xsf"), py::arg("h"), py::arg("hq"), py::arg("hsf"), py::arg("ys"), py::arg("sorted_pair"),

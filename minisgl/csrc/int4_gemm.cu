@@ -40,6 +40,7 @@
 #include <atomic>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.h"
@@ -633,14 +634,20 @@ void launch_bn(GArgs a, const GPlan& p, const CUtensorMap* tw, const CUtensorMap
 }
 
 template <int G, bool HALF>
-void launch_type(GArgs a, const void* scales, const void* x, int64_t ldx, int64_t K, cudaStream_t s) {
-  constexpr int group = G;
+GPlan plan_type(const GArgs& a) {
   GPlan p{0, 1, 0, -1};
   plan_bn<32, G, HALF>(a, p);
   plan_bn<64, G, HALF>(a, p);
   plan_bn<128, G, HALF>(a, p);
   plan_bn<192, G, HALF>(a, p);
   plan_bn<256, G, HALF>(a, p);
+  return p;
+}
+
+template <int G, bool HALF>
+void launch_type(GArgs a, const void* scales, const void* x, int64_t ldx, int64_t K, cudaStream_t s) {
+  constexpr int group = G;
+  const GPlan p = plan_type<G, HALF>(a);
   const int best = p.bn;
   a.x_blocks = K % 64 == 0;
   const CUtensorMap tm = a.x_blocks ? make_tmap_bf16_kblocks(x, a.M, K, ldx, best, 2) : make_tmap_bf16_2d_sw128(x, a.M, K, ldx, best);
@@ -685,6 +692,18 @@ std::array<int, 5> ring_of() {
 
 std::vector<std::array<int, 5>> int4_rings() {
   return {ring_of<32>(), ring_of<64>(), ring_of<128>(), ring_of<192>(), ring_of<256>()};
+}
+
+std::pair<int, int> int4_tiles(int64_t M, int64_t N, int64_t K, int group, bool half) {
+  GArgs a{};
+  a.M = static_cast<int>(M), a.N = static_cast<int>(N);
+  a.steps = static_cast<int>((K + 127) / 128), a.n_tiles = static_cast<int>((N + kRows - 1) / kRows);
+  const auto plan = [&](auto h) {
+    constexpr bool H = decltype(h)::value;
+    return group == 32 ? plan_type<32, H>(a) : group == 64 ? plan_type<64, H>(a) : plan_type<128, H>(a);
+  };
+  const GPlan p = half ? plan(std::true_type{}) : plan(std::false_type{});
+  return {p.bn, p.S};
 }
 
 void launch_int4_gemm(const Int4LinearArgs& r, cudaStream_t s) {

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <array>
+#include <utility>
 #include <vector>
 
 namespace minisgl {
@@ -474,6 +475,8 @@ void launch_int4_pack(void* packed, const uint8_t* codes, int64_t n, int64_t k, 
 bool launch_int4_stream(const Int4LinearArgs& a, cudaStream_t s);
 // the slots of the many-row product's tiles: {rows of x, slots of x, of codes, of unpacked weights, converter sets}
 std::vector<std::array<int, 5>> int4_rings();
+// how launch_int4_gemm cuts a product on the current device: rows of x in a tile, CTAs that share its columns
+std::pair<int, int> int4_tiles(int64_t M, int64_t N, int64_t K, int group, bool half);
 // any number of rows; E4M3 rows need x_wide
 void launch_int4_gemm(const Int4LinearArgs& a, cudaStream_t s);
 
