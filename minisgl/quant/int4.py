@@ -49,33 +49,66 @@ class Int4Weight:
     [tiles, groups rounded up to even, 8] or None, tiles = 2 ceil(N / 32), groups =
     128 ceil(K / 128) / group;
     ``row_pow`` float32 [16 tiles]: the power of two at or below a row's largest scale
-    (1 where that is 0), which fp16 products take out of the row."""
+    (1 where that is 0), which fp16 products take out of the row. The parts are not
+    replaced, since the native handle and captured graphs hold them; ``copy_`` puts
+    another weight of the same form into them. What is written to ``scales`` by hand
+    (by torch: a tensor's version shows it) the calls after it see; a graph captured
+    before sees it too, but keeps fp16 rows' powers, so there ``copy_`` is the way."""
 
-    __slots__ = ("_packed", "_scales", "_zeros", "_row_pow", "_n", "_k", "_group", "_handle")
+    __slots__ = ("_packed", "_scales", "_zeros", "_row_pow", "_n", "_k", "_group", "_handle", "_version")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor],
                  row_pow: torch.Tensor, n: int, k: int, group: int) -> None:
+        if scales.is_inference():  # those have no version
+            with torch.inference_mode(False):
+                scales = scales.clone()
         self._packed, self._scales, self._zeros, self._row_pow = packed, scales, zeros, row_pow
         self._n, self._k, self._group = n, k, group
         self._handle = None
+        self._version = scales._version  # of the scales that row_pow is of
 
-    # the parts may be written into, not replaced: the native handle holds them
     packed = property(lambda self: self._packed)
     scales = property(lambda self: self._scales)
     zeros = property(lambda self: self._zeros)
-    row_pow = property(lambda self: self._row_pow)
     n = property(lambda self: self._n)
     k = property(lambda self: self._k)
     group = property(lambda self: self._group)
 
-    def native(self):
-        """The weight as one argument of the native calls (made on the first)."""
-        if self._handle is None:
-            from minisgl import ops
+    @property
+    def row_pow(self) -> torch.Tensor:
+        return self._row_pow if self._scales._version == self._version else _row_powers(self._scales)
 
-            self._handle = ops.native().Int4Handle(self.packed, self.scales, self.zeros, self.row_pow, self.n, self.k,
-                                                   self.group, ops.error_word(self.device))
+    def native(self, powers: bool = False):
+        """The weight as one argument of the native calls (made on the first). ``powers``: for calls that read the
+        rows' powers; where the scales were written since, with powers of this call's own."""
+        if powers and self._scales._version != self._version:
+            return self._native_with(self.row_pow)
+        if self._handle is None:
+            self._handle = self._native_with(self._row_pow)
         return self._handle
+
+    def _native_with(self, row_pow: torch.Tensor):
+        from minisgl import ops
+
+        return ops.native().Int4Handle(self.packed, self.scales, self.zeros, row_pow, self.n, self.k, self.group,
+                                       ops.error_word(self.device))
+
+    def copy_(self, src: "Int4Weight") -> "Int4Weight":
+        """Put the values of ``src`` (same n, k, group, type of the scales, and zero points or none) into this
+        weight's parts, which captured graphs go on reading."""
+        if not isinstance(src, Int4Weight) or self._form() != src._form():
+            raise ValueError("Int4Weight.copy_: another weight of the same n, k, group and scale type, "
+                             "with zero points where this one has them")
+        self._packed.copy_(src.packed)
+        self._scales.copy_(src.scales)
+        if self._zeros is not None:
+            self._zeros.copy_(src.zeros)
+        self._row_pow.copy_(src.row_pow)
+        self._version = self._scales._version
+        return self
+
+    def _form(self):
+        return self.n, self.k, self.group, self.scales.dtype, self.zeros is not None
 
     def __reduce__(self):
         return Int4Weight, (self.packed, self.scales, self.zeros, self.row_pow, self.n, self.k, self.group)
@@ -97,6 +130,14 @@ def _tile_rows(t: torch.Tensor, groups: int) -> torch.Tensor:
     full = t.new_zeros(tiles * _TILE, groups)
     full[:n, :g] = t
     return full.view(tiles, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
+
+
+def _row_powers(tiled: torch.Tensor) -> torch.Tensor:
+    """Scales [tiles, groups, 8, 2] -> the power of two at or below each row's largest, 1 where that is 0 or not finite."""
+    top = tiled.float().abs().amax(1).transpose(1, 2).reshape(-1)  # [tile, g, h] -> row
+    live = (top > 0) & (top <= torch.finfo(torch.float32).max)
+    power = (top.view(torch.int32) & 0x7F800000).view(torch.float32)  # the exponent's bits alone
+    return torch.where(live & (power > 0), power, 1.0)
 
 
 def _pack_reference(codes: torch.Tensor) -> torch.Tensor:
@@ -154,11 +195,7 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
         z = _tile_rows(zeros, groups + groups % 2)  # whole 16-byte rows
         z = z[..., 0] | (z[..., 1] << 4)
     tiled = _tile_rows(scales, groups)
-    top = tiled.float().abs().amax(1).transpose(1, 2).reshape(-1)  # [tile, g, h] -> row
-    live = (top > 0) & (top <= torch.finfo(torch.float32).max)
-    power = (top.view(torch.int32) & 0x7F800000).view(torch.float32)  # the exponent's bits alone
-    row_pow = torch.where(live & (power > 0), power, 1.0)
-    w = Int4Weight(packed, tiled, z, row_pow, n, k, group)
+    w = Int4Weight(packed, tiled, z, _row_powers(tiled), n, k, group)
     if codes.is_cuda:
         w.native()  # checked and registered here, not inside somebody's graph capture
     return w

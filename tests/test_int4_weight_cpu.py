@@ -1,0 +1,50 @@
+"""4-bit weights whose parts are written after they were made, on the CPU."""
+
+import copy
+import pickle
+
+import pytest
+import torch
+
+from minisgl.quant import Int4Weight, dequantize_int4, int4_weight
+
+
+def _parts(n=40, k=264, group=64, zeros=True, seed=0, factor=1.0, dtype=torch.float16):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    scales = ((torch.rand(n, -(-k // group), generator=g) * 0.02 + 0.001) * factor).to(dtype)
+    z = torch.randint(0, 16, scales.shape, generator=g, dtype=torch.uint8) if zeros else None
+    return codes, scales, z, group
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_row_powers_follow_the_scales(inference):
+    with torch.inference_mode(inference):
+        w = int4_weight(*_parts())
+        other = int4_weight(*_parts(factor=1e3))
+        assert not torch.equal(w.row_pow, other.row_pow)
+        w.scales.copy_(other.scales)
+        for made in (w, w.to("cpu"), copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+            assert torch.equal(made.row_pow, other.row_pow)
+            assert torch.equal(made.scales, other.scales)
+
+
+def test_copy_into_a_weight():
+    w, new = int4_weight(*_parts()), int4_weight(*_parts(seed=1, factor=30.0))
+    parts = [t.data_ptr() for t in (w.packed, w.scales, w.zeros, w.row_pow)]
+    assert w.copy_(new) is w
+    assert [t.data_ptr() for t in (w.packed, w.scales, w.zeros, w.row_pow)] == parts
+    assert torch.equal(dequantize_int4(w), dequantize_int4(new)) and torch.equal(w.row_pow, new.row_pow)
+    w.scales.mul_(2)
+    new.copy_(w)  # from one whose own powers were left behind
+    assert torch.equal(new.row_pow, w.row_pow) and torch.equal(new.scales, w.scales)
+
+
+def test_copy_refusals():
+    w = int4_weight(*_parts())
+    for other in (dict(n=41), dict(n=80), dict(k=272), dict(group=32), dict(zeros=False), dict(dtype=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            w.copy_(int4_weight(*_parts(**other)))
+    with pytest.raises((ValueError, TypeError, AttributeError)):
+        w.copy_(torch.zeros(3))
+    assert isinstance(w, Int4Weight) and torch.equal(dequantize_int4(w), dequantize_int4(int4_weight(*_parts())))

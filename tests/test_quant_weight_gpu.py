@@ -1,0 +1,116 @@
+"""4-bit weights whose parts are written after they were made: products that read the rows' powers of two."""
+
+import copy
+
+import pytest
+import torch
+
+from minisgl import ops
+from minisgl.quant import int4_weight, quantize_int4
+from test_quant_tiles_gpu import _gen, _weight, check
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("factor,dtype", [(1e-6, torch.bfloat16), (1e6, torch.bfloat16), (1e3, torch.float16)])
+@pytest.mark.parametrize("m,k", [(40, 1032), (1, 700000)])  # the second: one row that takes the tiles
+def test_scales_written_after_the_weight_was_made(m, k, factor, dtype):
+    w = _weight(200 if m > 1 else 16, k, 64, True, 1, dtype)
+    x = (torch.randn(m, k, generator=_gen(m), device=DEV) * 1e-2).half()
+    check(ops.int4_linear(x, w, out_dtype=torch.float32), x.double(), w, None, True)
+    w.scales.copy_((w.scales.float() * factor).to(dtype))
+    fresh = int4_weight_like(w)
+    for made in (w, w.to(DEV), copy.deepcopy(w)):
+        y = ops.int4_linear(x, made, out_dtype=torch.float32)
+        check(y, x.double(), fresh, None, True)
+        assert torch.equal(y, ops.int4_linear(x, fresh, out_dtype=torch.float32))
+    ops.check_device_errors(torch.device(DEV))
+
+
+def int4_weight_like(w):
+    """The same weight, made from its scales as they are."""
+    from minisgl.quant import int4_codes
+
+    def rows(t):
+        return t.permute(0, 3, 2, 1).reshape(-1, t.shape[1])[: w.n, : -(-w.k // w.group)].contiguous()
+
+    c = int4_codes(w)
+    z = None if w.zeros is None else rows(torch.stack([w.zeros & 15, w.zeros >> 4], dim=-1))
+    return int4_weight((c[:, 0::2] | (c[:, 1::2] << 4)).contiguous(), rows(w.scales), z, w.group)
+
+
+@pytest.mark.parametrize("m", [4, 40])
+def test_a_captured_product_takes_the_weight_copied_in(m):
+    n, k = 200, 1032
+    w = _weight(n, k, 64, True, 1, torch.float16)
+    x = (torch.randn(m, k, generator=_gen(m), device=DEV) * 1e-2).half()
+    ops.int4_linear(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.int4_linear(x, w, out_dtype=torch.float32)
+    for seed, factor in [(2, 1e4), (3, 1.0), (4, 1e-3)]:
+        new = _weight(n, k, 64, True, seed, torch.float16)
+        new.scales.copy_((new.scales.float() * factor).half())
+        w.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.int4_linear(x, int4_weight_like(new), out_dtype=torch.float32))
+
+
+def test_scales_written_inside_a_capture():
+    w = _weight(200, 1032, 64, True, 1, torch.float16)
+    x = (torch.randn(40, 1032, generator=_gen(1), device=DEV) * 1e-2).half()
+    new = w.scales.clone()
+    ops.int4_linear(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.scales.copy_(new)
+        y = ops.int4_linear(x, w, out_dtype=torch.float32)
+    for factor in (1e4, 1e-7):
+        new.mul_(factor)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.int4_linear(x, int4_weight_like(w), out_dtype=torch.float32))
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_two_graphs_replayed_beside_one_another(rows):
+    """Norm, product, activation and product captured twice, each graph with tensors of its own that live as long as it
+    (the residual stream among them, which the graph writes), replayed on two streams at once."""
+    h, d = 512, 768
+    g = _gen(20)
+    norm = torch.ones(h, device=DEV, dtype=torch.bfloat16)
+    up, down = (quantize_int4(torch.randn(*s, generator=g, device=DEV) * 0.05, 64) for s in [(2 * d, h), (h, d)])
+
+    def layer(x, res):
+        q, sf = ops.rmsnorm_mx8(x, norm, 1e-6, residual=res)
+        a, asf = ops.silu_and_mul_mx8(ops.int4_linear(q, up, x_scales=sf))
+        return q, sf, res, a, asf, ops.int4_linear(a, down, x_scales=asf)
+
+    sides = []
+    for _ in range(2):
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        x, start = (torch.randn(rows, h, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+        res = start.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            res.copy_(start)
+            out = layer(x, res)
+        sides.append((stream, graph, x, start, out))
+    for turn in range(20):
+        want = []
+        for _, _, x, start, _ in sides:
+            x.copy_(torch.randn(rows, h, generator=g, device=DEV))
+            want.append([t.clone() for t in layer(x, start.clone())])
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for stream, graph, *_ in sides:
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for side, ws in zip(sides, want):
+            assert all(torch.equal(a, b) for a, b in zip(side[4], ws)), turn
+    ops.check_device_errors(torch.device(DEV))
