@@ -66,6 +66,8 @@ class Int4Weight:
         self._n, self._k, self._group = n, k, group
         self._handle = None
         self._version = scales._version  # of the scales that row_pow is of
+        if packed.is_cuda:
+            self.native()  # checked, and its device's error word made, here and not inside somebody's graph capture
 
     packed = property(lambda self: self._packed)
     scales = property(lambda self: self._scales)
@@ -79,7 +81,7 @@ class Int4Weight:
         return self._row_pow if self._scales._version == self._version else _row_powers(self._scales)
 
     def native(self, powers: bool = False):
-        """The weight as one argument of the native calls (made on the first). ``powers``: for calls that read the
+        """The weight as one argument of the native calls (made with a CUDA weight). ``powers``: for calls that read the
         rows' powers; where the scales were written since, with powers of this call's own."""
         if powers and self._scales._version != self._version:
             return self._native_with(self.row_pow)
@@ -195,10 +197,7 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
         z = _tile_rows(zeros, groups + groups % 2)  # whole 16-byte rows
         z = z[..., 0] | (z[..., 1] << 4)
     tiled = _tile_rows(scales, groups)
-    w = Int4Weight(packed, tiled, z, _row_powers(tiled), n, k, group)
-    if codes.is_cuda:
-        w.native()  # checked and registered here, not inside somebody's graph capture
-    return w
+    return Int4Weight(packed, tiled, z, _row_powers(tiled), n, k, group)
 
 
 def int4_codes(w: Int4Weight) -> torch.Tensor:

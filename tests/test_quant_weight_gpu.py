@@ -1,6 +1,7 @@
 """4-bit weights whose parts are written after they were made: products that read the rows' powers of two."""
 
 import copy
+import pickle
 
 import pytest
 import torch
@@ -114,3 +115,29 @@ def test_two_graphs_replayed_beside_one_another(rows):
         for side, ws in zip(sides, want):
             assert all(torch.equal(a, b) for a, b in zip(side[4], ws)), turn
     ops.check_device_errors(torch.device(DEV))
+
+
+@pytest.mark.parametrize("how", ["to", "pickle", "copy"])
+@pytest.mark.parametrize("m", [3, 40])
+def test_a_weight_that_was_moved_is_ready_for_a_capture(monkeypatch, how, m):
+    """The error word that its calls write to is not made inside a capture, where each replay would clear it."""
+    w = _weight(200, 1032, 64, True, 1, torch.float16)
+    x = (torch.randn(m, 1032, generator=_gen(1), device=DEV) * 1e-2).half()
+    want = ops.int4_linear(x, w)
+    ops.check_device_errors(torch.device(DEV))
+    data, cpu = pickle.dumps(w), w.to("cpu")
+    monkeypatch.setattr(ops, "_ERR_WORDS", {})  # as in a process that has used no kernel yet
+    moved = cpu.to(DEV) if how == "to" else pickle.loads(data) if how == "pickle" else copy.deepcopy(w)
+    assert len(ops._ERR_WORDS) == 1
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.int4_linear(x, moved)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+    word = ops.error_word(torch.device(DEV))
+    word[0] = 77
+    graph.replay()
+    assert word[0].item() == 77
+    word.zero_()
