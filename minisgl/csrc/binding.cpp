@@ -637,9 +637,11 @@ at::Tensor int4_pack(const at::Tensor& codes) {
   return packed;
 }
 
-at::Tensor int4_linear(const at::Tensor& x, const Int4Handle& w, const c10::optional<at::Tensor>& bias,
-                       const c10::optional<at::Tensor>& out_, const c10::optional<at::ScalarType>& out_dtype,
-                       const c10::optional<at::Tensor>& x_scales) {
+// The output and how many kernels it took.
+std::pair<at::Tensor, int> int4_linear(const at::Tensor& x, const Int4Handle& w, const c10::optional<at::Tensor>& bias,
+                                       const c10::optional<at::Tensor>& out_,
+                                       const c10::optional<at::ScalarType>& out_dtype,
+                                       const c10::optional<at::Tensor>& x_scales) {
   const int64_t N = w.N, K = w.K;
   MSG_CHECK(x.dim() == 2 && x.size(1) == K, "int4_linear: x must be [M, ", K, "], got ", x.sizes());
   check_cuda(x, "x");
@@ -697,15 +699,14 @@ at::Tensor int4_linear(const at::Tensor& x, const Int4Handle& w, const c10::opti
   a.scale_type = dtype_of(w.scales);
   a.out_type = dtype_of(out);
   a.err = err_ptr(w.err);
-  if (M == 0) return out;
-  if (!minisgl::launch_int4_stream(a, stream_of(x))) {
-    if (x_scales.has_value()) {  // MXFP8 rows are widened to bf16 for the tensor cores' tiles
-      x_wide = new_beside(x, {M, K}, at::kBFloat16);
-      a.x_wide = x_wide.data_ptr();
-    }
-    minisgl::launch_int4_gemm(a, stream_of(x));
+  if (M == 0) return {out, 0};
+  if (minisgl::launch_int4_stream(a, stream_of(x))) return {out, 1};
+  if (x_scales.has_value()) {  // MXFP8 rows are widened to bf16 for the tensor cores' tiles
+    x_wide = new_beside(x, {M, K}, at::kBFloat16);
+    a.x_wide = x_wide.data_ptr();
   }
-  return out;
+  minisgl::launch_int4_gemm(a, stream_of(x));
+  return {out, x_scales.has_value() ? 2 : 1};
 }
 
 // Block-scaled MX routed experts: align -> gather + MXFP8 quantise -> gate_up

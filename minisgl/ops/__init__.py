@@ -362,8 +362,9 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
     to 128 columns) and groups in fp32; longer batches sum fp32 products of
     the weight rounded once to x's 16-bit type."""
     if x.is_cuda:
-        _count(2 if x_scales is not None and x.shape[0] > 8 else 1)  # the MXFP8 rows of a long batch are widened first
-        return native().int4_linear(x, w.native(x.dtype == torch.float16), bias, out, out_dtype, x_scales)
+        y, launches = native().int4_linear(x, w.native(x.dtype == torch.float16), bias, out, out_dtype, x_scales)
+        _count(launches)
+        return y
     if x.dim() != 2 or x.shape[1] != w.k:
         raise ValueError(f"int4_linear: x must be [M, {w.k}], got {tuple(x.shape)}")
     if (x.dtype == torch.uint8) != (x_scales is not None):

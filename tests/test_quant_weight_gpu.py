@@ -141,3 +141,20 @@ def test_a_weight_that_was_moved_is_ready_for_a_capture(monkeypatch, how, m):
     graph.replay()
     assert word[0].item() == 77
     word.zero_()
+
+
+# MXFP8 rows that take the tiles are widened by a kernel of their own: more than 8, or too wide to stream
+@pytest.mark.parametrize("m,k,kind,launches", [(0, 1024, "bf16", 0), (8, 1024, "mx8", 1), (9, 1024, "mx8", 2),
+                                               (40, 1024, "bf16", 1), (1, 700000 // 32 * 32, "mx8", 2),
+                                               (1, 700000, "bf16", 1)])
+def test_launches_are_counted_as_they_happen(m, k, kind, launches):
+    w = _weight(32, k, 64, False, 1, torch.bfloat16)
+    if kind == "mx8":
+        x = torch.randint(0, 0x7E, (m, k), device=DEV, dtype=torch.uint8)
+        scales = torch.full((m, k // 32), 120, device=DEV, dtype=torch.uint8)
+    else:
+        x, scales = torch.zeros(m, k, device=DEV, dtype=torch.bfloat16), None
+    before = ops.LAUNCHES[0]
+    ops.int4_linear(x, w, x_scales=scales)
+    assert ops.LAUNCHES[0] - before == launches
+    ops.check_device_errors(torch.device(DEV))
