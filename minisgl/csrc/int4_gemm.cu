@@ -19,7 +19,8 @@
 //
 // W = (c - z) s is rounded once to bf16 (fp16): the one rounding besides those
 // of the float32 sums. fp16 weights are formed under each row's own power of
-// two, so that neither large nor tiny scales leave fp16's range.
+// two, which puts the row's largest scale into [2^11, 2^12): 15 of it fit fp16,
+// and scales down to 2^-25 of it stay normal (smaller ones lose bits).
 //
 // Few tiles (N small, M small): S CTAs of a cluster share a tile's columns and
 // add their sums through shared memory in rank order.

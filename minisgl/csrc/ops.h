@@ -458,7 +458,7 @@ struct Int4LinearArgs {
   const uint8_t* packed;    // [tiles = 2 ceil(N / 32), 2 ceil(K / 128), 512]
   const void* scales;       // bf16 / fp16 [tiles, groups, 8, 2]
   const uint8_t* zeros;     // [tiles, groups rounded up to even, 8] or nullptr (8 everywhere)
-  const float* row_pow;     // [16 tiles]: a power of two near each row's largest scale
+  const float* row_pow;     // [16 tiles]: a power of two near 2^-11 of each row's largest scale
   const void* bias;         // [N] or nullptr
   void* x_wide;             // launch_int4_gemm with E4M3 rows: bf16 [M, K] scratch
   void* out;                // [M, N], row stride ldo

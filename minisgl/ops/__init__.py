@@ -360,7 +360,8 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
     type, bf16 for MXFP8 rows). Products of up to 8
     rows sum exact integers (x as 22-bit integers under a power of two common
     to 128 columns) and groups in fp32; longer batches sum fp32 products of
-    the weight rounded once to x's 16-bit type."""
+    the weight rounded once to x's 16-bit type (fp16: under a power of two of its
+    row, where scales below 2^-25 of the row's largest lose bits)."""
     if x.is_cuda:
         y, launches = native().int4_linear(x, w.native(x.dtype == torch.float16), bias, out, out_dtype, x_scales)
         _count(launches)

@@ -48,7 +48,7 @@ class Int4Weight:
     ``scales`` bf16 / fp16 [tiles, groups, 8, 2] and ``zeros`` uint8
     [tiles, groups rounded up to even, 8] or None, tiles = 2 ceil(N / 32), groups =
     128 ceil(K / 128) / group;
-    ``row_pow`` float32 [16 tiles]: the power of two at or below a row's largest scale
+    ``row_pow`` float32 [16 tiles]: a power of two near 2^-11 of a row's largest scale
     (1 where that is 0), which fp16 products take out of the row. The parts are not
     replaced, since the native handle and captured graphs hold them; ``copy_`` puts
     another weight of the same form into them. What is written to ``scales`` by hand
@@ -135,11 +135,13 @@ def _tile_rows(t: torch.Tensor, groups: int) -> torch.Tensor:
 
 
 def _row_powers(tiled: torch.Tensor) -> torch.Tensor:
-    """Scales [tiles, groups, 8, 2] -> the power of two at or below each row's largest, 1 where that is 0 or not finite."""
+    """Scales [tiles, groups, 8, 2] -> 2^-11 of the power of two at or below each row's largest (not below 2^-126, whose
+    inverse is a float32), 1 where that is 0 or not finite. Under it the row's scales are below 2^12, 15 of which fp16
+    holds, and those down to 2^-25 of the largest keep all of their bits."""
     top = tiled.float().abs().amax(1).transpose(1, 2).reshape(-1)  # [tile, g, h] -> row
     live = (top > 0) & (top <= torch.finfo(torch.float32).max)
     power = (top.view(torch.int32) & 0x7F800000).view(torch.float32)  # the exponent's bits alone
-    return torch.where(live & (power > 0), power, 1.0)
+    return torch.where(live, (power * 2.0 ** -11).clamp(min=2.0 ** -126), 1.0)
 
 
 def _pack_reference(codes: torch.Tensor) -> torch.Tensor:

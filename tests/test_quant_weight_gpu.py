@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from minisgl import ops
-from minisgl.quant import int4_weight, quantize_int4
+from minisgl.quant import dequantize_int4, int4_weight, quantize_int4
 from test_quant_tiles_gpu import _gen, _weight, check
 
 pytestmark = pytest.mark.gpu
@@ -158,3 +158,33 @@ def test_launches_are_counted_as_they_happen(m, k, kind, launches):
     ops.int4_linear(x, w, x_scales=scales)
     assert ops.LAUNCHES[0] - before == launches
     ops.check_device_errors(torch.device(DEV))
+
+
+@pytest.mark.parametrize("dtype,low", [(torch.bfloat16, 2.0 ** -25), (torch.bfloat16, 1.3e-7), (torch.float16, 2.0 ** -20),
+                                       (torch.float16, 1e-5)])
+@pytest.mark.parametrize("m", [8, 40])
+def test_groups_far_below_a_rows_largest_scale(m, dtype, low):
+    """fp16 rows that meet only the groups of small scales: the weights are as good as 16-bit weights are, whatever
+    the scale of a group that x is zero under. 16-bit weights: half a step, 2^-11 of each, and the sums."""
+    k = 1024
+    g = _gen(1)
+    codes = torch.randint(0, 256, (200, k // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales = (low * (1 + torch.rand(200, k // 64, generator=g, device=DEV))).to(dtype)
+    scales[:, 3] = 1.0
+    w = int4_weight(codes, scales, None, 64)
+    x = torch.randn(m, k, generator=g, device=DEV).half()
+    x[:, 192:256] = 0
+    y = ops.int4_linear(x, w, out_dtype=torch.float32).double()
+    wd, xd = dequantize_int4(w, torch.float64), x.double()
+    room = xd.abs() @ wd.abs().t() * (2 ** -11 + (k // 16 * 17 + 104) * 2 ** -23)
+    err = (y - xd @ wd.t()).abs()
+    assert bool((err <= room).all()), (err / room).max().item()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -133, 2.0 ** -126, 2.0 ** -120, 2.0 ** 89])
+def test_rows_of_the_ends_of_bf16(scale):
+    w = int4_weight(torch.full((40, 64), 0x99, device=DEV, dtype=torch.uint8),
+                    torch.full((40, 1), scale, device=DEV, dtype=torch.bfloat16), None, 128)  # every code is 9: W = scale
+    x = torch.ones(16, 128, device=DEV, dtype=torch.float16) * 2.0 ** 10
+    y = ops.int4_linear(x, w, out_dtype=torch.float32)
+    assert torch.equal(y, torch.full_like(y, 2.0 ** 17 * scale))
