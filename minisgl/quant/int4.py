@@ -35,6 +35,7 @@ from typing import Optional
 import torch
 
 GROUPS = (32, 64, 128)
+MAX_SCALE = 2.0 ** 90  # times a group's integer sum, 2^37 at most, it is still a float32 (products of few rows)
 _TILE, _BLOCK, _STEP = 16, 64, 128  # rows are padded to two tiles, columns to a step
 
 
@@ -167,8 +168,9 @@ def _pack_reference(codes: torch.Tensor) -> torch.Tensor:
 def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
                 group: int = 128) -> Int4Weight:
     """``codes`` uint8 [N, K / 2] (column 2i in the low nibble of byte i),
-    ``scales`` bf16 / fp16 [N, ceil(K / group)], ``zeros`` uint8 (0..15) of the
-    same shape or None (8 everywhere) -> the kernels' layout, on the same device."""
+    ``scales`` bf16 / fp16 [N, ceil(K / group)], finite and not above 2^90,
+    ``zeros`` uint8 (0..15) of the same shape or None (8 everywhere) -> the
+    kernels' layout, on the same device."""
     if codes.dim() != 2 or codes.dtype != torch.uint8:
         raise ValueError("int4_weight: codes must be uint8 [N, K / 2]")
     n, k = codes.shape[0], 2 * codes.shape[1]
@@ -185,6 +187,8 @@ def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
         raise ValueError("int4_weight: codes, scales and zeros must be on one device")
     if zeros is not None and bool((zeros > 15).any()):
         raise ValueError("int4_weight: zero points must be 0..15")
+    if not bool((scales.abs() <= (MAX_SCALE if scales.dtype == torch.bfloat16 else 65504.0)).all()):
+        raise ValueError("int4_weight: scales must be finite and not above 2^90 in magnitude")
     if codes.is_cuda:
         from minisgl import ops
 

@@ -6,7 +6,7 @@ import pickle
 import pytest
 import torch
 
-from minisgl.quant import Int4Weight, dequantize_int4, int4_weight
+from minisgl.quant import Int4Weight, dequantize_int4, int4_weight, quantize_int4
 
 
 def _parts(n=40, k=264, group=64, zeros=True, seed=0, factor=1.0, dtype=torch.float16):
@@ -48,3 +48,27 @@ def test_copy_refusals():
     with pytest.raises((ValueError, TypeError, AttributeError)):
         w.copy_(torch.zeros(3))
     assert isinstance(w, Int4Weight) and torch.equal(dequantize_int4(w), dequantize_int4(int4_weight(*_parts())))
+
+
+@pytest.mark.parametrize("scale,dtype", [(2.0 ** 91, torch.bfloat16), (-(2.0 ** 91), torch.bfloat16),
+                                         (float("inf"), torch.bfloat16), (float("nan"), torch.bfloat16),
+                                         (float("inf"), torch.float16), (float("nan"), torch.float16)])
+def test_scales_beyond_the_products_are_refused(scale, dtype):
+    codes, scales, z, group = _parts(dtype=dtype)
+    scales[3, 1] = 2.0 ** 90 if dtype == torch.bfloat16 else 65504.0
+    int4_weight(codes, scales, z, group)
+    scales[3, 1] = scale
+    with pytest.raises(ValueError, match="finite"):
+        int4_weight(codes, scales, z, group)
+
+
+def test_weights_too_large_for_their_scales_are_refused():
+    w = torch.full((4, 64), 7e5)
+    quantize_int4(w, 64)
+    with pytest.raises(ValueError, match="finite"):
+        quantize_int4(w, 64, scale_dtype=torch.float16)  # 10^5 is beyond fp16
+    with pytest.raises(ValueError, match="finite"):
+        quantize_int4(w * 1e30, 64)
+    w[1, 3] = float("nan")
+    with pytest.raises(ValueError, match="finite"):
+        quantize_int4(w, 64)

@@ -188,3 +188,14 @@ def test_rows_of_the_ends_of_bf16(scale):
     x = torch.ones(16, 128, device=DEV, dtype=torch.float16) * 2.0 ** 10
     y = ops.int4_linear(x, w, out_dtype=torch.float32)
     assert torch.equal(y, torch.full_like(y, 2.0 ** 17 * scale))
+
+
+@pytest.mark.parametrize("m", [1, 8, 16])
+def test_the_largest_scales(m):
+    """A group's sum under the largest scale that a weight may have: 128 columns, codes 15 away from their zero point."""
+    w = int4_weight(torch.full((40, 64), 0xFF, device=DEV, dtype=torch.uint8),
+                    torch.full((40, 1), 2.0 ** 90, device=DEV, dtype=torch.bfloat16),
+                    torch.zeros(40, 1, device=DEV, dtype=torch.uint8), 128)
+    x = torch.full((m, 128), 1.9921875, device=DEV, dtype=torch.bfloat16)  # the largest below 2
+    y = ops.int4_linear(x, w, out_dtype=torch.float32)
+    assert torch.equal(y, torch.full_like(y, 1.9921875 * 128 * 15 * 2.0 ** 90))
