@@ -79,15 +79,16 @@ def _size(rows, kind, k, group, half):
     raise AssertionError(f"no size takes tiles of {rows} rows, {kind}")
 
 
+# x comes in one copy a step where K is a multiple of 64, else in two
 @pytest.mark.parametrize("rows,tiles", [(32, "one"), (32, "cluster"), (64, "one"), (64, "several"), (64, "cluster"),
                                         (128, "one"), (128, "several"), (128, "cluster"), (192, "one"),
                                         (192, "several"), (256, "one")])
-@pytest.mark.parametrize("kind,group,zeros,bias", [("bf16", 128, False, False), ("bf16", 32, True, True),
-                                                   ("fp16", 64, True, False), ("fp16", 128, False, True),
-                                                   ("mx8", 64, False, False)])
-def test_every_tile_width(rows, tiles, kind, group, zeros, bias):
-    """41 steps of 128 columns: every ring turns at least six times."""
-    k = 5152 if kind == "mx8" else 5128
+@pytest.mark.parametrize("kind,group,zeros,bias,k", [("bf16", 128, False, False, 5128), ("bf16", 32, True, True, 5128),
+                                                     ("fp16", 64, True, False, 5128), ("fp16", 128, False, True, 5128),
+                                                     ("mx8", 64, False, False, 5152), ("bf16", 128, True, False, 5120),
+                                                     ("fp16", 32, False, False, 5184), ("mx8", 128, True, True, 5120)])
+def test_every_tile_width(rows, tiles, kind, group, zeros, bias, k):
+    """40 or 41 steps of 128 columns: every ring turns at least six times."""
     half = kind == "fp16"
     t = torch.float16 if half else torch.bfloat16
     m, n = _size(rows, tiles, k, group, half)
@@ -158,3 +159,33 @@ def test_few_rows_as_wide_as_they_stream(m, k, group, zeros):
     assert bool((err <= room).all()), (err / room).max().item()
     rounded = xd @ rounded_weight(w, False).t()
     assert bool(((rounded - want).abs() > room).any())
+
+
+@pytest.mark.parametrize("m", [5, 40])
+def test_mx8_rows_of_wider_tensors(m):
+    """Rows and scales that ``rmsnorm_mx8`` wrote into parts of larger tensors."""
+    k, n = 1056, 200
+    w = _weight(n, k, 32, True, 2, torch.bfloat16)
+    q = torch.full((m + 2, k + 96), 0x7F, device=DEV, dtype=torch.uint8)[1:m + 1, 48:48 + k]
+    sf = torch.full((m + 2, k // 32 + 5), 0xFF, device=DEV, dtype=torch.uint8)[1:m + 1, 3:3 + k // 32]
+    ops.rmsnorm_mx8(torch.randn(m, k, generator=_gen(1), device=DEV), None, 1e-6, out=(q, sf))
+    y = ops.int4_linear(q, w, x_scales=sf, out_dtype=torch.float32)
+    assert torch.equal(y, ops.int4_linear(q.contiguous(), w, x_scales=sf.contiguous(), out_dtype=torch.float32))
+    if m > 8:
+        check(y, dequantize_mx8_rows(q, sf, torch.float64), w, None, False)
+    ops.check_device_errors(torch.device(DEV))
+
+
+@pytest.mark.parametrize("rows,cols", [(3, 96), (1500, 5120)])
+def test_residual_sum_over_the_norms_input(rows, cols):
+    """residual_out may be x itself, and x may be the residual stream too."""
+    g = _gen(rows)
+    x, res = (torch.randn(rows, cols, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    total = torch.empty_like(x)
+    want = ops.rmsnorm_mx8(x, None, 1e-6, residual=res, residual_out=total)
+    keep = x.clone()
+    got = ops.rmsnorm_mx8(x, None, 1e-6, residual=res, residual_out=x)
+    assert torch.equal(x, total) and all(torch.equal(a, b) for a, b in zip(got, want))
+    twice = (keep.float() * 2).to(torch.bfloat16)
+    got = ops.rmsnorm_mx8(keep, None, 1e-6, residual=keep)
+    assert torch.equal(keep, twice) and all(torch.equal(a, b) for a, b in zip(got, ops.rmsnorm_mx8(twice, None, 1e-6)))
