@@ -121,6 +121,7 @@ class Int4Weight:
         return self.packed.device
 
     def to(self, device) -> "Int4Weight":
+        device = torch.device(device)  # not a type: the parts keep theirs
         zeros = None if self.zeros is None else self.zeros.to(device)
         return Int4Weight(self.packed.to(device), self.scales.to(device), zeros, self.row_pow.to(device), self.n,
                           self.k, self.group)

@@ -72,3 +72,11 @@ def test_weights_too_large_for_their_scales_are_refused():
     w[1, 3] = float("nan")
     with pytest.raises(ValueError, match="finite"):
         quantize_int4(w, 64)
+
+
+def test_to_takes_a_device_alone():
+    w = int4_weight(*_parts())
+    for bad in (torch.float16, torch.zeros(1)):
+        with pytest.raises((TypeError, RuntimeError)):
+            w.to(bad)
+    assert w.to("cpu").packed.dtype == torch.uint8 and w.to(torch.device("cpu")).n == w.n
