@@ -322,6 +322,10 @@ def rmsnorm_mx8(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, residual
         return native().rmsnorm_mx8(x, w, eps, residual, residual_out, out)
     if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % 32 != 0:
         raise ValueError(f"rmsnorm_mx8: x must be [rows, a positive multiple of 32], got {tuple(x.shape)}")
+    if w is not None and (w.numel() != x.shape[1] or w.dtype != x.dtype):
+        raise ValueError(f"rmsnorm_mx8: w must be {x.dtype} with {x.shape[1]} elements")
+    if any(t is not None and (t.shape != x.shape or t.dtype != x.dtype) for t in (residual, residual_out)):
+        raise ValueError(f"rmsnorm_mx8: residual and residual_out must be {x.dtype} {tuple(x.shape)}")
     return _mx8_cpu(ref.rmsnorm_mx8(x, w, eps, residual, residual if residual_out is None else residual_out), out)
 
 
@@ -374,6 +378,10 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
         out_dtype = out.dtype if out is not None else x.dtype if x_scales is None else torch.bfloat16
     elif out is not None and out.dtype != out_dtype:
         raise ValueError(f"int4_linear: out is {out.dtype}, out_dtype {out_dtype}")
+    if out is not None and out.shape != (x.shape[0], w.n):
+        raise ValueError(f"int4_linear: out must be [{x.shape[0]}, {w.n}], got {tuple(out.shape)}")
+    if bias is not None and bias.numel() != w.n:
+        raise ValueError(f"int4_linear: bias must be a vector of {w.n} elements, got {tuple(bias.shape)}")
     y = ref.int4_linear(x, w, bias, out_dtype, x_scales)
     if out is not None:
         out.copy_(y)

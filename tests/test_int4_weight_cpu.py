@@ -6,6 +6,7 @@ import pickle
 import pytest
 import torch
 
+from minisgl import ops
 from minisgl.quant import Int4Weight, dequantize_int4, int4_weight, quantize_int4
 
 
@@ -80,3 +81,21 @@ def test_to_takes_a_device_alone():
         with pytest.raises((TypeError, RuntimeError)):
             w.to(bad)
     assert w.to("cpu").packed.dtype == torch.uint8 and w.to(torch.device("cpu")).n == w.n
+
+
+def test_shapes_that_the_cpu_form_refuses_as_the_kernels_do():
+    w = int4_weight(*_parts(n=40, k=264))
+    x = torch.zeros(1, 264, dtype=torch.float16)
+    for bad in (torch.zeros(3, 40, dtype=torch.float16), torch.zeros(40, dtype=torch.float16)):
+        with pytest.raises(ValueError, match="out must be"):
+            ops.int4_linear(x, w, out=bad)
+    for bias in (torch.zeros(1), torch.zeros(39)):
+        with pytest.raises(ValueError, match="bias must be"):
+            ops.int4_linear(x, w, bias)
+    y = torch.zeros(2, 64)
+    with pytest.raises(ValueError, match="residual"):
+        ops.rmsnorm_mx8(y, None, 1e-6, residual=torch.zeros(1, 64), residual_out=torch.zeros(2, 64))
+    with pytest.raises(ValueError, match="residual"):
+        ops.rmsnorm_mx8(y, None, 1e-6, residual=torch.zeros(2, 64), residual_out=torch.zeros(4, 2, 64))
+    with pytest.raises(ValueError, match="w must"):
+        ops.rmsnorm_mx8(y, torch.ones(1), 1e-6)
