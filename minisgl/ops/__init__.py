@@ -367,7 +367,8 @@ def int4_linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None, out: Op
     the weight rounded once to x's 16-bit type (fp16: under a power of two of its
     row, where scales below 2^-25 of the row's largest lose bits)."""
     if x.is_cuda:
-        y, launches = native().int4_linear(x, w.native(x.dtype == torch.float16), bias, out, out_dtype, x_scales)
+        handle = w.native(True) if x.dtype is torch.float16 else w.native()
+        y, launches = native().int4_linear(x, handle, bias, out, out_dtype, x_scales)
         _count(launches)
         return y
     if x.dim() != 2 or x.shape[1] != w.k:
