@@ -56,11 +56,10 @@ __device__ __forceinline__ float e8m0(uint32_t byte) {
 // The products are integer: a value of x under a power of two common to its
 // row's 128 columns is three 8-bit digits, a code minus 8 is a signed byte after
 // one mask, and the tensor cores sum 8-bit products exactly in 32 bits. That
-// takes 3 operations for 8 codes, where unpacking them to 16-bit floats takes 9:
-// at 6.5 TB/s an SM has about 90 cycles for the 2048 codes of a KB, and the
-// unpacking alone was the bound (B200, 1 x 51200 x 5120: 39 us with bf16
-// products). A group's scale (and z - 8 times the sum of x) is applied to its
-// finished sum.
+// takes 3 operations for 8 codes, where unpacking them to 16-bit floats takes 9
+// (B200, 1 x 51200 x 5120: 39 us with bf16 products, 30 so; at 6.5 TB/s an SM
+// has about 44 cycles for the 2048 codes of a KB). A group's scale (and z - 8
+// times the sum of x) is applied to its finished sum.
 //
 // A tile whose units lie in one warp's range is finished there. Where a range
 // starts or ends inside a tile, the warp parks its partial sums; after the one
@@ -71,10 +70,13 @@ __device__ __forceinline__ float e8m0(uint32_t byte) {
 //
 // Measured (B200, cold weights, bf16): 1 x 51200 x 5120 in groups of 128 29.9 us
 // (4.5 TB/s; a plain read of the bytes 20.6), 1 x 5120 x 25600 19.6, 8 x 5120 x
-// 25600 with zero points 24.9, 1 x 5120 x 5120 7.3. What bounds it is the issue of
-// instructions (some 120 a KB of codes, 1.7 a cycle and SM) and, in small calls,
-// about 4 us of launch, staging of x and the joins; deeper rings, 20 or 24 warps
-// and two batches of x in flight measured no better.
+// 25600 with zero points 24.9, 1 x 5120 x 5120 7.3. What bounds it is latency, not
+// the issue of instructions (117 a KB of codes, 2.0 a cycle of the 4 that an SM
+// can): with four warps to a scheduler each issues once in 7.4 cycles, of which it
+// waits 1.6 for the instruction before, 1.3 for the pipe of its product or
+// conversion, 1.1 for its turn and 0.8 for loads of x. In small calls it is some
+// 4 us of launch, staging of x and the joins. Deeper rings, 20 or 24 warps and two
+// batches of x in flight measured no better.
 // ---------------------------------------------------------------------------
 constexpr int kDepth = 3;
 constexpr int kMaxSmem = 227 * 1024;

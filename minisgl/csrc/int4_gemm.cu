@@ -25,13 +25,15 @@
 // Few tiles (N small, M small): S CTAs of a cluster share a tile's columns and
 // add their sums through shared memory in rank order.
 //
-// Measured (B200, bf16, groups of 128): 2000 x 8192 x 7168 190 us (1.24 PFLOP/s;
-// 214 where power holds the clock down, as it does a library product: 1.38 of
-// 1.63 PFLOP/s), 512 x 8192 x 7168 49, 128 x 8192 x 7168 22.5, 24 x 7168 x 8192
-// (groups of 64, MXFP8 rows) 19.5. Large tiles are bound by x on its way from L2
-// and by power, small ones (some 730 cycles a step) by instructions: 2200 a step
-// of 16384 codes, two thirds of them the converters'. More steps in tensor memory
-// or a third set of converters measured no better.
+// Measured (B200, bf16, groups of 128): 2000 x 8192 x 7168 187 to 193 us (1.22 to
+// 1.26 PFLOP/s; 212 where power holds the clock down, as it does a library
+// product: 1.38 of 1.63 PFLOP/s), 512 x 8192 x 7168 49, 128 x 8192 x 7168 22.5,
+// 24 x 7168 x 8192 (groups of 64, MXFP8 rows) 19.6. Large tiles are bound by x on
+// its way from L2 and by power. Small ones take some 730 cycles a step, most of
+// them in the converters (two thirds of the 2200 instructions a step of 16384
+// codes); the SM issues 2.0 of the 4 instructions a cycle that it can, so latency
+// between them counts more than their number. More steps in tensor memory or a
+// third set of converters measured no better.
 //
 // Every wait is bounded: a timeout records an error, raises an abort flag that
 // the other roles check, and the CTA drains its copies and returns.
@@ -518,7 +520,8 @@ __global__ void __launch_bounds__(GSmem<BN>::kThreads, 1)
   }
 }
 
-// MXFP8 rows as bf16: four significant bits times a power of two are exact
+// MXFP8 rows as bf16: four significant bits times a power of two are exact down to bf16's smallest subnormal, 2^-133
+// (scale bytes of 3 and more; under 0 to 2 the smallest elements are rounded to it)
 __global__ void __launch_bounds__(256) mx8_rows_bf16_kernel(uint4* out, const uint8_t* q, const uint8_t* sf, int64_t rows,
                                                           int K, int64_t ldq, int64_t ldsf) {
   pdl_launch_dependents();

@@ -278,9 +278,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 // meanwhile: each warp copies what it will read itself, so that only its own copies' arrival is waited for. Held in
 // registers (two vectors a lane, so that each load takes half sectors) the row ahead cost the occupancy that hides the
 // barrier and the conversions: B200, 8192 x 7168 bf16 with residual 98 us, now 73 (5.7 TB/s, 87% of a copy's rate); two
-// rows ahead cost it again (83). Short rows are bound by the instructions, some 30 an element: 8192 x 2048 without
-// residual 18.4 us, 2.8 TB/s. The sum of squares is held in double: the squares of 16-bit inputs are exact there, so the
-// statistic is exact but for the final additions.
+// rows ahead cost it again (83). Short rows are bound by the instructions, some 30 an element (72% of the issue slots):
+// 8192 x 2048 without residual 18.4 us, 2.8 TB/s. The sum of squares is held in double: the squares of 16-bit inputs are
+// exact there, so the statistic is exact but for the final additions.
 template <typename T, int NP, int THREADS>
 __global__ void __launch_bounds__(THREADS) rmsnorm_mx8_kernel(const NormArgs a) {
   pdl_launch_dependents();
