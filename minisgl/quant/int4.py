@@ -39,6 +39,12 @@ MAX_SCALE = 2.0 ** 90  # times a group's integer sum, 2^37 at most, it is still 
 _TILE, _BLOCK, _STEP = 16, 64, 128  # rows are padded to two tiles, columns to a step
 
 
+@torch.inference_mode(False)
+@torch.no_grad()
+def _ordinary(t: torch.Tensor) -> torch.Tensor:
+    return t.clone() if t.is_inference() else t
+
+
 def _tiles(n: int) -> int:
     return 2 * -(-n // (2 * _TILE))
 
@@ -60,9 +66,8 @@ class Int4Weight:
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor],
                  row_pow: torch.Tensor, n: int, k: int, group: int) -> None:
-        if scales.is_inference():  # those have no version
-            with torch.inference_mode(False):
-                scales = scales.clone()
+        # tensors of inference mode have no version, and are not written outside of it
+        packed, scales, zeros, row_pow = (t if t is None else _ordinary(t) for t in (packed, scales, zeros, row_pow))
         self._packed, self._scales, self._zeros, self._row_pow = packed, scales, zeros, row_pow
         self._n, self._k, self._group = n, k, group
         self._handle = None
@@ -166,6 +171,8 @@ def _pack_reference(codes: torch.Tensor) -> torch.Tensor:
     return packed.view(tiles, blocks, 512)
 
 
+@torch.inference_mode(False)
+@torch.no_grad()
 def int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
                 group: int = 128) -> Int4Weight:
     """``codes`` uint8 [N, K / 2] (column 2i in the low nibble of byte i),

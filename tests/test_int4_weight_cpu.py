@@ -99,3 +99,23 @@ def test_shapes_that_the_cpu_form_refuses_as_the_kernels_do():
         ops.rmsnorm_mx8(y, None, 1e-6, residual=torch.zeros(2, 64), residual_out=torch.zeros(4, 2, 64))
     with pytest.raises(ValueError, match="w must"):
         ops.rmsnorm_mx8(y, torch.ones(1), 1e-6)
+
+
+@pytest.mark.parametrize("how", ["made", "copied", "pickled"])
+def test_a_weight_of_inference_mode_is_copied_into_outside_of_it(how):
+    with torch.inference_mode():
+        w = int4_weight(*_parts())
+        w = w if how == "made" else copy.deepcopy(w) if how == "copied" else pickle.loads(pickle.dumps(w))
+    new = int4_weight(*_parts(seed=3, factor=40.0))
+    w.copy_(new)
+    w.scales.mul_(0.5)
+    assert torch.equal(w.packed, new.packed) and torch.equal(w.row_pow[:40], new.row_pow[:40] * 0.5)  # padding rows keep 1
+    with torch.inference_mode():
+        assert torch.equal(dequantize_int4(w), dequantize_int4(new.copy_(w)))
+
+
+def test_scales_of_a_parameter():
+    codes, scales, z, group = _parts()
+    w = int4_weight(codes, torch.nn.Parameter(scales), z, group)
+    assert not w.scales.requires_grad and not w.row_pow.requires_grad
+    assert w.copy_(int4_weight(*_parts(seed=5))) is w and copy.deepcopy(w).n == w.n
