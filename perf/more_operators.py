@@ -150,9 +150,9 @@ def prepare(case, seed):
         order = torch.randperm(pages, generator=g, device=DEV)
         s["slots"] = (order[at] * page + pos % page if rows <= 256 else order[at // page] * page + at % page).to(torch.int32)
         if own:
-            from minisgl.kvcache.kv4_pool import MHAKV4Cache
+            from minisgl.quant import kv4_block_bytes
 
-            s["pool"] = MHAKV4Cache(hk, 1, d, pages, page, torch.bfloat16, torch.device(DEV)).pool
+            s["pool"] = torch.zeros(2, 1, pages, hk, kv4_block_bytes(page, d), dtype=torch.uint8, device=DEV)
         return s
     keys, queries = _lens(case)
     batch = len(keys)
