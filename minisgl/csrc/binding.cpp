@@ -1429,6 +1429,260 @@ void prefill_attention(const at::Tensor& q, at::Tensor out, const at::Tensor& kv
   minisgl::launch_prefill_attention(a, stream_of(q));
 }
 
+// -------------------------------------------------------- 4-bit KV cache
+struct Kv4Pool {
+  uint8_t *k, *v;  // this layer's
+  int64_t slots;
+};
+Kv4Pool kv4_pool(const char* op, const at::Tensor& pool, int64_t layer, int64_t hk, int64_t d, int64_t page_size) {
+  check_cuda(pool, "kv_pool");
+  MSG_CHECK(d == 64 || d == 128, op, ": head_dim must be 64 or 128, got ", d);
+  MSG_CHECK(page_size >= 16 && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0, op,
+            ": page_size must be a power of two >= 16, got ", page_size);
+  MSG_CHECK(hk >= 1, op, ": hk must be positive");
+  const int64_t block = page_size * (d / 2 + d / 32);
+  MSG_CHECK(pool.scalar_type() == at::kByte && pool.dim() == 5 && pool.is_contiguous() && pool.size(0) == 2 &&
+                pool.size(3) == hk && pool.size(4) == block,
+            op, ": kv_pool must be contiguous uint8 [2, layers, pages, ", hk, ", ", block, "], got ", pool.sizes());
+  MSG_CHECK(layer >= 0 && layer < pool.size(1), op, ": layer out of range");
+  MSG_CHECK(reinterpret_cast<uintptr_t>(pool.data_ptr()) % 16 == 0, op, ": kv_pool must be 16-byte aligned");
+  const int64_t slots = pool.size(2) * page_size;
+  MSG_CHECK(slots <= 0x7fffffff, op, ": more token slots than int32 indexes");
+  const int64_t per_layer = pool.size(2) * hk * block;
+  uint8_t* base = pool.data_ptr<uint8_t>();
+  return {base + layer * per_layer, base + (pool.size(1) + layer) * per_layer, slots};
+}
+// rows of `width` bf16 values that 16-byte vectors can take
+void check_rows16(const char* op, const at::Tensor& x, const char* name, int64_t width, const at::Tensor& pool) {
+  MSG_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16, op, ": ", name, " must be a CUDA bfloat16 tensor");
+  MSG_CHECK(x.device() == pool.device(), op, ": ", name, " is on another device than kv_pool");
+  MSG_CHECK(x.dim() == 2 && x.size(1) >= width && (x.size(1) <= 1 || x.stride(1) == 1), op, ": ", name,
+            " must be [T, >= ", width, "] with unit column stride, got ", x.sizes());
+  MSG_CHECK(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && (x.size(0) <= 1 || x.stride(0) % 8 == 0), op, ": ",
+            name, " must have 16-byte aligned rows");
+  MSG_CHECK(x.size(0) <= 0x7fffffff / 2 && x.stride(0) >= 0 && x.stride(0) <= 0x7fffffff, op, ": ", name, " is too large");
+}
+void check_index(const char* op, const at::Tensor& x, const char* name, int64_t n, const at::Tensor& pool) {
+  MSG_CHECK(x.is_cuda() && x.scalar_type() == at::kInt && x.is_contiguous(), op, ": ", name,
+            " must be contiguous CUDA int32");
+  MSG_CHECK(x.device() == pool.device(), op, ": ", name, " is on another device than kv_pool");
+  MSG_CHECK(n < 0 || x.numel() == n, op, ": ", name, " must have ", n, " elements, got ", x.numel());
+}
+const void* norm_ptr(const char* op, const c10::optional<at::Tensor>& w, const char* name, int64_t d, const at::Tensor& pool) {
+  if (!w.has_value()) return nullptr;
+  MSG_CHECK(w->is_cuda() && w->scalar_type() == at::kBFloat16 && w->is_contiguous() && w->numel() == d &&
+                w->device() == pool.device(),
+            op, ": ", name, " must be a contiguous CUDA bfloat16 vector of ", d, " elements on kv_pool's device");
+  MSG_CHECK(reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0, op, ": ", name, " must be 16-byte aligned");
+  return w->data_ptr();
+}
+
+void kv4_store(const c10::optional<at::Tensor>& q, const c10::optional<at::Tensor>& q_out, const at::Tensor& k,
+               const at::Tensor& v, const c10::optional<at::Tensor>& positions,
+               const c10::optional<at::Tensor>& cos_sin, const c10::optional<at::Tensor>& q_norm_w,
+               const c10::optional<at::Tensor>& k_norm_w, const at::Tensor& pool, int64_t layer,
+               const at::Tensor& out_loc, int64_t hq, int64_t hk, int64_t d, int64_t page_size, double eps,
+               const c10::optional<at::Tensor>& err) {
+  const char* op = q.has_value() ? "rope_store_kv4" : "store_kv4";
+  const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
+  const int64_t T = k.size(0);
+  minisgl::Kv4StoreArgs a{};
+  if (q.has_value()) {
+    MSG_CHECK(hq >= 1 && q_out.has_value(), op, ": hq must be positive");
+    check_rows16(op, *q, "q", hq * d, pool);
+    check_rows16(op, *q_out, "q_out", hq * d, pool);
+    MSG_CHECK(q->size(0) == T && q_out->size(0) == T, op, ": q and q_out must have ", T, " rows");
+    a.q = q->data_ptr();
+    a.ld_q = static_cast<int>(q->stride(0));
+    a.q_out = q_out->data_ptr();
+    a.ld_qo = static_cast<int>(q_out->stride(0));
+    a.hq = static_cast<int>(hq);
+  }
+  check_rows16(op, k, "k", hk * d, pool);
+  check_rows16(op, v, "v", hk * d, pool);
+  MSG_CHECK(v.size(0) == T, op, ": k and v must have as many rows");
+  check_index(op, out_loc, "out_loc", T, pool);
+  if (cos_sin.has_value()) {
+    MSG_CHECK(positions.has_value(), op, ": positions are needed");
+    check_index(op, *positions, "positions", T, pool);
+    MSG_CHECK(cos_sin->is_cuda() && cos_sin->device() == pool.device() && cos_sin->scalar_type() == at::kFloat &&
+                  cos_sin->dim() == 2 && cos_sin->is_contiguous() && cos_sin->size(1) == d && cos_sin->size(0) >= 1 &&
+                  cos_sin->size(0) <= 0x7fffffff && reinterpret_cast<uintptr_t>(cos_sin->data_ptr()) % 16 == 0,
+              op, ": cos_sin must be contiguous CUDA float32 [max_pos, head_dim] on kv_pool's device");
+    a.cos_sin = cos_sin->data_ptr<float>();
+    a.max_pos = static_cast<int>(cos_sin->size(0));
+    a.positions = positions->data_ptr<int32_t>();
+  }
+  a.q_norm_w = norm_ptr(op, q_norm_w, "q_norm_w", d, pool);
+  a.k_norm_w = norm_ptr(op, k_norm_w, "k_norm_w", d, pool);
+  a.k = k.data_ptr();
+  a.ld_k = static_cast<int>(k.stride(0));
+  a.v = v.data_ptr();
+  a.ld_v = static_cast<int>(v.stride(0));
+  a.k_pool = p.k;
+  a.v_pool = p.v;
+  a.kv_slots = p.slots;
+  a.out_loc = out_loc.data_ptr<int32_t>();
+  a.T = static_cast<int>(T);
+  a.hk = static_cast<int>(hk);
+  a.d = static_cast<int>(d);
+  a.page_size = static_cast<int>(page_size);
+  a.eps = static_cast<float>(eps);
+  a.err = err_ptr(err);
+  const c10::cuda::CUDAGuard guard(pool.device());
+  minisgl::launch_kv4_store(a, stream_of(pool));
+}
+
+void kv4_load(const at::Tensor& pool, int64_t layer, const at::Tensor& slots, at::Tensor k_out, at::Tensor v_out,
+              int64_t hk, int64_t d, int64_t page_size, const c10::optional<at::Tensor>& err) {
+  const char* op = "load_kv4";
+  const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
+  check_index(op, slots, "slots", -1, pool);
+  const int64_t T = slots.numel();
+  MSG_CHECK(T <= 0x7fffffff / 2, op, ": too many rows");
+  for (const at::Tensor* x : {&k_out, &v_out})
+    MSG_CHECK(x->is_cuda() && x->device() == pool.device() && x->scalar_type() == at::kBFloat16 &&
+                  x->is_contiguous() && x->numel() == T * hk * d && reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0,
+              op, ": outputs must be contiguous bfloat16 [", T, ", ", hk, ", ", d, "] on kv_pool's device");
+  minisgl::Kv4LoadArgs a{};
+  a.k_pool = p.k;
+  a.v_pool = p.v;
+  a.kv_slots = p.slots;
+  a.slots = slots.data_ptr<int32_t>();
+  a.k_out = k_out.data_ptr();
+  a.v_out = v_out.data_ptr();
+  a.T = static_cast<int>(T);
+  a.hk = static_cast<int>(hk);
+  a.d = static_cast<int>(d);
+  a.page_size = static_cast<int>(page_size);
+  a.err = err_ptr(err);
+  const c10::cuda::CUDAGuard guard(pool.device());
+  minisgl::launch_kv4_load(a, stream_of(pool));
+}
+
+// Rows of a prefill plan as a bf16 pool [2, 1, R / 64, hk, 64, d].
+void kv4_expand(const at::Tensor& pool, int64_t layer, const at::Tensor& page_table, const at::Tensor& req_rows,
+                const at::Tensor& row_req, const at::Tensor& row_pos, at::Tensor out, int64_t hk, int64_t d,
+                int64_t page_size, const c10::optional<at::Tensor>& err) {
+  const char* op = "prefill_attention_kv4";
+  const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
+  const int64_t R = row_req.numel();
+  check_index(op, page_table, "page_table", -1, pool);
+  MSG_CHECK(page_table.dim() == 2, op, ": page_table must be [rows, positions]");
+  check_index(op, req_rows, "req_rows", -1, pool);
+  check_index(op, row_req, "the plan's rows", -1, pool);
+  check_index(op, row_pos, "the plan's positions", R, pool);
+  MSG_CHECK(R % 64 == 0 && R <= 0x7fffffff / 2, op, ": the plan's rows must be whole pages of 64");
+  MSG_CHECK(out.is_cuda() && out.device() == pool.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
+                out.numel() == 2 * R * hk * d,
+            op, ": compact pool must be bfloat16 [2, 1, R / 64, hk, 64, d]");
+  minisgl::Kv4LoadArgs a{};
+  a.k_pool = p.k;
+  a.v_pool = p.v;
+  a.kv_slots = p.slots;
+  a.row_req = row_req.data_ptr<int32_t>();
+  a.row_pos = row_pos.data_ptr<int32_t>();
+  a.page_table = page_table.data_ptr<int32_t>();
+  a.ld_pt = static_cast<int>(page_table.stride(0));
+  a.pt_rows = static_cast<int>(page_table.size(0));
+  a.req_rows = req_rows.data_ptr<int32_t>();
+  a.k_out = out.data_ptr();
+  a.v_out = static_cast<char*>(out.data_ptr()) + R * hk * d * 2;
+  a.T = static_cast<int>(R);
+  a.hk = static_cast<int>(hk);
+  a.d = static_cast<int>(d);
+  a.page_size = static_cast<int>(page_size);
+  a.err = err_ptr(err);
+  const c10::cuda::CUDAGuard guard(pool.device());
+  minisgl::launch_kv4_load(a, stream_of(pool));
+}
+
+// Few query rows over the 4-bit cache; cu_q absent: one token per request.
+void kv4_attention(const at::Tensor& q, at::Tensor out, const at::Tensor& pool, int64_t layer,
+                   const at::Tensor& page_table, const at::Tensor& req_rows, const at::Tensor& seq_lens,
+                   const c10::optional<at::Tensor>& cu_q, int64_t max_q, int64_t hq, int64_t hk, int64_t d,
+                   int64_t page_size, double scale, const c10::optional<at::Tensor>& err) {
+  const char* op = cu_q.has_value() ? "prefill_attention_kv4" : "decode_attention_kv4";
+  const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
+  MSG_CHECK(hq >= hk && hq % hk == 0, op, ": hq must be a multiple of hk");
+  MSG_CHECK(scale > 0 && scale <= 1e6, op, ": scale must be positive");
+  check_rows16(op, q, "q", hq * d, pool);
+  const int64_t T = q.size(0), B = req_rows.numel();
+  MSG_CHECK(out.is_cuda() && out.device() == pool.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
+                out.numel() == T * hq * d && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+            op, ": out must be contiguous bfloat16 [", T, ", ", hq * d, "] on kv_pool's device");
+  check_index(op, page_table, "page_table", -1, pool);
+  MSG_CHECK(page_table.dim() == 2, op, ": page_table must be [rows, positions]");
+  check_index(op, req_rows, "req_rows", -1, pool);
+  check_index(op, seq_lens, "seq_lens", B, pool);
+  if (cu_q.has_value()) check_index(op, *cu_q, "cu_q", B + 1, pool);
+  else MSG_CHECK(T == B, op, ": one query token per request, got ", T, " for ", B);
+  MSG_CHECK(B <= minisgl::kKv4MaxBatch, op, ": at most ", static_cast<int64_t>(minisgl::kKv4MaxBatch), " requests, got ", B);
+  if (B == 0 || T == 0) return;
+  MSG_CHECK(page_table.size(0) >= 1 && page_table.size(1) >= 1, op, ": page_table is empty");
+  const int64_t rows = (max_q * (hq / hk) + 7) / 8;
+  MSG_CHECK(B * hk * rows * ((page_table.size(1) + 127) / 128) < (int64_t{1} << 30), op, ": too many tiles of work");
+  const c10::cuda::CUDAGuard guard(pool.device());
+  const int ctas = minisgl::kv4_attn_ctas(at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+  // records of partial pieces, then the descriptors
+  const int64_t floats = static_cast<int64_t>(ctas) * 2 * 8 * (d + 2) + 4 * ctas;
+  at::Tensor work = at::detail::empty_cuda({floats}, at::kFloat, pool.device(), c10::nullopt);
+  minisgl::Kv4AttnArgs a{};
+  a.q = q.data_ptr();
+  a.ld_q = static_cast<int>(q.stride(0));
+  a.out = out.data_ptr();
+  a.k_pool = p.k;
+  a.v_pool = p.v;
+  a.kv_slots = p.slots;
+  a.page_table = page_table.data_ptr<int32_t>();
+  a.ld_pt = static_cast<int>(page_table.size(1));
+  a.pt_rows = static_cast<int>(page_table.size(0));
+  a.req_rows = req_rows.data_ptr<int32_t>();
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.cu_q = cu_q.has_value() ? cu_q->data_ptr<int32_t>() : nullptr;
+  a.B = static_cast<int>(B);
+  a.hq = static_cast<int>(hq);
+  a.hk = static_cast<int>(hk);
+  a.d = static_cast<int>(d);
+  a.page_size = static_cast<int>(page_size);
+  for (a.page_shift = 0; (int64_t{1} << a.page_shift) < page_size; ++a.page_shift) {}
+  a.scale = static_cast<float>(scale);
+  a.ctas = ctas;
+  float* w = work.data_ptr<float>();
+  a.desc = reinterpret_cast<int32_t*>(w);
+  a.part_ml = w + 4 * ctas;
+  a.part_o = a.part_ml + static_cast<int64_t>(ctas) * 2 * 8 * 2;
+  a.err = err_ptr(err);
+  minisgl::launch_kv4_attention(a, stream_of(pool));
+}
+
+// Pages src[i] -> dst[i] of every plane before `page_dim` of a pool.
+int64_t copy_pages(at::Tensor pool, const std::vector<int64_t>& src, const std::vector<int64_t>& dst, int64_t page_dim) {
+  check_cuda(pool, "pool");
+  MSG_CHECK(pool.is_contiguous() && page_dim >= 0 && page_dim < pool.dim(), "copy_pages: pool must be contiguous with a page "
+            "dimension, got ", pool.sizes(), " and page_dim ", page_dim);
+  const int64_t pages = pool.size(page_dim);
+  std::vector<int> s, d;
+  for (size_t i = 0; i < src.size(); ++i)
+    if (src[i] != dst[i]) s.push_back(static_cast<int>(src[i])), d.push_back(static_cast<int>(dst[i]));
+  if (s.empty() || pool.numel() == 0) return 0;
+  minisgl::CopyPagesArgs a{};
+  a.pool = pool.data_ptr();
+  int64_t planes = 1;
+  for (int64_t i = 0; i < page_dim; ++i) planes *= pool.size(i);
+  a.page_bytes = pool.numel() / planes / pages * pool.element_size();
+  a.plane_bytes = a.page_bytes * pages;
+  MSG_CHECK(planes <= 0x7fffffff && a.page_bytes % 16 == 0 && a.page_bytes / 16 <= 0x7fffffff / 2 &&
+                reinterpret_cast<uintptr_t>(a.pool) % 16 == 0,
+            "copy_pages: pages must be whole 16-byte vectors");
+  a.planes = static_cast<int>(planes);
+  a.src = s.data();
+  a.dst = d.data();
+  a.n = static_cast<int>(s.size());
+  const c10::cuda::CUDAGuard guard(pool.device());
+  return minisgl::launch_copy_pages(a, stream_of(pool));
+}
+
 // Keys of a prefill batch gathered for the kv_b expansion (row_req / row_pos
 // give each compact row's request and position; -1 pads).
 void mla_gather_keys(at::Tensor x, at::Tensor k_rope, const at::Tensor& latent, const at::Tensor& page_table,
@@ -1726,6 +1980,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("k_norm_w"), py::arg("k_cache"), py::arg("v_cache"), py::arg("out_loc"), py::arg("hq"),
         py::arg("hk"), py::arg("d"), py::arg("page_size"), py::arg("eps"), py::arg("err") = py::none());
   m.def("decode_attention", &decode_attention);
+  m.def("kv4_store", &kv4_store);
+  m.def("kv4_load", &kv4_load);
+  m.def("kv4_expand", &kv4_expand);
+  m.def("kv4_attention", &kv4_attention);
+  m.def("copy_pages", &copy_pages);
   m.def("gemm_fused", &gemm_fused);
   m.def("gemm_sample", &gemm_sample);
   m.def("moe_experts", &moe_experts, py::arg("out"), py::arg("x"), py::arg("w1"), py::arg("w2"), py::arg("topk_w"),

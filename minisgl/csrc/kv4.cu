@@ -1,0 +1,361 @@
+// Rows of the 4-bit paged KV cache: store (with the per-head norms and the
+// rotation of queries and keys in the same pass), read-back as bf16 rows or as
+// a compact bf16 pool, and copies of whole pages.
+//
+// The 16-bit counterpart of the store is rope_store.cu; the reference stores
+// 16-bit rows only (python/minisgl/kernel/csrc/jit/store.cu:25-53).
+#include <algorithm>
+#include <stdexcept>
+
+#include "kv4.cuh"
+#include "launch.h"
+#include "ops.h"
+
+namespace minisgl {
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+__device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// Codes of eight dims of one row, four lanes to a group of 32: the scale byte
+// and the word of nibbles (dim i in bits 4 i .. 4 i + 3). `lanes` are the
+// threads that call. amax / 7.5 is rounded up to four significant bits by
+// adding all but one unit of the dropped 20 bits; IEEE division keeps
+// max |x| = 7.5 s and the halves between codes exact for bf16 rows.
+__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t lanes, uint32_t& word) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));  // fmaxf drops NaN
+  top = fmaxf(top, __shfl_xor_sync(lanes, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(lanes, top, 2));
+  const int r = static_cast<int>((__float_as_uint(__fdiv_rn(top, 7.5f)) + 0xfffffu) >> 20);
+  const uint32_t byte = static_cast<uint32_t>(min(max(r - (106 << 3), 0), 255));
+  const float s = kv4::scale_f32(byte);
+  word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // clamped as a float (an infinity stays on its side); NaN converts to 0
+    const float t = __fdiv_rn(x[i], s);
+    const int c = __float2int_rn(fminf(fmaxf(t, -8.f), 7.f));
+    word |= static_cast<uint32_t>(t == t ? c + 8 : 8) << (4 * i);
+  }
+  return byte;
+}
+
+// ================================================================ store ====
+// Eight dims a thread, D / 8 threads a head. Blocks below `qk_blocks` take
+// queries and keys: a thread keeps the cosines and sines of its dims for `hpt`
+// heads of one token (they are as many bytes as the head itself). The others
+// take values, four tokens a thread, so that a run of tokens whose slots fill
+// whole rows of V codes is written in 16-byte chunks; other tokens' codes are
+// bytes between those of their neighbours. Every rounding of q is the one to
+// bf16 at the end, of k and v the one to codes.
+template <int D>
+__global__ void __launch_bounds__(256) kv4_store_kernel(Kv4StoreArgs a, int hpt, int qk_blocks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int kLanes = D / 8;        // threads of a head
+  constexpr int kHeads = 256 / kLanes;  // heads at once
+  constexpr int kNG = D / kv4::kGroup;
+  const ErrorSink err{a.err};
+  const int x = threadIdx.x % kLanes;
+  const uint32_t lanes = (kLanes == 16 ? 0xffffu : 0xffu) << ((threadIdx.x & 31) / kLanes * kLanes);
+  const int64_t block = static_cast<int64_t>(a.page_size) * kv4::row_bytes(D);
+
+  if (static_cast<int>(blockIdx.x) < qk_blocks) {
+    const int heads = a.hq + a.hk;
+    const int per = (heads + hpt - 1) / hpt;
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * kHeads + threadIdx.x / kLanes;
+    if (unit >= static_cast<int64_t>(a.T) * per) return;
+    const int t = static_cast<int>(unit / per);
+    const int h0 = static_cast<int>(unit % per) * hpt;
+    const bool first = x < kLanes / 2;
+    float c[8], s[8];
+    if (a.cos_sin != nullptr) {
+      int pos = a.positions[t];
+      if (pos < 0 || pos >= a.max_pos) {
+        if (x == 0) err.report(kErrBadIndex, 951);
+        pos = 0;
+      }
+      const float4* cs = reinterpret_cast<const float4*>(a.cos_sin + static_cast<int64_t>(pos) * D) + x % (kLanes / 2) * 2;
+      const float4 v[4] = {cs[0], cs[1], cs[D / 8], cs[D / 8 + 1]};
+      *reinterpret_cast<float4*>(c) = v[0], *reinterpret_cast<float4*>(c + 4) = v[1];
+      *reinterpret_cast<float4*>(s) = v[2], *reinterpret_cast<float4*>(s + 4) = v[3];
+    }
+    const int slot = a.out_loc[t];
+    const bool stored = slot >= 0 && slot < a.kv_slots;
+    for (int h = h0; h < min(h0 + hpt, heads); ++h) {
+      const bool is_q = h < a.hq;
+      const bf16* src = is_q ? static_cast<const bf16*>(a.q) + static_cast<int64_t>(t) * a.ld_q + h * D
+                             : static_cast<const bf16*>(a.k) + static_cast<int64_t>(t) * a.ld_k + (h - a.hq) * D;
+      float y[8];
+      unpack8(*(reinterpret_cast<const uint4*>(src) + x), y);
+      const bf16* nw = static_cast<const bf16*>(is_q ? a.q_norm_w : a.k_norm_w);
+      if (nw != nullptr) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += y[i] * y[i];
+#pragma unroll
+        for (int o = 1; o < kLanes; o *= 2) sum += __shfl_xor_sync(lanes, sum, o);
+        const float inv = rsqrtf(sum / D + a.eps);
+        float w[8];
+        unpack8(*(reinterpret_cast<const uint4*>(nw) + x), w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * w[i];
+      }
+      if (a.cos_sin != nullptr) {
+        // dim j turns with dim j + D / 2, which the thread D / 16 away holds
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float other = __shfl_xor_sync(lanes, y[i], kLanes / 2);
+          y[i] = first ? y[i] * c[i] - other * s[i] : y[i] * c[i] + other * s[i];
+        }
+      }
+      if (is_q) {
+        uint4 o;
+        o.x = pack_bf16x2(y[0], y[1]), o.y = pack_bf16x2(y[2], y[3]);
+        o.z = pack_bf16x2(y[4], y[5]), o.w = pack_bf16x2(y[6], y[7]);
+        *(reinterpret_cast<uint4*>(static_cast<bf16*>(a.q_out) + static_cast<int64_t>(t) * a.ld_qo + h * D) + x) = o;
+      } else {
+        uint32_t word;
+        const uint32_t byte = quantize8(y, lanes, word);
+        if (!stored) {
+          if (x == 0) err.report(kErrBadIndex, 952);
+          continue;
+        }
+        const int page = slot / a.page_size, tok = slot % a.page_size;
+        uint8_t* dst = a.k_pool + (static_cast<int64_t>(page) * a.hk + (h - a.hq)) * block;
+        reinterpret_cast<uint32_t*>(dst + tok * (D / 2))[kv4::k_word<D>(x)] = word;
+        if (x % 4 == 0) dst[a.page_size * (D / 2) + tok * kNG + x / 4] = static_cast<uint8_t>(byte);
+      }
+    }
+    return;
+  }
+
+  // ---- values: tokens 4 g - shift .. of one head, with shift the place of the
+  // first token in its row of codes
+  const int shift = a.out_loc[0] & 3;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x - qk_blocks) * kHeads + threadIdx.x / kLanes;
+  const int t0 = static_cast<int>(unit / a.hk) * 4 - shift;
+  const int h = static_cast<int>(unit % a.hk);
+  if (t0 >= a.T) return;
+  uint32_t word[4], byte[4];
+  int slot[4];
+  bool run = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = t0 + i;
+    slot[i] = -1;
+    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (t >= 0 && t < a.T) {
+      slot[i] = a.out_loc[t];
+      unpack8(*(reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.v) + static_cast<int64_t>(t) * a.ld_v + h * D) + x), y);
+      if (slot[i] < 0 || slot[i] >= a.kv_slots) {
+        if (x == 0) err.report(kErrBadIndex, 953);
+        slot[i] = -1;
+      }
+    }
+    byte[i] = quantize8(y, lanes, word[i]);
+    run = run && slot[i] >= 0 && slot[i] == slot[0] + i;
+  }
+  if (run && (slot[0] & 3) == 0) {
+    const int page = slot[0] / a.page_size, row = slot[0] % a.page_size / 4;
+    uint8_t* dst = a.v_pool + (static_cast<int64_t>(page) * a.hk + h) * block;
+    // byte j of token i's word to byte v_byte(i) of word j
+    const uint32_t e0 = __byte_perm(word[0], word[2], 0x5140), e1 = __byte_perm(word[0], word[2], 0x7362);
+    const uint32_t o0 = __byte_perm(word[1], word[3], 0x5140), o1 = __byte_perm(word[1], word[3], 0x7362);
+    uint4 q;  // tokens 0, 2, 1, 3 from the low byte up
+    q.x = __byte_perm(e0, o0, 0x5410), q.y = __byte_perm(e0, o0, 0x7632);
+    q.z = __byte_perm(e1, o1, 0x5410), q.w = __byte_perm(e1, o1, 0x7632);
+    *(reinterpret_cast<uint4*>(dst + row * (2 * D)) + kv4::v_chunk(row, x)) = q;
+    if (x % 4 == 0)
+      reinterpret_cast<uint32_t*>(dst + a.page_size * (D / 2))[row * kNG + x / 4] =
+          byte[0] | byte[2] << 8 | byte[1] << 16 | byte[3] << 24;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (slot[i] < 0) continue;
+    const int page = slot[i] / a.page_size, tok = slot[i] % a.page_size;
+    const int row = tok / 4, b = kv4::v_byte(tok & 3);
+    uint8_t* dst = a.v_pool + (static_cast<int64_t>(page) * a.hk + h) * block;
+    uint8_t* codes = dst + row * (2 * D) + kv4::v_chunk(row, x) * 16 + b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) codes[4 * j] = static_cast<uint8_t>(word[i] >> (8 * j));
+    if (x % 4 == 0) dst[a.page_size * (D / 2) + (row * kNG + x / 4) * 4 + b] = static_cast<uint8_t>(byte[i]);
+  }
+}
+
+// ================================================================= load ====
+// Eight dims of K and of V of one row and head a thread. Values are s (c - 8),
+// exact in bf16: 128 + c has the bits 0x4300 | c, and s (128 + c) - 136 s is one
+// fused multiply-add (136 s = 17 s 8 has at most 8 significant bits).
+__device__ __forceinline__ uint4 values8(uint32_t word, uint32_t byte) {
+  const uint32_t s2 = byte * 0x00100010u + kv4::kScaleBf16x2;
+  const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&s2);
+  const __nv_bfloat162 off = __hmul2(s, __float2bfloat162_rn(-136.f));
+  uint32_t p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // dims 2 i and 2 i + 1: nibbles 2 i and 2 i + 1 to the halves
+    const uint32_t n = word >> (8 * i);
+    const uint32_t c2 = (n & 0xfu) | ((n & 0xf0u) << 12) | 0x43004300u;
+    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&c2), s, off);
+    p[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(p[0], p[1], p[2], p[3]);
+}
+
+template <int D>
+__device__ __forceinline__ void load_row(const Kv4LoadArgs& a, int slot, int h, int x, uint4& k, uint4& v) {
+  constexpr int kNG = D / kv4::kGroup;
+  const int page = slot / a.page_size, tok = slot % a.page_size, row = tok / 4, b = kv4::v_byte(tok & 3);
+  const int64_t at = (static_cast<int64_t>(page) * a.hk + h) * a.page_size * kv4::row_bytes(D);
+  const uint8_t* kb = a.k_pool + at;
+  const uint8_t* vb = a.v_pool + at;
+  const int codes = a.page_size * (D / 2);
+  const uint32_t kw = reinterpret_cast<const uint32_t*>(kb + tok * (D / 2))[kv4::k_word<D>(x)];
+  const uint4 vq = *(reinterpret_cast<const uint4*>(vb + row * (2 * D)) + kv4::v_chunk(row, x));
+  const uint32_t ks = kb[codes + tok * kNG + x / 4], vs = vb[codes + (row * kNG + x / 4) * 4 + b];
+  const uint32_t lo = __byte_perm(vq.x, vq.y, (4 + b) << 4 | b), hi = __byte_perm(vq.z, vq.w, (4 + b) << 4 | b);
+  k = values8(kw, ks);
+  v = values8(__byte_perm(lo, hi, 0x5410), vs);
+}
+
+// Rows of a.slots to k_out / v_out [T, hk, D], or (a.row_req set) rows of a
+// prefill plan to a bf16 pool [2, 1, R / 64, hk, 64, D]: there row r is key
+// row_pos[r] of request row_req[r] (none: zeros) and one block takes 64-row
+// pages, whose rows of a head are side by side.
+template <int D>
+__global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int kLanes = D / 8;
+  const ErrorSink err{a.err};
+  const int x = threadIdx.x % kLanes;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  if (unit >= static_cast<int64_t>(a.T) * a.hk) return;
+  int r, h, slot;
+  int64_t to;
+  if (a.row_req != nullptr) {
+    const int page = static_cast<int>(unit / (64 * a.hk)), in = static_cast<int>(unit % (64 * a.hk));
+    h = in / 64, r = page * 64 + in % 64;
+    to = unit;
+    const int req = a.row_req[r];
+    slot = -1;
+    if (req >= 0) {
+      const int row = a.req_rows[req], pos = a.row_pos[r];
+      if (row >= 0 && row < a.pt_rows && pos < a.ld_pt) slot = a.page_table[static_cast<int64_t>(row) * a.ld_pt + pos];
+      if (slot < 0 || slot >= a.kv_slots) {
+        if (x == 0) err.report(kErrBadIndex, 955);
+        slot = -1;
+      }
+    }
+  } else {
+    r = static_cast<int>(unit / a.hk), h = static_cast<int>(unit % a.hk);
+    to = unit;
+    slot = a.slots[r];
+    if (slot < 0 || slot >= a.kv_slots) {
+      if (x == 0) err.report(kErrBadIndex, 954);
+      slot = -1;
+    }
+  }
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
+  if (slot >= 0) load_row<D>(a, slot, h, x, k, v);
+  *(reinterpret_cast<uint4*>(a.k_out) + to * kLanes + x) = k;
+  *(reinterpret_cast<uint4*>(a.v_out) + to * kLanes + x) = v;
+}
+
+// ================================================================= copy ====
+// Pages of every plane (K / V and layer) of a pool, pair by pair; the pairs
+// travel as a kernel argument, so a call is one launch and leaves nothing
+// behind on the device. grid (chunks of a page, pairs, planes in turn).
+template <int N>
+struct PagePairs {
+  int src[N], dst[N];
+};
+constexpr int kCopyVecs = 4;  // 16-byte vectors a thread
+
+template <int N>
+__global__ void __launch_bounds__(256) copy_pages_kernel(uint4* pool, int64_t plane_vecs, int page_vecs, int planes,
+                                                         const __grid_constant__ PagePairs<N> pairs) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int i0 = blockIdx.x * (256 * kCopyVecs) + threadIdx.x;
+  const int64_t src = static_cast<int64_t>(pairs.src[blockIdx.y]) * page_vecs;
+  const int64_t dst = static_cast<int64_t>(pairs.dst[blockIdx.y]) * page_vecs;
+  for (int p = blockIdx.z; p < planes; p += gridDim.z) {
+    uint4* base = pool + p * plane_vecs;
+    uint4 v[kCopyVecs];
+#pragma unroll
+    for (int i = 0; i < kCopyVecs; ++i)
+      if (i0 + i * 256 < page_vecs) v[i] = __ldcs(base + src + i0 + i * 256);
+#pragma unroll
+    for (int i = 0; i < kCopyVecs; ++i)
+      if (i0 + i * 256 < page_vecs) __stcs(base + dst + i0 + i * 256, v[i]);
+  }
+}
+
+template <int N>
+void copy_pairs(const CopyPagesArgs& a, int from, int n, cudaStream_t s) {
+  PagePairs<N> pairs;
+  for (int i = 0; i < n; ++i) pairs.src[i] = a.src[from + i], pairs.dst[i] = a.dst[from + i];
+  const int page_vecs = static_cast<int>(a.page_bytes / 16);
+  const int chunks = (page_vecs + 256 * kCopyVecs - 1) / (256 * kCopyVecs);
+  dim3 grid(chunks, n, std::min(a.planes, 65535));
+  launch_pdl(copy_pages_kernel<N>, grid, dim3(256), 0, s, static_cast<uint4*>(a.pool), a.plane_bytes / 16, page_vecs,
+             a.planes, pairs);
+}
+
+}  // namespace
+
+void launch_kv4_store(const Kv4StoreArgs& a, cudaStream_t s) {
+  if (a.T <= 0) return;
+  if (a.d != 64 && a.d != 128) throw std::runtime_error("minisgl.rope_store_kv4: head_dim must be 64 or 128");
+  const int per_block = 256 / (a.d / 8);
+  // one head a thread while that does not fill the GPU, then four
+  const int64_t heads = static_cast<int64_t>(a.T) * (a.hq + a.hk);
+  const int hpt = heads > 148 * 8 * per_block ? 4 : 1;
+  const int64_t qk = (static_cast<int64_t>(a.T) * ((a.hq + a.hk + hpt - 1) / hpt) + per_block - 1) / per_block;
+  const int64_t v = (static_cast<int64_t>((a.T + 6) / 4) * a.hk + per_block - 1) / per_block;
+  if (qk + v > 0x7fffffff) throw std::runtime_error("minisgl.rope_store_kv4: too many rows");
+  const dim3 grid(static_cast<unsigned>(qk + v));
+  auto kern = a.d == 128 ? kv4_store_kernel<128> : kv4_store_kernel<64>;
+  launch_pdl(kern, grid, dim3(256), 0, s, a, hpt, static_cast<int>(qk));
+}
+
+void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s) {
+  if (a.T <= 0) return;
+  if (a.d != 64 && a.d != 128) throw std::runtime_error("minisgl.load_kv4: head_dim must be 64 or 128");
+  const int per_block = 256 / (a.d / 8);
+  const int64_t blocks = (static_cast<int64_t>(a.T) * a.hk + per_block - 1) / per_block;
+  if (blocks > 0x7fffffff) throw std::runtime_error("minisgl.load_kv4: too many rows");
+  auto kern = a.d == 128 ? kv4_load_kernel<128> : kv4_load_kernel<64>;
+  launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
+}
+
+int launch_copy_pages(const CopyPagesArgs& a, cudaStream_t s) {
+  int launches = 0;
+  for (int from = 0; from < a.n; ++launches) {
+    const int left = a.n - from;
+    if (left <= 32) {
+      copy_pairs<32>(a, from, left, s);
+      from += left;
+    } else {
+      const int n = std::min(left, 480);  // pairs that fit 4 KB of arguments
+      copy_pairs<480>(a, from, n, s);
+      from += n;
+    }
+  }
+  return launches;
+}
+
+}  // namespace minisgl

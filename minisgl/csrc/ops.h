@@ -204,6 +204,73 @@ void launch_decode_attention(const AttnArgs& a, cudaStream_t s);
 void launch_prefill_attention(const AttnArgs& a, cudaStream_t s);
 void launch_mla_prefill_attention(const AttnArgs& a, cudaStream_t s);
 
+// -------------------------------------------------------- 4-bit KV cache ----
+// Rows into the cache: q (normed, rotated) to q_out, k (the same) and v as codes.
+struct Kv4StoreArgs {
+  const void* q;             // [T, hq * d] bf16, or nullptr with hq = 0
+  int ld_q;
+  void* q_out;               // may be q
+  int ld_qo;
+  const void *k, *v;         // [T, hk * d] bf16
+  int ld_k, ld_v;
+  const int32_t* positions;  // [T] (cos_sin set)
+  const float* cos_sin;      // [max_pos, d], or nullptr: no rotation
+  int max_pos;
+  const void *q_norm_w, *k_norm_w;  // [d] bf16 or nullptr
+  uint8_t *k_pool, *v_pool;  // this layer's [pages, hk, block bytes]
+  const int32_t* out_loc;    // [T]
+  int T, hq, hk, d, page_size;
+  float eps;
+  int64_t kv_slots;          // pages * page_size: other slots are reported, not written
+  int* err;
+};
+void launch_kv4_store(const Kv4StoreArgs& a, cudaStream_t s);
+struct Kv4LoadArgs {
+  const uint8_t *k_pool, *v_pool;  // this layer's
+  const int32_t* slots;      // [T], or (row_req set) nullptr
+  void *k_out, *v_out;       // [T, hk, d] bf16, or a layer's [T / 64, hk, 64, d]
+  int T, hk, d, page_size;
+  int64_t kv_slots;
+  // rows of a prefill plan: key row_pos[r] of request row_req[r] (-1: zeros)
+  const int32_t *row_req, *row_pos;
+  const int32_t* page_table;
+  int ld_pt, pt_rows;
+  const int32_t* req_rows;
+  int* err;
+};
+void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s);
+constexpr int kKv4MaxBatch = 8192;  // requests of one attention call (their tile sums sit in shared memory)
+struct Kv4AttnArgs {
+  const void* q;             // [T, >= hq * d] bf16
+  int ld_q;
+  void* out;                 // [T, hq * d] bf16
+  const uint8_t *k_pool, *v_pool;  // this layer's [pages, hk, block bytes]
+  int64_t kv_slots;
+  const int32_t* page_table;
+  int ld_pt, pt_rows;
+  const int32_t* req_rows;   // [B]
+  const int32_t* seq_lens;   // [B]
+  const int32_t* cu_q;       // [B + 1], or nullptr: one token per request
+  int B, hq, hk, d, page_size, page_shift;
+  float scale;
+  int ctas;                  // grid
+  float* part_o;             // [ctas, 2, 8, d] records of partial pieces
+  float* part_ml;            // [ctas, 2, 8, 2]
+  int32_t* desc;             // [ctas, 4]
+  int* err;
+};
+int kv4_attn_ctas(int sms);
+void launch_kv4_attention(const Kv4AttnArgs& a, cudaStream_t s);
+// Pages src[i] -> dst[i] of every plane of a pool; returns the launches made.
+struct CopyPagesArgs {
+  void* pool;
+  int64_t plane_bytes, page_bytes;  // multiples of 16
+  int planes;
+  const int *src, *dst;      // host
+  int n;
+};
+int launch_copy_pages(const CopyPagesArgs& a, cudaStream_t s);
+
 // ------------------------------------------------------------------ MLA ----
 struct MlaPrepareArgs {
   // either half may be absent: q == nullptr stores key rows only, latent ==

@@ -801,6 +801,201 @@ def prefill_attention(
     return out
 
 
+# ---------------------------------------------------- KV cache in 4 bits
+def _kv4_check(op: str, pool: torch.Tensor, layer: int, hk: int, d: int, page_size: int) -> None:
+    """The checks of a CPU pool (those of a GPU pool are the binding's)."""
+    from minisgl.quant.kv4 import kv4_block_bytes, kv4_check
+
+    kv4_check(page_size, d)
+    want = (hk, kv4_block_bytes(page_size, d))
+    if pool.dtype != torch.uint8 or pool.dim() != 5 or pool.shape[0] != 2 or tuple(pool.shape[3:]) != want:
+        raise ValueError(f"{op}: kv_pool must be uint8 [2, layers, pages, {want[0]}, {want[1]}], got {tuple(pool.shape)}")
+    if not 0 <= layer < pool.shape[1]:
+        raise ValueError(f"{op}: layer out of range")
+
+
+def store_kv4(k: torch.Tensor, v: torch.Tensor, kv_pool: torch.Tensor, layer: int, out_loc: torch.Tensor, hk: int,
+              d: int, page_size: int) -> None:
+    """Rows of k and v [T, >= hk * d] (bf16 on a GPU) as they are into the
+    4-bit pool [2, layers, pages, hk, block bytes] (``minisgl.quant.kv4``) at
+    the slots ``out_loc``; other rows keep their values. Slots are distinct
+    but for ones whose rows nobody reads."""
+    if kv_pool.is_cuda:
+        _count()
+        native().kv4_store(None, None, k, v, None, None, None, None, kv_pool, layer, out_loc, 0, hk, d, page_size, 0.0,
+                           error_word(kv_pool.device))
+        return
+    _kv4_check("store_kv4", kv_pool, layer, hk, d, page_size)
+    if k.shape[0] != v.shape[0] or k.shape[1] < hk * d or v.shape[1] < hk * d or out_loc.numel() != k.shape[0]:
+        raise ValueError(f"store_kv4: k and v must be [{out_loc.numel()}, >= {hk * d}]")
+    ref.store_kv4(k[:, :hk * d], v[:, :hk * d], kv_pool, layer, out_loc, hk, d, page_size)
+
+
+def rope_store_kv4(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, q_norm_w: Optional[torch.Tensor],
+                   k_norm_w: Optional[torch.Tensor], kv_pool: torch.Tensor, layer: int, out_loc: torch.Tensor, hq: int,
+                   hk: int, d: int, page_size: int, eps: float, q_out: Optional[torch.Tensor] = None) -> None:
+    """``rope_store`` into a 4-bit pool: per-head RMS norms of q and k (None:
+    none), NeoX rotation of both, q heads to ``q_out`` [T, >= hq * d] (None: in
+    place in ``qkv``), k and v as codes to the slots ``out_loc``. The k and v
+    columns of ``qkv`` keep their values. Norm and rotation are fp32 and
+    rounded once, to q's type and to the codes."""
+    q_out = qkv if q_out is None else q_out
+    if kv_pool.is_cuda:
+        if qkv.dim() != 2 or qkv.shape[1] < (hq + 2 * hk) * d:
+            raise ValueError(f"rope_store_kv4: qkv must be [T, >= {(hq + 2 * hk) * d}], got {tuple(qkv.shape)}")
+        k0, v0 = hq * d, (hq + hk) * d
+        _count()
+        native().kv4_store(qkv, q_out, qkv[:, k0:], qkv[:, v0:], positions, cos_sin, q_norm_w, k_norm_w, kv_pool, layer,
+                           out_loc, hq, hk, d, page_size, eps, error_word(kv_pool.device))
+        return
+    _kv4_check("rope_store_kv4", kv_pool, layer, hk, d, page_size)
+    T = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.shape[1] < (hq + 2 * hk) * d:
+        raise ValueError(f"rope_store_kv4: qkv must be [T, >= {(hq + 2 * hk) * d}], got {tuple(qkv.shape)}")
+    if positions.numel() != T or out_loc.numel() != T or q_out.shape[0] != T or q_out.shape[1] < hq * d:
+        raise ValueError(f"rope_store_kv4: positions, out_loc and q_out must have {T} rows")
+    x = qkv[:, :(hq + 2 * hk) * d].reshape(T, hq + 2 * hk, d)
+    cs = cos_sin[positions.long()]
+    q = ref.norm_rope(x[:, :hq], q_norm_w, cs, eps)
+    k = ref.norm_rope(x[:, hq:hq + hk], k_norm_w, cs, eps)
+    ref.store_kv4(k, x[:, hq + hk:], kv_pool, layer, out_loc, hk, d, page_size)
+    q_out[:, :hq * d] = q.reshape(T, hq * d).to(q_out.dtype)
+
+
+def load_kv4(kv_pool: torch.Tensor, layer: int, slots: torch.Tensor, hk: int, d: int, page_size: int,
+             dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of a 4-bit pool: (k, v) [T, hk, d] of the slots (int32 [T]), in
+    bf16, which holds the cache's values exactly (CPU: any ``dtype``). A slot
+    outside the pool is reported and its row is zero."""
+    if kv_pool.is_cuda:
+        if dtype != torch.bfloat16:
+            raise ValueError(f"load_kv4: rows come out in bfloat16 on a GPU, got {dtype}")
+        k = torch.empty(slots.numel(), hk, d, dtype=dtype, device=kv_pool.device)
+        v = torch.empty_like(k)
+        _count()
+        native().kv4_load(kv_pool, layer, slots, k, v, hk, d, page_size, error_word(kv_pool.device))
+        return k, v
+    _kv4_check("load_kv4", kv_pool, layer, hk, d, page_size)
+    return ref.load_kv4(kv_pool, layer, slots, hk, d, page_size, dtype)
+
+
+def _attention_kv4_cpu(op, q, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq, hk, d, page_size, scale, out):
+    _kv4_check(op, kv_pool, layer, hk, d, page_size)
+    if hq % hk or q.dim() != 2 or q.shape[1] < hq * d:
+        raise ValueError(f"{op}: q must be [T, >= {hq} * {d}] with whole groups of heads, got {tuple(q.shape)}")
+    if not scale > 0:
+        raise ValueError(f"{op}: scale must be positive")
+    qv = q[:, :hq * d].reshape(q.shape[0], hq, d)
+    y = ref.attention_kv4(qv, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq, hk, d, page_size, scale)
+    y = y.view(q.shape[0], hq * d)
+    if out is not None:
+        out.copy_(y)
+        return out
+    return y
+
+
+def decode_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, page_table: torch.Tensor,
+                         req_rows: torch.Tensor, seq_lens: torch.Tensor, hq: int, hk: int, d: int, page_size: int,
+                         scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``decode_attention`` over a 4-bit pool: one query token per request, q
+    [B, >= hq * d] (row stride free). The keys of all requests are split
+    evenly over the GPU whatever their lengths are; scratch is the call's
+    own. A request without keys gives zeros."""
+    if kv_pool.is_cuda:
+        if out is None:
+            out = torch.empty(q.shape[0], hq * d, dtype=q.dtype, device=q.device)
+        _count(2)
+        native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, None, 1, hq, hk, d, page_size,
+                               scale, error_word(kv_pool.device))
+        return out
+    cu = torch.arange(req_rows.numel() + 1, dtype=torch.int32)
+    return _attention_kv4_cpu("decode_attention_kv4", q, kv_pool, layer, page_table, req_rows, seq_lens, cu, hq, hk, d,
+                              page_size, scale, out)
+
+
+class KV4PrefillPlan(MlaPrefillPlan):
+    """Host-built layout of a batch's keys (its requests' key counts) for
+    ``prefill_attention_kv4`` over many query rows, which expands them once to
+    a compact bf16 pool. Built once per batch; used by every layer."""
+
+
+# query rows (tokens x heads of a group) of a request up to which the few-row
+# kernel, which expands codes for 8 rows at a time in registers, reads the
+# cache itself; beyond, keys are expanded once and the tcgen05 kernel takes over
+KV4_FEW_ROWS = 128
+
+
+def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, page_table: torch.Tensor,
+                          req_rows: torch.Tensor, seq_lens: torch.Tensor, cu_q: torch.Tensor, max_q: int, hq: int,
+                          hk: int, d: int, page_size: int, scale: float, plan: Optional[KV4PrefillPlan] = None,
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``prefill_attention`` over a 4-bit pool: causal attention of the last
+    query tokens of each request (cu_q [B + 1]; at most ``max_q`` each) over
+    its cached and new keys. A query before the first key gives zeros.
+
+    Up to KV4_FEW_ROWS query rows per KV head (drafted tokens, short extends),
+    and for heads of other than 128 dims, the decode kernel reads the codes.
+    More rows: the keys (``plan``: their layout, made from seq_lens if None,
+    which waits for the GPU) are expanded to a bf16 pool and go through
+    ``prefill_attention``; the expansion is exact."""
+    if not kv_pool.is_cuda:
+        return _attention_kv4_cpu("prefill_attention_kv4", q, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq,
+                                  hk, d, page_size, scale, out)
+    if out is None:
+        out = torch.empty(q.shape[0], hq * d, dtype=q.dtype, device=q.device)
+    err = error_word(kv_pool.device)
+    if d != 128 or max_q * (hq // max(1, hk)) <= KV4_FEW_ROWS:
+        _count(2)
+        native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, max_q, hq, hk, d, page_size,
+                               scale, err)
+        return out
+    if plan is None:
+        plan = KV4PrefillPlan(seq_lens.tolist(), kv_pool.device)
+    if plan.rows == 0:  # no request has a key
+        return out.zero_()
+    pool = torch.empty(2, 1, plan.rows // plan.PAGE, hk, plan.PAGE, d, dtype=q.dtype, device=q.device)
+    _count()
+    native().kv4_expand(kv_pool, layer, page_table, req_rows, plan.row_req, plan.row_pos, pool, hk, d, page_size, err)
+    return prefill_attention(q, pool, 0, plan.page_table, plan.rows_in_order, seq_lens, cu_q, max_q, hq, hk, d,
+                             plan.PAGE, scale, out=out)
+
+
+def copy_pages(pool: torch.Tensor, src, dst, page_dim: int = 2) -> torch.Tensor:
+    """Copy whole pages src[i] -> dst[i] over every plane (K / V and layer) of a
+    pool whose pages are dimension ``page_dim`` (2: the MHA pools, bf16 and
+    4-bit; 1: the MLA latent pool): forks of partly filled pages, compaction.
+    ``src`` and ``dst`` are host values (ints, or CPU tensors). A page may be
+    copied to several; a destination is named once and is no other pair's
+    source, so the order of the copies does not matter. Returns the pool."""
+    src, dst = _page_list(src), _page_list(dst)
+    if len(src) != len(dst):
+        raise ValueError(f"copy_pages: {len(src)} source and {len(dst)} destination pages")
+    if not 0 <= page_dim < pool.dim():
+        raise ValueError(f"copy_pages: page_dim {page_dim} of a pool {tuple(pool.shape)}")
+    pages = pool.shape[page_dim]
+    to = set(dst)
+    if src and (min(src) < 0 or max(src) >= pages or min(to) < 0 or max(to) >= pages):
+        raise IndexError(f"copy_pages: a page is outside the pool of {pages}")
+    if len(to) != len(dst):
+        raise ValueError("copy_pages: a page is the destination of two copies")
+    if not to.isdisjoint(src) and any(s in to and s != d for s, d in zip(src, dst)):
+        raise ValueError("copy_pages: a page is both a source and the destination of another copy")
+    if pool.is_cuda:
+        _count(native().copy_pages(pool, src, dst, page_dim))
+    elif src:
+        dim = (slice(None),) * page_dim
+        pool[dim + (torch.tensor(dst),)] = pool[dim + (torch.tensor(src),)]
+    return pool
+
+
+def _page_list(pages) -> List[int]:
+    if isinstance(pages, torch.Tensor):
+        if pages.is_cuda or pages.is_floating_point():
+            raise ValueError("copy_pages: page numbers are host integers (a CPU tensor or ints)")
+        return pages.reshape(-1).tolist()
+    return [int(p) for p in pages]
+
+
 # --------------------------------------------------------------- sampling
 def argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     if not logits.is_cuda:

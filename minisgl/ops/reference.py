@@ -223,6 +223,77 @@ def attention(
     return out
 
 
+def norm_rope(x: torch.Tensor, w: Optional[torch.Tensor], cs: torch.Tensor, eps: float) -> torch.Tensor:
+    """Per-head RMS norm (w None: none) and NeoX rotation of x [T, heads, d]
+    in fp32 (not rounded in between); cs [T, d]: d/2 cosines, d/2 sines."""
+    x = x.float()
+    if w is not None:
+        x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * w.float()
+    a, b = x.chunk(2, dim=-1)
+    c, s = cs[:, None].float().chunk(2, dim=-1)
+    return torch.cat([a * c - b * s, b * c + a * s], dim=-1)
+
+
+def _kv4_places(pool: torch.Tensor, slots: torch.Tensor, page_size: int, d: int):
+    """Pages [T], and K / V code and K / V scale byte places [T, .] of slots."""
+    from minisgl.quant.kv4 import _places
+
+    s = slots.long()
+    if s.numel() and (int(s.min()) < 0 or int(s.max()) >= pool.shape[2] * page_size):
+        raise IndexError("a KV slot is outside the cache")
+    return s // page_size, [p[s % page_size] for p in _places(page_size, d, pool.device)]
+
+
+def store_kv4(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, layer: int, slots: torch.Tensor, hk: int, d: int,
+              page_size: int) -> None:
+    """Rows of k and v [T, hk, d] as codes and scales into blocks of the pool."""
+    from minisgl.quant.kv4 import quantize_kv4_reference
+
+    page, places = _kv4_places(pool, slots, page_size, d)
+    head = torch.arange(hk, device=pool.device)[None, :, None]
+    for kv, x in enumerate((k, v)):
+        codes, sf = quantize_kv4_reference(x.reshape(-1, hk, d))
+        cache = pool[kv, layer]
+        cache[page[:, None, None], head, places[kv][:, None]] = codes[..., 0::2] | (codes[..., 1::2] << 4)
+        cache[page[:, None, None], head, places[2 + kv][:, None]] = sf
+
+
+def load_kv4(pool: torch.Tensor, layer: int, slots: torch.Tensor, hk: int, d: int, page_size: int, dtype: torch.dtype):
+    """(k, v) [T, hk, d] of the slots' rows."""
+    from minisgl.quant.kv4 import dequantize_kv4
+
+    page, places = _kv4_places(pool, slots, page_size, d)
+    head = torch.arange(hk, device=pool.device)[None, :, None]
+    out = []
+    for kv in range(2):
+        cache = pool[kv, layer]
+        c = cache[page[:, None, None], head, places[kv][:, None]]
+        sf = cache[page[:, None, None], head, places[2 + kv][:, None]]
+        out.append(dequantize_kv4(torch.stack([c & 15, c >> 4], dim=-1).flatten(-2), sf, dtype))
+    return tuple(out)
+
+
+def attention_kv4(q: torch.Tensor, pool: torch.Tensor, layer: int, page_table: torch.Tensor, req_rows: torch.Tensor,
+                  seq_lens: torch.Tensor, cu_q: torch.Tensor, hq: int, hk: int, d: int, page_size: int,
+                  scale: float) -> torch.Tensor:
+    """``attention`` over a 4-bit pool: q [T, hq, d] -> [T, hq, d]. A query
+    whose position is before the first key sees none: its row is zero."""
+    out = torch.zeros(q.shape[0], hq, d, dtype=q.dtype, device=q.device)
+    rows, lens, cu = req_rows.tolist(), seq_lens.tolist(), cu_q.tolist()
+    for b, (row, L) in enumerate(zip(rows, lens)):
+        s, e = cu[b], cu[b + 1]
+        if e <= s or L <= 0:
+            continue
+        k, v = load_kv4(pool, layer, page_table[row, :L], hk, d, page_size, torch.float32)
+        qb = q[s:e].float().reshape(e - s, hk, hq // hk, d)
+        scores = torch.einsum("nhgd,lhd->hgnl", qb, k) * scale
+        last = torch.arange(L - (e - s), L, device=q.device)
+        mask = torch.arange(L, device=q.device)[None, :] > last[:, None]
+        p = torch.softmax(scores.masked_fill(mask, float("-inf")), dim=-1).masked_fill(mask, 0.0)
+        out[s:e] = torch.einsum("hgnl,lhd->nhgd", p, v).reshape(e - s, hq, d).to(q.dtype)
+    return out
+
+
 def rope_interleaved(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor) -> torch.Tensor:
     """DeepSeek (GPT-J) rotary embedding: pairs (2i, 2i + 1) rotate by
     frequency i. x [T, ..., d]; cos_sin [max_pos, d] = d/2 cos then d/2 sin."""

@@ -41,6 +41,8 @@ SOURCES = [
     "minisgl/csrc/mx8_rows.cu",
     "minisgl/csrc/int4.cu",
     "minisgl/csrc/int4_gemm.cu",
+    "minisgl/csrc/kv4.cu",
+    "minisgl/csrc/kv4_attention.cu",
 ]
 
 
