@@ -1433,6 +1433,7 @@ void prefill_attention(const at::Tensor& q, at::Tensor out, const at::Tensor& kv
 struct Kv4Pool {
   uint8_t *k, *v;  // this layer's
   int64_t slots;
+  int shift;  // log2 of the page size
 };
 Kv4Pool kv4_pool(const char* op, const at::Tensor& pool, int64_t layer, int64_t hk, int64_t d, int64_t page_size) {
   check_cuda(pool, "kv_pool");
@@ -1450,7 +1451,9 @@ Kv4Pool kv4_pool(const char* op, const at::Tensor& pool, int64_t layer, int64_t 
   MSG_CHECK(slots <= 0x7fffffff, op, ": more token slots than int32 indexes");
   const int64_t per_layer = pool.size(2) * hk * block;
   uint8_t* base = pool.data_ptr<uint8_t>();
-  return {base + layer * per_layer, base + (pool.size(1) + layer) * per_layer, slots};
+  int shift = 4;
+  while ((int64_t{1} << shift) < page_size) ++shift;
+  return {base + layer * per_layer, base + (pool.size(1) + layer) * per_layer, slots, shift};
 }
 // rows of `width` bf16 values that 16-byte vectors can take
 void check_rows16(const char* op, const at::Tensor& x, const char* name, int64_t width, const at::Tensor& pool) {
@@ -1477,30 +1480,36 @@ const void* norm_ptr(const char* op, const c10::optional<at::Tensor>& w, const c
   return w->data_ptr();
 }
 
-void kv4_store(const c10::optional<at::Tensor>& q, const c10::optional<at::Tensor>& q_out, const at::Tensor& k,
-               const at::Tensor& v, const c10::optional<at::Tensor>& positions,
-               const c10::optional<at::Tensor>& cos_sin, const c10::optional<at::Tensor>& q_norm_w,
-               const c10::optional<at::Tensor>& k_norm_w, const at::Tensor& pool, int64_t layer,
-               const at::Tensor& out_loc, int64_t hq, int64_t hk, int64_t d, int64_t page_size, double eps,
-               const c10::optional<at::Tensor>& err) {
-  const char* op = q.has_value() ? "rope_store_kv4" : "store_kv4";
+// hq > 0: k holds rows of q, k and v heads side by side and there is no v.
+void kv4_store(const at::Tensor& k, const c10::optional<at::Tensor>& v, const c10::optional<at::Tensor>& q_out,
+               const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& cos_sin,
+               const c10::optional<at::Tensor>& q_norm_w, const c10::optional<at::Tensor>& k_norm_w,
+               const at::Tensor& pool, int64_t layer, const at::Tensor& out_loc, int64_t hq, int64_t hk, int64_t d,
+               int64_t page_size, double eps, const c10::optional<at::Tensor>& err) {
+  const bool fused = !v.has_value();
+  const char* op = fused ? "rope_store_kv4" : "store_kv4";
   const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
-  const int64_t T = k.size(0);
   minisgl::Kv4StoreArgs a{};
-  if (q.has_value()) {
-    MSG_CHECK(hq >= 1 && q_out.has_value(), op, ": hq must be positive");
-    check_rows16(op, *q, "q", hq * d, pool);
-    check_rows16(op, *q_out, "q_out", hq * d, pool);
-    MSG_CHECK(q->size(0) == T && q_out->size(0) == T, op, ": q and q_out must have ", T, " rows");
-    a.q = q->data_ptr();
-    a.ld_q = static_cast<int>(q->stride(0));
-    a.q_out = q_out->data_ptr();
-    a.ld_qo = static_cast<int>(q_out->stride(0));
+  if (fused) {
+    MSG_CHECK(hq >= 1, op, ": hq must be positive");
+    check_rows16(op, k, "qkv", (hq + 2 * hk) * d, pool);
+  } else {
+    check_rows16(op, k, "k", hk * d, pool);
+    check_rows16(op, *v, "v", hk * d, pool);
+    MSG_CHECK(v->size(0) == k.size(0), op, ": k and v must have as many rows");
+  }
+  const int64_t T = k.size(0);
+  const char* rows = static_cast<const char*>(k.data_ptr());
+  if (fused) {
+    const at::Tensor& out = q_out.has_value() ? *q_out : k;
+    check_rows16(op, out, "q_out", hq * d, pool);
+    MSG_CHECK(out.size(0) == T, op, ": q_out must have ", T, " rows");
+    a.q = rows;
+    a.ld_q = static_cast<int>(k.stride(0));
+    a.q_out = out.data_ptr();
+    a.ld_qo = static_cast<int>(out.stride(0));
     a.hq = static_cast<int>(hq);
   }
-  check_rows16(op, k, "k", hk * d, pool);
-  check_rows16(op, v, "v", hk * d, pool);
-  MSG_CHECK(v.size(0) == T, op, ": k and v must have as many rows");
   check_index(op, out_loc, "out_loc", T, pool);
   if (cos_sin.has_value()) {
     MSG_CHECK(positions.has_value(), op, ": positions are needed");
@@ -1515,10 +1524,10 @@ void kv4_store(const c10::optional<at::Tensor>& q, const c10::optional<at::Tenso
   }
   a.q_norm_w = norm_ptr(op, q_norm_w, "q_norm_w", d, pool);
   a.k_norm_w = norm_ptr(op, k_norm_w, "k_norm_w", d, pool);
-  a.k = k.data_ptr();
+  a.k = rows + a.hq * d * 2;
   a.ld_k = static_cast<int>(k.stride(0));
-  a.v = v.data_ptr();
-  a.ld_v = static_cast<int>(v.stride(0));
+  a.v = fused ? rows + (a.hq + hk) * d * 2 : v->data_ptr();
+  a.ld_v = static_cast<int>(fused ? k.stride(0) : v->stride(0));
   a.k_pool = p.k;
   a.v_pool = p.v;
   a.kv_slots = p.slots;
@@ -1527,23 +1536,23 @@ void kv4_store(const c10::optional<at::Tensor>& q, const c10::optional<at::Tenso
   a.hk = static_cast<int>(hk);
   a.d = static_cast<int>(d);
   a.page_size = static_cast<int>(page_size);
+  a.page_shift = p.shift;
   a.eps = static_cast<float>(eps);
   a.err = err_ptr(err);
   const c10::cuda::CUDAGuard guard(pool.device());
   minisgl::launch_kv4_store(a, stream_of(pool));
 }
 
-void kv4_load(const at::Tensor& pool, int64_t layer, const at::Tensor& slots, at::Tensor k_out, at::Tensor v_out,
-              int64_t hk, int64_t d, int64_t page_size, const c10::optional<at::Tensor>& err) {
+std::tuple<at::Tensor, at::Tensor> kv4_load(const at::Tensor& pool, int64_t layer, const at::Tensor& slots, int64_t hk,
+                                            int64_t d, int64_t page_size, const c10::optional<at::Tensor>& err) {
   const char* op = "load_kv4";
   const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
   check_index(op, slots, "slots", -1, pool);
   const int64_t T = slots.numel();
   MSG_CHECK(T <= 0x7fffffff / 2, op, ": too many rows");
-  for (const at::Tensor* x : {&k_out, &v_out})
-    MSG_CHECK(x->is_cuda() && x->device() == pool.device() && x->scalar_type() == at::kBFloat16 &&
-                  x->is_contiguous() && x->numel() == T * hk * d && reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0,
-              op, ": outputs must be contiguous bfloat16 [", T, ", ", hk, ", ", d, "] on kv_pool's device");
+  const c10::cuda::CUDAGuard guard(pool.device());
+  at::Tensor k_out = at::detail::empty_cuda({T, hk, d}, at::kBFloat16, pool.device(), c10::nullopt);
+  at::Tensor v_out = at::detail::empty_cuda({T, hk, d}, at::kBFloat16, pool.device(), c10::nullopt);
   minisgl::Kv4LoadArgs a{};
   a.k_pool = p.k;
   a.v_pool = p.v;
@@ -1555,9 +1564,10 @@ void kv4_load(const at::Tensor& pool, int64_t layer, const at::Tensor& slots, at
   a.hk = static_cast<int>(hk);
   a.d = static_cast<int>(d);
   a.page_size = static_cast<int>(page_size);
+  a.page_shift = p.shift;
   a.err = err_ptr(err);
-  const c10::cuda::CUDAGuard guard(pool.device());
   minisgl::launch_kv4_load(a, stream_of(pool));
+  return {k_out, v_out};
 }
 
 // Rows of a prefill plan as a bf16 pool [2, 1, R / 64, hk, 64, d].
@@ -1592,15 +1602,16 @@ void kv4_expand(const at::Tensor& pool, int64_t layer, const at::Tensor& page_ta
   a.hk = static_cast<int>(hk);
   a.d = static_cast<int>(d);
   a.page_size = static_cast<int>(page_size);
+  a.page_shift = p.shift;
   a.err = err_ptr(err);
   const c10::cuda::CUDAGuard guard(pool.device());
   minisgl::launch_kv4_load(a, stream_of(pool));
 }
 
 // Few query rows over the 4-bit cache; cu_q absent: one token per request.
-void kv4_attention(const at::Tensor& q, at::Tensor out, const at::Tensor& pool, int64_t layer,
-                   const at::Tensor& page_table, const at::Tensor& req_rows, const at::Tensor& seq_lens,
-                   const c10::optional<at::Tensor>& cu_q, int64_t max_q, int64_t hq, int64_t hk, int64_t d,
+at::Tensor kv4_attention(const at::Tensor& q, const c10::optional<at::Tensor>& dst, const at::Tensor& pool, int64_t layer,
+                         const at::Tensor& page_table, const at::Tensor& req_rows, const at::Tensor& seq_lens,
+                         const c10::optional<at::Tensor>& cu_q, int64_t max_q, int64_t hq, int64_t hk, int64_t d,
                    int64_t page_size, double scale, const c10::optional<at::Tensor>& err) {
   const char* op = cu_q.has_value() ? "prefill_attention_kv4" : "decode_attention_kv4";
   const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
@@ -1608,6 +1619,8 @@ void kv4_attention(const at::Tensor& q, at::Tensor out, const at::Tensor& pool, 
   MSG_CHECK(scale > 0 && scale <= 1e6, op, ": scale must be positive");
   check_rows16(op, q, "q", hq * d, pool);
   const int64_t T = q.size(0), B = req_rows.numel();
+  const c10::cuda::CUDAGuard guard(pool.device());
+  at::Tensor out = dst.has_value() ? *dst : at::Tensor(at::detail::empty_cuda({T, hq * d}, at::kBFloat16, pool.device(), c10::nullopt));
   MSG_CHECK(out.is_cuda() && out.device() == pool.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
                 out.numel() == T * hq * d && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
             op, ": out must be contiguous bfloat16 [", T, ", ", hq * d, "] on kv_pool's device");
@@ -1618,14 +1631,14 @@ void kv4_attention(const at::Tensor& q, at::Tensor out, const at::Tensor& pool, 
   if (cu_q.has_value()) check_index(op, *cu_q, "cu_q", B + 1, pool);
   else MSG_CHECK(T == B, op, ": one query token per request, got ", T, " for ", B);
   MSG_CHECK(B <= minisgl::kKv4MaxBatch, op, ": at most ", static_cast<int64_t>(minisgl::kKv4MaxBatch), " requests, got ", B);
-  if (B == 0 || T == 0) return;
+  if (B == 0 || T == 0) return out;
   MSG_CHECK(page_table.size(0) >= 1 && page_table.size(1) >= 1, op, ": page_table is empty");
   const int64_t rows = (max_q * (hq / hk) + 7) / 8;
-  MSG_CHECK(B * hk * rows * ((page_table.size(1) + 127) / 128) < (int64_t{1} << 30), op, ": too many tiles of work");
-  const c10::cuda::CUDAGuard guard(pool.device());
-  const int ctas = minisgl::kv4_attn_ctas(at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+  MSG_CHECK(B * hk * rows * ((page_table.size(1) + 127) / 128) < (int64_t{1} << 30) && T * hq <= 0x7fffffff, op,
+            ": too many tiles of work");
+  const int runs = minisgl::kv4_attn_runs(at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
   // records of partial pieces, then the descriptors
-  const int64_t floats = static_cast<int64_t>(ctas) * 2 * 8 * (d + 2) + 4 * ctas;
+  const int64_t floats = static_cast<int64_t>(runs) * 2 * 8 * (d + 2) + 4 * runs;
   at::Tensor work = at::detail::empty_cuda({floats}, at::kFloat, pool.device(), c10::nullopt);
   minisgl::Kv4AttnArgs a{};
   a.q = q.data_ptr();
@@ -1643,17 +1656,20 @@ void kv4_attention(const at::Tensor& q, at::Tensor out, const at::Tensor& pool, 
   a.B = static_cast<int>(B);
   a.hq = static_cast<int>(hq);
   a.hk = static_cast<int>(hk);
+  a.group = static_cast<int>(hq / hk);
+  for (a.pow2 = 1; 2 * a.pow2 <= a.B;) a.pow2 *= 2;
   a.d = static_cast<int>(d);
   a.page_size = static_cast<int>(page_size);
-  for (a.page_shift = 0; (int64_t{1} << a.page_shift) < page_size; ++a.page_shift) {}
+  a.page_shift = p.shift;
   a.scale = static_cast<float>(scale);
-  a.ctas = ctas;
+  a.runs = runs;
   float* w = work.data_ptr<float>();
   a.desc = reinterpret_cast<int32_t*>(w);
-  a.part_ml = w + 4 * ctas;
-  a.part_o = a.part_ml + static_cast<int64_t>(ctas) * 2 * 8 * 2;
+  a.part_ml = w + 4 * runs;
+  a.part_o = a.part_ml + static_cast<int64_t>(runs) * 2 * 8 * 2;
   a.err = err_ptr(err);
   minisgl::launch_kv4_attention(a, stream_of(pool));
+  return out;
 }
 
 // Pages src[i] -> dst[i] of every plane before `page_dim` of a pool.

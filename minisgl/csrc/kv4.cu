@@ -25,149 +25,184 @@ __device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
   }
 }
 
-// Codes of eight dims of one row, four lanes to a group of 32: the scale byte
-// and the word of nibbles (dim i in bits 4 i .. 4 i + 3). `lanes` are the
-// threads that call. amax / 7.5 is rounded up to four significant bits by
-// adding all but one unit of the dropped 20 bits; IEEE division keeps
-// max |x| = 7.5 s and the halves between codes exact for bf16 rows.
-__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t lanes, uint32_t& word) {
-  float top = 0.f;
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Codes of eight dims of one row, four lanes to a group of 32 (whole warps call):
+// the scale byte and the word of nibbles (dim i in bits 4 i .. 4 i + 3).
+//
+// top / 7.5 is rounded up to four significant bits by adding all but one unit of
+// the 20 bits that go. x / s is a product with the reciprocal and one correction
+// by its remainder (Markstein, IBM J. Res. Dev. 34, 1990): exact where the
+// quotient is a float, so that halves between codes, which rows of 8 bits meet
+// often, go to the even one as the format says. Adding 1.5 2^23 + 8 rounds it and
+// leaves the code in the low bits; words add up with the constants' bits and
+// lose those at the end.
+__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t& word) {
+  float top = fabsf(x[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));  // fmaxf drops NaN
-  top = fmaxf(top, __shfl_xor_sync(lanes, top, 1));
-  top = fmaxf(top, __shfl_xor_sync(lanes, top, 2));
-  const int r = static_cast<int>((__float_as_uint(__fdiv_rn(top, 7.5f)) + 0xfffffu) >> 20);
+  for (int i = 1; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
+  top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  if (top <= 7.5f * 1920.f) {
+    const int r = static_cast<int>((__float_as_uint(__fdiv_rn(top, 7.5f)) + 0xfffffu) >> 20);
+    const uint32_t byte = static_cast<uint32_t>(max(r - (106 << 3), 0));
+    const float s = kv4::scale_f32(byte), inv = __frcp_rn(s);
+    constexpr uint32_t kBits = 0x4b400000u;  // of 1.5 2^23
+    word = 0u - (kBits * 0x11111111u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float q = x[i] * inv;
+      q = fmaf(fmaf(-q, s, x[i]), inv, q);
+      word += __float_as_uint(fminf(q, 7.25f) + 12582920.f) << (4 * i);  // 7.5 would go to 8
+    }
+    return byte;
+  }
+  // beyond the range: an infinity's side, NaN as zero
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));  // drops NaN
+  const uint32_t four = 0xfu << (threadIdx.x & 28);
+  most = fmaxf(most, __shfl_xor_sync(four, most, 1));
+  most = fmaxf(most, __shfl_xor_sync(four, most, 2));
+  const int r = static_cast<int>((__float_as_uint(__fdiv_rn(most, 7.5f)) + 0xfffffu) >> 20);
   const uint32_t byte = static_cast<uint32_t>(min(max(r - (106 << 3), 0), 255));
   const float s = kv4::scale_f32(byte);
   word = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // clamped as a float (an infinity stays on its side); NaN converts to 0
-    const float t = __fdiv_rn(x[i], s);
-    const int c = __float2int_rn(fminf(fmaxf(t, -8.f), 7.f));
-    word |= static_cast<uint32_t>(t == t ? c + 8 : 8) << (4 * i);
+    const float q = __fdiv_rn(x[i], s);
+    const int c = __float2int_rn(fminf(fmaxf(q, -8.f), 7.f));
+    word |= static_cast<uint32_t>(q == q ? c + 8 : 8) << (4 * i);
   }
   return byte;
 }
 
 // ================================================================ store ====
-// Eight dims a thread, D / 8 threads a head. Blocks below `qk_blocks` take
-// queries and keys: a thread keeps the cosines and sines of its dims for `hpt`
-// heads of one token (they are as many bytes as the head itself). The others
-// take values, four tokens a thread, so that a run of tokens whose slots fill
+// Eight dims a thread, D / 8 threads a head, one role a block: queries and keys,
+// kHeads of one token a thread (its cosines and sines, as many bytes as a head,
+// are read once, and all its rows are on the way before the first is worked
+// on), or values, four tokens a thread, so that a run of tokens whose slots fill
 // whole rows of V codes is written in 16-byte chunks; other tokens' codes are
-// bytes between those of their neighbours. Every rounding of q is the one to
-// bf16 at the end, of k and v the one to codes.
-template <int D>
-__global__ void __launch_bounds__(256) kv4_store_kernel(Kv4StoreArgs a, int hpt, int qk_blocks) {
-  pdl_launch_dependents();
-  pdl_wait();
-  constexpr int kLanes = D / 8;        // threads of a head
-  constexpr int kHeads = 256 / kLanes;  // heads at once
-  constexpr int kNG = D / kv4::kGroup;
-  const ErrorSink err{a.err};
-  const int x = threadIdx.x % kLanes;
-  const uint32_t lanes = (kLanes == 16 ? 0xffffu : 0xffu) << ((threadIdx.x & 31) / kLanes * kLanes);
-  const int64_t block = static_cast<int64_t>(a.page_size) * kv4::row_bytes(D);
-
-  if (static_cast<int>(blockIdx.x) < qk_blocks) {
-    const int heads = a.hq + a.hk;
-    const int per = (heads + hpt - 1) / hpt;
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * kHeads + threadIdx.x / kLanes;
-    if (unit >= static_cast<int64_t>(a.T) * per) return;
-    const int t = static_cast<int>(unit / per);
-    const int h0 = static_cast<int>(unit % per) * hpt;
-    const bool first = x < kLanes / 2;
-    float c[8], s[8];
-    if (a.cos_sin != nullptr) {
-      int pos = a.positions[t];
-      if (pos < 0 || pos >= a.max_pos) {
-        if (x == 0) err.report(kErrBadIndex, 951);
-        pos = 0;
-      }
-      const float4* cs = reinterpret_cast<const float4*>(a.cos_sin + static_cast<int64_t>(pos) * D) + x % (kLanes / 2) * 2;
-      const float4 v[4] = {cs[0], cs[1], cs[D / 8], cs[D / 8 + 1]};
-      *reinterpret_cast<float4*>(c) = v[0], *reinterpret_cast<float4*>(c + 4) = v[1];
-      *reinterpret_cast<float4*>(s) = v[2], *reinterpret_cast<float4*>(s + 4) = v[3];
+// bytes between those of their neighbours. q is rounded once, to bf16 at the
+// end, k and v once, to codes.
+template <int D, int kHeads, bool kQuery>
+__device__ __forceinline__ void store_turned(const Kv4StoreArgs& a, int unit, int x, const ErrorSink& err) {
+  constexpr int kLanes = D / 8;  // threads of a head
+  const int heads = kQuery ? a.hq : a.hk;
+  const int per = (heads + kHeads - 1) / kHeads;
+  const bool live = unit < a.T * per;  // the others go along for the shuffles
+  const int t = live ? unit / per : 0;
+  const int h0 = live ? (unit - t * per) * kHeads : 0;
+  const bf16* src = static_cast<const bf16*>(kQuery ? a.q : a.k) + static_cast<int64_t>(t) * (kQuery ? a.ld_q : a.ld_k);
+  uint4 raw[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) raw[i] = *(reinterpret_cast<const uint4*>(src + min(h0 + i, heads - 1) * D) + x);
+  float c[8], s[8];
+  if (a.cos_sin != nullptr) {
+    int pos = a.positions[t];
+    if (pos < 0 || pos >= a.max_pos) {
+      if (live && x == 0) err.report(kErrBadIndex, 951);
+      pos = 0;
     }
-    const int slot = a.out_loc[t];
-    const bool stored = slot >= 0 && slot < a.kv_slots;
-    for (int h = h0; h < min(h0 + hpt, heads); ++h) {
-      const bool is_q = h < a.hq;
-      const bf16* src = is_q ? static_cast<const bf16*>(a.q) + static_cast<int64_t>(t) * a.ld_q + h * D
-                             : static_cast<const bf16*>(a.k) + static_cast<int64_t>(t) * a.ld_k + (h - a.hq) * D;
-      float y[8];
-      unpack8(*(reinterpret_cast<const uint4*>(src) + x), y);
-      const bf16* nw = static_cast<const bf16*>(is_q ? a.q_norm_w : a.k_norm_w);
-      if (nw != nullptr) {
-        float sum = 0.f;
+    const float4* cs = reinterpret_cast<const float4*>(a.cos_sin + static_cast<int64_t>(pos) * D) + x % (kLanes / 2) * 2;
+    const float4 v[4] = {cs[0], cs[1], cs[D / 8], cs[D / 8 + 1]};
+    *reinterpret_cast<float4*>(c) = v[0], *reinterpret_cast<float4*>(c + 4) = v[1];
+    *reinterpret_cast<float4*>(s) = v[2], *reinterpret_cast<float4*>(s + 4) = v[3];
+    if (x < kLanes / 2) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += y[i] * y[i];
-#pragma unroll
-        for (int o = 1; o < kLanes; o *= 2) sum += __shfl_xor_sync(lanes, sum, o);
-        const float inv = rsqrtf(sum / D + a.eps);
-        float w[8];
-        unpack8(*(reinterpret_cast<const uint4*>(nw) + x), w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * w[i];
-      }
-      if (a.cos_sin != nullptr) {
-        // dim j turns with dim j + D / 2, which the thread D / 16 away holds
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float other = __shfl_xor_sync(lanes, y[i], kLanes / 2);
-          y[i] = first ? y[i] * c[i] - other * s[i] : y[i] * c[i] + other * s[i];
-        }
-      }
-      if (is_q) {
-        uint4 o;
-        o.x = pack_bf16x2(y[0], y[1]), o.y = pack_bf16x2(y[2], y[3]);
-        o.z = pack_bf16x2(y[4], y[5]), o.w = pack_bf16x2(y[6], y[7]);
-        *(reinterpret_cast<uint4*>(static_cast<bf16*>(a.q_out) + static_cast<int64_t>(t) * a.ld_qo + h * D) + x) = o;
-      } else {
-        uint32_t word;
-        const uint32_t byte = quantize8(y, lanes, word);
-        if (!stored) {
-          if (x == 0) err.report(kErrBadIndex, 952);
-          continue;
-        }
-        const int page = slot / a.page_size, tok = slot % a.page_size;
-        uint8_t* dst = a.k_pool + (static_cast<int64_t>(page) * a.hk + (h - a.hq)) * block;
-        reinterpret_cast<uint32_t*>(dst + tok * (D / 2))[kv4::k_word<D>(x)] = word;
-        if (x % 4 == 0) dst[a.page_size * (D / 2) + tok * kNG + x / 4] = static_cast<uint8_t>(byte);
-      }
+      for (int i = 0; i < 8; ++i) s[i] = -s[i];
     }
-    return;
   }
+  int page = 0, tok = 0;
+  bool stored = live;
+  if constexpr (!kQuery) {
+    const int slot = a.out_loc[t];
+    stored = live && slot >= 0 && slot < a.kv_slots;
+    if (live && !stored && x == 0) err.report(kErrBadIndex, 952);
+    page = slot >> a.page_shift, tok = slot & (a.page_size - 1);
+  }
+  const bf16* nw = static_cast<const bf16*>(kQuery ? a.q_norm_w : a.k_norm_w);
+  uint4 raw_w;
+  if (nw != nullptr) raw_w = *(reinterpret_cast<const uint4*>(nw) + x);
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = h0 + i;
+    float y[8];
+    unpack8(raw[i], y);
+    if (nw != nullptr) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += y[j] * y[j];
+#pragma unroll
+      for (int o = 1; o < kLanes; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float inv = rsqrtf(sum / D + a.eps);
+      float w[8];
+      unpack8(raw_w, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = y[j] * inv * w[j];
+    }
+    if (a.cos_sin != nullptr) {
+      // dim j turns with dim j + D / 2, which the thread D / 16 away holds
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = y[j] * c[j] + __shfl_xor_sync(0xffffffffu, y[j], kLanes / 2) * s[j];
+    }
+    if constexpr (kQuery) {
+      uint4 o;
+      o.x = pack_bf16x2(y[0], y[1]), o.y = pack_bf16x2(y[2], y[3]);
+      o.z = pack_bf16x2(y[4], y[5]), o.w = pack_bf16x2(y[6], y[7]);
+      if (live && h < heads)
+        *(reinterpret_cast<uint4*>(static_cast<bf16*>(a.q_out) + static_cast<int64_t>(t) * a.ld_qo + h * D) + x) = o;
+    } else {
+      uint32_t word;
+      const uint32_t byte = quantize8(y, word);
+      if (stored && h < heads) {
+        uint8_t* dst = a.k_pool + (static_cast<int64_t>(page) * a.hk + h) * a.page_size * kv4::row_bytes(D);
+        reinterpret_cast<uint32_t*>(dst + tok * (D / 2))[kv4::k_word<D>(x)] = word;
+        if (x % 4 == 0) dst[a.page_size * (D / 2) + tok * (D / kv4::kGroup) + x / 4] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+}
 
-  // ---- values: tokens 4 g - shift .. of one head, with shift the place of the
-  // first token in its row of codes
+// Tokens 4 g - shift .. of one head's values, with shift the place of the first
+// token in its row of codes.
+template <int D>
+__device__ __forceinline__ void store_values(const Kv4StoreArgs& a, int unit, int x, const ErrorSink& err) {
+  constexpr int kNG = D / kv4::kGroup;
   const int shift = a.out_loc[0] & 3;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x - qk_blocks) * kHeads + threadIdx.x / kLanes;
-  const int t0 = static_cast<int>(unit / a.hk) * 4 - shift;
-  const int h = static_cast<int>(unit % a.hk);
-  if (t0 >= a.T) return;
-  uint32_t word[4], byte[4];
+  const int g = unit / a.hk, h = unit - g * a.hk;
+  const int t0 = g * 4 - shift;
+  uint4 raw[4];
   int slot[4];
-  bool run = true;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = t0 + i;
-    slot[i] = -1;
-    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (t >= 0 && t < a.T) {
-      slot[i] = a.out_loc[t];
-      unpack8(*(reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.v) + static_cast<int64_t>(t) * a.ld_v + h * D) + x), y);
-      if (slot[i] < 0 || slot[i] >= a.kv_slots) {
-        if (x == 0) err.report(kErrBadIndex, 953);
-        slot[i] = -1;
-      }
+    const bool live = t >= 0 && t < a.T;
+    raw[i] = *(reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.v) +
+                                              static_cast<int64_t>(min(max(t, 0), a.T - 1)) * a.ld_v + h * D) + x);
+    slot[i] = live ? a.out_loc[t] : -1;
+    if (live && (slot[i] < 0 || slot[i] >= a.kv_slots)) {
+      if (x == 0) err.report(kErrBadIndex, 953);
+      slot[i] = -1;
     }
-    byte[i] = quantize8(y, lanes, word[i]);
-    run = run && slot[i] >= 0 && slot[i] == slot[0] + i;
   }
-  if (run && (slot[0] & 3) == 0) {
-    const int page = slot[0] / a.page_size, row = slot[0] % a.page_size / 4;
+  uint32_t word[4], byte[4];
+  bool run = slot[0] >= 0 && (slot[0] & 3) == 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y[8];
+    unpack8(raw[i], y);
+    byte[i] = quantize8(y, word[i]);
+    run = run && slot[i] == slot[0] + i;
+  }
+  const int64_t block = static_cast<int64_t>(a.page_size) * kv4::row_bytes(D);
+  if (run) {
+    const int page = slot[0] >> a.page_shift, row = (slot[0] & (a.page_size - 1)) / 4;
     uint8_t* dst = a.v_pool + (static_cast<int64_t>(page) * a.hk + h) * block;
     // byte j of token i's word to byte v_byte(i) of word j
     const uint32_t e0 = __byte_perm(word[0], word[2], 0x5140), e1 = __byte_perm(word[0], word[2], 0x7362);
@@ -184,7 +219,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(Kv4StoreArgs a, int hpt,
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (slot[i] < 0) continue;
-    const int page = slot[i] / a.page_size, tok = slot[i] % a.page_size;
+    const int page = slot[i] >> a.page_shift, tok = slot[i] & (a.page_size - 1);
     const int row = tok / 4, b = kv4::v_byte(tok & 3);
     uint8_t* dst = a.v_pool + (static_cast<int64_t>(page) * a.hk + h) * block;
     uint8_t* codes = dst + row * (2 * D) + kv4::v_chunk(row, x) * 16 + b;
@@ -192,6 +227,20 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(Kv4StoreArgs a, int hpt,
     for (int j = 0; j < 4; ++j) codes[4 * j] = static_cast<uint8_t>(word[i] >> (8 * j));
     if (x % 4 == 0) dst[a.page_size * (D / 2) + (row * kNG + x / 4) * 4 + b] = static_cast<uint8_t>(byte[i]);
   }
+}
+
+template <int D, int kHeads>
+__global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ Kv4StoreArgs a, int q_blocks,
+                                                        int k_blocks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int kLanes = D / 8, kUnits = 256 / kLanes;
+  const ErrorSink err{a.err};
+  const int x = threadIdx.x % kLanes, in = threadIdx.x / kLanes;
+  const int block = blockIdx.x;
+  if (block < q_blocks) store_turned<D, kHeads, true>(a, block * kUnits + in, x, err);
+  else if (block < q_blocks + k_blocks) store_turned<D, kHeads, false>(a, (block - q_blocks) * kUnits + in, x, err);
+  else store_values<D>(a, (block - q_blocks - k_blocks) * kUnits + in, x, err);
 }
 
 // ================================================================= load ====
@@ -217,7 +266,7 @@ __device__ __forceinline__ uint4 values8(uint32_t word, uint32_t byte) {
 template <int D>
 __device__ __forceinline__ void load_row(const Kv4LoadArgs& a, int slot, int h, int x, uint4& k, uint4& v) {
   constexpr int kNG = D / kv4::kGroup;
-  const int page = slot / a.page_size, tok = slot % a.page_size, row = tok / 4, b = kv4::v_byte(tok & 3);
+  const int page = slot >> a.page_shift, tok = slot & (a.page_size - 1), row = tok / 4, b = kv4::v_byte(tok & 3);
   const int64_t at = (static_cast<int64_t>(page) * a.hk + h) * a.page_size * kv4::row_bytes(D);
   const uint8_t* kb = a.k_pool + at;
   const uint8_t* vb = a.v_pool + at;
@@ -317,19 +366,27 @@ void copy_pairs(const CopyPagesArgs& a, int from, int n, cudaStream_t s) {
 
 }  // namespace
 
+namespace {
+template <int D>
+void store_typed(const Kv4StoreArgs& a, cudaStream_t s) {
+  constexpr int kUnits = 256 / (D / 8);
+  // one head a thread while that does not fill the GPU, then four
+  const bool many = static_cast<int64_t>(a.T) * (a.hq + a.hk) > 148 * 8 * kUnits;
+  auto blocks = [&](int64_t units) { return (units + kUnits - 1) / kUnits; };
+  const int64_t q = blocks(static_cast<int64_t>(a.T) * (many ? (a.hq + 3) / 4 : a.hq));
+  const int64_t k = blocks(static_cast<int64_t>(a.T) * (many ? (a.hk + 3) / 4 : a.hk));
+  const int64_t v = blocks(static_cast<int64_t>((a.T + 6) / 4) * a.hk);
+  if (q + k + v > 0x7fffffff / kUnits) throw std::runtime_error("minisgl.rope_store_kv4: too many rows");
+  auto kern = many ? kv4_store_kernel<D, 4> : kv4_store_kernel<D, 1>;
+  launch_pdl(kern, dim3(static_cast<unsigned>(q + k + v)), dim3(256), 0, s, a, static_cast<int>(q), static_cast<int>(k));
+}
+}  // namespace
+
 void launch_kv4_store(const Kv4StoreArgs& a, cudaStream_t s) {
   if (a.T <= 0) return;
-  if (a.d != 64 && a.d != 128) throw std::runtime_error("minisgl.rope_store_kv4: head_dim must be 64 or 128");
-  const int per_block = 256 / (a.d / 8);
-  // one head a thread while that does not fill the GPU, then four
-  const int64_t heads = static_cast<int64_t>(a.T) * (a.hq + a.hk);
-  const int hpt = heads > 148 * 8 * per_block ? 4 : 1;
-  const int64_t qk = (static_cast<int64_t>(a.T) * ((a.hq + a.hk + hpt - 1) / hpt) + per_block - 1) / per_block;
-  const int64_t v = (static_cast<int64_t>((a.T + 6) / 4) * a.hk + per_block - 1) / per_block;
-  if (qk + v > 0x7fffffff) throw std::runtime_error("minisgl.rope_store_kv4: too many rows");
-  const dim3 grid(static_cast<unsigned>(qk + v));
-  auto kern = a.d == 128 ? kv4_store_kernel<128> : kv4_store_kernel<64>;
-  launch_pdl(kern, grid, dim3(256), 0, s, a, hpt, static_cast<int>(qk));
+  if (a.d == 128) store_typed<128>(a, s);
+  else if (a.d == 64) store_typed<64>(a, s);
+  else throw std::runtime_error("minisgl.rope_store_kv4: head_dim must be 64 or 128");
 }
 
 void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s) {

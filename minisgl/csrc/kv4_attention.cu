@@ -36,22 +36,39 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWarps = 8;                          // consumers; each takes 16 keys of a tile
-constexpr int kTile = 16 * kWarps;                 // keys per tile
+constexpr int kWarps = 4;                          // each takes 32 keys of a tile
+constexpr int kTile = 32 * kWarps;                 // keys per tile
 constexpr int kRows = 8;                           // query rows per tile
-constexpr int kThreads = (kWarps + 1) * 32;        // and one producer warp
-constexpr int kStages = 4;
+constexpr int kGroups = 3;                         // of kWarps warps in a CTA, one CTA per SM
+constexpr int kThreads = kGroups * (kWarps + 1) * 32;  // each group has a warp that fetches
+constexpr int kStages = 3;
 constexpr float kFloor = -1e30f;                   // maximum of a row that has seen no key
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d = a b
+__device__ __forceinline__ void mma_bf16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -75,64 +92,69 @@ __device__ __forceinline__ uint32_t mul_pair(uint32_t x, uint32_t y) {
       __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
-
-// Bytes of one stage: the K blocks of a tile, then its V blocks.
+// Bytes of one stage: the K blocks of a tile, its V blocks and, where a piece
+// begins, the query rows (16 bytes apart from multiples of 128: no bank twice).
 template <int D>
 constexpr int half_bytes() { return kTile * kv4::row_bytes(D); }
+template <int D>
+constexpr int q_pitch() { return 2 * D + 16; }
+template <int D>
+constexpr int stage_bytes() { return 2 * half_bytes<D>() + kRows * q_pitch<D>(); }
+constexpr int kLd = 64 + 4;  // padded row of the merge buffer (floats): 64 dims at a time
 
-// One request's place in the sequence of tiles.
-struct Piece {
-  int b, h, rt;       // request, KV head, row tile
-  int kt0, kt1, kts;  // key tiles [kt0, kt1) of kts
-};
+template <int D>
+constexpr int group_bytes() { return (kStages * stage_bytes<D>() + kWarps * kRows * (kLd + 2) * 4 + 2 * kStages * 8 + 127) / 128 * 128; }
 
+// Query rows (tokens x heads of a group) and keys of a request.
+template <bool kSingle>
 __device__ __forceinline__ int rows_of(const Kv4AttnArgs& a, int b) {
-  const int n = a.cu_q == nullptr ? 1 : max(0, a.cu_q[b + 1] - a.cu_q[b]);
-  return n * (a.hq / a.hk);
+  return (kSingle ? 1 : max(0, a.cu_q[b + 1] - a.cu_q[b])) * a.group;
 }
 __device__ __forceinline__ int keys_of(const Kv4AttnArgs& a, int b) { return min(max(a.seq_lens[b], 0), a.ld_pt); }
 __device__ __forceinline__ int key_tiles(int keys) { return max(1, (keys + kTile - 1) / kTile); }
 
-// The run [at, end) of this CTA as pieces, request by request (pre: sums of the
-// requests' tiles, in shared memory).
-struct Walk {
-  int at, end, b;
-  __device__ __forceinline__ bool next(const Kv4AttnArgs& a, const int* pre, Piece& p) {
-    if (at >= end) return false;
-    while (pre[b + 1] <= at) ++b;
-    const int kts = key_tiles(keys_of(a, b));
-    const int in = at - pre[b];
-    const int tile_rows = (rows_of(a, b) + kRows - 1) / kRows;
-    p.b = b, p.kts = kts;
-    p.kt0 = in % kts;
-    const int unit = in / kts;
-    p.rt = unit % tile_rows, p.h = unit / tile_rows;
-    p.kt1 = min(kts, p.kt0 + end - at);
-    at += p.kt1 - p.kt0;
-    return true;
-  }
+// One piece of a CTA's run: key tiles [kt0, kt1) of kts of a request, KV head
+// and tile of query rows.
+struct Piece {
+  int b, h, rt;
+  int kt0, kt1, kts;
 };
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(Kv4AttnArgs a) {
-  extern __shared__ uint8_t smem_raw[];
+__device__ __forceinline__ void group_sync(int group) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kWarps * 32) : "memory");
+}
+// A wait whose first try mostly succeeds; the bounded loop is kept out of line.
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* flag, int where) {
+  return mbar_wait(bar, parity, ErrorSink{flag}, where);
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* flag, int where) {
+  return mbar_try_wait(bar, parity) || wait_slow(bar, parity, flag, where);
+}
+
+// kSingle: one query token per request (row r of a KV head is its head r).
+template <int D, bool kSingle>
+__global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
+  extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kNG = D / kv4::kGroup;    // scale groups of a row
+  constexpr int kHalves = D / 64;         // 64-dim halves of V
   constexpr int kHalf = half_bytes<D>();
-  constexpr int kStage = 2 * kHalf;
-  constexpr int kLd = D + 4;              // padded row of the merge buffer (floats)
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
+  constexpr int kStage = stage_bytes<D>();
+  constexpr int kPitch = q_pitch<D>();
+  const ErrorSink err{a.err};
+  const int warp = (threadIdx.x >> 5) % kWarps, lane = threadIdx.x & 31;
+  const bool fetches = threadIdx.x >= kGroups * kWarps * 32;
+  const int group = fetches ? (threadIdx.x >> 5) - kGroups * kWarps : (threadIdx.x >> 5) / kWarps;
+  uint8_t* ring = smem + group * group_bytes<D>();
   float* so = reinterpret_cast<float*>(ring + kStages * kStage);  // [warps][rows][kLd]
   float* sm = so + kWarps * kRows * kLd;                          // [warps][rows]
   float* sl = sm + kWarps * kRows;
   uint64_t* full = reinterpret_cast<uint64_t*>(sl + kWarps * kRows);
   uint64_t* empty = full + kStages;
-  int* pre = reinterpret_cast<int*>(empty + kStages);  // [B + 1]
-  const ErrorSink err{a.err};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* pre = reinterpret_cast<int*>(smem + kGroups * group_bytes<D>());  // [B + 1] sums of tiles
+  int* len = pre + a.B + 1;                                              // [B] keys
 
   pdl_launch_dependents();
-  if (threadIdx.x == 0) {
+  if (fetches && lane == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], kWarps);
@@ -140,13 +162,13 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(Kv4AttnArgs a) {
     fence_barrier_init();
   }
   pdl_wait();
-  // sums of the requests' tiles
   for (int b = threadIdx.x; b < a.B; b += kThreads) {
-    const int rows = rows_of(a, b);
-    pre[b + 1] = key_tiles(keys_of(a, b)) * ((rows + kRows - 1) / kRows) * a.hk;
+    const int keys = keys_of(a, b);
+    len[b] = keys;
+    pre[b + 1] = key_tiles(keys) * ((rows_of<kSingle>(a, b) + kRows - 1) / kRows) * a.hk;
   }
   __syncthreads();
-  if (warp == 0) {
+  if (threadIdx.x < 32) {
     int carry = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       int v = b0 + lane < a.B ? pre[b0 + lane + 1] : 0;
@@ -161,372 +183,463 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_kernel(Kv4AttnArgs a) {
     if (lane == 0) pre[0] = 0;
   }
   __syncthreads();
+  // equal runs for the groups of all CTAs (CTA by CTA in the last place, so that
+  // few runs use every SM); none is empty among the first n, so the records of a
+  // chain of pieces are all written
   const int64_t total = pre[a.B];
-  // no run is empty among the first n CTAs, so the records of a chain are all written
-  const int n = min(static_cast<int>(gridDim.x), pre[a.B]), me = blockIdx.x;
-  Walk walk;
-  walk.at = me < n ? static_cast<int>(total * me / n) : 0;
-  walk.end = me < n ? static_cast<int>(total * (me + 1) / n) : 0;
-  {
-    int lo = 0, hi = a.B;  // last b with pre[b] <= at
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (pre[mid] <= walk.at) lo = mid; else hi = mid;
-    }
-    walk.b = lo;
-  }
-  int4* desc = reinterpret_cast<int4*>(a.desc) + me;
-  if (threadIdx.x == 0) *desc = make_int4(-1, 0, 0, 0);
-  const int page_size = a.page_size, shift = a.page_shift;
-  const int seg = min(page_size, kTile);       // keys that are side by side in the cache
+  const int n = min(kGroups * static_cast<int>(gridDim.x), pre[a.B]), me = group * gridDim.x + blockIdx.x;
+  const int first = me < n ? static_cast<int>(total * me / n) : 0;
+  const int count = me < n ? static_cast<int>(total * (me + 1) / n) - first : 0;
+  int b_at = 0;  // the request of tile `first`: the last b with pre[b] <= first
+  for (int step = a.pow2; step > 0; step /= 2)
+    if (b_at + step < a.B && pre[b_at + step] <= first) b_at += step;
+
+  const int seg = min(a.page_size, kTile);  // keys that are side by side in the cache
   const int segs = kTile / seg;
   const int seg_bytes = seg * kv4::row_bytes(D);
-  Piece p;
 
-  if (warp == kWarps) {
-    // ------------------------------------------------------------ producer ----
-    const int64_t block = static_cast<int64_t>(page_size) * kv4::row_bytes(D);
-    int it = 0;
-    bool ok = true;
-    while (ok && walk.next(a, pre, p)) {
-      const int row = a.req_rows[p.b];
-      const bool row_ok = row >= 0 && row < a.pt_rows;
-      if (!row_ok && lane == 0) err.report(kErrBadIndex, 961);
-      const int32_t* pt = a.page_table + static_cast<int64_t>(row_ok ? row : 0) * a.ld_pt;
-      const int keys = row_ok ? keys_of(a, p.b) : 0;
-      if (a.seq_lens[p.b] > a.ld_pt && lane == 0) err.report(kErrBadIndex, 962);
-      auto slot_of = [&](int kt) {
-        const int pos = kt * kTile + lane * seg;
-        return lane < segs && pos < keys ? pt[pos] : -1;
-      };
-      int slot = slot_of(p.kt0);
-      for (int kt = p.kt0; kt < p.kt1; ++kt, ++it) {
-        const int next = kt + 1 < p.kt1 ? slot_of(kt + 1) : -1;  // a tile ahead
-        const int s = it % kStages;
-        if (it >= kStages && !mbar_wait(&empty[s], ((it / kStages) & 1u) ^ 1u, err, 260)) {
-          ok = false;
-          break;
+  if (fetches) {
+    // ---- tiles of the run into the ring, page numbers read a tile ahead
+    if (lane == 0) reinterpret_cast<int4*>(a.desc)[me] = make_int4(-1, 0, 0, 0);
+    int b = b_at, kt = 0, kts = 0, unit = 0, keys = 0, rows = 0, tile_rows = 1, h = 0;
+    const int32_t* pt = a.page_table;
+    bool row_ok = true;
+    auto begin = [&](int at) {  // the request and unit of tile `at`
+      while (pre[b + 1] <= at) ++b;
+      keys = len[b], kts = key_tiles(keys);
+      rows = rows_of<kSingle>(a, b);
+      tile_rows = (rows + kRows - 1) / kRows;
+      unit = (at - pre[b]) / kts;
+      kt = at - pre[b] - unit * kts;
+      h = tile_rows == 1 ? unit : unit / tile_rows;
+      const int row = a.req_rows[b];
+      row_ok = row >= 0 && row < a.pt_rows;
+      pt = a.page_table + static_cast<int64_t>(row_ok ? row : 0) * a.ld_pt;
+      if (lane == 0 && (!row_ok || a.seq_lens[b] > a.ld_pt)) err.report(kErrBadIndex, row_ok ? 962 : 961);
+    };
+    auto page_of = [&] { return lane < segs && kt * kTile + lane * seg < keys && row_ok ? pt[kt * kTile + lane * seg] : -1; };
+    int slot = -1, issued = -1;
+    if (count > 0) begin(first), slot = page_of();
+    for (int j = 0; j < count; ++j) {
+      // this tile's copies, from what was looked up
+      const bool wanted = lane < segs && kt * kTile + lane * seg < keys && row_ok;
+      const bool good = wanted && slot >= 0 && slot < a.kv_slots;
+      const int64_t at = (static_cast<int64_t>(slot >> a.page_shift) * a.hk + h) * a.page_size * kv4::row_bytes(D);
+      const int off = slot & (a.page_size - 1) & ~(kTile - 1);
+      const bf16* q = nullptr;
+      if (kt == 0 || j == 0) {  // the piece's query rows
+        const int r = (unit - h * tile_rows) * kRows + lane;
+        if (lane < kRows && r < rows) {
+          const int tok = kSingle ? 0 : r / a.group;
+          q = static_cast<const bf16*>(a.q) + static_cast<int64_t>((kSingle ? b : a.cu_q[b]) + tok) * a.ld_q +
+              (h * a.group + r - tok * a.group) * D;
         }
-        const bool wanted = lane < segs && kt * kTile + lane * seg < keys;
-        const bool good = wanted && slot >= 0 && slot < a.kv_slots;
-        if (wanted && !good) err.report(kErrBadIndex, 963);
-        const int count = __popc(__ballot_sync(0xffffffffu, good));
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], 2 * count * seg_bytes);
-        __syncwarp();
-        if (good) {
-          const int off = slot & (page_size - 1);
-          const int64_t at = (static_cast<int64_t>(slot >> shift) * a.hk + p.h) * block;
-          uint8_t* dst = ring + s * kStage + lane * seg_bytes;
-          if (seg == page_size) {
-            bulk_load(dst, a.k_pool + at, seg_bytes, &full[s]);
-            bulk_load(dst + kHalf, a.v_pool + at, seg_bytes, &full[s]);
-          } else {  // part of a larger page: its codes and its scales
-            const int64_t codes = at + (off & ~(kTile - 1)) * (D / 2);
-            const int64_t scales = at + page_size * (D / 2) + (off & ~(kTile - 1)) * kNG;
-            bulk_load(dst, a.k_pool + codes, kTile * (D / 2), &full[s]);
-            bulk_load(dst + kTile * (D / 2), a.k_pool + scales, kTile * kNG, &full[s]);
-            bulk_load(dst + kHalf, a.v_pool + codes, kTile * (D / 2), &full[s]);
-            bulk_load(dst + kHalf + kTile * (D / 2), a.v_pool + scales, kTile * kNG, &full[s]);
-          }
-        }
-        slot = next;
       }
+      // the next tile's page numbers
+      if (++kt == kts && j + 1 < count) begin(first + j + 1);
+      slot = j + 1 < count ? page_of() : -1;
+
+      if (wanted && !good) err.report(kErrBadIndex, 963);
+      const int bytes = 2 * __popc(__ballot_sync(0xffffffffu, good)) * seg_bytes +
+                        __popc(__ballot_sync(0xffffffffu, q != nullptr)) * 2 * D;
+      const int s = j % kStages;
+      if (j >= kStages && !wait_for(&empty[s], (j / kStages - 1) & 1u, a.err, 260)) break;
+      if (lane == 0) mbar_arrive_expect_tx(&full[s], bytes);
+      __syncwarp();
+      uint8_t* st = ring + s * kStage;
+      if (good) {
+        uint8_t* dst = st + lane * seg_bytes;
+        if (seg == a.page_size) {
+          bulk_load(dst, a.k_pool + at, seg_bytes, &full[s]);
+          bulk_load(dst + kHalf, a.v_pool + at, seg_bytes, &full[s]);
+        } else {  // part of a larger page: its codes and its scales
+          const int64_t codes = at + off * (D / 2);
+          const int64_t scales = at + a.page_size * (D / 2) + off * kNG;
+          bulk_load(dst, a.k_pool + codes, kTile * (D / 2), &full[s]);
+          bulk_load(dst + kTile * (D / 2), a.k_pool + scales, kTile * kNG, &full[s]);
+          bulk_load(dst + kHalf, a.v_pool + codes, kTile * (D / 2), &full[s]);
+          bulk_load(dst + kHalf + kTile * (D / 2), a.v_pool + scales, kTile * kNG, &full[s]);
+        }
+      }
+      if (q != nullptr) bulk_load(st + 2 * kHalf + lane * kPitch, q, 2 * D, &full[s]);
+      issued = j;
     }
     // copies in flight land before the CTA's shared memory is given back
-    for (int j = max(0, it - kStages); j < it; ++j)
-      if (!mbar_wait(&full[j % kStages], (j / kStages) & 1u, err, 261)) break;
+    for (int j = max(0, issued - kStages + 1); j <= issued; ++j)
+      if (!wait_for(&full[j % kStages], (j / kStages) & 1u, a.err, 261)) break;
     return;
   }
 
-  // ------------------------------------------------------------- consumers ----
   const int g = lane >> 2, t = lane & 3;
-  const int G = a.hq / a.hk;
   const float c = a.scale * kLog2e;
-  // this lane's keys of the warp's 16 (rows g and g + 8 of S^T), the segment
-  // they lie in and the places of its codes and scales there
-  const int key0 = warp * 16 + 4 * (g >> 1) + (g & 1);
-  const int seg_at = (warp * 16 / seg) * seg_bytes;
-  const int in_seg = (warp * 16) & (seg - 1);
-  const int key_in = in_seg + 4 * (g >> 1) + (g & 1);
-  const int quad_in = in_seg / 4 + t;
-  const int k_at = seg_at + key_in * (D / 2) + t * (D / 8);
-  const int ks_at = seg_at + seg * (D / 2) + key_in * kNG;
-  const int v_at = kHalf + seg_at + quad_in * (2 * D) + ((g ^ (2 * t)) * 16);
-  const int vs_at = kHalf + seg_at + seg * (D / 2) + (quad_in * kNG + (g >> 2)) * 4;
-  constexpr int kHalves = D / 64;  // 64-dim halves of V
-  int it = 0;
+  // this lane's keys of the warp's first 16 (rows g and g + 8 of S^T are keys
+  // key0 and key0 + 2), the segment they lie in and the places of its codes and
+  // scales there; the second 16 keys are a constant distance away
+  const int key0 = warp * 32 + 4 * (g >> 1) + (g & 1);
+  int k_at[2], ks_at[2], v_at[2], vs_at[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int base = warp * 32 + u * 16;
+    const int seg_at = base / seg * seg_bytes, in_seg = base & (seg - 1);
+    const int key_in = in_seg + 4 * (g >> 1) + (g & 1), quad_in = in_seg / 4 + t;
+    k_at[u] = seg_at + key_in * (D / 2) + t * (D / 8);
+    ks_at[u] = seg_at + seg * (D / 2) + key_in * kNG;
+    v_at[u] = kHalf + seg_at + quad_in * (2 * D) + ((g ^ (2 * t)) * 16);
+    vs_at[u] = kHalf + seg_at + seg * (D / 2) + (quad_in * kNG + (g >> 2)) * 4;
+  }
+  int it = 0, s = 0;
+  uint32_t phase = 0;
   bool ok = true;
+  Piece p;
+  p.b = b_at;
 
-  while (walk.next(a, pre, p)) {
-    const int keys = keys_of(a, p.b);
-    const int q0 = a.cu_q == nullptr ? p.b : a.cu_q[p.b];
-    const int rows = rows_of(a, p.b);
-    const int q_len = rows / G;
-    // query fragments of row 8 rt + g, and the starts of its groups' sums
-    uint32_t qb[kNG][4];
-    float init[kNG][2];
+  while (it < count) {
+    // ---- the next piece
     {
-      const int r = p.rt * kRows + g;
-      const bool live = r < rows;
-      const bf16* src = static_cast<const bf16*>(a.q) + static_cast<int64_t>(q0 + (live ? r / G : 0)) * a.ld_q +
-                        (p.h * G + (live ? r % G : 0)) * D + 8 * t;
-#pragma unroll
-      for (int i = 0; i < kNG; ++i) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live) v = *reinterpret_cast<const uint4*>(src + 32 * i);
-        // dims 0..7 of the word -> (0, 4), (1, 5), (2, 6), (3, 7)
-        qb[i][0] = __byte_perm(v.x, v.z, 0x5410), qb[i][1] = __byte_perm(v.x, v.z, 0x7632);
-        qb[i][2] = __byte_perm(v.y, v.w, 0x5410), qb[i][3] = __byte_perm(v.y, v.w, 0x7632);
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum += __uint_as_float(qb[i][j] << 16) + __uint_as_float(qb[i][j] & 0xffff0000u);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= -136.f;
-        init[i][0] = __shfl_sync(0xffffffffu, sum, 8 * t);      // of row 2 t
-        init[i][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);  // of row 2 t + 1
-      }
+      const int at = first + it;
+      while (pre[p.b + 1] <= at) ++p.b;
+      p.kts = key_tiles(len[p.b]);
+      const int in = at - pre[p.b];
+      const int unit = in / p.kts;
+      p.kt0 = in - unit * p.kts;
+      p.kt1 = min(p.kts, p.kt0 + count - it);
+      const int tile_rows = (rows_of<kSingle>(a, p.b) + kRows - 1) / kRows;
+      p.h = tile_rows == 1 ? unit : unit / tile_rows;
+      p.rt = unit - p.h * tile_rows;
     }
+    const int keys = len[p.b];
+    const int rows = rows_of<kSingle>(a, p.b);
     // keys that rows 2 t and 2 t + 1 see, and that every row of the tile sees
-    const int r0 = p.rt * kRows + 2 * t;
-    const int see0 = r0 < rows ? keys - q_len + r0 / G + 1 : 0;
-    const int see1 = r0 + 1 < rows ? keys - q_len + (r0 + 1) / G + 1 : 0;
-    const int see_all = keys - q_len + p.rt * kRows / G + 1;
+    int see0 = keys, see1 = keys, see_all = keys;
+    if constexpr (!kSingle) {
+      const int q_len = rows / a.group, r0 = p.rt * kRows + 2 * t;
+      see0 = keys - q_len + r0 / a.group + 1;
+      see1 = keys - q_len + (r0 + 1) / a.group + 1;
+      see_all = keys - q_len + p.rt * kRows / a.group + 1;
+    }
+    uint32_t qb[kNG][4], off0, off1;
     float o[2 * kNG][4];
 #pragma unroll
     for (int i = 0; i < 2 * kNG; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = kFloor, m1 = kFloor, l0 = 0.f, l1 = 0.f;
-    float mc0 = kFloor * c, mc1 = kFloor * c;
+    float m0 = kFloor, m1 = kFloor, l0 = 0.f, l1 = 0.f, c0 = 0.f, c1 = 0.f;
 
     for (int kt = p.kt0; kt < p.kt1; ++kt, ++it) {
-      const int s = it % kStages;
-      if (ok) ok = mbar_wait(&full[s], (it / kStages) & 1u, err, 262);
       const uint8_t* st = ring + s * kStage;
-      // ---- S^T of 16 keys x 8 rows
-      float sc[4] = {0.f, 0.f, 0.f, 0.f};
-      {
-        uint32_t w0[kNG], w1[kNG];  // words of rows key0 and key0 + 2
-        if constexpr (D == 128) {
-          *reinterpret_cast<uint4*>(w0) = *reinterpret_cast<const uint4*>(st + k_at);
-          *reinterpret_cast<uint4*>(w1) = *reinterpret_cast<const uint4*>(st + k_at + D);
-        } else {
-          *reinterpret_cast<uint2*>(w0) = *reinterpret_cast<const uint2*>(st + k_at);
-          *reinterpret_cast<uint2*>(w1) = *reinterpret_cast<const uint2*>(st + k_at + D);
-        }
-        uint32_t s0, s1;  // the rows' scale bytes
-        if constexpr (D == 128) {
-          s0 = *reinterpret_cast<const uint32_t*>(st + ks_at);
-          s1 = *reinterpret_cast<const uint32_t*>(st + ks_at + 2 * kNG);
-        } else {
-          s0 = *reinterpret_cast<const uint16_t*>(st + ks_at);
-          s1 = *reinterpret_cast<const uint16_t*>(st + ks_at + 2 * kNG);
-        }
+      if (ok) ok = wait_for(&full[s], phase, a.err, 262);
+      if (kt == p.kt0) {
+        // Query fragments of row g in fp16: q 2^-x, 2^x the power of two that takes
+        // the row's largest to 2^14..2^15, which keeps the 8 bits of every element
+        // within 2^-18 of it; odd dims are divided by 16, because their codes are
+        // taken from where they stand, 4 bits up. And -8 times the groups' sums.
+        const bool live = p.rt * kRows + g < rows;
+        uint4 v[kNG];
+        float top = 0.f;
+        bool finite = true;
 #pragma unroll
         for (int i = 0; i < kNG; ++i) {
-          float acc[4] = {init[i][0], init[i][1], init[i][0], init[i][1]};
-          const uint32_t x[4] = {code_pair(w0[i]), code_pair(w1[i]), code_pair(w0[i] >> 4), code_pair(w1[i] >> 4)};
-          mma_bf16(acc, x, qb[i][0], qb[i][1]);
-          const uint32_t y[4] = {code_pair(w0[i] >> 8), code_pair(w1[i] >> 8), code_pair(w0[i] >> 12),
-                                 code_pair(w1[i] >> 12)};
-          mma_bf16(acc, y, qb[i][2], qb[i][3]);
-          const float f0 = kv4::scale_f32(__byte_perm(s0, 0, 0x4440 + i));
-          const float f1 = kv4::scale_f32(__byte_perm(s1, 0, 0x4440 + i));
-          sc[0] += acc[0] * f0, sc[1] += acc[1] * f0;
-          sc[2] += acc[2] * f1, sc[3] += acc[3] * f1;
-        }
-      }
-      const int pos = kt * kTile + key0;
-      if ((kt + 1) * kTile > see_all) {  // uniform over the CTA
-        if (pos >= see0) sc[0] = -INFINITY;
-        if (pos >= see1) sc[1] = -INFINITY;
-        if (pos + 2 >= see0) sc[2] = -INFINITY;
-        if (pos + 2 >= see1) sc[3] = -INFINITY;
-      }
-      // ---- running maximum
-      {
-        float x0 = fmaxf(sc[0], sc[2]), x1 = fmaxf(sc[1], sc[3]);
-        if (__any_sync(0xffffffffu, fmaxf(fmaf(x0, c, -mc0), fmaf(x1, c, -mc1)) > 8.f)) {
+          v[i] = *reinterpret_cast<const uint4*>(st + 2 * kHalf + g * kPitch + 64 * i + 16 * t);
+          if (!live) v[i] = make_uint4(0, 0, 0, 0);
+          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-          for (int sh = 4; sh < 32; sh *= 2) {
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, sh));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, sh));
+          for (int j = 0; j < 4; ++j) {
+            const float x = __uint_as_float(w[j] << 16), y = __uint_as_float(w[j] & 0xffff0000u);
+            top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
+            finite = finite && x == x && y == y;
           }
-          const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-          const float f0 = exp2_approx((m0 - n0) * c), f1 = exp2_approx((m1 - n1) * c);
-          m0 = n0, m1 = n1, mc0 = m0 * c, mc1 = m1 * c;
-          l0 *= f0, l1 *= f1;
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 24);
+        // an infinity or a NaN makes the row NaN, as it does in the formula
+        const float down = finite && ex < 255 ? __uint_as_float((268 - ex) << 23) : NAN;
+        const float up = c * 16777216.f * __uint_as_float((min(ex, 254) - 14) << 23);
+        c0 = __shfl_sync(0xffffffffu, up, 8 * t);      // of row 2 t
+        c1 = __shfl_sync(0xffffffffu, up, 8 * t + 4);  // of row 2 t + 1
+        float sum[kNG];
 #pragma unroll
-          for (int i = 0; i < 2 * kNG; ++i) o[i][0] *= f0, o[i][1] *= f1, o[i][2] *= f0, o[i][3] *= f1;
+        for (int i = 0; i < kNG; ++i) {
+          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          // dims 0..7 of the word -> (0, 4), (1, 5), (2, 6), (3, 7)
+          float z[8];
+          sum[i] = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            z[2 * j] = __uint_as_float(w[j] << 16) * down, z[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * down;
+            sum[i] += z[2 * j] + z[2 * j + 1];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float f = j & 1 ? 0.0625f : 1.f;
+            const __half2 h = __floats2half2_rn(z[j] * f, z[j + 4] * f);
+            qb[i][j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+          sum[i] *= -8.f / 16777216.f;  // codes are c 2^-24
+        }
+        // in three bf16 parts: D = 128: lanes t take groups t % 2 and t % 2 + 2
+        const float x = sum[D == 128 ? t & 1 : 0], y = sum[D == 128 ? 2 + (t & 1) : 1];
+        const uint32_t hi = pack_bf16x2(x, y);
+        const float x1 = x - __uint_as_float(hi << 16), y1 = y - __uint_as_float(hi & 0xffff0000u);
+        const uint32_t mid = pack_bf16x2(x1, y1);
+        const uint32_t lo = pack_bf16x2(x1 - __uint_as_float(mid << 16), y1 - __uint_as_float(mid & 0xffff0000u));
+        if constexpr (D == 128) {
+          off0 = t < 2 ? hi : mid, off1 = t < 2 ? lo : 0u;
+        } else {
+          off0 = t == 0 ? hi : t == 1 ? mid : t == 2 ? lo : 0u, off1 = 0u;
         }
       }
-      const float p0 = exp2_approx(fmaf(sc[0], c, -mc0)), p1 = exp2_approx(fmaf(sc[1], c, -mc1));
-      const float p2 = exp2_approx(fmaf(sc[2], c, -mc0)), p3 = exp2_approx(fmaf(sc[3], c, -mc1));
-      l0 += p0 + p2, l1 += p1 + p3;
-      const uint32_t b0 = transpose8x8(pack_bf16x2(p0, p1));
-      const uint32_t b1 = transpose8x8(pack_bf16x2(p2, p3));
-      // ---- O^T += V^T P^T
+      if (kt * kTile + warp * 32 < keys) {  // some key of the warp's is there
+        // ---- S^T of 2 x 16 keys x 8 rows
+        float sc[2][4];
 #pragma unroll
-      for (int hf = 0; hf < kHalves; ++hf) {
-        const uint4 v4 = *reinterpret_cast<const uint4*>(st + v_at + hf * 128);
-        const uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
-        const uint32_t sv = *reinterpret_cast<const uint32_t*>(st + vs_at + hf * 8);
-        const uint32_t sa = (sv & 0x00ff00ffu) * 16 + kv4::kScaleBf16x2;                        // tokens 0 and 1
-        const uint32_t sb = __byte_perm(sv, 0, 0x4341) * 16 + kv4::kScaleBf16x2;  // tokens 2 and 3
-        const uint32_t oa = mul_pair(sa, 0xc308c308u), ob = mul_pair(sb, 0xc308c308u);          // times -136
+        for (int u = 0; u < 2; ++u) {
+          uint32_t w0[kNG], w1[kNG], s0, s1;  // words and scale bytes of keys key0 and key0 + 2
+          if constexpr (D == 128) {
+            *reinterpret_cast<uint4*>(w0) = *reinterpret_cast<const uint4*>(st + k_at[u]);
+            *reinterpret_cast<uint4*>(w1) = *reinterpret_cast<const uint4*>(st + k_at[u] + D);
+            s0 = *reinterpret_cast<const uint32_t*>(st + ks_at[u]);
+            s1 = *reinterpret_cast<const uint32_t*>(st + ks_at[u] + 2 * kNG);
+          } else {
+            *reinterpret_cast<uint2*>(w0) = *reinterpret_cast<const uint2*>(st + k_at[u]);
+            *reinterpret_cast<uint2*>(w1) = *reinterpret_cast<const uint2*>(st + k_at[u] + D);
+            s0 = *reinterpret_cast<const uint16_t*>(st + ks_at[u]);
+            s1 = *reinterpret_cast<const uint16_t*>(st + ks_at[u] + 2 * kNG);
+          }
+          // the scales as bf16 pairs (groups 0 and 2, 1 and 3; D = 64: 0 and 1)
+          uint32_t e0, e1, d0, d1;
+          float f0[kNG], f1[kNG];
+          if constexpr (D == 128) {
+            e0 = (s0 & 0x00ff00ffu) * 16 + kv4::kScaleBf16x2, d0 = __byte_perm(s0, 0, 0x4341) * 16 + kv4::kScaleBf16x2;
+            e1 = (s1 & 0x00ff00ffu) * 16 + kv4::kScaleBf16x2, d1 = __byte_perm(s1, 0, 0x4341) * 16 + kv4::kScaleBf16x2;
+            f0[0] = __uint_as_float(e0 << 16), f0[2] = __uint_as_float(e0 & 0xffff0000u);
+            f0[1] = __uint_as_float(d0 << 16), f0[3] = __uint_as_float(d0 & 0xffff0000u);
+            f1[0] = __uint_as_float(e1 << 16), f1[2] = __uint_as_float(e1 & 0xffff0000u);
+            f1[1] = __uint_as_float(d1 << 16), f1[3] = __uint_as_float(d1 & 0xffff0000u);
+            if (t & 1) e0 = d0, e1 = d1;
+          } else {
+            e0 = __byte_perm(s0, 0, 0x4140) * 16 + kv4::kScaleBf16x2;
+            e1 = __byte_perm(s1, 0, 0x4140) * 16 + kv4::kScaleBf16x2;
+            f0[0] = __uint_as_float(e0 << 16), f0[1] = __uint_as_float(e0 & 0xffff0000u);
+            f1[0] = __uint_as_float(e1 << 16), f1[1] = __uint_as_float(e1 & 0xffff0000u);
+          }
+          const uint32_t po[4] = {e0, e1, e0, e1};
+          mma_bf16_zero(sc[u], po, off0, off1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t x[4] = {fma_pair(code_pair(w[j]), sa, oa), fma_pair(code_pair(w[j] >> 4), sa, oa),
-                                 fma_pair(code_pair(w[j] >> 8), sb, ob), fma_pair(code_pair(w[j] >> 12), sb, ob)};
-          mma_bf16(o[4 * hf + j], x, b0, b1);
+          for (int i = 0; i < kNG; ++i) {
+            float acc[4];
+            // codes as they stand, c or 16 c, are fp16 numbers c 2^-24 and c 2^-20
+            const uint32_t x[4] = {w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u};
+            mma_f16_zero(acc, x, qb[i][0], qb[i][1]);
+            const uint32_t z0 = w0[i] >> 8, z1 = w1[i] >> 8;
+            const uint32_t y[4] = {z0 & 0x000f000fu, z1 & 0x000f000fu, z0 & 0x00f000f0u, z1 & 0x00f000f0u};
+            mma_f16(acc, y, qb[i][2], qb[i][3]);
+            sc[u][0] += acc[0] * f0[i], sc[u][1] += acc[1] * f0[i];
+            sc[u][2] += acc[2] * f1[i], sc[u][3] += acc[3] * f1[i];
+          }
+        }
+        if ((kt + 1) * kTile > see_all) {  // uniform over the CTA
+          const int pos = kt * kTile + key0;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (pos + 16 * u >= see0) sc[u][0] = -INFINITY;
+            if (pos + 16 * u >= see1) sc[u][1] = -INFINITY;
+            if (pos + 16 * u + 2 >= see0) sc[u][2] = -INFINITY;
+            if (pos + 16 * u + 2 >= see1) sc[u][3] = -INFINITY;
+          }
+        }
+        // ---- running maximum (of the scores in powers of two)
+        {
+          float x0 = fmaxf(fmaxf(sc[0][0], sc[0][2]), fmaxf(sc[1][0], sc[1][2])) * c0;
+          float x1 = fmaxf(fmaxf(sc[0][1], sc[0][3]), fmaxf(sc[1][1], sc[1][3])) * c1;
+          if (__any_sync(0xffffffffu, x0 > m0 + 8.f || x1 > m1 + 8.f)) {
+#pragma unroll
+            for (int sh = 4; sh < 32; sh *= 2) {
+              x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, sh));
+              x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, sh));
+            }
+            const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+            const float f0 = exp2_approx(m0 - n0), f1 = exp2_approx(m1 - n1);
+            m0 = n0, m1 = n1;
+            l0 *= f0, l1 *= f1;
+#pragma unroll
+            for (int i = 0; i < 2 * kNG; ++i) o[i][0] *= f0, o[i][1] *= f1, o[i][2] *= f0, o[i][3] *= f1;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float p0 = exp2_approx(fmaf(sc[u][0], c0, -m0)), p1 = exp2_approx(fmaf(sc[u][1], c1, -m1));
+          const float p2 = exp2_approx(fmaf(sc[u][2], c0, -m0)), p3 = exp2_approx(fmaf(sc[u][3], c1, -m1));
+          l0 += p0 + p2, l1 += p1 + p3;
+          const uint32_t b0 = transpose8x8(pack_bf16x2(p0, p1));
+          const uint32_t b1 = transpose8x8(pack_bf16x2(p2, p3));
+          // ---- O^T += V^T P^T
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf) {
+            const uint4 v4 = *reinterpret_cast<const uint4*>(st + v_at[u] + hf * 128);
+            const uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
+            const uint32_t sv = *reinterpret_cast<const uint32_t*>(st + vs_at[u] + hf * 8);
+            const uint32_t sa = (sv & 0x00ff00ffu) * 16 + kv4::kScaleBf16x2;         // tokens 0 and 1
+            const uint32_t sb = __byte_perm(sv, 0, 0x4341) * 16 + kv4::kScaleBf16x2;  // tokens 2 and 3
+            const uint32_t oa = mul_pair(sa, 0xc308c308u), ob = mul_pair(sb, 0xc308c308u);  // times -136
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t x[4] = {fma_pair(code_pair(w[j]), sa, oa), fma_pair(code_pair(w[j] >> 4), sa, oa),
+                                     fma_pair(code_pair(w[j] >> 8), sb, ob), fma_pair(code_pair(w[j] >> 12), sb, ob)};
+              mma_bf16(o[4 * hf + j], x, b0, b1);
+            }
+          }
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
+      if (++s == kStages) s = 0, phase ^= 1u;
     }
 
-    // ---- the warps' states of the piece, joined
+    // ---- the warps' states of the piece, joined 64 dims at a time: row
+    // 2 warp + lane / 16, four dims a lane
 #pragma unroll
     for (int sh = 4; sh < 32; sh *= 2) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, sh);
       l1 += __shfl_xor_sync(0xffffffffu, l1, sh);
     }
-    consumers_sync();  // the previous piece's states have been read
-    {
+    const int jr = 2 * warp + lane / 16, jd = lane % 16 * 4;
+    const int r = p.rt * kRows + jr;
+    const bool whole = p.kt0 == 0 && p.kt1 == p.kts;
+    const int rec = (2 * me + (p.kt0 == 0 ? 1 : 0)) * kRows + jr;
+    float f[kWarps], inv = 0.f;
+#pragma unroll
+    for (int hf = 0; hf < kHalves; ++hf) {
+      group_sync(group);  // what was here has been read
       float* d0 = so + (warp * kRows + 2 * t) * kLd + 8 * g;
       float* d1 = d0 + kLd;
-#pragma unroll
-      for (int hf = 0; hf < kHalves; ++hf) {
-        const float(*v)[4] = o + 4 * hf;
-        *reinterpret_cast<float4*>(d0 + 64 * hf) = make_float4(v[0][0], v[0][2], v[1][0], v[1][2]);
-        *reinterpret_cast<float4*>(d0 + 64 * hf + 4) = make_float4(v[2][0], v[2][2], v[3][0], v[3][2]);
-        *reinterpret_cast<float4*>(d1 + 64 * hf) = make_float4(v[0][1], v[0][3], v[1][1], v[1][3]);
-        *reinterpret_cast<float4*>(d1 + 64 * hf + 4) = make_float4(v[2][1], v[2][3], v[3][1], v[3][3]);
+      const float(*v)[4] = o + 4 * hf;
+      *reinterpret_cast<float4*>(d0) = make_float4(v[0][0], v[0][2], v[1][0], v[1][2]);
+      *reinterpret_cast<float4*>(d0 + 4) = make_float4(v[2][0], v[2][2], v[3][0], v[3][2]);
+      *reinterpret_cast<float4*>(d1) = make_float4(v[0][1], v[0][3], v[1][1], v[1][3]);
+      *reinterpret_cast<float4*>(d1 + 4) = make_float4(v[2][1], v[2][3], v[3][1], v[3][3]);
+      if (hf == 0 && g == 0) {
+        *reinterpret_cast<float2*>(sm + warp * kRows + 2 * t) = make_float2(m0, m1);
+        *reinterpret_cast<float2*>(sl + warp * kRows + 2 * t) = make_float2(l0, l1);
       }
-      if (g == 0) {
-        sm[warp * kRows + 2 * t] = m0, sm[warp * kRows + 2 * t + 1] = m1;
-        sl[warp * kRows + 2 * t] = l0, sl[warp * kRows + 2 * t + 1] = l1;
-      }
-    }
-    consumers_sync();
-    {
-      constexpr int kE = D / 32;  // dims of a lane; row = warp
-      float top = kFloor;
+      group_sync(group);
+      if (hf == 0) {
+        float top = kFloor, l = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kRows + warp]);
-      float acc[kE] = {}, l = 0.f;
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kRows + jr]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          f[w] = exp2_approx(sm[w * kRows + jr] - top);
+          l += f[w] * sl[w * kRows + jr];
+        }
+        if (whole) {
+          inv = l > 0.f ? 1.f / l : l;  // no key: zeros; NaN stays
+        } else if (lane % 16 == 0) {
+          *reinterpret_cast<float2*>(a.part_ml + 2 * rec) = make_float2(top, l);
+        }
+      }
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2_approx((sm[w * kRows + warp] - top) * c);
-        l += f * sl[w * kRows + warp];
-        const float* v = so + (w * kRows + warp) * kLd + lane * kE;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) acc[e] += f * v[e];
+        const float4 x = *reinterpret_cast<const float4*>(so + (w * kRows + jr) * kLd + jd);
+        acc[0] += f[w] * x.x, acc[1] += f[w] * x.y, acc[2] += f[w] * x.z, acc[3] += f[w] * x.w;
       }
-      const int r = p.rt * kRows + warp;
-      if (p.kt0 == 0 && p.kt1 == p.kts) {
-        if (r < rows) {
-          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
-          uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<bf16*>(a.out) +
-                                                      (static_cast<int64_t>(q0 + r / G) * a.hq + p.h * G + r % G) * D + lane * kE);
-#pragma unroll
-          for (int e = 0; e < kE / 2; ++e) dst[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-        }
-      } else {
-        const int rec = (2 * me + (p.kt0 == 0 ? 1 : 0)) * kRows + warp;
-        float* dst = a.part_o + static_cast<int64_t>(rec) * D + lane * kE;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) dst[e] = acc[e];
-        if (lane == 0) a.part_ml[2 * rec] = top, a.part_ml[2 * rec + 1] = l;
-        if (p.kt0 == 0 && threadIdx.x == 0) {
-          // the CTA whose run holds the piece's last tile
-          const int64_t last = walk.at - 1 + p.kts - p.kt1;
-          *desc = make_int4(static_cast<int>(((last + 1) * n - 1) / total), p.b, p.h, p.rt);
-        }
+      if (!whole) {
+        *reinterpret_cast<float4*>(a.part_o + static_cast<int64_t>(rec) * D + 64 * hf + jd) =
+            make_float4(acc[0], acc[1], acc[2], acc[3]);
+      } else if (r < rows) {
+        const int tok = kSingle ? 0 : r / a.group;
+        bf16* dst = static_cast<bf16*>(a.out) +
+                    (static_cast<int64_t>((kSingle ? p.b : a.cu_q[p.b]) + tok) * a.hq + p.h * a.group + r - tok * a.group) * D;
+        *reinterpret_cast<uint2*>(dst + 64 * hf + jd) =
+            make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
       }
+    }
+    if (!whole && p.kt0 == 0 && warp == 0 && lane == 0) {
+      // the CTA whose run holds the piece's last tile
+      const int64_t last = static_cast<int64_t>(first) + it - 1 + p.kts - p.kt1;
+      reinterpret_cast<int4*>(a.desc)[me] = make_int4(static_cast<int>(((last + 1) * n - 1) / total), p.b, p.h, p.rt);
     }
   }
 }
 
-// Joins the records of the piece that CTA blockIdx.x began and others went on
-// with. Warp w: row w % 8, records w / 8 modulo 4 of the chain.
-template <int D>
-__global__ void __launch_bounds__(1024) kv4_join_kernel(Kv4AttnArgs a) {
+// Joins the records of the piece that run blockIdx.x began and others went on
+// with: row blockIdx.y, records i modulo 8 of the chain in warp i.
+template <int D, bool kSingle>
+__global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kE = D / 32;
-  __shared__ float so[3][kRows][D];
-  __shared__ float sml[3][kRows][2];
+  __shared__ float so[8][D], sl[8], sm[8];
   const int4 d = reinterpret_cast<const int4*>(a.desc)[blockIdx.x];
   if (d.x < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = warp % kRows, part = warp / kRows;
-  const float c = a.scale * kLog2e;
-  float m = kFloor, l = 0.f, acc[kE] = {};
-#pragma unroll 4
-  for (int i = static_cast<int>(blockIdx.x) + part; i <= d.x; i += 4) {
-    const int rec = (2 * i + (i == static_cast<int>(blockIdx.x) ? 1 : 0)) * kRows + row;
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * rec);
-    const float top = fmaxf(m, ml.x);
-    const float f = exp2_approx((m - top) * c), e = exp2_approx((ml.x - top) * c);
-    const float* v = a.part_o + static_cast<int64_t>(rec) * D + lane * kE;
-    m = top, l = l * f + ml.y * e;
-#pragma unroll
-    for (int k = 0; k < kE; ++k) acc[k] = acc[k] * f + v[k] * e;
-  }
-  if (part > 0) {
-#pragma unroll
-    for (int k = 0; k < kE; ++k) so[part - 1][row][lane * kE + k] = acc[k];
-    if (lane == 0) sml[part - 1][row][0] = m, sml[part - 1][row][1] = l;
-  }
+  const int row = blockIdx.y, begin = blockIdx.x, count = d.x - begin + 1;
+  const int G = a.group, r = d.w * kRows + row;
+  if (r >= rows_of<kSingle>(a, d.y)) return;
+  auto rec_of = [&](int i) { return (2 * (begin + i) + (i == 0 ? 1 : 0)) * kRows + row; };
+  float top = kFloor;
+  for (int i = threadIdx.x; i < count; i += 256) top = fmaxf(top, a.part_ml[2 * rec_of(i)]);
+  top = warp_max(top);
+  if (lane == 0) sm[warp] = top;
   __syncthreads();
-  if (part > 0) return;
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    const float top = fmaxf(m, sml[i][row][0]);
-    const float f = exp2_approx((m - top) * c), e = exp2_approx((sml[i][row][0] - top) * c);
-    m = top, l = l * f + sml[i][row][1] * e;
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, sm[w]);
+  float l = 0.f, acc[kE] = {};
+#pragma unroll 4
+  for (int i = warp; i < count; i += 8) {
+    const int rec = rec_of(i);
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * rec);
+    const float f = exp2_approx(ml.x - top);
+    const float* v = a.part_o + static_cast<int64_t>(rec) * D + lane * kE;
+    l += ml.y * f;
 #pragma unroll
-    for (int k = 0; k < kE; ++k) acc[k] = acc[k] * f + so[i][row][lane * kE + k] * e;
+    for (int k = 0; k < kE; ++k) acc[k] += v[k] * f;
   }
-  const int G = a.hq / a.hk;
-  const int r = d.w * kRows + row;
-  if (r >= rows_of(a, d.y)) return;
-  const int q0 = a.cu_q == nullptr ? d.y : a.cu_q[d.y];
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<bf16*>(a.out) +
-                                              (static_cast<int64_t>(q0 + r / G) * a.hq + d.z * G + r % G) * D + lane * kE);
 #pragma unroll
-  for (int e = 0; e < kE / 2; ++e) dst[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  for (int k = 0; k < kE; ++k) so[warp][lane * kE + k] = acc[k];
+  if (lane == 0) sl[warp] = l;
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  l = 0.f;
+  float x = 0.f, y = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) l += sl[w], x += so[w][2 * threadIdx.x], y += so[w][2 * threadIdx.x + 1];
+  const float inv = l > 0.f ? 1.f / l : l;
+  const int q0 = kSingle ? d.y : a.cu_q[d.y];
+  reinterpret_cast<uint32_t*>(static_cast<bf16*>(a.out) + (static_cast<int64_t>(q0 + r / G) * a.hq + d.z * G + r % G) * D)[threadIdx.x] =
+      pack_bf16x2(x * inv, y * inv);
 }
 
 template <int D>
 int attn_smem(int B) {
-  return 128 + kStages * 2 * half_bytes<D>() + kWarps * kRows * (D + 4 + 2) * 4 + 2 * kStages * 8 + (B + 1) * 4;
+  return kGroups * group_bytes<D>() + (2 * B + 1) * 4;
 }
 
-template <int D>
+template <int D, bool kSingle>
 void launch_typed(const Kv4AttnArgs& a, cudaStream_t s) {
   static bool done[64] = {};  // per device
   int dev = 0;
   cudaGetDevice(&dev);
-  const int most = attn_smem<D>(kKv4MaxBatch);
   if (!done[dev & 63]) {
-    if (cudaFuncSetAttribute(kv4_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+    if (cudaFuncSetAttribute(kv4_attn_kernel<D, kSingle>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             attn_smem<D>(kKv4MaxBatch)) != cudaSuccess)
       throw std::runtime_error("minisgl.attention_kv4: shared memory limit");
     done[dev & 63] = true;
   }
-  launch_pdl(kv4_attn_kernel<D>, dim3(a.ctas), dim3(kThreads), attn_smem<D>(a.B), s, a);
-  launch_pdl(kv4_join_kernel<D>, dim3(a.ctas), dim3(1024), 0, s, a);
+  launch_pdl(kv4_attn_kernel<D, kSingle>, dim3(a.runs / kGroups), dim3(kThreads), attn_smem<D>(a.B), s, a);
+  launch_pdl(kv4_join_kernel<D, kSingle>, dim3(a.runs, kRows), dim3(256), 0, s, a);
 }
 
 }  // namespace
 
-int kv4_attn_ctas(int sms) { return 2 * sms; }
+int kv4_attn_runs(int sms) { return kGroups * sms; }
 
 void launch_kv4_attention(const Kv4AttnArgs& a, cudaStream_t s) {
   if (a.B <= 0) return;
-  if (a.d == 128) launch_typed<128>(a, s);
-  else if (a.d == 64) launch_typed<64>(a, s);
+  const bool single = a.cu_q == nullptr;
+  if (a.d == 128) single ? launch_typed<128, true>(a, s) : launch_typed<128, false>(a, s);
+  else if (a.d == 64) single ? launch_typed<64, true>(a, s) : launch_typed<64, false>(a, s);
   else throw std::runtime_error("minisgl.attention_kv4: head_dim must be 64 or 128");
 }
 

@@ -219,7 +219,7 @@ struct Kv4StoreArgs {
   const void *q_norm_w, *k_norm_w;  // [d] bf16 or nullptr
   uint8_t *k_pool, *v_pool;  // this layer's [pages, hk, block bytes]
   const int32_t* out_loc;    // [T]
-  int T, hq, hk, d, page_size;
+  int T, hq, hk, d, page_size, page_shift;
   float eps;
   int64_t kv_slots;          // pages * page_size: other slots are reported, not written
   int* err;
@@ -229,7 +229,7 @@ struct Kv4LoadArgs {
   const uint8_t *k_pool, *v_pool;  // this layer's
   const int32_t* slots;      // [T], or (row_req set) nullptr
   void *k_out, *v_out;       // [T, hk, d] bf16, or a layer's [T / 64, hk, 64, d]
-  int T, hk, d, page_size;
+  int T, hk, d, page_size, page_shift;
   int64_t kv_slots;
   // rows of a prefill plan: key row_pos[r] of request row_req[r] (-1: zeros)
   const int32_t *row_req, *row_pos;
@@ -239,7 +239,7 @@ struct Kv4LoadArgs {
   int* err;
 };
 void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s);
-constexpr int kKv4MaxBatch = 8192;  // requests of one attention call (their tile sums sit in shared memory)
+constexpr int kKv4MaxBatch = 3584;  // requests of one attention call (their tile sums sit in shared memory)
 struct Kv4AttnArgs {
   const void* q;             // [T, >= hq * d] bf16
   int ld_q;
@@ -251,15 +251,16 @@ struct Kv4AttnArgs {
   const int32_t* req_rows;   // [B]
   const int32_t* seq_lens;   // [B]
   const int32_t* cu_q;       // [B + 1], or nullptr: one token per request
-  int B, hq, hk, d, page_size, page_shift;
+  int B, hq, hk, group, d, page_size, page_shift;  // group = hq / hk
+  int pow2;                  // largest power of two <= B
   float scale;
-  int ctas;                  // grid
-  float* part_o;             // [ctas, 2, 8, d] records of partial pieces
-  float* part_ml;            // [ctas, 2, 8, 2]
-  int32_t* desc;             // [ctas, 4]
+  int runs;                  // parts that the work is split into
+  float* part_o;             // [runs, 2, 8, d] records of partial pieces
+  float* part_ml;            // [runs, 2, 8, 2]
+  int32_t* desc;             // [runs, 4]
   int* err;
 };
-int kv4_attn_ctas(int sms);
+int kv4_attn_runs(int sms);
 void launch_kv4_attention(const Kv4AttnArgs& a, cudaStream_t s);
 // Pages src[i] -> dst[i] of every plane of a pool; returns the launches made.
 struct CopyPagesArgs {

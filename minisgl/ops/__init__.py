@@ -822,7 +822,7 @@ def store_kv4(k: torch.Tensor, v: torch.Tensor, kv_pool: torch.Tensor, layer: in
     but for ones whose rows nobody reads."""
     if kv_pool.is_cuda:
         _count()
-        native().kv4_store(None, None, k, v, None, None, None, None, kv_pool, layer, out_loc, 0, hk, d, page_size, 0.0,
+        native().kv4_store(k, v, None, None, None, None, None, kv_pool, layer, out_loc, 0, hk, d, page_size, 0.0,
                            error_word(kv_pool.device))
         return
     _kv4_check("store_kv4", kv_pool, layer, hk, d, page_size)
@@ -839,15 +839,12 @@ def rope_store_kv4(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Te
     place in ``qkv``), k and v as codes to the slots ``out_loc``. The k and v
     columns of ``qkv`` keep their values. Norm and rotation are fp32 and
     rounded once, to q's type and to the codes."""
-    q_out = qkv if q_out is None else q_out
     if kv_pool.is_cuda:
-        if qkv.dim() != 2 or qkv.shape[1] < (hq + 2 * hk) * d:
-            raise ValueError(f"rope_store_kv4: qkv must be [T, >= {(hq + 2 * hk) * d}], got {tuple(qkv.shape)}")
-        k0, v0 = hq * d, (hq + hk) * d
         _count()
-        native().kv4_store(qkv, q_out, qkv[:, k0:], qkv[:, v0:], positions, cos_sin, q_norm_w, k_norm_w, kv_pool, layer,
-                           out_loc, hq, hk, d, page_size, eps, error_word(kv_pool.device))
+        native().kv4_store(qkv, None, q_out, positions, cos_sin, q_norm_w, k_norm_w, kv_pool, layer, out_loc, hq, hk, d,
+                           page_size, eps, error_word(kv_pool.device))
         return
+    q_out = qkv if q_out is None else q_out
     _kv4_check("rope_store_kv4", kv_pool, layer, hk, d, page_size)
     T = qkv.shape[0]
     if qkv.dim() != 2 or qkv.shape[1] < (hq + 2 * hk) * d:
@@ -870,11 +867,8 @@ def load_kv4(kv_pool: torch.Tensor, layer: int, slots: torch.Tensor, hk: int, d:
     if kv_pool.is_cuda:
         if dtype != torch.bfloat16:
             raise ValueError(f"load_kv4: rows come out in bfloat16 on a GPU, got {dtype}")
-        k = torch.empty(slots.numel(), hk, d, dtype=dtype, device=kv_pool.device)
-        v = torch.empty_like(k)
         _count()
-        native().kv4_load(kv_pool, layer, slots, k, v, hk, d, page_size, error_word(kv_pool.device))
-        return k, v
+        return native().kv4_load(kv_pool, layer, slots, hk, d, page_size, error_word(kv_pool.device))
     _kv4_check("load_kv4", kv_pool, layer, hk, d, page_size)
     return ref.load_kv4(kv_pool, layer, slots, hk, d, page_size, dtype)
 
@@ -902,12 +896,9 @@ def decode_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pag
     evenly over the GPU whatever their lengths are; scratch is the call's
     own. A request without keys gives zeros."""
     if kv_pool.is_cuda:
-        if out is None:
-            out = torch.empty(q.shape[0], hq * d, dtype=q.dtype, device=q.device)
         _count(2)
-        native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, None, 1, hq, hk, d, page_size,
-                               scale, error_word(kv_pool.device))
-        return out
+        return native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, None, 1, hq, hk, d,
+                                      page_size, scale, error_word(kv_pool.device))
     cu = torch.arange(req_rows.numel() + 1, dtype=torch.int32)
     return _attention_kv4_cpu("decode_attention_kv4", q, kv_pool, layer, page_table, req_rows, seq_lens, cu, hq, hk, d,
                               page_size, scale, out)
@@ -941,14 +932,13 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
     if not kv_pool.is_cuda:
         return _attention_kv4_cpu("prefill_attention_kv4", q, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq,
                                   hk, d, page_size, scale, out)
-    if out is None:
-        out = torch.empty(q.shape[0], hq * d, dtype=q.dtype, device=q.device)
     err = error_word(kv_pool.device)
     if d != 128 or max_q * (hq // max(1, hk)) <= KV4_FEW_ROWS:
         _count(2)
-        native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, max_q, hq, hk, d, page_size,
-                               scale, err)
-        return out
+        return native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, max_q, hq, hk, d,
+                                      page_size, scale, err)
+    if out is None:
+        out = torch.empty(q.shape[0], hq * d, dtype=q.dtype, device=q.device)
     if plan is None:
         plan = KV4PrefillPlan(seq_lens.tolist(), kv_pool.device)
     if plan.rows == 0:  # no request has a key
