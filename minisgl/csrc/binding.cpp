@@ -1570,42 +1570,98 @@ std::tuple<at::Tensor, at::Tensor> kv4_load(const at::Tensor& pool, int64_t laye
   return {k_out, v_out};
 }
 
-// Rows of a prefill plan as a bf16 pool [2, 1, R / 64, hk, 64, d].
-void kv4_expand(const at::Tensor& pool, int64_t layer, const at::Tensor& page_table, const at::Tensor& req_rows,
-                const at::Tensor& row_req, const at::Tensor& row_pos, at::Tensor out, int64_t hk, int64_t d,
-                int64_t page_size, const c10::optional<at::Tensor>& err) {
+// Many query rows: the plan's rows expanded to tile images, then attention over them.
+at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst, const at::Tensor& pool, int64_t layer,
+                       const at::Tensor& page_table, const at::Tensor& req_rows, const at::Tensor& seq_lens,
+                       const at::Tensor& cu_q, int64_t hq, int64_t hk, int64_t d, int64_t page_size,
+                       double scale, const at::Tensor& plan_table, const at::Tensor& row_req, const at::Tensor& row_pos,
+                       const c10::optional<at::Tensor>& err) {
   const char* op = "prefill_attention_kv4";
   const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
-  const int64_t R = row_req.numel();
+  MSG_CHECK(hq >= hk && hq % hk == 0 && minisgl::kv4_prefill_takes(static_cast<int>(d), static_cast<int>(hq / hk)), op,
+            ": many rows take head_dim 128 and groups of up to 128 heads");
+  MSG_CHECK(scale > 0 && scale <= 1e6, op, ": scale must be positive");
+  check_rows16(op, q, "q", hq * d, pool);
+  const int64_t T = q.size(0), B = req_rows.numel(), R = row_req.numel();
+  const c10::cuda::CUDAGuard guard(pool.device());
+  at::Tensor out = dst.has_value() ? *dst : at::Tensor(at::detail::empty_cuda({T, hq * d}, at::kBFloat16, pool.device(), c10::nullopt));
+  MSG_CHECK(out.is_cuda() && out.device() == pool.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
+                out.numel() == T * hq * d && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+            op, ": out must be contiguous bfloat16 [", T, ", ", hq * d, "] on kv_pool's device");
   check_index(op, page_table, "page_table", -1, pool);
   MSG_CHECK(page_table.dim() == 2, op, ": page_table must be [rows, positions]");
   check_index(op, req_rows, "req_rows", -1, pool);
+  check_index(op, seq_lens, "seq_lens", B, pool);
+  check_index(op, cu_q, "cu_q", B + 1, pool);
   check_index(op, row_req, "the plan's rows", -1, pool);
   check_index(op, row_pos, "the plan's positions", R, pool);
-  MSG_CHECK(R % 64 == 0 && R <= 0x7fffffff / 2, op, ": the plan's rows must be whole pages of 64");
-  MSG_CHECK(out.is_cuda() && out.device() == pool.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
-                out.numel() == 2 * R * hk * d,
-            op, ": compact pool must be bfloat16 [2, 1, R / 64, hk, 64, d]");
-  minisgl::Kv4LoadArgs a{};
-  a.k_pool = p.k;
-  a.v_pool = p.v;
-  a.kv_slots = p.slots;
-  a.row_req = row_req.data_ptr<int32_t>();
-  a.row_pos = row_pos.data_ptr<int32_t>();
-  a.page_table = page_table.data_ptr<int32_t>();
-  a.ld_pt = static_cast<int>(page_table.stride(0));
-  a.pt_rows = static_cast<int>(page_table.size(0));
-  a.req_rows = req_rows.data_ptr<int32_t>();
-  a.k_out = out.data_ptr();
-  a.v_out = static_cast<char*>(out.data_ptr()) + R * hk * d * 2;
-  a.T = static_cast<int>(R);
+  check_index(op, plan_table, "the plan's table", -1, pool);
+  MSG_CHECK(plan_table.dim() == 2 && plan_table.size(0) == B && plan_table.size(1) >= 1, op, ": the plan is of ",
+            plan_table.dim() == 2 ? plan_table.size(0) : 0, " requests, not ", B);
+  MSG_CHECK(R % minisgl::kKv4TileKeys == 0 && R <= 0x7fffffff / 2, op, ": the plan's rows must be whole tiles");
+  MSG_CHECK(B <= minisgl::kKv4MaxBatch, op, ": at most ", static_cast<int64_t>(minisgl::kKv4MaxBatch), " requests, got ", B);
+  const int64_t pair = 2 * (minisgl::kKv4TileKeys / (hq / hk));
+  MSG_CHECK((T / pair + B) * hk * (page_table.size(1) / minisgl::kKv4TileKeys + 1) < (int64_t{1} << 30), op,
+            ": too many tiles of work");
+  if (B == 0 || T == 0) return out;
+  const int ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  // records of partial pieces, then runs and descriptors
+  const int64_t part = static_cast<int64_t>(ctas) * 2 * 256;
+  at::Tensor work = at::detail::empty_cuda({part * (d + 2) + 12 * ctas}, at::kFloat, pool.device(), c10::nullopt);
+  float* w = work.data_ptr<float>();
+  int32_t* runs = reinterpret_cast<int32_t*>(w + part * (d + 2));
+  at::Tensor images = at::detail::empty_cuda({2 * R * hk * d}, at::kBFloat16, pool.device(), c10::nullopt);
+  minisgl::Kv4LoadArgs l{};
+  l.k_pool = p.k;
+  l.v_pool = p.v;
+  l.kv_slots = p.slots;
+  l.row_req = row_req.data_ptr<int32_t>();
+  l.row_pos = row_pos.data_ptr<int32_t>();
+  l.page_table = page_table.data_ptr<int32_t>();
+  l.ld_pt = static_cast<int>(page_table.size(1));
+  l.pt_rows = static_cast<int>(page_table.size(0));
+  l.req_rows = req_rows.data_ptr<int32_t>();
+  l.k_out = images.data_ptr();
+  l.T = static_cast<int>(R);
+  l.hk = static_cast<int>(hk);
+  l.d = static_cast<int>(d);
+  l.page_size = static_cast<int>(page_size);
+  l.page_shift = p.shift;
+  l.runs = runs;
+  l.seq_lens = seq_lens.data_ptr<int32_t>();
+  l.cu_q = cu_q.data_ptr<int32_t>();
+  l.first_tile = plan_table.data_ptr<int32_t>();
+  l.ld_first = static_cast<int>(plan_table.size(1));
+  l.q_rows = static_cast<int>(T);
+  l.B = static_cast<int>(B);
+  l.group = static_cast<int>(hq / hk);
+  l.ctas = ctas;
+  l.err = err_ptr(err);
+  minisgl::launch_kv4_load(l, stream_of(pool));
+  minisgl::Kv4PrefillArgs a{};
+  a.q = q.data_ptr();
+  a.ld_q = static_cast<int>(q.stride(0));
+  a.out = out.data_ptr();
+  a.images = images.data_ptr();
+  a.first_tile = plan_table.data_ptr<int32_t>();
+  a.ld_first = static_cast<int>(plan_table.size(1));
+  a.tiles = static_cast<int>(R / minisgl::kKv4TileKeys);
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.cu_q = cu_q.data_ptr<int32_t>();
+  a.T = static_cast<int>(T);
+  a.B = static_cast<int>(B);
+  a.hq = static_cast<int>(hq);
   a.hk = static_cast<int>(hk);
-  a.d = static_cast<int>(d);
-  a.page_size = static_cast<int>(page_size);
-  a.page_shift = p.shift;
+  a.group = static_cast<int>(hq / hk);
+  a.scale = static_cast<float>(scale);
+  a.ctas = ctas;
+  a.runs = runs;
+  a.desc = runs + 8 * ctas;
+  a.part_o = w;
+  a.part_ml = w + part * d;
   a.err = err_ptr(err);
-  const c10::cuda::CUDAGuard guard(pool.device());
-  minisgl::launch_kv4_load(a, stream_of(pool));
+  minisgl::launch_kv4_prefill(a, stream_of(pool));
+  return out;
 }
 
 // Few query rows over the 4-bit cache; cu_q absent: one token per request.
@@ -1653,6 +1709,7 @@ at::Tensor kv4_attention(const at::Tensor& q, const c10::optional<at::Tensor>& d
   a.req_rows = req_rows.data_ptr<int32_t>();
   a.seq_lens = seq_lens.data_ptr<int32_t>();
   a.cu_q = cu_q.has_value() ? cu_q->data_ptr<int32_t>() : nullptr;
+  a.T = static_cast<int>(T);
   a.B = static_cast<int>(B);
   a.hq = static_cast<int>(hq);
   a.hk = static_cast<int>(hk);
@@ -1998,7 +2055,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention", &decode_attention);
   m.def("kv4_store", &kv4_store);
   m.def("kv4_load", &kv4_load);
-  m.def("kv4_expand", &kv4_expand);
+  m.def("kv4_prefill", &kv4_prefill);
   m.def("kv4_attention", &kv4_attention);
   m.def("copy_pages", &copy_pages);
   m.def("gemm_fused", &gemm_fused);

@@ -279,38 +279,131 @@ __device__ __forceinline__ void load_row(const Kv4LoadArgs& a, int slot, int h, 
   v = values8(__byte_perm(lo, hi, 0x5410), vs);
 }
 
-// Rows of a.slots to k_out / v_out [T, hk, D], or (a.row_req set) rows of a
-// prefill plan to a bf16 pool [2, 1, R / 64, hk, 64, D]: there row r is key
-// row_pos[r] of request row_req[r] (none: zeros) and one block takes 64-row
-// pages, whose rows of a head are side by side.
-template <int D>
-__global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadArgs a) {
+// Splits the key tiles of all (request, pair of row tiles, KV head) of a prefill
+// into runs of equal cost; one block. A row tile has 128 / group tokens. In the
+// sequence that is split a pair has kKv4PairCost places before its tiles, for
+// what a piece costs beside them (queries in, output out); a pair without any key
+// counts as one tile, so that somebody writes its zeros. Runs have four places at
+// least: a record costs about as much as a tile.
+__device__ void plan_runs(const Kv4LoadArgs& a, const ErrorSink& err) {
+  __shared__ int pre[kKv4MaxBatch + 1], units[kKv4MaxBatch + 1];  // sums over the requests: places, pairs x heads
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int W = 2 * (kKv4TileKeys / a.group);  // tokens of a pair
+  auto tiles = [&](int b, int q_len, int pair) {
+    const int keys = a.seq_lens[b];
+    return max(1, (keys - q_len + min(q_len, (pair + 1) * W) + kKv4TileKeys - 1) / kKv4TileKeys);
+  };
+  for (int b = warp; b < a.B; b += 8) {
+    const int q_len = kv4_query_tokens(a.cu_q, b, a.q_rows), keys = a.seq_lens[b];
+    const int first = a.first_tile[static_cast<int64_t>(b) * a.ld_first] / kKv4TileKeys;
+    if (lane == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.q_rows || first < 0 || keys > a.ld_pt ||
+                      (keys > 0 && first + (keys + kKv4TileKeys - 1) / kKv4TileKeys > a.T / kKv4TileKeys)))
+      err.report(kErrBadIndex, 956);
+    int sum = 0;
+    for (int p = lane; p * W < q_len; p += 32) sum += kKv4PairCost + tiles(b, q_len, p);
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) pre[b + 1] = sum * a.hk, units[b + 1] = (q_len + W - 1) / W * a.hk;
+  }
+  __syncthreads();
+  if (warp < 2) {
+    int* x = warp == 0 ? pre : units;
+    int carry = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      int v = b0 + lane < a.B ? x[b0 + lane + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (b0 + lane < a.B) x[b0 + lane + 1] = carry + v;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) x[0] = 0;
+  }
+  __syncthreads();
+  const int64_t total = pre[a.B];
+  const int n = static_cast<int>(min(static_cast<int64_t>(a.ctas), max(total / 4, static_cast<int64_t>(1))));
+  struct Place {
+    int b, pair, h, kt, at, real;  // at: of the pair; real: tiles before
+  };
+  auto find = [&](int v) {
+    Place p{0, 0, 0, 0, 0, 0};
+    if (v >= total) {
+      p.real = static_cast<int>(total) - kKv4PairCost * units[a.B];
+      return p;
+    }
+    int hi = a.B;  // the last b with pre[b] <= v
+    while (hi - p.b > 1) {
+      const int mid = (p.b + hi) / 2;
+      if (pre[mid] <= v) p.b = mid; else hi = mid;
+    }
+    const int q_len = kv4_query_tokens(a.cu_q, p.b, a.q_rows);
+    int in = v - pre[p.b], t = kKv4PairCost + tiles(p.b, q_len, 0);
+    while (in >= t * a.hk) in -= t * a.hk, t = kKv4PairCost + tiles(p.b, q_len, ++p.pair);
+    p.h = in / t;
+    p.kt = max(0, in - p.h * t - kKv4PairCost);
+    p.at = v - (in - p.h * t);
+    p.real = p.at - kKv4PairCost * (units[p.b] + p.pair * a.hk + p.h) + p.kt;
+    return p;
+  };
+  for (int i = threadIdx.x; i < a.ctas; i += 256) {
+    int4* run = reinterpret_cast<int4*>(a.runs) + 2 * i;
+    if (total == 0 || i >= n) {
+      run[0] = run[1] = make_int4(0, 0, 1, 1);
+      run[1].x = 0;
+      continue;
+    }
+    const Place p = find(static_cast<int>(total * i / n)), q = find(static_cast<int>(total * (i + 1) / n));
+    run[0] = make_int4(p.b, p.pair, p.h, p.kt);
+    run[1] = make_int4(q.real - p.real, p.at, static_cast<int>(total), n);
+  }
+}
+
+// Rows of a.slots to k_out / v_out [T, hk, D], or (kImages) rows of a prefill plan
+// to tile images: row r is key row_pos[r] of request row_req[r] (none: zeros);
+// 128 rows of a head are one K and one V image of D / 64 halves, 128 bytes a row
+// and half, whose 16-byte chunks are swizzled as the tcgen05 descriptors read
+// them (chunk c of row r at c ^ (r mod 8)).
+template <int D, bool kImages>
+__global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ Kv4LoadArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kLanes = D / 8;
   const ErrorSink err{a.err};
   const int x = threadIdx.x % kLanes;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  int64_t block = blockIdx.x;
+  if constexpr (kImages) {
+    if (block == 0) return plan_runs(a, err);
+    --block;
+  }
+  const int64_t unit = block * (256 / kLanes) + threadIdx.x / kLanes;
   if (unit >= static_cast<int64_t>(a.T) * a.hk) return;
-  int r, h, slot;
-  int64_t to;
-  if (a.row_req != nullptr) {
-    const int page = static_cast<int>(unit / (64 * a.hk)), in = static_cast<int>(unit % (64 * a.hk));
-    h = in / 64, r = page * 64 + in % 64;
-    to = unit;
+  int h, slot;
+  uint4 *k_to, *v_to;
+  if constexpr (kImages) {
+    const int tile = static_cast<int>(unit / (kKv4TileKeys * a.hk)), in = static_cast<int>(unit % (kKv4TileKeys * a.hk));
+    h = in / kKv4TileKeys;
+    const int row = in % kKv4TileKeys, r = tile * kKv4TileKeys + row;
+    k_to = static_cast<uint4*>(a.k_out) + (static_cast<int64_t>(tile) * a.hk + h) * (2 * kKv4TileKeys * kLanes) +
+           (x / 8) * (kKv4TileKeys * 8) + row * 8 + ((x ^ row) & 7);
+    v_to = k_to + kKv4TileKeys * kLanes;
     const int req = a.row_req[r];
     slot = -1;
     if (req >= 0) {
-      const int row = a.req_rows[req], pos = a.row_pos[r];
-      if (row >= 0 && row < a.pt_rows && pos < a.ld_pt) slot = a.page_table[static_cast<int64_t>(row) * a.ld_pt + pos];
+      const int table_row = a.req_rows[req], pos = a.row_pos[r];
+      if (table_row >= 0 && table_row < a.pt_rows && pos < a.ld_pt)
+        slot = a.page_table[static_cast<int64_t>(table_row) * a.ld_pt + pos];
       if (slot < 0 || slot >= a.kv_slots) {
         if (x == 0) err.report(kErrBadIndex, 955);
         slot = -1;
       }
     }
   } else {
-    r = static_cast<int>(unit / a.hk), h = static_cast<int>(unit % a.hk);
-    to = unit;
+    const int r = static_cast<int>(unit / a.hk);
+    h = static_cast<int>(unit - static_cast<int64_t>(r) * a.hk);
+    k_to = static_cast<uint4*>(a.k_out) + unit * kLanes + x;
+    v_to = static_cast<uint4*>(a.v_out) + unit * kLanes + x;
     slot = a.slots[r];
     if (slot < 0 || slot >= a.kv_slots) {
       if (x == 0) err.report(kErrBadIndex, 954);
@@ -319,8 +412,8 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadArgs a) {
   }
   uint4 k = make_uint4(0, 0, 0, 0), v = k;
   if (slot >= 0) load_row<D>(a, slot, h, x, k, v);
-  *(reinterpret_cast<uint4*>(a.k_out) + to * kLanes + x) = k;
-  *(reinterpret_cast<uint4*>(a.v_out) + to * kLanes + x) = v;
+  *k_to = k;
+  *v_to = v;
 }
 
 // ================================================================= copy ====
@@ -390,12 +483,15 @@ void launch_kv4_store(const Kv4StoreArgs& a, cudaStream_t s) {
 }
 
 void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s) {
-  if (a.T <= 0) return;
+  const bool images = a.row_req != nullptr;
+  if (a.T <= 0 && !images) return;
   if (a.d != 64 && a.d != 128) throw std::runtime_error("minisgl.load_kv4: head_dim must be 64 or 128");
   const int per_block = 256 / (a.d / 8);
-  const int64_t blocks = (static_cast<int64_t>(a.T) * a.hk + per_block - 1) / per_block;
+  const int64_t blocks = (static_cast<int64_t>(a.T) * a.hk + per_block - 1) / per_block + (images ? 1 : 0);
   if (blocks > 0x7fffffff) throw std::runtime_error("minisgl.load_kv4: too many rows");
-  auto kern = a.d == 128 ? kv4_load_kernel<128> : kv4_load_kernel<64>;
+  if (images && (a.d != 128 || a.T % kKv4TileKeys != 0))
+    throw std::runtime_error("minisgl.prefill_attention_kv4: tile images are of 128 keys and dims");
+  auto kern = images ? kv4_load_kernel<128, true> : a.d == 128 ? kv4_load_kernel<128, false> : kv4_load_kernel<64, false>;
   launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
 }
 

@@ -34,4 +34,11 @@ __device__ __forceinline__ int v_chunk(int a, int x) { return x ^ (2 * (a & 3));
 __device__ __forceinline__ float scale_f32(uint32_t byte) { return __uint_as_float((byte << 20) + kScaleF32); }
 
 }  // namespace kv4
+
+// Query tokens of request b; offsets outside q make none.
+__device__ __forceinline__ int kv4_query_tokens(const int32_t* cu_q, int b, int T) {
+  const int from = cu_q[b], to = cu_q[b + 1];
+  return from >= 0 && to <= T && to > from ? to - from : 0;
+}
+
 }  // namespace minisgl

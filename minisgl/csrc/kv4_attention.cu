@@ -108,7 +108,7 @@ constexpr int group_bytes() { return (kStages * stage_bytes<D>() + kWarps * kRow
 // Query rows (tokens x heads of a group) and keys of a request.
 template <bool kSingle>
 __device__ __forceinline__ int rows_of(const Kv4AttnArgs& a, int b) {
-  return (kSingle ? 1 : max(0, a.cu_q[b + 1] - a.cu_q[b])) * a.group;
+  return kSingle ? a.group : kv4_query_tokens(a.cu_q, b, a.T) * a.group;
 }
 __device__ __forceinline__ int keys_of(const Kv4AttnArgs& a, int b) { return min(max(a.seq_lens[b], 0), a.ld_pt); }
 __device__ __forceinline__ int key_tiles(int keys) { return max(1, (keys + kTile - 1) / kTile); }
@@ -123,12 +123,19 @@ struct Piece {
 __device__ __forceinline__ void group_sync(int group) {
   asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kWarps * 32) : "memory");
 }
-// A wait whose first try mostly succeeds; the bounded loop is kept out of line.
+// A wait that sleeps: the first try may suspend the thread for 20 us, so that it
+// leaves the issue slots to the others; the bounded loop is kept out of line.
 __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* flag, int where) {
   return mbar_wait(bar, parity, ErrorSink{flag}, where);
 }
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* flag, int where) {
-  return mbar_try_wait(bar, parity) || wait_slow(bar, parity, flag, where);
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0 || wait_slow(bar, parity, flag, where);
 }
 
 // kSingle: one query token per request (row r of a KV head is its head r).
@@ -166,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
     const int keys = keys_of(a, b);
     len[b] = keys;
     pre[b + 1] = key_tiles(keys) * ((rows_of<kSingle>(a, b) + kRows - 1) / kRows) * a.hk;
+    if (!kSingle && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.T) && blockIdx.x == 0) err.report(kErrBadIndex, 964);
   }
   __syncthreads();
   if (threadIdx.x < 32) {

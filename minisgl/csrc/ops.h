@@ -228,7 +228,7 @@ void launch_kv4_store(const Kv4StoreArgs& a, cudaStream_t s);
 struct Kv4LoadArgs {
   const uint8_t *k_pool, *v_pool;  // this layer's
   const int32_t* slots;      // [T], or (row_req set) nullptr
-  void *k_out, *v_out;       // [T, hk, d] bf16, or a layer's [T / 64, hk, 64, d]
+  void *k_out, *v_out;       // [T, hk, d] bf16, or (row_req set) k_out: images of the rows, 128 a tile
   int T, hk, d, page_size, page_shift;
   int64_t kv_slots;
   // rows of a prefill plan: key row_pos[r] of request row_req[r] (-1: zeros)
@@ -236,6 +236,12 @@ struct Kv4LoadArgs {
   const int32_t* page_table;
   int ld_pt, pt_rows;
   const int32_t* req_rows;
+  // (row_req set) one more block splits the work of the attention that follows:
+  // runs [ctas, 8]: request, pair of row tiles, KV head and key tile that a CTA
+  // begins with; tiles of its run, the pair's place, all places, runs
+  int32_t* runs;
+  const int32_t *seq_lens, *cu_q, *first_tile;
+  int ld_first, q_rows, B, group, ctas;
   int* err;
 };
 void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s);
@@ -251,7 +257,7 @@ struct Kv4AttnArgs {
   const int32_t* req_rows;   // [B]
   const int32_t* seq_lens;   // [B]
   const int32_t* cu_q;       // [B + 1], or nullptr: one token per request
-  int B, hq, hk, group, d, page_size, page_shift;  // group = hq / hk
+  int T, B, hq, hk, group, d, page_size, page_shift;  // group = hq / hk
   int pow2;                  // largest power of two <= B
   float scale;
   int runs;                  // parts that the work is split into
@@ -262,6 +268,30 @@ struct Kv4AttnArgs {
 };
 int kv4_attn_runs(int sms);
 void launch_kv4_attention(const Kv4AttnArgs& a, cudaStream_t s);
+// Many query rows over expanded keys: images [R / 128, hk, (K, V), 2 halves, 128
+// rows, 128 bytes] as launch_kv4_load writes them for a plan.
+constexpr int kKv4TileKeys = 128;
+constexpr int kKv4PairCost = 2;  // what a pair costs beside its tiles, in tiles
+struct Kv4PrefillArgs {
+  const void* q;             // [T, >= hq * 128] bf16
+  int ld_q;
+  void* out;                 // [T, hq * 128] bf16
+  const void* images;
+  const int32_t* first_tile; // [B] (stride ld_first): first row of each request's tiles
+  int ld_first, tiles;       // tiles in images
+  const int32_t* seq_lens;   // [B]
+  const int32_t* cu_q;       // [B + 1]
+  int T, B, hq, hk, group;
+  float scale;
+  int ctas;                  // grid
+  const int32_t* runs;       // [ctas, 8] (Kv4LoadArgs)
+  float* part_o;             // [ctas, 2, 256, 128] records of partial pieces
+  float* part_ml;            // [ctas, 2, 256, 2]
+  int32_t* desc;             // [ctas, 4]
+  int* err;
+};
+bool kv4_prefill_takes(int d, int group);
+void launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t s);
 // Pages src[i] -> dst[i] of every plane of a pool; returns the launches made.
 struct CopyPagesArgs {
   void* pool;

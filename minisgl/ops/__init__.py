@@ -907,12 +907,14 @@ def decode_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pag
 class KV4PrefillPlan(MlaPrefillPlan):
     """Host-built layout of a batch's keys (its requests' key counts) for
     ``prefill_attention_kv4`` over many query rows, which expands them once to
-    a compact bf16 pool. Built once per batch; used by every layer."""
+    bf16 tiles of 128 keys. Built once per batch; used by every layer."""
+
+    PAGE = 128
 
 
 # query rows (tokens x heads of a group) of a request up to which the few-row
 # kernel, which expands codes for 8 rows at a time in registers, reads the
-# cache itself; beyond, keys are expanded once and the tcgen05 kernel takes over
+# cache itself; beyond, keys are expanded once and a tcgen05 kernel takes over
 KV4_FEW_ROWS = 128
 
 
@@ -927,8 +929,8 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
     Up to KV4_FEW_ROWS query rows per KV head (drafted tokens, short extends),
     and for heads of other than 128 dims, the decode kernel reads the codes.
     More rows: the keys (``plan``: their layout, made from seq_lens if None,
-    which waits for the GPU) are expanded to a bf16 pool and go through
-    ``prefill_attention``; the expansion is exact."""
+    which waits for the GPU) are expanded to bf16 tiles, exactly, for a kernel
+    on the tensor cores."""
     if not kv_pool.is_cuda:
         return _attention_kv4_cpu("prefill_attention_kv4", q, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq,
                                   hk, d, page_size, scale, out)
@@ -937,17 +939,11 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
         _count(2)
         return native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, max_q, hq, hk, d,
                                       page_size, scale, err)
-    if out is None:
-        out = torch.empty(q.shape[0], hq * d, dtype=q.dtype, device=q.device)
     if plan is None:
         plan = KV4PrefillPlan(seq_lens.tolist(), kv_pool.device)
-    if plan.rows == 0:  # no request has a key
-        return out.zero_()
-    pool = torch.empty(2, 1, plan.rows // plan.PAGE, hk, plan.PAGE, d, dtype=q.dtype, device=q.device)
-    _count()
-    native().kv4_expand(kv_pool, layer, page_table, req_rows, plan.row_req, plan.row_pos, pool, hk, d, page_size, err)
-    return prefill_attention(q, pool, 0, plan.page_table, plan.rows_in_order, seq_lens, cu_q, max_q, hq, hk, d,
-                             plan.PAGE, scale, out=out)
+    _count(3)
+    return native().kv4_prefill(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq, hk, d, page_size,
+                                scale, plan.page_table, plan.row_req, plan.row_pos, err)
 
 
 def copy_pages(pool: torch.Tensor, src, dst, page_dim: int = 2) -> torch.Tensor:

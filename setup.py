@@ -43,6 +43,7 @@ SOURCES = [
     "minisgl/csrc/int4_gemm.cu",
     "minisgl/csrc/kv4.cu",
     "minisgl/csrc/kv4_attention.cu",
+    "minisgl/csrc/kv4_prefill.cu",
 ]
 
 

@@ -66,7 +66,7 @@ def attention(q, packed, sf, layer, table, rows, lens, queries, hq, hk, scale):
     for row, n, m in zip(rows.tolist(), lens, queries):
         at = table[row, :n].long()
         k, v, s = (x[at // page, :, at % page] for x in (k_all, v_all, s_all))  # [n, hk, .]
-        qb = q[first:first + m].reshape(m, hk, G, -1)
+        qb = q[first:first + m].reshape(m, hk, G, q.shape[-1])
         first += m
         o = torch.zeros(m, hk, G, q.shape[-1], dtype=torch.float64)
         e = torch.zeros_like(o)
@@ -81,8 +81,8 @@ def attention(q, packed, sf, layer, table, rows, lens, queries, hq, hk, scale):
             reach = torch.einsum("hgx,lhx->hgl", qb[i].abs().reshape(hk, G, -1, 32).sum(-1), s[:seen])
             es = (reach * 144 * scale * (2 * 17 * 2.0 ** -23 + 4 * 2.0 ** -24)).amax(-1, keepdim=True)
             e[i] = 2.0 ** -8 * o[i].abs() + (2.0 ** -8 + 2.0 ** -20 + 2 * es) * a
-        out.append(o.reshape(m, hq, -1))
-        bound.append(e.reshape(m, hq, -1))
+        out.append(o.reshape(m, hq, q.shape[-1]))
+        bound.append(e.reshape(m, hq, q.shape[-1]))
     return torch.cat(out), torch.cat(bound)
 
 

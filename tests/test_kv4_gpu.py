@@ -435,3 +435,17 @@ def test_other_device_than_the_current_one():
                                    torch.tensor([300], dtype=torch.int32, device="cuda:1"), 8, 1, 128, 16, 0.1)
     want, bound = oracle.attention(q.double().view(1, 8, 128), packed, sf, 0, table, rows, [300], [1], 8, 1, 0.1)
     _check(got.view(1, 8, 128), want, bound)
+
+
+# ------------------------------------------------- many query rows: split work
+@pytest.mark.parametrize("lens,queries,hq,hk", [
+    ([1300], [200], 8, 1),                            # one request over many CTAs
+    ([900, 0, 40, 2000, 5], [300, 0, 40, 33, 5], 14, 2),   # groups of 7, requests without tokens or keys
+    ([129, 128, 127, 256], [129, 128, 1, 200], 16, 16),    # heads of their own
+    ([60] * 40, [60] * 40, 16, 4),                    # many pairs in one run
+    ([500, 3, 700], [200, 9, 130], 40, 8),            # queries before the first key
+    ([300], [300], 100, 1),                           # a group of 100 heads: tiles of one token
+])
+def test_extend_many_rows_splits(lens, queries, hq, hk):
+    got, want, bound = _attend(lens, queries, hq, hk, 128, 64, few=None)
+    _check(got, want, 2 * bound)
