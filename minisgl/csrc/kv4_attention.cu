@@ -21,9 +21,10 @@
 //   two); other tiles neither reduce over lanes nor rescale the output.
 //
 // Work is split evenly whatever the lengths are: all key tiles of all requests,
-// heads and row tiles form one sequence, of which each CTA takes an equal run.
-// A run's first and last pieces may be parts of a longer one: those write
-// (m, l, O) records, which a second small kernel joins.
+// heads and row tiles form one sequence, with a place more for each unit of them
+// (what a piece costs beside its tiles), of which each group of warps takes an
+// equal run. A run's first and last pieces may be parts of a longer one: those
+// write (m, l, O) records, which a second small kernel joins.
 #include <stdexcept>
 
 #include "kv4.cuh"
@@ -40,8 +41,12 @@ constexpr int kWarps = 4;                          // each takes 32 keys of a ti
 constexpr int kTile = 32 * kWarps;                 // keys per tile
 constexpr int kRows = 8;                           // query rows per tile
 constexpr int kGroups = 3;                         // of kWarps warps in a CTA, one CTA per SM
-constexpr int kThreads = kGroups * (kWarps + 1) * 32;  // each group has a warp that fetches
+constexpr int kThreads = (kGroups + 1) * kWarps * 32;  // and a warp that fetches for each of them
 constexpr int kStages = 3;
+// registers: 16 warps are launched with 128; the last four, of which three fetch,
+// give up theirs to the others
+constexpr int kRegs = 152, kFetchRegs = 56;
+static_assert(kGroups == 3 && kWarps == 4 && 12 * kRegs + 4 * kFetchRegs == 16 * 128, "register split");
 constexpr float kFloor = -1e30f;                   // maximum of a row that has seen no key
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -103,7 +108,9 @@ constexpr int stage_bytes() { return 2 * half_bytes<D>() + kRows * q_pitch<D>();
 constexpr int kLd = 64 + 4;  // padded row of the merge buffer (floats): 64 dims at a time
 
 template <int D>
-constexpr int group_bytes() { return (kStages * stage_bytes<D>() + kWarps * kRows * (kLd + 2) * 4 + 2 * kStages * 8 + 127) / 128 * 128; }
+constexpr int group_bytes() {
+  return (kStages * stage_bytes<D>() + kWarps * kRows * (kLd + 2) * 4 + 16 * D + D + 2 * kStages * 8 + 127) / 128 * 128;
+}
 
 // Query rows (tokens x heads of a group) and keys of a request.
 template <bool kSingle>
@@ -113,19 +120,19 @@ __device__ __forceinline__ int rows_of(const Kv4AttnArgs& a, int b) {
 __device__ __forceinline__ int keys_of(const Kv4AttnArgs& a, int b) { return min(max(a.seq_lens[b], 0), a.ld_pt); }
 __device__ __forceinline__ int key_tiles(int keys) { return max(1, (keys + kTile - 1) / kTile); }
 
-// One piece of a CTA's run: key tiles [kt0, kt1) of kts of a request, KV head
-// and tile of query rows.
-struct Piece {
-  int b, h, rt;
-  int kt0, kt1, kts;
+constexpr int kUnitCost = 1;  // what a unit (request, KV head, tile of query rows) costs beside its key tiles, in tiles
+
+// A place in the work: request, unit of it (KV head x row tile) and key tile.
+struct Place {
+  int b, unit, kt;
 };
 
 __device__ __forceinline__ void group_sync(int group) {
   asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kWarps * 32) : "memory");
 }
 // A wait that sleeps: the first try may suspend the thread for 20 us, so that it
-// leaves the issue slots to the others; the bounded loop is kept out of line.
-__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* flag, int where) {
+// leaves the issue slots to the others. The bounded loop follows.
+__device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* flag, int where) {
   return mbar_wait(bar, parity, ErrorSink{flag}, where);
 }
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* flag, int where) {
@@ -150,18 +157,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
   const ErrorSink err{a.err};
   const int warp = (threadIdx.x >> 5) % kWarps, lane = threadIdx.x & 31;
   const bool fetches = threadIdx.x >= kGroups * kWarps * 32;
-  const int group = fetches ? (threadIdx.x >> 5) - kGroups * kWarps : (threadIdx.x >> 5) / kWarps;
+  const int group = fetches ? min((static_cast<int>(threadIdx.x) >> 5) - kGroups * kWarps, kGroups - 1) : (threadIdx.x >> 5) / kWarps;
+  const bool idle = threadIdx.x >= kGroups * (kWarps + 1) * 32;
   uint8_t* ring = smem + group * group_bytes<D>();
   float* so = reinterpret_cast<float*>(ring + kStages * kStage);  // [warps][rows][kLd]
   float* sm = so + kWarps * kRows * kLd;                          // [warps][rows]
   float* sl = sm + kWarps * kRows;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sl + kWarps * kRows);
+  uint4* sq = reinterpret_cast<uint4*>(sl + kWarps * kRows);  // [kNG][32 lanes] query fragments of the piece
+  float* ssum = reinterpret_cast<float*>(sq + kNG * 32);        // [kNG][rows] -8 times their groups' sums
+  uint64_t* full = reinterpret_cast<uint64_t*>(ssum + kNG * kRows);
   uint64_t* empty = full + kStages;
-  int* pre = reinterpret_cast<int*>(smem + kGroups * group_bytes<D>());  // [B + 1] sums of tiles
-  int* len = pre + a.B + 1;                                              // [B] keys
+  int* pre = reinterpret_cast<int*>(smem + kGroups * group_bytes<D>());  // [B + 1] sums of places
+  int* units = pre + a.B + 1;                                            // [B + 1] sums of units
+  int* len = units + a.B + 1;                                            // [B] keys
+  int* pt_row = len + a.B;                                               // [B] page-table rows (-1: outside)
 
   pdl_launch_dependents();
-  if (fetches && lane == 0) {
+  if (fetches && !idle && lane == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], kWarps);
@@ -172,67 +184,83 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
   for (int b = threadIdx.x; b < a.B; b += kThreads) {
     const int keys = keys_of(a, b);
     len[b] = keys;
-    pre[b + 1] = key_tiles(keys) * ((rows_of<kSingle>(a, b) + kRows - 1) / kRows) * a.hk;
+    const int row = a.req_rows[b];
+    const bool row_ok = row >= 0 && row < a.pt_rows;
+    pt_row[b] = row_ok ? row : -1;
+    if (blockIdx.x == 0 && (!row_ok || a.seq_lens[b] > a.ld_pt)) err.report(kErrBadIndex, row_ok ? 962 : 961);
+    const int n = (rows_of<kSingle>(a, b) + kRows - 1) / kRows * a.hk;
+    units[b + 1] = n, pre[b + 1] = n * (kUnitCost + key_tiles(keys));
     if (!kSingle && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.T) && blockIdx.x == 0) err.report(kErrBadIndex, 964);
   }
   __syncthreads();
-  if (threadIdx.x < 32) {
+  if (threadIdx.x < 64) {
+    int* x = threadIdx.x < 32 ? pre : units;
     int carry = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
-      int v = b0 + lane < a.B ? pre[b0 + lane + 1] : 0;
+      int v = b0 + lane < a.B ? x[b0 + lane + 1] : 0;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
       }
-      if (b0 + lane < a.B) pre[b0 + lane + 1] = carry + v;
+      if (b0 + lane < a.B) x[b0 + lane + 1] = carry + v;
       carry += __shfl_sync(0xffffffffu, v, 31);
     }
-    if (lane == 0) pre[0] = 0;
+    if (lane == 0) x[0] = 0;
   }
   __syncthreads();
   // equal runs for the groups of all CTAs (CTA by CTA in the last place, so that
-  // few runs use every SM); none is empty among the first n, so the records of a
-  // chain of pieces are all written
+  // few runs use every SM). Each has a place at least, so the runs that a unit's
+  // tiles span all have some of them, and their records are all written.
   const int64_t total = pre[a.B];
   const int n = min(kGroups * static_cast<int>(gridDim.x), pre[a.B]), me = group * gridDim.x + blockIdx.x;
-  const int first = me < n ? static_cast<int>(total * me / n) : 0;
-  const int count = me < n ? static_cast<int>(total * (me + 1) / n) - first : 0;
-  int b_at = 0;  // the request of tile `first`: the last b with pre[b] <= first
-  for (int step = a.pow2; step > 0; step /= 2)
-    if (b_at + step < a.B && pre[b_at + step] <= first) b_at += step;
+  auto find = [&](int v, Place& p) {  // the place and how many tiles are before it
+    if (v >= total) return pre[a.B] - kUnitCost * units[a.B];
+    p.b = 0;  // the last request with pre[b] <= v
+    for (int step = a.pow2; step > 0; step /= 2)
+      if (p.b + step < a.B && pre[p.b + step] <= v) p.b += step;
+    const int per = kUnitCost + key_tiles(len[p.b]), in = v - pre[p.b];
+    p.unit = in / per;
+    p.kt = max(0, in - p.unit * per - kUnitCost);
+    return pre[p.b] - kUnitCost * units[p.b] + p.unit * (per - kUnitCost) + p.kt;
+  };
+  Place at{0, 0, 0};
+  int count = 0;  // tiles of this run
+  if (me < n) {
+    Place end;
+    count = find(static_cast<int>(total * (me + 1) / n), end);
+    count -= find(static_cast<int>(total * me / n), at);
+  }
 
   const int seg = min(a.page_size, kTile);  // keys that are side by side in the cache
   const int segs = kTile / seg;
   const int seg_bytes = seg * kv4::row_bytes(D);
 
   if (fetches) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFetchRegs));
+    if (idle) return;
     // ---- tiles of the run into the ring, page numbers read a tile ahead
     if (lane == 0) reinterpret_cast<int4*>(a.desc)[me] = make_int4(-1, 0, 0, 0);
-    int b = b_at, kt = 0, kts = 0, unit = 0, keys = 0, rows = 0, tile_rows = 1, h = 0;
+    int b = at.b, kt = at.kt, kts = 0, unit = at.unit, left = 0, keys = 0, rows = 0, tile_rows = 1, h = 0;
     const int32_t* pt = a.page_table;
     bool row_ok = true;
-    auto begin = [&](int at) {  // the request and unit of tile `at`
-      while (pre[b + 1] <= at) ++b;
+    auto begin = [&] {  // request b
       keys = len[b], kts = key_tiles(keys);
       rows = rows_of<kSingle>(a, b);
       tile_rows = (rows + kRows - 1) / kRows;
-      unit = (at - pre[b]) / kts;
-      kt = at - pre[b] - unit * kts;
-      h = tile_rows == 1 ? unit : unit / tile_rows;
-      const int row = a.req_rows[b];
-      row_ok = row >= 0 && row < a.pt_rows;
-      pt = a.page_table + static_cast<int64_t>(row_ok ? row : 0) * a.ld_pt;
-      if (lane == 0 && (!row_ok || a.seq_lens[b] > a.ld_pt)) err.report(kErrBadIndex, row_ok ? 962 : 961);
+      left = units[b + 1] - units[b];
+      const int row = pt_row[b];
+      row_ok = row >= 0;
+      pt = a.page_table + static_cast<int64_t>(max(row, 0)) * a.ld_pt;
     };
     auto page_of = [&] { return lane < segs && kt * kTile + lane * seg < keys && row_ok ? pt[kt * kTile + lane * seg] : -1; };
     int slot = -1, issued = -1;
-    if (count > 0) begin(first), slot = page_of();
+    if (count > 0) begin(), h = unit / tile_rows, slot = page_of();
     for (int j = 0; j < count; ++j) {
       // this tile's copies, from what was looked up
       const bool wanted = lane < segs && kt * kTile + lane * seg < keys && row_ok;
       const bool good = wanted && slot >= 0 && slot < a.kv_slots;
-      const int64_t at = (static_cast<int64_t>(slot >> a.page_shift) * a.hk + h) * a.page_size * kv4::row_bytes(D);
+      const int64_t block = (static_cast<int64_t>(slot >> a.page_shift) * a.hk + h) * a.page_size * kv4::row_bytes(D);
       const int off = slot & (a.page_size - 1) & ~(kTile - 1);
       const bf16* q = nullptr;
       if (kt == 0 || j == 0) {  // the piece's query rows
@@ -244,7 +272,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
         }
       }
       // the next tile's page numbers
-      if (++kt == kts && j + 1 < count) begin(first + j + 1);
+      if (++kt == kts && j + 1 < count) {
+        kt = 0;
+        if (++unit == left) {
+          unit = 0;
+          do ++b; while (units[b + 1] == units[b]);  // past requests without queries: there is more to do
+          begin();
+        }
+        h = tile_rows == 1 ? unit : unit / tile_rows;
+      }
       slot = j + 1 < count ? page_of() : -1;
 
       if (wanted && !good) err.report(kErrBadIndex, 963);
@@ -258,11 +294,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
       if (good) {
         uint8_t* dst = st + lane * seg_bytes;
         if (seg == a.page_size) {
-          bulk_load(dst, a.k_pool + at, seg_bytes, &full[s]);
-          bulk_load(dst + kHalf, a.v_pool + at, seg_bytes, &full[s]);
+          bulk_load(dst, a.k_pool + block, seg_bytes, &full[s]);
+          bulk_load(dst + kHalf, a.v_pool + block, seg_bytes, &full[s]);
         } else {  // part of a larger page: its codes and its scales
-          const int64_t codes = at + off * (D / 2);
-          const int64_t scales = at + a.page_size * (D / 2) + off * kNG;
+          const int64_t codes = block + off * (D / 2);
+          const int64_t scales = block + a.page_size * (D / 2) + off * kNG;
           bulk_load(dst, a.k_pool + codes, kTile * (D / 2), &full[s]);
           bulk_load(dst + kTile * (D / 2), a.k_pool + scales, kTile * kNG, &full[s]);
           bulk_load(dst + kHalf, a.v_pool + codes, kTile * (D / 2), &full[s]);
@@ -278,6 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
     return;
   }
 
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
   const int g = lane >> 2, t = lane & 3;
   const float c = a.scale * kLog2e;
   // this lane's keys of the warp's first 16 (rows g and g + 8 of S^T are keys
@@ -295,51 +332,42 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
     v_at[u] = kHalf + seg_at + quad_in * (2 * D) + ((g ^ (2 * t)) * 16);
     vs_at[u] = kHalf + seg_at + seg * (D / 2) + (quad_in * kNG + (g >> 2)) * 4;
   }
-  int it = 0, s = 0;
+  int left = count, s = 0;
   uint32_t phase = 0;
   bool ok = true;
-  Piece p;
-  p.b = b_at;
 
-  while (it < count) {
-    // ---- the next piece
-    {
-      const int at = first + it;
-      while (pre[p.b + 1] <= at) ++p.b;
-      p.kts = key_tiles(len[p.b]);
-      const int in = at - pre[p.b];
-      const int unit = in / p.kts;
-      p.kt0 = in - unit * p.kts;
-      p.kt1 = min(p.kts, p.kt0 + count - it);
-      const int tile_rows = (rows_of<kSingle>(a, p.b) + kRows - 1) / kRows;
-      p.h = tile_rows == 1 ? unit : unit / tile_rows;
-      p.rt = unit - p.h * tile_rows;
-    }
-    const int keys = len[p.b];
-    const int rows = rows_of<kSingle>(a, p.b);
+  while (left > 0) {
+    // ---- the next piece: key tiles [kt0, kt1) of kts of the unit `at`
+    while (at.unit == units[at.b + 1] - units[at.b]) at.unit = 0, ++at.b;
+    const int keys = len[at.b], kts = key_tiles(keys);
+    const int kt0 = at.kt, kt1 = min(kts, kt0 + left);
+    const int rows = rows_of<kSingle>(a, at.b), tile_rows = (rows + kRows - 1) / kRows;
+    const int h = tile_rows == 1 ? at.unit : at.unit / tile_rows, rt = at.unit - h * tile_rows;
+    left -= kt1 - kt0;
     // keys that rows 2 t and 2 t + 1 see, and that every row of the tile sees
     int see0 = keys, see1 = keys, see_all = keys;
     if constexpr (!kSingle) {
-      const int q_len = rows / a.group, r0 = p.rt * kRows + 2 * t;
+      const int q_len = rows / a.group, r0 = rt * kRows + 2 * t;
       see0 = keys - q_len + r0 / a.group + 1;
       see1 = keys - q_len + (r0 + 1) / a.group + 1;
-      see_all = keys - q_len + p.rt * kRows / a.group + 1;
+      see_all = keys - q_len + rt * kRows / a.group + 1;
     }
-    uint32_t qb[kNG][4], off0, off1;
+    uint32_t off0, off1;
     float o[2 * kNG][4];
 #pragma unroll
     for (int i = 0; i < 2 * kNG; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = kFloor, m1 = kFloor, l0 = 0.f, l1 = 0.f, c0 = 0.f, c1 = 0.f;
 
-    for (int kt = p.kt0; kt < p.kt1; ++kt, ++it) {
+    for (int kt = kt0; kt < kt1; ++kt) {
       const uint8_t* st = ring + s * kStage;
       if (ok) ok = wait_for(&full[s], phase, a.err, 262);
-      if (kt == p.kt0) {
-        // Query fragments of row g in fp16: q 2^-x, 2^x the power of two that takes
-        // the row's largest to 2^14..2^15, which keeps the 8 bits of every element
-        // within 2^-18 of it; odd dims are divided by 16, because their codes are
-        // taken from where they stand, 4 bits up. And -8 times the groups' sums.
-        const bool live = p.rt * kRows + g < rows;
+      if (kt == kt0) {
+        // Query fragments in fp16, row g by the lanes g: q 2^-x, 2^x the power of two
+        // that takes the row's largest to 2^14..2^15, which keeps the 8 bits of every
+        // element within 2^-18 of it; odd dims are divided by 16, because their codes
+        // are taken from where they stand, 4 bits up. And -8 times the groups' sums.
+        // Warp i writes group i for all four.
+        const bool live = rt * kRows + g < rows;
         uint4 v[kNG];
         float top = 0.f;
         bool finite = true;
@@ -363,30 +391,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
         const float up = c * 16777216.f * __uint_as_float((min(ex, 254) - 14) << 23);
         c0 = __shfl_sync(0xffffffffu, up, 8 * t);      // of row 2 t
         c1 = __shfl_sync(0xffffffffu, up, 8 * t + 4);  // of row 2 t + 1
-        float sum[kNG];
+        if (warp < kNG) {
+          uint4 mine = v[0];
 #pragma unroll
-        for (int i = 0; i < kNG; ++i) {
-          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          for (int i = 1; i < kNG; ++i)
+            if (warp == i) mine = v[i];
+          const uint32_t w[4] = {mine.x, mine.y, mine.z, mine.w};
           // dims 0..7 of the word -> (0, 4), (1, 5), (2, 6), (3, 7)
-          float z[8];
-          sum[i] = 0.f;
+          float z[8], sum = 0.f;
+          uint32_t q[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             z[2 * j] = __uint_as_float(w[j] << 16) * down, z[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * down;
-            sum[i] += z[2 * j] + z[2 * j + 1];
+            sum += z[2 * j] + z[2 * j + 1];
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float f = j & 1 ? 0.0625f : 1.f;
-            const __half2 h = __floats2half2_rn(z[j] * f, z[j + 4] * f);
-            qb[i][j] = *reinterpret_cast<const uint32_t*>(&h);
+            const __half2 hh = __floats2half2_rn(z[j] * f, z[j + 4] * f);
+            q[j] = *reinterpret_cast<const uint32_t*>(&hh);
           }
-          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-          sum[i] *= -8.f / 16777216.f;  // codes are c 2^-24
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          sq[warp * 32 + lane] = make_uint4(q[0], q[1], q[2], q[3]);
+          if (t == 0) ssum[warp * kRows + g] = sum * (-8.f / 16777216.f);  // codes are c 2^-24
         }
-        // in three bf16 parts: D = 128: lanes t take groups t % 2 and t % 2 + 2
-        const float x = sum[D == 128 ? t & 1 : 0], y = sum[D == 128 ? 2 + (t & 1) : 1];
+        group_sync(group);
+        // the sums in three bf16 parts: D = 128: lanes t take groups t % 2 and t % 2 + 2
+        const float x = ssum[(D == 128 ? t & 1 : 0) * kRows + g], y = ssum[(D == 128 ? 2 + (t & 1) : 1) * kRows + g];
         const uint32_t hi = pack_bf16x2(x, y);
         const float x1 = x - __uint_as_float(hi << 16), y1 = y - __uint_as_float(hi & 0xffff0000u);
         const uint32_t mid = pack_bf16x2(x1, y1);
@@ -400,50 +432,55 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
       if (kt * kTile + warp * 32 < keys) {  // some key of the warp's is there
         // ---- S^T of 2 x 16 keys x 8 rows
         float sc[2][4];
+        uint32_t w0[2][kNG], w1[2][kNG];  // words of keys key0 and key0 + 2
+        float f0[2][kNG], f1[2][kNG];     // and their scales
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          uint32_t w0[kNG], w1[kNG], s0, s1;  // words and scale bytes of keys key0 and key0 + 2
+          uint32_t s0, s1;
           if constexpr (D == 128) {
-            *reinterpret_cast<uint4*>(w0) = *reinterpret_cast<const uint4*>(st + k_at[u]);
-            *reinterpret_cast<uint4*>(w1) = *reinterpret_cast<const uint4*>(st + k_at[u] + D);
+            *reinterpret_cast<uint4*>(w0[u]) = *reinterpret_cast<const uint4*>(st + k_at[u]);
+            *reinterpret_cast<uint4*>(w1[u]) = *reinterpret_cast<const uint4*>(st + k_at[u] + D);
             s0 = *reinterpret_cast<const uint32_t*>(st + ks_at[u]);
             s1 = *reinterpret_cast<const uint32_t*>(st + ks_at[u] + 2 * kNG);
           } else {
-            *reinterpret_cast<uint2*>(w0) = *reinterpret_cast<const uint2*>(st + k_at[u]);
-            *reinterpret_cast<uint2*>(w1) = *reinterpret_cast<const uint2*>(st + k_at[u] + D);
+            *reinterpret_cast<uint2*>(w0[u]) = *reinterpret_cast<const uint2*>(st + k_at[u]);
+            *reinterpret_cast<uint2*>(w1[u]) = *reinterpret_cast<const uint2*>(st + k_at[u] + D);
             s0 = *reinterpret_cast<const uint16_t*>(st + ks_at[u]);
             s1 = *reinterpret_cast<const uint16_t*>(st + ks_at[u] + 2 * kNG);
           }
           // the scales as bf16 pairs (groups 0 and 2, 1 and 3; D = 64: 0 and 1)
           uint32_t e0, e1, d0, d1;
-          float f0[kNG], f1[kNG];
           if constexpr (D == 128) {
             e0 = (s0 & 0x00ff00ffu) * 16 + kv4::kScaleBf16x2, d0 = __byte_perm(s0, 0, 0x4341) * 16 + kv4::kScaleBf16x2;
             e1 = (s1 & 0x00ff00ffu) * 16 + kv4::kScaleBf16x2, d1 = __byte_perm(s1, 0, 0x4341) * 16 + kv4::kScaleBf16x2;
-            f0[0] = __uint_as_float(e0 << 16), f0[2] = __uint_as_float(e0 & 0xffff0000u);
-            f0[1] = __uint_as_float(d0 << 16), f0[3] = __uint_as_float(d0 & 0xffff0000u);
-            f1[0] = __uint_as_float(e1 << 16), f1[2] = __uint_as_float(e1 & 0xffff0000u);
-            f1[1] = __uint_as_float(d1 << 16), f1[3] = __uint_as_float(d1 & 0xffff0000u);
+            f0[u][0] = __uint_as_float(e0 << 16), f0[u][2] = __uint_as_float(e0 & 0xffff0000u);
+            f0[u][1] = __uint_as_float(d0 << 16), f0[u][3] = __uint_as_float(d0 & 0xffff0000u);
+            f1[u][0] = __uint_as_float(e1 << 16), f1[u][2] = __uint_as_float(e1 & 0xffff0000u);
+            f1[u][1] = __uint_as_float(d1 << 16), f1[u][3] = __uint_as_float(d1 & 0xffff0000u);
             if (t & 1) e0 = d0, e1 = d1;
           } else {
             e0 = __byte_perm(s0, 0, 0x4140) * 16 + kv4::kScaleBf16x2;
             e1 = __byte_perm(s1, 0, 0x4140) * 16 + kv4::kScaleBf16x2;
-            f0[0] = __uint_as_float(e0 << 16), f0[1] = __uint_as_float(e0 & 0xffff0000u);
-            f1[0] = __uint_as_float(e1 << 16), f1[1] = __uint_as_float(e1 & 0xffff0000u);
+            f0[u][0] = __uint_as_float(e0 << 16), f0[u][1] = __uint_as_float(e0 & 0xffff0000u);
+            f1[u][0] = __uint_as_float(e1 << 16), f1[u][1] = __uint_as_float(e1 & 0xffff0000u);
           }
           const uint32_t po[4] = {e0, e1, e0, e1};
           mma_bf16_zero(sc[u], po, off0, off1);
+        }
 #pragma unroll
-          for (int i = 0; i < kNG; ++i) {
+        for (int i = 0; i < kNG; ++i) {
+          const uint4 q = sq[i * 32 + lane];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
             float acc[4];
             // codes as they stand, c or 16 c, are fp16 numbers c 2^-24 and c 2^-20
-            const uint32_t x[4] = {w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u};
-            mma_f16_zero(acc, x, qb[i][0], qb[i][1]);
-            const uint32_t z0 = w0[i] >> 8, z1 = w1[i] >> 8;
+            const uint32_t x[4] = {w0[u][i] & 0x000f000fu, w1[u][i] & 0x000f000fu, w0[u][i] & 0x00f000f0u, w1[u][i] & 0x00f000f0u};
+            mma_f16_zero(acc, x, q.x, q.y);
+            const uint32_t z0 = w0[u][i] >> 8, z1 = w1[u][i] >> 8;
             const uint32_t y[4] = {z0 & 0x000f000fu, z1 & 0x000f000fu, z0 & 0x00f000f0u, z1 & 0x00f000f0u};
-            mma_f16(acc, y, qb[i][2], qb[i][3]);
-            sc[u][0] += acc[0] * f0[i], sc[u][1] += acc[1] * f0[i];
-            sc[u][2] += acc[2] * f1[i], sc[u][3] += acc[3] * f1[i];
+            mma_f16(acc, y, q.z, q.w);
+            sc[u][0] += acc[0] * f0[u][i], sc[u][1] += acc[1] * f0[u][i];
+            sc[u][2] += acc[2] * f1[u][i], sc[u][3] += acc[3] * f1[u][i];
           }
         }
         if ((kt + 1) * kTile > see_all) {  // uniform over the CTA
@@ -512,9 +549,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
       l1 += __shfl_xor_sync(0xffffffffu, l1, sh);
     }
     const int jr = 2 * warp + lane / 16, jd = lane % 16 * 4;
-    const int r = p.rt * kRows + jr;
-    const bool whole = p.kt0 == 0 && p.kt1 == p.kts;
-    const int rec = (2 * me + (p.kt0 == 0 ? 1 : 0)) * kRows + jr;
+    const int r = rt * kRows + jr;
+    const bool whole = kt0 == 0 && kt1 == kts;
+    const int rec = (2 * me + (kt0 == 0 ? 1 : 0)) * kRows + jr;
     float f[kWarps], inv = 0.f;
 #pragma unroll
     for (int hf = 0; hf < kHalves; ++hf) {
@@ -558,44 +595,39 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
       } else if (r < rows) {
         const int tok = kSingle ? 0 : r / a.group;
         bf16* dst = static_cast<bf16*>(a.out) +
-                    (static_cast<int64_t>((kSingle ? p.b : a.cu_q[p.b]) + tok) * a.hq + p.h * a.group + r - tok * a.group) * D;
+                    (static_cast<int64_t>((kSingle ? at.b : a.cu_q[at.b]) + tok) * a.hq + h * a.group + r - tok * a.group) * D;
         *reinterpret_cast<uint2*>(dst + 64 * hf + jd) =
             make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
       }
     }
-    if (!whole && p.kt0 == 0 && warp == 0 && lane == 0) {
-      // the CTA whose run holds the piece's last tile
-      const int64_t last = static_cast<int64_t>(first) + it - 1 + p.kts - p.kt1;
-      reinterpret_cast<int4*>(a.desc)[me] = make_int4(static_cast<int>(((last + 1) * n - 1) / total), p.b, p.h, p.rt);
+    if (!whole && kt0 == 0 && warp == 0 && lane == 0) {
+      // the run that has the unit's last tile
+      const int64_t last = pre[at.b] + static_cast<int64_t>(at.unit + 1) * (kUnitCost + kts);
+      reinterpret_cast<int4*>(a.desc)[me] = make_int4(static_cast<int>((last * n - 1) / total), at.b, h, rt);
     }
+    at.kt = 0, ++at.unit;  // if this was not its end, the run is over
   }
 }
 
-// Joins the records of the piece that run blockIdx.x began and others went on
-// with: row blockIdx.y, records i modulo 8 of the chain in warp i.
+// Joins the records of the unit that run blockIdx.x began and others went on
+// with. Warp w: row w % 8, records w / 8 modulo 4 of the chain.
 template <int D, bool kSingle>
-__global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(1024) kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kE = D / 32;
-  __shared__ float so[8][D], sl[8], sm[8];
+  __shared__ float so[3][kRows][D], sl[3][kRows];
   const int4 d = reinterpret_cast<const int4*>(a.desc)[blockIdx.x];
   if (d.x < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.y, begin = blockIdx.x, count = d.x - begin + 1;
-  const int G = a.group, r = d.w * kRows + row;
-  if (r >= rows_of<kSingle>(a, d.y)) return;
+  const int row = warp % kRows, part = warp / kRows, begin = blockIdx.x, count = d.x - begin + 1;
   auto rec_of = [&](int i) { return (2 * (begin + i) + (i == 0 ? 1 : 0)) * kRows + row; };
   float top = kFloor;
-  for (int i = threadIdx.x; i < count; i += 256) top = fmaxf(top, a.part_ml[2 * rec_of(i)]);
+  for (int i = lane; i < count; i += 32) top = fmaxf(top, a.part_ml[2 * rec_of(i)]);
   top = warp_max(top);
-  if (lane == 0) sm[warp] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, sm[w]);
   float l = 0.f, acc[kE] = {};
-#pragma unroll 4
-  for (int i = warp; i < count; i += 8) {
+#pragma unroll 8
+  for (int i = part; i < count; i += 4) {
     const int rec = rec_of(i);
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * rec);
     const float f = exp2_approx(ml.x - top);
@@ -604,24 +636,32 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
 #pragma unroll
     for (int k = 0; k < kE; ++k) acc[k] += v[k] * f;
   }
+  if (part > 0) {
 #pragma unroll
-  for (int k = 0; k < kE; ++k) so[warp][lane * kE + k] = acc[k];
-  if (lane == 0) sl[warp] = l;
+    for (int k = 0; k < kE; ++k) so[part - 1][row][lane * kE + k] = acc[k];
+    if (lane == 0) sl[part - 1][row] = l;
+  }
   __syncthreads();
-  if (threadIdx.x >= D / 2) return;
-  l = 0.f;
-  float x = 0.f, y = 0.f;
+  const int G = a.group, r = d.w * kRows + row;
+  if (part > 0 || r >= rows_of<kSingle>(a, d.y)) return;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) l += sl[w], x += so[w][2 * threadIdx.x], y += so[w][2 * threadIdx.x + 1];
+  for (int i = 0; i < 3; ++i) {
+    l += sl[i][row];
+#pragma unroll
+    for (int k = 0; k < kE; ++k) acc[k] += so[i][row][lane * kE + k];
+  }
   const float inv = l > 0.f ? 1.f / l : l;
-  const int q0 = kSingle ? d.y : a.cu_q[d.y];
-  reinterpret_cast<uint32_t*>(static_cast<bf16*>(a.out) + (static_cast<int64_t>(q0 + r / G) * a.hq + d.z * G + r % G) * D)[threadIdx.x] =
-      pack_bf16x2(x * inv, y * inv);
+  const int tok = kSingle ? 0 : r / G;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(
+      static_cast<bf16*>(a.out) +
+      (static_cast<int64_t>((kSingle ? d.y : a.cu_q[d.y]) + tok) * a.hq + d.z * G + r - tok * G) * D + lane * kE);
+#pragma unroll
+  for (int k = 0; k < kE / 2; ++k) dst[k] = pack_bf16x2(acc[2 * k] * inv, acc[2 * k + 1] * inv);
 }
 
 template <int D>
 int attn_smem(int B) {
-  return kGroups * group_bytes<D>() + (2 * B + 1) * 4;
+  return kGroups * group_bytes<D>() + (4 * B + 2) * 4;
 }
 
 template <int D, bool kSingle>
@@ -636,7 +676,7 @@ void launch_typed(const Kv4AttnArgs& a, cudaStream_t s) {
     done[dev & 63] = true;
   }
   launch_pdl(kv4_attn_kernel<D, kSingle>, dim3(a.runs / kGroups), dim3(kThreads), attn_smem<D>(a.B), s, a);
-  launch_pdl(kv4_join_kernel<D, kSingle>, dim3(a.runs, kRows), dim3(256), 0, s, a);
+  launch_pdl(kv4_join_kernel<D, kSingle>, dim3(a.runs), dim3(1024), 0, s, a);
 }
 
 }  // namespace

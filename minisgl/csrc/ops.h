@@ -245,7 +245,7 @@ struct Kv4LoadArgs {
   int* err;
 };
 void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s);
-constexpr int kKv4MaxBatch = 3584;  // requests of one attention call (their tile sums sit in shared memory)
+constexpr int kKv4MaxBatch = 1280;  // requests of one attention call (their tile sums sit in shared memory)
 struct Kv4AttnArgs {
   const void* q;             // [T, >= hq * d] bf16
   int ld_q;
