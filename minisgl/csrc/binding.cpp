@@ -4,6 +4,7 @@
 // tensor arguments on the host (the role of the reference's TensorMatcher,
 // python/minisgl/kernel/csrc/include/minisgl/tensor.h) and then calls the
 // plain launchers declared in ops.h on the current CUDA stream.
+#include <algorithm>
 #include <cstring>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -1729,15 +1730,51 @@ at::Tensor kv4_attention(const at::Tensor& q, const c10::optional<at::Tensor>& d
   return out;
 }
 
-// Pages src[i] -> dst[i] of every plane before `page_dim` of a pool.
-int64_t copy_pages(at::Tensor pool, const std::vector<int64_t>& src, const std::vector<int64_t>& dst, int64_t page_dim) {
+// Page numbers from a host tensor or a sequence of integers.
+std::vector<int> page_list(const py::object& pages) {
+  std::vector<int> out;
+  auto push = [&](int64_t v) {
+    if (v < 0 || v > 0x7fffffff) throw py::index_error("copy_pages: a page is outside the pool");
+    out.push_back(static_cast<int>(v));
+  };
+  if (THPVariable_Check(pages.ptr())) {
+    const at::Tensor& t = THPVariable_Unpack(pages.ptr());
+    if (t.is_cuda() || !at::isIntegralType(t.scalar_type(), false))
+      throw py::value_error("copy_pages: page numbers are host integers (a CPU tensor or ints)");
+    const at::Tensor c = t.to(at::kLong).reshape({-1}).contiguous();
+    for (int64_t i = 0; i < c.numel(); ++i) push(c.data_ptr<int64_t>()[i]);
+  } else {
+    for (const py::handle& p : py::iter(pages)) {
+      const int64_t v = PyLong_AsLongLong(p.ptr());
+      if (v == -1 && PyErr_Occurred()) throw py::error_already_set();
+      push(v);
+    }
+  }
+  return out;
+}
+// Pages src[i] -> dst[i] of every plane before `page_dim` of a pool; refuses pairs
+// whose copies could see one another.
+int64_t copy_pages(at::Tensor pool, const py::object& src, const py::object& dst, int64_t page_dim) {
+  if (page_dim < 0 || page_dim >= pool.dim()) throw py::value_error("copy_pages: the pool has no such page dimension");
   check_cuda(pool, "pool");
-  MSG_CHECK(pool.is_contiguous() && page_dim >= 0 && page_dim < pool.dim(), "copy_pages: pool must be contiguous with a page "
-            "dimension, got ", pool.sizes(), " and page_dim ", page_dim);
+  MSG_CHECK(pool.is_contiguous(), "copy_pages: pool must be contiguous");
+  std::vector<int> s = page_list(src), d = page_list(dst);
+  if (s.size() != d.size()) throw py::value_error("copy_pages: as many source as destination pages are needed");
   const int64_t pages = pool.size(page_dim);
-  std::vector<int> s, d;
-  for (size_t i = 0; i < src.size(); ++i)
-    if (src[i] != dst[i]) s.push_back(static_cast<int>(src[i])), d.push_back(static_cast<int>(dst[i]));
+  for (size_t i = 0; i < s.size(); ++i)
+    if (s[i] >= pages || d[i] >= pages) throw py::index_error("copy_pages: a page is outside the pool");
+  std::vector<int> to = d;
+  std::sort(to.begin(), to.end());
+  if (std::adjacent_find(to.begin(), to.end()) != to.end())
+    throw py::value_error("copy_pages: a page is the destination of two copies");
+  size_t n = 0;
+  for (size_t i = 0; i < s.size(); ++i) {
+    if (s[i] == d[i]) continue;
+    if (std::binary_search(to.begin(), to.end(), s[i]))
+      throw py::value_error("copy_pages: a page is both a source and the destination of another copy");
+    s[n] = s[i], d[n++] = d[i];
+  }
+  s.resize(n), d.resize(n);
   if (s.empty() || pool.numel() == 0) return 0;
   minisgl::CopyPagesArgs a{};
   a.pool = pool.data_ptr();

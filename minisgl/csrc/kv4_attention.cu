@@ -212,8 +212,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
   // equal runs for the groups of all CTAs (CTA by CTA in the last place, so that
   // few runs use every SM). Each has a place at least, so the runs that a unit's
   // tiles span all have some of them, and their records are all written.
-  const int64_t total = pre[a.B];
-  const int n = min(kGroups * static_cast<int>(gridDim.x), pre[a.B]), me = group * gridDim.x + blockIdx.x;
+  const int total = pre[a.B];
+  const int n = max(1, min(kGroups * static_cast<int>(gridDim.x), total)), me = group * gridDim.x + blockIdx.x;
+  const int each = total / n, more = total - each * n;  // places of a run; the runs share `more` others
+  auto start_of = [&](int i) { return each * i + more * i / n; };  // of run i: total i / n without 64 bits
   auto find = [&](int v, Place& p) {  // the place and how many tiles are before it
     if (v >= total) return pre[a.B] - kUnitCost * units[a.B];
     p.b = 0;  // the last request with pre[b] <= v
@@ -226,10 +228,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
   };
   Place at{0, 0, 0};
   int count = 0;  // tiles of this run
-  if (me < n) {
+  if (me < n && total > 0) {
     Place end;
-    count = find(static_cast<int>(total * (me + 1) / n), end);
-    count -= find(static_cast<int>(total * me / n), at);
+    count = find(start_of(me + 1), end);
+    count -= find(start_of(me), at);
   }
 
   const int seg = min(a.page_size, kTile);  // keys that are side by side in the cache
@@ -601,9 +603,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
       }
     }
     if (!whole && kt0 == 0 && warp == 0 && lane == 0) {
-      // the run that has the unit's last tile
-      const int64_t last = pre[at.b] + static_cast<int64_t>(at.unit + 1) * (kUnitCost + kts);
-      reinterpret_cast<int4*>(a.desc)[me] = make_int4(static_cast<int>((last * n - 1) / total), at.b, h, rt);
+      // the run that has the unit's last place
+      const int last = pre[at.b] + (at.unit + 1) * (kUnitCost + kts) - 1;
+      int i = min(n - 1, static_cast<int>(static_cast<float>(last) / static_cast<float>(total) * n));
+      while (i > me && start_of(i) > last) --i;
+      while (i + 1 < n && start_of(i + 1) <= last) ++i;
+      reinterpret_cast<int4*>(a.desc)[me] = make_int4(i, at.b, h, rt);
     }
     at.kt = 0, ++at.unit;  // if this was not its end, the run is over
   }

@@ -953,6 +953,9 @@ def copy_pages(pool: torch.Tensor, src, dst, page_dim: int = 2) -> torch.Tensor:
     ``src`` and ``dst`` are host values (ints, or CPU tensors). A page may be
     copied to several; a destination is named once and is no other pair's
     source, so the order of the copies does not matter. Returns the pool."""
+    if pool.is_cuda:
+        _count(native().copy_pages(pool, src, dst, page_dim))
+        return pool
     src, dst = _page_list(src), _page_list(dst)
     if len(src) != len(dst):
         raise ValueError(f"copy_pages: {len(src)} source and {len(dst)} destination pages")
@@ -966,9 +969,7 @@ def copy_pages(pool: torch.Tensor, src, dst, page_dim: int = 2) -> torch.Tensor:
         raise ValueError("copy_pages: a page is the destination of two copies")
     if not to.isdisjoint(src) and any(s in to and s != d for s, d in zip(src, dst)):
         raise ValueError("copy_pages: a page is both a source and the destination of another copy")
-    if pool.is_cuda:
-        _count(native().copy_pages(pool, src, dst, page_dim))
-    elif src:
+    if src:
         dim = (slice(None),) * page_dim
         pool[dim + (torch.tensor(dst),)] = pool[dim + (torch.tensor(src),)]
     return pool
