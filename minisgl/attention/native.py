@@ -48,6 +48,7 @@ class NativeAttnMetadata(BaseAttnMetadata):
     max_q: int
     max_splits: int
     last_indices: Optional[torch.Tensor] = None  # int64 [B] (prefill)
+    plan: Optional[ops.KV4PrefillPlan] = None    # 4-bit pools: the keys' layout (prefill of many rows)
 
     def get_last_indices(self, bs: int) -> torch.Tensor:
         if self.last_indices is None:  # decode: one token per request
@@ -67,6 +68,7 @@ class NativeAttnBackend(BaseAttnBackend):
         self.kv = ctx.kv_cache
         self.device = self.kv.device
         self.max_batch = max_batch
+        self.kv4 = config.kv_quant == "int4"
         self._scratch_bs = 0
         self.part_o: Optional[torch.Tensor] = None
         self.part_lse: Optional[torch.Tensor] = None
@@ -76,7 +78,7 @@ class NativeAttnBackend(BaseAttnBackend):
 
     # ---------------------------------------------------------------- scratch
     def _ensure_scratch(self, bs: int) -> None:
-        if bs <= self._scratch_bs or self.device.type != "cuda":
+        if bs <= self._scratch_bs or self.device.type != "cuda" or self.kv4:
             return
         self._scratch_bs = bs
         self.part_o = torch.empty(bs * self.hq * MAX_SPLITS * self.d, dtype=torch.float32, device=self.device)
@@ -88,6 +90,12 @@ class NativeAttnBackend(BaseAttnBackend):
         assert isinstance(md, NativeAttnMetadata)
         pool = self.kv.pool
         pt = get_global_ctx().page_table
+        if self.kv4:
+            if batch.is_decode:
+                return ops.decode_attention_kv4(qkv, pool, layer_id, pt, md.req_rows, md.seq_lens, self.hq, self.hk,
+                                                self.d, self.page_size, self.scale)
+            return ops.prefill_attention_kv4(qkv, pool, layer_id, pt, md.req_rows, md.seq_lens, md.cu_q, md.max_q,
+                                             self.hq, self.hk, self.d, self.page_size, self.scale, md.plan)
         if batch.is_decode:
             return ops.decode_attention(qkv, pool, layer_id, pt, md.req_rows, md.seq_lens, self.hq, self.hk, self.d,
                                         self.page_size, self.scale, self.part_o, self.part_lse, md.max_splits)
@@ -114,9 +122,12 @@ class NativeAttnBackend(BaseAttnBackend):
         host = torch.tensor(rows + lens + cu, dtype=torch.int32, pin_memory=on_gpu)
         dev = host.to(self.device, non_blocking=True)
         cu_q = dev[2 * B :]
+        plan = None
+        if self.kv4 and on_gpu and ops.kv4_prefill_expands(max(qlens), self.hq, self.hk, self.d):
+            plan = ops.KV4PrefillPlan(lens, self.device)
         batch.attn_metadata = NativeAttnMetadata(
             req_rows=dev[:B], seq_lens=dev[B : 2 * B], cu_q=cu_q, max_q=max(qlens), max_splits=1,
-            last_indices=(cu_q[1:] - 1).long(),
+            last_indices=(cu_q[1:] - 1).long(), plan=plan,
         )
 
     # ------------------------------------------------------------ CUDA graphs

@@ -42,6 +42,7 @@ class EngineConfig:
     cp_size: int = 1                  # context parallelism (sequence split across ranks)
     enable_dp_attention: bool = False
     moe_quant: str = "none"           # "none" | "mxfp4" | "mxfp4-a8"
+    kv_quant: str = "none"            # "none" (K and V in dtype) | "int4" (minisgl.quant.kv4)
     comm: str = "fused"               # "fused" (in-kernel NVLink collectives) | "nccl" (baseline)
     weight_seed: int = 0
     dummy_weight_device: Optional[str] = None  # draw random weights here ("cpu" for bit-identical tests)
@@ -67,7 +68,7 @@ class EngineConfig:
         cfg = ModelConfig.from_hf(self.hf_config)
         # DP attention splits the routed experts over every rank
         ep = self.tp_info.size if self.enable_dp_attention else (self.ep_size if self.ep_size > 1 else 1)
-        return dataclasses.replace(cfg, moe_quant=self.moe_quant, ep_size=ep,
+        return dataclasses.replace(cfg, moe_quant=self.moe_quant, kv_quant=self.kv_quant, ep_size=ep,
                                    ep_rank=self.tp_info.rank % ep if ep > 1 else 0)
 
     @property

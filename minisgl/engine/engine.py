@@ -68,8 +68,29 @@ def _valid_page(p: int) -> bool:
     return p >= 16 and (p & (p - 1)) == 0
 
 
+def _check_kv_quant(config: EngineConfig) -> None:
+    """What a 4-bit KV cache cannot hold or serve, before anything is set up."""
+    if config.kv_quant == "none":
+        return
+    from minisgl.quant.kv4 import kv4_check
+
+    m = config.model_config
+    if config.kv_quant != "int4":
+        raise ValueError(f"kv_quant must be none or int4, got {config.kv_quant!r}")
+    if m.is_mla:
+        raise ValueError("a KV cache in 4 bits is for MHA / GQA models: an MLA latent stays in 16 bits")
+    on_cpu = config.device == "cpu"
+    kv4_check(config.page_size if on_cpu or _valid_page(config.page_size) else 64, m.head_dim)
+    if config.max_running_req >= ops.KV4_MAX_BATCH:
+        raise ValueError(f"a 4-bit KV cache serves at most {ops.KV4_MAX_BATCH - 1} running requests, not "
+                         f"{config.max_running_req}")
+    if not on_cpu and config.dtype != torch.bfloat16:
+        raise ValueError(f"a KV cache in 4 bits takes rows of bfloat16 on a GPU, got {config.dtype}")
+
+
 class Engine:
     def __init__(self, config: EngineConfig) -> None:
+        _check_kv_quant(config)
         if config.cp_size > 1:
             # context parallelism: every rank holds the model (the routed
             # experts split over the ranks with --ep cp) and the attention over
@@ -316,6 +337,10 @@ class Engine:
         from minisgl.utils import div_even
 
         kv = div_even(m.num_kv_heads, get_tp_info().size, allow_replicate=True)
+        if m.kv_quant == "int4":
+            from minisgl.quant.kv4 import kv4_block_bytes
+
+            return 2 * m.num_layers * kv * kv4_block_bytes(self.page_size, m.head_dim)
         return 2 * m.num_layers * kv * self.page_size * m.head_dim * itemsize
 
     def _sync_get_memory(self) -> Tuple[int, int]:

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 from abc import ABC, abstractmethod
 from dataclasses import dataclass
-from typing import NamedTuple
+from typing import NamedTuple, Sequence
 
 import torch
 
@@ -25,6 +25,10 @@ class BaseKVCachePool(ABC):
 
     @abstractmethod
     def store_kv(self, k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, layer: int) -> None: ...
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Copy whole pages src[i] -> dst[i] in every layer (``ops.copy_pages``)."""
+        raise NotImplementedError(f"{type(self).__name__} does not copy pages")
 
     @property
     @abstractmethod

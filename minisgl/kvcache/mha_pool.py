@@ -11,8 +11,11 @@ hold non-finite values.
 
 from __future__ import annotations
 
+from typing import Sequence
+
 import torch
 
+from minisgl import ops
 from minisgl.parallel import get_tp_info
 from minisgl.utils import div_even
 
@@ -43,6 +46,9 @@ class MHAKVCache(BaseKVCachePool):
         shape = (-1, self.local_kv_heads, self.head_dim)
         self.pool[0, layer][page, :, off] = k.reshape(shape)
         self.pool[1, layer][page, :, off] = v.reshape(shape)
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        ops.copy_pages(self.pool, src, dst)
 
     @property
     def device(self) -> torch.device:

@@ -16,7 +16,11 @@ guarantees) sits at local page g // cp.
 
 from __future__ import annotations
 
+from typing import Sequence
+
 import torch
+
+from minisgl import ops
 
 from .base import BaseKVCachePool
 
@@ -54,6 +58,10 @@ class MLAKVCache(BaseKVCachePool):
     def store_kv(self, k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, layer: int) -> None:
         """k: the full latent rows (v is the leading part of the same rows)."""
         self.store_latent(k, out_loc, layer)
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Pages of this rank's pool (local pages under context parallelism)."""
+        ops.copy_pages(self.pool, src, dst, page_dim=1)
 
     @property
     def device(self) -> torch.device:

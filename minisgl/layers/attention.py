@@ -29,7 +29,7 @@ if TYPE_CHECKING:
 class AttentionLayer(StateLessOP):
     def __init__(self, layer_id: int, num_qo_heads: int, num_kv_heads: int, head_dim: int,
                  rotary_config: "RotaryConfig", q_norm: Optional["RMSNorm"] = None,
-                 k_norm: Optional["RMSNorm"] = None, eps: float = 1e-6) -> None:
+                 k_norm: Optional["RMSNorm"] = None, eps: float = 1e-6, kv_quant: str = "none") -> None:
         assert num_qo_heads % num_kv_heads == 0
         tp = get_tp_info().size
         self.layer_id = layer_id
@@ -44,6 +44,7 @@ class AttentionLayer(StateLessOP):
         self._q_norm = q_norm
         self._k_norm = k_norm
         self.eps = q_norm.eps if q_norm is not None else eps
+        self._kv4 = kv_quant == "int4"
 
     def rope_args(self) -> dict:
         """Arguments of the fused qkv-GEMM epilogue (q/k norm, RoPE, KV store)
@@ -66,18 +67,23 @@ class AttentionLayer(StateLessOP):
 
     @property
     def fusable(self) -> bool:
-        """Whether the fused qkv epilogue can replace ``rope_store``."""
-        return self.head_dim == 128
+        """Whether the fused qkv epilogue can replace ``rope_store`` (it
+        stores rows of 16 bits only)."""
+        return self.head_dim == 128 and not self._kv4
 
     def forward(self, qkv: torch.Tensor) -> torch.Tensor:
         ctx = get_global_ctx()
         batch = ctx.batch
         kv = ctx.kv_cache
+        norms = (None if self._q_norm is None else self._q_norm.weight,
+                 None if self._k_norm is None else self._k_norm.weight)
+        if self._kv4:
+            ops.rope_store_kv4(qkv, batch.positions, self.rotary.cos_sin_cache, *norms, kv.pool, self.layer_id,
+                               batch.out_loc, self.num_qo_heads, self.num_kv_heads, self.head_dim, ctx.page_size,
+                               self.eps)
+            return ctx.attn_backend.forward(qkv, self.layer_id, batch)
         ops.rope_store(
-            qkv, batch.positions, self.rotary.cos_sin_cache,
-            None if self._q_norm is None else self._q_norm.weight,
-            None if self._k_norm is None else self._k_norm.weight,
-            kv.k_cache(self.layer_id), kv.v_cache(self.layer_id), batch.out_loc,
+            qkv, batch.positions, self.rotary.cos_sin_cache, *norms, kv.k_cache(self.layer_id), kv.v_cache(self.layer_id), batch.out_loc,
             self.num_qo_heads, self.num_kv_heads, self.head_dim, ctx.page_size, self.eps,
         )
         return ctx.attn_backend.forward(qkv, self.layer_id, batch)

@@ -12,6 +12,8 @@ from typing import Dict, List
 
 import torch
 
+from minisgl.quant import dequantize_kv4, quantize_kv4_reference
+
 from .config import ModelConfig
 
 
@@ -71,6 +73,8 @@ def dense_logits(state: Dict[str, torch.Tensor], cfg: ModelConfig, tokens: List[
             q = _rms(q, W[p + "self_attn.q_norm.weight"], eps)
             k = _rms(k, W[p + "self_attn.k_norm.weight"], eps)
         q, k = _rotate(q, cos, sin), _rotate(k, cos, sin)
+        if cfg.kv_quant == "int4":  # keys and values as a 4-bit cache holds them
+            k, v = (dequantize_kv4(*quantize_kv4_reference(t)) for t in (k, v))
         g = hq // hk
         k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
         s = torch.einsum("qhd,khd->hqk", q, k) * d ** -0.5

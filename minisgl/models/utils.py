@@ -92,7 +92,7 @@ class RopeAttn(BaseOP):
         self.q_norm = RMSNorm(d, config.rms_norm_eps) if has_qk_norm else None
         self.k_norm = RMSNorm(d, config.rms_norm_eps) if has_qk_norm else None
         self.attn = AttentionLayer(layer_id, config.num_qo_heads, config.num_kv_heads, d, config.rotary_config,
-                                   self.q_norm, self.k_norm, eps=config.rms_norm_eps)
+                                   self.q_norm, self.k_norm, eps=config.rms_norm_eps, kv_quant=config.kv_quant)
         self.o_proj = LinearOProj(d * config.num_qo_heads, config.hidden_size, has_bias=False)
 
     @nvtx_annotate("MHA")

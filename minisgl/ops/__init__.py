@@ -916,6 +916,12 @@ class KV4PrefillPlan(MlaPrefillPlan):
 # kernel, which expands codes for 8 rows at a time in registers, reads the
 # cache itself; beyond, keys are expanded once and a tcgen05 kernel takes over
 KV4_FEW_ROWS = 128
+KV4_MAX_BATCH = 1280  # requests of one attention call over a 4-bit pool
+
+
+def kv4_prefill_expands(max_q: int, hq: int, hk: int, d: int) -> bool:
+    """Whether ``prefill_attention_kv4`` expands the keys first (and so takes a plan)."""
+    return d == 128 and max_q * (hq // max(1, hk)) > KV4_FEW_ROWS
 
 
 def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, page_table: torch.Tensor,
@@ -935,7 +941,7 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
         return _attention_kv4_cpu("prefill_attention_kv4", q, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq,
                                   hk, d, page_size, scale, out)
     err = error_word(kv_pool.device)
-    if d != 128 or max_q * (hq // max(1, hk)) <= KV4_FEW_ROWS:
+    if not kv4_prefill_expands(max_q, hq, hk, d):
         _count(2)
         return native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, max_q, hq, hk, d,
                                       page_size, scale, err)

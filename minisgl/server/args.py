@@ -3,7 +3,7 @@
 Every flag of the reference (python/minisgl/server/args.py:54-268) is kept
 with the same names, aliases and defaults. Added: ``--ep-size/--ep``,
 ``--cp-size/--cp``, ``--enable-dp-attention``, ``--moe-quant``,
-``--random-init`` (alias of ``--dummy-weight``: seeded N(0, 0.02) weights),
+``--kv-quant``, ``--random-init`` (alias of ``--dummy-weight``: seeded N(0, 0.02) weights),
 ``--comm {fused,nccl}`` (default fused; ``--disable-pynccl`` selects nccl)
 and ``--device``. ``--model synthetic:<shape>``
 serves a synthetic model folder (see ``minisgl.utils.synthetic``).
@@ -80,6 +80,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--moe-quant", choices=["none", "mxfp4", "mxfp4-a8"], default="none",
                    help="routed experts: bf16, MXFP4 weights with bf16 activations, or MXFP4 weights x MXFP8 "
                         "activations on the block-scaled tensor cores")
+    p.add_argument("--kv-quant", choices=["none", "int4"], default="none",
+                   help="keys and values of MHA / GQA models cached as they are, or in 4 bits with a scale per 32 "
+                        "dims (3.76 times the tokens in the same memory)")
     p.add_argument("--comm", choices=["nccl", "fused"], default="fused",
                    help="TP collectives: in-kernel NVLink collectives (default) or NCCL (baseline); "
                         "ignored on --device cpu")
