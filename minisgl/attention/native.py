@@ -123,7 +123,7 @@ class NativeAttnBackend(BaseAttnBackend):
         dev = host.to(self.device, non_blocking=True)
         cu_q = dev[2 * B :]
         plan = None
-        if self.kv4 and on_gpu and ops.kv4_prefill_expands(max(qlens), self.hq, self.hk, self.d):
+        if self.kv4 and on_gpu and ops.kv4_prefill_expands(max(qlens), self.hq, self.hk):
             plan = ops.KV4PrefillPlan(lens, self.device)
         batch.attn_metadata = NativeAttnMetadata(
             req_rows=dev[:B], seq_lens=dev[B : 2 * B], cu_q=cu_q, max_q=max(qlens), max_splits=1,

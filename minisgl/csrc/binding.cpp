@@ -1580,7 +1580,7 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
   const char* op = "prefill_attention_kv4";
   const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
   MSG_CHECK(hq >= hk && hq % hk == 0 && minisgl::kv4_prefill_takes(static_cast<int>(d), static_cast<int>(hq / hk)), op,
-            ": many rows take head_dim 128 and groups of up to 128 heads");
+            ": many rows take groups of up to 128 heads");
   MSG_CHECK(scale > 0 && scale <= 1e6, op, ": scale must be positive");
   check_rows16(op, q, "q", hq * d, pool);
   const int64_t T = q.size(0), B = req_rows.numel(), R = row_req.numel();
@@ -1641,7 +1641,7 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
   minisgl::launch_kv4_load(l, stream_of(pool));
   minisgl::Kv4PrefillArgs a{};
   a.q = q.data_ptr();
-  a.ld_q = static_cast<int>(q.stride(0));
+  a.ld_q = static_cast<int>(T > 1 ? q.stride(0) : hq * d);  // the tensor map takes no other stride
   a.out = out.data_ptr();
   a.images = images.data_ptr();
   a.first_tile = plan_table.data_ptr<int32_t>();
@@ -1655,6 +1655,7 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
   a.hk = static_cast<int>(hk);
   a.group = static_cast<int>(hq / hk);
   a.scale = static_cast<float>(scale);
+  a.d = static_cast<int>(d);
   a.ctas = ctas;
   a.runs = runs;
   a.desc = runs + 8 * ctas;
@@ -1668,8 +1669,8 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
 // Few query rows over the 4-bit cache; cu_q absent: one token per request.
 at::Tensor kv4_attention(const at::Tensor& q, const c10::optional<at::Tensor>& dst, const at::Tensor& pool, int64_t layer,
                          const at::Tensor& page_table, const at::Tensor& req_rows, const at::Tensor& seq_lens,
-                         const c10::optional<at::Tensor>& cu_q, int64_t max_q, int64_t hq, int64_t hk, int64_t d,
-                   int64_t page_size, double scale, const c10::optional<at::Tensor>& err) {
+                         const c10::optional<at::Tensor>& cu_q, int64_t hq, int64_t hk, int64_t d,
+                         int64_t page_size, double scale, const c10::optional<at::Tensor>& err) {
   const char* op = cu_q.has_value() ? "prefill_attention_kv4" : "decode_attention_kv4";
   const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
   MSG_CHECK(hq >= hk && hq % hk == 0, op, ": hq must be a multiple of hk");
@@ -1690,9 +1691,9 @@ at::Tensor kv4_attention(const at::Tensor& q, const c10::optional<at::Tensor>& d
   MSG_CHECK(B <= minisgl::kKv4MaxBatch, op, ": at most ", static_cast<int64_t>(minisgl::kKv4MaxBatch), " requests, got ", B);
   if (B == 0 || T == 0) return out;
   MSG_CHECK(page_table.size(0) >= 1 && page_table.size(1) >= 1, op, ": page_table is empty");
-  const int64_t rows = (max_q * (hq / hk) + 7) / 8;
-  MSG_CHECK(B * hk * rows * ((page_table.size(1) + 127) / 128) < (int64_t{1} << 30) && T * hq <= 0x7fffffff, op,
-            ": too many tiles of work");
+  // tiles of 8 query rows, each with a place of its own and its key tiles
+  const int64_t units = (T * (hq / hk) / 8 + B) * hk;
+  MSG_CHECK(units * (page_table.size(1) / 128 + 2) <= 0x7fffffff && T * hq <= 0x7fffffff, op, ": too many tiles of work");
   const int runs = minisgl::kv4_attn_runs(at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
   // records of partial pieces, then the descriptors
   const int64_t floats = static_cast<int64_t>(runs) * 2 * 8 * (d + 2) + 4 * runs;

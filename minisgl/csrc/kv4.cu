@@ -1,6 +1,6 @@
 // Rows of the 4-bit paged KV cache: store (with the per-head norms and the
 // rotation of queries and keys in the same pass), read-back as bf16 rows or as
-// a compact bf16 pool, and copies of whole pages.
+// tile images for the attention of many query rows, and copies of whole pages.
 //
 // The 16-bit counterpart of the store is rope_store.cu; the reference stores
 // 16-bit rows only (python/minisgl/kernel/csrc/jit/store.cu:25-53).
@@ -83,25 +83,36 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t& wor
 }
 
 // ================================================================ store ====
-// Eight dims a thread, D / 8 threads a head, one role a block: queries and keys,
-// kHeads of one token a thread (its cosines and sines, as many bytes as a head,
-// are read once, and all its rows are on the way before the first is worked
-// on), or values, four tokens a thread, so that a run of tokens whose slots fill
-// whole rows of V codes is written in 16-byte chunks; other tokens' codes are
-// bytes between those of their neighbours. q is rounded once, to bf16 at the
-// end, k and v once, to codes.
+// One role a block: queries and keys, kHeads of one token a thread, or values.
+//
+// A thread has dims 8 x .. 8 x + 7 and those that they turn with, D / 2 on, of its
+// heads: no lane waits for another in the rotation, one read of the token's
+// cosines and sines (as many bytes as a head) serves 16 dims of each, and all its
+// rows are on the way before the first is worked on. Values, four tokens of eight
+// dims a thread, so that a run of tokens whose slots fill whole rows of V codes is
+// written in 16-byte chunks; other tokens' codes are bytes between those of their
+// neighbours. q is rounded once, to bf16 at the end, k and v once, to codes.
+//
+// Bound by memory where there are many rows, but for the work on each: 8189 rows
+// of 64 + 2 x 8 heads, 315 MB read and written, take 65.5 us, 4.8 TB/s (74 % of the
+// copy rate). With eight dims a thread and a shuffle for each partner 73, with IEEE
+// division calls for the codes 113. A few rows: by the launch and one round of
+// loads, 2.3 us for one.
 template <int D, int kHeads, bool kQuery>
 __device__ __forceinline__ void store_turned(const Kv4StoreArgs& a, int unit, int x, const ErrorSink& err) {
-  constexpr int kLanes = D / 8;  // threads of a head
+  constexpr int kLanes = D / 16;  // threads of a head
   const int heads = kQuery ? a.hq : a.hk;
   const int per = (heads + kHeads - 1) / kHeads;
   const bool live = unit < a.T * per;  // the others go along for the shuffles
   const int t = live ? unit / per : 0;
   const int h0 = live ? (unit - t * per) * kHeads : 0;
   const bf16* src = static_cast<const bf16*>(kQuery ? a.q : a.k) + static_cast<int64_t>(t) * (kQuery ? a.ld_q : a.ld_k);
-  uint4 raw[kHeads];
+  uint4 raw[kHeads][2];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) raw[i] = *(reinterpret_cast<const uint4*>(src + min(h0 + i, heads - 1) * D) + x);
+  for (int i = 0; i < kHeads; ++i) {
+    const uint4* head = reinterpret_cast<const uint4*>(src + min(h0 + i, heads - 1) * D) + x;
+    raw[i][0] = head[0], raw[i][1] = head[kLanes];
+  }
   float c[8], s[8];
   if (a.cos_sin != nullptr) {
     int pos = a.positions[t];
@@ -109,17 +120,12 @@ __device__ __forceinline__ void store_turned(const Kv4StoreArgs& a, int unit, in
       if (live && x == 0) err.report(kErrBadIndex, 951);
       pos = 0;
     }
-    const float4* cs = reinterpret_cast<const float4*>(a.cos_sin + static_cast<int64_t>(pos) * D) + x % (kLanes / 2) * 2;
-    const float4 v[4] = {cs[0], cs[1], cs[D / 8], cs[D / 8 + 1]};
-    *reinterpret_cast<float4*>(c) = v[0], *reinterpret_cast<float4*>(c + 4) = v[1];
-    *reinterpret_cast<float4*>(s) = v[2], *reinterpret_cast<float4*>(s + 4) = v[3];
-    if (x < kLanes / 2) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = -s[i];
-    }
+    const float4* cs = reinterpret_cast<const float4*>(a.cos_sin + static_cast<int64_t>(pos) * D) + 2 * x;
+    *reinterpret_cast<float4*>(c) = cs[0], *reinterpret_cast<float4*>(c + 4) = cs[1];
+    *reinterpret_cast<float4*>(s) = cs[D / 8], *reinterpret_cast<float4*>(s + 4) = cs[D / 8 + 1];
   }
+  bool stored = false;
   int page = 0, tok = 0;
-  bool stored = live;
   if constexpr (!kQuery) {
     const int slot = a.out_loc[t];
     stored = live && slot >= 0 && slot < a.kv_slots;
@@ -127,43 +133,55 @@ __device__ __forceinline__ void store_turned(const Kv4StoreArgs& a, int unit, in
     page = slot >> a.page_shift, tok = slot & (a.page_size - 1);
   }
   const bf16* nw = static_cast<const bf16*>(kQuery ? a.q_norm_w : a.k_norm_w);
-  uint4 raw_w;
-  if (nw != nullptr) raw_w = *(reinterpret_cast<const uint4*>(nw) + x);
+  uint4 raw_w[2];
+  if (nw != nullptr) raw_w[0] = *(reinterpret_cast<const uint4*>(nw) + x), raw_w[1] = *(reinterpret_cast<const uint4*>(nw) + kLanes + x);
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     const int h = h0 + i;
-    float y[8];
-    unpack8(raw[i], y);
+    float y[2][8];
+    unpack8(raw[i][0], y[0]), unpack8(raw[i][1], y[1]);
     if (nw != nullptr) {
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += y[j] * y[j];
+      for (int j = 0; j < 8; ++j) sum += y[0][j] * y[0][j] + y[1][j] * y[1][j];
 #pragma unroll
       for (int o = 1; o < kLanes; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       const float inv = rsqrtf(sum / D + a.eps);
-      float w[8];
-      unpack8(raw_w, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = y[j] * inv * w[j];
+      for (int u = 0; u < 2; ++u) {
+        float w[8];
+        unpack8(raw_w[u], w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[u][j] = y[u][j] * inv * w[j];
+      }
     }
     if (a.cos_sin != nullptr) {
-      // dim j turns with dim j + D / 2, which the thread D / 16 away holds
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = y[j] * c[j] + __shfl_xor_sync(0xffffffffu, y[j], kLanes / 2) * s[j];
+      for (int j = 0; j < 8; ++j) {
+        const float lo = y[0][j], hi = y[1][j];
+        y[0][j] = lo * c[j] - hi * s[j], y[1][j] = hi * c[j] + lo * s[j];
+      }
     }
     if constexpr (kQuery) {
-      uint4 o;
-      o.x = pack_bf16x2(y[0], y[1]), o.y = pack_bf16x2(y[2], y[3]);
-      o.z = pack_bf16x2(y[4], y[5]), o.w = pack_bf16x2(y[6], y[7]);
-      if (live && h < heads)
-        *(reinterpret_cast<uint4*>(static_cast<bf16*>(a.q_out) + static_cast<int64_t>(t) * a.ld_qo + h * D) + x) = o;
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<bf16*>(a.q_out) + static_cast<int64_t>(t) * a.ld_qo + h * D) + x;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint4 o;
+        o.x = pack_bf16x2(y[u][0], y[u][1]), o.y = pack_bf16x2(y[u][2], y[u][3]);
+        o.z = pack_bf16x2(y[u][4], y[u][5]), o.w = pack_bf16x2(y[u][6], y[u][7]);
+        if (live && h < heads) dst[u * kLanes] = o;
+      }
     } else {
-      uint32_t word;
-      const uint32_t byte = quantize8(y, word);
-      if (stored && h < heads) {
-        uint8_t* dst = a.k_pool + (static_cast<int64_t>(page) * a.hk + h) * a.page_size * kv4::row_bytes(D);
-        reinterpret_cast<uint32_t*>(dst + tok * (D / 2))[kv4::k_word<D>(x)] = word;
-        if (x % 4 == 0) dst[a.page_size * (D / 2) + tok * (D / kv4::kGroup) + x / 4] = static_cast<uint8_t>(byte);
+      uint8_t* dst = a.k_pool + (static_cast<int64_t>(page) * a.hk + h) * a.page_size * kv4::row_bytes(D);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t word;
+        const uint32_t byte = quantize8(y[u], word);
+        if (stored && h < heads) {
+          reinterpret_cast<uint32_t*>(dst + tok * (D / 2))[kv4::k_word<D>(u * kLanes + x)] = word;
+          if (x % 4 == 0)
+            dst[a.page_size * (D / 2) + tok * (D / kv4::kGroup) + (u * kLanes + x) / 4] = static_cast<uint8_t>(byte);
+        }
       }
     }
   }
@@ -229,24 +247,25 @@ __device__ __forceinline__ void store_values(const Kv4StoreArgs& a, int unit, in
   }
 }
 
-template <int D, int kHeads>
-__global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ Kv4StoreArgs a, int q_blocks,
+template <int D, int kHeads, int kMin>
+__global__ void __launch_bounds__(256, kMin) kv4_store_kernel(const __grid_constant__ Kv4StoreArgs a, int q_blocks,
                                                         int k_blocks) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int kLanes = D / 8, kUnits = 256 / kLanes;
+  constexpr int kLanes = D / 16, kUnits = 256 / kLanes;
   const ErrorSink err{a.err};
   const int x = threadIdx.x % kLanes, in = threadIdx.x / kLanes;
-  const int block = blockIdx.x;
+  const int block = blockIdx.x, thread = threadIdx.x;
   if (block < q_blocks) store_turned<D, kHeads, true>(a, block * kUnits + in, x, err);
   else if (block < q_blocks + k_blocks) store_turned<D, kHeads, false>(a, (block - q_blocks) * kUnits + in, x, err);
-  else store_values<D>(a, (block - q_blocks - k_blocks) * kUnits + in, x, err);
+  else store_values<D>(a, (block - q_blocks - k_blocks) * (kUnits / 2) + thread / (D / 8), thread % (D / 8), err);
 }
 
 // ================================================================= load ====
 // Eight dims of K and of V of one row and head a thread. Values are s (c - 8),
 // exact in bf16: 128 + c has the bits 0x4300 | c, and s (128 + c) - 136 s is one
-// fused multiply-add (136 s = 17 s 8 has at most 8 significant bits).
+// fused multiply-add (136 s = 17 s 8 has at most 8 significant bits). Bound by
+// what it writes, 512 bytes for 136 read of a row of 128 dims.
 __device__ __forceinline__ uint4 values8(uint32_t word, uint32_t byte) {
   const uint32_t s2 = byte * 0x00100010u + kv4::kScaleBf16x2;
   const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&s2);
@@ -390,9 +409,9 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ K
     v_to = k_to + kKv4TileKeys * kLanes;
     const int req = a.row_req[r];
     slot = -1;
-    if (req >= 0) {
+    if (req >= 0 && req < a.B) {
       const int table_row = a.req_rows[req], pos = a.row_pos[r];
-      if (table_row >= 0 && table_row < a.pt_rows && pos < a.ld_pt)
+      if (table_row >= 0 && table_row < a.pt_rows && pos >= 0 && pos < a.ld_pt)
         slot = a.page_table[static_cast<int64_t>(table_row) * a.ld_pt + pos];
       if (slot < 0 || slot >= a.kv_slots) {
         if (x == 0) err.report(kErrBadIndex, 955);
@@ -418,8 +437,11 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ K
 
 // ================================================================= copy ====
 // Pages of every plane (K / V and layer) of a pool, pair by pair; the pairs
-// travel as a kernel argument, so a call is one launch and leaves nothing
-// behind on the device. grid (chunks of a page, pairs, planes in turn).
+// travel as a kernel argument (32 of them, or 480 where there are more: 256 bytes
+// or 4 KB to send with a launch), so a call of up to 480 is one launch and leaves
+// nothing behind on the device. grid (chunks of a page, pairs, planes in turn).
+// Bound by memory: 500 pages of 64 layers x 8 heads (4-bit, 4.46 GB read and
+// written) 659 us, 6.8 TB/s, 103 % of the copy rate; one page 3.1 us.
 template <int N>
 struct PagePairs {
   int src[N], dst[N];
@@ -462,15 +484,19 @@ void copy_pairs(const CopyPagesArgs& a, int from, int n, cudaStream_t s) {
 namespace {
 template <int D>
 void store_typed(const Kv4StoreArgs& a, cudaStream_t s) {
-  constexpr int kUnits = 256 / (D / 8);
-  // one head a thread while that does not fill the GPU, then four
-  const bool many = static_cast<int64_t>(a.T) * (a.hq + a.hk) > 148 * 8 * kUnits;
-  auto blocks = [&](int64_t units) { return (units + kUnits - 1) / kUnits; };
-  const int64_t q = blocks(static_cast<int64_t>(a.T) * (many ? (a.hq + 3) / 4 : a.hq));
-  const int64_t k = blocks(static_cast<int64_t>(a.T) * (many ? (a.hk + 3) / 4 : a.hk));
-  const int64_t v = blocks(static_cast<int64_t>((a.T + 6) / 4) * a.hk);
+  constexpr int kUnits = 256 / (D / 16);  // of queries and keys in a block; of values half as many
+  // One head a thread while they all fit the GPU at once, two up to four times as
+  // many, then four. us with 1, 2 and 4 for rows of 64 + 2 x 8 heads of 128 dims:
+  // 256 rows 4.3, 4.5, 6.4; 512 7.3, 7.0, 7.5; 1024 12.1, 10.8, 11.4; 2048 19.9,
+  // 19.6, 17.1; 8189 74.2, 77.9, 65.5.
+  const int64_t wave = int64_t{148} * 5 * kUnits, all = static_cast<int64_t>(a.T) * (a.hq + a.hk);
+  const int heads = all <= wave ? 1 : all <= 4 * wave ? 2 : 4;
+  auto blocks = [](int64_t units, int per) { return (units + per - 1) / per; };
+  const int64_t q = blocks(static_cast<int64_t>(a.T) * ((a.hq + heads - 1) / heads), kUnits);
+  const int64_t k = blocks(static_cast<int64_t>(a.T) * ((a.hk + heads - 1) / heads), kUnits);
+  const int64_t v = blocks(static_cast<int64_t>((a.T + 6) / 4) * a.hk, kUnits / 2);
   if (q + k + v > 0x7fffffff / kUnits) throw std::runtime_error("minisgl.rope_store_kv4: too many rows");
-  auto kern = many ? kv4_store_kernel<D, 4> : kv4_store_kernel<D, 1>;
+  auto kern = heads == 1 ? kv4_store_kernel<D, 1, 5> : heads == 2 ? kv4_store_kernel<D, 2, 2> : kv4_store_kernel<D, 4, 3>;
   launch_pdl(kern, dim3(static_cast<unsigned>(q + k + v)), dim3(256), 0, s, a, static_cast<int>(q), static_cast<int>(k));
 }
 }  // namespace
@@ -489,9 +515,10 @@ void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s) {
   const int per_block = 256 / (a.d / 8);
   const int64_t blocks = (static_cast<int64_t>(a.T) * a.hk + per_block - 1) / per_block + (images ? 1 : 0);
   if (blocks > 0x7fffffff) throw std::runtime_error("minisgl.load_kv4: too many rows");
-  if (images && (a.d != 128 || a.T % kKv4TileKeys != 0))
-    throw std::runtime_error("minisgl.prefill_attention_kv4: tile images are of 128 keys and dims");
-  auto kern = images ? kv4_load_kernel<128, true> : a.d == 128 ? kv4_load_kernel<128, false> : kv4_load_kernel<64, false>;
+  if (images && a.T % kKv4TileKeys != 0)
+    throw std::runtime_error("minisgl.prefill_attention_kv4: tile images are of 128 keys");
+  auto kern = a.d == 128 ? (images ? kv4_load_kernel<128, true> : kv4_load_kernel<128, false>)
+                         : (images ? kv4_load_kernel<64, true> : kv4_load_kernel<64, false>);
   launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a);
 }
 

@@ -4,21 +4,37 @@
 //   o_r = sum_j p_rj v_j / sum_j p_rj,  p_rj = 2^((q_r . k_j - m_r) c),  c = scale log2 e,
 //
 // with k_j and v_j in 4-bit codes, 136 bytes of cache per token and 128-dim
-// head. Bound by what a warp has to do per code, not by the tensor pipe, so
-// everything is laid out to keep that small:
+// head. Bound by what a warp has to do per code, on the integer and half2 pipes:
+// 256 requests of up to 4096 keys and 8 KV heads take 140 us, 4.1 TB/s of codes
+// (63 % of the copy rate), one of 131072 keys 45 us. Everything is laid out to
+// keep that small:
 //
 // * The products are taken the other way round, S^T = K q^T and O^T = V^T P^T
-//   (warp-level m16n8k16 bf16 MMA): keys and dims fill the 16 rows of A, and
-//   the query rows, 8 at a time, are the 8 columns of B, so nothing is wasted
-//   on padding for groups of up to 8 heads. tcgen05 would need 128 rows.
+//   (warp-level m16n8k16 MMA): keys and dims fill the 16 rows of A, and the query
+//   rows, 8 at a time, are the 8 columns of B, so nothing is wasted on padding for
+//   groups of up to 8 heads. tcgen05 would need 128 rows, and the codes written
+//   out to shared memory.
 // * The cache's byte order is the A fragments' order: a lane's 16 bytes from
-//   shared memory are the codes of two MMAs (K) or four (V), and a code pair
-//   becomes two bf16 numbers by one mask: 128 + c has the bits 0x4300 | c.
-// * K: the product starts at -136 sum(q) instead of 0, which turns 128 + c into
-//   c - 8, and a group's scale multiplies its four sums. V: s (128 + c) - 136 s
-//   in one packed fused multiply-add, exact in bf16.
+//   shared memory are the codes of two MMAs (K) or four (V).
+// * K: the bits of a code c, where they stand, are the fp16 number c 2^-24 (or
+//   16 c 2^-24 four bits up): a mask makes a pair, with no exponent to set. q is
+//   taken to fp16 by a power of two for each row, odd dims with 1/16 of it. The 8
+//   that codes are above their values is a product of its own: a group's scale
+//   with -8 sum(q) of its dims, in three bf16 parts. A group's scale multiplies
+//   its four sums. Against bf16 numbers 128 + c that start at -136 sum(q): 172
+//   for 173 us, and 8-bit floats, which the warp-level MMA converts first: 205.
+// * V: 128 + c has the bf16 bits 0x4300 | c, and s (128 + c) - 136 s is one packed
+//   fused multiply-add, exact in bf16.
 // * The running maximum moves only when a score exceeds it by 8 (in powers of
 //   two); other tiles neither reduce over lanes nor rescale the output.
+// * Weights p are rounded to bf16, as V is held; their sum is of fp32 weights.
+//
+// A CTA, one an SM, is three groups of four warps, 32 keys of a tile each, and a
+// warp for each group that fetches its tiles by bulk copies, page numbers a tile
+// ahead: those take few registers, so the launch's 128 a thread are dealt anew
+// (152 and 56). Without the split, eight warps at a time: 164 us instead of 140;
+// sixteen of 112 registers: 144. Four CTAs of one group, which fetches for
+// itself: 188.
 //
 // Work is split evenly whatever the lengths are: all key tiles of all requests,
 // heads and row tiles form one sequence, with a place more for each unit of them
@@ -615,7 +631,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
 }
 
 // Joins the records of the unit that run blockIdx.x began and others went on
-// with. Warp w: row w % 8, records w / 8 modulo 4 of the chain.
+// with. Warp w: row w % 8, records w / 8 modulo 4 of the chain. Bound by latency:
+// with a warp for all records of a row a chain of 55 (one request of 131072 keys)
+// took 55 us in all instead of 45.
 template <int D, bool kSingle>
 __global__ void __launch_bounds__(1024) kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
   pdl_launch_dependents();

@@ -4,8 +4,11 @@
 //   S = Q K^T,  P = 2^(S scale log2 e - m),  O += P V,  out = O / sum P
 //
 // on tcgen05. Bound by the tensor pipe (4 d flops per query row and key) and,
-// close behind, by the exponentials: 128 x 128 scores take 1024 cycles of MMA
-// for both products and 1024 of the special-function unit.
+// close behind, by the exponentials: 128 x 128 scores of 128 dims take 1024 cycles
+// of MMA for both products and 1024 of the special-function unit (64 dims: 640).
+// 2048 queries of 64 heads over 16384 keys: 822 to 838 us with the expansion, 1230
+// to 1250 TFLOP/s, 90 % of what cuBLAS sustains under the power limit. 4 prompts
+// of 2048 tokens, 32 heads of 64 dims: 146 us.
 //
 // Query rows are (token, head of the group): TT = 128 / G tokens are a tile, so
 // every group size fills its 128 rows (G = 7: 126 of them) and all heads of a
@@ -14,15 +17,18 @@
 // tile's products run. 128-key tiles: an MMA of 128 x 128 x 16 takes 64 cycles,
 // of 128 x 64 x 16 48 (measured), so 64-key tiles would leave a quarter unused.
 //
+// Weights are rounded to bf16 for the second product, their sums are of fp32
+// ones; a row's maximum is taken up to bf16, which does for a reference.
+//
 // Work is split evenly: the key tiles of all row-tile pairs form one sequence, of
 // which each CTA (one an SM) takes an equal run; a pair whose tiles fall to
 // several CTAs leaves (m, l, O) records, joined by a second kernel. 2048 queries
 // of 8 KV heads are 512 pairs, 3.46 a CTA: as whole pairs they took 4 turns.
 //
-// Keys come as shared-memory images: 128 rows of K (or V) of a head are two
-// 64-dim halves of 128-byte rows, swizzled as the MMA descriptors expect, so one
-// plain bulk copy of 32 KB brings each. Tensor memory: O of tile X at columns
-// 128 X, S of it at 256 + 128 X with P (bf16 pairs) over its first 64.
+// Keys come as shared-memory images: 128 rows of K (or V) of a head are 64-dim
+// halves of 128-byte rows, swizzled as the MMA descriptors expect, so one plain
+// bulk copy of 32 KB (64 dims: 16) brings each. Tensor memory: O of tile X at
+// columns 128 X, S of it at 256 + 128 X with P (bf16 pairs) over its first 64.
 #include <algorithm>
 #include <stdexcept>
 
@@ -35,11 +41,9 @@
 namespace minisgl {
 namespace {
 
-constexpr int kD = 128;
 constexpr int kRows = 128;                 // query rows of a tile
 constexpr int kKeys = kKv4TileKeys;        // keys of a tile
 constexpr int kHalf = kRows * 128;         // 64 dims of 128 rows (16 KB)
-constexpr int kImage = 2 * kHalf;          // K or V of a tile (32 KB)
 constexpr int kSlots = 5;                  // images in flight: K_0, V_0, K_1, ...
 constexpr int kLoader = 16, kIssuer = 17;  // after eight softmax warps a tile
 constexpr int kThreads = 576;
@@ -48,9 +52,12 @@ constexpr int kPolyPairs = 2;              // of 8 pairs of exponentials, on the
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;            // the running maximum moves by more than this or not at all
 constexpr int kAhead = 4;                  // pieces whose descriptions are kept
-constexpr int kSmem = 1024 + 2 * kImage + kSlots * kImage + 256 + 2 * 4 * 128 + kAhead * 48;
-static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 static_assert(kKeys == 128, "tiles of 128 keys");
+template <int kD>
+constexpr int image_bytes() { return kD / 64 * kHalf; }  // K or V of a tile (32 KB, 16 KB)
+template <int kD>
+constexpr int smem_bytes() { return 1024 + (2 + kSlots) * image_bytes<kD>() + 256 + 2 * 4 * 128 + kAhead * 48; }
+static_assert(smem_bytes<128>() <= 227 * 1024, "shared memory of a CTA");
 
 // Waits that sleep: a first try that may suspend the thread for 20 us leaves the
 // issue slots of its scheduler to the softmax warps (spinning waits took a third
@@ -147,9 +154,12 @@ __device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
 // Tiles of row tile x in the piece.
 __device__ __forceinline__ int tiles_in(const Piece& p, int x) { return max(0, min(p.kt1, x == 0 ? p.n0 : p.n1) - p.kt0); }
 
+template <int kD>
 __global__ void __launch_bounds__(kThreads, 1)
     kv4_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ Kv4PrefillArgs a) {
   extern __shared__ uint8_t smem_raw[];
+  constexpr int kHalves = kD / 64;
+  constexpr int kImage = image_bytes<kD>();
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = smem;  // [tile][64-dim half]
   uint8_t* sKV = sQ + 2 * kImage;
@@ -199,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
   }
   // rows that no query fills are zeros
-  for (int i = threadIdx.x; i < 4 * (kRows - TT * G) * 8; i += kThreads) {
+  for (int i = threadIdx.x; i < 2 * kHalves * (kRows - TT * G) * 8; i += kThreads) {
     const int part = i / ((kRows - TT * G) * 8), at = i % ((kRows - TT * G) * 8);
     reinterpret_cast<uint4*>(sQ + part * kHalf + TT * G * 128)[at] = make_uint4(0, 0, 0, 0);
   }
@@ -253,11 +263,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         image(src);
         if (ok && pieces > 0) ok = wait_asleep(q_empty, (pieces - 1) & 1, err, 270, s_abort);
         if (!ok) break;
-        mbar_arrive_expect_tx(q_full, 4 * TT * G * 128);
+        mbar_arrive_expect_tx(q_full, 2 * kHalves * TT * G * 128);
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < kHalves; ++c)
             tma_load_3d(sQ + x * kImage + c * kHalf, &tm_q, q_full, 64 * c, p.h * G, p.q_begin + p.tok0 + x * TT);
         ++pieces;
         image(src + kImage);
@@ -279,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto qk = [&](int x, int e) {  // S_x = Q_x K^T of entry e
       const uint64_t k = k_desc + static_cast<uint64_t>((e % kSlots) * (kImage >> 4));
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < kHalves; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           tc_mma_f16(tmem + kSCol + 128 * x, q_desc + static_cast<uint64_t>((x * kImage + c * kHalf + i * 32) >> 4),
@@ -359,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x = warp >> 3, part = (warp >> 2) & 1, quad = warp & 3;
     const int r = 32 * quad + lane;  // this thread's row (TMEM lane)
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * quad) << 16);
-    const uint32_t s_col = lane_base + kSCol + 128 * x, o_col = lane_base + 128 * x + 64 * part;
+    const uint32_t s_col = lane_base + kSCol + 128 * x, o_col = lane_base + 128 * x + kD / 2 * part;
     uint8_t* swap = s_swap + (4 * x + quad) * 128;
     __nv_bfloat16* mine = reinterpret_cast<__nv_bfloat16*>(swap) + 32 * part + lane;
     const __nv_bfloat16* other = reinterpret_cast<const __nv_bfloat16*>(swap) + 32 * (1 - part) + lane;
@@ -413,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // read and written (tcgen05.ld / st take whole warps)
         if (__any_sync(0xffffffffu, grow) && j > 0) {
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < kD / 32; ++q) {
             uint32_t ov[16];
             tmem_ld_32x32b_x16(o_col + 16 * q, ov);
             tc_wait_ld();
@@ -466,10 +476,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       pair_sync();
       if (part == 1) l = reinterpret_cast<const float*>(swap)[lane];
       pair_sync();
-      uint32_t ov[64] = {};
+      uint32_t ov[kD / 2] = {};
       if (ok && nx > 0) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) tmem_ld_32x32b_x32(o_col + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(ov + 32 * q));
+        for (int q = 0; q < kHalves; ++q) tmem_ld_32x32b_x32(o_col + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(ov + 32 * q));
         tc_wait_ld();
         tc_fence_before();
         __syncwarp();
@@ -481,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // side (of 16 bytes a row each they took the load-store unit 4000 cycles a piece)
         const int64_t row = live ? static_cast<int64_t>(p.q_begin + t) * a.hq + p.h * G + r % G : -1;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < kHalves; ++q) {
           uint4 v[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -496,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i) {  // of the row of lane (lane & ~3) + i
             const int64_t to = __shfl_sync(0xffffffffu, row, (lane & ~3) + i);
             if (to >= 0)
-              reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + to * kD + 64 * part + 32 * q)[lane & 3] = v[i];
+              reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + to * kD + kD / 2 * part + 32 * q)[lane & 3] = v[i];
           }
         }
       } else {
@@ -504,9 +514,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // (vectors of four dims, a warp's rows side by side)
         const int64_t rec = 2 * static_cast<int>(blockIdx.x) + (p.kt0 == 0 ? 1 : 0);
         if (part == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (rec * (2 * kRows) + x * kRows + r)) = make_float2(m, l);
-        uint4* dst = reinterpret_cast<uint4*>(a.part_o + rec * (2 * kRows) * kD) + ((4 * x + quad) * 32 + 16 * part) * 32 + lane;
+        uint4* dst = reinterpret_cast<uint4*>(a.part_o + rec * (2 * kRows) * kD) + ((4 * x + quad) * (kD / 4) + kD / 8 * part) * 32 + lane;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dst[32 * i] = make_uint4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
+        for (int i = 0; i < kD / 8; ++i) dst[32 * i] = make_uint4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
       }
     }
     if (!ok && lane == 0) atomicExch(s_abort, 1);
@@ -526,13 +536,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Joins the records of the pair that CTA blockIdx.x began and others went on
 // with: a lane a row, four dims of 32 rows a warp.
+template <int kD>
 __global__ void __launch_bounds__(256) kv4_prefill_join_kernel(const __grid_constant__ Kv4PrefillArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int4 d = reinterpret_cast<const int4*>(a.desc)[blockIdx.x];
   if (d.x < 0) return;
   const int lane = threadIdx.x & 31;
-  const int block = blockIdx.y / 4, vec = blockIdx.y % 4 * 8 + (threadIdx.x >> 5);  // 32 rows, 4 dims
+  const int block = blockIdx.y / (kD / 32), vec = blockIdx.y % (kD / 32) * 8 + (threadIdx.x >> 5);  // 32 rows, 4 dims
   const int G = a.group, TT = kRows / G, row = 32 * block + lane, r = row % kRows;
   const int t = d.z * 2 * TT + row / kRows * TT + r / G;
   if (r >= TT * G || t >= kv4_query_tokens(a.cu_q, d.y, a.T)) return;
@@ -545,7 +556,7 @@ __global__ void __launch_bounds__(256) kv4_prefill_join_kernel(const __grid_cons
   for (int i = begin; i <= d.x; ++i) {
     const int64_t rec = rec_of(i);
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (rec + row));
-    const float4 v = reinterpret_cast<const float4*>(a.part_o + rec * kD)[(block * 32 + vec) * 32 + lane];
+    const float4 v = reinterpret_cast<const float4*>(a.part_o + rec * kD)[(block * (kD / 4) + vec) * 32 + lane];
     const float f = ml.x == -INFINITY ? 0.f : ex2_fast(ml.x - top);  // no key of the row there
     l += ml.y * f;
     acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
@@ -556,17 +567,14 @@ __global__ void __launch_bounds__(256) kv4_prefill_join_kernel(const __grid_cons
   dst[vec] = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
 }
 
-}  // namespace
-
-bool kv4_prefill_takes(int d, int group) { return d == kD && group >= 1 && group <= kRows; }
-
-void launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t s) {
-  if (a.B <= 0 || a.T <= 0) return;
-  static bool done[64] = {};
+template <int kD>
+void launch_typed(const Kv4PrefillArgs& a, cudaStream_t s) {
+  constexpr int kSmem = smem_bytes<kD>();
+  static bool done[64] = {};  // per device
   int dev = 0;
   cudaGetDevice(&dev);
   if (!done[dev & 63]) {
-    if (cudaFuncSetAttribute(kv4_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(kv4_prefill_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
       throw std::runtime_error("minisgl.prefill_attention_kv4: shared memory limit");
     done[dev & 63] = true;
   }
@@ -576,8 +584,19 @@ void launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t s) {
   const uint64_t strides[2] = {kD * 2, static_cast<uint64_t>(a.ld_q) * 2};
   const uint32_t box[3] = {64, static_cast<uint32_t>(a.group), static_cast<uint32_t>(TT)};
   const CUtensorMap tq = make_tmap(a.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-  launch_pdl(kv4_prefill_kernel, dim3(a.ctas), dim3(kThreads), kSmem, s, tq, a);
-  launch_pdl(kv4_prefill_join_kernel, dim3(a.ctas, 2 * kRows / 8), dim3(256), 0, s, a);
+  launch_pdl(kv4_prefill_kernel<kD>, dim3(a.ctas), dim3(kThreads), kSmem, s, tq, a);
+  launch_pdl(kv4_prefill_join_kernel<kD>, dim3(a.ctas, 2 * kRows / 32 * (kD / 32)), dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+bool kv4_prefill_takes(int d, int group) { return (d == 64 || d == 128) && group >= 1 && group <= kRows; }
+
+void launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t s) {
+  if (a.B <= 0 || a.T <= 0) return;
+  if (a.d == 128) launch_typed<128>(a, s);
+  else if (a.d == 64) launch_typed<64>(a, s);
+  else throw std::runtime_error("minisgl.prefill_attention_kv4: head_dim must be 64 or 128");
 }
 
 }  // namespace minisgl

@@ -273,19 +273,19 @@ void launch_kv4_attention(const Kv4AttnArgs& a, cudaStream_t s);
 constexpr int kKv4TileKeys = 128;
 constexpr int kKv4PairCost = 2;  // what a pair costs beside its tiles, in tiles
 struct Kv4PrefillArgs {
-  const void* q;             // [T, >= hq * 128] bf16
+  const void* q;             // [T, >= hq * d] bf16
   int ld_q;
-  void* out;                 // [T, hq * 128] bf16
-  const void* images;
+  void* out;                 // [T, hq * d] bf16
+  const void* images;        // [tiles, hk, K and V, d / 64, 128 keys] rows of 128 bytes, swizzled
   const int32_t* first_tile; // [B] (stride ld_first): first row of each request's tiles
   int ld_first, tiles;       // tiles in images
   const int32_t* seq_lens;   // [B]
   const int32_t* cu_q;       // [B + 1]
-  int T, B, hq, hk, group;
+  int T, B, hq, hk, group, d;
   float scale;
   int ctas;                  // grid
   const int32_t* runs;       // [ctas, 8] (Kv4LoadArgs)
-  float* part_o;             // [ctas, 2, 256, 128] records of partial pieces
+  float* part_o;             // [ctas, 2, 256, d] records of partial pieces
   float* part_ml;            // [ctas, 2, 256, 2]
   int32_t* desc;             // [ctas, 4]
   int* err;

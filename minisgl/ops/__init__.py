@@ -897,7 +897,7 @@ def decode_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pag
     own. A request without keys gives zeros."""
     if kv_pool.is_cuda:
         _count(2)
-        return native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, None, 1, hq, hk, d,
+        return native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, None, hq, hk, d,
                                       page_size, scale, error_word(kv_pool.device))
     cu = torch.arange(req_rows.numel() + 1, dtype=torch.int32)
     return _attention_kv4_cpu("decode_attention_kv4", q, kv_pool, layer, page_table, req_rows, seq_lens, cu, hq, hk, d,
@@ -912,16 +912,24 @@ class KV4PrefillPlan(MlaPrefillPlan):
     PAGE = 128
 
 
-# query rows (tokens x heads of a group) of a request up to which the few-row
+# Query rows (tokens x heads of a group) of a request up to which the few-row
 # kernel, which expands codes for 8 rows at a time in registers, reads the
-# cache itself; beyond, keys are expanded once and a tcgen05 kernel takes over
-KV4_FEW_ROWS = 128
+# cache itself; beyond, keys are expanded once and a tcgen05 kernel takes over.
+# Its time grows with the rows, the other's hardly does. At 64 and 128 rows, few
+# rows against many in us: 20.6, 28.2 / 24.7, 25.2 (8 KV heads of 128 dims, one
+# request of 4096 keys), 70.9, 127 / 88.4, 88.7 (one of 32768), 74.1, 132 /
+# 89.3, 91.2 (8 of 4096), 48.0, 81.1 / 54.4, 55.9 (16 of 1024): they meet at 78
+# to 101 rows.
+KV4_FEW_ROWS = 80
 KV4_MAX_BATCH = 1280  # requests of one attention call over a 4-bit pool
 
 
-def kv4_prefill_expands(max_q: int, hq: int, hk: int, d: int) -> bool:
-    """Whether ``prefill_attention_kv4`` expands the keys first (and so takes a plan)."""
-    return d == 128 and max_q * (hq // max(1, hk)) > KV4_FEW_ROWS
+def kv4_prefill_expands(max_q: int, hq: int, hk: int) -> bool:
+    """Whether ``prefill_attention_kv4`` expands the keys first (and so takes a
+    plan): for more than KV4_FEW_ROWS query rows, where a group's heads fit a
+    tile of 128 rows."""
+    group = hq // max(1, hk)
+    return group <= 128 and max_q * group > KV4_FEW_ROWS
 
 
 def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, page_table: torch.Tensor,
@@ -932,18 +940,17 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
     query tokens of each request (cu_q [B + 1]; at most ``max_q`` each) over
     its cached and new keys. A query before the first key gives zeros.
 
-    Up to KV4_FEW_ROWS query rows per KV head (drafted tokens, short extends),
-    and for heads of other than 128 dims, the decode kernel reads the codes.
-    More rows: the keys (``plan``: their layout, made from seq_lens if None,
+    Up to KV4_FEW_ROWS query rows per KV head (drafted tokens, short extends)
+    the decode kernel reads the codes. More rows: the keys (``plan``: their layout, made from seq_lens if None,
     which waits for the GPU) are expanded to bf16 tiles, exactly, for a kernel
     on the tensor cores."""
     if not kv_pool.is_cuda:
         return _attention_kv4_cpu("prefill_attention_kv4", q, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq,
                                   hk, d, page_size, scale, out)
     err = error_word(kv_pool.device)
-    if not kv4_prefill_expands(max_q, hq, hk, d):
+    if not kv4_prefill_expands(max_q, hq, hk):
         _count(2)
-        return native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, max_q, hq, hk, d,
+        return native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq, hk, d,
                                       page_size, scale, err)
     if plan is None:
         plan = KV4PrefillPlan(seq_lens.tolist(), kv_pool.device)

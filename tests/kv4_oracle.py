@@ -55,9 +55,11 @@ def attention(q, packed, sf, layer, table, rows, lens, queries, hq, hk, scale):
     """(out, bound) float64 [T, hq, d] of causal attention; q [T, hq, d] as float64.
 
     Bound: the output's rounding to bf16 (2^-8 |out|), that of every weight p to bf16 (2^-8 of
-    sum p |v|), and the error of the scores, which weights take on twice (numerator and sum): a
-    group's sum of 32 products and its start at -136 sum(q) is two tensor-core sums of 16 + 1
-    terms no larger than 144 sum |q|, each kept to 2^-23, and four sums to 2^-24."""
+    sum p |v|), and the error of the scores, which weights take on twice (numerator and sum).
+    Few rows: a group's 32 products q c are two tensor-core sums of 16 + 1 terms no larger than
+    15 sum |q|, each kept to 2^-23, the offset of all groups, -8 s sum(q), one such sum, and
+    five more sums are kept to 2^-24: (2 * 17 * 15 + 17 * 8 + 5 * 23 / 2) 2^-23 s sum |q| = 704.
+    Many rows: 128 products q s (c - 8) in eight tensor-core sums, 8 * 17 * 8 = 1088. So 1100."""
     page = packed.shape[-2]
     k_all, v_all = values(packed[0, layer], sf[0, layer]), values(packed[1, layer], sf[1, layer])
     s_all = scales(sf[0, layer])
@@ -79,7 +81,7 @@ def attention(q, packed, sf, layer, table, rows, lens, queries, hq, hk, scale):
             o[i] = torch.einsum("hgl,lhd->hgd", p, v[:seen])
             a = torch.einsum("hgl,lhd->hgd", p, v[:seen].abs())
             reach = torch.einsum("hgx,lhx->hgl", qb[i].abs().reshape(hk, G, -1, 32).sum(-1), s[:seen])
-            es = (reach * 144 * scale * (2 * 17 * 2.0 ** -23 + 4 * 2.0 ** -24)).amax(-1, keepdim=True)
+            es = (reach * 1100 * 2.0 ** -23 * scale).amax(-1, keepdim=True)
             e[i] = 2.0 ** -8 * o[i].abs() + (2.0 ** -8 + 2.0 ** -20 + 2 * es) * a
         out.append(o.reshape(m, hq, q.shape[-1]))
         bound.append(e.reshape(m, hq, q.shape[-1]))

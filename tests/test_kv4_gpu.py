@@ -217,7 +217,7 @@ def test_decode_scores_that_rise():
 def test_extend_few_rows(d, page, hq, hk):
     lens, queries = [5, 70, 500, 129, 4, 9], [5, 3, 4, 1, 4, 2]
     if hq // hk * 5 > ops.KV4_FEW_ROWS:
-        lens, queries = lens[1:], [3, 2, 1, 4, 2]
+        lens, queries = lens[1:], [2, 2, 1, 2, 2]
     _check(*_attend(lens, queries, hq, hk, d, page, few=None))
 
 
@@ -227,19 +227,19 @@ def test_extend_with_more_queries_than_keys():
     assert (got[:2] == 0).all() and (got[5:7] == 0).all()
 
 
-def test_extend_d64_many_rows():
-    _check(*_attend([300, 41], [100, 41], 14, 2, 64, 32, few=None))
-
-
-@pytest.mark.parametrize("page", [16, 64, 256])
-@pytest.mark.parametrize("hq,hk", [(8, 8), (16, 2)])
-def test_extend_many_rows(page, hq, hk):
-    """The expanded path: its weights are rounded once more (scores of the tcgen05 kernel are
-    of q times scale log2 e rounded to bf16 in none of its forms that take aligned rows), so
-    the same bound with the tensor-core sums of 128 products."""
+@pytest.mark.parametrize("d,page", [(128, 16), (128, 64), (128, 256), (64, 32), (64, 128)])
+@pytest.mark.parametrize("hq,hk", [(8, 8), (16, 2), (14, 2)])
+def test_extend_many_rows(d, page, hq, hk):
+    """The expanded path. A quarter of its weights come from a polynomial that is off by 7.5e-5,
+    twice (numerator and sum), and its products keep n keys' sums to (17 / 16) n 2^-23, 1.6e-4 for
+    1300 keys: together 0.08 of the 2^-8 of the weights' rounding."""
     lens, queries = [700, 150, 260], [300, 150, 1]
-    got, want, bound = _attend(lens, queries, hq, hk, 128, page, few=None)
-    _check(got, want, 2 * bound)
+    got, want, bound = _attend(lens, queries, hq, hk, d, page, few=None)
+    _check(got, want, 1.1 * bound)
+
+
+def test_extend_of_more_heads_than_a_tile_has_rows():
+    _check(*_attend([40, 9], [3, 9], 130, 1, 64, 16, few=None))
 
 
 # ----------------------------------------------------------- graphs and streams
@@ -320,7 +320,7 @@ def test_used_together():
         packed, sf = unpack_kv4(pool.cpu(), page, d)
         want, bound = oracle.attention(qkv[:, :hq * d].double().cpu().view(n, hq, d), packed, sf, 1, table, rows.cpu(),
                                        [done], [n], hq, hk, d ** -0.5)
-        _check(got.view(n, hq, d), want, 2 * bound)
+        _check(got.view(n, hq, d), want, 1.1 * bound)
         if n == 3:  # the request moves to other pages, and its old ones are overwritten
             free = [p for p in range(pages) if p not in order.tolist()][:11]
             ops.copy_pages(pool, order, free)
@@ -438,6 +438,7 @@ def test_other_device_than_the_current_one():
 
 
 # ------------------------------------------------- many query rows: split work
+@pytest.mark.parametrize("d", [128, 64])
 @pytest.mark.parametrize("lens,queries,hq,hk", [
     ([1300], [200], 8, 1),                            # one request over many CTAs
     ([900, 0, 40, 2000, 5], [300, 0, 40, 33, 5], 14, 2),   # groups of 7, requests without tokens or keys
@@ -446,6 +447,6 @@ def test_other_device_than_the_current_one():
     ([500, 3, 700], [200, 9, 130], 40, 8),            # queries before the first key
     ([300], [300], 100, 1),                           # a group of 100 heads: tiles of one token
 ])
-def test_extend_many_rows_splits(lens, queries, hq, hk):
-    got, want, bound = _attend(lens, queries, hq, hk, 128, 64, few=None)
-    _check(got, want, 2 * bound)
+def test_extend_many_rows_splits(lens, queries, hq, hk, d):
+    got, want, bound = _attend(lens, queries, hq, hk, d, 64, few=None)
+    _check(got, want, 1.1 * bound)
