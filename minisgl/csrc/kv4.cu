@@ -315,7 +315,7 @@ __device__ void plan_runs(const Kv4LoadArgs& a, const ErrorSink& err) {
   for (int b = warp; b < a.B; b += 8) {
     const int q_len = kv4_query_tokens(a.cu_q, b, a.q_rows), keys = a.seq_lens[b];
     const int first = a.first_tile[static_cast<int64_t>(b) * a.ld_first] / kKv4TileKeys;
-    if (lane == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.q_rows || first < 0 || keys > a.ld_pt ||
+    if (lane == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.q_rows || a.cu_q[b + 1] < a.cu_q[b] || first < 0 || keys > a.ld_pt ||
                       (keys > 0 && first + (keys + kKv4TileKeys - 1) / kKv4TileKeys > a.T / kKv4TileKeys)))
       err.report(kErrBadIndex, 956);
     int sum = 0;
@@ -509,7 +509,7 @@ void launch_kv4_store(const Kv4StoreArgs& a, cudaStream_t s) {
 }
 
 void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s) {
-  const bool images = a.row_req != nullptr;
+  const bool images = a.runs != nullptr;  // (a plan without keys has no rows)
   if (a.T <= 0 && !images) return;
   if (a.d != 64 && a.d != 128) throw std::runtime_error("minisgl.load_kv4: head_dim must be 64 or 128");
   const int per_block = 256 / (a.d / 8);

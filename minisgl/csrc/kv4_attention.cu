@@ -206,7 +206,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
     if (blockIdx.x == 0 && (!row_ok || a.seq_lens[b] > a.ld_pt)) err.report(kErrBadIndex, row_ok ? 962 : 961);
     const int n = (rows_of<kSingle>(a, b) + kRows - 1) / kRows * a.hk;
     units[b + 1] = n, pre[b + 1] = n * (kUnitCost + key_tiles(keys));
-    if (!kSingle && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.T) && blockIdx.x == 0) err.report(kErrBadIndex, 964);
+    if (!kSingle && blockIdx.x == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.T || a.cu_q[b + 1] < a.cu_q[b]))
+      err.report(kErrBadIndex, 964);
   }
   __syncthreads();
   if (threadIdx.x < 64) {

@@ -227,8 +227,8 @@ struct Kv4StoreArgs {
 void launch_kv4_store(const Kv4StoreArgs& a, cudaStream_t s);
 struct Kv4LoadArgs {
   const uint8_t *k_pool, *v_pool;  // this layer's
-  const int32_t* slots;      // [T], or (row_req set) nullptr
-  void *k_out, *v_out;       // [T, hk, d] bf16, or (row_req set) k_out: images of the rows, 128 a tile
+  const int32_t* slots;      // [T], or (runs set) nullptr
+  void *k_out, *v_out;       // [T, hk, d] bf16, or (runs set) k_out: images of the rows, 128 a tile
   int T, hk, d, page_size, page_shift;
   int64_t kv_slots;
   // rows of a prefill plan: key row_pos[r] of request row_req[r] (-1: zeros)
@@ -236,7 +236,7 @@ struct Kv4LoadArgs {
   const int32_t* page_table;
   int ld_pt, pt_rows;
   const int32_t* req_rows;
-  // (row_req set) one more block splits the work of the attention that follows:
+  // (runs set) one more block splits the work of the attention that follows:
   // runs [ctas, 8]: request, pair of row tiles, KV head and key tile that a CTA
   // begins with; tiles of its run, the pair's place, all places, runs
   int32_t* runs;

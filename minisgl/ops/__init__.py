@@ -938,7 +938,8 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``prefill_attention`` over a 4-bit pool: causal attention of the last
     query tokens of each request (cu_q [B + 1]; at most ``max_q`` each) over
-    its cached and new keys. A query before the first key gives zeros.
+    its cached and new keys. A query before the first key gives zeros; rows
+    of ``out`` that no request has keep their values.
 
     Up to KV4_FEW_ROWS query rows per KV head (drafted tokens, short extends)
     the decode kernel reads the codes. More rows: the keys (``plan``: their layout, made from seq_lens if None,

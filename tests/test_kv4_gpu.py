@@ -242,6 +242,81 @@ def test_extend_of_more_heads_than_a_tile_has_rows():
     _check(*_attend([40, 9], [3, 9], 130, 1, 64, 16, few=None))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("queries", [[3, 1], [150, 20]], ids=["few", "many"])
+def test_extend_of_nothing(d, queries):
+    """No request has a key: zeros, by either path (the plan of the second has no rows)."""
+    got, _, _ = _attend([0, 0], queries, 4, 1, d, 16, few=None)
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("queries", [[2, 1], [90, 40]], ids=["few", "many"])
+def test_rows_behind_the_last_request(queries):
+    """Padded rows of q are read by nobody's product and their rows of out stay as they are."""
+    lens, hq, hk, d, page = [200, 130], 8, 4, 128, 64
+    packed, sf, pool, table, rows = oracle.make_cache(lens, hk, d, page)
+    n, T = sum(queries), sum(queries) + 37
+    q = torch.randn(T, hq * d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    q[n:] = float("nan")
+    out = torch.full((T, hq * d), 3.0, dtype=torch.bfloat16, device=DEV)
+    cu = torch.tensor([0, queries[0], n], dtype=torch.int32, device=DEV)
+    seq = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    got = ops.prefill_attention_kv4(q.to(DEV), pool.to(DEV), 1, table.to(DEV), rows.to(DEV), seq, cu, max(queries), hq,
+                                    hk, d, page, 0.1, out=out)
+    _done()
+    assert got is out and (out[n:] == 3).all()
+    want, bound = oracle.attention(q[:n].double().view(n, hq, d), packed, sf, 1, table, rows, lens, queries, hq, hk, 0.1)
+    _check(out[:n].view(n, hq, d), want, 1.1 * bound)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("queries", [[1, 3], [100, 30]], ids=["few", "many"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_queries_that_are_not_finite(bad, queries, d):
+    """Such a row is NaN, as by the formula; its neighbours in the same tiles are what they are."""
+    lens, hq, hk, page = [300, 150], 4, 2, 32
+    packed, sf, pool, table, rows = oracle.make_cache(lens, hk, d, page)
+    T = sum(queries)
+    q = torch.randn(T, hq * d, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    hit = torch.zeros(T, hq, dtype=torch.bool)
+    for t, h, at in ((0, 1, 5), (T - 1, 3, d - 1), (T - 2, 0, 33)):
+        q[t, h * d + at] = bad
+        hit[t, h] = True
+    cu = torch.tensor([0, queries[0], T], dtype=torch.int32, device=DEV)
+    seq = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    got = ops.prefill_attention_kv4(q.to(DEV), pool.to(DEV), 1, table.to(DEV), rows.to(DEV), seq, cu, max(queries), hq,
+                                    hk, d, page, d ** -0.5).view(T, hq, d)
+    _done()
+    assert got[hit.to(DEV)].isnan().all()
+    clean = q.double().view(T, hq, d).nan_to_num(0.0, 0.0, 0.0)
+    want, bound = oracle.attention(clean, packed, sf, 1, table, rows, lens, queries, hq, hk, d ** -0.5)
+    _check(got[~hit.to(DEV)], want[~hit], 1.1 * bound[~hit])
+
+
+def test_one_token_of_a_large_group_with_any_stride():
+    """A single row's stride says nothing, whatever it is."""
+    lens, hq, d, page = [77], 100, 128, 16
+    packed, sf, pool, table, rows = oracle.make_cache(lens, 1, d, page)
+    q = torch.randn(1, hq * d, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    seq, cu = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (lens, [0, 1]))
+    got = ops.prefill_attention_kv4(q.to(DEV).as_strided((1, hq * d), (1, 1)), pool.to(DEV), 1, table.to(DEV),
+                                    rows.to(DEV), seq, cu, 1, hq, 1, d, page, 0.1)
+    _done()
+    want, bound = oracle.attention(q.double().view(1, hq, d), packed, sf, 1, table, rows, lens, [1], hq, 1, 0.1)
+    _check(got.view(1, hq, d), want, 1.1 * bound)
+
+
+def test_offsets_of_queries_that_fall_are_reported():
+    pool, table, rows = (x.to(DEV) for x in oracle.make_cache([50, 40], 1, 128, 16)[2:])
+    q = torch.zeros(9, 4 * 128, dtype=torch.bfloat16, device=DEV)
+    seq = torch.tensor([50, 40], dtype=torch.int32, device=DEV)
+    for max_q in (9, 90):  # by either path
+        cu = torch.tensor([0, 9, 4], dtype=torch.int32, device=DEV)
+        ops.prefill_attention_kv4(q, pool, 1, table, rows, seq, cu, max_q, 4, 1, 128, 16, 0.1)
+        with pytest.raises(ops.DeviceIndexError):
+            _done()
+
+
 # ----------------------------------------------------------- graphs and streams
 def test_graph_replays_follow_their_buffers():
     lens, d, page, hq, hk = [700, 33, 260], 128, 16, 16, 2
@@ -272,6 +347,39 @@ def test_graph_replays_follow_their_buffers():
                                        d ** -0.5)
         for _, out in graphs:
             _check(out.view(3, hq, d), want, bound)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_graphs_replay_on_two_streams(d):
+    """The many-row path captured with its plan, twice, replayed at once with other queries."""
+    lens, queries, hq, hk, page = [400, 90], [130, 90], 8, 2, 64
+    packed, sf, pool, table, rows = oracle.make_cache(lens, hk, d, page, layers=1)
+    T = sum(queries)
+    dev = [x.to(DEV) for x in (pool, table, rows)]
+    seq, cu = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (lens, [0, 130, 220]))
+    q = torch.zeros(T, hq * d, dtype=torch.bfloat16, device=DEV)
+    plan = ops.KV4PrefillPlan(lens, torch.device(DEV))
+    run = lambda: ops.prefill_attention_kv4(q, *dev[:1], 0, *dev[1:], seq, cu, 130, hq, hk, d, page, d ** -0.5,  # noqa: E731
+                                            plan=plan)
+    run()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        graphs.append((graph, out))
+    for seed in range(2):
+        x = torch.randn(T, hq * d, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16)
+        q.copy_(x)
+        torch.cuda.synchronize()
+        for graph, _ in graphs:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                graph.replay()
+        _done()
+        want, bound = oracle.attention(x.double().view(T, hq, d), packed, sf, 0, table, rows, lens, queries, hq, hk,
+                                       d ** -0.5)
+        for _, out in graphs:
+            _check(out.view(T, hq, d), want, 1.1 * bound)
 
 
 def test_same_bits_every_time_and_on_another_stream():
