@@ -1504,7 +1504,8 @@ void kv4_store(const at::Tensor& k, const c10::optional<at::Tensor>& v, const c1
   if (fused) {
     const at::Tensor& out = q_out.has_value() ? *q_out : k;
     check_rows16(op, out, "q_out", hq * d, pool);
-    MSG_CHECK(out.size(0) == T, op, ": q_out must have ", T, " rows");
+    MSG_CHECK(out.size(0) == T && (T <= 1 || out.stride(0) >= hq * d), op, ": q_out must have ", T, " rows of their own");
+    MSG_CHECK(cos_sin.has_value(), op, ": cos_sin is needed");
     a.q = rows;
     a.ld_q = static_cast<int>(k.stride(0));
     a.q_out = out.data_ptr();

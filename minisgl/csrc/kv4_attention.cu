@@ -5,8 +5,8 @@
 //
 // with k_j and v_j in 4-bit codes, 136 bytes of cache per token and 128-dim
 // head. Bound by what a warp has to do per code, on the integer and half2 pipes:
-// 256 requests of up to 4096 keys and 8 KV heads take 140 us, 4.1 TB/s of codes
-// (63 % of the copy rate), one of 131072 keys 45 us. Everything is laid out to
+// 256 requests of up to 4096 keys and 8 KV heads take 139 us, 4.2 TB/s of codes
+// (64 % of the copy rate), one of 131072 keys 46 us. Everything is laid out to
 // keep that small:
 //
 // * The products are taken the other way round, S^T = K q^T and O^T = V^T P^T
@@ -21,8 +21,9 @@
 //   taken to fp16 by a power of two for each row, odd dims with 1/16 of it. The 8
 //   that codes are above their values is a product of its own: a group's scale
 //   with -8 sum(q) of its dims, in three bf16 parts. A group's scale multiplies
-//   its four sums. Against bf16 numbers 128 + c that start at -136 sum(q): 172
-//   for 173 us, and 8-bit floats, which the warp-level MMA converts first: 205.
+//   its four sums. (256 requests took 172 us at that stage; with bf16 numbers
+//   128 + c, whose exponents have to be set, 173; with 8-bit floats, which the
+//   warp-level MMA converts first, 205.)
 // * V: 128 + c has the bf16 bits 0x4300 | c, and s (128 + c) - 136 s is one packed
 //   fused multiply-add, exact in bf16.
 // * The running maximum moves only when a score exceeds it by 8 (in powers of
@@ -37,7 +38,7 @@
 // itself: 188.
 //
 // Work is split evenly whatever the lengths are: all key tiles of all requests,
-// heads and row tiles form one sequence, with a place more for each unit of them
+// heads and row tiles form one sequence, with two places more for each unit of them
 // (what a piece costs beside its tiles), of which each group of warps takes an
 // equal run. A run's first and last pieces may be parts of a longer one: those
 // write (m, l, O) records, which a second small kernel joins.
@@ -136,7 +137,10 @@ __device__ __forceinline__ int rows_of(const Kv4AttnArgs& a, int b) {
 __device__ __forceinline__ int keys_of(const Kv4AttnArgs& a, int b) { return min(max(a.seq_lens[b], 0), a.ld_pt); }
 __device__ __forceinline__ int key_tiles(int keys) { return max(1, (keys + kTile - 1) / kTile); }
 
-constexpr int kUnitCost = 1;  // what a unit (request, KV head, tile of query rows) costs beside its key tiles, in tiles
+// What a unit (request, KV head, tile of query rows) costs beside its key tiles, in
+// tiles. With 0, 1, 2, 3: 256 ragged requests 151, 140, 139, 143 us; 8 of five tokens
+// each 48.9, 42.4, 41.3, 41.8.
+constexpr int kUnitCost = 2;
 
 // A place in the work: request, unit of it (KV head x row tile) and key tile.
 struct Place {

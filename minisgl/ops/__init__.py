@@ -835,7 +835,7 @@ def rope_store_kv4(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Te
                    k_norm_w: Optional[torch.Tensor], kv_pool: torch.Tensor, layer: int, out_loc: torch.Tensor, hq: int,
                    hk: int, d: int, page_size: int, eps: float, q_out: Optional[torch.Tensor] = None) -> None:
     """``rope_store`` into a 4-bit pool: per-head RMS norms of q and k (None:
-    none), NeoX rotation of both, q heads to ``q_out`` [T, >= hq * d] (None: in
+    none), NeoX rotation of both (``cos_sin`` [max_pos, d]), q heads to ``q_out`` [T, >= hq * d] (None: in
     place in ``qkv``), k and v as codes to the slots ``out_loc``. The k and v
     columns of ``qkv`` keep their values. Norm and rotation are fp32 and
     rounded once, to q's type and to the codes."""
@@ -851,6 +851,10 @@ def rope_store_kv4(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Te
         raise ValueError(f"rope_store_kv4: qkv must be [T, >= {(hq + 2 * hk) * d}], got {tuple(qkv.shape)}")
     if positions.numel() != T or out_loc.numel() != T or q_out.shape[0] != T or q_out.shape[1] < hq * d:
         raise ValueError(f"rope_store_kv4: positions, out_loc and q_out must have {T} rows")
+    if T > 1 and q_out.stride(0) < hq * d:
+        raise ValueError("rope_store_kv4: the rows of q_out must be their own")
+    if cos_sin.dim() != 2 or cos_sin.shape[1] != d:
+        raise ValueError(f"rope_store_kv4: cos_sin must be [max_pos, {d}], got {tuple(cos_sin.shape)}")
     x = qkv[:, :(hq + 2 * hk) * d].reshape(T, hq + 2 * hk, d)
     cs = cos_sin[positions.long()]
     q = ref.norm_rope(x[:, :hq], q_norm_w, cs, eps)

@@ -137,6 +137,10 @@ def test_refusals_on_the_cpu():
         lambda: ops.load_kv4(pool, 0, i3 + 64, hk, d, page),
         lambda: ops.load_kv4(pool, -1, i3, hk, d, page),
         lambda: ops.rope_store_kv4(q, i3, oracle.cos_sin(8, d), None, None, pool, 0, i3, 4, hk, d, page, 1e-6),
+        lambda: ops.rope_store_kv4(torch.zeros(3, 8 * d), i3, oracle.cos_sin(8, 32), None, None, pool, 0, i3, 4, hk, d,
+                                   page, 1e-6),
+        lambda: ops.rope_store_kv4(torch.zeros(3, 8 * d), i3, oracle.cos_sin(8, d), None, None, pool, 0, i3, 4, hk, d,
+                                   page, 1e-6, q_out=q[:1].expand(3, -1)),
         lambda: ops.decode_attention_kv4(q, pool, 0, pt, i3, i3, 3, hk, d, page, 0.1),
         lambda: ops.decode_attention_kv4(q, pool, 0, pt, i3, i3, 4, hk, d, page, -0.1),
         lambda: ops.decode_attention_kv4(q, pool, 0, pt, i3, i3, 8, hk, d, page, 0.1),

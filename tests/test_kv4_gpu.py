@@ -482,6 +482,7 @@ def test_refusals():
     i3 = torch.zeros(3, dtype=torch.int32, device=DEV)
     pt = torch.zeros(3, 64, dtype=torch.int32, device=DEV)
     q = torch.zeros(3, 4 * d, dtype=torch.bfloat16, device=DEV)
+    wide = torch.zeros(3, 8 * d, dtype=torch.bfloat16, device=DEV)
     bad = [
         lambda: ops.store_kv4(x.float(), x, pool, 0, i3, hk, d, page),
         lambda: ops.store_kv4(x, x[:2], pool, 0, i3, hk, d, page),
@@ -498,6 +499,10 @@ def test_refusals():
         lambda: ops.rope_store_kv4(q, i3, oracle.cos_sin(8, d).to(DEV), x[0, :64], None, pool[:, :, :, :1].contiguous(),
                                    0, i3, 2, 1, d, page, 1e-6),
         lambda: ops.rope_store_kv4(q, i3, oracle.cos_sin(8, d).to(DEV), None, None, pool, 0, i3, 4, hk, d, page, 1e-6),
+        lambda: ops.rope_store_kv4(wide, i3, oracle.cos_sin(8, 64).to(DEV), None, None, pool, 0, i3, 4, hk, d, page, 1e-6),
+        lambda: ops.rope_store_kv4(wide, i3, None, None, None, pool, 0, i3, 4, hk, d, page, 1e-6),
+        lambda: ops.rope_store_kv4(wide, i3, oracle.cos_sin(8, d).to(DEV), None, None, pool, 0, i3, 4, hk, d, page, 1e-6,
+                                   q_out=q[:1].expand(3, -1)),
         lambda: ops.decode_attention_kv4(q, pool, 0, pt, i3, i3, 3, hk, d, page, 0.1),
         lambda: ops.decode_attention_kv4(q, pool, 0, pt, i3, i3, 4, hk, d, page, 0.0),
         lambda: ops.decode_attention_kv4(q, pool, 0, pt, i3, i3[:2], 4, hk, d, page, 0.1),
