@@ -9,6 +9,7 @@ falling back. CPU tensors run the fp32 PyTorch restatement in
 from __future__ import annotations
 
 import functools
+import operator
 from typing import List, Optional, Tuple
 
 import torch
@@ -998,7 +999,7 @@ def _page_list(pages) -> List[int]:
         if pages.is_cuda or pages.is_floating_point():
             raise ValueError("copy_pages: page numbers are host integers (a CPU tensor or ints)")
         return pages.reshape(-1).tolist()
-    return [int(p) for p in pages]
+    return [operator.index(p) for p in pages]
 
 
 # --------------------------------------------------------------- sampling

@@ -114,7 +114,7 @@ def test_copy_pages_on_the_cpu():
 
 @pytest.mark.parametrize("src,dst,error", [
     ([0], [9], IndexError), ([-1], [2], IndexError), ([0, 1], [2], ValueError), ([0, 1], [2, 2], ValueError),
-    ([0, 2], [2, 3], ValueError), ([3, 3], [3, 3], ValueError), (torch.tensor([1.0]), [2], ValueError)])
+    ([0, 2], [2, 3], ValueError), ([3, 3], [3, 3], ValueError), (torch.tensor([1.0]), [2], ValueError), ([0.5], [2], TypeError)])
 def test_copy_pages_refuses(src, dst, error):
     pool = torch.zeros(2, 3, 9, 2, 16, dtype=torch.uint8)
     with pytest.raises(error):

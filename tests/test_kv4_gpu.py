@@ -460,6 +460,25 @@ def test_copy_pages(shape, dtype, page_dim, n):
     assert torch.equal(dev.cpu(), want)
 
 
+@pytest.mark.parametrize("n", [2, 16, 17, 600])
+def test_copies_that_see_one_another_are_refused(n):
+    """Few pairs and many are looked over differently."""
+    pool = torch.randint(0, 256, (2, 1, 1300, 1, 16 * 68), dtype=torch.uint8, device=DEV)
+    before = pool.clone()
+    src, dst = list(range(n)), list(range(n, 2 * n))
+    for a, b in ((src, dst[:-1] + [dst[0]]), (src[:-1] + [dst[0]], dst), (src, dst[:-1] + [src[0]]), (src, dst[:-1] + [1300]),
+                 (src, dst[:-1] + [-1]), (src, dst[:-1])):
+        with pytest.raises((ValueError, IndexError)):
+            ops.copy_pages(pool, a, b)
+    _done()
+    assert torch.equal(pool, before)
+    ops.copy_pages(pool, tuple(src), torch.tensor(dst))
+    before[:, :, dst] = before[:, :, src]
+    assert torch.equal(pool, before)
+    ops.copy_pages(pool, dst, dst)  # onto themselves
+    assert torch.equal(pool, before)
+
+
 def test_copy_many_pages():
     """More pairs than one launch takes, a page copied to itself, none at all."""
     pool = torch.randint(0, 256, (2, 2, 2100, 1, 16 * 34), dtype=torch.uint8)
