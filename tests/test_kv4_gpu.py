@@ -238,6 +238,19 @@ def test_extend_many_rows(d, page, hq, hk):
     _check(got, want, 1.1 * bound)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("first", [1, 3, 100], ids=["one token", "few rows", "many rows"])
+def test_as_many_requests_as_a_call_takes(d, first):
+    lens = [130] + [1 + i % 20 for i in range(ops.KV4_MAX_BATCH - 1)]
+    got, want, bound = _attend(lens, [first] + [1] * (len(lens) - 1), 2, 2, d, 16)
+    _check(got, want, 1.1 * bound)
+    x = torch.zeros(len(lens) + 1, dtype=torch.int32, device=DEV)
+    pool = torch.zeros(2, 1, 1, 2, 16 * (d // 2 + d // 32), dtype=torch.uint8, device=DEV)
+    with pytest.raises(RuntimeError, match="at most"):
+        ops.decode_attention_kv4(torch.zeros(len(lens) + 1, 2 * d, dtype=torch.bfloat16, device=DEV), pool, 0,
+                                 x[:16].view(1, 16).contiguous(), x, x, 2, 2, d, 16, 0.1)
+
+
 def test_extend_of_more_heads_than_a_tile_has_rows():
     _check(*_attend([40, 9], [3, 9], 130, 1, 64, 16, few=None))
 
@@ -315,6 +328,40 @@ def test_offsets_of_queries_that_fall_are_reported():
         ops.prefill_attention_kv4(q, pool, 1, table, rows, seq, cu, max_q, 4, 1, 128, 16, 0.1)
         with pytest.raises(ops.DeviceIndexError):
             _done()
+
+
+def test_offsets_beyond_32_bits():
+    """The last pages of a layer of 4.5 GB: stored, read back, attended by both paths, copied."""
+    hk, hq, d, page, pages = 8, 16, 128, 64, 130000
+    pool = torch.zeros(2, 1, pages, hk, page * 68, dtype=torch.uint8, device=DEV)
+    n = 100
+    at = torch.arange(n, dtype=torch.int32, device=DEV)
+    slots = at + (pages - 2) * page
+    g = torch.Generator(device=DEV).manual_seed(0)
+    k, v = (torch.randn(n, hk * d, device=DEV, generator=g).to(torch.bfloat16) for _ in range(2))
+    ops.store_kv4(k, v, pool, 0, slots, hk, d, page)
+    got = [x.double().cpu() for x in ops.load_kv4(pool, 0, slots, hk, d, page)]
+    for x, y in zip((k, v), got):
+        c, byte = oracle.quantize(x.double().cpu().view(n, hk, d))
+        assert torch.equal(y, oracle.values(c[..., 0::2] | (c[..., 1::2] << 4), byte))
+    table = torch.zeros(1, 128, dtype=torch.int32, device=DEV)
+    table[0, :n] = slots
+    row, seq, cu = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0], [n], [0, n]))
+    q = torch.randn(n, hq * d, device=DEV, generator=g).to(torch.bfloat16)
+    one = ops.decode_attention_kv4(q[-1:], pool, 0, table, row, seq, hq, hk, d, page, 0.1)
+    many = ops.prefill_attention_kv4(q, pool, 0, table, row, seq, cu, n, hq, hk, d, page, 0.1)
+    _done()
+    kk, vv = (x.repeat_interleave(hq // hk, 1) for x in got)
+    sc = torch.einsum("qhd,khd->hqk", q.double().cpu().view(n, hq, d), kk) * 0.1
+    p = torch.softmax(sc.masked_fill(~torch.ones(n, n, dtype=torch.bool).tril(), float("-inf")), -1)
+    want, a = (torch.einsum("hqk,khd->qhd", p, x) for x in (vv, vv.abs()))
+    # the output's and the weights' rounding; scores of 128 products, below 2^-8 of the weights' rounding
+    bound = 2.0 ** -8 * want.abs() + 1.1 * 2.0 ** -8 * a
+    _check(many.view(n, hq, d), want, bound)
+    _check(one.view(1, hq, d), want[-1:], bound[-1:])
+    ops.copy_pages(pool, [pages - 2, pages - 1], [0, pages // 2])
+    back = ops.load_kv4(pool, 0, at[:64], hk, d, page)
+    assert all(torch.equal(x.double().cpu(), y[:64]) for x, y in zip(back, got))
 
 
 # ----------------------------------------------------------- graphs and streams
