@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import TYPE_CHECKING, Dict, List, Optional
+from typing import TYPE_CHECKING, Dict, List, NamedTuple, Optional, Sequence
 
 import torch
 
@@ -32,12 +32,28 @@ if TYPE_CHECKING:
 
 NUM_SMS = 148
 MAX_SPLITS = 16
+# keys that one prefill call over a 4-bit pool expands (512 bytes each per 128-dim
+# KV head: 1 GB at 8 heads): batches with more cached keys take several calls
+KV4_PLAN_KEYS = 1 << 18
 
 
 def decode_splits(batch_size: int, kv_heads: int) -> int:
     """Splits per (request, kv head) so that about two CTAs run per SM."""
     want = math.ceil(2 * NUM_SMS / max(1, batch_size * kv_heads))
     return max(1, min(MAX_SPLITS, want))
+
+
+class KV4Part(NamedTuple):
+    """Requests [first, last) of a prefill batch, their rows of q and the layout
+    of their keys (None: few rows, which need none)."""
+
+    first: int
+    last: int
+    q0: int
+    q1: int
+    cu_q: torch.Tensor
+    max_q: int
+    plan: Optional[ops.KV4PrefillPlan]
 
 
 @dataclass
@@ -48,7 +64,7 @@ class NativeAttnMetadata(BaseAttnMetadata):
     max_q: int
     max_splits: int
     last_indices: Optional[torch.Tensor] = None  # int64 [B] (prefill)
-    plan: Optional[ops.KV4PrefillPlan] = None    # 4-bit pools: the keys' layout (prefill of many rows)
+    parts: Sequence["KV4Part"] = ()              # 4-bit pools: prefill calls over requests in turn
 
     def get_last_indices(self, bs: int) -> torch.Tensor:
         if self.last_indices is None:  # decode: one token per request
@@ -94,8 +110,12 @@ class NativeAttnBackend(BaseAttnBackend):
             if batch.is_decode:
                 return ops.decode_attention_kv4(qkv, pool, layer_id, pt, md.req_rows, md.seq_lens, self.hq, self.hk,
                                                 self.d, self.page_size, self.scale)
-            return ops.prefill_attention_kv4(qkv, pool, layer_id, pt, md.req_rows, md.seq_lens, md.cu_q, md.max_q,
-                                             self.hq, self.hk, self.d, self.page_size, self.scale, md.plan)
+            out = torch.empty(qkv.shape[0], self.hq * self.d, dtype=qkv.dtype, device=qkv.device)
+            for p in md.parts:
+                ops.prefill_attention_kv4(qkv[p.q0 : p.q1], pool, layer_id, pt, md.req_rows[p.first : p.last],
+                                          md.seq_lens[p.first : p.last], p.cu_q, p.max_q, self.hq, self.hk, self.d,
+                                          self.page_size, self.scale, p.plan, out=out[p.q0 : p.q1])
+            return out
         if batch.is_decode:
             return ops.decode_attention(qkv, pool, layer_id, pt, md.req_rows, md.seq_lens, self.hq, self.hk, self.d,
                                         self.page_size, self.scale, self.part_o, self.part_lse, md.max_splits)
@@ -122,13 +142,25 @@ class NativeAttnBackend(BaseAttnBackend):
         host = torch.tensor(rows + lens + cu, dtype=torch.int32, pin_memory=on_gpu)
         dev = host.to(self.device, non_blocking=True)
         cu_q = dev[2 * B :]
-        plan = None
-        if self.kv4 and on_gpu and ops.kv4_prefill_expands(max(qlens), self.hq, self.hk):
-            plan = ops.KV4PrefillPlan(lens, self.device)
+        parts = self._kv4_parts(lens, qlens, cu, cu_q) if self.kv4 else ()
         batch.attn_metadata = NativeAttnMetadata(
             req_rows=dev[:B], seq_lens=dev[B : 2 * B], cu_q=cu_q, max_q=max(qlens), max_splits=1,
-            last_indices=(cu_q[1:] - 1).long(), plan=plan,
+            last_indices=(cu_q[1:] - 1).long(), parts=parts,
         )
+
+    def _kv4_parts(self, lens: List[int], qlens: List[int], cu: List[int], cu_q: torch.Tensor) -> List[KV4Part]:
+        parts, first, keys = [], 0, 0
+        for b in range(1, len(lens) + 1):
+            keys += lens[b - 1]
+            if b < len(lens) and keys + lens[b] <= KV4_PLAN_KEYS:
+                continue
+            max_q = max(qlens[first:b])
+            many = cu_q.is_cuda and ops.kv4_prefill_expands(max_q, self.hq, self.hk)
+            plan = ops.KV4PrefillPlan(lens[first:b], self.device) if many else None
+            parts.append(KV4Part(first, b, cu[first], cu[b], cu_q[first : b + 1] - cu[first] if first else cu_q[: b + 1],
+                                 max_q, plan))
+            first, keys = b, 0
+        return parts
 
     # ------------------------------------------------------------ CUDA graphs
     def init_capture_graph(self, max_seq_len: int, bs_list: List[int]) -> None:

@@ -58,6 +58,43 @@ def test_engine_follows_the_quantised_oracle(shape):
         llm.shutdown()
 
 
+def test_parts_of_a_prefill_batch(monkeypatch):
+    """Requests of a batch fall into calls of a bounded number of keys, in order, none left out."""
+    from minisgl.attention import native
+
+    backend = native.NativeAttnBackend.__new__(native.NativeAttnBackend)
+    backend.hq, backend.hk, backend.device = 8, 2, torch.device("cpu")
+    lens, qlens = [100, 250, 40, 10, 900, 5, 5], [30, 1, 40, 2, 7, 5, 1]
+    cu = [0]
+    for n in qlens:
+        cu.append(cu[-1] + n)
+    cu_q = torch.tensor(cu, dtype=torch.int32)
+    for limit, want in ((1 << 18, [(0, 7)]), (300, [(0, 1), (1, 4), (4, 5), (5, 7)]), (1, [(i, i + 1) for i in range(7)])):
+        monkeypatch.setattr(native, "KV4_PLAN_KEYS", limit)
+        parts = backend._kv4_parts(lens, qlens, cu, cu_q)
+        assert [(p.first, p.last) for p in parts] == want
+        for p in parts:
+            assert (p.q0, p.q1, p.max_q) == (cu[p.first], cu[p.last], max(qlens[p.first:p.last]))
+            assert p.cu_q.dtype == torch.int32 and p.cu_q.tolist() == [c - p.q0 for c in cu[p.first:p.last + 1]]
+
+
+def test_a_batch_in_parts_gives_the_same_tokens(monkeypatch):
+    from minisgl.attention import native
+
+    rng = random.Random(3)
+    prompts = [[rng.randrange(1024) for _ in range(rng.randint(1, 30))] for _ in range(6)]
+    outs = []
+    for limit in (native.KV4_PLAN_KEYS, 25):
+        monkeypatch.setattr(native, "KV4_PLAN_KEYS", limit)
+        llm = _make(max_extend_tokens=256)
+        try:
+            outs.append(llm.generate(prompts, SamplingParams(temperature=0.0, max_tokens=4, ignore_eos=True)))
+            for p, o in zip(prompts, outs[-1]):
+                _near_best(llm, p, o["token_ids"])
+        finally:
+            llm.shutdown()
+
+
 def test_pool_bytes_and_pages():
     """A page costs what its codes and scales take, and pages copy whole."""
     llm = _make()

@@ -18,6 +18,7 @@ import pytest
 import torch
 
 from minisgl import ops
+from minisgl.attention import native
 from minisgl.core import SamplingParams
 from minisgl.llm import LLM
 from minisgl.models.oracle import dense_logits
@@ -60,6 +61,26 @@ def test_engine_follows_the_quantised_oracle(page):
                     assert row[t] >= row.max() - 0.12 * row.abs().max(), (t, int(row.argmax()))
     finally:
         llm.shutdown()
+
+
+def test_batches_of_many_cached_keys_take_several_calls(monkeypatch):
+    """With a limit of 300 keys a call, prompts go through in parts, each token near the oracle's best."""
+    outs = []
+    for limit in (native.KV4_PLAN_KEYS, 300):
+        monkeypatch.setattr(native, "KV4_PLAN_KEYS", limit)
+        llm = _make(16, gemm_autotune=False, max_extend_tokens=2048)
+        try:
+            prompts = _prompts(12, 5)
+            outs.append([o["token_ids"] for o in llm.generate(prompts, SamplingParams(temperature=0.0, max_tokens=1,
+                                                                                      ignore_eos=True))])
+            ops.check_device_errors(torch.device("cuda:0"))
+            state, cfg = llm.engine.model.state_dict(), llm.engine.model_config
+            for p, (t,) in zip(prompts, outs[-1]):
+                row = dense_logits(state, cfg, p, fused_layout=llm.engine.model.fused_layout)[-1]
+                assert row[t] >= row.max() - 0.12 * row.abs().max()
+        finally:
+            llm.shutdown()
+    assert len(outs[0]) == len(outs[1]) == 12
 
 
 def test_graph_decode_equals_eager_decode():
