@@ -17,8 +17,9 @@
 // tile's products run. 128-key tiles: an MMA of 128 x 128 x 16 takes 64 cycles,
 // of 128 x 64 x 16 48 (measured), so 64-key tiles would leave a quarter unused.
 //
-// Weights are rounded to bf16 for the second product, their sums are of fp32
-// ones; a row's maximum is taken up to bf16, which does for a reference.
+// Weights are rounded to bf16 for the second product; their sums are of fp32
+// ones, and a row's maximum is fp32: it is taken off scores of any size, where a
+// rounding of its own would take the weights out of fp32's range.
 //
 // Work is split evenly: the key tiles of all row-tile pairs form one sequence, of
 // which each CTA (one an SM) takes an equal run; a pair whose tiles fall to
@@ -56,7 +57,7 @@ static_assert(kKeys == 128, "tiles of 128 keys");
 template <int kD>
 constexpr int image_bytes() { return kD / 64 * kHalf; }  // K or V of a tile (32 KB, 16 KB)
 template <int kD>
-constexpr int smem_bytes() { return 1024 + (2 + kSlots) * image_bytes<kD>() + 256 + 2 * 4 * 128 + kAhead * 48; }
+constexpr int smem_bytes() { return (2 + kSlots) * image_bytes<kD>() + 256 + 2 * 4 * 256 + kAhead * 48; }
 static_assert(smem_bytes<128>() <= 227 * 1024, "shared memory of a CTA");
 
 // Waits that sleep: a first try that may suspend the thread for 20 us leaves the
@@ -157,10 +158,9 @@ __device__ __forceinline__ int tiles_in(const Piece& p, int x) { return max(0, m
 template <int kD>
 __global__ void __launch_bounds__(kThreads, 1)
     kv4_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ Kv4PrefillArgs a) {
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   constexpr int kHalves = kD / 64;
   constexpr int kImage = image_bytes<kD>();
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = smem;  // [tile][64-dim half]
   uint8_t* sKV = sQ + 2 * kImage;
   uint64_t* full = reinterpret_cast<uint64_t*>(sKV + kSlots * kImage);  // [kSlots]
@@ -175,9 +175,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* d_empty = d_full + kAhead;                                  // [kAhead]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_empty + kAhead);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
-  uint8_t* s_swap = reinterpret_cast<uint8_t*>(full + 32);  // [2 tiles][4 quadrants][128 bytes]
-  Piece* s_piece = reinterpret_cast<Piece*>(s_swap + 2 * 4 * 128);  // [kAhead]
+  float* s_swap = reinterpret_cast<float*>(full + 32);          // [2 tiles][4 quadrants][2 halves][32 rows]
+  Piece* s_piece = reinterpret_cast<Piece*>(s_swap + 2 * 4 * 64);  // [kAhead]
   const ErrorSink err{a.err};
+  if ((smem_u32(smem) & 1023) != 0) {  // the swizzled tiles' alignment, as declared: nothing runs without it
+    pdl_wait();
+    if (threadIdx.x == 0) {
+      err.report(kErrBadIndex, 285);
+      reinterpret_cast<int4*>(a.desc)[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    }
+    return;
+  }
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
   const int G = a.group, TT = kRows / G;  // tokens of a row tile
 
@@ -365,14 +373,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------- softmax ----
     // Two warps a quadrant of 32 rows, 64 keys of a tile each; a row's two threads
     // swap their maxima, which also tells that both have read their scores before
-    // weights are written over them.
+    // weights are written over them. (Neither is at the next tile's maximum before
+    // the other has read this one's: its scores come after products of both threads'
+    // weights.)
     const int x = warp >> 3, part = (warp >> 2) & 1, quad = warp & 3;
     const int r = 32 * quad + lane;  // this thread's row (TMEM lane)
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * quad) << 16);
     const uint32_t s_col = lane_base + kSCol + 128 * x, o_col = lane_base + 128 * x + kD / 2 * part;
-    uint8_t* swap = s_swap + (4 * x + quad) * 128;
-    __nv_bfloat16* mine = reinterpret_cast<__nv_bfloat16*>(swap) + 32 * part + lane;
-    const __nv_bfloat16* other = reinterpret_cast<const __nv_bfloat16*>(swap) + 32 * (1 - part) + lane;
+    volatile float* mine = s_swap + ((4 * x + quad) * 2 + part) * 32 + lane;
+    const volatile float* other = s_swap + ((4 * x + quad) * 2 + 1 - part) * 32 + lane;
     auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * x + quad) : "memory"); };
     const float c = a.scale * kLog2e;
     bool ok = true;
@@ -393,7 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_32x32b_x32(s_col + 64 * part + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(sv + 32 * q));
         tc_wait_ld();
         const int lim = see - (p.kt0 + j) * kKeys - 64 * part;
-        if (__any_sync(0xffffffffu, lim < 64)) {
+        const bool cut = __any_sync(0xffffffffu, lim < 64);  // some row does not see all of the tile
+        if (cut) {
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             if (i >= lim) sv[i] = __float_as_uint(-INFINITY);
@@ -407,11 +417,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int q = 0; q < 4; ++q)
             m4[q] = max3(m4[q], __uint_as_float(sv[i + 2 * q]), __uint_as_float(sv[i + 2 * q + 1]));
         }
-        // to bf16, which does for a reference that both share
-        const __nv_bfloat16 top = __float2bfloat16_rn(max3(m4[0], m4[1], fmaxf(m4[2], m4[3])) * c);
+        const float top = max3(m4[0], m4[1], fmaxf(m4[2], m4[3])) * c;
         *mine = top;
         pair_sync();
-        const float mt = fmaxf(__bfloat162float(top), __bfloat162float(*other));
+        const float mt = fmaxf(top, *other);
         const bool grow = mt > m + kRescale;
         float alpha = 1.f;
         if (grow) {
@@ -446,6 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             float lo, hi;
             if ((i % 8) < kPolyPairs) {
               exp2_poly_pair(x2, lo, hi);
+              // its least weight is 2^-126; a hidden key's is 0
+              if (cut) lo = 2 * i < lim ? lo : 0.f, hi = 2 * i + 1 < lim ? hi : 0.f;
             } else {
               float y0, y1;
               f2_unpack(x2, y0, y1);
@@ -467,14 +478,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------------------------------------------------- epilogue ----
       if (ok && nx > 0) ok = __all_sync(0xffffffffu, wait_asleep(&o_done[x], (done - 1) & 1, err, 278, s_abort));
       tc_fence_after();
-      if (see <= p.kt0 * kKeys) m = -INFINITY, l = 0.f;  // a row without keys here (masked weights are 2^-126, not 0)
       // the row's sum over both halves of the keys
       pair_sync();
-      if (part == 1) reinterpret_cast<float*>(swap)[lane] = l;
+      *mine = l;
       pair_sync();
-      if (part == 0) reinterpret_cast<float*>(swap)[lane] = l += reinterpret_cast<const float*>(swap)[lane];
-      pair_sync();
-      if (part == 1) l = reinterpret_cast<const float*>(swap)[lane];
+      l += *other;
       pair_sync();
       uint32_t ov[kD / 2] = {};
       if (ok && nx > 0) {
