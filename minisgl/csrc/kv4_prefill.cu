@@ -152,6 +152,18 @@ __device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
   swap_vec(v[0], v[2], 2, lane & 2), swap_vec(v[1], v[3], 2, lane & 2);
 }
 
+// Maxima that keep a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Tiles of row tile x in the piece.
 __device__ __forceinline__ int tiles_in(const Piece& p, int x) { return max(0, min(p.kt1, x == 0 ? p.n0 : p.n1) - p.kt0); }
 
@@ -410,18 +422,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float m4[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) m4[q] = fmaxf(__uint_as_float(sv[2 * q]), __uint_as_float(sv[2 * q + 1]));
+        for (int q = 0; q < 4; ++q) m4[q] = max_nan(__uint_as_float(sv[2 * q]), __uint_as_float(sv[2 * q + 1]));
 #pragma unroll
         for (int i = 8; i < 64; i += 8) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            m4[q] = max3(m4[q], __uint_as_float(sv[i + 2 * q]), __uint_as_float(sv[i + 2 * q + 1]));
+            m4[q] = max3_nan(m4[q], __uint_as_float(sv[i + 2 * q]), __uint_as_float(sv[i + 2 * q + 1]));
         }
-        const float top = max3(m4[0], m4[1], fmaxf(m4[2], m4[3])) * c;
+        const float top = max3_nan(m4[0], m4[1], max_nan(m4[2], m4[3])) * c;
         *mine = top;
         pair_sync();
-        const float mt = fmaxf(top, *other);
-        const bool grow = mt > m + kRescale;
+        float mt = max_nan(top, *other);
+        // scores that are not finite (queries are not) make the row NaN, as in the formula;
+        // the weights alone would not: the polynomial takes NaN for its least argument
+        if (lim + 64 * part > 0 && !(fabsf(mt) < INFINITY)) mt = NAN;
+        const bool grow = !(mt <= m + kRescale);
         float alpha = 1.f;
         if (grow) {
           alpha = ex2_fast(m - mt);  // 0 on the first tile (m = -inf)

@@ -1,5 +1,5 @@
-"""Attention over the 4-bit KV cache at scores that are large, or rise or fall along the keys, by the
-few-row and the many-row path.
+"""Attention over the 4-bit KV cache at scores that are large, rise or fall along the keys, or are not
+finite, by the few-row and the many-row path.
 
 Scores here are exact: queries are integers, codes are integers, scales and the softmax scale are powers of
 two, and every sum of products keeps to 24 bits. So the only errors are those of the output's rounding and of
@@ -107,3 +107,23 @@ def test_scores_that_rise_and_fall(lens, queries, hq, hk, d, way, base):
     case[0][..., :32] = base
     got = _run(*case, lens, queries, 64, hq, hk, d)
     _check(got, *_want(*case, lens, queries, hq, hk, 64))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("queries", [[150, 90], [2, 1]], ids=["many", "few"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_first_tokens_that_are_not_finite(bad, queries, d):
+    """A prompt's first tokens see one to six keys; with a query that is not finite their rows are NaN, as by
+    the formula, and the rows beside them are what they are."""
+    hq, hk, page = 4, 2, 16
+    case = _case(queries, queries, hq, hk, d, page, lambda at, n: torch.full((n,), 1))
+    q = case[0]
+    want, bound = _want(*case, queries, queries, hq, hk, page)
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool)
+    for t, h, at in ((0, 0, 0), (0, 3, 40), (1, 1, 9), (2, 2, 33), (4, 0, 1), (5, 1, d - 1), (queries[0], 2, 3)):
+        if t < q.shape[0]:
+            q[t, h, at] = bad
+            hit[t, h] = True
+    got = _run(*case, queries, queries, page, hq, hk, d)
+    assert got[hit.to(DEV)].isnan().all()
+    _check(got[~hit.to(DEV)], want[~hit], bound[~hit])
