@@ -394,19 +394,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_col = lane_base + kSCol + 128 * x, o_col = lane_base + 128 * x + kD / 2 * part;
     volatile float* mine = s_swap + ((4 * x + quad) * 2 + part) * 32 + lane;
     const volatile float* other = s_swap + ((4 * x + quad) * 2 + 1 - part) * 32 + lane;
+    // Meetings of the two warps have no time limit, so both come to as many whichever
+    // wait runs out for one of them: they go on to a piece together or not at all, and
+    // a failed wait (ok) leaves out later waits, never a tile or a meeting.
     auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * x + quad) : "memory"); };
+    auto agree = [&](bool yes) {  // a meeting that tells whether every lane of both says so
+      uint32_t both;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(both)
+          : "r"(static_cast<uint32_t>(yes)), "r"(1 + 4 * x + quad)
+          : "memory");
+      return both != 0;
+    };
     const float c = a.scale * kLog2e;
     bool ok = true;
     int done = 0;
-    for (int k = 0; ok && __all_sync(0xffffffffu, describe(k)); ++k) {
+    for (int k = 0; agree(ok && __all_sync(0xffffffffu, describe(k))); ++k) {
       if (lane == 0) mbar_arrive(&d_empty[k % kAhead]);
       const int t = p.tok0 + x * TT + r / G;
       const bool live = r < TT * G && t < p.q_len;
       const int see = live ? p.keys - p.q_len + t + 1 : 1 << 30;  // keys that this row sees
       const int nx = tiles_in(p, x);
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; ok && j < nx; ++j, ++done) {
-        ok = __all_sync(0xffffffffu, wait_asleep(&s_full[x], done & 1, err, 277, s_abort));
+      for (int j = 0; j < nx; ++j, ++done) {
+        if (ok) ok = __all_sync(0xffffffffu, wait_asleep(&s_full[x], done & 1, err, 277, s_abort));
         tc_fence_after();
         uint32_t sv[64];
 #pragma unroll
@@ -498,7 +510,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       *mine = l;
       pair_sync();
       l += *other;
-      pair_sync();
       uint32_t ov[kD / 2] = {};
       if (ok && nx > 0) {
 #pragma unroll
