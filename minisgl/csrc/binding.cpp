@@ -1648,6 +1648,7 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
   a.first_tile = plan_table.data_ptr<int32_t>();
   a.ld_first = static_cast<int>(plan_table.size(1));
   a.tiles = static_cast<int>(R / minisgl::kKv4TileKeys);
+  a.ld_pt = l.ld_pt;
   a.seq_lens = seq_lens.data_ptr<int32_t>();
   a.cu_q = cu_q.data_ptr<int32_t>();
   a.T = static_cast<int>(T);

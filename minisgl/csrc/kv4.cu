@@ -309,13 +309,13 @@ __device__ void plan_runs(const Kv4LoadArgs& a, const ErrorSink& err) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int W = 2 * (kKv4TileKeys / a.group);  // tokens of a pair
   auto tiles = [&](int b, int q_len, int pair) {
-    const int keys = a.seq_lens[b];
+    const int keys = kv4_keys(a.seq_lens, b, a.ld_pt);
     return max(1, (keys - q_len + min(q_len, (pair + 1) * W) + kKv4TileKeys - 1) / kKv4TileKeys);
   };
   for (int b = warp; b < a.B; b += 8) {
-    const int q_len = kv4_query_tokens(a.cu_q, b, a.q_rows), keys = a.seq_lens[b];
+    const int q_len = kv4_query_tokens(a.cu_q, b, a.q_rows), keys = kv4_keys(a.seq_lens, b, a.ld_pt);
     const int first = a.first_tile[static_cast<int64_t>(b) * a.ld_first] / kKv4TileKeys;
-    if (lane == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.q_rows || a.cu_q[b + 1] < a.cu_q[b] || first < 0 || keys > a.ld_pt ||
+    if (lane == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.q_rows || a.cu_q[b + 1] < a.cu_q[b] || first < 0 || a.seq_lens[b] > a.ld_pt ||
                       (keys > 0 && first + (keys + kKv4TileKeys - 1) / kKv4TileKeys > a.T / kKv4TileKeys)))
       err.report(kErrBadIndex, 956);
     int sum = 0;

@@ -40,5 +40,7 @@ __device__ __forceinline__ int kv4_query_tokens(const int32_t* cu_q, int b, int 
   const int from = cu_q[b], to = cu_q[b + 1];
   return from >= 0 && to <= T && to > from ? to - from : 0;
 }
+// Keys of request b, of no more positions than the page table has.
+__device__ __forceinline__ int kv4_keys(const int32_t* seq_lens, int b, int ld_pt) { return min(max(seq_lens[b], 0), ld_pt); }
 
 }  // namespace minisgl

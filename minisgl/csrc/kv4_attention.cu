@@ -134,7 +134,6 @@ template <bool kSingle>
 __device__ __forceinline__ int rows_of(const Kv4AttnArgs& a, int b) {
   return kSingle ? a.group : kv4_query_tokens(a.cu_q, b, a.T) * a.group;
 }
-__device__ __forceinline__ int keys_of(const Kv4AttnArgs& a, int b) { return min(max(a.seq_lens[b], 0), a.ld_pt); }
 __device__ __forceinline__ int key_tiles(int keys) { return max(1, (keys + kTile - 1) / kTile); }
 
 // What a unit (request, KV head, tile of query rows) costs beside its key tiles, in
@@ -202,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
   }
   pdl_wait();
   for (int b = threadIdx.x; b < a.B; b += kThreads) {
-    const int keys = keys_of(a, b);
+    const int keys = kv4_keys(a.seq_lens, b, a.ld_pt);
     len[b] = keys;
     const int row = a.req_rows[b];
     const bool row_ok = row >= 0 && row < a.pt_rows;

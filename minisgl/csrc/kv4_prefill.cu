@@ -101,11 +101,11 @@ struct Walk {
   int64_t at;  // place of the pair in the sequence that is split (kPairCost, then its tiles)
   int first;   // of the piece: image tile of the request's key 0
   __device__ __forceinline__ bool next(const Kv4PrefillArgs& a, Piece& p) {
-    if (left <= 0) return false;
+    if (left <= 0 || b >= a.B) return false;
     const int TT = kRows / a.group;
     p.h = h;
     p.q_begin = a.cu_q[b], p.q_len = kv4_query_tokens(a.cu_q, b, a.T);
-    p.keys = a.seq_lens[b];
+    p.keys = kv4_keys(a.seq_lens, b, a.ld_pt);
     first = a.first_tile[static_cast<int64_t>(b) * a.ld_first] / kKeys;
     p.tok0 = pair * 2 * TT;
     const int cached = p.keys - p.q_len;
@@ -130,7 +130,7 @@ struct Walk {
         h = 0, ++pair;
         if (pair * 2 * TT >= p.q_len && left > 0) {
           pair = 0, ++b;
-          while (kv4_query_tokens(a.cu_q, b, a.T) == 0) ++b;  // there is more to do, so there is one
+          while (b < a.B && kv4_query_tokens(a.cu_q, b, a.T) == 0) ++b;  // there is more to do, so there is one
         }
       }
     }

@@ -282,6 +282,7 @@ struct Kv4PrefillArgs {
   const int32_t* first_tile; // [B] (stride ld_first): first row of each request's tiles
   int ld_first, tiles;       // tiles in images
   const int32_t* seq_lens;   // [B]
+  int ld_pt;                 // positions of the page table: no request has more keys
   const int32_t* cu_q;       // [B + 1]
   int T, B, hq, hk, group, d;
   float scale;

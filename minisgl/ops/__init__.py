@@ -944,7 +944,8 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
     """``prefill_attention`` over a 4-bit pool: causal attention of the last
     query tokens of each request (cu_q [B + 1]; at most ``max_q`` each) over
     its cached and new keys. A query before the first key gives zeros; rows
-    of ``out`` that no request has keep their values.
+    of ``out`` that no request has keep their values. A length beyond the
+    page table is reported and cut to it.
 
     Up to KV4_FEW_ROWS query rows per KV head (drafted tokens, short extends)
     the decode kernel reads the codes. More rows: the keys (``plan``: their layout, made from seq_lens if None,
@@ -959,7 +960,10 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
         return native().kv4_attention(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq, hk, d,
                                       page_size, scale, err)
     if plan is None:
-        plan = KV4PrefillPlan(seq_lens.tolist(), kv_pool.device)
+        lens = seq_lens.tolist()
+        if max(lens, default=0) > page_table.shape[-1]:
+            raise ValueError(f"prefill_attention_kv4: {max(lens)} keys in a page table of {page_table.shape[-1]} positions")
+        plan = KV4PrefillPlan(lens, kv_pool.device)
     _count(3)
     return native().kv4_prefill(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq, hk, d, page_size,
                                 scale, plan.page_table, plan.row_req, plan.row_pos, err)

@@ -1,0 +1,81 @@
+"""Lengths, offsets and plans on the device that the host cannot check: attention over the 4-bit KV cache reports
+them and reads nothing outside its tensors."""
+
+import pytest
+import torch
+
+from minisgl import ops
+
+import kv4_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _done():
+    torch.cuda.synchronize()
+    ops.check_device_errors(torch.device(DEV))
+
+
+def _reported():
+    with pytest.raises(ops.DeviceIndexError):
+        _done()
+
+
+class _Batch:
+    """Requests of `lens` keys and `queries` tokens, and what attention over them gives."""
+
+    def __init__(self, lens, queries, hq=8, hk=2, d=128, page=16):
+        self.lens, self.queries, self.heads = lens, queries, (hq, hk, d, page)
+        self.packed, self.sf, pool, table, rows = oracle.make_cache(lens, hk, d, page, layers=1)
+        self.table, self.rows = table, rows
+        self.pool, self.pt, self.rr = pool.to(DEV), table.to(DEV), rows.to(DEV)
+        self.cu = [0]
+        for n in queries:
+            self.cu.append(self.cu[-1] + n)
+        self.q = torch.randn(self.cu[-1], hq * d, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16)
+
+    def run(self, lens=None, cu=None, plan=None, out=None):
+        hq, hk, d, page = self.heads
+        seq = torch.tensor(self.lens if lens is None else lens, dtype=torch.int32, device=DEV)
+        cu = torch.tensor(self.cu if cu is None else cu, dtype=torch.int32, device=DEV)
+        return ops.prefill_attention_kv4(self.q.to(DEV), self.pool, 0, self.pt, self.rr, seq, cu, max(self.queries), hq,
+                                         hk, d, page, d ** -0.5, plan=plan, out=out).view(-1, hq, d)
+
+    def check(self, got, request, lens=None):
+        """The rows of one request, with as many keys as `lens` says."""
+        hq, hk, d, _ = self.heads
+        lo, hi = self.cu[request], self.cu[request + 1]
+        n = (lens or self.lens)[request]
+        want, bound = oracle.attention(self.q[lo:hi].double().view(-1, hq, d), self.packed, self.sf, 0, self.table,
+                                       self.rows[request:request + 1], [n], [hi - lo], hq, hk, d ** -0.5)
+        assert ((got[lo:hi].double().cpu() - want).abs() <= 1.1 * bound + 1e-30).all()
+
+
+@pytest.mark.parametrize("queries", [[150, 90, 30], [3, 2, 1]], ids=["many", "few"])
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 100000])
+def test_lengths_beyond_the_table(queries, length):
+    batch = _Batch([300, 200, 90], queries)
+    for at in range(3):
+        lens = list(batch.lens)
+        lens[at] = length
+        plan = ops.KV4PrefillPlan(batch.lens, torch.device(DEV)) if queries[0] > 3 else None
+        got = batch.run(lens, plan=plan)
+        _reported()
+        for other in range(3):
+            if other != at:
+                batch.check(got, other)
+    if queries[0] > 3:  # the host makes no plan of such lengths
+        with pytest.raises(ValueError, match="positions"):
+            batch.run(lens)
+
+
+@pytest.mark.parametrize("queries", [[150, 90, 30], [3, 2, 1]], ids=["many", "few"])
+def test_negative_lengths_are_no_keys(queries):
+    batch = _Batch([300, 200, 90], queries)
+    plan = ops.KV4PrefillPlan(batch.lens, torch.device(DEV)) if queries[0] > 3 else None
+    for length in (-1, -2 ** 31):
+        got = batch.run([300, length, 90], plan=plan)
+        _done()
+        assert (got[batch.cu[1]:batch.cu[2]] == 0).all()
+        batch.check(got, 0), batch.check(got, 2)
