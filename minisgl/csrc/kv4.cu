@@ -312,8 +312,10 @@ __device__ void plan_runs(const Kv4LoadArgs& a, const ErrorSink& err) {
     const int keys = kv4_keys(a.seq_lens, b, a.ld_pt);
     return max(1, (keys - q_len + min(q_len, (pair + 1) * W) + kKv4TileKeys - 1) / kKv4TileKeys);
   };
+  bool falls = false;
   for (int b = warp; b < a.B; b += 8) {
     const int q_len = kv4_query_tokens(a.cu_q, b, a.q_rows), keys = kv4_keys(a.seq_lens, b, a.ld_pt);
+    falls = falls || kv4_offsets_fall(a.cu_q, b);
     const int first = a.first_tile[static_cast<int64_t>(b) * a.ld_first] / kKv4TileKeys;
     if (lane == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.q_rows || a.cu_q[b + 1] < a.cu_q[b] || first < 0 || a.seq_lens[b] > a.ld_pt ||
                       (keys > 0 && first + (keys + kKv4TileKeys - 1) / kKv4TileKeys > a.T / kKv4TileKeys)))
@@ -324,7 +326,7 @@ __device__ void plan_runs(const Kv4LoadArgs& a, const ErrorSink& err) {
     for (int o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) pre[b + 1] = sum * a.hk, units[b + 1] = (q_len + W - 1) / W * a.hk;
   }
-  __syncthreads();
+  const bool none = __syncthreads_or(falls) != 0;
   if (warp < 2) {
     int* x = warp == 0 ? pre : units;
     int carry = 0;
@@ -341,7 +343,7 @@ __device__ void plan_runs(const Kv4LoadArgs& a, const ErrorSink& err) {
     if (lane == 0) x[0] = 0;
   }
   __syncthreads();
-  const int64_t total = pre[a.B];
+  const int64_t total = none ? 0 : pre[a.B];
   const int n = static_cast<int>(min(static_cast<int64_t>(a.ctas), max(total / 4, static_cast<int64_t>(1))));
   struct Place {
     int b, pair, h, kt, at, real;  // at: of the pair; real: tiles before

@@ -40,6 +40,9 @@ __device__ __forceinline__ int kv4_query_tokens(const int32_t* cu_q, int b, int 
   const int from = cu_q[b], to = cu_q[b + 1];
   return from >= 0 && to <= T && to > from ? to - from : 0;
 }
+// Whether request b's offsets fall. One that does leaves the whole call without work:
+// rows counted twice would take the sums of tiles out of 32 bits.
+__device__ __forceinline__ bool kv4_offsets_fall(const int32_t* cu_q, int b) { return cu_q[b + 1] < cu_q[b]; }
 // Keys of request b, of no more positions than the page table has.
 __device__ __forceinline__ int kv4_keys(const int32_t* seq_lens, int b, int ld_pt) { return min(max(seq_lens[b], 0), ld_pt); }
 

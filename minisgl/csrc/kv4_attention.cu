@@ -200,8 +200,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
     fence_barrier_init();
   }
   pdl_wait();
+  bool falls = false;
   for (int b = threadIdx.x; b < a.B; b += kThreads) {
     const int keys = kv4_keys(a.seq_lens, b, a.ld_pt);
+    if constexpr (!kSingle) falls = falls || kv4_offsets_fall(a.cu_q, b);
     len[b] = keys;
     const int row = a.req_rows[b];
     const bool row_ok = row >= 0 && row < a.pt_rows;
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
     if (!kSingle && blockIdx.x == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.T || a.cu_q[b + 1] < a.cu_q[b]))
       err.report(kErrBadIndex, 964);
   }
-  __syncthreads();
+  const bool none = __syncthreads_or(falls) != 0;
   if (threadIdx.x < 64) {
     int* x = threadIdx.x < 32 ? pre : units;
     int carry = 0;
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const __grid_cons
   // equal runs for the groups of all CTAs (CTA by CTA in the last place, so that
   // few runs use every SM). Each has a place at least, so the runs that a unit's
   // tiles span all have some of them, and their records are all written.
-  const int total = pre[a.B];
+  const int total = none ? 0 : pre[a.B];
   const int n = max(1, min(kGroups * static_cast<int>(gridDim.x), total)), me = group * gridDim.x + blockIdx.x;
   const int each = total / n, more = total - each * n;  // places of a run; the runs share `more` others
   auto start_of = [&](int i) { return each * i + more * i / n; };  // of run i: total i / n without 64 bits

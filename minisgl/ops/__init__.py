@@ -944,8 +944,9 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
     """``prefill_attention`` over a 4-bit pool: causal attention of the last
     query tokens of each request (cu_q [B + 1]; at most ``max_q`` each) over
     its cached and new keys. A query before the first key gives zeros; rows
-    of ``out`` that no request has keep their values. A length beyond the
-    page table is reported and cut to it.
+    of ``out`` that no request has keep their values. Offsets that fall are
+    reported and nothing is computed; a length beyond the page table is
+    reported and cut to it.
 
     Up to KV4_FEW_ROWS query rows per KV head (drafted tokens, short extends)
     the decode kernel reads the codes. More rows: the keys (``plan``: their layout, made from seq_lens if None,

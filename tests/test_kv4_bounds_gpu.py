@@ -79,3 +79,20 @@ def test_negative_lengths_are_no_keys(queries):
         _done()
         assert (got[batch.cu[1]:batch.cu[2]] == 0).all()
         batch.check(got, 0), batch.check(got, 2)
+
+
+@pytest.mark.parametrize("queries", [[150, 90, 30], [3, 2, 1]], ids=["many", "few"])
+def test_offsets_that_fall_leave_no_work(queries):
+    """Rows of several requests at once would add up to more tiles than a call counts."""
+    batch = _Batch([300, 200, 90], queries)
+    T = batch.cu[-1]
+    plan = ops.KV4PrefillPlan(batch.lens, torch.device(DEV)) if queries[0] > 3 else None
+    for cu in ([0, T, 0, T], [0, T, T - 1, T], [0, 2, T, -4]):
+        out = torch.full((T, 8 * 128), 3.0, dtype=torch.bfloat16, device=DEV)
+        batch.run(cu=cu, plan=plan, out=out)
+        _reported()
+        assert (out == 3).all()
+    got = batch.run(plan=plan)
+    _done()
+    for request in range(3):
+        batch.check(got, request)
