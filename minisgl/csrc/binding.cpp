@@ -1607,9 +1607,9 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
             ": too many tiles of work");
   if (B == 0 || T == 0) return out;
   const int ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  // records of partial pieces, then runs and descriptors
+  // records of partial pieces, then runs, descriptors and where requests begin
   const int64_t part = static_cast<int64_t>(ctas) * 2 * 256;
-  at::Tensor work = at::detail::empty_cuda({part * (d + 2) + 12 * ctas}, at::kFloat, pool.device(), c10::nullopt);
+  at::Tensor work = at::detail::empty_cuda({part * (d + 2) + 12 * ctas + B}, at::kFloat, pool.device(), c10::nullopt);
   float* w = work.data_ptr<float>();
   int32_t* runs = reinterpret_cast<int32_t*>(w + part * (d + 2));
   at::Tensor images = at::detail::empty_cuda({2 * R * hk * d}, at::kBFloat16, pool.device(), c10::nullopt);
@@ -1630,6 +1630,7 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
   l.page_size = static_cast<int>(page_size);
   l.page_shift = p.shift;
   l.runs = runs;
+  l.starts = runs + 12 * ctas;
   l.seq_lens = seq_lens.data_ptr<int32_t>();
   l.cu_q = cu_q.data_ptr<int32_t>();
   l.first_tile = plan_table.data_ptr<int32_t>();
@@ -1645,9 +1646,7 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
   a.ld_q = static_cast<int>(T > 1 ? q.stride(0) : hq * d);  // the tensor map takes no other stride
   a.out = out.data_ptr();
   a.images = images.data_ptr();
-  a.first_tile = plan_table.data_ptr<int32_t>();
-  a.ld_first = static_cast<int>(plan_table.size(1));
-  a.tiles = static_cast<int>(R / minisgl::kKv4TileKeys);
+  a.starts = l.starts;
   a.ld_pt = l.ld_pt;
   a.seq_lens = seq_lens.data_ptr<int32_t>();
   a.cu_q = cu_q.data_ptr<int32_t>();

@@ -312,13 +312,21 @@ __device__ void plan_runs(const Kv4LoadArgs& a, const ErrorSink& err) {
     const int keys = kv4_keys(a.seq_lens, b, a.ld_pt);
     return max(1, (keys - q_len + min(q_len, (pair + 1) * W) + kKv4TileKeys - 1) / kKv4TileKeys);
   };
+  // where each request's images begin; a plan that does not hold all of its keys,
+  // from its first to its last, has none of them
+  for (int b = threadIdx.x; b < a.B; b += 256) {
+    const int keys = kv4_keys(a.seq_lens, b, a.ld_pt), row = a.first_tile[static_cast<int64_t>(b) * a.ld_first];
+    auto holds = [&](int at, int pos) { return a.row_req[at] == b && a.row_pos[at] == pos; };
+    const bool all = keys == 0 || (row >= 0 && row % kKv4TileKeys == 0 && row <= a.T - keys && holds(row, 0) &&
+                                   holds(row + keys - 1, keys - 1));
+    if (!all) err.report(kErrBadIndex, 957);
+    a.starts[b] = all ? row / kKv4TileKeys : -1;
+  }
   bool falls = false;
   for (int b = warp; b < a.B; b += 8) {
-    const int q_len = kv4_query_tokens(a.cu_q, b, a.q_rows), keys = kv4_keys(a.seq_lens, b, a.ld_pt);
+    const int q_len = kv4_query_tokens(a.cu_q, b, a.q_rows);
     falls = falls || kv4_offsets_fall(a.cu_q, b);
-    const int first = a.first_tile[static_cast<int64_t>(b) * a.ld_first] / kKv4TileKeys;
-    if (lane == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.q_rows || a.cu_q[b + 1] < a.cu_q[b] || first < 0 || a.seq_lens[b] > a.ld_pt ||
-                      (keys > 0 && first + (keys + kKv4TileKeys - 1) / kKv4TileKeys > a.T / kKv4TileKeys)))
+    if (lane == 0 && (a.cu_q[b] < 0 || a.cu_q[b + 1] > a.q_rows || a.cu_q[b + 1] < a.cu_q[b] || a.seq_lens[b] > a.ld_pt))
       err.report(kErrBadIndex, 956);
     int sum = 0;
     for (int p = lane; p * W < q_len; p += 32) sum += kKv4PairCost + tiles(b, q_len, p);

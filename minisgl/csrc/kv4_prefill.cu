@@ -106,7 +106,7 @@ struct Walk {
     p.h = h;
     p.q_begin = a.cu_q[b], p.q_len = kv4_query_tokens(a.cu_q, b, a.T);
     p.keys = kv4_keys(a.seq_lens, b, a.ld_pt);
-    first = a.first_tile[static_cast<int64_t>(b) * a.ld_first] / kKeys;
+    first = a.starts[b];
     p.tok0 = pair * 2 * TT;
     const int cached = p.keys - p.q_len;
     auto tiles = [&](int t) { return t >= p.q_len ? 0 : max(0, (cached + min(p.q_len, t + TT) + kKeys - 1) / kKeys); };
@@ -120,8 +120,7 @@ struct Walk {
       reinterpret_cast<int4*>(a.desc)[blockIdx.x] =
           make_int4(static_cast<int>(((at + kKv4PairCost + n) * more.w - 1) / more.z), b, pair, h);
     }
-    // images that the plan does not have: none (the planning block has reported it)
-    if (first < 0 || (p.keys > 0 && first + (p.keys + kKeys - 1) / kKeys > a.tiles)) p.n0 = p.n1 = 0;
+    if (first < 0) p.n0 = p.n1 = 0;  // keys that the plan does not have: none (the planning block has reported it)
     if (p.kt1 < n) {
       kt = p.kt1;
     } else {

@@ -240,6 +240,7 @@ struct Kv4LoadArgs {
   // runs [ctas, 8]: request, pair of row tiles, KV head and key tile that a CTA
   // begins with; tiles of its run, the pair's place, all places, runs
   int32_t* runs;
+  int32_t* starts;           // [B] first image tile of each request (-1: the plan does not hold its keys)
   const int32_t *seq_lens, *cu_q, *first_tile;
   int ld_first, q_rows, B, group, ctas;
   int* err;
@@ -279,8 +280,7 @@ struct Kv4PrefillArgs {
   int ld_q;
   void* out;                 // [T, hq * d] bf16
   const void* images;        // [tiles, hk, K and V, d / 64, 128 keys] rows of 128 bytes, swizzled
-  const int32_t* first_tile; // [B] (stride ld_first): first row of each request's tiles
-  int ld_first, tiles;       // tiles in images
+  const int32_t* starts;     // [B] first tile of each request in images (Kv4LoadArgs)
   const int32_t* seq_lens;   // [B]
   int ld_pt;                 // positions of the page table: no request has more keys
   const int32_t* cu_q;       // [B + 1]

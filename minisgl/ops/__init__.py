@@ -912,7 +912,9 @@ def decode_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pag
 class KV4PrefillPlan(MlaPrefillPlan):
     """Host-built layout of a batch's keys (its requests' key counts) for
     ``prefill_attention_kv4`` over many query rows, which expands them once to
-    bf16 tiles of 128 keys. Built once per batch; used by every layer."""
+    bf16 tiles of 128 keys. Built once per batch; used by every layer. It may
+    hold more keys than a request has; a request with more than it holds is
+    reported and its rows are zeros."""
 
     PAGE = 128
 

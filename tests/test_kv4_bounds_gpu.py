@@ -96,3 +96,24 @@ def test_offsets_that_fall_leave_no_work(queries):
     _done()
     for request in range(3):
         batch.check(got, request)
+
+
+@pytest.mark.parametrize("planned", [[300, 200, 90], [200, 200, 200], [310, 150, 90], [305, 200, 80], [90, 200, 310]],
+                         ids=lambda x: "-".join(map(str, x)))
+def test_a_plan_of_fewer_keys_than_a_request_has(planned):
+    """Growth within a tile, beyond one, of any request: reported, the request's rows zeros, the others' right.
+    A plan may hold more keys than a request has."""
+    lens = [310, 200, 90]
+    batch = _Batch(lens, [150, 90, 30])
+    got = batch.run(plan=ops.KV4PrefillPlan(planned, torch.device(DEV)))
+    _reported()
+    for request, (n, m) in enumerate(zip(lens, planned)):
+        if n <= m:
+            batch.check(got, request)
+        else:
+            assert (got[batch.cu[request]:batch.cu[request + 1]] == 0).all()
+    for now in ([310, 200, 90], [7, 129, 128], [256, 0, 1]):
+        got = batch.run(now, plan=ops.KV4PrefillPlan([310, 200, 130], torch.device(DEV)))
+        _done()
+        for request in range(3):
+            batch.check(got, request, now)
