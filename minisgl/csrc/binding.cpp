@@ -1576,7 +1576,7 @@ std::tuple<at::Tensor, at::Tensor> kv4_load(const at::Tensor& pool, int64_t laye
 at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst, const at::Tensor& pool, int64_t layer,
                        const at::Tensor& page_table, const at::Tensor& req_rows, const at::Tensor& seq_lens,
                        const at::Tensor& cu_q, int64_t hq, int64_t hk, int64_t d, int64_t page_size,
-                       double scale, const at::Tensor& plan_table, const at::Tensor& row_req, const at::Tensor& row_pos,
+                       double scale, const at::Tensor& first_row, const at::Tensor& row_req, const at::Tensor& row_pos,
                        const c10::optional<at::Tensor>& err) {
   const char* op = "prefill_attention_kv4";
   const auto p = kv4_pool(op, pool, layer, hk, d, page_size);
@@ -1597,9 +1597,8 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
   check_index(op, cu_q, "cu_q", B + 1, pool);
   check_index(op, row_req, "the plan's rows", -1, pool);
   check_index(op, row_pos, "the plan's positions", R, pool);
-  check_index(op, plan_table, "the plan's table", -1, pool);
-  MSG_CHECK(plan_table.dim() == 2 && plan_table.size(0) == B && plan_table.size(1) >= 1, op, ": the plan is of ",
-            plan_table.dim() == 2 ? plan_table.size(0) : 0, " requests, not ", B);
+  check_index(op, first_row, "the plan's first rows", -1, pool);
+  MSG_CHECK(first_row.numel() == B, op, ": the plan is of ", first_row.numel(), " requests, not ", B);
   MSG_CHECK(R % minisgl::kKv4TileKeys == 0 && R <= 0x7fffffff / 2, op, ": the plan's rows must be whole tiles");
   MSG_CHECK(B <= minisgl::kKv4MaxBatch, op, ": at most ", static_cast<int64_t>(minisgl::kKv4MaxBatch), " requests, got ", B);
   const int64_t pair = 2 * (minisgl::kKv4TileKeys / (hq / hk));
@@ -1633,8 +1632,7 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
   l.starts = runs + 12 * ctas;
   l.seq_lens = seq_lens.data_ptr<int32_t>();
   l.cu_q = cu_q.data_ptr<int32_t>();
-  l.first_tile = plan_table.data_ptr<int32_t>();
-  l.ld_first = static_cast<int>(plan_table.size(1));
+  l.first_row = first_row.data_ptr<int32_t>();
   l.q_rows = static_cast<int>(T);
   l.B = static_cast<int>(B);
   l.group = static_cast<int>(hq / hk);

@@ -315,7 +315,7 @@ __device__ void plan_runs(const Kv4LoadArgs& a, const ErrorSink& err) {
   // where each request's images begin; a plan that does not hold all of its keys,
   // from its first to its last, has none of them
   for (int b = threadIdx.x; b < a.B; b += 256) {
-    const int keys = kv4_keys(a.seq_lens, b, a.ld_pt), row = a.first_tile[static_cast<int64_t>(b) * a.ld_first];
+    const int keys = kv4_keys(a.seq_lens, b, a.ld_pt), row = a.first_row[b];
     auto holds = [&](int at, int pos) { return a.row_req[at] == b && a.row_pos[at] == pos; };
     const bool all = keys == 0 || (row >= 0 && row % kKv4TileKeys == 0 && row <= a.T - keys && holds(row, 0) &&
                                    holds(row + keys - 1, keys - 1));

@@ -241,8 +241,8 @@ struct Kv4LoadArgs {
   // begins with; tiles of its run, the pair's place, all places, runs
   int32_t* runs;
   int32_t* starts;           // [B] first image tile of each request (-1: the plan does not hold its keys)
-  const int32_t *seq_lens, *cu_q, *first_tile;
-  int ld_first, q_rows, B, group, ctas;
+  const int32_t *seq_lens, *cu_q, *first_row;
+  int q_rows, B, group, ctas;
   int* err;
 };
 void launch_kv4_load(const Kv4LoadArgs& a, cudaStream_t s);

@@ -909,14 +909,34 @@ def decode_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pag
                               page_size, scale, out)
 
 
-class KV4PrefillPlan(MlaPrefillPlan):
+class KV4PrefillPlan:
     """Host-built layout of a batch's keys (its requests' key counts) for
     ``prefill_attention_kv4`` over many query rows, which expands them once to
-    bf16 tiles of 128 keys. Built once per batch; used by every layer. It may
-    hold more keys than a request has; a request with more than it holds is
-    reported and its rows are zeros."""
+    bf16 tiles of 128 keys: the compact row at which each request begins and
+    each row's (request, position), -1 in what pads a request's last tile. 8
+    bytes a key. Built once per batch; used by every layer. It may hold more
+    keys than a request has; a request with more than it holds is reported
+    and its rows are zeros."""
 
-    PAGE = 128
+    TILE = 128
+
+    def __init__(self, lens: List[int], device: torch.device) -> None:
+        import numpy as np
+
+        keys = np.maximum(np.asarray(lens, dtype=np.int64), 0)
+        rows = -(-keys // self.TILE) * self.TILE
+        first = np.cumsum(rows) - rows
+        B, self.rows = len(keys), int(rows.sum())
+        pos = np.arange(self.rows) - np.repeat(first, rows)
+        real = pos < np.repeat(keys, rows)
+        host = torch.from_numpy(np.concatenate([first, np.where(real, np.repeat(np.arange(B), rows), -1),
+                                                np.where(real, pos, 0)]).astype(np.int32))
+        if device.type == "cuda":
+            host = host.pin_memory()
+        dev = host.to(device, non_blocking=True)
+        self.first_row = dev[:B]
+        self.row_req = dev[B:B + self.rows]
+        self.row_pos = dev[B + self.rows:]
 
 
 # Query rows (tokens x heads of a group) of a request up to which the few-row
@@ -969,7 +989,7 @@ def prefill_attention_kv4(q: torch.Tensor, kv_pool: torch.Tensor, layer: int, pa
         plan = KV4PrefillPlan(lens, kv_pool.device)
     _count(3)
     return native().kv4_prefill(q, out, kv_pool, layer, page_table, req_rows, seq_lens, cu_q, hq, hk, d, page_size,
-                                scale, plan.page_table, plan.row_req, plan.row_pos, err)
+                                scale, plan.first_row, plan.row_req, plan.row_pos, err)
 
 
 def copy_pages(pool: torch.Tensor, src, dst, page_dim: int = 2) -> torch.Tensor:

@@ -117,3 +117,15 @@ def test_a_plan_of_fewer_keys_than_a_request_has(planned):
         _done()
         for request in range(3):
             batch.check(got, request, now)
+
+
+@pytest.mark.parametrize("max_q", [200, 1], ids=["many", "few"])
+def test_a_batch_of_no_requests(max_q):
+    hq, hk, d, page = 8, 2, 128, 16
+    pool = torch.zeros(2, 1, 4, hk, page * 68, dtype=torch.uint8, device=DEV)
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    table, cu = torch.zeros(1, 64, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    q = torch.zeros(0, hq * d, dtype=torch.bfloat16, device=DEV)
+    got = ops.prefill_attention_kv4(q, pool, 0, table, none, none, cu, max_q, hq, hk, d, page, 0.1)
+    _done()
+    assert got.shape == (0, hq * d)
