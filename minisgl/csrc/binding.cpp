@@ -1572,6 +1572,13 @@ std::tuple<at::Tensor, at::Tensor> kv4_load(const at::Tensor& pool, int64_t laye
   return {k_out, v_out};
 }
 
+// Places of the sequence that attention splits into runs, at most: each unit of query
+// rows has those of its cost and one a key tile (one where it has no key). The kernels
+// count them in 32 bits.
+int64_t kv4_places(int64_t units, int64_t cost, int64_t positions) {
+  return units * (cost + std::max<int64_t>(1, (positions + minisgl::kKv4TileKeys - 1) / minisgl::kKv4TileKeys));
+}
+
 // Many query rows: the plan's rows expanded to tile images, then attention over them.
 at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst, const at::Tensor& pool, int64_t layer,
                        const at::Tensor& page_table, const at::Tensor& req_rows, const at::Tensor& seq_lens,
@@ -1602,7 +1609,7 @@ at::Tensor kv4_prefill(const at::Tensor& q, const c10::optional<at::Tensor>& dst
   MSG_CHECK(R % minisgl::kKv4TileKeys == 0 && R <= 0x7fffffff / 2, op, ": the plan's rows must be whole tiles");
   MSG_CHECK(B <= minisgl::kKv4MaxBatch, op, ": at most ", static_cast<int64_t>(minisgl::kKv4MaxBatch), " requests, got ", B);
   const int64_t pair = 2 * (minisgl::kKv4TileKeys / (hq / hk));
-  MSG_CHECK((T / pair + B) * hk * (page_table.size(1) / minisgl::kKv4TileKeys + 1) < (int64_t{1} << 30), op,
+  MSG_CHECK(kv4_places((T / pair + B) * hk, minisgl::kKv4PairCost, page_table.size(1)) <= 0x7fffffff, op,
             ": too many tiles of work");
   if (B == 0 || T == 0) return out;
   const int ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
@@ -1690,9 +1697,9 @@ at::Tensor kv4_attention(const at::Tensor& q, const c10::optional<at::Tensor>& d
   MSG_CHECK(B <= minisgl::kKv4MaxBatch, op, ": at most ", static_cast<int64_t>(minisgl::kKv4MaxBatch), " requests, got ", B);
   if (B == 0 || T == 0) return out;
   MSG_CHECK(page_table.size(0) >= 1 && page_table.size(1) >= 1, op, ": page_table is empty");
-  // tiles of 8 query rows, each with a place of its own and its key tiles
-  const int64_t units = (T * (hq / hk) / 8 + B) * hk;
-  MSG_CHECK(units * (page_table.size(1) / 128 + 2) <= 0x7fffffff && T * hq <= 0x7fffffff, op, ": too many tiles of work");
+  MSG_CHECK(kv4_places((T * (hq / hk) / 8 + B) * hk, minisgl::kKv4UnitCost, page_table.size(1)) <= 0x7fffffff &&
+                T * hq <= 0x7fffffff,
+            op, ": too many tiles of work");
   const int runs = minisgl::kv4_attn_runs(at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
   // records of partial pieces, then the descriptors
   const int64_t floats = static_cast<int64_t>(runs) * 2 * 8 * (d + 2) + 4 * runs;

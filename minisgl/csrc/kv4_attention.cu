@@ -136,10 +136,7 @@ __device__ __forceinline__ int rows_of(const Kv4AttnArgs& a, int b) {
 }
 __device__ __forceinline__ int key_tiles(int keys) { return max(1, (keys + kTile - 1) / kTile); }
 
-// What a unit (request, KV head, tile of query rows) costs beside its key tiles, in
-// tiles. With 0, 1, 2, 3: 256 ragged requests 151, 140, 139, 143 us; 8 of five tokens
-// each 48.9, 42.4, 41.3, 41.8.
-constexpr int kUnitCost = 2;
+constexpr int kUnitCost = kKv4UnitCost;
 
 // A place in the work: request, unit of it (KV head x row tile) and key tile.
 struct Place {

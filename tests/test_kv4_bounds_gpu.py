@@ -129,3 +129,24 @@ def test_a_batch_of_no_requests(max_q):
     got = ops.prefill_attention_kv4(q, pool, 0, table, none, none, cu, max_q, hq, hk, d, page, 0.1)
     _done()
     assert got.shape == (0, hq * d)
+
+
+@pytest.mark.parametrize("rows,tiles,max_q", [(16383, 131078, 1), (16383, 131078, 100)], ids=["few", "many"])
+def test_more_tiles_than_32_bits_count(rows, tiles, max_q):
+    """A unit of query rows (8 of them, or 256) may have a tile for each 128 positions of the table, the last
+    one begun, and two for what it costs beside them. The call with one tile too many is refused, the one
+    before it runs."""
+    d, page = 64, 16
+    T = (rows - 1) * (8 if max_q == 1 else 256)
+    assert rows * (2 + tiles) <= 2 ** 31 - 1 < rows * (2 + tiles + 1)
+    pool = torch.zeros(2, 1, 4, 1, page * 34, dtype=torch.uint8, device=DEV)
+    row, seq, cu = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0], [5], [0, T]))
+    q = torch.zeros(1, d, dtype=torch.bfloat16, device=DEV).expand(T, -1)
+    table = torch.zeros(tiles * 128 + 1, dtype=torch.int32, device=DEV)
+    call = lambda n: ops.prefill_attention_kv4(q, pool, 0, table[:n].view(1, n), row, seq, cu, max_q, 1, 1, d, page, 0.1)  # noqa: E731
+    with pytest.raises(RuntimeError, match="too many tiles"):
+        call(tiles * 128 + 1)
+    out = call(tiles * 128)
+    _done()
+    # rows before the first key are zeros; a pool of zero bytes holds -8 at a scale of 2^-21 everywhere
+    assert (out[:-5] == 0).all() and (out[-5:] == -2.0 ** -18).all()
