@@ -37,6 +37,16 @@ MAX_SPLITS = 16
 KV4_PLAN_KEYS = 1 << 18
 
 
+def kv4_scratch_bytes(kv_heads: int, head_dim: int, longest: int, requests: int) -> int:
+    """What a prefill call over a 4-bit pool takes beside the pool, at most: K and
+    V of its keys in bf16, in whole tiles of each request, and the records of
+    split work (fp32, two of 256 rows an SM). A request longer than
+    KV4_PLAN_KEYS is a call of its own."""
+    keys = min(max(KV4_PLAN_KEYS, longest), requests * longest)
+    rows = keys + requests * (ops.KV4PrefillPlan.TILE - 1)
+    return 4 * kv_heads * head_dim * rows + 4 * NUM_SMS * 2 * 256 * (head_dim + 2)
+
+
 def decode_splits(batch_size: int, kv_heads: int) -> int:
     """Splits per (request, kv head) so that about two CTAs run per SM."""
     want = math.ceil(2 * NUM_SMS / max(1, batch_size * kv_heads))

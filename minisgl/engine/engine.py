@@ -319,7 +319,7 @@ class Engine:
             pages = config.num_page_override
         elif self.is_cuda:
             model_bytes = init_free - self._sync_get_memory()[1]
-            pages = int(config.memory_ratio * init_free - model_bytes) // per_page
+            pages = int(config.memory_ratio * init_free - model_bytes - self._attention_scratch(config)) // per_page
         else:
             pages = (config.max_running_req * min(config.max_seq_len, 4096)) // self.page_size
         if pages <= 1:
@@ -327,6 +327,17 @@ class Engine:
         logger.info_rank0(f"KV cache: {pages * self.page_size} tokens in {pages} pages of {self.page_size} "
                           f"({mem_GB(pages * per_page)}), model {mcfg.architectures[0]}")
         return pages
+
+    def _attention_scratch(self, config: EngineConfig) -> int:
+        """Bytes that attention calls take beside the pool and that grow with its keys."""
+        m = self.model_config
+        if m.kv_quant != "int4":
+            return 0
+        from minisgl.attention.native import kv4_scratch_bytes
+        from minisgl.utils import div_even
+
+        kv = div_even(m.num_kv_heads, get_tp_info().size, allow_replicate=True)
+        return kv4_scratch_bytes(kv, m.head_dim, config.max_seq_len, config.max_running_req)
 
     def _bytes_per_page(self) -> int:
         m = self.model_config
