@@ -67,9 +67,15 @@ class AttentionLayer(StateLessOP):
 
     @property
     def fusable(self) -> bool:
-        """Whether the fused qkv epilogue can replace ``rope_store`` (it
-        stores rows of 16 bits only)."""
-        return self.head_dim == 128 and not self._kv4
+        """Whether the layer has a fused form (norms, activation and residual
+        adds in the GEMMs' epilogues)."""
+        return self.head_dim == 128
+
+    @property
+    def stores_in_epilogue(self) -> bool:
+        """Whether the fused form's qkv epilogue also takes the place of
+        ``rope_store``: it stores rows of 16 bits only."""
+        return self.fusable and not self._kv4
 
     def forward(self, qkv: torch.Tensor) -> torch.Tensor:
         ctx = get_global_ctx()

@@ -109,7 +109,7 @@ class DecoderLayer(BaseOP):
         attn = self.self_attn
         fused = fused and self._fused_attn
         xt = x[:T]
-        if fused:  # q/k norm, RoPE and the KV store in the qkv GEMM's epilogue
+        if fused and attn.attn.stores_in_epilogue:  # q/k norm, RoPE and the KV store in the qkv GEMM's epilogue
             q = torch.empty(T, attn.attn.qo_attn_dim, dtype=x.dtype, device=x.device)
             ops.gemm_fused(xt, attn.qkv_proj.weight, bias=attn.qkv_proj.bias, rope=attn.attn.rope_args(), out=q)
             o = attn.attn.attend(q)
@@ -252,7 +252,9 @@ class DecoderForCausalLM(BaseLLMModel):
         for layer in self.model.layers.op_list:
             attn = layer.self_attn
             hq, hk = attn.attn.num_qo_heads, attn.attn.num_kv_heads
-            out[tuple(attn.qkv_proj.weight.shape)] = (norm | ops.EPI_ROPE, hq, hk)
+            qkv = norm | (ops.EPI_ROPE if attn.attn.stores_in_epilogue else 0)
+            if qkv:
+                out[tuple(attn.qkv_proj.weight.shape)] = (qkv, hq, hk)
             if not sp:
                 out[tuple(attn.o_proj.weight.shape)] = (ops.EPI_RESIDUAL, hq, hk)
             if layer._fused_mlp:

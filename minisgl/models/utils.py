@@ -101,7 +101,11 @@ class RopeAttn(BaseOP):
 
     def forward_fused(self, r: "torch.Tensor", norm_eps: float) -> "torch.Tensor":
         """r + o_proj(attention(rmsnorm(r))): the norm, q/k-norm, RoPE and
-        KV store in the qkv GEMM epilogue, the add in the o_proj epilogue."""
+        KV store in the qkv GEMM epilogue, the add in the o_proj epilogue. A
+        4-bit cache takes its rows from the qkv rows in a kernel of its own."""
+        if not self.attn.stores_in_epilogue:
+            qkv = ops.gemm_fused(r, self.qkv_proj.weight, bias=self.qkv_proj.bias, norm_eps=norm_eps)
+            return self.o_proj.forward_residual(self.attn.forward(qkv), r)
         q = torch.empty(r.shape[0], self.attn.qo_attn_dim, dtype=r.dtype, device=r.device)
         ops.gemm_fused(r, self.qkv_proj.weight, bias=self.qkv_proj.bias, norm_eps=norm_eps,
                        rope=self.attn.rope_args(), out=q)

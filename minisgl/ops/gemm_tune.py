@@ -118,7 +118,9 @@ def _time_runs(run, ws: List[torch.Tensor], reps: int = 8) -> float:
 def _fused_candidates(M: int, K: int, kind: int) -> List[Plan]:
     """Plans a fused-epilogue GEMM of this kind accepts: weight-major tiles,
     token-major tiles (with whole 128-feature heads / gate|up blocks when the
-    epilogue needs them)."""
+    epilogue needs them; a norm alone, the qkv rows of a 4-bit KV cache, keeps
+    to those too, since plans are kept by shape and another engine may run
+    the shape with the whole epilogue)."""
     from minisgl import ops
 
     num_kb = (K + 63) // 64
@@ -126,7 +128,7 @@ def _fused_candidates(M: int, K: int, kind: int) -> List[Plan]:
     if kind == ops.EPI_SAMPLE:  # the sampling epilogue needs weight-major tiles
         return out
     if M >= 64:
-        whole = (kind & (ops.EPI_ROPE | ops.EPI_SILU)) != 0
+        whole = (kind & (ops.EPI_ROPE | ops.EPI_SILU | ops.EPI_NORM)) != 0
         for bn in (128, 256) if whole else (64, 128, 256):
             for s in (1, 2, 4, 8):
                 if s <= num_kb:
