@@ -417,10 +417,10 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ K
     k_to = static_cast<uint4*>(a.k_out) + (static_cast<int64_t>(tile) * a.hk + h) * (2 * kKv4TileKeys * kLanes) +
            (x / 8) * (kKv4TileKeys * 8) + row * 8 + ((x ^ row) & 7);
     v_to = k_to + kKv4TileKeys * kLanes;
-    const int req = a.row_req[r];
+    const int req = a.row_req[r], pos = a.row_pos[r];
     slot = -1;
-    if (req >= 0 && req < a.B) {
-      const int table_row = a.req_rows[req], pos = a.row_pos[r];
+    if (req >= 0 && req < a.B && pos < a.seq_lens[req]) {  // a plan may hold more keys than there are now
+      const int table_row = a.req_rows[req];
       if (table_row >= 0 && table_row < a.pt_rows && pos >= 0 && pos < a.ld_pt)
         slot = a.page_table[static_cast<int64_t>(table_row) * a.ld_pt + pos];
       if (slot < 0 || slot >= a.kv_slots) {

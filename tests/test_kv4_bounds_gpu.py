@@ -150,3 +150,29 @@ def test_more_tiles_than_32_bits_count(rows, tiles, max_q):
     _done()
     # rows before the first key are zeros; a pool of zero bytes holds -8 at a scale of 2^-21 everywhere
     assert (out[:-5] == 0).all() and (out[-5:] == -2.0 ** -18).all()
+
+
+def test_a_captured_prompt_with_shorter_lengths():
+    """A plan holds the keys of the capture; replays with fewer keys read nothing of the table behind them,
+    where entries are of no page."""
+    lens = [400, 200, 90]
+    batch = _Batch(lens, [150, 90, 30])
+    hq, hk, d, page = batch.heads
+    seq = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    cu = torch.tensor(batch.cu, dtype=torch.int32, device=DEV)
+    q, plan = batch.q.to(DEV), ops.KV4PrefillPlan(lens, torch.device(DEV))
+    call = lambda: ops.prefill_attention_kv4(q, batch.pool, 0, batch.pt, batch.rr, seq, cu, 150, hq, hk, d, page,  # noqa: E731
+                                             d ** -0.5, plan=plan)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for now in ([400, 200, 90], [150, 100, 31], [300, 0, 1], [129, 128, 90]):
+        seq.copy_(torch.tensor(now, dtype=torch.int32))
+        for row, n in zip(batch.rows.tolist(), now):
+            batch.pt[row, n:] = -1 if n % 2 else 2 ** 31 - 1
+            batch.pt[row, :n] = batch.table[row, :n].to(DEV)
+        graph.replay()
+        _done()
+        for request in range(3):
+            batch.check(out.view(-1, hq, d), request, now)
