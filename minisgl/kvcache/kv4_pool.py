@@ -48,8 +48,9 @@ class MHAKV4Cache(BaseKVCachePool):
         return self.pool[1, layer]
 
     def store_kv(self, k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, layer: int) -> None:
-        """Rows of k and v [T, heads * head_dim] as they are (no norm, no rotation)."""
-        ops.store_kv4(k, v, self.pool, layer, out_loc, self.local_kv_heads, self.head_dim, self.page_size)
+        """Rows of k and v [T, heads * head_dim] or [T, heads, head_dim] as they are (no norm, no rotation)."""
+        ops.store_kv4(k.flatten(1), v.flatten(1), self.pool, layer, out_loc, self.local_kv_heads,
+                      self.head_dim, self.page_size)
 
     def load_kv(self, slots: torch.Tensor, layer: int):
         """The rows of ``slots`` as (k, v) [T, heads, head_dim]."""

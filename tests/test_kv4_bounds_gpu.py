@@ -176,3 +176,18 @@ def test_a_captured_prompt_with_shorter_lengths():
         _done()
         for request in range(3):
             batch.check(out.view(-1, hq, d), request, now)
+
+
+@pytest.mark.parametrize("queries", [[150, 90, 30], [3, 2, 1]], ids=["many", "few"])
+def test_same_bits_every_time(queries):
+    """Records of split work are joined in the order of their runs, so calls repeat bit for bit."""
+    batch = _Batch([2000, 900, 90], queries)
+    first = batch.run()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            again = batch.run()
+        torch.cuda.synchronize()
+        assert torch.equal(first, again)
+    _done()
