@@ -5,9 +5,10 @@
 //
 // with k_j and v_j in 4-bit codes, 136 bytes of cache per token and 128-dim
 // head. Bound by what a warp has to do per code, on the integer and half2 pipes:
-// 256 requests of up to 4096 keys and 8 KV heads take 139 us, 4.2 TB/s of codes
-// (64 % of the copy rate), one of 131072 keys 46 us. Everything is laid out to
-// keep that small:
+// 256 requests of up to 4096 keys and 8 KV heads take 139 us in bursts (a graph of
+// 20 calls, the best of five), 4.2 TB/s (64 % of the copy rate), and 150 in a stream
+// of calls (59 %), one of 131072 keys 46 us. Everything is laid out to keep that
+// small:
 //
 // * The products are taken the other way round, S^T = K q^T and O^T = V^T P^T
 //   (warp-level m16n8k16 MMA): keys and dims fill the 16 rows of A, and the query

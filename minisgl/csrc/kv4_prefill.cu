@@ -6,9 +6,11 @@
 // on tcgen05. Bound by the tensor pipe (4 d flops per query row and key) and,
 // close behind, by the exponentials: 128 x 128 scores of 128 dims take 1024 cycles
 // of MMA for both products and 1024 of the special-function unit (64 dims: 640).
-// 2048 queries of 64 heads over 16384 keys: 822 to 838 us with the expansion, 1230
-// to 1250 TFLOP/s, 90 % of what cuBLAS sustains under the power limit. 4 prompts
-// of 2048 tokens, 32 heads of 64 dims: 146 us.
+// 2048 queries of 64 heads over 16384 keys, with the expansion: 935 us in a stream
+// of calls, where the power limit takes the clock down, 1100 TFLOP/s, 80 % of what
+// cuBLAS sustains; 811 us in bursts (a graph of 20 calls, the best of five), 1270
+// TFLOP/s, 78 % of cuBLAS's own burst. 4 prompts of 2048 tokens, 32 heads of 64
+// dims: 147 us (burst).
 //
 // Query rows are (token, head of the group): TT = 128 / G tokens are a tile, so
 // every group size fills its 128 rows (G = 7: 126 of them) and all heads of a

@@ -277,7 +277,7 @@ void launch_kv4_attention(const Kv4AttnArgs& a, cudaStream_t s);
 // rows, 128 bytes] as launch_kv4_load writes them for a plan.
 constexpr int kKv4TileKeys = 128;
 // What a pair of row tiles costs beside its key tiles, in tiles. Six prompts of up to
-// 1500 tokens with 0, 1, 2, 3, 4: 149, 109, 94, 96, 97 us.
+// 1500 tokens with 0, 1, 2, 3, 4: 119, 89, 90, 92, 92 us (a graph of 20 calls).
 constexpr int kKv4PairCost = 2;
 struct Kv4PrefillArgs {
   const void* q;             // [T, >= hq * d] bf16

@@ -942,11 +942,12 @@ class KV4PrefillPlan:
 # Query rows (tokens x heads of a group) of a request up to which the few-row
 # kernel, which expands codes for 8 rows at a time in registers, reads the
 # cache itself; beyond, keys are expanded once and a tcgen05 kernel takes over.
-# Its time grows with the rows, the other's hardly does. At 64 and 128 rows, few
-# rows against many in us: 20.6, 28.2 / 24.7, 25.2 (8 KV heads of 128 dims, one
-# request of 4096 keys), 70.9, 127 / 88.4, 88.7 (one of 32768), 74.1, 132 /
-# 89.3, 91.2 (8 of 4096), 48.0, 81.1 / 54.4, 55.9 (16 of 1024): they meet at 78
-# to 101 rows.
+# Its time grows with the rows, the other's hardly does. At 64, 80 and 96 rows of 8
+# KV heads, few rows / many in us: of 128 dims 20.1, 22.4, 25.4 / 23.5 (one request
+# of 4096 keys), 71.9, 86.1, 101 / 84.4 (one of 32768), 74.4, 89.0, 107 / 83.5 (8 of
+# 4096), 47.2, 56.0, 68.3 / 51.9 (16 of 1024): they meet at 72 to 86 rows. Of 64 dims
+# 15.8, 17.3, 18.8 / 19.6, 48.5, 57.9, 67.0 / 57.4, 51.8, 61.0, 70.9 / 56.4 and 33.9,
+# 39.7, 46.6 / 32.7: at about 61 to 105.
 KV4_FEW_ROWS = 80
 KV4_MAX_BATCH = 1280  # requests of one attention call over a 4-bit pool
 
