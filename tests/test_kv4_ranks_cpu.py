@@ -27,6 +27,7 @@ def _run(rank, world, folder, port, sp, out_q):
     llm = LLM(folder, tp_info=DistributedInfo(rank, world), distributed_port=port, **ARGS)
     if sp:  # token-sharded residual stream, token counts padded to the ranks
         DistributedCommunicator.plugins[-1].sequence_parallel = True
+    assert llm.engine.model.model.fusable
     heads = llm.engine.kv_cache.pool.shape[3]
     outs = llm.generate(PROMPTS, [SamplingParams(temperature=0.0, max_tokens=m, ignore_eos=True) for m in (8, 5)])
     out_q.put((rank, ([o["token_ids"] for o in outs], heads)))
@@ -39,7 +40,9 @@ def checkpoint():
 
     folder = tempfile.mkdtemp(prefix="minisgl_kv4_ranks_")
     shutil.rmtree(folder)
-    make_model_dir("tiny-qwen3", folder=folder, overrides={"tie_word_embeddings": False})
+    # 128-dim heads and halves of 128 columns a rank: layers have a fused form
+    make_model_dir("tiny-qwen3", folder=folder, overrides={"tie_word_embeddings": False, "head_dim": 128,
+                                                           "intermediate_size": 1024})
     write_random_checkpoint(folder, seed=3, std=0.05)
     yield folder
     shutil.rmtree(folder, ignore_errors=True)
